@@ -47,7 +47,7 @@ class TaggedTensor:
     """A backend tensor with its dtype tag (interpreter/types.rs:15-98).  Owns one
     reference to the library handle; copying the Python object shares it."""
 
-    __slots__ = ("_b", "_h", "_dtype", "_shape")
+    __slots__ = ("_b", "_h", "_dtype", "_shape", "_memory")
 
     # dtype and shape are the library's, and never change.  Most results of an op stream are only passed on, so they are
     # asked for when they are read, and then once (a prompt of 61 tokens through the trait methods: 2.24 -> 2.00 ms).
@@ -350,6 +350,11 @@ class CudaBackend(TraitBackend):
             ("cg_randn", [vp, _c_i64p, i32, C.c_uint64, f32, f32, out], i32),
             ("cg_probe_wait_timeout", [vp], i32),
             ("cg_lazy_stats", [vp, _c_i64p, _c_i64p, _c_i64p], i32),
+            ("cg_tensor_from_device", [vp, vp, i32, _c_i64p, _c_i64p, i32, out], i32),
+            ("cg_paged_append", [vp, vp, vp, vp, vp, vp, f32, i32, vp, vp, i32, vp, vp, vp, vp, vp, vp], i32),
+            ("cg_paged_attention", [vp, vp, vp, vp, vp, vp, vp, i64, f32, i64, f32, vp], i32),
+            ("cg_beam_select", [vp, vp, vp, vp, C.c_uint32, vp, vp, vp, vp], i32),
+            ("cg_paged_reorder", [vp, vp, vp, vp, vp, vp, vp], i32),
             ("cg_rope_tables", [vp, f32, i32, f32, f32, f32, f32, f32, i32, i64, i64, out, out], i32),
         ]:
             fn = getattr(L, name)
@@ -456,3 +461,63 @@ class CudaBackend(TraitBackend):
         self._check(self._lib.cg_fused_moe(self._ctx, x._h, router._h, gate._h, up._h, down._h, int(top_k),
                                            int(norm_topk), int(act), C.byref(o), C.byref(ids)))
         return self._wrap(o), self._wrap(ids)
+
+    # a paged key/value cache and beam search ---------------------------------------
+    def from_device(self, x) -> TaggedTensor:
+        """A tensor over the device memory of `x` (a torch CUDA tensor: f32, bf16, or 32-bit integers as U32), which it
+        keeps alive.  Nothing is copied.  Work of other streams on that memory is the caller's to order."""
+        storage = {"torch.float32": 0, "torch.int32": 1, "torch.uint32": 1, "torch.bfloat16": 2}.get(str(x.dtype))
+        if storage is None:
+            raise TypeError(f"no storage for {x.dtype}")
+        if not x.is_cuda:
+            raise TypeError("not a CUDA tensor")
+        d, r = _dims(x.shape)
+        s, _ = _dims(x.stride())
+        t = self._ext1("cg_tensor_from_device", x.data_ptr(), storage, d, s, r)
+        t._memory = x
+        return t
+
+    def paged_append(self, k, v, k_pages, v_pages, table, starts, lens, q=None, q_out=None, cos=None, sin=None, q_gain=None, k_gain=None,
+                     eps=1e-6, plus_one=False, rot_half=True):
+        """Norms per head (with gains), rotation (with tables), and k, v into their pages (cg_paged_append); returns q_out,
+        a new tensor of zeros behind the last row's token if none is given."""
+        if q is not None and q_out is None:
+            q_out = self._empty_like_pages(q.shape, k_pages)
+        h = [None if t is None else t._h for t in (q, k, v, q_gain, k_gain)]
+        st = self._lib.cg_paged_append(self._ctx, *h, eps, plus_one, cos and cos._h, sin and sin._h, rot_half, table._h, starts._h, lens._h,
+                                       k_pages._h, v_pages._h, q_out and q_out._h)
+        if st:
+            self._check(st)
+        return q_out
+
+    def paged_attention(self, q, k_pages, v_pages, table, starts, lens, max_new=0, scale=0.0, window=0, softcap=0.0, out=None):
+        """Causal attention of the new tokens over the paged cache (cg_paged_attention)."""
+        if out is None:
+            out = self._empty_like_pages(q.shape, k_pages)
+        st = self._lib.cg_paged_attention(self._ctx, q._h, k_pages._h, v_pages._h, table._h, starts._h, lens._h, max_new, scale, window, softcap,
+                                          out._h)
+        if st:
+            self._check(st)
+        return out
+
+    def beam_select(self, logits, scores, k, finished=None, end=0xFFFFFFFF, out=None):
+        """(scores, tokens, parents, finished) [B, k] of a step of beam search (cg_beam_select)."""
+        if out is None:
+            shape = (logits.shape[0], k)
+            out = (self.zeros(shape, F32), *(self.zeros(shape, U32) for _ in range(3)))
+        elif any(t.shape[-1:] != (k,) for t in out):
+            raise BackendPanic(1, "Shape mismatch in operation: an output")
+        st = self._lib.cg_beam_select(self._ctx, logits._h, scores._h, finished and finished._h, end, *(t._h for t in out))
+        if st:
+            self._check(st)
+        return out
+
+    def paged_reorder(self, parents, lens, own, table, k_pages, v_pages):
+        """Every beam's cache goes on from its parent's, in place (cg_paged_reorder)."""
+        st = self._lib.cg_paged_reorder(self._ctx, parents._h, lens._h, own._h, table._h, k_pages._h, v_pages._h)
+        if st:
+            self._check(st)
+
+    def _empty_like_pages(self, shape, pages):
+        t = self.zeros(shape, F32)
+        return self.to_bf16(t) if self.storage_of(pages) == 2 else t

@@ -1,0 +1,291 @@
+// paged_attn.cu — causal attention of new tokens over a paged key/value cache:
+//   o = sum_t softmax_t(cap tanh(scale q k_t / cap)) v_t   over   p - window < t <= p
+// for a query at position p (catgrad-llm/src/models/llama.rs:97-108 after repeat_kv, helpers.rs:147-161), one pass over the
+// keys with the running maximum and sum of the softmax in f32.
+#include <algorithm>
+
+#include "mma.cuh"
+#include "paged.h"
+
+namespace cg {
+
+namespace {
+
+struct PagedAttnArgs {
+  PagedRows rows;
+  const void *q, *k_pages, *v_pages;
+  void* out;
+  int64_t q_ld, q_hs;   // from one token and one head of q to the next
+  int64_t most;         // new tokens of a row, at most
+  int64_t window;       // 0 = none
+  float scale, cap;     // cap 0 = none
+  int nh, nkv, d;
+};
+
+__device__ __forceinline__ void load8(const float* p, float* x) {
+  const float4 a = *(const float4*)p, b = *((const float4*)p + 1);
+  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float* x) {
+  const uint4 u = *(const uint4*)p;
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void store_as(float* p, float x) { *p = x; }
+__device__ __forceinline__ void store_as(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
+__device__ __forceinline__ float load_as(const float* p) { return *p; }
+__device__ __forceinline__ float load_as(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+
+// Every type and head size, on the CUDA cores.  A block has QR queries of one row and key head (query x is token x / rep,
+// head x % rep of the group) and a share of the visible keys, 32 at a time; the blocks of a cluster share the
+// keys and are joined through shared memory.  Eight lanes have a query row (or four rows): a score is a key's, an output value
+// four neighbouring columns'.  D: head size, rounded up to 64, 128 or 256.
+constexpr int GK = 32;  // keys of a tile
+template <typename T, int D, int QR>
+__global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
+  constexpr int LD = D + 4;
+  constexpr int RT = QR / 16;      // query rows of a thread
+  constexpr int CT = D / 32;       // groups of four output columns of a thread
+  extern __shared__ __align__(16) float sm[];
+  float* qs = sm;                  // [QR][LD]
+  float* ks = qs + QR * LD;        // [GK][LD]
+  float* vs = ks + GK * LD;        // [GK][LD]
+  float* ps = vs + GK * LD;        // [QR][GK + 1]
+  __shared__ float ml[2][QR];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int tid = threadIdx.x, ty = tid >> 3, tx = tid & 7;
+  const int rep = a.nh / a.nkv, kvh = (int)blockIdx.x % a.nkv;
+  const int64_t row = blockIdx.y, x0 = (int64_t)(blockIdx.x / a.nkv) * QR;
+  const int slices = (int)gridDim.z, slice = (int)blockIdx.z;
+  int64_t tok0, n, len;
+  if (!row_span(a.rows, row, a.most, &tok0, &n, &len) || x0 >= n * rep) return;  // (the same in all blocks of a cluster)
+  const int64_t pos0 = len - n, i0 = x0 / rep, i1 = min(n - 1, (x0 + QR - 1) / rep);
+  const int64_t lo = a.window > 0 ? max((int64_t)0, pos0 + i0 - a.window + 1) : 0, hi = pos0 + i1;
+  const int64_t first = lo / GK, tiles = hi / GK + 1 - first, per = (tiles + slices - 1) / slices;
+  const int64_t t0 = first + slice * per, t1 = min(first + tiles, t0 + per);
+
+  for (int i = tid; i < QR * (D / 8); i += 128) {
+    const int r = i / (D / 8), c = i % (D / 8) * 8;
+    const int64_t x = x0 + r;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (x < n * rep && c < a.d) {
+      const T* p = (const T*)a.q + (tok0 + x / rep) * a.q_ld + (kvh * rep + x % rep) * a.q_hs + c;
+      for (int e = 0; e < 8; ++e) v[e] = load_as(p + e);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) qs[r * LD + c + e] = v[e];
+  }
+  float o[RT][CT][4], m[RT], l[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) o[r][c][0] = o[r][c][1] = o[r][c][2] = o[r][c][3] = 0.f;
+  }
+  const int64_t page_mask = ((int64_t)1 << a.rows.lg) - 1;
+  for (int64_t t = t0; t < t1; ++t) {
+    __syncthreads();
+    for (int i = tid; i < GK * (D / 8); i += 128) {
+      const int r = i / (D / 8), c = i % (D / 8) * 8;
+      const int64_t key = t * GK + r;
+      float kx[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, vx[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (key >= lo && key <= hi && c < a.d) {
+        const int64_t page = page_of(a.rows, row, key);
+        if (page >= 0) {
+          const int64_t at = (((page * a.nkv + kvh) << a.rows.lg) + (key & page_mask)) * a.d + c;
+          load8((const T*)a.k_pages + at, kx);
+          load8((const T*)a.v_pages + at, vx);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        ks[r * LD + c + e] = kx[e];
+        vs[r * LD + c + e] = vx[e];
+      }
+    }
+    __syncthreads();
+    float s[RT][4];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) s[r][0] = s[r][1] = s[r][2] = s[r][3] = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < D; c += 4) {
+      float4 kk[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) kk[j] = *(const float4*)(ks + (tx + 8 * j) * LD + c);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const float4 qq = *(const float4*)(qs + (ty * RT + r) * LD + c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[r][j] = fmaf(qq.x, kk[j].x, fmaf(qq.y, kk[j].y, fmaf(qq.z, kk[j].z, fmaf(qq.w, kk[j].w, s[r][j]))));
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const int64_t pos = pos0 + (x0 + ty * RT + r) / rep;
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t key = t * GK + tx + 8 * j;
+        const bool seen = key <= pos && (a.window <= 0 || key > pos - a.window);
+        float x = s[r][j] * a.scale;
+        if (a.cap > 0.f) x = a.cap * tanhf(x / a.cap);
+        s[r][j] = seen ? x : -INFINITY;
+        top = fmaxf(top, s[r][j]);
+      }
+#pragma unroll
+      for (int w = 4; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+      const float m_new = fmaxf(m[r], top), base = m_new == -INFINITY ? 0.f : m_new;
+      const float corr = expf(m[r] - base);
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float e = expf(s[r][j] - base);
+        sum += e;
+        ps[(ty * RT + r) * (GK + 1) + tx + 8 * j] = e;
+      }
+#pragma unroll
+      for (int w = 4; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+      l[r] = l[r] * corr + sum;
+      m[r] = m_new;
+#pragma unroll
+      for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[r][c][e] *= corr;
+    }
+    __syncwarp();
+#pragma unroll 4
+    for (int k = 0; k < GK; ++k) {
+      float p[RT];
+#pragma unroll
+      for (int r = 0; r < RT; ++r) p[r] = ps[(ty * RT + r) * (GK + 1) + k];
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        const float4 v = *(const float4*)(vs + k * LD + tx * 4 + c * 32);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          o[r][c][0] = fmaf(p[r], v.x, o[r][c][0]);
+          o[r][c][1] = fmaf(p[r], v.y, o[r][c][1]);
+          o[r][c][2] = fmaf(p[r], v.z, o[r][c][2]);
+          o[r][c][3] = fmaf(p[r], v.w, o[r][c][3]);
+        }
+      }
+    }
+    __syncwarp();
+  }
+  auto put = [&](int64_t x, int col, float v) {
+    if (x < n * rep && col < a.d) store_as((T*)a.out + ((tok0 + x / rep) * a.nh + kvh * rep + x % rep) * a.d + col, v);
+  };
+  if (slices == 1) {
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const float f = l[r] > 0.f ? 1.f / l[r] : 0.f;
+#pragma unroll
+      for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) put(x0 + ty * RT + r, tx * 4 + c * 32 + e, o[r][c][e] * f);
+    }
+    return;
+  }
+  // the shares are joined: a block has some of the rows
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const int x = ty * RT + r;
+    if (tx == 0) { ml[0][x] = m[r]; ml[1][x] = l[r]; }
+#pragma unroll
+    for (int c = 0; c < CT; ++c) *(float4*)(qs + x * LD + tx * 4 + c * 32) = make_float4(o[r][c][0], o[r][c][1], o[r][c][2], o[r][c][3]);
+  }
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  auto remote = [](const float* p, int rank) {
+    uint32_t at;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"((uint32_t)rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+  };
+  for (int x = slice; x < QR && x0 + x < n * rep; x += slices) {
+    float top = -INFINITY, sum = 0.f;
+    for (int s = 0; s < slices; ++s) top = fmaxf(top, remote(&ml[0][x], s));
+    const float base = top == -INFINITY ? 0.f : top;
+    for (int s = 0; s < slices; ++s) sum += remote(&ml[1][x], s) * expf(remote(&ml[0][x], s) - base);
+    const float f = sum > 0.f ? 1.f / sum : 0.f;
+    for (int c = tid; c < a.d; c += 128) {
+      float v = 0.f;
+      for (int s = 0; s < slices; ++s) v += remote(qs + x * LD + c, s) * expf(remote(&ml[0][x], s) - base);
+      put(x0 + x, c, v * f);
+    }
+  }
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <typename T, int D, int QR>
+int launch_any(cg_ctx* c, const PagedAttnArgs& a) {
+  constexpr size_t smem = (size_t)((QR + 2 * GK) * (D + 4) + QR * (GK + 1)) * 4;
+  static PerDeviceFlag configured_on;
+  bool& configured = configured_on.at(c->core->device);
+  if (!configured) {
+    CG_CUDA(c, cudaFuncSetAttribute(k_paged_attn<T, D, QR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    configured = true;
+  }
+  const int64_t tiles = (a.most * (a.nh / a.nkv) + QR - 1) / QR * a.nkv;
+  if (tiles > 0x7FFFFFFFll) return fail(c, CG_ERR_UNSUPPORTED, "too many tokens");
+  int slices = 1;  // blocks that share the keys: until the GPU is full
+  while (slices < 8 && tiles * a.rows.rows * slices < 148 * 2) slices *= 2;
+  CG_CUDA(c, launch_kernel(c, k_paged_attn<T, D, QR>, dim3((unsigned)tiles, (unsigned)a.rows.rows, (unsigned)slices), dim3(128), smem, slices, a));
+  CG_LAUNCHED(c);
+  return CG_OK;
+}
+
+template <typename T>
+int launch_typed(cg_ctx* c, const PagedAttnArgs& a) {
+  const bool few = a.most * (a.nh / a.nkv) <= 32;
+  if (a.d <= 64) return few ? launch_any<T, 64, 16>(c, a) : launch_any<T, 64, 64>(c, a);
+  if (a.d <= 128) return few ? launch_any<T, 128, 16>(c, a) : launch_any<T, 128, 64>(c, a);
+  return few ? launch_any<T, 256, 16>(c, a) : launch_any<T, 256, 64>(c, a);
+}
+
+}  // namespace
+
+}  // namespace cg
+
+using namespace cg;
+
+extern "C" int32_t cg_paged_attention(cg_ctx* c, const cg_tensor* q, const cg_tensor* k_pages, const cg_tensor* v_pages, const cg_tensor* table,
+                                      const cg_tensor* starts, const cg_tensor* lens, int64_t max_new, float scale, int64_t window, float softcap,
+                                      cg_tensor* out) {
+  if (!c) return CG_ERR_INVALID;
+  CG_LAZY_EAGER_SCOPE(c);
+  OnDevice on(c);
+  if (!q || !out) return fail(c, CG_ERR_INVALID, "null argument");
+  PagedAttnArgs a = {};
+  int lg;
+  CG_TRY(check_pages(c, k_pages, v_pages, false, &lg));
+  const int64_t nkv = k_pages->dims[1], d = k_pages->dims[3], any[3] = {-1, -1, d};
+  CG_TRY(check_tensor(c, q, "q", CG_F32, 3, any, false));
+  const int64_t M = q->dims[0], nh = q->dims[1];
+  CG_TRY(check_tensor(c, out, "out", CG_F32, 3, q->dims));
+  CG_TRY(check_rows(c, table, starts, lens, M, k_pages->dims[0], lg, &a.rows));
+  if (q->storage != k_pages->storage || out->storage != k_pages->storage) return fail(c, CG_ERR_DTYPE, "q and out are stored as the pages are");
+  if (M > 0 && q->strides[2] != 1) return fail(c, CG_ERR_UNSUPPORTED, "q: the last axis must be contiguous");
+  if (nkv < 1 || nkv > 65535 || nh > 65535) return fail(c, CG_ERR_UNSUPPORTED, "too many heads");
+  if (nh % nkv) return fail(c, CG_ERR_SHAPE, "query heads are a multiple of key heads");
+  if (max_new < 0 || window < 0 || !(softcap >= 0.f) || !(scale >= 0.f) || scale > 3e38f || softcap > 3e38f) return fail(c, CG_ERR_INVALID, "bad argument");
+  for (const cg_tensor* in : {q, k_pages, v_pages, table, starts, lens})
+    if (overlap(in, out)) return fail(c, CG_ERR_INVALID, "out overlaps an input");
+  if (M == 0 || nh == 0 || a.rows.rows == 0) return CG_OK;
+  a.q = q->data(); a.k_pages = k_pages->data(); a.v_pages = v_pages->data(); a.out = out->data();
+  a.q_ld = q->strides[0]; a.q_hs = q->strides[1];
+  a.most = max_new > 0 ? std::min(max_new, M) : M;
+  a.window = window;
+  a.scale = scale > 0.f ? scale : 1.f / sqrtf((float)d);
+  a.cap = softcap;
+  a.nh = (int)nh; a.nkv = (int)nkv; a.d = (int)d;
+  written(out);
+  return q->storage == ST_BF16 ? launch_typed<__nv_bfloat16>(c, a) : launch_typed<float>(c, a);
+}

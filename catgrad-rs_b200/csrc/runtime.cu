@@ -372,6 +372,51 @@ int32_t cg_sync(cg_ctx* c) {
 }
 
 void* cg_ctx_stream(cg_ctx* c) { return c ? (void*)c->core->stream : nullptr; }
+int32_t cg_tensor_from_device(cg_ctx* c, void* data, int32_t storage, const int64_t* dims, const int64_t* strides, int32_t rank, cg_tensor** out) {
+  if (!c || !out || rank < 0 || rank > CG_MAX_RANK || (rank && !dims)) return fail(c, CG_ERR_INVALID, "bad argument");
+  if (storage != ST_F32 && storage != ST_U32 && storage != ST_BF16) return fail(c, CG_ERR_DTYPE, "unknown storage");
+  int64_t n = 1, last = 0, step = 1;
+  int64_t st[CG_MAX_RANK];
+  for (int i = rank - 1; i >= 0; --i) {
+    st[i] = strides ? strides[i] : step;
+    if (dims[i] < 0 || st[i] < 0) return fail(c, CG_ERR_SHAPE, "negative dimension or stride");
+    if (__builtin_mul_overflow(n, dims[i], &n) || __builtin_mul_overflow(step, std::max<int64_t>(dims[i], 1), &step)) return fail(c, CG_ERR_SHAPE, "too large");
+    int64_t far;
+    if (__builtin_mul_overflow(std::max<int64_t>(dims[i], 1) - 1, st[i], &far) || __builtin_add_overflow(last, far, &last) || last > (1ll << 60))
+      return fail(c, CG_ERR_SHAPE, "too large");
+  }
+  if ((uintptr_t)data % storage_bytes(storage)) return fail(c, CG_ERR_INVALID, "data is not aligned to its elements");
+  if (n) {
+    cudaPointerAttributes at;
+    if (!data || cudaPointerGetAttributes(&at, data) != cudaSuccess || (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged) ||
+        (at.type == cudaMemoryTypeDevice && at.device != c->core->device)) {
+      cudaGetLastError();
+      return fail(c, CG_ERR_INVALID, "data is not memory of the context's device");
+    }
+  }
+  try {
+    auto buf = std::make_shared<Buffer>();
+    buf->core = c->core;
+    buf->ptr = data;
+    buf->bytes = n ? (size_t)(last + 1) * storage_bytes(storage) : 0;
+    buf->owned = false;
+    auto* t = new cg_tensor();
+    t->ctx = c;
+    t->tag = storage == ST_U32 ? CG_U32 : CG_F32;
+    t->storage = storage;
+    t->rank = rank;
+    for (int i = 0; i < rank; ++i) {
+      t->dims[i] = dims[i];
+      t->strides[i] = st[i];
+    }
+    t->buf = buf;
+    *out = t;
+  } catch (const std::bad_alloc&) {
+    return CG_ERR_OOM;
+  }
+  return CG_OK;
+}
+
 int64_t cg_launch_count(cg_ctx* c) { return c ? c->launches : 0; }
 int64_t cg_bytes_reserved(cg_ctx* c) { return c ? c->core->reserved : 0; }
 

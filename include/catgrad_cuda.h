@@ -272,6 +272,69 @@ int32_t cg_fused_moe(cg_ctx*, const cg_tensor* x, const cg_tensor* router, const
                      const cg_tensor* up, const cg_tensor* down, int32_t top_k, int32_t norm_topk,
                      int32_t act, cg_tensor** out, cg_tensor** ids_out);
 
+/* A tensor over device memory of the caller (storage as cg_storage_of; strides in elements, not
+ * negative, NULL = contiguous): nothing is copied, and the memory stays the caller's, who keeps it
+ * while the tensor or a view of it lives and orders its own work on other streams against the
+ * context's.  Tensors are written by the operators below, which say so, and by cg_comm_all_reduce. */
+int32_t cg_tensor_from_device(cg_ctx*, void* data, int32_t storage, const int64_t* dims, const int64_t* strides,
+                              int32_t rank, cg_tensor** out);
+
+/* --- several sequences over a paged key/value cache, and beam search.  No counterpart in the
+ * reference, whose caches are contiguous and whose decoding is greedy; the mathematics is that of
+ * cg_fused_rmsnorm, cg_fused_rope and cg_fused_attention.
+ * A cache (per layer) is k_pages and v_pages [n_pages, kv heads, page, d], stored alike in f32 or
+ * bf16: page 8, 16, .. 1024 tokens, d a multiple of 8 up to 256, on a 16-byte boundary.  Row r of a
+ * batch has the packed tokens starts[r] .. starts[r + 1] (U32 [rows + 1], ascending; possibly none);
+ * lens[r] (U32 [rows]) of its tokens are cached, the new ones among them, so its new token i of n
+ * stands at position lens[r] - n + i; position p lies in page table[r][p / page] (U32 [rows, cols])
+ * at place p % page.  All these live on the device and may change between replays of a captured
+ * graph: the operators take no memory and wait for nothing.  They write into tensors the caller
+ * holds (contiguous; they overlap no input) and leave what belongs to no row's token as it was.
+ * A table entry, length or token count that is out of range is not followed: the next cg_sync
+ * returns CG_ERR_INDEX, and what depends on it is not written (in attention, keys and values of a
+ * page that does not exist count as zeros).  Rows must not name the same place for two tokens. */
+
+/* Each new token's k and v (and q, may be NULL with q_out) [tokens, heads, d], f32 or bf16, any
+ * strides but the last: with gains [d] q and k become x / sqrt(mean x^2 + eps) * gain (1 + gain with
+ * plus_one), head by head; with cos, sin [T, n] f32 (cg_rope_tables), n <= d / 2, their first 2 n
+ * components are then turned by the angles of the token's position, component i with i + n
+ * (rot_half) or 2 i with 2 i + 1.  All in f32, rounded once to the pages' type: k, v go to their
+ * pages, q to q_out [tokens, heads, d]. */
+int32_t cg_paged_append(cg_ctx*, const cg_tensor* q, const cg_tensor* k, const cg_tensor* v, const cg_tensor* q_gain,
+                        const cg_tensor* k_gain, float eps, int32_t plus_one, const cg_tensor* cos, const cg_tensor* sin,
+                        int32_t rot_half, const cg_tensor* table, const cg_tensor* starts, const cg_tensor* lens,
+                        cg_tensor* k_pages, cg_tensor* v_pages, cg_tensor* q_out);
+/* Attention of the new tokens q [tokens, heads, d] over their rows' cached tokens up to their own
+ * position (so after cg_paged_append), into out [tokens, heads, d]; q and out are stored as the
+ * pages.  heads is a multiple of kv heads, grouped as in cg_fused_attention.  max_new: no row has
+ * more new tokens (0 = not known); a row that has more is left out (CG_ERR_INDEX).  scale 0 =
+ * 1 / sqrt(d).  window > 0: only the last `window` tokens are seen; pages before all windows of a
+ * row are not read, so their table entries may be stale.  softcap > 0 as in cg_fused_attention.
+ * What is cached at a row's positions is finite. */
+int32_t cg_paged_attention(cg_ctx*, const cg_tensor* q, const cg_tensor* k_pages, const cg_tensor* v_pages,
+                           const cg_tensor* table, const cg_tensor* starts, const cg_tensor* lens, int64_t max_new,
+                           float scale, int64_t window, float softcap, cg_tensor* out);
+/* One step of beam search for groups of J beams: of the continuations (beam j, token v) with
+ *   scores[j] + log softmax(logits[j])[v]
+ * the K largest in descending order, equal ones by j, then v.  logits [B, J, V] f32 or bf16, scores
+ * [B, J] f32 (-inf: a beam that is not there), finished U32 [B, J] or NULL: a finished beam's only
+ * continuation is `end` at an unchanged score.  NaN logits count as -inf; a beam whose largest logit
+ * or score is not finite has -inf everywhere.  Outputs [B, K] (K <= V, J and K at most 32): scores,
+ * tokens, parents (beams of the group) and finished (the parent was, or the token is `end`).
+ * scores_out and finished_out may be scores and finished themselves when K = J. */
+int32_t cg_beam_select(cg_ctx*, const cg_tensor* logits, const cg_tensor* scores, const cg_tensor* finished, uint32_t end,
+                       cg_tensor* scores_out, cg_tensor* tokens_out, cg_tensor* parents_out, cg_tensor* finished_out);
+/* The caches of B groups of K beams (rows b K + j of lens [B K] and table [B K, cols]) go on from
+ * parents U32 [B, K] (of the group), in place.  own U32 [B K, cols]: the page a row writes itself in
+ * each column; from the column on that its length has begun, no two rows' are the same.  With n full pages: columns below n of
+ * table become the parent's, the others own's, and the tokens in the begun page (column n of own)
+ * are copied from the parent's, in k_pages and v_pages, which here may be all layers'
+ * [layers, n_pages, ..] at once.  The rows of a group are equally long, else (or with a parent that
+ * is not of the group) the group is left as it was and CG_ERR_INDEX raised.  Before the first
+ * step all rows' tables are own's; a group's first step may have all parents 0, which shares the prompt's pages. */
+int32_t cg_paged_reorder(cg_ctx*, const cg_tensor* parents, const cg_tensor* lens, const cg_tensor* own, cg_tensor* table,
+                         cg_tensor* k_pages, cg_tensor* v_pages);
+
 /* --- decoder runner: the greedy loop of catgrad-llm/examples/llama/main.rs:118-169 with a
  * device KV cache (cache semantics of catgrad-llm/src/legacy/models/utils.rs:210-228). --- */
 

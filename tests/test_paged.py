@@ -1,0 +1,710 @@
+"""The operators on a paged key/value cache and beam search against plain restatements in 64 bits.
+
+Tolerances.  2^-24 is half a step of f32, 2^-8 of bf16, relative to the value; every bound below counts roundings.
+
+* append, f32: a sum of at most 256 squares in a tree of 4 + 5 levels and 4 products (10 roundings, halved by the root), the root,
+  the division, two products, then two products and a sum of the rotation: under 16 half steps of |u| + |w|, the pair's sizes.
+  Kept in bf16 one half step of 2^-8 more.
+* attention, f32: a score is a sum of d products (d + 2 roundings of the sum of their sizes), of which an exponential takes the
+  difference to the maximum; a probability is then off by twice that, and the exponential's, the sums' and the division's
+  roundings; the output by as much of the largest value.
+* attention, bf16: products of bf16 values are exact in f32 and their sums as above; the probabilities may be rounded to bf16, above
+  and below the fraction: 2 half steps of sum p |v|; the result one more.
+"""
+import ctypes
+import math
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+from conftest import ROOT, cg
+
+gpu = pytest.mark.gpu
+F32, BF16 = 2.0 ** -24, 2.0 ** -8
+
+
+# ---------------------------------------------------------------- on the GPU box
+
+
+def put(B, a, store="f32"):
+    """A device tensor of the library over torch memory, and that memory."""
+    import torch
+    a = np.asarray(a)
+    t = torch.from_numpy(a.astype(np.int64) if a.dtype.kind in "ui" else a).cuda()
+    t = t.to(torch.int32) if a.dtype.kind in "ui" else t.to({"f32": torch.float32, "bf16": torch.bfloat16}[store])
+    t = t.contiguous()
+    torch.cuda.synchronize()
+    return B.from_device(t), t
+
+
+def rounded(a, store):
+    return cg.synth.bf16_round(np.asarray(a, np.float32)) if store == "bf16" else np.asarray(a, np.float32)
+
+
+def back(B, t):
+    B.sync()
+    return t.float().cpu().numpy().astype(np.float64) if t.is_floating_point() else t.cpu().numpy()
+
+
+class Batch:
+    """Rows with new[r] of total[r] cached tokens, pages in any order; `spare` more packed tokens behind the last row, `extra` more columns and
+    pages."""
+
+    def __init__(self, new, total, page, seed=0, spare=0, extra=1):
+        rng = np.random.default_rng(seed)
+        self.new, self.total, self.page = new, total, page
+        self.starts = np.concatenate([[0], np.cumsum(new)]).astype(np.uint32)
+        self.M = int(self.starts[-1]) + spare
+        self.cols = max(-(-t // page) for t in total) + extra
+        self.n_pages = len(new) * self.cols + 3
+        self.table = rng.permutation(self.n_pages)[:len(new) * self.cols].reshape(len(new), self.cols).astype(np.uint32)
+        self.lens = np.array(total, np.uint32)
+        self.rng = rng
+
+    def up(self, B):
+        return [put(B, x)[0] for x in (self.table, self.starts, self.lens)]
+
+    def gather(self, pages, r):
+        """[tokens, heads, d] of row r's cached tokens."""
+        t = self.total[r]
+        at = np.arange(t)
+        return pages[self.table[r, at // self.page], :, at % self.page]
+
+    def tokens(self):
+        """(packed token, row, position)"""
+        for r, (n, t) in enumerate(zip(self.new, self.total)):
+            for i in range(n):
+                yield int(self.starts[r]) + i, r, t - n + i
+
+
+SHAPES = [([1], [1], 8), ([1, 1, 1], [5, 16, 17], 16), ([3, 0, 7, 1], [3, 0, 12, 64], 8), ([0, 0, 2], [9, 0, 2], 16), ([70, 1, 33], [70, 200, 40], 64),
+          ([5] * 40, [5 + r for r in range(40)], 32)]
+
+
+@gpu
+@pytest.mark.parametrize("into,pages", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16"), ("bf16", "f32")])
+@pytest.mark.parametrize("nh,nkv,d,turned", [(4, 2, 64, 64), (3, 1, 128, 128), (8, 8, 256, 64), (2, 1, 8, 8), (5, 5, 24, 16), (4, 4, 40, 0), (7, 1, 96, 96)])
+@pytest.mark.parametrize("norms,halves,plus", [(False, True, False), (True, True, False), (True, False, True)])
+def test_append(cuda, into, pages, nh, nkv, d, turned, norms, halves, plus):
+    for i, (new, total, page) in enumerate(SHAPES):
+        check_append(cuda, Batch(new, total, page, seed=i, spare=i % 3), into, pages, nh, nkv, d, turned, norms, halves, plus)
+
+
+def check_append(B, b, into, pages, nh, nkv, d, turned, norms, halves, plus, split=False):
+    import torch
+    rng = b.rng
+    q, k, v = (rounded(rng.standard_normal((b.M, h, d)) * 1.5, into) for h in (nh, nkv, nkv))
+    gains = [rounded(1.0 + 0.2 * rng.standard_normal(d), "f32") for _ in range(2)] if norms else [None, None]
+    T = max(b.total) + 2
+    angle = np.arange(T)[:, None] * 100.0 ** (-np.arange(turned // 2) / max(1, turned // 2))
+    cos, sin = np.cos(angle).astype(np.float32), np.sin(angle).astype(np.float32)
+    old = [rounded(rng.standard_normal((b.n_pages, nkv, b.page, d)), pages) for _ in range(2)]
+    kp, vp = (put(B, x, pages) for x in old)
+    q_old = rounded(rng.standard_normal((b.M, nh, d)), pages)
+    qo = put(B, q_old, pages)
+    if split:   # three parts of one projection, from an odd place on
+        both = torch.from_numpy(np.concatenate([q, k, v], 1)).to(torch.bfloat16 if into == "bf16" else torch.float32)
+        flat = torch.zeros(both.numel() + 3, dtype=both.dtype, device="cuda")
+        flat[3:] = both.reshape(-1).cuda()
+        whole = flat[3:].reshape(b.M, nh + 2 * nkv, d)
+        torch.cuda.synchronize()
+        qd, kd, vd = (B.from_device(x) for x in (whole[:, :nh], whole[:, nh:nh + nkv], whole[:, nh + nkv:]))
+    else:
+        qd, kd, vd = (put(B, x, into)[0] for x in (q, k, v))
+    table, starts, lens = b.up(B)
+    g = [None if x is None else put(B, x)[0] for x in gains]
+    angles = [put(B, x)[0] for x in (cos, sin)] if turned else [None, None]
+    B.paged_append(kd, vd, kp[0], vp[0], table, starts, lens, q=qd, q_out=qo[0], cos=angles[0], sin=angles[1], q_gain=g[0], k_gain=g[1], eps=1e-5,
+                   plus_one=plus, rot_half=halves)
+    want_q, want_k, want_v = q_old.astype(np.float64), old[0].astype(np.float64), old[1].astype(np.float64)
+    lim_q, lim_k = np.zeros_like(want_q), np.zeros_like(want_k)
+    n = turned // 2
+    a0 = np.arange(n) if halves else 2 * np.arange(n)
+    a1 = a0 + n if halves else a0 + 1
+    for m, r, pos in b.tokens():
+        done = []
+        for x, gain in ((q[m], gains[0]), (k[m], gains[1])):
+            x = x.astype(np.float64)
+            if gain is not None:
+                x = x / np.sqrt((x * x).mean(-1, keepdims=True) + 1e-5) * (gain.astype(np.float64) + plus)
+            size = np.abs(x)
+            u, w = x[:, a0].copy(), x[:, a1].copy()
+            c, s = cos[pos].astype(np.float64), sin[pos].astype(np.float64)
+            x[:, a0], x[:, a1] = u * c - w * s, w * c + u * s
+            size[:, a0] = size[:, a1] = np.abs(u) + np.abs(w)
+            done.append((x, 16 * F32 * size + (BF16 * np.abs(x) * (1 + 2.0 ** -8) if pages == "bf16" else 0)))
+        at, place = b.table[r, pos // b.page], pos % b.page
+        want_q[m], lim_q[m] = done[0]
+        want_k[at, :, place], lim_k[at, :, place] = done[1]
+        want_v[at, :, place] = rounded(v[m], pages)
+    assert (np.abs(back(B, qo[1]) - want_q) <= lim_q).all()
+    assert (np.abs(back(B, kp[1]) - want_k) <= lim_k).all()
+    assert np.array_equal(back(B, vp[1]), want_v)
+
+
+@gpu
+@pytest.mark.parametrize("into,pages", [("f32", "bf16"), ("bf16", "bf16"), ("f32", "f32")])
+@pytest.mark.parametrize("nh,nkv,d", [(4, 2, 64), (3, 1, 128), (2, 2, 40)])
+def test_append_parts_of_a_projection(cuda, into, pages, nh, nkv, d):
+    check_append(cuda, Batch([3, 1, 40], [3, 66, 41], 16, spare=2), into, pages, nh, nkv, d, d, True, True, False, split=True)
+
+
+def attention(q, k, v, pos, scale, window, cap):
+    """One query [heads, d] of kv-grouped keys [t, kv heads, d]: (output, sum p |v|, score size)."""
+    rep = q.shape[0] // k.shape[1]
+    t = np.arange(k.shape[0])
+    seen = (t <= pos) & ((t > pos - window) if window else True)
+    k, v = np.repeat(k[seen], rep, 1), np.repeat(v[seen], rep, 1)
+    x = np.einsum("hd,thd->ht", q, k) * scale
+    size = (np.einsum("hd,thd->ht", np.abs(q), np.abs(k)) * scale).max(1)
+    if cap:
+        x = cap * np.tanh(x / cap)
+    p = np.exp(x - x.max(1, keepdims=True))
+    p /= p.sum(1, keepdims=True)
+    return np.einsum("ht,thd->hd", p, v), np.einsum("ht,thd->hd", p, np.abs(v)), size
+
+
+def check_attention(B, b, store, nh, nkv, d, window=0, cap=0.0, scale=0.0, spread=1.0, stale=None, strided=False, max_new=None, check=None):
+    import torch
+    rng = b.rng
+    q = rounded(rng.standard_normal((b.M, nh, d)) * spread, store)
+    k, v = (rounded(rng.standard_normal((b.n_pages, nkv, b.page, d)), store) for _ in range(2))
+    if stale is not None:   # whatever is no row's token
+        used = np.zeros((b.n_pages, b.page), bool)
+        for r, t in enumerate(b.total):
+            first = max(0, t - b.new[r] - window + 1) // b.page * b.page if window else 0
+            at = np.arange(first, t)
+            used[b.table[r, at // b.page], at % b.page] = True
+        for x in (k, v):
+            x.transpose(0, 2, 1, 3)[~used] = stale
+    old = rounded(rng.standard_normal((b.M, nh, d)), store)
+    out, kd, vd = put(B, old, store), put(B, k, store), put(B, v, store)
+    if strided:
+        wide = torch.zeros(b.M, nh + 3, d + 8, device="cuda").to(kd[1].dtype)
+        wide[:, :nh, :d] = torch.from_numpy(q).cuda()
+        torch.cuda.synchronize()
+        qd = (B.from_device(wide[:, :nh, :d]), wide)
+    else:
+        qd = put(B, q, store)
+    table, starts, lens = b.up(B)
+    B.paged_attention(qd[0], kd[0], vd[0], table, starts, lens, max_new=max(b.new) if max_new is None else max_new, scale=scale, window=window,
+                      softcap=cap, out=out[0])
+    got = back(B, out[1])
+    want, lim = old.astype(np.float64), np.zeros((b.M, nh, d))
+    f = scale or 1.0 / math.sqrt(d)
+    cache = {}
+    for m, r, pos in b.tokens():
+        if check is not None and m not in check:
+            want[m] = got[m]
+            continue
+        if r not in cache:
+            cache = {r: (b.gather(k, r).astype(np.float64), b.gather(v, r).astype(np.float64))}
+        kk, vv = cache[r]
+        lo = max(0, pos - window + 1) if window else 0
+        want[m], mass, size = attention(q[m].astype(np.float64), kk[lo:pos + 1], vv[lo:pos + 1], pos - lo, f, 0, cap)
+        off = 2 * (d + 6) * F32 * size[:, None] + (pos - lo + 24) * F32
+        lim[m] = off * np.abs(vv[lo:pos + 1]).max() + (BF16 * (np.abs(want[m]) + 2 * mass) * (1 + 2.0 ** -7) if store == "bf16" else 0)
+    bad = ~(np.abs(got - want) <= lim)
+    assert not bad.any(), (bad.sum(), np.argwhere(bad)[:4], np.abs(got - want).max())
+
+
+HEADS = [(4, 2, 64), (8, 1, 128), (2, 2, 256), (3, 3, 24), (6, 2, 96), (5, 1, 64), (32, 1, 128), (2, 1, 8), (8, 2, 40)]
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+@pytest.mark.parametrize("nh,nkv,d", HEADS)
+@pytest.mark.parametrize("window,cap", [(0, 0.0), (7, 0.0), (0, 3.0), (33, 20.0)])
+def test_attention(cuda, store, nh, nkv, d, window, cap):
+    for i, (new, total, page) in enumerate(SHAPES):
+        check_attention(cuda, Batch(new, total, page, seed=i, spare=i % 3), store, nh, nkv, d, window, cap, spread=2.0, strided=i % 2 == 1,
+                        scale=0.0 if i % 3 else 0.3)
+
+
+# around tiles of 16 to 128 keys and queries, shares of the keys, pages that end inside a tile
+EDGES = [1, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 257, 300]
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+@pytest.mark.parametrize("nh,nkv,d", [(8, 2, 64), (4, 4, 128), (4, 2, 256), (16, 1, 64)])
+@pytest.mark.parametrize("page", [8, 16, 128, 1024])
+def test_attention_single_tokens(cuda, store, nh, nkv, d, page):
+    """One token each over every length; the number of rows decides how many shares the keys have."""
+    for lengths in (EDGES, EDGES[-3:], EDGES[-1:], [1], EDGES * 6):
+        check_attention(cuda, Batch([1] * len(lengths), lengths, page), store, nh, nkv, d, spread=2.0, stale=np.nan)
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+@pytest.mark.parametrize("nh,nkv,d", [(4, 2, 64), (2, 1, 128), (2, 2, 256), (1, 1, 80)])
+@pytest.mark.parametrize("page,window", [(8, 0), (16, 20), (64, 64), (256, 0), (32, 130)])
+def test_attention_prompts(cuda, store, nh, nkv, d, page, window):
+    """Rows of every length behind nothing and behind cached tokens; what is nobody's is NaN."""
+    check_attention(cuda, Batch(EDGES, EDGES, page), store, nh, nkv, d, window, spread=2.0, stale=np.nan)
+    check_attention(cuda, Batch(EDGES, [n + c for n, c in zip(EDGES, [90, 3, 64, 0, 1, 200, 31, 128, 5, 7, 61, 62, 63, 64, 65, 1])], page), store, nh, nkv, d,
+                    window, spread=2.0, stale=np.nan)
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attention_long(cuda, store, d):
+    """Long contexts of unequal length, single tokens and a prompt's end; some tokens are checked."""
+    check_attention(cuda, Batch([1, 1, 1], [9001, 40, 4096], 64), store, 4, 2, d, spread=3.0)
+    check_attention(cuda, Batch([1], [33333], 16), store, 8, 1, d, spread=3.0)
+    b = Batch([1500, 300], [2500, 4111], 32)
+    check_attention(cuda, b, store, 4, 2, d, spread=3.0, check={0, 127, 128, 700, 1499, 1500, 1799})
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+@pytest.mark.parametrize("d,n", [(64, 1), (64, 100), (128, 1), (128, 100), (256, 1), (256, 40)])
+def test_attention_skips_pages_before_the_window(cuda, store, d, n):
+    """Their table entries are stale: pages that do not exist, or that others filled with NaN."""
+    for page in (8, 16, 64):
+        b = Batch([n, n, 1], [n + 500, n + 77, 900], page)
+        window = 70
+        for r, (m, t) in enumerate(zip(b.new, b.total)):
+            gone = max(0, t - m - window + 1) // page
+            b.table[r, :gone] = 0xFFFFFFFF if r % 2 == 0 else b.n_pages - 1   # (the last page is nobody's, NaN)
+        check_stale(cuda, b, store, d, window)
+
+
+def check_stale(B, b, store, d, window):
+    used = set(b.table[b.table < b.n_pages].tolist()) - {b.n_pages - 1}
+    # the page that stands for freed ones belongs to no live column
+    for r, t in enumerate(b.total):
+        live = b.table[r, max(0, t - b.new[r] - window + 1) // b.page:]
+        for i, p in enumerate(live):
+            if p == b.n_pages - 1:
+                live[i] = next(x for x in range(b.n_pages - 1) if x not in used)
+                used.add(int(live[i]))
+    rng = b.rng
+    nh, nkv = 4, 2
+    q = rounded(rng.standard_normal((b.M, nh, d)), store)
+    k, v = (rounded(rng.standard_normal((b.n_pages, nkv, b.page, d)), store) for _ in range(2))
+    k[-1], v[-1] = np.nan, np.nan
+    out = put(B, np.zeros((b.M, nh, d), np.float32), store)
+    qd, kd, vd = (put(B, x, store)[0] for x in (q, k, v))
+    table, starts, lens = b.up(B)
+    B.paged_attention(qd, kd, vd, table, starts, lens, max_new=max(b.new), window=window, out=out[0])
+    got = back(B, out[1])      # (back() syncs: no error was raised)
+    for m, r, pos in b.tokens():
+        at = np.arange(max(0, pos - window + 1), pos + 1)
+        ids = b.table[r, at // b.page]
+        want, mass, size = attention(q[m].astype(np.float64), k[ids, :, at % b.page].astype(np.float64), v[ids, :, at % b.page].astype(np.float64), len(at) - 1,
+                                     1.0 / math.sqrt(d), 0, 0.0)
+        lim = (2 * (d + 6) * F32 * size.max() + 100 * F32) * 6 + (BF16 * (np.abs(want) + 2 * mass) * (1 + 2.0 ** -7) if store == "bf16" else 0)
+        assert (np.abs(got[m] - want) <= lim).all(), (m, r, pos)
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [1, 40])
+def test_bad_tables_are_reported_and_harm_nobody_else(cuda, store, n):
+    """A page that does not exist, a length beyond the table, more new tokens than the length or than max_new."""
+    def fresh():
+        return Batch([n, n, n], [n + 20, n + 5, n + 33], 16)
+    good = run_simple(cuda, fresh(), store)
+    cuda.sync()
+    spoil = [lambda b: b.table.__setitem__((1, 0), b.n_pages), lambda b: b.table.__setitem__((1, 0), 0xFFFFFFFF),
+             lambda b: b.lens.__setitem__(1, b.cols * 16 + 1), lambda b: b.lens.__setitem__(1, n - 1), lambda b: b.lens.__setitem__(1, 0xFFFFFFFF)]
+    for i, change in enumerate(spoil):
+        b = fresh()
+        change(b)
+        with pytest.raises(cg.BackendPanic) as e:
+            run_simple(cuda, b, store)
+        assert e.value.status == 6
+        got = run_simple(cuda, b, store, sync=False)
+        for part, want in zip(got, good):
+            if part.shape[0] == 3 * n:   # per token: the other rows' are right
+                assert np.array_equal(part[:n], want[:n]) and np.array_equal(part[2 * n:], want[2 * n:])
+                if i >= 2:
+                    assert (part[n:2 * n] == 0).all()
+    # a row of more tokens than the caller said
+    b = fresh()
+    with pytest.raises(cg.BackendPanic):
+        run_simple(cuda, b, store, max_new=n - 1 if n > 1 else None, bad_starts=n == 1)
+    cuda.sync()
+
+
+def run_simple(B, b, store, sync=True, max_new=None, bad_starts=False, d=64):
+    import torch
+    rng = np.random.default_rng(5)
+    nh, nkv = 4, 2
+    q, k, v = (rounded(rng.standard_normal((b.M, h, d)), store) for h in (nh, nkv, nkv))
+    kp, vp = (put(B, rounded(rng.standard_normal((b.n_pages, nkv, b.page, d)), store), store) for _ in range(2))
+    qo, out = (put(B, np.zeros((b.M, nh, d), np.float32), store) for _ in range(2))
+    qd, kd, vd = (put(B, x, store)[0] for x in (q, k, v))
+    if bad_starts:
+        b.starts[-1] = b.M + 1
+    table, starts, lens = b.up(B)
+    B.paged_append(kd, vd, kp[0], vp[0], table, starts, lens, q=qd, q_out=qo[0])
+    B.paged_attention(qd, kp[0], vp[0], table, starts, lens, max_new=max(b.new) if max_new is None else max_new, out=out[0])
+    if sync:
+        B.sync()
+    torch.cuda.synchronize()
+    try:
+        B.sync()
+    except cg.BackendPanic:
+        pass
+    return [t.float().cpu().numpy() for t in (qo[1], out[1], kp[1], vp[1])]
+
+
+@gpu
+def test_new_outputs_and_empty_batches(cuda):
+    b = Batch([2, 1], [5, 9], 8, spare=2)
+    rng = b.rng
+    q, k = (put(cuda, rng.standard_normal((b.M, h, 64)), "bf16") for h in (4, 2))
+    kp, vp = (put(cuda, np.zeros((b.n_pages, 2, 8, 64)), "bf16") for _ in range(2))
+    table, starts, lens = b.up(cuda)
+    q_out = cuda.paged_append(k[0], k[0], kp[0], vp[0], table, starts, lens, q=q[0])
+    out = cuda.paged_attention(q_out, kp[0], vp[0], table, starts, lens)
+    assert out.shape == (b.M, 4, 64) and cuda.storage_of(out) == 2
+    got = cuda.to_numpy(out)
+    assert np.abs(got[:3]).min(axis=(1, 2)).max() > 0 and (got[3:] == 0).all() and np.array_equal(cuda.to_numpy(q_out)[:3], back(cuda, q[1])[:3])
+    assert cuda.paged_append(k[0], k[0], kp[0], vp[0], table, starts, lens) is None
+    none = put(cuda, np.zeros((0, 4, 64)), "bf16")[0]
+    assert cuda.paged_attention(none, kp[0], vp[0], table, put(cuda, np.zeros(3, np.uint32))[0], lens).shape == (0, 4, 64)
+    cuda.sync()
+
+
+# ---------------------------------------------------------------- beam search
+
+
+def best(logits, scores, K, finished=None, end=None):
+    B, J, V = logits.shape
+    x = np.where(np.isnan(logits), -np.inf, logits).astype(np.float64) + 0.0
+    total = np.full((B, J, V), -np.inf)
+    for b in range(B):
+        for j in range(J):
+            s, m = float(scores[b, j]), x[b, j].max()
+            if not np.isfinite(s):
+                continue
+            if finished is not None and finished[b, j]:
+                total[b, j, end] = s
+            elif np.isfinite(m):
+                d = x[b, j] - m
+                total[b, j] = s + (d - np.log(np.exp(d).sum()))
+    flat = total.reshape(B, -1)
+    order = np.argsort(-flat, axis=1, kind="stable")[:, :K]
+    parent, token = order // V, order % V
+    done = (np.take_along_axis(finished, parent, 1) != 0 if finished is not None else False) | (token == (end if end is not None else -1))
+    return np.take_along_axis(flat, order, 1), token, parent, np.broadcast_to(done, order.shape)
+
+
+def check_select(B, logits, scores, K, finished=None, end=None, store="f32", pitch=0):
+    import torch
+    x = rounded(logits, store)
+    if pitch:
+        wide = torch.full((*x.shape[:2], x.shape[2] + pitch), 1e9, device="cuda", dtype=torch.bfloat16 if store == "bf16" else torch.float32)
+        wide[..., :x.shape[2]] = torch.from_numpy(x).cuda()
+        torch.cuda.synchronize()
+        ld = B.from_device(wide[..., :x.shape[2]])
+    else:
+        ld = put(B, x, store)[0]
+    scores = np.asarray(scores, np.float32)
+    fd = None if finished is None else put(B, finished.astype(np.uint32))[0]
+    more = {} if end is None else {"end": end}
+    got = B.beam_select(ld, put(B, scores)[0], K, finished=fd, **more)
+    s, t, p, f = (B.to_numpy(a) for a in got)
+    ws, wt, wp, wf = best(x, scores, K, finished, end)
+    assert np.array_equal(t, wt) and np.array_equal(p, wp) and np.array_equal(f, wf.astype(np.uint32)), (t, wt, p, wp)
+    # sums of exponentials 2^-20 of their value (f32 of 32 values, 5 levels of a warp; the exponential 2^-22 and its argument's rounding
+    # 2^-24 of up to 100), the result one rounding
+    fine = np.isfinite(ws)
+    assert np.array_equal(fine, np.isfinite(s)) and (np.abs(s[fine] - ws[fine]) <= F32 * np.abs(ws[fine]) + 2.0 ** -17).all()
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+@pytest.mark.parametrize("B,J,K,V", [(1, 1, 1, 1), (1, 1, 4, 5), (2, 3, 3, 31), (3, 4, 4, 999), (1, 8, 16, 8191), (2, 2, 2, 8193), (1, 4, 4, 32000), (5, 1, 32, 50257),
+                                     (1, 32, 32, 4097), (2, 16, 8, 65537), (1, 2, 32, 256000)])
+def test_select(cuda, store, B, J, K, V):
+    """Distinct values (in bf16 with ties between tokens, which go to the lower one)."""
+    rng = np.random.default_rng(B + J + K + V)
+    logits = rng.standard_normal((B, J, V)) * 3
+    scores = -10 - 3 * np.abs(rng.standard_normal((B, J)))
+    check_select(cuda, logits, scores, K, store=store)
+    done = (rng.random((B, J)) < 0.4).astype(np.uint32)
+    check_select(cuda, logits, scores, K, done, V // 3, store=store)
+    check_select(cuda, logits, scores, K, done * 0, V - 1, store=store, pitch=(V % 5) + 1)
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [40, 3000, 20001, 70000])
+def test_select_ties_and_masks(cuda, store, V):
+    rng = np.random.default_rng(V)
+    J, K = 4, 6
+    scores = np.float32([[-1.0, -1.0, -3.0, -2.0]])
+    level = np.zeros((1, J, V))
+    check_select(cuda, level, scores, K, store=store)                           # all alike: the lowest places of the best beam
+    check_select(cuda, level, np.float32([[-2.0] * 4]), K, store=store)         # of all beams
+    check_select(cuda, level - 0.0 * np.sign(rng.standard_normal(level.shape)), scores, K, store=store)   # 0 and -0
+    steps = np.floor(rng.standard_normal((1, J, V)) * 2)                         # few distinct values
+    check_select(cuda, steps, scores, K, store=store)
+    lowest = float(np.finfo(np.float32).min) if store == "f32" else -3.3895313892515355e38
+    for masked in (-np.inf, lowest, np.nan):
+        x = rng.standard_normal((1, J, V)) * 3
+        x[:, :, rng.random(V) < 0.9] = masked
+        check_select(cuda, x, scores, K, store=store)
+        x[:, :, :] = masked
+        x[:, 1, V - 1] = x[:, 2, 5] = 0.5                                        # one token left, or none
+        check_select(cuda, x, scores, K, store=store)
+        check_select(cuda, x, np.float32([[-np.inf, -np.inf, -3.0, np.nan]]), K, store=store)
+        check_select(cuda, x, scores, K, np.uint32([[0, 1, 0, 1]]), 7, store=store)
+    check_select(cuda, level - np.inf, scores, K, store=store)
+    x = rng.standard_normal((1, J, V))
+    x[0, 1, 3] = np.inf
+    check_select(cuda, x, scores, K, store=store)
+    check_select(cuda, rng.standard_normal((1, J, V)) * 3, np.float32([[0.0, -np.inf, -np.inf, -np.inf]]), K, store=store)   # the first step
+    check_select(cuda, rng.standard_normal((1, J, V)) * 3, np.float32([[-np.inf, np.inf, -5.0, -np.inf]]), K, np.uint32([[1, 1, 0, 0]]), 3, store=store)
+
+
+@gpu
+def test_select_in_place(cuda):
+    rng = np.random.default_rng(1)
+    x, s, f = rng.standard_normal((3, 4, 1000)) * 3, -np.abs(rng.standard_normal((3, 4))).astype(np.float32), np.uint32(rng.random((3, 4)) < 0.3)
+    x32 = rounded(x, "f32")
+    ld, sd, fd = put(cuda, x32)[0], put(cuda, s), put(cuda, f)
+    t, p = (put(cuda, np.zeros((3, 4), np.uint32)) for _ in range(2))
+    cuda.beam_select(ld, sd[0], 4, finished=fd[0], end=9, out=(sd[0], t[0], p[0], fd[0]))
+    ws, wt, wp, wf = best(x32, s, 4, f, 9)
+    assert np.array_equal(back(cuda, t[1]), wt) and np.array_equal(back(cuda, p[1]), wp) and np.array_equal(back(cuda, fd[1]), wf)
+    assert np.abs(back(cuda, sd[1]) - ws).max() < 1e-5
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+@pytest.mark.parametrize("K,layers,page,d,length", [(1, 0, 8, 64, 5), (2, 1, 16, 8, 16), (4, 3, 16, 64, 37), (5, 2, 8, 24, 40), (8, 2, 64, 128, 63), (16, 1, 32, 64, 33),
+                                                    (32, 2, 8, 64, 21), (3, 0, 32, 256, 1), (4, 1, 16, 64, 0)])
+def test_reorder(cuda, store, K, layers, page, d, length):
+    import torch
+    B, nkv = 3, 2
+    rng = np.random.default_rng(K + page)
+    cols = length // page + 2
+    n_pages = B * K * cols + 2
+    own = rng.permutation(n_pages)[:B * K * cols].reshape(B * K, cols).astype(np.uint32)
+    table = own.copy()
+    for b in range(B):
+        table[b * K:(b + 1) * K, :length // page] = own[b * K + rng.integers(0, K, (K, length // page)), np.arange(length // page)]
+    shape = (layers,) * (layers > 0) + (n_pages, nkv, page, d)
+    k, v = (rounded(rng.standard_normal(shape), store) for _ in range(2))
+    parents = np.stack([np.roll(np.arange(K), 1), np.zeros(K, np.int64), rng.integers(0, K, K)]).astype(np.uint32)   # a cycle, one for all, any
+    kd, vd, td = put(cuda, k, store), put(cuda, v, store), put(cuda, table)
+    pd, ld, od = put(cuda, parents)[0], put(cuda, np.full(B * K, length, np.uint32))[0], put(cuda, own)[0]
+    cuda.paged_reorder(pd, ld, od, td[0], kd[0], vd[0])
+    full, begun = divmod(length, page)
+    want_t, want = own.copy(), [k.copy(), v.copy()]
+    for b in range(B):
+        for j in range(K):
+            parent = b * K + int(parents[b, j])
+            want_t[b * K + j, :full] = table[parent, :full]
+            for to, x in zip(want, (k, v)):
+                to[..., own[b * K + j, full], :, :begun, :] = x[..., own[parent, full], :, :begun, :]
+    assert np.array_equal(back(cuda, td[1]).view(np.uint32), want_t)
+    assert np.array_equal(back(cuda, kd[1]), want[0]) and np.array_equal(back(cuda, vd[1]), want[1])
+
+
+@gpu
+def test_reorder_leaves_a_bad_group_as_it_was(cuda):
+    B, K, cols, page = 3, 4, 3, 8
+    rng = np.random.default_rng(3)
+    own = rng.permutation(40)[:B * K * cols].reshape(B * K, cols).astype(np.uint32)
+    k = rounded(rng.standard_normal((40, 2, page, 16)), "f32")
+    parents = np.uint32([[1, 1, 1, 1]] * B)
+    for name, change in [("parent", lambda p, l, o: p.__setitem__((1, 2), 4)), ("lens", lambda p, l, o: l.__setitem__(5, 12)),
+                         ("long", lambda p, l, o: l.__setitem__(slice(4, 8), 25)), ("page", lambda p, l, o: o.__setitem__((6, 1), 40)),
+                         ("same", lambda p, l, o: o.__setitem__((6, 1), o[5, 1]))]:
+        p, l, o, t = parents.copy(), np.full(B * K, 13, np.uint32), own.copy(), own.copy()
+        change(p, l, o)
+        kd, vd, td = put(cuda, k), put(cuda, k), put(cuda, t)
+        cuda.paged_reorder(put(cuda, p)[0], put(cuda, l)[0], put(cuda, o)[0], td[0], kd[0], vd[0])
+        with pytest.raises(cg.BackendPanic) as e:
+            cuda.sync()
+        assert e.value.status == 6, name
+        got_t, got = back(cuda, td[1]).view(np.uint32), back(cuda, kd[1])
+        assert np.array_equal(got_t[4:8], own[4:8]), name
+        for b in (0, 2):
+            assert (got_t[b * K:(b + 1) * K, 0] == own[b * K + 1, 0]).all() and np.array_equal(got[own[b * K + 3, 1]][:, :5], k[own[b * K + 1, 1]][:, :5])
+        mine = own[4:8, 1]
+        assert np.array_equal(got[mine], k[mine].astype(np.float64)), name
+
+
+# ---------------------------------------------------------------- refusals and index arithmetic, without a device
+
+
+@pytest.fixture(scope="module")
+def host(tmp_path_factory):
+    """The library's entry points with a context and tensors that no device stands behind: what is refused is refused before anything
+    is launched."""
+    cg.load_library()
+    out = str(tmp_path_factory.mktemp("paged") / "paged_host.so")
+    csrc = os.path.join(ROOT, "catgrad-rs_b200", "csrc")
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-fPIC", "-shared", "-I", csrc, "-I", f"{cuda}/include", os.path.join(ROOT, "tests", "paged_host.cpp"), "-o", out,
+                           cg.library_path(), f"-Wl,-rpath,{os.path.dirname(cg.library_path())}", "-L", f"{cuda}/lib64", "-lcudart"])
+    L = ctypes.CDLL(out)
+    vp, i64p = ctypes.c_void_p, ctypes.POINTER(ctypes.c_int64)
+    L.host_ctx.restype = vp
+    L.host_tensor.restype, L.host_tensor.argtypes = vp, [vp, ctypes.c_uint64, ctypes.c_int, ctypes.c_int, i64p, i64p]
+    L.host_device.argtypes = [vp, ctypes.c_int]
+    L.host_row_span.argtypes = [vp, vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, vp, vp]
+    L.host_page_of.argtypes = [vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, vp]
+    L.host_page_of.restype = ctypes.c_int64
+    return L
+
+
+class Host:
+    """Calls with named arguments that can be changed one at a time."""
+
+    def __init__(self, L):
+        self.L, self.ctx, self.next = L, ctypes.c_void_p(L.host_ctx()), 1 << 40
+        self.lib = ctypes.CDLL(cg.library_path())   # (functions of its own: their argument types are set here)
+        self.lib.cg_last_error.restype = ctypes.c_char_p
+        self.lib.cg_last_error.argtypes = [ctypes.c_void_p]
+
+    def t(self, *dims, store="f32", strides=None, at=None, shift=0):
+        n = len(dims)
+        if strides is None:
+            strides = [int(np.prod(dims[i + 1:], dtype=np.int64)) for i in range(n)]
+        if at is None:
+            at, self.next = self.next, self.next + (1 << 32)
+        a = lambda v: (ctypes.c_int64 * max(1, n))(*v)
+        return ctypes.c_void_p(self.L.host_tensor(self.ctx, at + shift, {"f32": 0, "u32": 1, "bf16": 2}[store], n, a(dims), a(strides)))
+
+    def _call(self, fn, wrap):
+        fn.argtypes = [ctypes.c_void_p] + [type(w) if w is not None else ctypes.c_void_p for w in wrap]
+        fn.restype = ctypes.c_int32
+        return fn(self.ctx, *wrap)
+
+
+def test_append_refusals(host):
+    """Every call here is refused (a call that were not would return CG_ERR_CUDA: there is no device)."""
+    H = Host(host)
+    u, t = (lambda *d: H.t(*d, store="u32")), H.t
+
+    def call(**kw):
+        a = dict(q=t(6, 4, 64), k=t(6, 2, 64), v=t(6, 2, 64), q_gain=t(64), k_gain=t(64), eps=1e-6, plus=0, cos=t(50, 32), sin=t(50, 32), half=1, table=u(3, 5),
+                 starts=u(4), lens=u(3), k_pages=t(20, 2, 16, 64, store="bf16"), v_pages=t(20, 2, 16, 64, store="bf16"), q_out=t(6, 4, 64, store="bf16"))
+        a.update(kw)
+        order = ("q", "k", "v", "q_gain", "k_gain", "eps", "plus", "cos", "sin", "half", "table", "starts", "lens", "k_pages", "v_pages", "q_out")
+        wrap = [ctypes.c_int32(a[n]) if n in ("plus", "half") else ctypes.c_float(a[n]) if n == "eps" else a[n] for n in order]
+        return H._call(H.lib.cg_paged_append, wrap)
+
+    SHAPE, DTYPE, INVALID, UNSUPPORTED = 1, 2, 3, 8
+    for name in ("k", "v", "table", "starts", "lens", "k_pages", "v_pages", "q", "q_out", "cos", "sin"):
+        assert call(**{name: None}) == INVALID, name
+    cases = [(SHAPE, dict(k=t(6, 3, 64))), (SHAPE, dict(v=t(5, 2, 64))), (SHAPE, dict(q=t(7, 4, 64))), (SHAPE, dict(q=t(6, 4, 32))), (SHAPE, dict(k=t(6, 128))),
+             (SHAPE, dict(q_out=t(6, 5, 64, store="bf16"))), (SHAPE, dict(k_gain=t(32))), (SHAPE, dict(cos=t(50, 40), sin=t(50, 40))), (SHAPE, dict(sin=t(49, 32))),
+             (SHAPE, dict(starts=u(3))), (SHAPE, dict(lens=u(4))), (SHAPE, dict(v_pages=t(20, 2, 16, 32, store="bf16"))), (SHAPE, dict(table=u(15))),
+             (DTYPE, dict(k=t(6, 2, 64, store="bf16"))), (DTYPE, dict(q_out=t(6, 4, 64))), (DTYPE, dict(v_pages=t(20, 2, 16, 64))), (DTYPE, dict(table=t(3, 5))),
+             (DTYPE, dict(lens=t(3))), (DTYPE, dict(cos=t(50, 32, store="bf16"))), (DTYPE, dict(q_gain=t(64, store="bf16"))), (DTYPE, dict(k=u(6, 2, 64))),
+             (UNSUPPORTED, dict(k=t(6, 2, 64, strides=[256, 128, 2]))), (UNSUPPORTED, dict(q_out=t(6, 4, 64, store="bf16", strides=[512, 64, 1]))),
+             (UNSUPPORTED, dict(k_pages=t(20, 2, 16, 64, store="bf16", strides=[4096, 2048, 128, 1]))), (UNSUPPORTED, dict(table=H.t(3, 5, store="u32", strides=[6, 1]))),
+             (UNSUPPORTED, dict(k_pages=t(20, 2, 16, 64, store="bf16", shift=2)))]
+    for page, d in ((12, 64), (4, 64), (2048, 64), (16, 12), (16, 264), (16, 4)):
+        cases.append((UNSUPPORTED, dict(k=t(6, 2, d), v=t(6, 2, d), q=t(6, 4, d), k_pages=t(20, 2, page, d, store="bf16"), v_pages=t(20, 2, page, d, store="bf16"))))
+    at = 7 << 44
+    cases += [(INVALID, dict(k_pages=t(20, 2, 16, 64, store="bf16", at=at), v_pages=t(20, 2, 16, 64, store="bf16", at=at))),
+              (INVALID, dict(k=t(6, 2, 64, at=at), k_pages=t(20, 2, 16, 64, store="bf16", at=at))),
+              (INVALID, dict(q_out=t(6, 4, 64, store="bf16", at=at), v_pages=t(20, 2, 16, 64, store="bf16", at=at, shift=64))),
+              (INVALID, dict(lens=H.t(3, store="u32", at=at), q_out=t(6, 4, 64, store="bf16", at=at)))]
+    for i, (want, kw) in enumerate(cases):
+        assert call(**kw) == want, (i, want, H.lib.cg_last_error(H.ctx))
+    far = t(6, 2, 64)
+    host.host_device(far, 1)
+    assert call(v=far) == INVALID and b"another device" in H.lib.cg_last_error(H.ctx)
+
+
+def test_attention_refusals(host):
+    H = Host(host)
+    u, t = (lambda *d: H.t(*d, store="u32")), (lambda *d, **k: H.t(*d, **{"store": "bf16", **k}))
+
+    def call(**kw):
+        a = dict(q=t(6, 4, 64), k_pages=t(20, 2, 16, 64), v_pages=t(20, 2, 16, 64), table=u(3, 5), starts=u(4), lens=u(3), most=6, scale=0.0, window=0, cap=0.0, out=t(6, 4, 64))
+        a.update(kw)
+        order = ("q", "k_pages", "v_pages", "table", "starts", "lens", "most", "scale", "window", "cap", "out")
+        wrap = [ctypes.c_int64(a[n]) if n in ("most", "window") else ctypes.c_float(a[n]) if n in ("scale", "cap") else a[n] for n in order]
+        return H._call(H.lib.cg_paged_attention, wrap)
+
+    SHAPE, DTYPE, INVALID, UNSUPPORTED = 1, 2, 3, 8
+    for name in ("q", "k_pages", "v_pages", "table", "starts", "lens", "out"):
+        assert call(**{name: None}) == INVALID, name
+    at = 7 << 44
+    for i, (want, kw) in enumerate([(SHAPE, dict(q=t(6, 5, 64), out=t(6, 5, 64))), (SHAPE, dict(q=t(6, 4, 32), out=t(6, 4, 32))), (SHAPE, dict(out=t(6, 4, 32))), (SHAPE, dict(q=t(24, 64))),
+                                    (SHAPE, dict(starts=u(5))), (DTYPE, dict(q=t(6, 4, 64, store="f32"))), (DTYPE, dict(out=t(6, 4, 64, store="f32"))), (DTYPE, dict(starts=t(4))),
+                                    (INVALID, dict(most=-1)), (INVALID, dict(window=-1)), (INVALID, dict(cap=-1.0)), (INVALID, dict(cap=float("nan"))), (INVALID, dict(scale=float("inf"))),
+                                    (INVALID, dict(scale=-0.5)), (UNSUPPORTED, dict(q=t(6, 4, 64, strides=[512, 128, 2]))), (UNSUPPORTED, dict(out=t(6, 4, 64, strides=[512, 64, 1]))),
+                                    (UNSUPPORTED, dict(k_pages=t(20, 2, 24, 64), v_pages=t(20, 2, 24, 64))), (INVALID, dict(q=t(6, 4, 64, at=at), out=t(6, 4, 64, at=at))),
+                                    (INVALID, dict(k_pages=t(20, 2, 16, 64, at=at), out=t(6, 4, 64, at=at, shift=1024)))]):
+        assert call(**kw) == want, (i, want, H.lib.cg_last_error(H.ctx))
+
+
+def test_select_and_reorder_refusals(host):
+    H = Host(host)
+    u, t = (lambda *d, **k: H.t(*d, store="u32", **k)), H.t
+    SHAPE, DTYPE, INVALID, UNSUPPORTED = 1, 2, 3, 8
+
+    def select(**kw):
+        a = dict(logits=t(2, 4, 100), scores=t(2, 4), finished=u(2, 4), end=7, so=t(2, 3), to=u(2, 3), po=u(2, 3), fo=u(2, 3))
+        a.update(kw)
+        return H._call(H.lib.cg_beam_select, [a["logits"], a["scores"], a["finished"], ctypes.c_uint32(a["end"]), a["so"], a["to"], a["po"], a["fo"]])
+
+    for name in ("logits", "scores", "so", "to", "po", "fo"):
+        assert select(**{name: None}) == INVALID, name
+    at = 7 << 44
+    wide = lambda k: dict(so=t(2, k), to=u(2, k), po=u(2, k), fo=u(2, k))
+    for i, (want, kw) in enumerate([(SHAPE, dict(scores=t(2, 5))), (SHAPE, dict(logits=t(8, 100))), (SHAPE, dict(so=t(3, 3))), (SHAPE, dict(po=u(2, 4))), (SHAPE, dict(finished=u(8))),
+                                    (SHAPE, dict(logits=t(2, 4, 2), end=1)), (DTYPE, dict(logits=u(2, 4, 100))), (DTYPE, dict(scores=t(2, 4, store="bf16"))), (DTYPE, dict(so=t(2, 3, store="bf16"))),
+                                    (DTYPE, dict(to=t(2, 3))), (INVALID, dict(end=100)), (UNSUPPORTED, dict(logits=t(2, 4, 100, strides=[800, 200, 2]))), (UNSUPPORTED, wide(33)),
+                                    (UNSUPPORTED, dict(logits=t(2, 33, 100), scores=t(2, 33), finished=u(2, 33))), (UNSUPPORTED, dict(to=u(2, 3, strides=[4, 1]))),
+                                    (SHAPE, dict(logits=t(2, 0, 100), scores=t(2, 0), finished=u(2, 0))), (UNSUPPORTED, dict(logits=t(1, 32, 1 << 24), scores=t(1, 32), finished=None, **{k: v for k, v in dict(so=t(1, 32), to=u(1, 32), po=u(1, 32), fo=u(1, 32)).items()})),
+                                    (INVALID, dict(scores=t(2, 4, at=at), so=t(2, 3, at=at))), (INVALID, dict(to=u(2, 3, at=at), po=u(2, 3, at=at))),
+                                    (INVALID, dict(logits=t(2, 4, 100, at=at), fo=u(2, 3, at=at))), (INVALID, dict(scores=t(2, 4, at=at), **{**wide(4), "so": t(2, 4, at=at, shift=4)}))]):
+        assert select(**kw) == want, (i, want, H.lib.cg_last_error(H.ctx))
+
+    def reorder(**kw):
+        a = dict(parents=u(2, 4), lens=u(8), own=u(8, 5), table=u(8, 5), k=t(3, 20, 2, 16, 64), v=t(3, 20, 2, 16, 64))
+        a.update(kw)
+        return H._call(H.lib.cg_paged_reorder, [a[n] for n in ("parents", "lens", "own", "table", "k", "v")])
+
+    for name in ("parents", "lens", "own", "table", "k", "v"):
+        assert reorder(**{name: None}) == INVALID, name
+    for i, (want, kw) in enumerate([(SHAPE, dict(parents=u(8))), (SHAPE, dict(lens=u(7))), (SHAPE, dict(own=u(8, 6))), (SHAPE, dict(table=u(7, 5))), (SHAPE, dict(k=t(20, 2, 16, 64))),
+                                    (SHAPE, dict(k=t(3, 20, 64), v=t(3, 20, 64))), (DTYPE, dict(parents=t(2, 4))), (DTYPE, dict(v=t(3, 20, 2, 16, 64, store="bf16"))),
+                                    (UNSUPPORTED, dict(parents=u(1, 33), lens=u(33), own=u(33, 5), table=u(33, 5))), (UNSUPPORTED, dict(table=u(8, 5, strides=[6, 1]))),
+                                    (INVALID, dict(own=u(8, 5, at=at), table=u(8, 5, at=at))), (INVALID, dict(lens=u(8, at=at), k=t(3, 20, 2, 16, 64, at=at))),
+                                    (INVALID, dict(table=u(8, 5, at=at), v=t(3, 20, 2, 16, 64, at=at)))]):
+        assert reorder(**kw) == want, (i, want, H.lib.cg_last_error(H.ctx))
+
+
+def test_rows_that_cannot_be_are_not_followed(host):
+    """row_span and page_of, on the CPU: everything they let through lies inside the tensors."""
+    rng = np.random.default_rng(0)
+    vp = lambda a: a.ctypes.data_as(ctypes.c_void_p)
+    some = 0
+    for _ in range(4000):
+        rows, cols, lg, M = int(rng.integers(1, 6)), int(rng.integers(1, 5)), 4, int(rng.integers(0, 40))
+        starts = np.sort(rng.integers(0, 40, rows + 1)).astype(np.uint32)
+        if rng.random() < 0.3:
+            starts[rng.integers(0, rows + 1)] = rng.choice([0, 5, 41, 0xFFFFFFFF, 0x80000000])
+        lens = rng.choice([0, 1, 7, 16, 30, cols * 16, cols * 16 + 1, 0xFFFFFFFF, 0x7FFFFFFF], rows).astype(np.uint32)
+        most = int(rng.choice([1, 5, 40]))
+        for r in range(rows):
+            out, err = np.zeros(3, np.int64), np.zeros(1, np.int32)
+            ok = host.host_row_span(vp(starts), vp(lens), rows, cols, lg, M, r, most, vp(out), vp(err))
+            a, b, n = int(starts[r]), int(starts[r + 1]), int(lens[r])
+            good = a < b <= M and b - a <= min(most, n) and n <= cols * 16
+            assert bool(ok) == good and err[0] == (0 if good or a == b else 1)
+            if ok:
+                some += 1
+                assert 0 <= out[0] and out[0] + out[1] <= M and 0 <= out[2] - out[1] and out[2] <= cols << lg
+    assert some > 300
+    table, err = np.uint32([3, 9, 10, 0xFFFFFFFF, 0, 1, 2, 4]), np.zeros(1, np.int32)
+    got = [host.host_page_of(vp(table), 4, 10, 4, r, p, vp(err)) for r in (0, 1) for p in (0, 15, 16, 31, 63, 47)]
+    assert got == [3, 3, 9, 9, -1, -1, 0, 0, 1, 1, 4, 2] and err[0] == 1
