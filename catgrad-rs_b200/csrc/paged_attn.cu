@@ -5,22 +5,11 @@
 #include <algorithm>
 
 #include "mma.cuh"
-#include "paged.h"
+#include "paged_attn.h"
 
 namespace cg {
 
 namespace {
-
-struct PagedAttnArgs {
-  PagedRows rows;
-  const void *q, *k_pages, *v_pages;
-  void* out;
-  int64_t q_ld, q_hs;   // from one token and one head of q to the next
-  int64_t most;         // new tokens of a row, at most
-  int64_t window;       // 0 = none
-  float scale, cap;     // cap 0 = none
-  int nh, nkv, d;
-};
 
 __device__ __forceinline__ void load8(const float* p, float* x) {
   const float4 a = *(const float4*)p, b = *((const float4*)p + 1);
@@ -287,5 +276,6 @@ extern "C" int32_t cg_paged_attention(cg_ctx* c, const cg_tensor* q, const cg_te
   a.cap = softcap;
   a.nh = (int)nh; a.nkv = (int)nkv; a.d = (int)d;
   written(out);
+  if (q->storage == ST_BF16 && paged_fa_supported(a)) return paged_fa(c, a);
   return q->storage == ST_BF16 ? launch_typed<__nv_bfloat16>(c, a) : launch_typed<float>(c, a);
 }
