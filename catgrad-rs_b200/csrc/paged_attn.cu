@@ -277,5 +277,6 @@ extern "C" int32_t cg_paged_attention(cg_ctx* c, const cg_tensor* q, const cg_te
   a.nh = (int)nh; a.nkv = (int)nkv; a.d = (int)d;
   written(out);
   if (q->storage == ST_BF16 && paged_fa_supported(a)) return paged_fa(c, a);
+  if (q->storage == ST_BF16 && paged_dec_supported(a)) return paged_dec(c, a);
   return q->storage == ST_BF16 ? launch_typed<__nv_bfloat16>(c, a) : launch_typed<float>(c, a);
 }

@@ -16,8 +16,11 @@ struct PagedAttnArgs {
   int nh, nkv, d;
 };
 
-// Prompts of bf16 heads of 64, 128 and 256 on tcgen05 (paged_fa.cu)
+// Prompts in bf16 on tcgen05 (paged_fa.cu)
 bool paged_fa_supported(const PagedAttnArgs& a);
 int paged_fa(cg_ctx* c, const PagedAttnArgs& a);
+// A few tokens per row, bf16 (paged_dec.cu)
+bool paged_dec_supported(const PagedAttnArgs& a);
+int paged_dec(cg_ctx* c, const PagedAttnArgs& a);
 
 }  // namespace cg

@@ -1,0 +1,366 @@
+// paged_dec.cu — attention of a few tokens per row over a paged cache in bf16: the form of decode steps.
+//
+// The query rows of a key head (token x / rep, head x % rep of the group) fill the rows of one mma.sync tile, 8 or
+// 16 at a time, so a key is read once for all of them.  A cluster has a row's keys and a key head; its blocks have equal
+// shares of the keys, a block's four warps every fourth tile of KT keys, each through a ring of its own that TMA fills.
+//   S [rows, keys] = Q K^T     (Q's fragments stay in registers)
+//   O^T [d, rows] += V^T P^T   (S's accumulators are P^T's fragments; 8 rows fill the 8 columns)
+// What bounds it is the bytes of the cache, and for short contexts the chain tables -> page table -> keys -> product -> joining.
+//
+// Probabilities are split into two bf16 parts (the second product costs nothing where bytes bound the kernel), so that the output is
+// rounded once.  Exponents' references lag behind the maxima by up to 2^8, so that tiles need no shuffles.
+#include <algorithm>
+
+#include "mma.cuh"
+#include "paged_attn.h"
+#include "tc_common.cuh"
+
+namespace cg {
+
+namespace {
+
+using namespace tc;
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LAG = 8.f;
+
+struct DecArgs {
+  PagedRows rows;
+  const __nv_bfloat16* q;
+  __nv_bfloat16* out;
+  int64_t q_ld, q_hs, most, window, pool_rows;
+  int nh, nkv, rep, d;
+  float scale_log2e, cap_log2e, cap_unit;
+};
+
+// keys of a warp's tile, tiles of its ring
+template <int D>
+__host__ __device__ constexpr int dec_keys() { return D == 64 ? 32 : 16; }
+constexpr int RING = 3;
+template <int D>
+__host__ __device__ constexpr size_t dec_ring() { return (size_t)4 * RING * 2 * dec_keys<D>() * D * 2; }
+template <int D>
+__host__ __device__ constexpr size_t dec_smem() { return 1024 + dec_ring<D>() + 4 * RING * 8; }
+
+template <int D, int ROWS, bool CAP>
+__global__ void __launch_bounds__(128)
+k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, DecArgs p) {
+  constexpr int KT = dec_keys<D>(), SUB = D / 64, NB = ROWS / 8, KS = D / 16, LD = D + 4;
+  constexpr uint32_t BOX = KT * 128, TILE = SUB * BOX;  // bytes of 64 components, of a tile
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ float red_m[4][ROWS], red_l[4][ROWS], cta_m[ROWS], cta_l[ROWS];
+  __shared__ int aborted;
+  static_assert((size_t)4 * ROWS * LD * 4 + (size_t)ROWS * LD * 4 <= dec_ring<D>(), "the warps' outputs lie over the ring");
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  float* red_o = (float*)(smem_raw + (base - raw));       // [4][ROWS][LD]
+  float* part = red_o + 4 * ROWS * LD;                    // [ROWS][LD]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t2 = (lane & 3) * 2;
+  const uint32_t ring = base + warp * (RING * 2 * TILE), bars = base + (uint32_t)dec_ring<D>() + warp * (RING * 8);
+  if (lane == 0)
+    for (int i = 0; i < RING; ++i) mbar_init(bars + 8 * i, 1);
+  if (tid == 0) aborted = 0;
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  const int kvh = (int)blockIdx.x % p.nkv;
+  const int64_t row = blockIdx.y, x0 = (int64_t)(blockIdx.x / p.nkv) * ROWS;
+  const int slices = (int)gridDim.z, slice = (int)blockIdx.z;
+  int64_t tok0, n, len;
+  if (!row_span(p.rows, row, p.most, &tok0, &n, &len) || x0 >= n * p.rep) return;  // (the same in all blocks of a cluster)
+  const int64_t pos0 = len - n, i0 = x0 / p.rep, i1 = min(n - 1, (x0 + ROWS - 1) / p.rep);
+  const int64_t lo = p.window > 0 ? max((int64_t)0, pos0 + i0 - p.window + 1) : 0, hi = pos0 + i1;
+  const int64_t first = lo / KT, tiles = hi / KT + 1 - first, share = (tiles + slices - 1) / slices;
+  const int64_t end = min(first + tiles, first + (slice + 1) * share);
+
+  // A lane has a page of a tile (or the whole tile, if pages are longer); pages without a visible key are not looked up and read
+  // as zeros (a box behind the pool's end).
+  const int lg = p.rows.lg, box = min(1 << lg, KT), parts = KT / box;
+  const int off_end = (int)p.pool_rows;
+  auto place = [&](int64_t t) {
+    const int64_t key = t * KT + lane * box;
+    if (lane >= parts || key > hi || key + box <= lo) return off_end;
+    const int64_t id = page_of(p.rows, row, key);
+    return id < 0 ? off_end : (int)(((id * p.nkv + kvh) << lg) + (key & ((1 << lg) - 1)));
+  };
+  auto request = [&](int stage, int at) {
+    const uint32_t bar = bars + 8 * stage, to = ring + stage * (2 * TILE) + lane * box * 128;
+    if (lane == 0) mbar_expect_tx(bar, 2 * TILE);
+    __syncwarp();
+    if (lane < parts) {
+#pragma unroll
+      for (int s = 0; s < SUB; ++s) tma_load_2d(to + s * BOX, &map_k, s * 64, at, bar);
+#pragma unroll
+      for (int s = 0; s < SUB; ++s) tma_load_2d(to + TILE + s * BOX, &map_v, s * 64, at, bar);
+    }
+  };
+  int64_t t = first + slice * share + warp;
+  {
+    int at[RING];
+#pragma unroll
+    for (int i = 0; i < RING; ++i) at[i] = t + 4 * i < end ? place(t + 4 * i) : off_end;
+#pragma unroll
+    for (int i = 0; i < RING; ++i)
+      if (t + 4 * i < end) request(i, at[i]);
+  }
+
+  // rows g and g + 8 of the tile
+  uint32_t qf[KS][2 * NB];
+  int64_t qpos[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int64_t x = x0 + g + 8 * b, i = x / p.rep;
+    const bool there = x < n * p.rep;
+    qpos[b] = pos0 + i;
+    const __nv_bfloat16* src = p.q + (tok0 + (there ? i : 0)) * p.q_ld + (kvh * p.rep + (there ? x % p.rep : 0)) * p.q_hs;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const int c = k * 16 + t2;
+      qf[k][b] = there && c < p.d ? *(const uint32_t*)(src + c) : 0u;
+      qf[k][NB + b] = there && c + 8 < p.d ? *(const uint32_t*)(src + c + 8) : 0u;
+    }
+  }
+  float o[KS][NB][4], m[NB], l[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    m[b] = -INFINITY;
+    l[b] = 0.f;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) o[k][b][0] = o[k][b][1] = o[k][b][2] = o[k][b][3] = 0.f;
+  }
+  // ldmatrix: lane's key and 16-byte piece within 16 keys x 16 components
+  const int lkey = (lane >> 4) * 8 + (lane & 7), lpiece = (lane >> 3) & 1;
+  bool ok = true;
+  int it = 0;
+  for (; t < end; t += 4, ++it) {
+    const int stage = it % RING;
+    const int64_t ahead = t + 4 * RING;
+    const int next = ahead < end ? place(ahead) : off_end;
+    ok = __all_sync(0xffffffffu, mbar_wait(bars + 8 * stage, (uint32_t)(it / RING) & 1u, &aborted, p.rows.err));
+    if (!ok) break;
+    const uint32_t kt = ring + stage * (2 * TILE), vt = kt + TILE;
+    const int64_t k0 = t * KT;
+    if (k0 + KT - 1 > hi) {
+      // the values behind the last visible key are nobody's: a probability of 0 times an infinity would not be 0.  (The row's last
+      // tile: nothing is loaded over it.)
+      for (int i = lane; i < SUB * (int)(k0 + KT - 1 - hi) * 8; i += 32) {
+        const int rows = (int)(k0 + KT - 1 - hi), s = i / (rows * 8), x = i - s * rows * 8;
+        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vt + s * BOX + (uint32_t)(KT - rows) * 128u + (uint32_t)x * 16u), "r"(0) : "memory");
+      }
+      __syncwarp();
+    }
+    float s[KT / 8][4];
+#pragma unroll
+    for (int i = 0; i < KT / 8; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int i = 0; i < KT / 16; ++i) {
+        const int key = i * 16 + lkey, piece = (k * 2 + lpiece) & 7;
+        uint32_t b0, b1, b2, b3;
+        ldsm_x4(kt + (k / 4) * BOX + key * 128 + ((piece ^ (key & 7)) << 4), b0, b1, b2, b3);
+        mma_bf16(s[2 * i], qf[k][0], NB == 2 ? qf[k][1] : 0u, qf[k][NB], NB == 2 ? qf[k][NB + 1] : 0u, b0, b1);
+        mma_bf16(s[2 * i + 1], qf[k][0], NB == 2 ? qf[k][1] : 0u, qf[k][NB], NB == 2 ? qf[k][NB + 1] : 0u, b2, b3);
+      }
+    const bool masked = k0 + KT - 1 > pos0 + i0 || (p.window > 0 && k0 <= hi - p.window);
+    float top[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) top[b] = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < KT / 8; ++i)
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float& x = s[i][2 * b + e];
+          if (CAP) x = fmaf(2.f * p.cap_log2e, rcp_newton(1.f + fast_exp2(x * p.cap_unit)), -p.cap_log2e);
+          else x *= p.scale_log2e;
+          if (masked) {
+            const int64_t key = k0 + i * 8 + t2 + e;
+            if (key > qpos[b] || (p.window > 0 && key <= qpos[b] - p.window)) x = -INFINITY;
+          }
+          top[b] = fmaxf(top[b], x);
+        }
+    bool grown = false;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) grown = grown || top[b] > m[b] + LAG;
+    if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        float w = fmaxf(top[b], __shfl_xor_sync(0xffffffffu, top[b], 1));
+        w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, 2));
+        const float m_new = fmaxf(m[b], w), corr = m_new == -INFINITY ? 1.f : fast_exp2(m[b] - m_new);
+        m[b] = m_new;
+        l[b] *= corr;
+        const float c0 = __shfl_sync(0xffffffffu, corr, t2 * 4), c1 = __shfl_sync(0xffffffffu, corr, t2 * 4 + 4);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          o[k][b][0] *= c0; o[k][b][1] *= c1;
+          o[k][b][2] *= c0; o[k][b][3] *= c1;
+        }
+      }
+    }
+    uint32_t ph[KT / 8][NB], pl[KT / 8][NB];  // probabilities, and what their rounding left
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const float mc = m[b] == -INFINITY ? 0.f : m[b];
+#pragma unroll
+      for (int i = 0; i < KT / 8; ++i) {
+        const float e0 = fast_exp2(s[i][2 * b] - mc), e1 = fast_exp2(s[i][2 * b + 1] - mc);
+        l[b] += e0 + e1;
+        ph[i][b] = pack_bf16(e0, e1);
+        pl[i][b] = pack_bf16(e0 - __uint_as_float(ph[i][b] << 16), e1 - __uint_as_float(ph[i][b] & 0xffff0000u));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < KT / 16; ++i)
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const int key = i * 16 + lkey, piece = (k * 2 + lpiece) & 7;
+        uint32_t a0, a1, a2, a3;
+        ldsm_x4_t(vt + (k / 4) * BOX + key * 128 + ((piece ^ (key & 7)) << 4), a0, a1, a2, a3);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          mma_bf16(o[k][b], a0, a1, a2, a3, ph[2 * i][b], ph[2 * i + 1][b]);
+          mma_bf16(o[k][b], a0, a1, a2, a3, pl[2 * i][b], pl[2 * i + 1][b]);
+        }
+      }
+    __syncwarp();
+    if (ahead < end) request(stage, next);
+  }
+  if (!ok) {  // copies on their way are waited for: what lies over the ring is written next
+    for (int i = 0; i < RING && t + 4 * i < end; ++i) mbar_drain(bars + 8 * ((it + i) % RING), (uint32_t)((it + i) / RING) & 1u, p.rows.err);
+    aborted = 1;
+  }
+
+  // ---- the warps' shares ----
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    l[b] += __shfl_xor_sync(0xffffffffu, l[b], 1);
+    l[b] += __shfl_xor_sync(0xffffffffu, l[b], 2);
+    if (t2 == 0) { red_m[warp][g + 8 * b] = m[b]; red_l[warp][g + 8 * b] = l[b]; }
+  }
+  __syncthreads();  // (all rings are empty, or given up on)
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) red_o[(warp * ROWS + b * 8 + t2 + (e & 1)) * LD + k * 16 + g + (e >> 1) * 8] = o[k][b][e];
+  __syncthreads();
+  auto out_at = [&](int64_t x) { return p.out + ((tok0 + x / p.rep) * p.nh + kvh * p.rep + x % p.rep) * (int64_t)p.d; };
+  for (int i = tid; i < ROWS * (D / 4); i += 128) {
+    const int r = i / (D / 4), c = i % (D / 4) * 4;
+    const float top = fmaxf(fmaxf(red_m[0][r], red_m[1][r]), fmaxf(red_m[2][r], red_m[3][r])), mc = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = fast_exp2(red_m[w][r] - mc);
+      const float4 u = *(const float4*)(red_o + (w * ROWS + r) * LD + c);
+      sum += red_l[w][r] * f;
+      v.x = fmaf(u.x, f, v.x); v.y = fmaf(u.y, f, v.y); v.z = fmaf(u.z, f, v.z); v.w = fmaf(u.w, f, v.w);
+    }
+    if (slices > 1) {
+      *(float4*)(part + r * LD + c) = v;
+      if (c == 0) { cta_m[r] = top; cta_l[r] = sum; }
+    } else if (x0 + r < n * p.rep && c < p.d && !aborted) {
+      const float f = sum > 0.f ? 1.f / sum : 0.f;
+      *(uint2*)(out_at(x0 + r) + c) = make_uint2(pack_bf16(v.x * f, v.y * f), pack_bf16(v.z * f, v.w * f));
+    }
+  }
+  if (slices == 1) return;
+
+  // ---- the blocks' shares: each finishes some of the values ----
+  cluster_sync_all();
+  const int rows = (int)min((int64_t)ROWS, n * p.rep - x0);
+  for (int i = slice * 128 + tid; i < rows * (D / 4); i += 128 * slices) {
+    const int r = i / (D / 4), c = i % (D / 4) * 4;
+    float ms[16], top = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < 16; ++s) {
+      ms[s] = s < slices ? ld_cluster_f32(smem_u32(&cta_m[r]), (uint32_t)s) : -INFINITY;
+      top = fmaxf(top, ms[s]);
+    }
+    const float mc = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int s = 0; s < 16; ++s) {
+      if (s >= slices) break;
+      const float f = fast_exp2(ms[s] - mc);
+      uint32_t at;
+      float4 u;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(part + r * LD + c)), "r"(s));
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(u.x), "=f"(u.y), "=f"(u.z), "=f"(u.w) : "r"(at) : "memory");
+      sum = fmaf(ld_cluster_f32(smem_u32(&cta_l[r]), (uint32_t)s), f, sum);
+      v.x = fmaf(u.x, f, v.x); v.y = fmaf(u.y, f, v.y); v.z = fmaf(u.z, f, v.z); v.w = fmaf(u.w, f, v.w);
+    }
+    if (c < p.d && !aborted) {
+      const float f = sum > 0.f ? 1.f / sum : 0.f;
+      *(uint2*)(out_at(x0 + r) + c) = make_uint2(pack_bf16(v.x * f, v.y * f), pack_bf16(v.z * f, v.w * f));
+    }
+  }
+  cluster_sync_all();
+}
+
+template <int D, int ROWS, bool CAP>
+int launch(cg_ctx* c, const PagedAttnArgs& a) {
+  constexpr size_t smem = dec_smem<D>();
+  static PerDeviceFlag configured_on;
+  bool& configured = configured_on.at(c->core->device);
+  if (!configured) {
+    CG_CUDA(c, cudaFuncSetAttribute(k_paged_dec<D, ROWS, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    configured = true;
+  }
+  DecArgs p;
+  p.rows = a.rows;
+  p.q = (const __nv_bfloat16*)a.q;
+  p.out = (__nv_bfloat16*)a.out;
+  p.q_ld = a.q_ld; p.q_hs = a.q_hs;
+  p.most = a.most;
+  p.window = a.window;
+  p.pool_rows = (a.rows.n_pages * a.nkv) << a.rows.lg;
+  p.nh = a.nh; p.nkv = a.nkv; p.rep = a.nh / a.nkv; p.d = a.d;
+  p.scale_log2e = a.scale * LOG2E;
+  p.cap_log2e = p.cap_unit = 0.f;
+  if (CAP) {
+    p.cap_log2e = a.cap * LOG2E;
+    p.cap_unit = -2.f * p.scale_log2e / a.cap;
+  }
+  CUtensorMap mk, mv;
+  const int box = std::min(1 << a.rows.lg, dec_keys<D>());
+  CG_TRY(make_map(c, &mk, a.k_pages, p.pool_rows, a.d, a.d, box));
+  CG_TRY(make_map(c, &mv, a.v_pages, p.pool_rows, a.d, a.d, box));
+  const int64_t groups = (a.most * p.rep + ROWS - 1) / ROWS * a.nkv, longest = a.rows.cols << a.rows.lg;
+  // Shares of the keys: until two blocks per SM have work, but no shares of less than a tile per warp.
+  int slices = 1;
+  while (slices < 8 && groups * a.rows.rows * slices < 2 * 148 && (int64_t)slices * 4 * dec_keys<D>() < longest) slices *= 2;
+  CG_CUDA(c, launch_kernel(c, k_paged_dec<D, ROWS, CAP>, dim3((unsigned)groups, (unsigned)a.rows.rows, (unsigned)slices), dim3(128), smem, slices, mk, mv, p));
+  CG_LAUNCHED(c);
+  return CG_OK;
+}
+
+template <int D>
+int pick(cg_ctx* c, const PagedAttnArgs& a) {
+  const bool cap = a.cap > 0.f;
+  if (a.most * (a.nh / a.nkv) <= 8) return cap ? launch<D, 8, true>(c, a) : launch<D, 8, false>(c, a);
+  return cap ? launch<D, 16, true>(c, a) : launch<D, 16, false>(c, a);
+}
+
+}  // namespace
+
+bool paged_dec_supported(const PagedAttnArgs& a) {
+  return ((a.rows.n_pages * a.nkv) << a.rows.lg) < 0x7FFFFFFFll && (a.most * (a.nh / a.nkv) + 7) / 8 * a.nkv < 0x7FFFFFFFll && ((uintptr_t)a.q % 4) == 0 &&
+         ((uintptr_t)a.out % 8) == 0 && a.q_ld % 2 == 0 && a.q_hs % 2 == 0;
+}
+
+int paged_dec(cg_ctx* c, const PagedAttnArgs& a) {
+  if (a.d <= 64) return pick<64>(c, a);
+  if (a.d <= 128) return pick<128>(c, a);
+  return pick<256>(c, a);
+}
+
+}  // namespace cg

@@ -1,4 +1,5 @@
-// paged_fa.cu — attention of prompts over a paged cache on tcgen05 / TMEM: bf16, head sizes 64, 128 and 256.
+// paged_fa.cu — attention of prompts over a paged cache on tcgen05 / TMEM, in bf16.  D is the head size, rounded up to 64, 128
+// or 256: what is read beyond a head is zeros.
 //
 // A tile is 128 query rows, the query heads of a key head side by side: row r of a tile that begins at token i0 is token
 // i0 + r / rep, head r % rep of the group.  Keys come 64 at a time, by one TMA box per page (or per 64 keys of a longer
@@ -35,7 +36,7 @@ struct FaArgs {
   PagedRows rows;
   __nv_bfloat16* out;
   int64_t most, window, pool_rows;  // pool_rows: rows of d values in each pool, n_pages nkv page
-  int nh, nkv, rep, per;            // per: tokens of a query tile
+  int nh, nkv, rep, per, d;         // per: tokens of a query tile
   float scale_log2e, cap_log2e, cap_unit;  // soft-cap c: c log2(e), -2 log2(e) score factor / c
 };
 
@@ -183,18 +184,20 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
       const int64_t id = page_of(p.rows, row, key);
       return id < 0 ? off_end : (int)(((id * p.nkv + kvh) << lg) + (key & ((1 << lg) - 1)));
     };
-    int at = place(j0);
-    for (int j = 0; j < nt; ++j) {
+    int at = place(j0), j = 0;
+    bool ok = true, half = false;  // half: of tile j the keys have been asked for
+    for (; j < nt; ++j) {
       const int stage = j % KS;
       const uint32_t ph = (uint32_t)(j / KS) & 1u;
       const int next = j + 1 < nt ? place(j0 + j + 1) : off_end;  // (on its way while this tile waits for room)
-      bool ok = true;
+      half = false;
       if (j >= KS) ok = __all_sync(0xffffffffu, mbar_wait(b_k_empty + 8 * stage, ph ^ 1u, cta_abort, p.rows.err));
       if (!ok) break;
       if (lane == 0) mbar_expect_tx(b_k_full + 8 * stage, KV_BYTES);
       __syncwarp();
       if (lane < pages)
         for (int s = 0; s < SUB; ++s) tma_load_2d(sk + stage * KV_BYTES + s * KBOX + lane * box * 128, &map_k, s * 64, at, b_k_full + 8 * stage);
+      half = true;
       if (j >= KS) ok = __all_sync(0xffffffffu, mbar_wait(b_v_empty + 8 * stage, ph ^ 1u, cta_abort, p.rows.err));
       if (!ok) break;
       if (lane == 0) mbar_expect_tx(b_v_full + 8 * stage, KV_BYTES);
@@ -203,6 +206,11 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
         for (int s = 0; s < SUB; ++s) tma_load_2d(sv + stage * KV_BYTES + s * KBOX + lane * box * 128, &map_v, s * 64, at, b_v_full + 8 * stage);
       at = next;
     }
+    if (!ok)  // the block does not leave before its copies have arrived
+      for (int i = max(0, j - KS + 1); i <= j; ++i) {
+        if (i < j || half) mbar_drain(b_k_full + 8 * (i % KS), (uint32_t)(i / KS) & 1u, p.rows.err);
+        if (i < j) mbar_drain(b_v_full + 8 * (i % KS), (uint32_t)(i / KS) & 1u, p.rows.err);
+      }
   } else if (warp == 1 || (NQ == 2 && warp == 3)) {
     // ---- products ----
     if (lane == 0) {
@@ -366,7 +374,7 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const float inv = l > 0.f ? 1.f / l : 0.f;
     const bool out = ok && r < p.per * p.rep && ti < n;
-    __nv_bfloat16* dst = p.out + ((tok0 + ti) * p.nh + head) * (int64_t)D;
+    __nv_bfloat16* dst = p.out + ((tok0 + ti) * p.nh + head) * (int64_t)p.d;
 #pragma unroll 1
     for (int c0 = 0; c0 < D; c0 += 32) {
       uint32_t v[32];
@@ -375,6 +383,7 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
       if (out) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
+          if (c0 + 8 * u >= p.d) break;
           uint32_t x[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) x[i] = pack_bf16(__uint_as_float(v[8 * u + 2 * i]) * inv, __uint_as_float(v[8 * u + 2 * i + 1]) * inv);
@@ -423,6 +432,7 @@ int launch(cg_ctx* c, const PagedAttnArgs& a) {
   p.nh = a.nh; p.nkv = a.nkv;
   p.rep = a.nh / a.nkv;
   p.per = 128 / p.rep;
+  p.d = a.d;
   p.scale_log2e = a.scale * LOG2E;
   p.cap_log2e = p.cap_unit = 0.f;
   if (CAP) {
@@ -431,8 +441,8 @@ int launch(cg_ctx* c, const PagedAttnArgs& a) {
   }
   CUtensorMap mq, mk, mv;
   const int box = std::min(1 << a.rows.lg, KT);
-  CG_TRY(make_map(c, &mk, a.k_pages, p.pool_rows, D, D, box));
-  CG_TRY(make_map(c, &mv, a.v_pages, p.pool_rows, D, D, box));
+  CG_TRY(make_map(c, &mk, a.k_pages, p.pool_rows, a.d, a.d, box));
+  CG_TRY(make_map(c, &mv, a.v_pages, p.pool_rows, a.d, a.d, box));
   CG_TRY(make_q_map(c, &mq, a, p.per, p.rep));
   const int64_t tiles = (a.most + (int64_t)NQ * p.per - 1) / ((int64_t)NQ * p.per);
   CG_CUDA(c, launch_kernel(c, k_paged_fa<D, NQ, CAP>, dim3((unsigned)tiles, (unsigned)a.nkv, (unsigned)a.rows.rows), dim3(NQ == 2 ? 384 : 256), smem, 1, mq, mk, mv, p));
@@ -454,14 +464,14 @@ int pick(cg_ctx* c, const PagedAttnArgs& a) {
 
 bool paged_fa_supported(const PagedAttnArgs& a) {
   const int64_t rep = a.nh / a.nkv;
-  return (a.d == 64 || a.d == 128 || a.d == 256) && rep <= 128 && a.most > 1 && a.most * rep > 16 && a.nkv <= 65535 &&
+  return rep <= 128 && a.most > 1 && a.most * rep > 16 && a.nkv <= 65535 &&
          ((a.rows.n_pages * a.nkv) << a.rows.lg) < 0x7FFFFFFFll && ((uintptr_t)a.q % 16) == 0 && ((uintptr_t)a.out % 16) == 0 && a.q_ld % 8 == 0 &&
          a.q_hs % 8 == 0 && a.q_ld > 0 && a.q_hs > 0 && a.q_ld < (1ll << 38) && a.q_hs < (1ll << 38);
 }
 
 int paged_fa(cg_ctx* c, const PagedAttnArgs& a) {
-  if (a.d == 64) return pick<64>(c, a);
-  if (a.d == 128) return pick<128>(c, a);
+  if (a.d <= 64) return pick<64>(c, a);
+  if (a.d <= 128) return pick<128>(c, a);
   return pick<256>(c, a);
 }
 
