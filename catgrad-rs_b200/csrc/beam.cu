@@ -6,13 +6,17 @@
 // total(j, end) = s_j.  What has no number (NaN logits; all of a beam whose largest logit or own score is not finite)
 // is -inf, as are masked logits.
 //
-// The logits are read once, 32 values a thread at a time, and stay in registers.  Within a beam totals are in the
-// order of the logits, so a block keeps the K largest of each piece it reads: the K-th largest of 32 disjoint groups'
-// maxima is no larger than the piece's K-th largest value, and the few values that reach it are ranked by counting.
-// Where more reach it than the list holds (masked or level logits) the block takes K rounds of a block-wide
-// maximum instead.  Exponentials are f32, their sums over more than a warp, the logarithm and the totals 64 bits: totals of
-// different beams may lie close together.  A group is a thread-block cluster: its blocks share the vocabulary, each then
-// finishes some of the beams from all blocks' lists, and the first one takes the K best of those.
+// The logits are read once: 256 threads take 32 KB of a beam at a time and hold them in registers.
+// Within a beam totals are in the order of the logits, so of each such piece the K largest are kept: the smallest of K disjoint groups'
+// maxima is no larger than the piece's K-th largest value, and the few values that reach it (some K ln K) are ranked by
+// counting, several pieces at a time so that a warp has each.  Where more reach it than a list holds, the K-th largest of 32
+// groups' maxima is the bound, what is above it is taken, and of what is equal to it (masked, level logits) the first K;
+// where even that is too much (logits in descending order), K rounds of a common maximum.
+// A group of beams is a thread-block cluster, over whose blocks, each of up to four times 256 threads, the pieces of its beams are
+// dealt; a warp then joins all sorted lists of a beam, and one warp those of the beams.
+//
+// Exponentials are f32, their sums over more than a warp, the logarithm and the totals 64 bits: totals of different
+// beams may lie close together.
 #include <algorithm>
 
 #include "mma.cuh"
@@ -22,10 +26,9 @@ namespace cg {
 
 namespace {
 
-constexpr int BT = 256;            // threads
-constexpr int PER = 32;            // values a thread holds
-constexpr int PIECE = BT * PER;    // values of a piece
-constexpr int LIST = 512;          // values that may reach the bound
+constexpr int BT = 256;            // threads that share a piece
+constexpr int VECS = 8;            // 16-byte vectors of a piece that a thread holds
+constexpr float LOG2E = 1.4426950408889634f;
 
 struct SelectArgs {
   const void* logits;
@@ -33,9 +36,9 @@ struct SelectArgs {
   const float* scores;              // [B, J]
   const uint32_t* finished;         // [B, J] or null
   uint32_t end;
-  int J, K, pieces;                 // pieces per block and beam
-  int pool;                         // keys that the pool holds: LIST or all lists of a beam
-  int64_t V, share;                 // share: values per block, a multiple of 16 bytes
+  int J, K, V;
+  int pieces, rounds;               // of a beam; of a block (each of its times 256 threads has a piece a round)
+  int joiners;                      // warps of a block that join lists
   float* out_scores;                // [B, K]
   uint32_t *out_tokens, *out_parents, *out_finished;
 };
@@ -68,263 +71,594 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// number, -0 as 0, NaN as -inf
-__device__ __forceinline__ float clean(float x) { return x == x ? x + 0.f : -INFINITY; }
+__device__ __forceinline__ uint64_t key_at(float x, int i) { return key_of(x == x ? x + 0.f : -INFINITY, (uint32_t)i); }  // (NaN as -inf, -0 as 0)
 
-template <typename T>
-__device__ __forceinline__ void load_piece(const T* row, int64_t first, int64_t stop, float* x, int* valid) {
-  // value i of vector w: place first + (w BT + tid) per + i
-  constexpr int per = 16 / sizeof(T), vectors = PER / per;
-  *valid = 0;
-#pragma unroll
-  for (int w = 0; w < vectors; ++w) {
-    const int64_t at = first + (int64_t)(w * BT + (int)threadIdx.x) * per;
-    const T* p = row + at;
-    float* to = x + w * per;
-    if (at + per <= stop && ((uintptr_t)p & 15) == 0) {
-      const uint4 u = __ldg((const uint4*)p);
-      const uint32_t b[4] = {u.x, u.y, u.z, u.w};
-      if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) to[i] = clean(__uint_as_float(b[i]));
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          to[2 * i] = clean(__uint_as_float(b[i] << 16));
-          to[2 * i + 1] = clean(__uint_as_float(b[i] & 0xffff0000u));
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < per; ++i) to[i] = at + i < stop ? clean((float)p[i]) : -INFINITY;
-    }
-  }
+// the largest of the warp's keys, and the first lane that has it
+__device__ __forceinline__ uint64_t warp_best(uint64_t key, int* lane) {
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(key >> 32));
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(key >> 32) == hi ? (uint32_t)key : 0u);
+  const uint64_t best = (uint64_t)hi << 32 | lo;
+  *lane = __ffs(__ballot_sync(0xffffffffu, key == best)) - 1;
+  return best;
 }
 
+constexpr int MAX_OWN = 4;         // pieces of a beam: at most 32 times this
+constexpr int POOL = 1024;         // values that reach their bounds, of several pieces
+struct PieceWork {                 // of 256 threads
+  float groups[2][32];             // (taking turns)
+  int count[8];                    // by slot: up to 8 pieces are ranked together
+  float peak[8], part[8][BT / 32];
+  uint64_t best[BT / 32];
+  int equal[BT / 32];
+  uint64_t pool[POOL];
+};
+
+// Sums of 2^((x - peak) log2 e), two values at a time on the packed f32 units.
+struct ExpSums {
+  uint64_t s = 0, less, unit;
+  __device__ __forceinline__ explicit ExpSums(float peak) {
+    const float minus = -peak, l = LOG2E;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(less) : "f"(minus));
+    asm("mov.b64 %0, {%1, %1};" : "=l"(unit) : "f"(l));
+  }
+  __device__ __forceinline__ void add(uint32_t x0, uint32_t x1) {
+    uint64_t x, d, e;
+    float e0, e1;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "r"(x0), "r"(x1));
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(less));
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(e) : "l"(d), "l"(unit));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(e0), "=f"(e1) : "l"(e));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(fast_exp2(e0)), "f"(fast_exp2(e1)));
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(s) : "l"(x));
+  }
+  __device__ __forceinline__ float sum() const {
+    float a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(s));
+    return a + b;
+  }
+};
+
+// word i of 16, which stay in registers
+__device__ __forceinline__ uint32_t word_of(const uint32_t* w, int i) {
+  uint32_t a[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) a[k] = i & 1 ? w[2 * k + 1] : w[2 * k];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) a[k] = i & 2 ? a[2 * k + 1] : a[2 * k];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) a[k] = i & 4 ? a[2 * k + 1] : a[2 * k];
+  return i & 8 ? a[1] : a[0];
+}
+
+// Four 16-byte vectors' values (16 words).  (-inf stands for what lies outside.)
 template <typename T>
-__global__ void __launch_bounds__(BT) k_beam_select(SelectArgs a) {
+struct Values;
+template <>
+struct Values<float> {
+  static constexpr int per = 4, n = 16;
+  static constexpr uint32_t lowest = 0xff800000u;
+  static __device__ __forceinline__ float at(const uint32_t* w, int i) { return __uint_as_float(w[i]); }
+  static __device__ __forceinline__ float largest(const uint32_t* w) {  // (NaNs are passed over)
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < n; ++i) m = fmaxf(m, at(w, i));
+    return m;
+  }
+  static __device__ __forceinline__ uint32_t reach(const uint32_t* w, float bound) {  // a bit per value
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < n; ++i) m |= at(w, i) >= bound ? 1u << i : 0u;
+    return m;
+  }
+  static __device__ __forceinline__ int value_of(int bit) { return bit; }
+  static __device__ __forceinline__ float pick(const uint32_t* w, int i) { return __uint_as_float(word_of(w, i)); }
+  static __device__ __forceinline__ float exps(const uint32_t* w, float peak) {
+    ExpSums s(peak);
+#pragma unroll
+    for (int i = 0; i < n; i += 2) s.add(w[i], w[i + 1]);
+    return s.sum();
+  }
+};
+template <>
+struct Values<__nv_bfloat16> {
+  static constexpr int per = 8, n = 32;
+  static constexpr uint32_t lowest = 0xff80ff80u;
+  static __device__ __forceinline__ float at(const uint32_t* w, int i) { return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16); }
+  static __device__ __forceinline__ float largest(const uint32_t* w) {
+    __nv_bfloat162 m = *(const __nv_bfloat162*)&w[0];
+#pragma unroll
+    for (int i = 1; i < n / 2; ++i) m = __hmax2(m, *(const __nv_bfloat162*)&w[i]);
+    const float lo = __low2float(m), hi = __high2float(m);
+    return fmaxf(fmaxf(lo, hi), -INFINITY);
+  }
+  // (bit i: value 2 i, bit 16 + i: value 2 i + 1)
+  static __device__ __forceinline__ uint32_t reach(const uint32_t* w, float bound) {
+    const __nv_bfloat162 b = __float2bfloat162_rn(bound);  // (a value of the piece)
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < n / 2; ++i) m |= __hge2_mask(*(const __nv_bfloat162*)&w[i], b) & (0x00010001u << i);
+    return m;
+  }
+  static __device__ __forceinline__ int value_of(int bit) { return bit < 16 ? 2 * bit : 2 * bit - 31; }
+  static __device__ __forceinline__ float pick(const uint32_t* w, int i) {
+    const uint32_t two = word_of(w, i >> 1);
+    return __uint_as_float(i & 1 ? two & 0xffff0000u : two << 16);
+  }
+  static __device__ __forceinline__ float exps(const uint32_t* w, float peak) {
+    ExpSums s(peak);
+#pragma unroll
+    for (int i = 0; i < n / 2; ++i) s.add(w[i] << 16, w[i] & 0xffff0000u);
+    return s.sum();
+  }
+};
+
+// A vector of which some values lie outside [0, limit).
+template <typename T>
+__device__ __noinline__ uint4 load_edge(const T* row, int at, int limit) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      w[i] = at + i >= 0 && at + i < limit ? *(const uint32_t*)(row + at + i) : Values<T>::lowest;
+    } else {
+      const int lo = at + 2 * i, hi = lo + 1;
+      w[i] = (lo >= 0 && lo < limit ? *(const uint16_t*)(row + lo) : Values<T>::lowest & 0xffffu) |
+             (hi >= 0 && hi < limit ? *(const uint16_t*)(row + hi) : Values<T>::lowest & 0xffffu) << 16;
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// dynamic shared memory: PieceWork [SB]; lists u64 [rounds][SB][K]; sums f64 [rounds][SB]; totals u64 [J][K]; places u64 [J][K];
+// tops f32 [rounds][SB]; marks u32 [J]; then per joining warp a beam's lists of all blocks, u64 [pieces][K]
+template <typename T, int SB>
+__global__ void __launch_bounds__(SB * BT, 4 / SB) k_beam_select(SelectArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  constexpr int per = 16 / sizeof(T);
+  using Vals = Values<T>;
+  constexpr int per = Vals::per;
   extern __shared__ uint64_t smem[];
   const int J = a.J, K = a.K, units = J * a.pieces;
-  // every block's: the K largest keys, maximum and sum of each unit (beam, piece); the beams' scores and marks
-  uint64_t* lists = smem;                       // [units][K]
-  uint64_t* top = lists + units * K;            // first block: [J][K] totals of the beams' best
-  uint64_t* place = top + J * K;                // first block: [J][K] j V + v
-  double* sums = (double*)(place + J * K);      // [units]
-  uint64_t* pool = (uint64_t*)(sums + units);   // [a.pool]
-  float* tops = (float*)(pool + a.pool);        // [units]
-  uint32_t* marks = (uint32_t*)(tops + units);  // [J]
-  __shared__ float groups[32], bound_s, peak_s;
-  __shared__ float part[BT / 32];
-  __shared__ uint64_t best_s[BT / 32];
-  __shared__ int count;
+  PieceWork* works = (PieceWork*)smem;
+  uint64_t* lists = (uint64_t*)(works + SB);
+  double* sums = (double*)(lists + a.rounds * SB * K);
+  uint64_t* totals = (uint64_t*)(sums + a.rounds * SB);
+  uint64_t* places = totals + J * K;
+  float* tops = (float*)(places + J * K);
+  uint32_t* marks = (uint32_t*)(tops + a.rounds * SB);
+  uint64_t* all = (uint64_t*)(((uintptr_t)(marks + J) + 7) & ~(uintptr_t)7);
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int sb = threadIdx.x / BT, tid = threadIdx.x % BT, warp = tid >> 5, lane = tid & 31;
+  PieceWork& w = works[sb];
+  auto sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(sb + 1), "r"(BT) : "memory"); };
   uint32_t rank, n_ranks;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n_ranks));
   const int64_t b = blockIdx.y;
-  const T* logits = (const T*)a.logits + b * a.ld_b;
-  if (tid < J) marks[tid] = a.finished ? a.finished[b * J + tid] : 0;
-  const int64_t lo = (int64_t)rank * a.share, hi = lo + a.share < a.V ? lo + a.share : a.V;
+  if ((int)threadIdx.x < J) marks[threadIdx.x] = a.finished ? a.finished[b * J + threadIdx.x] : 0;
+  if (tid < 8) w.count[tid] = 0;
+  const int room = K <= 8 ? 128 : K <= 16 ? 256 : 512, slots = POOL / room;  // (more than `room` in one piece in 10^6)
+  int least_groups = 1;
+  while (least_groups < K) least_groups *= 2;
 
-  for (int u = 0; u < units; ++u) {
+  // Unit u, piece u % pieces of beam u / pieces, belongs to round i of 256 threads of a block where u = (i n_ranks + rank) SB + sb.
+  // Vectors begin on 16-byte boundaries, a beam's first one up to `per` - 1 values before the beam; those of this thread are BT
+  // apart, and their values count in [0, V).
+  const T* row;
+  int at0;
+  auto locate = [&](int u) {
     const int j = u / a.pieces;
-    const T* row = logits + (int64_t)j * a.ld_j;
-    const int64_t first = lo + (int64_t)(u - j * a.pieces) * PIECE, stop = first + PIECE < hi ? first + PIECE : hi;
-    float x[PER];
-    int valid;
-    load_piece(row, first, stop, x, &valid);
-    float mx = x[0];
+    row = (const T*)a.logits + b * a.ld_b + (int64_t)j * a.ld_j;
+    at0 = ((u - j * a.pieces) * (BT * VECS) + tid) * per - (int)(((uintptr_t)row & 15) / sizeof(T));
+  };
+  auto load = [&](uint32_t* x) {
+    bool edge = false;  // (all whole vectors are asked for before any is waited for)
 #pragma unroll
-    for (int i = 1; i < PER; ++i) mx = fmaxf(mx, x[i]);
-    if (tid == 0) count = 0;
+    for (int v = 0; v < VECS; ++v) {
+      const int at = at0 + v * BT * per;
+      uint4 q = make_uint4(Vals::lowest, Vals::lowest, Vals::lowest, Vals::lowest);
+      const bool whole = at >= 0 && at + per <= a.V;
+      if (whole) q = __ldg((const uint4*)(row + at));
+      edge = edge || (!whole && at < a.V && at + per > 0);
+      x[4 * v] = q.x; x[4 * v + 1] = q.y; x[4 * v + 2] = q.z; x[4 * v + 3] = q.w;
+    }
+    if (edge)
+#pragma unroll
+      for (int v = 0; v < VECS; ++v) {
+        const int at = at0 + v * BT * per;
+        if (!(at >= 0 && at + per <= a.V) && at < a.V && at + per > 0) {
+          const uint4 q = load_edge<T>(row, at, a.V);
+          x[4 * v] = q.x; x[4 * v + 1] = q.y; x[4 * v + 2] = q.z; x[4 * v + 3] = q.w;
+        }
+      }
+  };
+  auto take = [&](int slot, int at, float v) {
+    const int n = atomicAdd(&w.count[slot], 1);
+    if (n < room) w.pool[slot * room + n] = key_at(v, at);
+  };
+  // The largest values of a piece whose list ran over: those above the K-th largest of 32 groups' maxima and, in the order of their
+  // places, K that are equal to it; or K rounds of a common maximum.
+  auto again = [&](int u, int slot) {
+    locate(u);
+    float mx = -INFINITY;
+#pragma unroll 1
+    for (int v = 0; v < VECS; ++v)
+#pragma unroll
+      for (int i = 0; i < per; ++i) {
+        const int at = at0 + v * BT * per + i;
+        if (at >= 0 && at < a.V) mx = fmaxf(mx, (float)row[at]);
+      }
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    if ((lane & 7) == 0) groups[tid >> 3] = mx;
-    __syncthreads();
-    if (warp == 0) {
-      const float g = groups[lane];
-      float peak = g;
-#pragma unroll
-      for (int o = 16; o; o >>= 1) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, o));
-      int above = 0;  // groups before this one in the order of size, then number
-#pragma unroll
-      for (int o = 0; o < 32; ++o) {
-        const float other = __shfl_sync(0xffffffffu, g, o);
-        above += other > g || (other == g && o < lane);
-      }
-      if (above == K - 1) bound_s = g;
-      if (lane == 0) peak_s = peak;
+    sync();
+    if ((lane & 7) == 0) w.groups[0][tid >> 3] = mx;
+    if (tid == 0) w.count[slot] = 0;
+    sync();
+    uint32_t left = up(w.groups[0][lane]), kth = 0;
+    for (int r = 0; r < K; ++r) {
+      kth = __reduce_max_sync(0xffffffffu, left);
+      if (lane == __ffs(__ballot_sync(0xffffffffu, left == kth)) - 1) left = 0;
     }
-    __syncthreads();
-    const float bound = bound_s, peak = peak_s;
-    const bool live = peak > -INFINITY && peak < INFINITY;
-    float sum = 0.f;
+    const float bound = down(kth);
+    auto side = [&](int at) {  // 1 above the bound, 0 at it, -1 below
+      const float v = (float)row[at], c = v == v ? v : -INFINITY;
+      return c > bound ? 1 : c == bound ? 0 : -1;
+    };
+    if (mx > bound)
+#pragma unroll 1
+      for (int v = 0; v < VECS; ++v)
+#pragma unroll 1
+        for (int i = 0; i < per; ++i) {
+          const int at = at0 + v * BT * per + i;
+          if (at >= 0 && at < a.V && side(at) > 0) take(slot, at, (float)row[at]);
+        }
+    sync();
+    const int above = w.count[slot];
+    if (above + K <= room) {
+      int have = 0;
+#pragma unroll 1
+      for (int v = 0; v < VECS && have < K; ++v) {
+        uint32_t level = 0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      if (live) sum += fast_exp2((x[i] - peak) * 1.4426950408889634f);
-      const int64_t at = first + (int64_t)((i / per) * BT + tid) * per + i % per;
-      if (x[i] >= bound && at < stop) {
-        const int n = atomicAdd(&count, 1);
-        if (n < LIST) pool[n] = key_of(x[i], (uint32_t)at);
-      }
-    }
+        for (int i = 0; i < per; ++i) {
+          const int at = at0 + v * BT * per + i;
+          if (at >= 0 && at < a.V && side(at) == 0) level |= 1u << i;
+        }
+        int before = __popc(level);
 #pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) part[warp] = sum;
-    __syncthreads();
-    const int n = count;
-    if (tid == 0) {
-      double s = 0.;
-      for (int i = 0; i < BT / 32; ++i) s += (double)part[i];
-      sums[u] = s;
-      tops[u] = peak;
-    }
-    if (n <= LIST) {
-      for (int i = tid; i < K; i += BT) if (i >= n) lists[u * K + i] = 0;
-      for (int i = tid; i < n; i += BT) {
-        const uint64_t key = pool[i];
-        int above = 0;
-        for (int o = 0; o < n; ++o) above += pool[o] > key;
-        if (above < K) lists[u * K + above] = key;
+        for (int o = 1; o < 32; o <<= 1) {
+          const int more = __shfl_up_sync(0xffffffffu, before, o);
+          if (lane >= o) before += more;
+        }
+        if (lane == 31) w.equal[warp] = before;
+        sync();
+        before -= __popc(level);
+        int all_of = 0;
+        for (int i = 0; i < BT / 32; ++i) {
+          if (i < warp) before += w.equal[i];
+          all_of += w.equal[i];
+        }
+        for (int n = have + before; level && n < K; ++n, level &= level - 1) {
+          const int at = at0 + v * BT * per + __ffs(level) - 1;
+          w.pool[slot * room + above + n] = key_at((float)row[at], at);
+        }
+        have += all_of;
+        sync();
       }
+      if (tid == 0) w.count[slot] = above + min(have, K);
     } else {
       uint64_t last = ~0ull;
       for (int r = 0; r < K; ++r) {
         uint64_t best = 0;
+#pragma unroll 1
+        for (int v = 0; v < VECS; ++v)
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const int64_t at = first + (int64_t)((i / per) * BT + tid) * per + i % per;
-          const uint64_t key = at < stop ? key_of(x[i], (uint32_t)at) : 0;
-          if (key < last && key > best) best = key;
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) {
-          const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
-          best = other > best ? other : best;
-        }
-        if (lane == 0) best_s[warp] = best;
-        __syncthreads();
-        for (int w = 0; w < BT / 32; ++w) best = best_s[w] > best ? best_s[w] : best;
-        if (tid == 0) lists[u * K + r] = best;
+          for (int i = 0; i < per; ++i) {
+            const int at = at0 + v * BT * per + i;
+            const uint64_t key = at >= 0 && at < a.V ? key_at((float)row[at], at) : 0;
+            if (key < last && key > best) best = key;
+          }
+        int who;
+        best = warp_best(best, &who);
+        if (lane == 0) w.best[warp] = best;
+        sync();
+        for (int i = 0; i < BT / 32; ++i) best = w.best[i] > best ? w.best[i] : best;
+        if (tid == 0) w.pool[slot * room + r] = best;
         last = best;
-        __syncthreads();
+        sync();
       }
+      if (tid == 0) w.count[slot] = K;  // (places without a value are 0)
     }
-    __syncthreads();
+    sync();
+  };
+
+  int slot = 0, begun = 0;  // the round of slot 0
+  for (int i = 0; i < a.rounds; ++i) {
+    const int u = (i * (int)n_ranks + (int)rank) * SB + sb;
+    if (u < units) {
+      locate(u);
+      uint32_t x[4 * VECS];
+      load(x);
+      float mine = Vals::largest(x);
+#pragma unroll
+      for (int q = 16; q < 4 * VECS; q += 16) mine = fmaxf(mine, Vals::largest(x + q));
+      float mx = mine;
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      if ((lane & 7) == 0) w.groups[i & 1][tid >> 3] = mx;
+      sync();
+      // every warp finds the smallest of 1, 2, .. 32 >= K groups' maxima
+      uint32_t g = up(w.groups[i & 1][lane]);
+      const uint32_t none = up(-INFINITY);
+      const float peak = down(__reduce_max_sync(0xffffffffu, g));
+      for (int o = 16; o >= least_groups; o >>= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
+      // (groups without a value are left out where the others are enough)
+      const int some = __popc(__ballot_sync(0xffffffffu, g > none));
+      if (g == none && some >= K * (32 / least_groups)) g = 0xffffffffu;
+      const float bound = down(__reduce_min_sync(0xffffffffu, g));
+      if (bound == -INFINITY) {
+        if (tid == 0) w.count[slot] = room + 1;
+      } else if (__any_sync(0xffffffffu, mine >= bound)) {
+        // places in the list for all of the warp's at once
+        uint32_t m[VECS / 4];
+        int mine_n = 0;
+#pragma unroll
+        for (int q = 0; q < VECS / 4; ++q) {
+          m[q] = Vals::reach(x + 16 * q, bound);
+          mine_n += __popc(m[q]);
+        }
+        int n = mine_n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int more = __shfl_up_sync(0xffffffffu, n, o);
+          if (lane >= o) n += more;
+        }
+        int from = 0;
+        if (lane == 31) from = atomicAdd(&w.count[slot], n);
+        n += __shfl_sync(0xffffffffu, from, 31) - mine_n;
+        if (mine_n) {
+#pragma unroll
+          for (int q = 0; q < VECS / 4; ++q)
+            for (; m[q]; m[q] &= m[q] - 1, ++n) {
+              const int e = Vals::value_of(__ffs(m[q]) - 1);
+              if (n < room) w.pool[slot * room + n] = key_at(Vals::pick(x + 16 * q, e), at0 + (4 * q + e / per) * BT * per + e % per);
+            }
+        }
+      }
+      // (differences to the peak first: the largest value's term is exactly 1, so that equal beams stay equal)
+      float sum = 0.f;
+      if (peak > -INFINITY && peak < INFINITY) {
+#pragma unroll
+        for (int q = 0; q < 4 * VECS; q += 16) sum += Vals::exps(x + q, peak);
+        if (!(sum == sum)) {  // some are NaN
+          sum = 0.f;
+#pragma unroll
+          for (int q = 0; q < 4 * VECS; q += 16)
+#pragma unroll
+            for (int e = 0; e < Vals::n; ++e) {
+              const float v = Vals::at(x + q, e);
+              sum += v == v ? fast_exp2((v - peak) * LOG2E) : 0.f;
+            }
+        }
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) w.part[slot][warp] = sum;
+      if (tid == 0) w.peak[slot] = peak;
+      ++slot;
+    }
+    if (slot > 0 && (slot == slots || i + 1 == a.rounds)) {  // the slots' lists: a warp has slots warp, warp + 8
+      sync();
+      for (int q = 0; q < slot; ++q)
+        if (w.count[q] > room) again(((begun + q) * (int)n_ranks + (int)rank) * SB + sb, q);
+      for (int q = warp; q < slot; q += BT / 32) {
+        const int place = (begun + q) * SB + sb, n = w.count[q];
+        double s = lane < BT / 32 ? (double)w.part[q][lane] : 0.;
+#pragma unroll
+        for (int o = 4; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (lane == 0) {
+          sums[place] = s;
+          tops[place] = w.peak[q];
+        }
+        const uint64_t* keys = w.pool + q * room;
+        uint64_t* list = lists + place * K;
+        if (lane < K) list[lane] = 0;
+        __syncwarp();
+        for (int k = lane; k < n; k += 32) {
+          const uint64_t key = keys[k];
+          int above = 0;
+#pragma unroll 8
+          for (int o = 0; o < n; ++o) above += (int)(keys[o] > key);
+          if (above < K && key) list[above] = key;
+        }
+        __syncwarp();
+        if (lane == 0) w.count[q] = 0;
+      }
+      sync();
+      slot = 0;
+      begun = i + 1;
+    }
   }
+  __syncthreads();
   cluster_barrier();
 
-  // this block's beams: the K largest of all blocks' lists, and their totals, into the first block
-  const uint32_t top0 = remote_addr(top, 0), place0 = remote_addr(place, 0);
-  for (int j = (int)rank; j < J; j += (int)n_ranks) {
-    const int per_rank = a.pieces * K, n = (int)n_ranks * per_rank;
-    uint64_t* all = pool;
-    for (int i = tid; i < n; i += BT) all[i] = remote_ld64(remote_addr(lists + j * per_rank + i % per_rank, (uint32_t)(i / per_rank)));
-    __shared__ double sum_s;
-    __shared__ float max_s;
-    if (warp == 0) {
-      const int parts = (int)n_ranks * a.pieces;
-      float m = -INFINITY;
-      for (int i = lane; i < parts; i += 32) {
-        float v;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote_addr(tops + j * a.pieces + i % a.pieces, (uint32_t)(i / a.pieces))) : "memory");
-        m = fmaxf(m, v);
-      }
+  // A warp joins a beam's sorted lists, and puts its K best totals into the first block.
+  const uint32_t totals0 = remote_addr(totals, 0), places0 = remote_addr(places, 0);
+  const int me = sb * (BT / 32) + warp, P = a.pieces;
+  if (me < a.joiners)
+    for (int j = (int)rank + me * (int)n_ranks; j < J; j += a.joiners * (int)n_ranks) {
+      uint64_t* mine = all + me * P * K;
+      // (a lane has pieces lane, lane + 32, ..: their list, maximum and sum)
+      float m = -INFINITY, v[MAX_OWN];
+      double part[MAX_OWN];
+      const float score = a.scores[b * J + j];
 #pragma unroll
-      for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      double s = 0.;
-      for (int i = lane; i < parts; i += 32) {
-        float v;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote_addr(tops + j * a.pieces + i % a.pieces, (uint32_t)(i / a.pieces))) : "memory");
-        const double part_sum = __longlong_as_double((long long)remote_ld64(remote_addr(sums + j * a.pieces + i % a.pieces, (uint32_t)(i / a.pieces))));
-        if (part_sum > 0.) s += part_sum * exp((double)v - (double)m);
+      for (int i = 0; i < MAX_OWN; ++i) {
+        const int p = lane + 32 * i;
+        v[i] = -INFINITY;
+        part[i] = 0.;
+        if (p < P) {
+          const int u = j * P + p, block = u / SB, round = block / (int)n_ranks, at = round * SB + u % SB;
+          const uint32_t r = (uint32_t)(block - round * (int)n_ranks), from = remote_addr(lists + at * K, r);
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[i]) : "r"(remote_addr(tops + at, r)) : "memory");
+          part[i] = __longlong_as_double((long long)remote_ld64(remote_addr(sums + at, r)));
+#pragma unroll 4
+          for (int k = 0; k < K; ++k) mine[p * K + k] = remote_ld64(from + (uint32_t)k * 8u);
+          m = fmaxf(m, v[i]);
+        }
       }
+      m = down(__reduce_max_sync(0xffffffffu, up(m)));
+      double s = 0.;
+#pragma unroll
+      for (int i = 0; i < MAX_OWN; ++i)
+        if (part[i] > 0.) s += part[i] * (double)fast_exp2((v[i] - m) * LOG2E);
 #pragma unroll
       for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (lane == 0) { sum_s = s; max_s = m; }
-    }
-    __syncthreads();
-    const double score = (double)a.scores[b * J + j], log_sum = log(sum_s);
-    const float m = max_s;
-    const bool dead = !(m > -INFINITY && m < INFINITY) || !(score > -INFINITY && score < INFINITY);
-    const uint64_t j0 = (uint64_t)j * (uint64_t)a.V;
-    if (dead || marks[j]) {
-      // -inf all over, in the order of the vocabulary, behind the end token of a finished beam
-      for (int i = tid; i < K; i += BT) {
-        const bool ends = marks[j] && score > -INFINITY && score < INFINITY;
-        uint64_t v = (uint64_t)i;
-        double total = -INFINITY;
-        if (ends) {
-          v = i == 0 ? a.end : (uint64_t)(i - 1) + ((uint32_t)(i - 1) >= a.end ? 1u : 0u);
-          if (i == 0) total = score;
+      const double log_sum = log(s);
+      const bool known = score > -INFINITY && score < INFINITY;
+      const uint64_t j0 = (uint64_t)j * (uint64_t)a.V;
+      auto put = [&](int i, double total, uint64_t v) {
+        remote_st64(totals0 + (uint32_t)(j * K + i) * 8u, up64(total));
+        remote_st64(places0 + (uint32_t)(j * K + i) * 8u, j0 + v);
+      };
+      if (marks[j] && known) {
+        // the end token, then -inf in the order of the vocabulary
+        for (int i = lane; i < K; i += 32) put(i, i == 0 ? (double)score : -INFINITY, i == 0 ? a.end : (uint32_t)(i - 1) + ((uint32_t)(i - 1) >= a.end ? 1u : 0u));
+      } else if (!known || !(m > -INFINITY && m < INFINITY)) {
+        for (int i = lane; i < K; i += 32) put(i, -INFINITY, (uint64_t)i);
+      } else {
+        __syncwarp();
+        // K times the largest of the lists' heads; a lane has lists lane, lane + 32, ..
+        uint64_t got = 0;
+        int taken = 0;  // of list `lane`, where that is the lane's only one
+        for (int r = 0; r < K; ++r) {
+          uint64_t best = 0;
+          int from = lane, who;
+          if (P <= 32) {
+            if (lane < P && taken < K) best = mine[lane * K + taken];
+          } else {
+            for (int l = lane; l < P; l += 32)
+              if (mine[l * K] > best) { best = mine[l * K]; from = l; }
+          }
+          const uint64_t top = warp_best(best, &who);
+          if (lane == who) {  // (keys differ: they hold the token)
+            if (P <= 32) {
+              ++taken;
+            } else {
+              uint64_t* list = mine + from * K;
+              for (int i = 0; i + 1 < K && list[i]; ++i) list[i] = list[i + 1];
+              list[K - 1] = 0;
+            }
+          }
+          if (lane == (r & 31)) got = top;
+          __syncwarp();
         }
-        remote_st64(top0 + (uint32_t)(j * K + i) * 8u, up64(total));
-        remote_st64(place0 + (uint32_t)(j * K + i) * 8u, j0 + v);
-      }
-    } else {
-      for (int i = tid; i < n; i += BT) {
-        const uint64_t key = all[i];
-        int above = 0;
-        for (int o = 0; o < n; ++o) above += all[o] > key;
-        if (above < K && key) {
-          const float x = down((uint32_t)(key >> 32));
-          const double total = score + (((double)x - (double)m) - log_sum);
-          remote_st64(top0 + (uint32_t)(j * K + above) * 8u, up64(total));
-          remote_st64(place0 + (uint32_t)(j * K + above) * 8u, j0 + (0xffffffffu - (uint32_t)key));
-        }
+        if (lane < K) put(lane, (double)score + (((double)down((uint32_t)(got >> 32)) - (double)m) - log_sum), 0xffffffffu - (uint32_t)got);
       }
     }
-    __syncthreads();
-  }
   cluster_barrier();
 
-  if (rank == 0) {
-    for (int i = tid; i < J * K; i += BT) {
-      const uint64_t t = top[i], p = place[i];
-      int above = 0;
-      for (int o = 0; o < J * K; ++o) above += top[o] > t || (top[o] == t && place[o] < p);
-      if (above < K) {
-        const uint32_t parent = (uint32_t)(p / (uint64_t)a.V), token = (uint32_t)(p - parent * (uint64_t)a.V);
-        const int64_t at = b * K + above;
-        a.out_scores[at] = (float)down64(t);
-        a.out_tokens[at] = token;
-        a.out_parents[at] = parent;
-        a.out_finished[at] = marks[parent] || token == a.end;
+  // the best of the beams' sorted totals: a lane has a beam
+  if (rank == 0 && threadIdx.x < 32) {
+    int at = 0;
+    for (int r = 0; r < K; ++r) {
+      const uint64_t key = lane < J && at < K ? totals[lane * K + at] : 0;
+      int who;
+      const uint64_t best = warp_best(key, &who);  // (of equal totals the lowest beam's)
+      if (lane == who) {
+        const uint32_t token = (uint32_t)(places[lane * K + at] - (uint64_t)lane * (uint64_t)a.V);
+        ++at;
+        const int64_t to = b * K + r;
+        a.out_scores[to] = (float)down64(best);
+        a.out_tokens[to] = token;
+        a.out_parents[to] = (uint32_t)lane;
+        a.out_finished[to] = marks[lane] || token == a.end;
       }
     }
   }
 }
 
-size_t select_smem(const SelectArgs& a) {
-  const size_t units = (size_t)a.J * a.pieces;
-  return (units * a.K + 2 * (size_t)a.J * a.K + units + a.pool) * 8 + units * 4 + (size_t)a.J * 4;
-}
+template <typename T, int SB>
+struct Blocks {
+  static cudaError_t configure(int device) {
+    static PerDeviceFlag configured_on;
+    bool& configured = configured_on.at(device);
+    if (configured) return cudaSuccess;
+    cudaError_t e = cudaFuncSetAttribute(k_beam_select<T, SB>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_beam_select<T, SB>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    configured = e == cudaSuccess;
+    return e;
+  }
+  // clusters of this many blocks that run at a time (asked once)
+  static int at_a_time(int device, int ranks) {
+    static int known[64][17];
+    int& n = known[device & 63][ranks];
+    if (n == 0) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3((unsigned)ranks, 1024);
+      cfg.blockDim = dim3(SB * BT);
+      cfg.dynamicSmemBytes = SB * sizeof(PieceWork) + 16384;
+      cudaLaunchAttribute attr;
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = (unsigned)ranks;
+      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      int got = 0;
+      if (configure(device) != cudaSuccess || cudaOccupancyMaxActiveClusters(&got, k_beam_select<T, SB>, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        got = 0;
+      }
+      n = got > 0 ? got : -1;
+    }
+    return n;
+  }
+  static int launch(cg_ctx* c, SelectArgs a, int64_t B, int ranks) {
+    a.rounds = (int)(((int64_t)a.J * a.pieces + ranks * SB - 1) / (ranks * SB));
+    const size_t places = (size_t)a.rounds * SB, list = (size_t)a.pieces * a.K * 8;
+    const size_t fixed = SB * sizeof(PieceWork) + (places * a.K + places + 2 * (size_t)a.J * a.K) * 8 + (places + a.J) * 4 + 8;
+    a.joiners = std::min(SB * BT / 32, (a.J + ranks - 1) / ranks);
+    while (a.joiners > 1 && fixed + a.joiners * list > (SB == 4 ? 160 : 50) * 1024) --a.joiners;
+    const size_t smem = fixed + a.joiners * list;
+    if (smem > 200 * 1024) return fail(c, CG_ERR_UNSUPPORTED, "beams times vocabulary too large");
+    CG_CUDA(c, configure(c->core->device));
+    CG_CUDA(c, launch_kernel(c, k_beam_select<T, SB>, dim3((unsigned)ranks, (unsigned)B), dim3(SB * BT), smem, -ranks, a));
+    CG_LAUNCHED(c);
+    return CG_OK;
+  }
+};
 
 template <typename T>
 int launch_select(cg_ctx* c, SelectArgs a, int64_t B) {
-  // blocks of a group: enough that each has about one piece of a beam, at most 8
-  int ranks = 1;
-  while (ranks < 8 && (int64_t)ranks * PIECE < a.V) ranks *= 2;
-  constexpr int64_t per = 16 / sizeof(T);
-  a.share = ((a.V + ranks - 1) / ranks + per - 1) / per * per;
-  a.pieces = (int)((a.share + PIECE - 1) / PIECE);
-  if (a.pieces > 64) return fail(c, CG_ERR_UNSUPPORTED, "vocabulary too large");
-  a.pool = std::max(LIST, ranks * a.pieces * a.K);
-  const size_t smem = select_smem(a);
-  if (smem > 200 * 1024) return fail(c, CG_ERR_UNSUPPORTED, "beams times vocabulary too large");
-  static PerDeviceFlag configured_on;
-  bool& configured = configured_on.at(c->core->device);
-  if (!configured) {
-    CG_CUDA(c, cudaFuncSetAttribute(k_beam_select<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
-    configured = true;
-  }
-  CG_CUDA(c, launch_kernel(c, k_beam_select<T>, dim3((unsigned)ranks, (unsigned)B), dim3(BT), smem, -ranks, a));
-  CG_LAUNCHED(c);
-  return CG_OK;
+  constexpr int64_t per = 16 / sizeof(T), piece = BT * VECS;  // vectors of a piece
+  const int64_t all = (a.V + 2 * per - 2) / per;              // a beam's vectors, where it does not begin on a boundary
+  const int64_t pieces = (all + piece - 1) / piece, units = a.J * pieces;
+  if (pieces > 32 * MAX_OWN) return fail(c, CG_ERR_UNSUPPORTED, "vocabulary too large");
+  a.pieces = (int)pieces;
+  // Blocks of a group and times 256 threads of a block: what takes the least time by rounds of pieces, a round being a chain of
+  // 1.5 us and 0.7 per 256 threads that an SM has.
+  int best_ranks = 0, best_sb = 1;
+  double best = 1e300;
+  const int device = c->core->device;
+  for (int ranks : {1, 2, 3, 4, 5, 6, 8, 12, 16})
+    for (int sb : {1, 2, 4}) {
+      if (ranks * sb > 1 && (ranks * sb + 1) / 2 >= units + 1) continue;
+      const int n = sb == 1 ? Blocks<T, 1>::at_a_time(device, ranks) : sb == 2 ? Blocks<T, 2>::at_a_time(device, ranks) : Blocks<T, 4>::at_a_time(device, ranks);
+      if (n <= 0) continue;
+      const double waves = (double)((B + n - 1) / n), rounds = (double)((units + ranks * sb - 1) / (ranks * sb));
+      if (rounds * sb * a.K * 8 > 100 * 1024) continue;
+      const double per_sm = std::max((double)sb, (double)(std::min<int64_t>(B, n) * ranks * sb) / 148.);
+      const double cost = waves * rounds * (1.5 + 0.7 * per_sm) + 0.1 * ranks;
+      if (cost < best) {
+        best = cost;
+        best_ranks = ranks;
+        best_sb = sb;
+      }
+    }
+  if (best_ranks == 0) return fail(c, CG_ERR_UNSUPPORTED, "beams times vocabulary too large");
+  if (best_sb == 4) return Blocks<T, 4>::launch(c, a, B, best_ranks);
+  if (best_sb == 2) return Blocks<T, 2>::launch(c, a, B, best_ranks);
+  return Blocks<T, 1>::launch(c, a, B, best_ranks);
 }
 
 }  // namespace
@@ -353,7 +687,7 @@ extern "C" int32_t cg_beam_select(cg_ctx* c, const cg_tensor* logits, const cg_t
   if (J > 32 || K > 32) return fail(c, CG_ERR_UNSUPPORTED, "at most 32 beams");
   if (B > 65535) return fail(c, CG_ERR_UNSUPPORTED, "at most 65535 groups");
   if (K > V) return fail(c, CG_ERR_SHAPE, "more beams than the vocabulary has");
-  if (V > 0x7FFFFFFFll) return fail(c, CG_ERR_UNSUPPORTED, "vocabulary too large");
+  if (V > 1ll << 30) return fail(c, CG_ERR_UNSUPPORTED, "vocabulary too large");
   if (finished && (int64_t)end >= V) return fail(c, CG_ERR_INVALID, "the end token is not in the vocabulary");
   // the scores and marks of a group are read before its new ones are written, so they may take their place
   const cg_tensor* outs[4] = {scores_out, tokens_out, parents_out, finished_out};
@@ -373,7 +707,7 @@ extern "C" int32_t cg_beam_select(cg_ctx* c, const cg_tensor* logits, const cg_t
   a.scores = (const float*)scores->data();
   a.finished = finished ? (const uint32_t*)finished->data() : nullptr;
   a.end = end;
-  a.J = (int)J; a.K = (int)K; a.V = V;
+  a.J = (int)J; a.K = (int)K; a.V = (int)V;
   a.out_scores = (float*)scores_out->data();
   a.out_tokens = (uint32_t*)tokens_out->data();
   a.out_parents = (uint32_t*)parents_out->data();

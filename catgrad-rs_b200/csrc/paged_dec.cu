@@ -337,7 +337,7 @@ int launch(cg_ctx* c, const PagedAttnArgs& a) {
   const int64_t groups = (a.most * p.rep + ROWS - 1) / ROWS * a.nkv, longest = a.rows.cols << a.rows.lg;
   // Shares of the keys: until two blocks per SM have work, but no shares of less than a tile per warp.
   int slices = 1;
-  while (slices < 8 && groups * a.rows.rows * slices < 2 * 148 && (int64_t)slices * 4 * dec_keys<D>() < longest) slices *= 2;
+  while (slices < 8 && groups * a.rows.rows * slices * (longest > 4096 ? 1 : 2) <= 2 * 148 && (int64_t)slices * 4 * dec_keys<D>() < longest) slices *= 2;
   CG_CUDA(c, launch_kernel(c, k_paged_dec<D, ROWS, CAP>, dim3((unsigned)groups, (unsigned)a.rows.rows, (unsigned)slices), dim3(128), smem, slices, mk, mv, p));
   CG_LAUNCHED(c);
   return CG_OK;
