@@ -111,6 +111,156 @@ __global__ void __launch_bounds__(256) k_paged_append(AppendArgs a) {
   }
 }
 
+// Eight neighbouring values, loaded as they are stored.
+template <typename T>
+struct Eight;
+template <>
+struct Eight<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) { a = __ldg((const float4*)p); b = __ldg((const float4*)p + 1); }
+  __device__ __forceinline__ void get(float* x) const { x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w; }
+  static __device__ __forceinline__ void put(float* p, const float* x) {
+    *(float4*)p = make_float4(x[0], x[1], x[2], x[3]);
+    *((float4*)p + 1) = make_float4(x[4], x[5], x[6], x[7]);
+  }
+};
+template <>
+struct Eight<__nv_bfloat16> {
+  uint4 a;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { a = __ldg((const uint4*)p); }
+  __device__ __forceinline__ void get(float* x) const {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+  }
+  static __device__ __forceinline__ void put(__nv_bfloat16* p, const float* x) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *(const uint32_t*)&v;
+    }
+    *(uint4*)p = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+// The same for head sizes 16 G, G a power of two, aligned vectors and angles in eights: G lanes have a vector, each two pieces of eight values,
+// which are the two sides of its eight pairs (with `rot_half` where they turn), or 16 neighbours.  A warp has a token, or one of
+// `parts` shares of its heads; its angles stay in registers over all heads.  U vectors are on their way at a time.
+template <typename TI, typename TO, int G>
+__global__ void __launch_bounds__(256) k_paged_append_vec(AppendArgs a, int parts) {
+  constexpr int VPI = 32 / G, U = sizeof(TI) == 2 ? 4 : 2;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int lane = threadIdx.x & 31, g = lane % G;
+  const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), m = w / parts;
+  if (m >= a.rows.M) return;
+  const int heads = a.nh + 2 * a.nkv, step = parts * VPI;
+  int h0 = (int)(w - m * parts) * VPI + lane / G;
+  // this lane's two pieces of every vector
+  const int turned = a.half / 8;  // lanes whose pairs turn, with rot_half
+  const int c0 = a.rot_half ? (g < turned ? 8 * g : 2 * a.half + 16 * (g - turned)) : 16 * g, c1 = a.rot_half && g < turned ? c0 + a.half : c0 + 8;
+  auto source = [&](int h) {
+    return h < a.nh ? (const TI*)a.q + m * a.q_ld + h * a.q_hs
+                    : h < a.nh + a.nkv ? (const TI*)a.k + m * a.k_ld + (h - a.nh) * a.k_hs : (const TI*)a.v + m * a.v_ld + (h - a.nh - a.nkv) * a.v_hs;
+  };
+  Eight<TI> in[U][2];
+  auto request = [&](int h) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (h + u * step < heads) {
+        const TI* src = source(h + u * step);
+        in[u][0].load(src + c0);
+        in[u][1].load(src + c1);
+      }
+  };
+  request(h0);
+  // the token's row (as many rows as end at or before it), position and page
+  int64_t row = 0;
+  for (int64_t i = lane; i - lane < a.rows.rows; i += 32)
+    row += __popc(__ballot_sync(0xffffffffu, i < a.rows.rows && a.rows.starts[i + 1] <= m));
+  if (row >= a.rows.rows) return;  // behind the last row
+  int64_t tok0, n, len;
+  if (!row_span(a.rows, row, a.rows.M, &tok0, &n, &len) || m < tok0) return;
+  const int64_t pos = len - n + (m - tok0);
+  if (a.cos_t && pos >= a.T) {
+    *a.rows.err = DEV_INDEX;
+    return;
+  }
+  const int64_t page = page_of(a.rows, row, pos);
+  const int64_t at = page < 0 ? 0 : (((page * a.nkv) << a.rows.lg) + (pos & ((1 << a.rows.lg) - 1))) * a.d;
+  // (pair i: components c0 + i and c1 + i with rot_half, else neighbours c0 + 2 i and c0 + 2 i + 1)
+  float cs[8], sn[8];
+  const bool turns = a.rot_half ? g < turned : 8 * g < a.half;
+  if (turns) {
+    Eight<float> t;
+    t.load(a.cos_t + pos * a.half + 8 * g);
+    t.get(cs);
+    t.load(a.sin_t + pos * a.half + 8 * g);
+    t.get(sn);
+  }
+  const float one = a.plus_one ? 1.f : 0.f;
+  for (; h0 - lane / G < heads; h0 += U * step) {
+    if (U * step < heads && h0 >= step * U) request(h0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + u * step;
+      if (h - lane / G >= heads) break;  // (uniform)
+      float x[8], y[8];
+      in[u][0].get(x);
+      in[u][1].get(y);
+      const int which = h < a.nh ? 0 : h < a.nh + a.nkv ? 1 : 2;
+      const float* gain = which == 0 ? a.q_gain : which == 1 ? a.k_gain : nullptr;
+      if (a.q_gain || a.k_gain) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss += x[i] * x[i] + y[i] * y[i];
+#pragma unroll
+        for (int o = G / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (gain) {
+          const float f = 1.f / sqrtf(ss / (float)a.d + a.eps);
+          float gx[8], gy[8];
+          Eight<float> t;
+          t.load(gain + c0);
+          t.get(gx);
+          t.load(gain + c1);
+          t.get(gy);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            x[i] = x[i] * f * (one + gx[i]);
+            y[i] = y[i] * f * (one + gy[i]);
+          }
+        }
+      }
+      if (turns && which < 2) {
+        if (a.rot_half) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float t = x[i] * cs[i] - y[i] * sn[i];
+            y[i] = y[i] * cs[i] + x[i] * sn[i];
+            x[i] = t;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float t = x[2 * i] * cs[i] - x[2 * i + 1] * sn[i], r = y[2 * i] * cs[4 + i] - y[2 * i + 1] * sn[4 + i];
+            x[2 * i + 1] = x[2 * i + 1] * cs[i] + x[2 * i] * sn[i];
+            y[2 * i + 1] = y[2 * i + 1] * cs[4 + i] + y[2 * i] * sn[4 + i];
+            x[2 * i] = t;
+            y[2 * i] = r;
+          }
+        }
+      }
+      if (h < heads && (which == 0 || page >= 0)) {
+        TO* dst = which == 0 ? (TO*)a.q_out + (m * a.nh + h) * a.d
+                             : (which == 1 ? (TO*)a.k_pages : (TO*)a.v_pages) + at + ((int64_t)(h - a.nh - (which == 2 ? a.nkv : 0)) << a.rows.lg) * a.d;
+        Eight<TO>::put(dst + c0, x);
+        Eight<TO>::put(dst + c1, y);
+      }
+    }
+  }
+}
+
 struct ReorderArgs {
   const uint32_t *parents, *lens, *own;
   uint32_t* table;
@@ -190,8 +340,29 @@ int check_vectors(cg_ctx* c, const cg_tensor* t, const char* what, int64_t M, in
   return CG_OK;
 }
 
+template <typename TI, typename TO, int G>
+int launch_vec(cg_ctx* c, const AppendArgs& a) {
+  // A warp per token where there are enough of them, else the heads are shared until every SM has four warps.
+  const int heads = a.nh + 2 * a.nkv, most = (heads + 32 / G - 1) / (32 / G);
+  int parts = 1;
+  while (2 * parts <= most && a.rows.M * parts < 148 * 32) parts *= 2;
+  CG_CUDA(c, launch_kernel(c, k_paged_append_vec<TI, TO, G>, dim3((unsigned)((a.rows.M * parts + 7) / 8)), dim3(256), 0, 1, a, parts));
+  CG_LAUNCHED(c);
+  return CG_OK;
+}
+
 template <typename TI, typename TO>
 int launch_append(cg_ctx* c, const AppendArgs& a) {
+  constexpr int64_t in = 16 / sizeof(TI);
+  const bool aligned = ((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.q_out | (uintptr_t)a.cos_t | (uintptr_t)a.sin_t | (uintptr_t)a.q_gain |
+                        (uintptr_t)a.k_gain) % 16 == 0 &&
+                       (a.q_ld | a.q_hs | a.k_ld | a.k_hs | a.v_ld | a.v_hs) % in == 0 && a.half % 8 == 0;
+  if (aligned) {
+    if (a.d == 32) return launch_vec<TI, TO, 2>(c, a);
+    if (a.d == 64) return launch_vec<TI, TO, 4>(c, a);
+    if (a.d == 128) return launch_vec<TI, TO, 8>(c, a);
+    if (a.d == 256) return launch_vec<TI, TO, 16>(c, a);
+  }
   const int64_t vectors = a.rows.M * (a.nh + 2 * a.nkv);
   CG_CUDA(c, launch_kernel(c, k_paged_append<TI, TO>, dim3((unsigned)((vectors + 7) / 8)), dim3(256), 0, 1, a));
   CG_LAUNCHED(c);

@@ -92,7 +92,7 @@ def test_append(cuda, into, pages, nh, nkv, d, turned, norms, halves, plus):
         check_append(cuda, Batch(new, total, page, seed=i, spare=i % 3), into, pages, nh, nkv, d, turned, norms, halves, plus)
 
 
-def check_append(B, b, into, pages, nh, nkv, d, turned, norms, halves, plus, split=False):
+def check_append(B, b, into, pages, nh, nkv, d, turned, norms, halves, plus, split=None):
     import torch
     rng = b.rng
     q, k, v = (rounded(rng.standard_normal((b.M, h, d)) * 1.5, into) for h in (nh, nkv, nkv))
@@ -104,11 +104,11 @@ def check_append(B, b, into, pages, nh, nkv, d, turned, norms, halves, plus, spl
     kp, vp = (put(B, x, pages) for x in old)
     q_old = rounded(rng.standard_normal((b.M, nh, d)), pages)
     qo = put(B, q_old, pages)
-    if split:   # three parts of one projection, from an odd place on
+    if split is not None:   # three parts of one projection, from this place on
         both = torch.from_numpy(np.concatenate([q, k, v], 1)).to(torch.bfloat16 if into == "bf16" else torch.float32)
-        flat = torch.zeros(both.numel() + 3, dtype=both.dtype, device="cuda")
-        flat[3:] = both.reshape(-1).cuda()
-        whole = flat[3:].reshape(b.M, nh + 2 * nkv, d)
+        flat = torch.zeros(both.numel() + split, dtype=both.dtype, device="cuda")
+        flat[split:] = both.reshape(-1).cuda()
+        whole = flat[split:].reshape(b.M, nh + 2 * nkv, d)
         torch.cuda.synchronize()
         qd, kd, vd = (B.from_device(x) for x in (whole[:, :nh], whole[:, nh:nh + nkv], whole[:, nh + nkv:]))
     else:
@@ -146,9 +146,17 @@ def check_append(B, b, into, pages, nh, nkv, d, turned, norms, halves, plus, spl
 
 @gpu
 @pytest.mark.parametrize("into,pages", [("f32", "bf16"), ("bf16", "bf16"), ("f32", "f32")])
-@pytest.mark.parametrize("nh,nkv,d", [(4, 2, 64), (3, 1, 128), (2, 2, 40)])
-def test_append_parts_of_a_projection(cuda, into, pages, nh, nkv, d):
-    check_append(cuda, Batch([3, 1, 40], [3, 66, 41], 16, spare=2), into, pages, nh, nkv, d, d, True, True, False, split=True)
+@pytest.mark.parametrize("nh,nkv,d", [(4, 2, 64), (3, 1, 128), (2, 2, 40), (32, 4, 128), (5, 3, 32), (8, 4, 256), (32, 8, 64)])
+@pytest.mark.parametrize("offset", [3, 8])
+def test_append_parts_of_a_projection(cuda, into, pages, nh, nkv, d, offset):
+    check_append(cuda, Batch([3, 1, 40], [3, 66, 41], 16, spare=2), into, pages, nh, nkv, d, d, True, True, False, split=offset)
+
+
+@gpu
+@pytest.mark.parametrize("nh,nkv,d", [(32, 4, 128), (32, 8, 64)])
+def test_append_of_many_tokens(cuda, nh, nkv, d):
+    """As many tokens as give each warp one."""
+    check_append(cuda, Batch([2500, 1, 2400], [2500, 66, 2441], 64, spare=2), "bf16", "bf16", nh, nkv, d, d, True, False, False, split=0)
 
 
 def attention(q, k, v, pos, scale, window, cap):
