@@ -145,18 +145,20 @@ struct Eight<__nv_bfloat16> {
 };
 
 // The same for head sizes 16 G, G a power of two, aligned vectors and angles in eights: G lanes have a vector, each two pieces of eight values,
-// which are the two sides of its eight pairs (with `rot_half` where they turn), or 16 neighbours.  A warp has a token, or one of
-// `parts` shares of its heads; its angles stay in registers over all heads.  U vectors are on their way at a time.
+// which are the two sides of its eight pairs (with `rot_half` where they turn), or 16 neighbours.  A warp has one of `parts` shares of a
+// token's heads, U times 32 / G of them, all on their way before the token's row is looked up.
+template <typename TI>
+constexpr int append_vectors() { return sizeof(TI) == 2 ? 4 : 2; }
 template <typename TI, typename TO, int G>
-__global__ void __launch_bounds__(256) k_paged_append_vec(AppendArgs a, int parts) {
-  constexpr int VPI = 32 / G, U = sizeof(TI) == 2 ? 4 : 2;
+__global__ void __launch_bounds__(128, 5) k_paged_append_vec(AppendArgs a, int parts) {
+  constexpr int VPI = 32 / G, U = append_vectors<TI>();
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31, g = lane % G;
-  const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), m = w / parts;
+  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5), m = w / parts;
   if (m >= a.rows.M) return;
   const int heads = a.nh + 2 * a.nkv, step = parts * VPI;
-  int h0 = (int)(w - m * parts) * VPI + lane / G;
+  const int h0 = (int)(w - m * parts) * VPI + lane / G;
   // this lane's two pieces of every vector
   const int turned = a.half / 8;  // lanes whose pairs turn, with rot_half
   const int c0 = a.rot_half ? (g < turned ? 8 * g : 2 * a.half + 16 * (g - turned)) : 16 * g, c1 = a.rot_half && g < turned ? c0 + a.half : c0 + 8;
@@ -165,16 +167,13 @@ __global__ void __launch_bounds__(256) k_paged_append_vec(AppendArgs a, int part
                     : h < a.nh + a.nkv ? (const TI*)a.k + m * a.k_ld + (h - a.nh) * a.k_hs : (const TI*)a.v + m * a.v_ld + (h - a.nh - a.nkv) * a.v_hs;
   };
   Eight<TI> in[U][2];
-  auto request = [&](int h) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (h + u * step < heads) {
-        const TI* src = source(h + u * step);
-        in[u][0].load(src + c0);
-        in[u][1].load(src + c1);
-      }
-  };
-  request(h0);
+  for (int u = 0; u < U; ++u)
+    if (h0 + u * step < heads) {
+      const TI* src = source(h0 + u * step);
+      in[u][0].load(src + c0);
+      in[u][1].load(src + c1);
+    }
   // the token's row (as many rows as end at or before it), position and page
   int64_t row = 0;
   for (int64_t i = lane; i - lane < a.rows.rows; i += 32)
@@ -200,63 +199,60 @@ __global__ void __launch_bounds__(256) k_paged_append_vec(AppendArgs a, int part
     t.get(sn);
   }
   const float one = a.plus_one ? 1.f : 0.f;
-  for (; h0 - lane / G < heads; h0 += U * step) {
-    if (U * step < heads && h0 >= step * U) request(h0);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = h0 + u * step;
-      if (h - lane / G >= heads) break;  // (uniform)
-      float x[8], y[8];
-      in[u][0].get(x);
-      in[u][1].get(y);
-      const int which = h < a.nh ? 0 : h < a.nh + a.nkv ? 1 : 2;
-      const float* gain = which == 0 ? a.q_gain : which == 1 ? a.k_gain : nullptr;
-      if (a.q_gain || a.k_gain) {
-        float ss = 0.f;
+  for (int u = 0; u < U; ++u) {
+    const int h = h0 + u * step;
+    if (h - lane / G >= heads) break;  // (uniform)
+    float x[8], y[8];
+    in[u][0].get(x);
+    in[u][1].get(y);
+    const int which = h < a.nh ? 0 : h < a.nh + a.nkv ? 1 : 2;
+    const float* gain = which == 0 ? a.q_gain : which == 1 ? a.k_gain : nullptr;
+    if (a.q_gain || a.k_gain) {
+      float ss = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss += x[i] * x[i] + y[i] * y[i];
+      for (int i = 0; i < 8; ++i) ss += x[i] * x[i] + y[i] * y[i];
 #pragma unroll
-        for (int o = G / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (gain) {
-          const float f = 1.f / sqrtf(ss / (float)a.d + a.eps);
-          float gx[8], gy[8];
-          Eight<float> t;
-          t.load(gain + c0);
-          t.get(gx);
-          t.load(gain + c1);
-          t.get(gy);
+      for (int o = G / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (gain) {
+        const float f = 1.f / sqrtf(ss / (float)a.d + a.eps);
+        float gx[8], gy[8];
+        Eight<float> t;
+        t.load(gain + c0);
+        t.get(gx);
+        t.load(gain + c1);
+        t.get(gy);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            x[i] = x[i] * f * (one + gx[i]);
-            y[i] = y[i] * f * (one + gy[i]);
-          }
+        for (int i = 0; i < 8; ++i) {
+          x[i] = x[i] * f * (one + gx[i]);
+          y[i] = y[i] * f * (one + gy[i]);
         }
       }
-      if (turns && which < 2) {
-        if (a.rot_half) {
+    }
+    if (turns && which < 2) {
+      if (a.rot_half) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float t = x[i] * cs[i] - y[i] * sn[i];
-            y[i] = y[i] * cs[i] + x[i] * sn[i];
-            x[i] = t;
-          }
-        } else {
+        for (int i = 0; i < 8; ++i) {
+          const float t = x[i] * cs[i] - y[i] * sn[i];
+          y[i] = y[i] * cs[i] + x[i] * sn[i];
+          x[i] = t;
+        }
+      } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float t = x[2 * i] * cs[i] - x[2 * i + 1] * sn[i], r = y[2 * i] * cs[4 + i] - y[2 * i + 1] * sn[4 + i];
-            x[2 * i + 1] = x[2 * i + 1] * cs[i] + x[2 * i] * sn[i];
-            y[2 * i + 1] = y[2 * i + 1] * cs[4 + i] + y[2 * i] * sn[4 + i];
-            x[2 * i] = t;
-            y[2 * i] = r;
-          }
+        for (int i = 0; i < 4; ++i) {
+          const float t = x[2 * i] * cs[i] - x[2 * i + 1] * sn[i], r = y[2 * i] * cs[4 + i] - y[2 * i + 1] * sn[4 + i];
+          x[2 * i + 1] = x[2 * i + 1] * cs[i] + x[2 * i] * sn[i];
+          y[2 * i + 1] = y[2 * i + 1] * cs[4 + i] + y[2 * i] * sn[4 + i];
+          x[2 * i] = t;
+          y[2 * i] = r;
         }
       }
-      if (h < heads && (which == 0 || page >= 0)) {
-        TO* dst = which == 0 ? (TO*)a.q_out + (m * a.nh + h) * a.d
-                             : (which == 1 ? (TO*)a.k_pages : (TO*)a.v_pages) + at + ((int64_t)(h - a.nh - (which == 2 ? a.nkv : 0)) << a.rows.lg) * a.d;
-        Eight<TO>::put(dst + c0, x);
-        Eight<TO>::put(dst + c1, y);
-      }
+    }
+    if (h < heads && (which == 0 || page >= 0)) {
+      TO* dst = which == 0 ? (TO*)a.q_out + (m * a.nh + h) * a.d
+                           : (which == 1 ? (TO*)a.k_pages : (TO*)a.v_pages) + at + ((int64_t)(h - a.nh - (which == 2 ? a.nkv : 0)) << a.rows.lg) * a.d;
+      Eight<TO>::put(dst + c0, x);
+      Eight<TO>::put(dst + c1, y);
     }
   }
 }
@@ -342,11 +338,11 @@ int check_vectors(cg_ctx* c, const cg_tensor* t, const char* what, int64_t M, in
 
 template <typename TI, typename TO, int G>
 int launch_vec(cg_ctx* c, const AppendArgs& a) {
-  // A warp per token where there are enough of them, else the heads are shared until every SM has four warps.
+  // Shares of a token: as many vectors as a lane holds; of few tokens smaller ones, until every SM has 32 warps.
   const int heads = a.nh + 2 * a.nkv, most = (heads + 32 / G - 1) / (32 / G);
-  int parts = 1;
+  int parts = (most + append_vectors<TI>() - 1) / append_vectors<TI>();
   while (2 * parts <= most && a.rows.M * parts < 148 * 32) parts *= 2;
-  CG_CUDA(c, launch_kernel(c, k_paged_append_vec<TI, TO, G>, dim3((unsigned)((a.rows.M * parts + 7) / 8)), dim3(256), 0, 1, a, parts));
+  CG_CUDA(c, launch_kernel(c, k_paged_append_vec<TI, TO, G>, dim3((unsigned)((a.rows.M * parts + 3) / 4)), dim3(128), 0, 1, a, parts));
   CG_LAUNCHED(c);
   return CG_OK;
 }
