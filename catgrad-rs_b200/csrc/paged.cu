@@ -157,8 +157,8 @@ __global__ void __launch_bounds__(128, 5) k_paged_append_vec(AppendArgs a, int p
   const int lane = threadIdx.x & 31, g = lane % G;
   const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5), m = w / parts;
   if (m >= a.rows.M) return;
-  const int heads = a.nh + 2 * a.nkv, step = parts * VPI;
-  const int h0 = (int)(w - m * parts) * VPI + lane / G;
+  const int heads = a.nh + 2 * a.nkv, share = (heads + VPI * parts - 1) / (VPI * parts);  // (at most U)
+  const int h0 = (int)(w - m * parts) * share * VPI + lane / G, stop = min(heads, h0 - lane / G + share * VPI);
   // this lane's two pieces of every vector
   const int turned = a.half / 8;  // lanes whose pairs turn, with rot_half
   const int c0 = a.rot_half ? (g < turned ? 8 * g : 2 * a.half + 16 * (g - turned)) : 16 * g, c1 = a.rot_half && g < turned ? c0 + a.half : c0 + 8;
@@ -169,8 +169,8 @@ __global__ void __launch_bounds__(128, 5) k_paged_append_vec(AppendArgs a, int p
   Eight<TI> in[U][2];
 #pragma unroll
   for (int u = 0; u < U; ++u)
-    if (h0 + u * step < heads) {
-      const TI* src = source(h0 + u * step);
+    if (h0 + u * VPI < stop) {
+      const TI* src = source(h0 + u * VPI);
       in[u][0].load(src + c0);
       in[u][1].load(src + c1);
     }
@@ -198,11 +198,13 @@ __global__ void __launch_bounds__(128, 5) k_paged_append_vec(AppendArgs a, int p
     t.load(a.sin_t + pos * a.half + 8 * g);
     t.get(sn);
   }
-  const float one = a.plus_one ? 1.f : 0.f;
+  const float one = a.plus_one ? 1.f : 0.f, over_d = 1.f / (float)a.d;
+  const float* have = nullptr;
+  float gx[8], gy[8];  // the gains at `have`
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int h = h0 + u * step;
-    if (h - lane / G >= heads) break;  // (uniform)
+    const int h = h0 + u * VPI;
+    if (h - lane / G >= stop) break;  // (uniform)
     float x[8], y[8];
     in[u][0].get(x);
     in[u][1].get(y);
@@ -215,17 +217,21 @@ __global__ void __launch_bounds__(128, 5) k_paged_append_vec(AppendArgs a, int p
 #pragma unroll
       for (int o = G / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
       if (gain) {
-        const float f = 1.f / sqrtf(ss / (float)a.d + a.eps);
-        float gx[8], gy[8];
-        Eight<float> t;
-        t.load(gain + c0);
-        t.get(gx);
-        t.load(gain + c1);
-        t.get(gy);
+        if (gain != have) {
+          Eight<float> t;
+          t.load(gain + c0);
+          t.get(gx);
+          t.load(gain + c1);
+          t.get(gy);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) { gx[i] += one; gy[i] += one; }
+          have = gain;
+        }
+        const float f = rsqrtf(ss * over_d + a.eps);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          x[i] = x[i] * f * (one + gx[i]);
-          y[i] = y[i] * f * (one + gy[i]);
+          x[i] = x[i] * f * gx[i];
+          y[i] = y[i] * f * gy[i];
         }
       }
     }
@@ -248,7 +254,7 @@ __global__ void __launch_bounds__(128, 5) k_paged_append_vec(AppendArgs a, int p
         }
       }
     }
-    if (h < heads && (which == 0 || page >= 0)) {
+    if (h < stop && (which == 0 || page >= 0)) {
       TO* dst = which == 0 ? (TO*)a.q_out + (m * a.nh + h) * a.d
                            : (which == 1 ? (TO*)a.k_pages : (TO*)a.v_pages) + at + ((int64_t)(h - a.nh - (which == 2 ? a.nkv : 0)) << a.rows.lg) * a.d;
       Eight<TO>::put(dst + c0, x);
