@@ -29,22 +29,28 @@ __device__ __forceinline__ void store_as(__nv_bfloat16* p, float x) { *p = __flo
 __device__ __forceinline__ float load_as(const float* p) { return *p; }
 __device__ __forceinline__ float load_as(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
-// Every type and head size, on the CUDA cores.  A block has QR queries of one row and key head (query x is token x / rep,
-// head x % rep of the group) and a share of the visible keys, 32 at a time; the blocks of a cluster share the
+// f32, and whatever the tensor-core kernels do not take, on the CUDA cores.  A block has QR queries of one row and key head (query x
+// is token x / rep, head x % rep of the group) and a share of the visible keys, 32 at a time; the blocks of a cluster share the
 // keys and are joined through shared memory.  Eight lanes have a query row (or four rows): a score is a key's, an output value
-// four neighbouring columns'.  D: head size, rounded up to 64, 128 or 256.
+// four neighbouring columns', so that of a thread's 4 x 4 products eight vectors are read.  f32 keys and values come by
+// asynchronous copies, a ring of tiles ahead, their places looked up a tile before that.  D: head size, rounded up to 64,
+// 128 or 256.
 constexpr int GK = 32;  // keys of a tile
+template <typename T, int D>
+__host__ __device__ constexpr int any_ring() { return sizeof(T) == 2 ? 1 : D == 256 ? 2 : 3; }
+template <typename T, int D, int QR>
+__host__ __device__ constexpr size_t any_smem() { return (size_t)((QR + 2 * any_ring<T, D>() * GK) * (D + 4) + QR * (GK + 1)) * 4; }
 template <typename T, int D, int QR>
 __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
-  constexpr int LD = D + 4;
+  constexpr int LD = D + 4, RING = any_ring<T, D>();
   constexpr int RT = QR / 16;      // query rows of a thread
   constexpr int CT = D / 32;       // groups of four output columns of a thread
   extern __shared__ __align__(16) float sm[];
   float* qs = sm;                  // [QR][LD]
-  float* ks = qs + QR * LD;        // [GK][LD]
-  float* vs = ks + GK * LD;        // [GK][LD]
-  float* ps = vs + GK * LD;        // [QR][GK + 1]
+  float* ring = qs + QR * LD;      // [RING] keys [GK][LD], values [GK][LD]
+  float* ps = ring + RING * 2 * GK * LD;  // [QR][GK + 1]
   __shared__ float ml[2][QR];
+  __shared__ int64_t places[2][GK];  // of the keys of the next tile to be asked for; -1: zeros
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int tid = threadIdx.x, ty = tid >> 3, tx = tid & 7;
@@ -57,6 +63,56 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
   const int64_t lo = a.window > 0 ? max((int64_t)0, pos0 + i0 - a.window + 1) : 0, hi = pos0 + i1;
   const int64_t first = lo / GK, tiles = hi / GK + 1 - first, per = (tiles + slices - 1) / slices;
   const int64_t t0 = first + slice * per, t1 = min(first + tiles, t0 + per);
+  const int64_t page_mask = ((int64_t)1 << a.rows.lg) - 1;
+  auto look_up = [&](int64_t t) {  // by the first warp
+    const int64_t key = t * GK + tid;
+    int64_t at = -1;
+    if (t < t1 && key >= lo && key <= hi) {
+      const int64_t page = page_of(a.rows, row, key);
+      if (page >= 0) at = (((page * a.nkv + kvh) << a.rows.lg) + (key & page_mask)) * a.d;
+    }
+    places[t & 1][tid] = at;
+  };
+  auto request = [&](int64_t t) {
+    float* ks = ring + (int)((t - t0) % RING) * 2 * GK * LD;
+    float* vs = ks + GK * LD;
+    if constexpr (sizeof(T) == 4) {
+      if (t < t1)
+        for (int i = tid; i < GK * (D / 4); i += 128) {
+          const int r = i / (D / 4), c = i % (D / 4) * 4;
+          const int64_t at = places[t & 1][r];
+          const bool there = at >= 0 && c < a.d;
+          const float* k = (const float*)a.k_pages + (there ? at + c : 0);
+          const float* v = (const float*)a.v_pages + (there ? at + c : 0);
+          cp_async16((uint32_t)__cvta_generic_to_shared(ks + r * LD + c), k, there ? 16 : 0);
+          cp_async16((uint32_t)__cvta_generic_to_shared(vs + r * LD + c), v, there ? 16 : 0);
+        }
+      cp_async_commit();
+    } else {
+      for (int i = tid; i < GK * (D / 8); i += 128) {
+        const int r = i / (D / 8), c = i % (D / 8) * 8;
+        const int64_t at = places[t & 1][r];
+        float kx[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, vx[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (at >= 0 && c < a.d) {
+          load8((const T*)a.k_pages + at + c, kx);
+          load8((const T*)a.v_pages + at + c, vx);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          ks[r * LD + c + e] = kx[e];
+          vs[r * LD + c + e] = vx[e];
+        }
+      }
+    }
+  };
+  if (tid < GK) look_up(t0);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < RING - 1; ++i) {  // (two tiles' places take turns)
+    request(t0 + i);
+    if (tid < GK) look_up(t0 + i + 1);
+    __syncthreads();
+  }
 
   for (int i = tid; i < QR * (D / 8); i += 128) {
     const int r = i / (D / 8), c = i % (D / 8) * 8;
@@ -64,6 +120,7 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (x < n * rep && c < a.d) {
       const T* p = (const T*)a.q + (tok0 + x / rep) * a.q_ld + (kvh * rep + x % rep) * a.q_hs + c;
+#pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = load_as(p + e);
     }
 #pragma unroll
@@ -77,28 +134,20 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
 #pragma unroll
     for (int c = 0; c < CT; ++c) o[r][c][0] = o[r][c][1] = o[r][c][2] = o[r][c][3] = 0.f;
   }
-  const int64_t page_mask = ((int64_t)1 << a.rows.lg) - 1;
   for (int64_t t = t0; t < t1; ++t) {
-    __syncthreads();
-    for (int i = tid; i < GK * (D / 8); i += 128) {
-      const int r = i / (D / 8), c = i % (D / 8) * 8;
-      const int64_t key = t * GK + r;
-      float kx[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, vx[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (key >= lo && key <= hi && c < a.d) {
-        const int64_t page = page_of(a.rows, row, key);
-        if (page >= 0) {
-          const int64_t at = (((page * a.nkv + kvh) << a.rows.lg) + (key & page_mask)) * a.d + c;
-          load8((const T*)a.k_pages + at, kx);
-          load8((const T*)a.v_pages + at, vx);
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        ks[r * LD + c + e] = kx[e];
-        vs[r * LD + c + e] = vx[e];
-      }
+    if constexpr (RING > 1) {
+      cp_async_wait_group<RING - 2>();
+      __syncthreads();  // tile t is there, and everyone is done with the one before
+      request(t + RING - 1);
+      if (tid < GK) look_up(t + RING);
+    } else {
+      __syncthreads();
+      request(t);
+      __syncthreads();
+      if (tid < GK) look_up(t + 1);
     }
-    __syncthreads();
+    const float* ks = ring + (int)((t - t0) % RING) * 2 * GK * LD;
+    const float* vs = ks + GK * LD;
     float s[RT][4];
 #pragma unroll
     for (int r = 0; r < RT; ++r) s[r][0] = s[r][1] = s[r][2] = s[r][3] = 0.f;
@@ -114,18 +163,19 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
         for (int j = 0; j < 4; ++j) s[r][j] = fmaf(qq.x, kk[j].x, fmaf(qq.y, kk[j].y, fmaf(qq.z, kk[j].z, fmaf(qq.w, kk[j].w, s[r][j]))));
       }
     }
+    const bool masked = t * GK + GK - 1 > pos0 + i0 || (a.window > 0 && t * GK <= hi - a.window);
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      const int64_t pos = pos0 + (x0 + ty * RT + r) / rep;
+      const int64_t pos = masked ? pos0 + (x0 + ty * RT + r) / rep : 0;
       float top = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int64_t key = t * GK + tx + 8 * j;
-        const bool seen = key <= pos && (a.window <= 0 || key > pos - a.window);
         float x = s[r][j] * a.scale;
         if (a.cap > 0.f) x = a.cap * tanhf(x / a.cap);
-        s[r][j] = seen ? x : -INFINITY;
-        top = fmaxf(top, s[r][j]);
+        if (masked && !(key <= pos && (a.window <= 0 || key > pos - a.window))) x = -INFINITY;
+        s[r][j] = x;
+        top = fmaxf(top, x);
       }
 #pragma unroll
       for (int w = 4; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
@@ -138,14 +188,13 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
         sum += e;
         ps[(ty * RT + r) * (GK + 1) + tx + 8 * j] = e;
       }
-#pragma unroll
-      for (int w = 4; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-      l[r] = l[r] * corr + sum;
+      l[r] = l[r] * corr + sum;  // (of this lane's keys)
       m[r] = m_new;
+      if (corr != 1.f)
 #pragma unroll
-      for (int c = 0; c < CT; ++c)
+        for (int c = 0; c < CT; ++c)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[r][c][e] *= corr;
+          for (int e = 0; e < 4; ++e) o[r][c][e] *= corr;
     }
     __syncwarp();
 #pragma unroll 4
@@ -167,21 +216,26 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
     }
     __syncwarp();
   }
-  auto put = [&](int64_t x, int col, float v) {
-    if (x < n * rep && col < a.d) store_as((T*)a.out + ((tok0 + x / rep) * a.nh + kvh * rep + x % rep) * a.d + col, v);
+  if constexpr (RING > 1) cp_async_wait_group<0>();
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int w = 4; w; w >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], w);
+  auto put4 = [&](int64_t x, int col, float4 v) {
+    if (x >= n * rep || col >= a.d) return;
+    T* to = (T*)a.out + ((tok0 + x / rep) * a.nh + kvh * rep + x % rep) * a.d + col;
+    store_as(to, v.x); store_as(to + 1, v.y); store_as(to + 2, v.z); store_as(to + 3, v.w);
   };
   if (slices == 1) {
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       const float f = l[r] > 0.f ? 1.f / l[r] : 0.f;
 #pragma unroll
-      for (int c = 0; c < CT; ++c)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) put(x0 + ty * RT + r, tx * 4 + c * 32 + e, o[r][c][e] * f);
+      for (int c = 0; c < CT; ++c) put4(x0 + ty * RT + r, tx * 4 + c * 32, make_float4(o[r][c][0] * f, o[r][c][1] * f, o[r][c][2] * f, o[r][c][3] * f));
     }
     return;
   }
-  // the shares are joined: a block has some of the rows
+  // the shares are joined: a block has some of the values
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
@@ -193,39 +247,57 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   auto remote = [](const float* p, int rank) {
     uint32_t at;
-    float v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"((uint32_t)rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-    return v;
+    return at;
   };
-  for (int x = slice; x < QR && x0 + x < n * rep; x += slices) {
-    float top = -INFINITY, sum = 0.f;
-    for (int s = 0; s < slices; ++s) top = fmaxf(top, remote(&ml[0][x], s));
-    const float base = top == -INFINITY ? 0.f : top;
-    for (int s = 0; s < slices; ++s) sum += remote(&ml[1][x], s) * expf(remote(&ml[0][x], s) - base);
-    const float f = sum > 0.f ? 1.f / sum : 0.f;
-    for (int c = tid; c < a.d; c += 128) {
-      float v = 0.f;
-      for (int s = 0; s < slices; ++s) v += remote(qs + x * LD + c, s) * expf(remote(&ml[0][x], s) - base);
-      put(x0 + x, c, v * f);
+  const int rows = (int)min((int64_t)QR, n * rep - x0);
+  for (int i = slice * 128 + tid; i < rows * (D / 4); i += 128 * slices) {
+    const int x = i / (D / 4), c = i % (D / 4) * 4;
+    float ms[8], ls[8];
+    float4 os[8];  // (all on their way at once)
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      ms[s] = -INFINITY;
+      ls[s] = 0.f;
+      os[s] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (s < slices) {
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(ms[s]) : "r"(remote(&ml[0][x], s)) : "memory");
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(ls[s]) : "r"(remote(&ml[1][x], s)) : "memory");
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(os[s].x), "=f"(os[s].y), "=f"(os[s].z), "=f"(os[s].w) : "r"(remote(qs + x * LD + c, s)) : "memory");
+      }
     }
+    float top = ms[0];
+#pragma unroll
+    for (int s = 1; s < 8; ++s) top = fmaxf(top, ms[s]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const float f = expf(ms[s] - base);
+      sum = fmaf(ls[s], f, sum);
+      v.x = fmaf(os[s].x, f, v.x); v.y = fmaf(os[s].y, f, v.y); v.z = fmaf(os[s].z, f, v.z); v.w = fmaf(os[s].w, f, v.w);
+    }
+    const float f = sum > 0.f ? 1.f / sum : 0.f;
+    put4(x0 + x, c, make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
   }
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 template <typename T, int D, int QR>
 int launch_any(cg_ctx* c, const PagedAttnArgs& a) {
-  constexpr size_t smem = (size_t)((QR + 2 * GK) * (D + 4) + QR * (GK + 1)) * 4;
+  constexpr size_t smem = any_smem<T, D, QR>();
   static PerDeviceFlag configured_on;
   bool& configured = configured_on.at(c->core->device);
   if (!configured) {
     CG_CUDA(c, cudaFuncSetAttribute(k_paged_attn<T, D, QR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     configured = true;
   }
-  const int64_t tiles = (a.most * (a.nh / a.nkv) + QR - 1) / QR * a.nkv;
+  const int64_t tiles = (a.most * (a.nh / a.nkv) + QR - 1) / QR * a.nkv, longest = a.rows.cols << a.rows.lg;
   if (tiles > 0x7FFFFFFFll) return fail(c, CG_ERR_UNSUPPORTED, "too many tokens");
-  int slices = 1;  // blocks that share the keys: until the GPU is full
-  while (slices < 8 && tiles * a.rows.rows * slices < 148 * 2) slices *= 2;
+  // Blocks that share the keys: until there are two per SM, but no shares of less than two tiles.
+  int slices = 1;
+  while (slices < 8 && tiles * a.rows.rows * slices < 148 * 2 && (int64_t)slices * 2 * GK < longest) slices *= 2;
   CG_CUDA(c, launch_kernel(c, k_paged_attn<T, D, QR>, dim3((unsigned)tiles, (unsigned)a.rows.rows, (unsigned)slices), dim3(128), smem, slices, a));
   CG_LAUNCHED(c);
   return CG_OK;
