@@ -11,10 +11,6 @@ namespace cg {
 
 namespace {
 
-__device__ __forceinline__ void load8(const float* p, float* x) {
-  const float4 a = *(const float4*)p, b = *((const float4*)p + 1);
-  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
 __device__ __forceinline__ void load8(const __nv_bfloat16* p, float* x) {
   const uint4 u = *(const uint4*)p;
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -29,17 +25,32 @@ __device__ __forceinline__ void store_as(__nv_bfloat16* p, float x) { *p = __flo
 __device__ __forceinline__ float load_as(const float* p) { return *p; }
 __device__ __forceinline__ float load_as(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
+// two f32 at a time
+__device__ __forceinline__ void fma2(uint64_t& c, uint64_t a, uint64_t b) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b)); }
+__device__ __forceinline__ void mul2(uint64_t& c, uint64_t a) { asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(c) : "l"(a)); }
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ float2 both(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+
 // f32, and whatever the tensor-core kernels do not take, on the CUDA cores.  A block has QR queries of one row and key head (query x
 // is token x / rep, head x % rep of the group) and a share of the visible keys, 32 at a time; the blocks of a cluster share the
 // keys and are joined through shared memory.  Eight lanes have a query row (or four rows): a score is a key's, an output value
-// four neighbouring columns', so that of a thread's 4 x 4 products eight vectors are read.  f32 keys and values come by
+// four neighbouring columns', so that for a thread's 4 x 4 products eight vectors are read; two products are
+// one instruction, and probabilities lie in shared memory twice for that.  f32 keys and values come by
 // asynchronous copies, a ring of tiles ahead, their places looked up a tile before that.  D: head size, rounded up to 64,
 // 128 or 256.
 constexpr int GK = 32;  // keys of a tile
 template <typename T, int D>
 __host__ __device__ constexpr int any_ring() { return sizeof(T) == 2 ? 1 : D == 256 ? 2 : 3; }
 template <typename T, int D, int QR>
-__host__ __device__ constexpr size_t any_smem() { return (size_t)((QR + 2 * any_ring<T, D>() * GK) * (D + 4) + QR * (GK + 1)) * 4; }
+__host__ __device__ constexpr size_t any_smem() { return (size_t)((QR + 2 * any_ring<T, D>() * GK) * (D + 4) + 2 * QR * (GK + 1)) * 4; }
 template <typename T, int D, int QR>
 __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
   constexpr int LD = D + 4, RING = any_ring<T, D>();
@@ -48,7 +59,7 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
   extern __shared__ __align__(16) float sm[];
   float* qs = sm;                  // [QR][LD]
   float* ring = qs + QR * LD;      // [RING] keys [GK][LD], values [GK][LD]
-  float* ps = ring + RING * 2 * GK * LD;  // [QR][GK + 1]
+  uint64_t* ps = (uint64_t*)(ring + RING * 2 * GK * LD);  // [QR][GK + 1]: each probability twice
   __shared__ float ml[2][QR];
   __shared__ int64_t places[2][GK];  // of the keys of the next tile to be asked for; -1: zeros
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -126,13 +137,14 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) qs[r * LD + c + e] = v[e];
   }
-  float o[RT][CT][4], m[RT], l[RT];
+  float m[RT], l[RT];
+  uint64_t o[RT][CT][2];
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     m[r] = -INFINITY;
     l[r] = 0.f;
 #pragma unroll
-    for (int c = 0; c < CT; ++c) o[r][c][0] = o[r][c][1] = o[r][c][2] = o[r][c][3] = 0.f;
+    for (int c = 0; c < CT; ++c) o[r][c][0] = o[r][c][1] = 0;
   }
   for (int64_t t = t0; t < t1; ++t) {
     if constexpr (RING > 1) {
@@ -148,33 +160,36 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
     }
     const float* ks = ring + (int)((t - t0) % RING) * 2 * GK * LD;
     const float* vs = ks + GK * LD;
-    float s[RT][4];
+    uint64_t s2[RT][4];
 #pragma unroll
-    for (int r = 0; r < RT; ++r) s[r][0] = s[r][1] = s[r][2] = s[r][3] = 0.f;
+    for (int r = 0; r < RT; ++r) s2[r][0] = s2[r][1] = s2[r][2] = s2[r][3] = 0;
 #pragma unroll 4
     for (int c = 0; c < D; c += 4) {
-      float4 kk[4];
+      ulonglong2 kk[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) kk[j] = *(const float4*)(ks + (tx + 8 * j) * LD + c);
+      for (int j = 0; j < 4; ++j) kk[j] = *(const ulonglong2*)(ks + (tx + 8 * j) * LD + c);
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
-        const float4 qq = *(const float4*)(qs + (ty * RT + r) * LD + c);
+        const ulonglong2 qq = *(const ulonglong2*)(qs + (ty * RT + r) * LD + c);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[r][j] = fmaf(qq.x, kk[j].x, fmaf(qq.y, kk[j].y, fmaf(qq.z, kk[j].z, fmaf(qq.w, kk[j].w, s[r][j]))));
+        for (int j = 0; j < 4; ++j) fma2(s2[r][j], qq.x, kk[j].x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) fma2(s2[r][j], qq.y, kk[j].y);
       }
     }
     const bool masked = t * GK + GK - 1 > pos0 + i0 || (a.window > 0 && t * GK <= hi - a.window);
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       const int64_t pos = masked ? pos0 + (x0 + ty * RT + r) / rep : 0;
-      float top = -INFINITY;
+      float top = -INFINITY, s[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int64_t key = t * GK + tx + 8 * j;
-        float x = s[r][j] * a.scale;
+        const float2 f = both(s2[r][j]);
+        float x = (f.x + f.y) * a.scale;
         if (a.cap > 0.f) x = a.cap * tanhf(x / a.cap);
         if (masked && !(key <= pos && (a.window <= 0 || key > pos - a.window))) x = -INFINITY;
-        s[r][j] = x;
+        s[j] = x;
         top = fmaxf(top, x);
       }
 #pragma unroll
@@ -184,33 +199,32 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float e = expf(s[r][j] - base);
+        const float e = expf(s[j] - base);
         sum += e;
-        ps[(ty * RT + r) * (GK + 1) + tx + 8 * j] = e;
+        ps[(ty * RT + r) * (GK + 1) + tx + 8 * j] = pair(e, e);
       }
       l[r] = l[r] * corr + sum;  // (of this lane's keys)
       m[r] = m_new;
       if (corr != 1.f)
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[r][c][e] *= corr;
+        for (int c = 0; c < CT; ++c) {
+          mul2(o[r][c][0], pair(corr, corr));
+          mul2(o[r][c][1], pair(corr, corr));
+        }
     }
     __syncwarp();
 #pragma unroll 4
     for (int k = 0; k < GK; ++k) {
-      float p[RT];
+      uint64_t p[RT];
 #pragma unroll
       for (int r = 0; r < RT; ++r) p[r] = ps[(ty * RT + r) * (GK + 1) + k];
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
-        const float4 v = *(const float4*)(vs + k * LD + tx * 4 + c * 32);
+        const ulonglong2 v = *(const ulonglong2*)(vs + k * LD + tx * 4 + c * 32);
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-          o[r][c][0] = fmaf(p[r], v.x, o[r][c][0]);
-          o[r][c][1] = fmaf(p[r], v.y, o[r][c][1]);
-          o[r][c][2] = fmaf(p[r], v.z, o[r][c][2]);
-          o[r][c][3] = fmaf(p[r], v.w, o[r][c][3]);
+          fma2(o[r][c][0], p[r], v.x);
+          fma2(o[r][c][1], p[r], v.y);
         }
       }
     }
@@ -221,6 +235,10 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
   for (int r = 0; r < RT; ++r)
 #pragma unroll
     for (int w = 4; w; w >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], w);
+  auto values = [&](int r, int c, float f) {
+    const float2 u = both(o[r][c][0]), w = both(o[r][c][1]);
+    return make_float4(u.x * f, u.y * f, w.x * f, w.y * f);
+  };
   auto put4 = [&](int64_t x, int col, float4 v) {
     if (x >= n * rep || col >= a.d) return;
     T* to = (T*)a.out + ((tok0 + x / rep) * a.nh + kvh * rep + x % rep) * a.d + col;
@@ -231,7 +249,7 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
     for (int r = 0; r < RT; ++r) {
       const float f = l[r] > 0.f ? 1.f / l[r] : 0.f;
 #pragma unroll
-      for (int c = 0; c < CT; ++c) put4(x0 + ty * RT + r, tx * 4 + c * 32, make_float4(o[r][c][0] * f, o[r][c][1] * f, o[r][c][2] * f, o[r][c][3] * f));
+      for (int c = 0; c < CT; ++c) put4(x0 + ty * RT + r, tx * 4 + c * 32, values(r, c, f));
     }
     return;
   }
@@ -242,7 +260,7 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
     const int x = ty * RT + r;
     if (tx == 0) { ml[0][x] = m[r]; ml[1][x] = l[r]; }
 #pragma unroll
-    for (int c = 0; c < CT; ++c) *(float4*)(qs + x * LD + tx * 4 + c * 32) = make_float4(o[r][c][0], o[r][c][1], o[r][c][2], o[r][c][3]);
+    for (int c = 0; c < CT; ++c) *(float4*)(qs + x * LD + tx * 4 + c * 32) = values(r, c, 1.f);
   }
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   auto remote = [](const float* p, int rank) {
