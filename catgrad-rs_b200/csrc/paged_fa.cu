@@ -87,6 +87,13 @@ __device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, in
 }
 __device__ __forceinline__ void arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 
+// one lane of a converged warp
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+  return yes != 0;
+}
+
 template <int D, int NQ>
 __host__ __device__ constexpr int fa_stages() { return NQ == 2 ? 4 : D == 64 ? 4 : 2; }
 template <int D, int NQ>
@@ -117,7 +124,7 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
   volatile uint32_t* tmem_slot = (volatile uint32_t*)(gen + (b_v_ready + 8 - base));
   volatile int* cta_abort = (volatile int*)(gen + (b_v_ready + 12 - base));
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;  // (warp: known to be uniform)
   // q, the tables and the pages are written by the preceding kernels
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int qt = (int)gridDim.x - 1 - (int)blockIdx.x, kvh = blockIdx.y;  // longest first
@@ -213,48 +220,58 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
       }
   } else if (warp == 1 || (NQ == 2 && warp == 3)) {
     // ---- products ----
-    if (lane == 0) {
-      const int t = warp >> 1;
-      constexpr uint32_t idesc_s = umma_idesc(KT), idesc_o = umma_idesc(D) | (1u << 16);  // (V: MN-major)
-      const uint64_t dq = umma_desc(sq + t * Q_BYTES), dk = umma_desc(sk), dv = desc_mn(sv, KBOX);
-      const uint32_t cols = tmem_base + t * TILE_COLS, o_cols = cols + 2 * KT;
-      const uint32_t b_s = b_tile + 40 * t, b_p = b_s + 16, b_o = b_s + 32;
-      auto qk = [&](int j) {
-        const uint32_t buf = (uint32_t)j & 1u, stage = (uint32_t)(j % KS), ph = (uint32_t)(j / KS) & 1u;
-        if (!mbar_wait(b_k_full + 8 * stage, ph, cta_abort, p.rows.err)) return false;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    // The whole warp goes through the loop and one lane issues: descriptors then are uniform values, which an issue takes as they are.
+    // (A single lane's loop: some 70 cycles an issue where a product of 64 keys takes 48.)
+    const int t = warp >> 1;
+    const bool issues = elect_one();
+    constexpr uint32_t idesc_s = umma_idesc(KT), idesc_o = umma_idesc(D) | (1u << 16);  // (V: MN-major)
+    const uint64_t dq = umma_desc(sq + t * Q_BYTES), dk = umma_desc(sk), dv = desc_mn(sv, KBOX);
+    const uint32_t cols = tmem_base + t * TILE_COLS, o_cols = cols + 2 * KT;
+    const uint32_t b_s = b_tile + 40 * t, b_p = b_s + 16, b_o = b_s + 32;
+    auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, cta_abort, p.rows.err)) != 0; };
+    auto qk = [&](int j) {
+      const uint32_t buf = (uint32_t)j & 1u, stage = (uint32_t)(j % KS), ph = (uint32_t)(j / KS) & 1u;
+      if (!wait(b_k_full + 8 * stage, ph)) return false;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (issues) {
+        const uint64_t dks = dk + ((stage * KV_BYTES) >> 4);
 #pragma unroll
         for (int kk = 0; kk < D / UMMA_K; ++kk) {
           const uint64_t oq = ((uint32_t)(kk / 4) * BOX + (uint32_t)(kk % 4) * 32u) >> 4, ok = ((uint32_t)(kk / 4) * KBOX + (uint32_t)(kk % 4) * 32u) >> 4;
-          umma_bf16(cols + buf * KT, dq + oq, dk + ((stage * KV_BYTES) >> 4) + ok, idesc_s, kk > 0 ? 1u : 0u);
+          umma_bf16(cols + buf * KT, dq + oq, dks + ok, idesc_s, kk > 0 ? 1u : 0u);
         }
         umma_commit(b_s + 8 * buf);
         umma_commit(b_k_empty + 8 * stage);
-        return true;
-      };
-      auto pv = [&](int j) {
-        const uint32_t buf = (uint32_t)j & 1u, stage = (uint32_t)(j % KS), ph = (uint32_t)(j / KS) & 1u;
-        if (!mbar_wait(b_v_full + 8 * stage, ph, cta_abort, p.rows.err)) return false;
-        if (j == nt - 1 && seen < KT) {
-          // (warp 2 clears what no query sees while the softmax runs)
-          if (t == 0) arrive(b_v_last);
-          if (!mbar_wait(b_v_ready, 0, cta_abort, p.rows.err)) return false;
-        }
-        if (!mbar_wait(b_p + 8 * buf, (uint32_t)(j >> 1) & 1u, cta_abort, p.rows.err)) return false;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      }
+      __syncwarp();
+      return true;
+    };
+    auto pv = [&](int j) {
+      const uint32_t buf = (uint32_t)j & 1u, stage = (uint32_t)(j % KS), ph = (uint32_t)(j / KS) & 1u;
+      if (!wait(b_v_full + 8 * stage, ph)) return false;
+      if (j == nt - 1 && seen < KT) {
+        // (warp 2 clears what no query sees while the softmax runs)
+        if (t == 0 && issues) arrive(b_v_last);
+        if (!wait(b_v_ready, 0)) return false;
+      }
+      if (!wait(b_p + 8 * buf, (uint32_t)(j >> 1) & 1u)) return false;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (issues) {
+        const uint64_t dvs = dv + ((stage * KV_BYTES) >> 4);
 #pragma unroll
         for (int kk = 0; kk < KT / UMMA_K; ++kk)
-          umma_ts(o_cols, cols + buf * KT + kk * (UMMA_K / 2), dv + ((stage * KV_BYTES + (uint32_t)kk * (UMMA_K * 128u)) >> 4), idesc_o, j > 0 || kk > 0 ? 1u : 0u);
+          umma_ts(o_cols, cols + buf * KT + kk * (UMMA_K / 2), dvs + (((uint32_t)kk * (UMMA_K * 128u)) >> 4), idesc_o, j > 0 || kk > 0 ? 1u : 0u);
         umma_commit(b_o);
         umma_commit(b_v_empty + 8 * stage);
-        return true;
-      };
-      // Scores overwrite the probabilities that lay in their columns, and products with different accumulators are not
-      // ordered among themselves: the product that reads them is waited for.
-      auto done = [&](int j) { return mbar_wait(b_o, (uint32_t)j & 1u, cta_abort, p.rows.err); };
-      bool ok = mbar_wait(b_q, 0, cta_abort, p.rows.err) && qk(0);
-      for (int j = 0; j < nt && ok; ++j) ok = (j + 1 >= nt || ((j == 0 || done(j - 1)) && qk(j + 1))) && pv(j);
-    }
+      }
+      __syncwarp();
+      return true;
+    };
+    // Scores overwrite the probabilities that lay in their columns, and products with different accumulators are not
+    // ordered among themselves: the product that reads them is waited for.
+    auto done = [&](int j) { return wait(b_o, (uint32_t)j & 1u); };
+    bool ok = wait(b_q, 0) && qk(0);
+    for (int j = 0; j < nt && ok; ++j) ok = (j + 1 >= nt || ((j == 0 || done(j - 1)) && qk(j + 1))) && pv(j);
   } else if (warp == 2) {
     if (seen < KT) {
       const uint32_t stage = (uint32_t)((nt - 1) % KS);
@@ -295,15 +312,17 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
       ld32(s_addr + 32, v + 32);
       asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
       // uniform: some key may be masked for some row
-      if (k0 + KT - 1 > tile_first || (p.window > 0 && k0 <= tile_last - p.window)) {
+      const bool masked = k0 + KT - 1 > tile_first || (p.window > 0 && k0 <= tile_last - p.window);
+      uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
+      if (masked) {
         // column c is visible to this row iff low <= c <= lim
         const int64_t lim64 = qpos - k0, low64 = p.window > 0 ? lim64 - p.window + 1 : 0;
         const int lim = lim64 > KT ? KT : (lim64 < -1 ? -1 : (int)lim64), low = low64 < 0 ? 0 : (low64 > KT ? KT : (int)low64);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const uint32_t vis = bits_below(lim + 1 - c * 32) & ~bits_below(low - c * 32);
+          vis[c] = bits_below(lim + 1 - c * 32) & ~bits_below(low - c * 32);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[c * 32 + i] = vis & (1u << i) ? v[c * 32 + i] : 0xff800000u;
+          for (int i = 0; i < 32; ++i) v[c * 32 + i] = vis[c] & (1u << i) ? v[c * 32 + i] : 0xff800000u;
         }
       }
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -340,25 +359,24 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
       }
       const float mc = m == -INFINITY ? 0.f : m;
       float ls[2] = {0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      // probabilities of a half of the tile; `exponent` of a score
+      auto half = [&](int c, auto exponent) {
         uint32_t pk[16];
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-          float e[2];
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const float x = __uint_as_float(v[c * 32 + i + u]);
-            // (masked scores are -inf; their cap would be finite)
-            if (CAP) e[u] = x == -INFINITY ? 0.f : fast_exp2(fmaf(2.f * p.cap_log2e, rcp_newton(1.f + fast_exp2(x * p.cap_unit)), -p.cap_log2e - mc));
-            else e[u] = fast_exp2(fmaf(x, p.scale_log2e, -mc));
-          }
-          const __nv_bfloat162 pr = __floats2bfloat162_rn(e[0], e[1]);
-          pk[i / 2] = *(const uint32_t*)&pr;
+          const float e0 = fast_exp2(exponent(__uint_as_float(v[c * 32 + i]))), e1 = fast_exp2(exponent(__uint_as_float(v[c * 32 + i + 1])));
+          pk[i / 2] = pack_bf16(e0, e1);
+          // (masked scores are -inf, whose cap is not)
+          if (CAP && masked) pk[i / 2] &= (vis[c] >> i & 1u ? 0xffffu : 0u) | (vis[c] >> i & 2u ? 0xffff0000u : 0u);
           ls[0] += __uint_as_float(pk[i / 2] << 16);
           ls[1] += __uint_as_float(pk[i / 2] & 0xffff0000u);
         }
         st16(s_addr + (uint32_t)c * 16u, pk);
+      };
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        if (CAP) half(c, [&](float x) { return fmaf(2.f * p.cap_log2e, rcp_newton(1.f + fast_exp2(x * p.cap_unit)), -p.cap_log2e - mc); });
+        else half(c, [&](float x) { return fmaf(x, p.scale_log2e, -mc); });
       }
       // (This warp may be a whole product ahead of the tensor core, and a parity tells only neighbouring phases apart: the
       // last product but one is waited for here, where the last cannot have been issued.)
