@@ -483,9 +483,8 @@ class CudaBackend(TraitBackend):
         a new tensor of zeros behind the last row's token if none is given."""
         if q is not None and q_out is None:
             q_out = self._empty_like_pages(q.shape, k_pages)
-        h = [None if t is None else t._h for t in (q, k, v, q_gain, k_gain)]
-        st = self._lib.cg_paged_append(self._ctx, *h, eps, plus_one, cos and cos._h, sin and sin._h, rot_half, table._h, starts._h, lens._h,
-                                       k_pages._h, v_pages._h, q_out and q_out._h)
+        st = self._lib.cg_paged_append(self._ctx, q and q._h, k._h, v._h, q_gain and q_gain._h, k_gain and k_gain._h, eps, plus_one, cos and cos._h,
+                                       sin and sin._h, rot_half, table._h, starts._h, lens._h, k_pages._h, v_pages._h, q_out and q_out._h)
         if st:
             self._check(st)
         return q_out
@@ -505,9 +504,10 @@ class CudaBackend(TraitBackend):
         if out is None:
             shape = (logits.shape[0], k)
             out = (self.zeros(shape, F32), *(self.zeros(shape, U32) for _ in range(3)))
-        elif any(t.shape[-1:] != (k,) for t in out):
-            raise BackendPanic(1, "Shape mismatch in operation: an output")
-        st = self._lib.cg_beam_select(self._ctx, logits._h, scores._h, finished and finished._h, end, *(t._h for t in out))
+        s, t, p, f = out
+        if s.shape[-1:] != (k,):
+            raise BackendPanic(1, "Shape mismatch in operation: scores")
+        st = self._lib.cg_beam_select(self._ctx, logits._h, scores._h, finished and finished._h, end, s._h, t._h, p._h, f._h)
         if st:
             self._check(st)
         return out

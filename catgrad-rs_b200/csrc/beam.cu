@@ -209,6 +209,126 @@ __device__ __noinline__ uint4 load_edge(const T* row, int at, int limit) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// What is rare is kept out of the kernel's way (instructions are read once a call, so their number counts).
+// The largest values of a piece whose list ran over: those above the K-th largest of 32 groups' maxima and, in the order of their
+// places, K that are equal to it; or K rounds of a common maximum.  By all of its 256 threads.
+template <typename T>
+__device__ __noinline__ void rank_again(PieceWork& w, const T* row, int at0, int V, int K, int room, int slot) {
+  constexpr int per = Values<T>::per;
+  const int sb = threadIdx.x / BT, tid = threadIdx.x % BT, warp = tid >> 5, lane = tid & 31;
+  auto sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(sb + 1), "r"(BT) : "memory"); };
+  auto take = [&](int at, float v) {
+    const int n = atomicAdd(&w.count[slot], 1);
+    if (n < room) w.pool[slot * room + n] = key_at(v, at);
+  };
+  float mx = -INFINITY;
+#pragma unroll 1
+  for (int v = 0; v < VECS; ++v)
+#pragma unroll
+    for (int i = 0; i < per; ++i) {
+      const int at = at0 + v * BT * per + i;
+      if (at >= 0 && at < V) mx = fmaxf(mx, (float)row[at]);
+    }
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  sync();
+  if ((lane & 7) == 0) w.groups[0][tid >> 3] = mx;
+  if (tid == 0) w.count[slot] = 0;
+  sync();
+  uint32_t left = up(w.groups[0][lane]), kth = 0;
+  for (int r = 0; r < K; ++r) {
+    kth = __reduce_max_sync(0xffffffffu, left);
+    if (lane == __ffs(__ballot_sync(0xffffffffu, left == kth)) - 1) left = 0;
+  }
+  const float bound = down(kth);
+  auto side = [&](int at) {  // 1 above the bound, 0 at it, -1 below
+    const float v = (float)row[at], c = v == v ? v : -INFINITY;
+    return c > bound ? 1 : c == bound ? 0 : -1;
+  };
+  if (mx > bound)
+#pragma unroll 1
+    for (int v = 0; v < VECS; ++v)
+#pragma unroll 1
+      for (int i = 0; i < per; ++i) {
+        const int at = at0 + v * BT * per + i;
+        if (at >= 0 && at < V && side(at) > 0) take(at, (float)row[at]);
+      }
+  sync();
+  const int above = w.count[slot];
+  if (above + K <= room) {
+    int have = 0;
+#pragma unroll 1
+    for (int v = 0; v < VECS && have < K; ++v) {
+      uint32_t level = 0;
+#pragma unroll
+      for (int i = 0; i < per; ++i) {
+        const int at = at0 + v * BT * per + i;
+        if (at >= 0 && at < V && side(at) == 0) level |= 1u << i;
+      }
+      int before = __popc(level);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int more = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += more;
+      }
+      if (lane == 31) w.equal[warp] = before;
+      sync();
+      before -= __popc(level);
+      int all_of = 0;
+      for (int i = 0; i < BT / 32; ++i) {
+        if (i < warp) before += w.equal[i];
+        all_of += w.equal[i];
+      }
+      for (int n = have + before; level && n < K; ++n, level &= level - 1) {
+        const int at = at0 + v * BT * per + __ffs(level) - 1;
+        w.pool[slot * room + above + n] = key_at((float)row[at], at);
+      }
+      have += all_of;
+      sync();
+    }
+    if (tid == 0) w.count[slot] = above + min(have, K);
+  } else {
+    uint64_t last = ~0ull;
+    for (int r = 0; r < K; ++r) {
+      uint64_t best = 0;
+#pragma unroll 1
+      for (int v = 0; v < VECS; ++v)
+#pragma unroll
+        for (int i = 0; i < per; ++i) {
+          const int at = at0 + v * BT * per + i;
+          const uint64_t key = at >= 0 && at < V ? key_at((float)row[at], at) : 0;
+          if (key < last && key > best) best = key;
+        }
+      int who;
+      best = warp_best(best, &who);
+      if (lane == 0) w.best[warp] = best;
+      sync();
+      for (int i = 0; i < BT / 32; ++i) best = w.best[i] > best ? w.best[i] : best;
+      if (tid == 0) w.pool[slot * room + r] = best;
+      last = best;
+      sync();
+    }
+    if (tid == 0) w.count[slot] = K;  // (places without a value are 0)
+  }
+  sync();
+}
+// This thread's sum of exponentials where some values are NaN.
+template <typename T>
+__device__ __noinline__ float sum_of_numbers(const T* row, int at0, int V, float peak) {
+  constexpr int per = Values<T>::per;
+  float sum = 0.f;
+#pragma unroll 1
+  for (int v = 0; v < VECS; ++v)
+#pragma unroll 1
+    for (int i = 0; i < per; ++i) {
+      const int at = at0 + v * BT * per + i;
+      if (at < 0 || at >= V) continue;
+      const float x = (float)row[at];
+      if (x == x) sum += fast_exp2((x - peak) * LOG2E);
+    }
+  return sum;
+}
+
 // dynamic shared memory: PieceWork [SB]; lists u64 [rounds][SB][K]; sums f64 [rounds][SB]; totals u64 [J][K]; places u64 [J][K];
 // tops f32 [rounds][SB]; marks u32 [J]; then per joining warp a beam's lists of all blocks, u64 [pieces][K]
 template <typename T, int SB>
@@ -272,106 +392,6 @@ __global__ void __launch_bounds__(SB * BT, 4 / SB) k_beam_select(SelectArgs a) {
         }
       }
   };
-  auto take = [&](int slot, int at, float v) {
-    const int n = atomicAdd(&w.count[slot], 1);
-    if (n < room) w.pool[slot * room + n] = key_at(v, at);
-  };
-  // The largest values of a piece whose list ran over: those above the K-th largest of 32 groups' maxima and, in the order of their
-  // places, K that are equal to it; or K rounds of a common maximum.
-  auto again = [&](int u, int slot) {
-    locate(u);
-    float mx = -INFINITY;
-#pragma unroll 1
-    for (int v = 0; v < VECS; ++v)
-#pragma unroll
-      for (int i = 0; i < per; ++i) {
-        const int at = at0 + v * BT * per + i;
-        if (at >= 0 && at < a.V) mx = fmaxf(mx, (float)row[at]);
-      }
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    sync();
-    if ((lane & 7) == 0) w.groups[0][tid >> 3] = mx;
-    if (tid == 0) w.count[slot] = 0;
-    sync();
-    uint32_t left = up(w.groups[0][lane]), kth = 0;
-    for (int r = 0; r < K; ++r) {
-      kth = __reduce_max_sync(0xffffffffu, left);
-      if (lane == __ffs(__ballot_sync(0xffffffffu, left == kth)) - 1) left = 0;
-    }
-    const float bound = down(kth);
-    auto side = [&](int at) {  // 1 above the bound, 0 at it, -1 below
-      const float v = (float)row[at], c = v == v ? v : -INFINITY;
-      return c > bound ? 1 : c == bound ? 0 : -1;
-    };
-    if (mx > bound)
-#pragma unroll 1
-      for (int v = 0; v < VECS; ++v)
-#pragma unroll 1
-        for (int i = 0; i < per; ++i) {
-          const int at = at0 + v * BT * per + i;
-          if (at >= 0 && at < a.V && side(at) > 0) take(slot, at, (float)row[at]);
-        }
-    sync();
-    const int above = w.count[slot];
-    if (above + K <= room) {
-      int have = 0;
-#pragma unroll 1
-      for (int v = 0; v < VECS && have < K; ++v) {
-        uint32_t level = 0;
-#pragma unroll
-        for (int i = 0; i < per; ++i) {
-          const int at = at0 + v * BT * per + i;
-          if (at >= 0 && at < a.V && side(at) == 0) level |= 1u << i;
-        }
-        int before = __popc(level);
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int more = __shfl_up_sync(0xffffffffu, before, o);
-          if (lane >= o) before += more;
-        }
-        if (lane == 31) w.equal[warp] = before;
-        sync();
-        before -= __popc(level);
-        int all_of = 0;
-        for (int i = 0; i < BT / 32; ++i) {
-          if (i < warp) before += w.equal[i];
-          all_of += w.equal[i];
-        }
-        for (int n = have + before; level && n < K; ++n, level &= level - 1) {
-          const int at = at0 + v * BT * per + __ffs(level) - 1;
-          w.pool[slot * room + above + n] = key_at((float)row[at], at);
-        }
-        have += all_of;
-        sync();
-      }
-      if (tid == 0) w.count[slot] = above + min(have, K);
-    } else {
-      uint64_t last = ~0ull;
-      for (int r = 0; r < K; ++r) {
-        uint64_t best = 0;
-#pragma unroll 1
-        for (int v = 0; v < VECS; ++v)
-#pragma unroll
-          for (int i = 0; i < per; ++i) {
-            const int at = at0 + v * BT * per + i;
-            const uint64_t key = at >= 0 && at < a.V ? key_at((float)row[at], at) : 0;
-            if (key < last && key > best) best = key;
-          }
-        int who;
-        best = warp_best(best, &who);
-        if (lane == 0) w.best[warp] = best;
-        sync();
-        for (int i = 0; i < BT / 32; ++i) best = w.best[i] > best ? w.best[i] : best;
-        if (tid == 0) w.pool[slot * room + r] = best;
-        last = best;
-        sync();
-      }
-      if (tid == 0) w.count[slot] = K;  // (places without a value are 0)
-    }
-    sync();
-  };
-
   int slot = 0, begun = 0;  // the round of slot 0
   for (int i = 0; i < a.rounds; ++i) {
     const int u = (i * (int)n_ranks + (int)rank) * SB + sb;
@@ -430,16 +450,7 @@ __global__ void __launch_bounds__(SB * BT, 4 / SB) k_beam_select(SelectArgs a) {
       if (peak > -INFINITY && peak < INFINITY) {
 #pragma unroll
         for (int q = 0; q < 4 * VECS; q += 16) sum += Vals::exps(x + q, peak);
-        if (!(sum == sum)) {  // some are NaN
-          sum = 0.f;
-#pragma unroll
-          for (int q = 0; q < 4 * VECS; q += 16)
-#pragma unroll
-            for (int e = 0; e < Vals::n; ++e) {
-              const float v = Vals::at(x + q, e);
-              sum += v == v ? fast_exp2((v - peak) * LOG2E) : 0.f;
-            }
-        }
+        if (!(sum == sum)) sum = sum_of_numbers<T>(row, at0, a.V, peak);
       }
 #pragma unroll
       for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -450,7 +461,10 @@ __global__ void __launch_bounds__(SB * BT, 4 / SB) k_beam_select(SelectArgs a) {
     if (slot > 0 && (slot == slots || i + 1 == a.rounds)) {  // the slots' lists: a warp has slots warp, warp + 8
       sync();
       for (int q = 0; q < slot; ++q)
-        if (w.count[q] > room) again(((begun + q) * (int)n_ranks + (int)rank) * SB + sb, q);
+        if (w.count[q] > room) {
+          locate(((begun + q) * (int)n_ranks + (int)rank) * SB + sb);
+          rank_again<T>(w, row, at0, a.V, K, room, q);
+        }
       for (int q = warp; q < slot; q += BT / 32) {
         const int place = (begun + q) * SB + sb, n = w.count[q];
         double s = lane < BT / 32 ? (double)w.part[q][lane] : 0.;
@@ -690,15 +704,10 @@ extern "C" int32_t cg_beam_select(cg_ctx* c, const cg_tensor* logits, const cg_t
   if (V > 1ll << 30) return fail(c, CG_ERR_UNSUPPORTED, "vocabulary too large");
   if (finished && (int64_t)end >= V) return fail(c, CG_ERR_INVALID, "the end token is not in the vocabulary");
   // the scores and marks of a group are read before its new ones are written, so they may take their place
-  const cg_tensor* outs[4] = {scores_out, tokens_out, parents_out, finished_out};
-  for (int i = 0; i < 4; ++i) {
-    for (int j = 0; j < i; ++j)
-      if (overlap(outs[i], outs[j])) return fail(c, CG_ERR_INVALID, "outputs overlap");
-    const bool whole = K == J;
-    const bool bad = overlap(outs[i], logits) || (overlap(outs[i], scores) && !(whole && i == 0 && scores_out->data() == scores->data())) ||
-                     (finished && overlap(outs[i], finished) && !(whole && i == 3 && finished_out->data() == finished->data()));
-    if (bad) return fail(c, CG_ERR_INVALID, "an output overlaps an input");
-  }
+  const bool whole = K == J, same_scores = whole && scores_out->data() == scores->data(), same_marks = whole && finished && finished_out->data() == finished->data();
+  if (overlap_any({logits, same_scores ? nullptr : scores, same_marks ? nullptr : finished}, {scores_out, tokens_out, parents_out, finished_out}) ||
+      (same_scores && finished && overlap(Extent(scores), Extent(finished))) || (same_marks && overlap(Extent(finished), Extent(scores))))
+    return fail(c, CG_ERR_INVALID, "an output overlaps an input or another one");
   if (B == 0 || K == 0) return CG_OK;
   if (J == 0) return fail(c, CG_ERR_SHAPE, "no beams");
   SelectArgs a = {};

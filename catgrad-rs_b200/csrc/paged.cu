@@ -428,10 +428,8 @@ int32_t cg_paged_append(cg_ctx* c, const cg_tensor* q, const cg_tensor* k, const
     if (cos_t->storage != ST_F32 || sin_t->storage != ST_F32) return fail(c, CG_ERR_DTYPE, "angles are f32");
     if (2 * cos_t->dims[1] > d) return fail(c, CG_ERR_SHAPE, "more angles than pairs of a head");
   }
-  for (const cg_tensor* in : {q, k, v, q_gain, k_gain, cos_t, sin_t, table, starts, lens})
-    for (const cg_tensor* o : {(const cg_tensor*)k_pages, (const cg_tensor*)v_pages, (const cg_tensor*)q_out})
-      if (in && o && overlap(in, o)) return fail(c, CG_ERR_INVALID, "an input overlaps what is written");
-  if (q_out && (overlap(q_out, k_pages) || overlap(q_out, v_pages))) return fail(c, CG_ERR_INVALID, "q_out overlaps the pages");
+  if (overlap_any({q, k, v, q_gain, k_gain, cos_t, sin_t, table, starts, lens}, {k_pages, v_pages, q_out}))
+    return fail(c, CG_ERR_INVALID, "what is written overlaps an input or each other");
   if (M == 0 || a.rows.rows == 0) return CG_OK;
   a.q = q ? q->data() : nullptr; a.k = k->data(); a.v = v->data();
   if (q) { a.q_ld = q->strides[0]; a.q_hs = q->strides[1]; }
@@ -475,9 +473,7 @@ int32_t cg_paged_reorder(cg_ctx* c, const cg_tensor* parents, const cg_tensor* l
   CG_TRY(check_tensor(c, own, "own", CG_U32, 2, table->dims));
   if (K > 32) return fail(c, CG_ERR_UNSUPPORTED, "at most 32 beams");
   if (B > 65535 || L > 32767 || dims[1] > 65535) return fail(c, CG_ERR_UNSUPPORTED, "too many groups, layers or heads");
-  for (const cg_tensor* in : {parents, lens, own})
-    if (overlap(in, table) || overlap(in, k_pages) || overlap(in, v_pages)) return fail(c, CG_ERR_INVALID, "an input overlaps what is written");
-  if (overlap(table, k_pages) || overlap(table, v_pages)) return fail(c, CG_ERR_INVALID, "table overlaps the pages");
+  if (overlap_any({parents, lens, own}, {table, k_pages, v_pages})) return fail(c, CG_ERR_INVALID, "what is written overlaps an input or each other");
   if (B == 0 || K == 0 || table->dims[1] == 0 || L == 0) return CG_OK;
   a.parents = (const uint32_t*)parents->data();
   a.lens = (const uint32_t*)lens->data();

@@ -72,21 +72,37 @@ inline int check_tensor(cg_ctx* c, const cg_tensor* t, const char* what, int tag
   if (contiguous && t->numel() && !t->contiguous()) return fail(c, CG_ERR_UNSUPPORTED, std::string(what) + " must be contiguous");
   return same_device(c, t, what);
 }
-inline void bytes_of(const cg_tensor* t, uintptr_t* lo, uintptr_t* hi) {
-  int64_t last = 0, n = 1;
-  for (int i = 0; i < t->rank; ++i) {
-    n *= t->dims[i];
-    last += (t->dims[i] - 1) * t->strides[i];
+// Where a tensor's memory lies (its whole extent); nowhere: null or without elements.
+struct Extent {
+  uintptr_t lo = 0, hi = 0;
+  Extent() = default;
+  Extent(const cg_tensor* t) {
+    if (!t) return;
+    int64_t last = 0;
+    for (int i = 0; i < t->rank; ++i) {
+      if (t->dims[i] == 0) return;
+      last += (t->dims[i] - 1) * t->strides[i];
+    }
+    lo = (uintptr_t)t->data();
+    hi = lo + (size_t)(last + 1) * t->esize();
   }
-  *lo = (uintptr_t)t->data();
-  *hi = n ? *lo + (size_t)(last + 1) * t->esize() : *lo;
-}
-// Whether two tensors' memory touches (their whole extents are compared).
-inline bool overlap(const cg_tensor* a, const cg_tensor* b) {
-  uintptr_t a0, a1, b0, b1;
-  bytes_of(a, &a0, &a1);
-  bytes_of(b, &b0, &b1);
-  return a0 < b1 && b0 < a1;
+};
+inline bool overlap(const Extent& a, const Extent& b) { return a.lo < b.hi && b.lo < a.hi; }
+// Whether what is written touches an input, or one of the others that are written.
+template <int NI, int NO>
+inline bool overlap_any(const cg_tensor* const (&in)[NI], const cg_tensor* const (&out)[NO]) {
+  Extent o[NO];
+  for (int i = 0; i < NO; ++i) {
+    o[i] = Extent(out[i]);
+    for (int j = 0; j < i; ++j)
+      if (overlap(o[i], o[j])) return true;
+  }
+  for (const cg_tensor* t : in) {
+    const Extent e(t);
+    for (const Extent& x : o)
+      if (overlap(e, x)) return true;
+  }
+  return false;
 }
 // `t` is written in place: no two of its elements share memory (contiguous), a cached GEMM operand copy is stale, and a literal's value
 // is no longer known.
@@ -108,7 +124,6 @@ inline int check_pages(cg_ctx* c, const cg_tensor* k, const cg_tensor* v, bool l
   if (d < 8 || d > 256 || d % 8) return fail(c, CG_ERR_UNSUPPORTED, "head sizes are multiples of 8 up to 256");
   if (k->dims[rank - 4] > 0xFFFFFFFFll) return fail(c, CG_ERR_UNSUPPORTED, "too many pages");
   if (((uintptr_t)k->data() | (uintptr_t)v->data()) % 16) return fail(c, CG_ERR_UNSUPPORTED, "pages begin on a 16-byte boundary");
-  if (overlap(k, v)) return fail(c, CG_ERR_INVALID, "k_pages and v_pages overlap");
   int b = 0;
   while ((int64_t)1 << b < page) ++b;
   *lg = b;

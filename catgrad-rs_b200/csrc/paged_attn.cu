@@ -355,8 +355,7 @@ extern "C" int32_t cg_paged_attention(cg_ctx* c, const cg_tensor* q, const cg_te
   if (nkv < 1 || nkv > 65535 || nh > 65535) return fail(c, CG_ERR_UNSUPPORTED, "too many heads");
   if (nh % nkv) return fail(c, CG_ERR_SHAPE, "query heads are a multiple of key heads");
   if (max_new < 0 || window < 0 || !(softcap >= 0.f) || !(scale >= 0.f) || scale > 3e38f || softcap > 3e38f) return fail(c, CG_ERR_INVALID, "bad argument");
-  for (const cg_tensor* in : {q, k_pages, v_pages, table, starts, lens})
-    if (overlap(in, out)) return fail(c, CG_ERR_INVALID, "out overlaps an input");
+  if (overlap_any({q, k_pages, v_pages, table, starts, lens}, {out})) return fail(c, CG_ERR_INVALID, "out overlaps an input");
   if (M == 0 || nh == 0 || a.rows.rows == 0) return CG_OK;
   a.q = q->data(); a.k_pages = k_pages->data(); a.v_pages = v_pages->data(); a.out = out->data();
   a.q_ld = q->strides[0]; a.q_hs = q->strides[1];
