@@ -269,69 +269,68 @@ struct ReorderArgs {
   char *k_pages, *v_pages;
   int64_t cols, n_pages, layer_bytes;  // bytes of a layer's pages
   int lg, K, nkv, token_bytes;         // bytes of a head's token
+  int pools;                           // layers, keys and values
   int32_t* err;
 };
 
-// Group blockIdx.y; z: the layer's keys (even) or values (odd).  All of a group's copies go through the registers of the
-// thread that makes them: it has read the K sources of its 16 bytes before it writes them, so pages may change
-// places.  The sources are the parents' own pages, which nobody else's targets are.
+// Group blockIdx.y.  All of a group's copies go through the registers of the thread that makes them: it has read the K sources of
+// its 16 bytes before it writes them, so pages may change places.  The sources are the parents' own pages, which nobody
+// else's targets are.  What bounds it is the bytes; a block looks its group up once and then has pieces of all layers.
 template <int KM>
 __global__ void __launch_bounds__(256) k_paged_reorder(ReorderArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ int64_t src[KM], dst[KM];
   __shared__ int par[KM];
-  __shared__ int bad;
   const int64_t row0 = (int64_t)blockIdx.y * a.K;
   const int j = threadIdx.x;
-  if (j == 0) bad = 0;
-  __syncthreads();
   const int64_t len = a.lens[row0], cur = len >> a.lg;
   const int begun = (int)(len & ((1 << a.lg) - 1));
+  bool ok = true;
   if (j < a.K) {
     const uint32_t p = a.parents[row0 + j];
+    ok = p < (uint32_t)a.K && a.lens[row0 + j] == len && cur + (begun > 0) <= a.cols;
     par[j] = (int)p;
     src[j] = dst[j] = 0;
-    bool ok = p < (uint32_t)a.K && a.lens[row0 + j] == len && cur + (begun > 0) <= a.cols;
     if (ok && begun) {
       src[j] = a.own[(row0 + p) * a.cols + cur];
       dst[j] = a.own[(row0 + j) * a.cols + cur];
       ok = src[j] < a.n_pages && dst[j] < a.n_pages;
-      for (int i = 0; i < j; ++i) ok = ok && a.own[(row0 + i) * a.cols + cur] != dst[j];  // (a page of its own)
     }
-    if (!ok) bad = 1;
   }
   __syncthreads();
-  if (bad) {
+  if (begun && j < a.K)
+    for (int i = 0; i < j; ++i) ok = ok && dst[i] != dst[j];  // (a page of its own)
+  if (__syncthreads_or(!ok)) {
     if (j == 0) *a.err = DEV_INDEX;
     return;
   }
   const int64_t t0 = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, step = (int64_t)gridDim.x * blockDim.x;
   if (begun) {
-    char* base = (blockIdx.z & 1 ? a.v_pages : a.k_pages) + (int64_t)(blockIdx.z >> 1) * a.layer_bytes;
-    const int64_t head_bytes = (int64_t)a.token_bytes << a.lg;
-    const int64_t per = (int64_t)begun * a.token_bytes / 16;  // 16-byte pieces of a head
-    for (int64_t i = t0; i < per * a.nkv; i += step) {
-      const int64_t h = i / per, at = h * head_bytes + (i - h * per) * 16;
+    const uint32_t head_bytes = (uint32_t)a.token_bytes << a.lg, per = (uint32_t)begun * (uint32_t)a.token_bytes / 16;  // 16-byte pieces of a head
+    const int64_t page_bytes = (int64_t)a.nkv * head_bytes, all = (int64_t)per * a.nkv * a.pools;
+    for (int64_t i = t0; i < all; i += step) {
+      const int64_t ph = i / per;
+      const uint32_t pool = (uint32_t)(ph / a.nkv), h = (uint32_t)(ph - (int64_t)pool * a.nkv), off = (uint32_t)(i - ph * per) * 16u;
+      char* base = (pool & 1 ? a.v_pages : a.k_pages) + (int64_t)(pool >> 1) * a.layer_bytes + (int64_t)h * head_bytes + off;
       uint4 x[KM];
 #pragma unroll
       for (int q = 0; q < KM; ++q)
-        if (q < a.K && par[q] != q) x[q] = *(const uint4*)(base + src[q] * a.nkv * head_bytes + at);
+        if (q < a.K && par[q] != q) x[q] = *(const uint4*)(base + src[q] * page_bytes);
 #pragma unroll
       for (int q = 0; q < KM; ++q)
-        if (q < a.K && par[q] != q) *(uint4*)(base + dst[q] * a.nkv * head_bytes + at) = x[q];
+        if (q < a.K && par[q] != q) *(uint4*)(base + dst[q] * page_bytes) = x[q];
     }
   }
-  if (blockIdx.z == 0)
-    for (int64_t p = t0; p < a.cols; p += step) {
-      uint32_t x[KM];
+  for (int64_t p = t0; p < a.cols; p += step) {
+    uint32_t x[KM];
 #pragma unroll
-      for (int q = 0; q < KM; ++q)
-        if (q < a.K) x[q] = p < cur ? a.table[(row0 + par[q]) * a.cols + p] : a.own[(row0 + q) * a.cols + p];
+    for (int q = 0; q < KM; ++q)
+      if (q < a.K) x[q] = p < cur ? a.table[(row0 + par[q]) * a.cols + p] : a.own[(row0 + q) * a.cols + p];
 #pragma unroll
-      for (int q = 0; q < KM; ++q)
-        if (q < a.K) a.table[(row0 + q) * a.cols + p] = x[q];
-    }
+    for (int q = 0; q < KM; ++q)
+      if (q < a.K) a.table[(row0 + q) * a.cols + p] = x[q];
+  }
 }
 
 // [M, heads, d], the components next to each other
@@ -372,10 +371,11 @@ int launch_append(cg_ctx* c, const AppendArgs& a) {
 }
 
 template <int KM>
-int launch_reorder(cg_ctx* c, const ReorderArgs& a, int64_t groups, int64_t layers) {
-  const int64_t pieces = std::max<int64_t>(((int64_t)a.nkv * a.token_bytes << a.lg) / 32, a.cols);
-  dim3 grid((unsigned)std::min<int64_t>((pieces + 255) / 256, 1024), (unsigned)groups, (unsigned)(2 * layers));
-  CG_CUDA(c, launch_kernel(c, k_paged_reorder<KM>, grid, dim3(256), 0, 1, a));
+int launch_reorder(cg_ctx* c, const ReorderArgs& a, int64_t groups) {
+  // At most what runs at a time (four blocks of 256 per SM), at least a block per group.
+  const int64_t pieces = std::max<int64_t>((((int64_t)a.nkv * a.token_bytes) << a.lg) / 16 * a.pools, a.cols);
+  const int64_t blocks = std::min<int64_t>((pieces + 255) / 256, std::max<int64_t>(148 * 4 / groups, 1));
+  CG_CUDA(c, launch_kernel(c, k_paged_reorder<KM>, dim3((unsigned)blocks, (unsigned)groups), dim3(256), 0, 1, a));
   CG_LAUNCHED(c);
   return CG_OK;
 }
@@ -472,7 +472,7 @@ int32_t cg_paged_reorder(cg_ctx* c, const cg_tensor* parents, const cg_tensor* l
   CG_TRY(check_tensor(c, table, "table", CG_U32, 2, tab));
   CG_TRY(check_tensor(c, own, "own", CG_U32, 2, table->dims));
   if (K > 32) return fail(c, CG_ERR_UNSUPPORTED, "at most 32 beams");
-  if (B > 65535 || L > 32767 || dims[1] > 65535) return fail(c, CG_ERR_UNSUPPORTED, "too many groups, layers or heads");
+  if (B > 65535 || L > 1ll << 24 || dims[1] > 65535) return fail(c, CG_ERR_UNSUPPORTED, "too many groups, layers or heads");
   if (overlap_any({parents, lens, own}, {table, k_pages, v_pages})) return fail(c, CG_ERR_INVALID, "what is written overlaps an input or each other");
   if (B == 0 || K == 0 || table->dims[1] == 0 || L == 0) return CG_OK;
   a.parents = (const uint32_t*)parents->data();
@@ -487,14 +487,15 @@ int32_t cg_paged_reorder(cg_ctx* c, const cg_tensor* parents, const cg_tensor* l
   a.nkv = (int)dims[1];
   a.token_bytes = (int)(dims[3] * k_pages->esize());
   a.layer_bytes = dims[0] * dims[1] * dims[2] * a.token_bytes;
+  a.pools = (int)(2 * L);
   a.err = c->core->dev_err;
   written(table);
   written(k_pages);
   written(v_pages);
-  if (K <= 4) return launch_reorder<4>(c, a, B, L);
-  if (K <= 8) return launch_reorder<8>(c, a, B, L);
-  if (K <= 16) return launch_reorder<16>(c, a, B, L);
-  return launch_reorder<32>(c, a, B, L);
+  if (K <= 4) return launch_reorder<4>(c, a, B);
+  if (K <= 8) return launch_reorder<8>(c, a, B);
+  if (K <= 16) return launch_reorder<16>(c, a, B);
+  return launch_reorder<32>(c, a, B);
 }
 
 }  // extern "C"
