@@ -75,28 +75,26 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
   const int64_t first = lo / KT, tiles = hi / KT + 1 - first, share = (tiles + slices - 1) / slices;
   const int64_t end = min(first + tiles, first + (slice + 1) * share);
 
-  // A lane has a page of a tile (or the whole tile, if pages are longer); pages without a visible key are not looked up and read
-  // as zeros (a box behind the pool's end).
+  // A lane has a box of a tile: 64 components of a page's keys or values (of the whole tile's, if pages are longer).  Pages without a
+  // visible key are not looked up and read as zeros (a box behind the pool's end).
   const int lg = p.rows.lg, box = min(1 << lg, KT), parts = KT / box;
+  const int my_part = lane % parts, my_sub = lane / parts % SUB, my_pool = lane / (parts * SUB);  // (keys, values; others have nothing)
   const int off_end = (int)p.pool_rows;
   auto place = [&](int64_t t) {
-    const int64_t key = t * KT + lane * box;
-    if (lane >= parts || key > hi || key + box <= lo) return off_end;
+    const int64_t key = t * KT + my_part * box;
+    if (key > hi || key + box <= lo) return off_end;
     const int64_t id = page_of(p.rows, row, key);
     return id < 0 ? off_end : (int)(((id * p.nkv + kvh) << lg) + (key & ((1 << lg) - 1)));
   };
   auto request = [&](int stage, int at) {
-    const uint32_t bar = bars + 8 * stage, to = ring + stage * (2 * TILE) + lane * box * 128;
+    const uint32_t bar = bars + 8 * stage;
     if (lane == 0) mbar_expect_tx(bar, 2 * TILE);
     __syncwarp();
-    if (lane < parts) {
-#pragma unroll
-      for (int s = 0; s < SUB; ++s) tma_load_2d(to + s * BOX, &map_k, s * 64, at, bar);
-#pragma unroll
-      for (int s = 0; s < SUB; ++s) tma_load_2d(to + TILE + s * BOX, &map_v, s * 64, at, bar);
-    }
+    if (my_pool < 2)
+      tma_load_2d(ring + stage * (2 * TILE) + my_pool * TILE + my_sub * BOX + my_part * box * 128, my_pool ? &map_v : &map_k, my_sub * 64, at, bar);
   };
   int64_t t = first + slice * share + warp;
+  int ahead_at = off_end;  // place of the tile that is asked for next
   {
     int at[RING];
 #pragma unroll
@@ -104,6 +102,7 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
 #pragma unroll
     for (int i = 0; i < RING; ++i)
       if (t + 4 * i < end) request(i, at[i]);
+    if (t + 4 * RING < end) ahead_at = place(t + 4 * RING);
   }
 
   // rows g and g + 8 of the tile
@@ -137,7 +136,7 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
   for (; t < end; t += 4, ++it) {
     const int stage = it % RING;
     const int64_t ahead = t + 4 * RING;
-    const int next = ahead < end ? place(ahead) : off_end;
+    const int next = ahead + 4 < end ? place(ahead + 4) : off_end;  // (a whole round before it is asked for)
     ok = __all_sync(0xffffffffu, mbar_wait(bars + 8 * stage, (uint32_t)(it / RING) & 1u, &aborted, p.rows.err));
     if (!ok) break;
     const uint32_t kt = ring + stage * (2 * TILE), vt = kt + TILE;
@@ -151,9 +150,9 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
       }
       __syncwarp();
     }
-    float s[KT / 8][4];
+    float s[KT / 8][4], s2[KT / 8][4];  // (even and odd 16 components: two shorter chains)
 #pragma unroll
-    for (int i = 0; i < KT / 8; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+    for (int i = 0; i < KT / 8; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = s2[i][0] = s2[i][1] = s2[i][2] = s2[i][3] = 0.f;
 #pragma unroll
     for (int k = 0; k < KS; ++k)
 #pragma unroll
@@ -161,9 +160,14 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
         const int key = i * 16 + lkey, piece = (k * 2 + lpiece) & 7;
         uint32_t b0, b1, b2, b3;
         ldsm_x4(kt + (k / 4) * BOX + key * 128 + ((piece ^ (key & 7)) << 4), b0, b1, b2, b3);
-        mma_bf16(s[2 * i], qf[k][0], NB == 2 ? qf[k][1] : 0u, qf[k][NB], NB == 2 ? qf[k][NB + 1] : 0u, b0, b1);
-        mma_bf16(s[2 * i + 1], qf[k][0], NB == 2 ? qf[k][1] : 0u, qf[k][NB], NB == 2 ? qf[k][NB + 1] : 0u, b2, b3);
+        float (*to)[4] = k & 1 ? s2 : s;
+        mma_bf16(to[2 * i], qf[k][0], NB == 2 ? qf[k][1] : 0u, qf[k][NB], NB == 2 ? qf[k][NB + 1] : 0u, b0, b1);
+        mma_bf16(to[2 * i + 1], qf[k][0], NB == 2 ? qf[k][1] : 0u, qf[k][NB], NB == 2 ? qf[k][NB + 1] : 0u, b2, b3);
       }
+#pragma unroll
+    for (int i = 0; i < KT / 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 2 * NB; ++e) s[i][e] += s2[i][e];
     const bool masked = k0 + KT - 1 > pos0 + i0 || (p.window > 0 && k0 <= hi - p.window);
     float top[NB];
 #pragma unroll
@@ -228,7 +232,8 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
         }
       }
     __syncwarp();
-    if (ahead < end) request(stage, next);
+    if (ahead < end) request(stage, ahead_at);
+    ahead_at = next;
   }
   if (!ok) {  // copies on their way are waited for: what lies over the ring is written next
     for (int i = 0; i < RING && t + 4 * i < end; ++i) mbar_drain(bars + 8 * ((it + i) % RING), (uint32_t)((it + i) / RING) & 1u, p.rows.err);
@@ -306,6 +311,32 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
   cluster_sync_all();
 }
 
+// clusters of this many blocks that run at a time (asked once)
+template <int D, int ROWS, bool CAP>
+int at_a_time(int device, int slices) {
+  static int known[64][17];
+  int& n = known[device & 63][slices];
+  if (n == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1024, 1, (unsigned)slices);
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = dec_smem<D>();
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = (unsigned)slices;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int got = 0;
+    if (cudaOccupancyMaxActiveClusters(&got, k_paged_dec<D, ROWS, CAP>, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      got = 0;
+    }
+    n = got > 0 ? got : -1;
+  }
+  return n;
+}
+
 template <int D, int ROWS, bool CAP>
 int launch(cg_ctx* c, const PagedAttnArgs& a) {
   constexpr size_t smem = dec_smem<D>();
@@ -313,6 +344,7 @@ int launch(cg_ctx* c, const PagedAttnArgs& a) {
   bool& configured = configured_on.at(c->core->device);
   if (!configured) {
     CG_CUDA(c, cudaFuncSetAttribute(k_paged_dec<D, ROWS, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    CG_CUDA(c, cudaFuncSetAttribute(k_paged_dec<D, ROWS, CAP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     configured = true;
   }
   DecArgs p;
@@ -335,9 +367,29 @@ int launch(cg_ctx* c, const PagedAttnArgs& a) {
   CG_TRY(make_map(c, &mk, a.k_pages, p.pool_rows, a.d, a.d, box));
   CG_TRY(make_map(c, &mv, a.v_pages, p.pool_rows, a.d, a.d, box));
   const int64_t groups = (a.most * p.rep + ROWS - 1) / ROWS * a.nkv, longest = a.rows.cols << a.rows.lg;
-  // Shares of the keys: until two blocks per SM have work, but no shares of less than a tile per warp.
+  // Shares of the keys.  A block takes 4 us and 0.7 to 1.25 per round of its warps, joining 2 to 4.5; clusters that do not run at the same
+  // time take turns (between whole turns and their mean, as rows differ).  Us with 1 / 2 / 4 / 8 / 16 shares, [the rule's]:
+  //   8 rows x 8 key heads, 578 keys, d 64      8.7   8.2 [7.4]  13.5  37
+  //   8 x 8, 2000, d 128                       29.4  19.7 [16.8] 23.8  48
+  //   1 x 8, 4096, d 128                       52.2  29.9  18.0  12.5 [11.5]
+  //   1 x 8, 32000, d 128                      394   200   104   57.6 [38.3]
+  //   32 x 8, 530, d 128                      [16.2] 23.7  34.0  59.9  147
+  //   4 x 4, 2080, d 256                       44.8  26.5 [17.2] 24.0  31.8
+  //   12 x 4, 167, d 256                       [8.4]  8.6  14.3  29.2  59
+  const int64_t clusters = groups * a.rows.rows, tiles = longest / dec_keys<D>() + 1;
+  constexpr double join[5] = {0., 2., 2., 2.5, 4.5}, round = D == 64 ? 0.7 : D == 128 ? 0.75 : 1.25;
   int slices = 1;
-  while (slices < 8 && groups * a.rows.rows * slices * (longest > 4096 ? 1 : 2) <= 2 * 148 && (int64_t)slices * 4 * dec_keys<D>() < longest) slices *= 2;
+  double best = 1e300;
+  for (int i = 0; i < 5; ++i) {
+    const int n = at_a_time<D, ROWS, CAP>(c->core->device, 1 << i);
+    if (n <= 0) continue;
+    const double turns = std::max(1., 0.5 * ((double)((clusters + n - 1) / n) + (double)clusters / n));
+    const double cost = turns * (4. + join[i] + round * (double)((tiles + (4 << i) - 1) / (4 << i)));
+    if (cost < best) {
+      best = cost;
+      slices = 1 << i;
+    }
+  }
   CG_CUDA(c, launch_kernel(c, k_paged_dec<D, ROWS, CAP>, dim3((unsigned)groups, (unsigned)a.rows.rows, (unsigned)slices), dim3(128), smem, slices, mk, mv, p));
   CG_LAUNCHED(c);
   return CG_OK;
