@@ -25,46 +25,58 @@ __device__ __forceinline__ void store_as(__nv_bfloat16* p, float x) { *p = __flo
 __device__ __forceinline__ float load_as(const float* p) { return *p; }
 __device__ __forceinline__ float load_as(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
-// two f32 at a time
-__device__ __forceinline__ void fma2(uint64_t& c, uint64_t a, uint64_t b) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b)); }
-__device__ __forceinline__ void mul2(uint64_t& c, uint64_t a) { asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(c) : "l"(a)); }
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
-  return v;
+// 19 leading bits of an f32 and what they leave, as operands of the tensor cores' tf32 products
+__device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
+  hi = __float_as_uint(x) & 0xffffe000u;
+  lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
 }
-__device__ __forceinline__ float2 both(uint64_t v) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-  return f;
+__device__ __forceinline__ void mma_tf32(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// f32, and whatever the tensor-core kernels do not take, on the CUDA cores.  A block has QR queries of one row and key head (query x
-// is token x / rep, head x % rep of the group) and a share of the visible keys, 32 at a time; the blocks of a cluster share the
-// keys and are joined through shared memory.  Eight lanes have a query row (or four rows): a score is a key's, an output value
-// four neighbouring columns', so that for a thread's 4 x 4 products eight vectors are read; two products are
-// one instruction, and probabilities lie in shared memory twice for that.  f32 keys and values come by
-// asynchronous copies, a ring of tiles ahead, their places looked up a tile before that.  D: head size, rounded up to 64,
-// 128 or 256.
-constexpr int GK = 32;  // keys of a tile
-template <typename T, int D>
-__host__ __device__ constexpr int any_ring() { return sizeof(T) == 2 ? 1 : D == 256 ? 2 : 3; }
+// f32, and bf16 that the other kernels do not take (its values are widened on the way in).  Operands are split into two parts of
+// 11 bits, and three of the four products are summed in f32: what is left out is 2^-22 of a product, less than f32 sums of as
+// many terms are off by.  On the CUDA cores the same tiles are bound by shared memory, four or eight vectors for 16
+// products a thread: 7200 cycles for 64 queries and 32 keys of 64, against about 2000 here.
+//
+// A block has QR queries of one row and key head (query x is token x / rep, head x % rep of the group) and a share of the visible
+// keys, GK at a time; its four warps share the rows (QR = 64) or the keys (QR = 16) of a tile, 16 rows each.  The blocks of a
+// cluster share the keys and are joined through shared memory.  Tiles come by asynchronous copies, a ring of them ahead, their pages
+// asked for before that.  Components, and columns, are dealt to the fragments so that a lane reads 16 bytes at a time and has eight
+// neighbouring output values.  D: head size, rounded up to 64, 128 or 256.
+template <int D, int QR>
+struct Shape {
+  static constexpr int GK = QR == 64 ? (D == 256 ? 16 : 32) : (D == 64 ? 128 : D == 128 ? 64 : 32);
+  static constexpr int LK = D + 16, LV = D + 4;  // rows of keys (and queries), of values: conflict-free reads
+  static constexpr int STAGE = GK * (LK + LV);   // floats of a tile
+};
+template <typename T>
+constexpr int any_ring() { return sizeof(T) == 2 ? 1 : 2; }
 template <typename T, int D, int QR>
-__host__ __device__ constexpr size_t any_smem() { return (size_t)((QR + 2 * any_ring<T, D>() * GK) * (D + 4) + 2 * QR * (GK + 1)) * 4; }
+constexpr size_t any_smem() {
+  using S = Shape<D, QR>;
+  const size_t ring = (size_t)any_ring<T>() * S::STAGE, joined = (size_t)(QR == 64 ? 64 : 80) * S::LV;
+  return ((size_t)2 * QR * S::LK + (ring > joined ? ring : joined)) * 4;
+}
 template <typename T, int D, int QR>
 __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
-  constexpr int LD = D + 4, RING = any_ring<T, D>();
-  constexpr int RT = QR / 16;      // query rows of a thread
-  constexpr int CT = D / 32;       // groups of four output columns of a thread
+  using S = Shape<D, QR>;
+  constexpr int GK = S::GK, LK = S::LK, LV = S::LV, RING = any_ring<T>();
+  constexpr int WK = QR == 64 ? 1 : 4, NT = GK / WK / 8;  // warps that share the keys, 8 keys of a warp
+  constexpr int DG = D / 32;                             // 32 columns of the output
   extern __shared__ __align__(16) float sm[];
-  float* qs = sm;                  // [QR][LD]
-  float* ring = qs + QR * LD;      // [RING] keys [GK][LD], values [GK][LD]
-  uint64_t* ps = (uint64_t*)(ring + RING * 2 * GK * LD);  // [QR][GK + 1]: each probability twice
-  __shared__ float ml[2][QR];
-  __shared__ int64_t places[2][GK];  // of the keys of the next tile to be asked for; -1: zeros
+  float* qh = sm;                       // [QR][LK] upper and
+  float* ql = qh + QR * LK;             // lower parts of the queries
+  float* ring = ql + QR * LK;           // [RING] keys [GK][LK], values [GK][LV]
+  float* part = ring;                   // behind the loop: the warps' outputs [4][16][LV] and, with WK = 4, the block's [16][LV]
+  __shared__ float red[2][64], ml[2][QR];
+  __shared__ int64_t places[2][GK];     // of the keys of the next tile to be asked for; -1: zeros
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int tid = threadIdx.x, ty = tid >> 3, tx = tid & 7;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int rep = a.nh / a.nkv, kvh = (int)blockIdx.x % a.nkv;
   const int64_t row = blockIdx.y, x0 = (int64_t)(blockIdx.x / a.nkv) * QR;
   const int slices = (int)gridDim.z, slice = (int)blockIdx.z;
@@ -75,18 +87,22 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
   const int64_t first = lo / GK, tiles = hi / GK + 1 - first, per = (tiles + slices - 1) / slices;
   const int64_t t0 = first + slice * per, t1 = min(first + tiles, t0 + per);
   const int64_t page_mask = ((int64_t)1 << a.rows.lg) - 1;
-  auto look_up = [&](int64_t t) {  // by the first warp
+  // By the first GK threads: the page of a key of tile t, asked for early and written down late.
+  auto ask = [&](int64_t t) {
     const int64_t key = t * GK + tid;
-    int64_t at = -1;
-    if (t < t1 && key >= lo && key <= hi) {
-      const int64_t page = page_of(a.rows, row, key);
-      if (page >= 0) at = (((page * a.nkv + kvh) << a.rows.lg) + (key & page_mask)) * a.d;
+    const bool seen = tid < GK && t < t1 && key >= lo && key <= hi;
+    return seen ? (int64_t)a.rows.table[row * a.rows.cols + (key >> a.rows.lg)] : -1;
+  };
+  auto note = [&](int64_t t, int64_t page) {
+    if (page >= a.rows.n_pages) {
+      *a.rows.err = DEV_INDEX;
+      page = -1;
     }
-    places[t & 1][tid] = at;
+    if (tid < GK) places[t & 1][tid] = page < 0 ? -1 : (((page * a.nkv + kvh) << a.rows.lg) + ((t * GK + tid) & page_mask)) * a.d;
   };
   auto request = [&](int64_t t) {
-    float* ks = ring + (int)((t - t0) % RING) * 2 * GK * LD;
-    float* vs = ks + GK * LD;
+    float* ks = ring + (int)((t - t0) % RING) * S::STAGE;
+    float* vs = ks + GK * LK;
     if constexpr (sizeof(T) == 4) {
       if (t < t1)
         for (int i = tid; i < GK * (D / 4); i += 128) {
@@ -95,8 +111,8 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
           const bool there = at >= 0 && c < a.d;
           const float* k = (const float*)a.k_pages + (there ? at + c : 0);
           const float* v = (const float*)a.v_pages + (there ? at + c : 0);
-          cp_async16((uint32_t)__cvta_generic_to_shared(ks + r * LD + c), k, there ? 16 : 0);
-          cp_async16((uint32_t)__cvta_generic_to_shared(vs + r * LD + c), v, there ? 16 : 0);
+          cp_async16((uint32_t)__cvta_generic_to_shared(ks + r * LK + c), k, there ? 16 : 0);
+          cp_async16((uint32_t)__cvta_generic_to_shared(vs + r * LV + c), v, there ? 16 : 0);
         }
       cp_async_commit();
     } else {
@@ -110,21 +126,20 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          ks[r * LD + c + e] = kx[e];
-          vs[r * LD + c + e] = vx[e];
+          ks[r * LK + c + e] = kx[e];
+          vs[r * LV + c + e] = vx[e];
         }
       }
     }
   };
-  if (tid < GK) look_up(t0);
+  note(t0, ask(t0));
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < RING - 1; ++i) {  // (two tiles' places take turns)
     request(t0 + i);
-    if (tid < GK) look_up(t0 + i + 1);
+    note(t0 + i + 1, ask(t0 + i + 1));
     __syncthreads();
   }
-
   for (int i = tid; i < QR * (D / 8); i += 128) {
     const int r = i / (D / 8), c = i % (D / 8) * 8;
     const int64_t x = x0 + r;
@@ -135,133 +150,179 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
       for (int e = 0; e < 8; ++e) v[e] = load_as(p + e);
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) qs[r * LD + c + e] = v[e];
+    for (int e = 0; e < 8; ++e) {
+      uint32_t h, l;
+      split(v[e], h, l);
+      qh[r * LK + c + e] = __uint_as_float(h);
+      ql[r * LK + c + e] = __uint_as_float(l);
+    }
   }
-  float m[RT], l[RT];
-  uint64_t o[RT][CT][2];
+  // this lane's rows g and g + 8 of the warp's 16
+  const int r0 = (QR == 64 ? warp * 16 : 0) + g, key0 = QR == 64 ? 0 : warp * (GK / 4);
+  const int64_t qpos[2] = {pos0 + (x0 + r0) / rep, pos0 + (x0 + r0 + 8) / rep};
+  const float scale = a.scale * 1.4426950408889634f, cap2 = a.cap * 1.4426950408889634f, cap_unit = a.cap > 0.f ? -2.f * scale / a.cap : 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[DG][4][4];
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    m[r] = -INFINITY;
-    l[r] = 0.f;
+  for (int c = 0; c < DG; ++c)
 #pragma unroll
-    for (int c = 0; c < CT; ++c) o[r][c][0] = o[r][c][1] = 0;
-  }
+    for (int i = 0; i < 4; ++i) o[c][i][0] = o[c][i][1] = o[c][i][2] = o[c][i][3] = 0.f;
   for (int64_t t = t0; t < t1; ++t) {
+    int64_t page;
     if constexpr (RING > 1) {
       cp_async_wait_group<RING - 2>();
       __syncthreads();  // tile t is there, and everyone is done with the one before
       request(t + RING - 1);
-      if (tid < GK) look_up(t + RING);
+      page = ask(t + RING);
     } else {
       __syncthreads();
       request(t);
       __syncthreads();
-      if (tid < GK) look_up(t + 1);
+      page = ask(t + 1);
     }
-    const float* ks = ring + (int)((t - t0) % RING) * 2 * GK * LD;
-    const float* vs = ks + GK * LD;
-    uint64_t s2[RT][4];
+    const float* ks = ring + (int)((t - t0) % RING) * S::STAGE;
+    const float* vs = ks + GK * LK;
+    ks += key0 * LK;
+    vs += key0 * LV;
+    const int64_t k0 = t * GK + key0;
+    float s[NT][4];
 #pragma unroll
-    for (int r = 0; r < RT; ++r) s2[r][0] = s2[r][1] = s2[r][2] = s2[r][3] = 0;
-#pragma unroll 4
-    for (int c = 0; c < D; c += 4) {
-      ulonglong2 kk[4];
+    for (int i = 0; i < NT; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+#pragma unroll 2
+    for (int c = 0; c < D; c += 16) {  // components c + 4 t4 .. + 3: places t4 and t4 + 4 of two products
+      uint32_t ah[2][4], al[2][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) kk[j] = *(const ulonglong2*)(ks + (tx + 8 * j) * LD + c);
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        const ulonglong2 qq = *(const ulonglong2*)(qs + (ty * RT + r) * LD + c);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) fma2(s2[r][j], qq.x, kk[j].x);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) fma2(s2[r][j], qq.y, kk[j].y);
-      }
-    }
-    const bool masked = t * GK + GK - 1 > pos0 + i0 || (a.window > 0 && t * GK <= hi - a.window);
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const int64_t pos = masked ? pos0 + (x0 + ty * RT + r) / rep : 0;
-      float top = -INFINITY, s[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t key = t * GK + tx + 8 * j;
-        const float2 f = both(s2[r][j]);
-        float x = (f.x + f.y) * a.scale;
-        if (a.cap > 0.f) x = a.cap * tanhf(x / a.cap);
-        if (masked && !(key <= pos && (a.window <= 0 || key > pos - a.window))) x = -INFINITY;
-        s[j] = x;
-        top = fmaxf(top, x);
+      for (int q = 0; q < 2; ++q) {
+        const uint4 h = *(const uint4*)(qh + (r0 + 8 * q) * LK + c + 4 * t4), w = *(const uint4*)(ql + (r0 + 8 * q) * LK + c + 4 * t4);
+        ah[0][q] = h.x; ah[0][2 + q] = h.y; ah[1][q] = h.z; ah[1][2 + q] = h.w;
+        al[0][q] = w.x; al[0][2 + q] = w.y; al[1][q] = w.z; al[1][2 + q] = w.w;
       }
 #pragma unroll
-      for (int w = 4; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-      const float m_new = fmaxf(m[r], top), base = m_new == -INFINITY ? 0.f : m_new;
-      const float corr = expf(m[r] - base);
-      float sum = 0.f;
+      for (int i = 0; i < NT; ++i) {
+        const float4 k = *(const float4*)(ks + (i * 8 + g) * LK + c + 4 * t4);
+        uint32_t h[4], w[4];
+        split(k.x, h[0], w[0]); split(k.y, h[1], w[1]); split(k.z, h[2], w[2]); split(k.w, h[3], w[3]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float e = expf(s[j] - base);
-        sum += e;
-        ps[(ty * RT + r) * (GK + 1) + tx + 8 * j] = pair(e, e);
-      }
-      l[r] = l[r] * corr + sum;  // (of this lane's keys)
-      m[r] = m_new;
-      if (corr != 1.f)
-#pragma unroll
-        for (int c = 0; c < CT; ++c) {
-          mul2(o[r][c][0], pair(corr, corr));
-          mul2(o[r][c][1], pair(corr, corr));
-        }
-    }
-    __syncwarp();
-#pragma unroll 4
-    for (int k = 0; k < GK; ++k) {
-      uint64_t p[RT];
-#pragma unroll
-      for (int r = 0; r < RT; ++r) p[r] = ps[(ty * RT + r) * (GK + 1) + k];
-#pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        const ulonglong2 v = *(const ulonglong2*)(vs + k * LD + tx * 4 + c * 32);
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          fma2(o[r][c][0], p[r], v.x);
-          fma2(o[r][c][1], p[r], v.y);
+        for (int u = 0; u < 2; ++u) {
+          mma_tf32(s[i], al[u], h[2 * u], h[2 * u + 1]);
+          mma_tf32(s[i], ah[u], w[2 * u], w[2 * u + 1]);
+          mma_tf32(s[i], ah[u], h[2 * u], h[2 * u + 1]);
         }
       }
     }
-    __syncwarp();
+    // (scores and maxima in units of log2)
+    const bool masked = k0 + GK / WK - 1 > pos0 + i0 || k0 < lo || (a.window > 0 && k0 <= hi - a.window);
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float x = s[i][e];
+        if (a.cap > 0.f) x = fmaf(2.f * cap2, rcp_newton(1.f + fast_exp2(x * cap_unit)), -cap2);
+        else x *= scale;
+        const int64_t key = k0 + i * 8 + 2 * t4 + (e & 1), pos = qpos[e >> 1];
+        if (masked && (key > pos || (a.window > 0 && key <= pos - a.window))) x = -INFINITY;
+        s[i][e] = x;
+        top[e >> 1] = fmaxf(top[e >> 1], x);
+      }
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      top[q] = fmaxf(top[q], __shfl_xor_sync(0xffffffffu, top[q], 1));
+      top[q] = fmaxf(top[q], __shfl_xor_sync(0xffffffffu, top[q], 2));
+      top[q] = fmaxf(top[q], m[q]);
+    }
+    if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
+      const float f0 = top[0] == -INFINITY ? 1.f : fast_exp2(m[0] - top[0]), f1 = top[1] == -INFINITY ? 1.f : fast_exp2(m[1] - top[1]);
+      m[0] = top[0];
+      m[1] = top[1];
+      l[0] *= f0;
+      l[1] *= f1;
+#pragma unroll
+      for (int c = 0; c < DG; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          o[c][i][0] *= f0; o[c][i][1] *= f0;
+          o[c][i][2] *= f1; o[c][i][3] *= f1;
+        }
+    }
+    const float base[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      // probabilities of 8 keys as they lie are the left operand whose places t4 and t4 + 4 are keys 2 t4 and 2 t4 + 1
+      uint32_t ph[4], pl[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = fast_exp2(s[i][e] - base[e >> 1]);
+        l[e >> 1] += x;
+        split(x, ph[(e & 1) * 2 + (e >> 1)], pl[(e & 1) * 2 + (e >> 1)]);
+      }
+#pragma unroll
+      for (int c = 0; c < DG; ++c) {  // columns 32 c + 4 g + j are place g of product j
+        const float4 v0 = *(const float4*)(vs + (i * 8 + 2 * t4) * LV + 32 * c + 4 * g), v1 = *(const float4*)(vs + (i * 8 + 2 * t4 + 1) * LV + 32 * c + 4 * g);
+        const float b0[4] = {v0.x, v0.y, v0.z, v0.w}, b1[4] = {v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t h0, w0, h1, w1;
+          split(b0[j], h0, w0);
+          split(b1[j], h1, w1);
+          mma_tf32(o[c][j], pl, h0, h1);
+          mma_tf32(o[c][j], ph, w0, w1);
+          mma_tf32(o[c][j], ph, h0, h1);
+        }
+      }
+    }
+    note(t + RING, page);
   }
   if constexpr (RING > 1) cp_async_wait_group<0>();
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int w = 4; w; w >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], w);
-  auto values = [&](int r, int c, float f) {
-    const float2 u = both(o[r][c][0]), w = both(o[r][c][1]);
-    return make_float4(u.x * f, u.y * f, w.x * f, w.y * f);
-  };
-  auto put4 = [&](int64_t x, int col, float4 v) {
-    if (x >= n * rep || col >= a.d) return;
-    T* to = (T*)a.out + ((tok0 + x / rep) * a.nh + kvh * rep + x % rep) * a.d + col;
-    store_as(to, v.x); store_as(to + 1, v.y); store_as(to + 2, v.z); store_as(to + 3, v.w);
-  };
-  if (slices == 1) {
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const float f = l[r] > 0.f ? 1.f / l[r] : 0.f;
-#pragma unroll
-      for (int c = 0; c < CT; ++c) put4(x0 + ty * RT + r, tx * 4 + c * 32, values(r, c, f));
-    }
-    return;
+  for (int q = 0; q < 2; ++q) {
+    l[q] += __shfl_xor_sync(0xffffffffu, l[q], 1);
+    l[q] += __shfl_xor_sync(0xffffffffu, l[q], 2);
+    if (t4 == 0) { red[0][warp * 16 + g + 8 * q] = m[q]; red[1][warp * 16 + g + 8 * q] = l[q]; }
   }
-  // the shares are joined: a block has some of the values
+  __syncthreads();  // (nobody reads the ring any more)
+#pragma unroll
+  for (int c = 0; c < DG; ++c)
+#pragma unroll
+    for (int q = 0; q < 2; ++q)  // columns 32 c + 8 t4 .. + 7
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        *(float4*)(part + (warp * 16 + g + 8 * q) * LV + 32 * c + 8 * t4 + 4 * e) = make_float4(o[c][0][2 * q + e], o[c][1][2 * q + e], o[c][2][2 * q + e], o[c][3][2 * q + e]);
   __syncthreads();
+  auto put4 = [&](int x, int col, float4 v, float f) {
+    if (x0 + x >= n * rep || col >= a.d) return;
+    T* to = (T*)a.out + ((tok0 + (x0 + x) / rep) * a.nh + kvh * rep + (x0 + x) % rep) * a.d + col;
+    store_as(to, v.x * f); store_as(to + 1, v.y * f); store_as(to + 2, v.z * f); store_as(to + 3, v.w * f);
+  };
+  const float* joined = QR == 64 ? part : part + 64 * LV;
+  if (QR == 16 || slices == 1)
+    for (int i = tid; i < QR * (D / 4); i += 128) {
+      const int x = i / (D / 4), c = i % (D / 4) * 4;
+      float top = red[0][x], sum = red[1][x];
+      float4 v = *(const float4*)(part + x * LV + c);
+      if (QR == 16) {  // the warps' shares of the keys
+        top = fmaxf(fmaxf(red[0][x], red[0][16 + x]), fmaxf(red[0][32 + x], red[0][48 + x]));
+        const float at = top == -INFINITY ? 0.f : top;
+        sum = 0.f;
+        v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const int x = ty * RT + r;
-    if (tx == 0) { ml[0][x] = m[r]; ml[1][x] = l[r]; }
-#pragma unroll
-    for (int c = 0; c < CT; ++c) *(float4*)(qs + x * LD + tx * 4 + c * 32) = values(r, c, 1.f);
-  }
+        for (int w = 0; w < 4; ++w) {
+          const float f = fast_exp2(red[0][w * 16 + x] - at);
+          const float4 u = *(const float4*)(part + (w * 16 + x) * LV + c);
+          sum = fmaf(red[1][w * 16 + x], f, sum);
+          v.x = fmaf(u.x, f, v.x); v.y = fmaf(u.y, f, v.y); v.z = fmaf(u.z, f, v.z); v.w = fmaf(u.w, f, v.w);
+        }
+      }
+      if (slices == 1) {
+        put4(x, c, v, sum > 0.f ? 1.f / sum : 0.f);
+      } else {
+        *(float4*)(part + (64 + x) * LV + c) = v;
+        if (c == 0) { ml[0][x] = top; ml[1][x] = sum; }
+      }
+    }
+  if (slices == 1) return;
+  if (QR == 64 && tid < QR) { ml[0][tid] = red[0][tid]; ml[1][tid] = red[1][tid]; }
+
+  // the blocks' shares: a block has some of the values
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   auto remote = [](const float* p, int rank) {
     uint32_t at;
@@ -281,7 +342,7 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
       if (s < slices) {
         asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(ms[s]) : "r"(remote(&ml[0][x], s)) : "memory");
         asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(ls[s]) : "r"(remote(&ml[1][x], s)) : "memory");
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(os[s].x), "=f"(os[s].y), "=f"(os[s].z), "=f"(os[s].w) : "r"(remote(qs + x * LD + c, s)) : "memory");
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(os[s].x), "=f"(os[s].y), "=f"(os[s].z), "=f"(os[s].w) : "r"(remote(joined + x * LV + c, s)) : "memory");
       }
     }
     float top = ms[0];
@@ -292,12 +353,11 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
-      const float f = expf(ms[s] - base);
+      const float f = fast_exp2(ms[s] - base);
       sum = fmaf(ls[s], f, sum);
       v.x = fmaf(os[s].x, f, v.x); v.y = fmaf(os[s].y, f, v.y); v.z = fmaf(os[s].z, f, v.z); v.w = fmaf(os[s].w, f, v.w);
     }
-    const float f = sum > 0.f ? 1.f / sum : 0.f;
-    put4(x0 + x, c, make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
+    put4(x, c, v, sum > 0.f ? 1.f / sum : 0.f);
   }
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -313,9 +373,15 @@ int launch_any(cg_ctx* c, const PagedAttnArgs& a) {
   }
   const int64_t tiles = (a.most * (a.nh / a.nkv) + QR - 1) / QR * a.nkv, longest = a.rows.cols << a.rows.lg;
   if (tiles > 0x7FFFFFFFll) return fail(c, CG_ERR_UNSUPPORTED, "too many tokens");
-  // Blocks that share the keys: until there are two per SM, but no shares of less than two tiles.
-  int slices = 1;
-  while (slices < 8 && tiles * a.rows.rows * slices < 148 * 2 && (int64_t)slices * 2 * GK < longest) slices *= 2;
+  // Shares of the keys.  Us in f32, heads of 64, with 1 / 2 / 4 / 8:
+  //   3 rows of 213 behind 1500, 2 x 2 heads    137  72.9  51.9  56.6
+  //   1 row of 1000                             81.9 46.4  31.2  33.3
+  //   8 single tokens of 600                    18.6 13.6  10.9  15.3
+  //   32 of 1800                                54.1 33.5  36.6  52.8
+  //   1 of 4000                                 95.7 51.3  28.4  16.6
+  static AtATime known;
+  const int slices = pick_shares([&](int i) { return at_a_time(known, c->core->device, i, k_paged_attn<T, D, QR>, 128, smem); }, 8, tiles * a.rows.rows, longest,
+                                 Shape<D, QR>::GK, 4.5, QR == 16 ? 2.8 : D == 64 ? 2.4 : D == 128 ? 4.5 : 5., true);
   CG_CUDA(c, launch_kernel(c, k_paged_attn<T, D, QR>, dim3((unsigned)tiles, (unsigned)a.rows.rows, (unsigned)slices), dim3(128), smem, slices, a));
   CG_LAUNCHED(c);
   return CG_OK;

@@ -23,4 +23,58 @@ int paged_fa(cg_ctx* c, const PagedAttnArgs& a);
 bool paged_dec_supported(const PagedAttnArgs& a);
 int paged_dec(cg_ctx* c, const PagedAttnArgs& a);
 
+// ---- into how many shares a row's keys are cut ----
+constexpr int SHARES = 5;  // 1, 2, 4, 8 or 16: the blocks of a cluster
+
+// Clusters of 1, 2, .. blocks along z that run at a time (asked once per kernel, which keeps `known`); -1: none.
+struct AtATime {
+  int n[64][SHARES] = {};
+};
+template <typename... KArgs>
+int at_a_time(AtATime& known, int device, int i, void (*kernel)(KArgs...), int threads, size_t smem) {
+  int& n = known.n[device & 63][i];
+  if (n == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1024, 1, 1u << i);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1u << i;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int got = 0;
+    if (cudaOccupancyMaxActiveClusters(&got, kernel, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      got = 0;
+    }
+    n = got > 0 ? got : -1;
+  }
+  return n;
+}
+// The shares of least time: a block takes `base` us and `round` for each of its rounds of `keys` keys, joining 2 to 4.5.  What does not run
+// at the same time takes turns: clusters beyond at_a_time (between whole turns and their mean, as rows differ), and with
+// `sm_bound`, where one block keeps an SM's units busy, blocks beyond the SMs.
+template <typename F>
+int pick_shares(F&& n_of, int most, int64_t clusters, int64_t keys_of_row, int keys, double base, double round, bool sm_bound) {
+  constexpr double join[SHARES] = {0., 2., 2., 2.5, 4.5};
+  int shares = 1;
+  double best = 1e300;
+  for (int i = 0; i < SHARES && 1 << i <= most; ++i) {
+    const int n = n_of(i);
+    if (n <= 0) continue;
+    auto turns_of = [](double x) { return 0.5 * (x + (double)(int64_t)(x + 0.999999)); };
+    double turns = turns_of((double)clusters / n);
+    if (sm_bound && (double)(clusters << i) / 148. > turns) turns = (double)(clusters << i) / 148.;
+    const int64_t tiles = keys_of_row / keys + 1;
+    const double cost = (turns > 1. ? turns : 1.) * (base + join[i] + round * (double)((tiles + (1 << i) - 1) >> i));
+    if (cost < best) {
+      best = cost;
+      shares = 1 << i;
+    }
+  }
+  return shares;
+}
+
 }  // namespace cg

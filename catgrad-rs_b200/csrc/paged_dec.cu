@@ -311,32 +311,6 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
   cluster_sync_all();
 }
 
-// clusters of this many blocks that run at a time (asked once)
-template <int D, int ROWS, bool CAP>
-int at_a_time(int device, int slices) {
-  static int known[64][17];
-  int& n = known[device & 63][slices];
-  if (n == 0) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(1024, 1, (unsigned)slices);
-    cfg.blockDim = dim3(128);
-    cfg.dynamicSmemBytes = dec_smem<D>();
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = attr.val.clusterDim.y = 1;
-    attr.val.clusterDim.z = (unsigned)slices;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    int got = 0;
-    if (cudaOccupancyMaxActiveClusters(&got, k_paged_dec<D, ROWS, CAP>, &cfg) != cudaSuccess) {
-      cudaGetLastError();
-      got = 0;
-    }
-    n = got > 0 ? got : -1;
-  }
-  return n;
-}
-
 template <int D, int ROWS, bool CAP>
 int launch(cg_ctx* c, const PagedAttnArgs& a) {
   constexpr size_t smem = dec_smem<D>();
@@ -367,8 +341,7 @@ int launch(cg_ctx* c, const PagedAttnArgs& a) {
   CG_TRY(make_map(c, &mk, a.k_pages, p.pool_rows, a.d, a.d, box));
   CG_TRY(make_map(c, &mv, a.v_pages, p.pool_rows, a.d, a.d, box));
   const int64_t groups = (a.most * p.rep + ROWS - 1) / ROWS * a.nkv, longest = a.rows.cols << a.rows.lg;
-  // Shares of the keys.  A block takes 4 us and 0.7 to 1.25 per round of its warps, joining 2 to 4.5; clusters that do not run at the same
-  // time take turns (between whole turns and their mean, as rows differ).  Us with 1 / 2 / 4 / 8 / 16 shares, [the rule's]:
+  // Shares of the keys.  Us with 1 / 2 / 4 / 8 / 16, [the rule's]:
   //   8 rows x 8 key heads, 578 keys, d 64      8.7   8.2 [7.4]  13.5  37
   //   8 x 8, 2000, d 128                       29.4  19.7 [16.8] 23.8  48
   //   1 x 8, 4096, d 128                       52.2  29.9  18.0  12.5 [11.5]
@@ -376,20 +349,9 @@ int launch(cg_ctx* c, const PagedAttnArgs& a) {
   //   32 x 8, 530, d 128                      [16.2] 23.7  34.0  59.9  147
   //   4 x 4, 2080, d 256                       44.8  26.5 [17.2] 24.0  31.8
   //   12 x 4, 167, d 256                       [8.4]  8.6  14.3  29.2  59
-  const int64_t clusters = groups * a.rows.rows, tiles = longest / dec_keys<D>() + 1;
-  constexpr double join[5] = {0., 2., 2., 2.5, 4.5}, round = D == 64 ? 0.7 : D == 128 ? 0.75 : 1.25;
-  int slices = 1;
-  double best = 1e300;
-  for (int i = 0; i < 5; ++i) {
-    const int n = at_a_time<D, ROWS, CAP>(c->core->device, 1 << i);
-    if (n <= 0) continue;
-    const double turns = std::max(1., 0.5 * ((double)((clusters + n - 1) / n) + (double)clusters / n));
-    const double cost = turns * (4. + join[i] + round * (double)((tiles + (4 << i) - 1) / (4 << i)));
-    if (cost < best) {
-      best = cost;
-      slices = 1 << i;
-    }
-  }
+  static AtATime known;
+  const int slices = pick_shares([&](int i) { return at_a_time(known, c->core->device, i, k_paged_dec<D, ROWS, CAP>, 128, smem); }, 16, groups * a.rows.rows, longest,
+                                 4 * dec_keys<D>(), 4., D == 64 ? 0.7 : D == 128 ? 0.75 : 1.25, false);
   CG_CUDA(c, launch_kernel(c, k_paged_dec<D, ROWS, CAP>, dim3((unsigned)groups, (unsigned)a.rows.rows, (unsigned)slices), dim3(128), smem, slices, mk, mv, p));
   CG_LAUNCHED(c);
   return CG_OK;
