@@ -381,7 +381,8 @@ int launch_any(cg_ctx* c, const PagedAttnArgs& a) {
   //   1 of 4000                                 95.7 51.3  28.4  16.6
   static AtATime known;
   const int slices = pick_shares([&](int i) { return at_a_time(known, c->core->device, i, k_paged_attn<T, D, QR>, 128, smem); }, 8, tiles * a.rows.rows, longest,
-                                 Shape<D, QR>::GK, 4.5, QR == 16 ? 2.8 : D == 64 ? 2.4 : D == 128 ? 4.5 : 5., true);
+                                 Shape<D, QR>::GK, QR == 16 ? 4.5 : 3.5, QR == 16 ? 2.8 : D == 64 ? 2.4 : D == 128 ? 4.5 : 5.,
+                                 std::max(0.5, 1. - 0.5 * (double)a.most / (double)std::max<int64_t>(longest, 1)));
   CG_CUDA(c, launch_kernel(c, k_paged_attn<T, D, QR>, dim3((unsigned)tiles, (unsigned)a.rows.rows, (unsigned)slices), dim3(128), smem, slices, a));
   CG_LAUNCHED(c);
   return CG_OK;

@@ -54,10 +54,11 @@ int at_a_time(AtATime& known, int device, int i, void (*kernel)(KArgs...), int t
   return n;
 }
 // The shares of least time: a block takes `base` us and `round` for each of its rounds of `keys` keys, joining 2 to 4.5.  What does not run
-// at the same time takes turns: clusters beyond at_a_time (between whole turns and their mean, as rows differ), and with
-// `sm_bound`, where one block keeps an SM's units busy, blocks beyond the SMs.
+// at the same time takes turns (between whole turns and their mean, as rows differ): clusters beyond at_a_time, and, where one
+// block keeps an SM's units busy, blocks beyond the SMs; part_seen is what of a row a query sees in the mean, 0 where that
+// does not count.
 template <typename F>
-int pick_shares(F&& n_of, int most, int64_t clusters, int64_t keys_of_row, int keys, double base, double round, bool sm_bound) {
+int pick_shares(F&& n_of, int most, int64_t clusters, int64_t keys_of_row, int keys, double base, double round, double part_seen) {
   constexpr double join[SHARES] = {0., 2., 2., 2.5, 4.5};
   int shares = 1;
   double best = 1e300;
@@ -66,7 +67,8 @@ int pick_shares(F&& n_of, int most, int64_t clusters, int64_t keys_of_row, int k
     if (n <= 0) continue;
     auto turns_of = [](double x) { return 0.5 * (x + (double)(int64_t)(x + 0.999999)); };
     double turns = turns_of((double)clusters / n);
-    if (sm_bound && (double)(clusters << i) / 148. > turns) turns = (double)(clusters << i) / 148.;
+    const double by_sm = turns_of((double)(clusters << i) * part_seen / 148.);
+    if (part_seen > 0. && by_sm > turns) turns = by_sm;
     const int64_t tiles = keys_of_row / keys + 1;
     const double cost = (turns > 1. ? turns : 1.) * (base + join[i] + round * (double)((tiles + (1 << i) - 1) >> i));
     if (cost < best) {

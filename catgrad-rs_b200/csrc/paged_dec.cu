@@ -351,7 +351,7 @@ int launch(cg_ctx* c, const PagedAttnArgs& a) {
   //   12 x 4, 167, d 256                       [8.4]  8.6  14.3  29.2  59
   static AtATime known;
   const int slices = pick_shares([&](int i) { return at_a_time(known, c->core->device, i, k_paged_dec<D, ROWS, CAP>, 128, smem); }, 16, groups * a.rows.rows, longest,
-                                 4 * dec_keys<D>(), 4., D == 64 ? 0.7 : D == 128 ? 0.75 : 1.25, false);
+                                 4 * dec_keys<D>(), 4., D == 64 ? 0.7 : D == 128 ? 0.75 : 1.25, 0.);
   CG_CUDA(c, launch_kernel(c, k_paged_dec<D, ROWS, CAP>, dim3((unsigned)groups, (unsigned)a.rows.rows, (unsigned)slices), dim3(128), smem, slices, mk, mv, p));
   CG_LAUNCHED(c);
   return CG_OK;
