@@ -424,6 +424,7 @@ extern "C" int32_t cg_paged_attention(cg_ctx* c, const cg_tensor* q, const cg_te
   if (max_new < 0 || window < 0 || !(softcap >= 0.f) || !(scale >= 0.f) || scale > 3e38f || softcap > 3e38f) return fail(c, CG_ERR_INVALID, "bad argument");
   if (overlap_any({q, k_pages, v_pages, table, starts, lens}, {out})) return fail(c, CG_ERR_INVALID, "out overlaps an input");
   if (M == 0 || nh == 0 || a.rows.rows == 0) return CG_OK;
+  if (k_pages->dims[0] == 0) return fail(c, CG_ERR_SHAPE, "no pages");
   a.q = q->data(); a.k_pages = k_pages->data(); a.v_pages = v_pages->data(); a.out = out->data();
   a.q_ld = q->strides[0]; a.q_hs = q->strides[1];
   a.most = max_new > 0 ? std::min(max_new, M) : M;

@@ -543,6 +543,207 @@ def test_reorder_leaves_a_bad_group_as_it_was(cuda):
         assert np.array_equal(got[mine], k[mine].astype(np.float64)), name
 
 
+# ---------------------------------------------------------------- together
+
+
+def net(rng, hidden, nh, nkv, d, vocab, layers, std=0.35):
+    """A small pre-norm attention model with norms per head; weights of about unit gain, so that choices are clear."""
+    w = lambda *s: (rng.standard_normal(s) * std / math.sqrt(s[-1] / 8)).astype(np.float32)
+    return {"embed": rng.standard_normal((vocab, hidden)).astype(np.float32), "head": w(vocab, hidden) * 4,
+            "layers": [{"qkv": w((nh + 2 * nkv) * d, hidden), "o": w(hidden, nh * d), "n": 1 + 0.1 * rng.standard_normal(hidden).astype(np.float32),
+                        "qg": 1 + 0.1 * rng.standard_normal(d).astype(np.float32), "kg": 1 + 0.1 * rng.standard_normal(d).astype(np.float32)} for _ in range(layers)]}
+
+
+def plain_logits(W, tokens, nh, nkv, d, cos, sin, window):
+    """The logits behind the last token, in 64 bits, without a cache."""
+    x = W["embed"][tokens].astype(np.float64)
+    T = len(tokens)
+    c, s = cos[:T, None].astype(np.float64), sin[:T, None].astype(np.float64)
+
+    def turn(v):
+        a, b = v[..., :d // 2], v[..., d // 2:]
+        return np.concatenate([a * c - b * s, b * c + a * s], -1)
+
+    norm = lambda v, g: v / np.sqrt((v * v).mean(-1, keepdims=True) + 1e-6) * g
+    for L in W["layers"]:
+        y = norm(x, L["n"]) @ L["qkv"].T.astype(np.float64)
+        q, k, v = (y.reshape(T, -1, d)[:, a:b] for a, b in ((0, nh), (nh, nh + nkv), (nh + nkv, nh + 2 * nkv)))
+        q, k = turn(norm(q, L["qg"])), turn(norm(k, L["kg"]))
+        o = np.stack([attention(q[t], k, v, t, 1 / math.sqrt(d), window, 0.0)[0] for t in range(T)])
+        x = x + o.reshape(T, -1) @ L["o"].T.astype(np.float64)
+    return x[-1] @ W["head"].T.astype(np.float64)
+
+
+@gpu
+@pytest.mark.parametrize("page,window", [(8, 0), (16, 9)])
+def test_beam_search_over_the_cache(cuda, page, window):
+    """Prompts of unequal length, one row each; then a step of the search selects, reorders all layers' caches at once, and
+    runs the new tokens, against a search that keeps whole sequences and no cache.  Selections are the same, and scores as close
+    as f32 layers are: 2 layers of sums of at most 128 products, 2^-24 each, far below 1e-4 of scores of some 10."""
+    import torch
+    rng = np.random.default_rng(page)
+    hidden, nh, nkv, d, vocab, layers, K, steps = 64, 4, 2, 32, 211, 2, 4, 12
+    W = net(rng, hidden, nh, nkv, d, vocab, layers)
+    prompts = [rng.integers(0, vocab, n) for n in (11, 24, 3)]
+    G, end, T = len(prompts), 7, 64
+    cos_t, sin_t = cuda.rope_tables(10000.0, T, d)
+    cos, sin = cuda.to_numpy(cos_t), cuda.to_numpy(sin_t)
+    up = lambda a: cuda.from_numpy(np.ascontiguousarray(a))
+    Wd = {"embed": up(W["embed"]), "head": up(W["head"]), "layers": [{n: up(a) for n, a in L.items()} for L in W["layers"]]}
+    cols = T // page
+    own = np.arange(G * K * cols, dtype=np.uint32).reshape(G * K, cols)[:, ::-1].copy()
+    own_d, table = put(cuda, own)[0], put(cuda, own)[0]
+    kc, vc = (torch.zeros(layers, G * K * cols, nkv, page, d, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    pools = [(cuda.from_device(kc[i]), cuda.from_device(vc[i])) for i in range(layers)]
+    whole = cuda.from_device(kc), cuda.from_device(vc)
+
+    def forward(tokens, table, new, total):
+        """[packed tokens] -> logits of every token; rows with `new` tokens each."""
+        starts, lens = put(cuda, np.concatenate([[0], np.cumsum(new)]).astype(np.uint32))[0], put(cuda, np.uint32(total))[0]
+        M = len(tokens)
+        x = cuda.index(Wd["embed"], 0, cuda.from_numpy(np.uint32(tokens)))
+        for L, (kp, vp) in zip(Wd["layers"], pools):
+            y = cuda.reshape(cuda.linear(cuda.fused_rmsnorm(x, L["n"], 1e-6), L["qkv"]), (M, nh + 2 * nkv, d))
+            q, k, v = cuda.slice(y, 1, 0, nh), cuda.slice(y, 1, nh, nkv), cuda.slice(y, 1, nh + nkv, nkv)
+            q = cuda.paged_append(k, v, kp, vp, table, starts, lens, q=q, cos=cos_t, sin=sin_t, q_gain=L["qg"], k_gain=L["kg"], eps=1e-6)
+            o = cuda.paged_attention(q, kp, vp, table, starts, lens, max_new=max(new), window=window)
+            x = cuda.add(x, cuda.linear(cuda.reshape(o, (M, nh * d)), L["o"]))
+        return cuda.linear(x, Wd["head"])
+
+    # prompts: the rows of each group's first beam
+    first = [put(cuda, own[g * K:g * K + 1])[0] for g in range(G)]
+    logits = [cuda.slice(forward(p, first[g], [len(p)], [len(p)]), 0, len(p) - 1, 1) for g, p in enumerate(prompts)]
+    x = cuda.concat(cuda.concat(logits[0], logits[1], 0), logits[2], 0)
+    scores, tokens, parents, finished = cuda.beam_select(cuda.reshape(x, (G, 1, vocab)), cuda.zeros((G, 1), 0), K, finished=cuda.zeros((G, 1), 1), end=end)
+    rows = [[(0.0, list(p), False)] for p in prompts]
+    for step in range(steps):
+        # the plain search, and the same step's selection on the device
+        for g in range(G):
+            logit = np.stack([plain_logits(W, np.array(t), nh, nkv, d, cos, sin, window) for _, t, _ in rows[g]])[None]
+            s, t, p, f = best(logit, np.array([[r[0] for r in rows[g]]]), K, np.array([[int(r[2]) for r in rows[g]]]), end)
+            assert np.array_equal(cuda.to_numpy(tokens)[g], t[0]) and np.array_equal(cuda.to_numpy(parents)[g], p[0]), (step, g)
+            assert np.array_equal(cuda.to_numpy(finished)[g], f[0].astype(np.uint32))
+            assert np.abs(cuda.to_numpy(scores)[g] - s[0]).max() < 1e-4
+            rows[g] = [(float(cuda.to_numpy(scores)[g, j]), rows[g][p[0, j]][1] + [int(t[0, j])], bool(f[0, j])) for j in range(K)]
+        total = np.repeat([len(p) + step for p in prompts], K).astype(np.uint32)
+        cuda.paged_reorder(parents, put(cuda, total)[0], own_d, table, *whole)
+        logits = forward(cuda.to_numpy(tokens).reshape(-1), table, [1] * (G * K), total + 1)
+        scores, tokens, parents, finished = cuda.beam_select(cuda.reshape(logits, (G, K, vocab)), scores, K, finished=finished, end=end)
+    cuda.sync()
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+def test_captured_steps_replay_with_new_lengths_and_tables(store):
+    """A step of each operator in a graph of its own, captured twice over the same buffers and replayed by turns while lengths, tables and
+    inputs change: the operators keep nothing between calls, and take no memory."""
+    import torch
+    dtype = torch.bfloat16 if store == "bf16" else torch.float32
+    S = torch.cuda.Stream()
+    B = cg.CudaBackend(0, cg.PREC_F32, stream=S.cuda_stream)
+    G, K, nh, nkv, d, page, cols, V = 2, 4, 4, 2, 64, 16, 6, 1000
+    R = G * K
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    rnd = lambda *s: torch.randn(s, generator=gen, device="cuda").to(dtype)
+    q, k, v, logits = rnd(R, nh, d), rnd(R, nkv, d), rnd(R, nkv, d), rnd(G, K, V)
+    kp, vp = rnd(R * cols, nkv, page, d), rnd(R * cols, nkv, page, d)
+    own = torch.randperm(R * cols, generator=gen, device="cuda").int().reshape(R, cols).contiguous()
+    table, lens, starts = own.clone(), torch.full((R,), 40, device="cuda", dtype=torch.int32), torch.arange(R + 1, device="cuda").int()
+    q_out, out, scores = torch.zeros_like(q), torch.zeros_like(q), torch.zeros(G, K, device="cuda")
+    ints = [torch.zeros(G, K, device="cuda", dtype=torch.int32) for _ in range(3)]
+    torch.cuda.synchronize()
+    h = {n: B.from_device(t) for n, t in dict(q=q, k=k, v=v, logits=logits, kp=kp, vp=vp, own=own, table=table, lens=lens, starts=starts, q_out=q_out, out=out, scores=scores).items()}
+    hi = [B.from_device(t) for t in ints]
+
+    def step():
+        B.paged_append(h["k"], h["v"], h["kp"], h["vp"], h["table"], h["starts"], h["lens"], q=h["q"], q_out=h["q_out"])
+        B.paged_attention(h["q_out"], h["kp"], h["vp"], h["table"], h["starts"], h["lens"], max_new=1, out=h["out"])
+        B.beam_select(h["logits"], h["scores"], K, finished=hi[2], end=3, out=(h["scores"], *hi))
+        B.paged_reorder(hi[1], h["lens"], h["own"], h["table"], h["kp"], h["vp"])
+
+    everything = (kp, vp, table, q_out, out, scores, *ints)
+    with torch.cuda.stream(S):
+        step()   # (what is set up on first use)
+    S.synchronize()
+    reserved = B.bytes_reserved()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=S, capture_error_mode="relaxed"):
+            step()
+        graphs.append(g)
+    for i in range(6):
+        with torch.cuda.stream(S):
+            q.copy_(rnd(R, nh, d)); k.copy_(rnd(R, nkv, d)); v.copy_(rnd(R, nkv, d)); logits.copy_(rnd(G, K, V) * 3)
+            lens.fill_(1 + 19 * i)
+            table.copy_(own)   # (lengths begin anew, so rows share no pages)
+            before = [t.clone() for t in everything]
+            graphs[i % 2].replay()
+        S.synchronize()
+        replayed = [t.clone() for t in everything]
+        for t, b in zip(everything, before):
+            t.copy_(b)
+        torch.cuda.synchronize()
+        step()
+        B.sync()
+        torch.cuda.synchronize()
+        for t, r in zip(everything, replayed):
+            assert torch.equal(t, r)
+    assert B.bytes_reserved() == reserved
+    B.close()
+
+
+@gpu
+def test_recorded_mode_and_two_contexts(cuda):
+    """What is recorded runs first (lazy mode); two contexts' calls at the same time, on streams of their own, do not meet."""
+    import torch
+    L = cg.CudaBackend(0, cg.PREC_F32)
+    L.set_option("lazy", 1)
+    b = Batch([3, 1], [5, 18], 8)
+    q, k = (rounded(b.rng.standard_normal((b.M, h, 64)), "f32") for h in (4, 2))
+    results = []
+    for B in (cuda, L):
+        kp, vp = (put(B, np.zeros((b.n_pages, 2, 8, 64)))[0] for _ in range(2))
+        table, starts, lens = b.up(B)
+        qd, kd = B.add(B.from_numpy(q), B.from_numpy(q)), B.add(B.from_numpy(k), B.from_numpy(k))
+        q2 = B.paged_append(kd, kd, kp, vp, table, starts, lens, q=qd)
+        o = B.paged_attention(B.add(q2, q2), kp, vp, table, starts, lens)
+        results.append(B.to_numpy(B.add(o, o)))
+    assert np.array_equal(*results) and np.abs(results[0]).max() > 0
+    L.close()
+    two = [cg.CudaBackend(0, cg.PREC_F32) for _ in range(2)]
+    x = [rounded(np.random.default_rng(i).standard_normal((4, 4, 70001)) * 3, "f32") for i in range(2)]
+    s = np.zeros((4, 4), np.float32)
+    held = [(put(B, x[i])[0], put(B, s)[0]) for i, B in enumerate(two)]
+    for _ in range(20):
+        got = [B.beam_select(l, t, 4) for B, (l, t) in zip(two, held)]
+    for i, B in enumerate(two):
+        want = best(x[i], s, 4)
+        assert np.array_equal(B.to_numpy(got[i][1]), want[1]) and np.array_equal(B.to_numpy(got[i][2]), want[2])
+        B.close()
+
+
+@gpu
+def test_tensors_over_device_memory(cuda):
+    import torch
+    t = torch.arange(24, device="cuda", dtype=torch.float32).reshape(2, 3, 4)
+    torch.cuda.synchronize()
+    assert np.array_equal(cuda.to_numpy(cuda.from_device(t)), t.cpu().numpy())
+    view = t.transpose(0, 2)[:, 1:]
+    assert np.array_equal(cuda.to_numpy(cuda.add(cuda.from_device(view), cuda.from_device(view))), 2 * view.cpu().numpy())
+    b = cuda.from_device(t.bfloat16())
+    del t
+    assert cuda.storage_of(b) == 2 and np.array_equal(cuda.to_numpy(cuda.to_f32(b)).ravel(), np.arange(24))
+    with pytest.raises(TypeError):
+        cuda.from_device(torch.zeros(3, device="cuda", dtype=torch.float16))
+    with pytest.raises(TypeError):
+        cuda.from_device(torch.zeros(3))
+    with pytest.raises(cg.BackendPanic) as e:
+        cuda._ext1("cg_tensor_from_device", np.zeros(4, np.float32).ctypes.data, 0, (ctypes.c_int64 * 1)(4), None, 1)
+    assert e.value.status == 3
+
+
 # ---------------------------------------------------------------- refusals and index arithmetic, without a device
 
 
@@ -648,7 +849,7 @@ def test_attention_refusals(host):
                                     (SHAPE, dict(starts=u(5))), (DTYPE, dict(q=t(6, 4, 64, store="f32"))), (DTYPE, dict(out=t(6, 4, 64, store="f32"))), (DTYPE, dict(starts=t(4))),
                                     (INVALID, dict(most=-1)), (INVALID, dict(window=-1)), (INVALID, dict(cap=-1.0)), (INVALID, dict(cap=float("nan"))), (INVALID, dict(scale=float("inf"))),
                                     (INVALID, dict(scale=-0.5)), (UNSUPPORTED, dict(q=t(6, 4, 64, strides=[512, 128, 2]))), (UNSUPPORTED, dict(out=t(6, 4, 64, strides=[512, 64, 1]))),
-                                    (UNSUPPORTED, dict(k_pages=t(20, 2, 24, 64), v_pages=t(20, 2, 24, 64))), (INVALID, dict(q=t(6, 4, 64, at=at), out=t(6, 4, 64, at=at))),
+                                    (UNSUPPORTED, dict(k_pages=t(20, 2, 24, 64), v_pages=t(20, 2, 24, 64))), (SHAPE, dict(k_pages=t(0, 2, 16, 64), v_pages=t(0, 2, 16, 64))), (INVALID, dict(q=t(6, 4, 64, at=at), out=t(6, 4, 64, at=at))),
                                     (INVALID, dict(k_pages=t(20, 2, 16, 64, at=at), out=t(6, 4, 64, at=at, shift=1024)))]):
         assert call(**kw) == want, (i, want, H.lib.cg_last_error(H.ctx))
 
