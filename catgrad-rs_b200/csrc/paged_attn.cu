@@ -25,9 +25,10 @@ __device__ __forceinline__ void store_as(__nv_bfloat16* p, float x) { *p = __flo
 __device__ __forceinline__ float load_as(const float* p) { return *p; }
 __device__ __forceinline__ float load_as(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
-// 19 leading bits of an f32 and what they leave, as operands of the tensor cores' tf32 products
+// An f32 as the sum of two tf32 values of 11 bits, operands of the tensor cores.  The upper one is rounded to nearest (an infinity stays
+// one, near the largest value it may become one), so that the lower one, cut off, has either sign.
 __device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
-  hi = __float_as_uint(x) & 0xffffe000u;
+  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
   lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
 }
 __device__ __forceinline__ void mma_tf32(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -38,9 +39,10 @@ __device__ __forceinline__ void mma_tf32(float* c, const uint32_t* a, uint32_t b
 }
 
 // f32, and bf16 that the other kernels do not take (its values are widened on the way in).  Operands are split into two parts of
-// 11 bits, and three of the four products are summed in f32: what is left out is 2^-22 of a product, less than f32 sums of as
-// many terms are off by.  On the CUDA cores the same tiles are bound by shared memory, four or eight vectors for 16
-// products a thread: 7200 cycles for 64 queries and 32 keys of 64, against about 2000 here.
+// 11 bits, and three of the four products are summed in f32: what is left out is 2^-24 of a product.  The tensor cores cut sums off
+// instead of rounding them, so sums over more than a tile are made outside.  Error against 64 bits, 3 rows of up to 1713
+// tokens, heads of 64: 6.7e-7, of f32 sums 8.3e-7 (with one accumulator for all 2.1e-6, with parts cut off 3.1e-6).  On the
+// CUDA cores the same tiles are bound by shared memory, eight vectors for 16 x 4 products of a thread: 43 us, here 32.
 //
 // A block has QR queries of one row and key head (query x is token x / rep, head x % rep of the group) and a share of the visible
 // keys, GK at a time; its four warps share the rows (QR = 64) or the keys (QR = 16) of a tile, 16 rows each.  The blocks of a
@@ -184,9 +186,9 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
     ks += key0 * LK;
     vs += key0 * LV;
     const int64_t k0 = t * GK + key0;
-    float s[NT][4];
+    float s[NT][4], less[NT][4];  // (the small products apart)
 #pragma unroll
-    for (int i = 0; i < NT; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+    for (int i = 0; i < NT; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = less[i][0] = less[i][1] = less[i][2] = less[i][3] = 0.f;
 #pragma unroll 2
     for (int c = 0; c < D; c += 16) {  // components c + 4 t4 .. + 3: places t4 and t4 + 4 of two products
       uint32_t ah[2][4], al[2][4];
@@ -203,8 +205,8 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
         split(k.x, h[0], w[0]); split(k.y, h[1], w[1]); split(k.z, h[2], w[2]); split(k.w, h[3], w[3]);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          mma_tf32(s[i], al[u], h[2 * u], h[2 * u + 1]);
-          mma_tf32(s[i], ah[u], w[2 * u], w[2 * u + 1]);
+          mma_tf32(less[i], al[u], h[2 * u], h[2 * u + 1]);
+          mma_tf32(less[i], ah[u], w[2 * u], w[2 * u + 1]);
           mma_tf32(s[i], ah[u], h[2 * u], h[2 * u + 1]);
         }
       }
@@ -216,7 +218,7 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
     for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float x = s[i][e];
+        float x = s[i][e] + less[i][e];
         if (a.cap > 0.f) x = fmaf(2.f * cap2, rcp_newton(1.f + fast_exp2(x * cap_unit)), -cap2);
         else x *= scale;
         const int64_t key = k0 + i * 8 + 2 * t4 + (e & 1), pos = qpos[e >> 1];
@@ -245,18 +247,25 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
         }
     }
     const float base[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+    // probabilities of 8 keys as they lie are the left operand whose places t4 and t4 + 4 are keys 2 t4 and 2 t4 + 1
+    uint32_t ph[NT][4], pl[NT][4];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      // probabilities of 8 keys as they lie are the left operand whose places t4 and t4 + 4 are keys 2 t4 and 2 t4 + 1
-      uint32_t ph[4], pl[4];
+    for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float x = fast_exp2(s[i][e] - base[e >> 1]);
         l[e >> 1] += x;
-        split(x, ph[(e & 1) * 2 + (e >> 1)], pl[(e & 1) * 2 + (e >> 1)]);
+        split(x, ph[i][(e & 1) * 2 + (e >> 1)], pl[i][(e & 1) * 2 + (e >> 1)]);
       }
+    // (a tile's sums begin at 0 and are added to the output by rounded additions: the tensor cores' own cut bits off, which over a
+    // long row would lean one way)
 #pragma unroll
-      for (int c = 0; c < DG; ++c) {  // columns 32 c + 4 g + j are place g of product j
+    for (int c = 0; c < DG; ++c) {  // columns 32 c + 4 g + j are place g of product j
+      float sum[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[j][0] = sum[j][1] = sum[j][2] = sum[j][3] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
         const float4 v0 = *(const float4*)(vs + (i * 8 + 2 * t4) * LV + 32 * c + 4 * g), v1 = *(const float4*)(vs + (i * 8 + 2 * t4 + 1) * LV + 32 * c + 4 * g);
         const float b0[4] = {v0.x, v0.y, v0.z, v0.w}, b1[4] = {v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
@@ -264,11 +273,15 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
           uint32_t h0, w0, h1, w1;
           split(b0[j], h0, w0);
           split(b1[j], h1, w1);
-          mma_tf32(o[c][j], pl, h0, h1);
-          mma_tf32(o[c][j], ph, w0, w1);
-          mma_tf32(o[c][j], ph, h0, h1);
+          mma_tf32(sum[j], pl[i], h0, h1);
+          mma_tf32(sum[j], ph[i], w0, w1);
+          mma_tf32(sum[j], ph[i], h0, h1);
         }
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[c][j][e] += sum[j][e];
     }
     note(t + RING, page);
   }
