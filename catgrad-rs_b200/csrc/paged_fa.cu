@@ -14,6 +14,9 @@
 // the largest probability, which is exactly 1 against the exact maximum; the denominator sums the
 // probabilities as bf16 holds them, so that a row that one key decides loses nothing either way.
 //
+// Where there are few tiles, or a little more than a whole number of turns, a cluster of 2 or 4 blocks shares a tile's keys; their outputs
+// are joined through shared memory.
+//
 // Every mbarrier wait is bounded; on expiry the error word is raised, all roles leave their loops, TMEM is freed and the kernel
 // returns.
 #include <algorithm>
@@ -37,6 +40,7 @@ struct FaArgs {
   __nv_bfloat16* out;
   int64_t most, window, pool_rows;  // pool_rows: rows of d values in each pool, n_pages nkv page
   int nh, nkv, rep, per, d;         // per: tokens of a query tile
+  int slices;                       // blocks that share a tile's keys
   float scale_log2e, cap_log2e, cap_unit;  // soft-cap c: c log2(e), -2 log2(e) score factor / c
   float cap_in, cap_poly[6];               // score factor / c; c log2(e) times tanh's series
 };
@@ -128,7 +132,8 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;  // (warp: known to be uniform)
   // q, the tables and the pages are written by the preceding kernels
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int qt = (int)gridDim.x - 1 - (int)blockIdx.x, kvh = blockIdx.y;  // longest first
+  const int slice = (int)blockIdx.x % p.slices;
+  const int qt = ((int)gridDim.x - 1 - (int)blockIdx.x) / p.slices, kvh = blockIdx.y;  // longest first
   const int64_t row = blockIdx.z;
   int64_t tok0, n, len;
   if (!row_span(p.rows, row, p.most, &tok0, &n, &len)) return;   // uniform over the CTA, before anything is allocated
@@ -136,11 +141,13 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
   if (i0 >= n) return;
   const int64_t pos0 = len - n, last = pos0 + min(n, i0 + NQ * p.per) - 1;  // position of the last query
   const int64_t lo = p.window > 0 ? max((int64_t)0, pos0 + i0 - p.window + 1) : 0;  // first visible key
-  const int64_t j0 = lo / KT;
-  const int nt = (int)(last / KT + 1 - j0);
+  // this block's share of the key tiles: [j0, j0 + nt)
+  const int all = (int)(last / KT + 1 - lo / KT), share = (all + p.slices - 1) / p.slices;
+  const int64_t j0 = lo / KT + (int64_t)slice * share;
+  const int nt = min(share, max(0, all - slice * share));
   // Keys of the last tile that some query sees.  The values behind them (what nothing or another sequence wrote) are
   // cleared in shared memory: a probability of 0 times an infinity would not be 0
-  const int seen = (int)(last % KT) + 1;
+  const int seen = nt > 0 && slice * share + nt == all ? (int)(last % KT) + 1 : KT;
 
   if (tid == 0) {
     mbar_init(b_q, 1);
@@ -175,7 +182,8 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
   const uint32_t tmem_base = *tmem_slot;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  if (warp == 0) {
+  float m = -INFINITY, l = 0.f;  // of a row (m in units of log2: what a score is in the exponent of 2)
+  if (warp == 0 && nt > 0) {
     // ---- loads ----
     if (lane == 0) {
       mbar_expect_tx(b_q, NQ * SUB * (uint32_t)(p.per * p.rep) * 128u);
@@ -219,7 +227,7 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
         if (i < j || half) mbar_drain(b_k_full + 8 * (i % KS), (uint32_t)(i / KS) & 1u, p.rows.err);
         if (i < j) mbar_drain(b_v_full + 8 * (i % KS), (uint32_t)(i / KS) & 1u, p.rows.err);
       }
-  } else if (warp == 1 || (NQ == 2 && warp == 3)) {
+  } else if (nt > 0 && (warp == 1 || (NQ == 2 && warp == 3))) {
     // ---- products ----
     // The whole warp goes through the loop and one lane issues: descriptors then are uniform values, which an issue takes as they are.
     // (A single lane's loop: some 70 cycles an issue where a product of 64 keys takes 48.)
@@ -308,7 +316,6 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
     const int head = kvh * p.rep + r % p.rep;
     const int64_t qpos = pos0 + ti;
     const int64_t tile_last = min(pos0 + first + p.per - 1, last), tile_first = pos0 + first;
-    float m = -INFINITY, l = 0.f;  // (m in units of log2: what a score is in the exponent of 2)
     bool ok = true;
     for (int j = 0; j < nt && ok; ++j) {
       const int buf = j & 1;
@@ -443,14 +450,14 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
       if (lane == 0) arrive(b_p + 8 * buf);
       l += ls[0] + ls[1];
     }
-    ok = ok && mbar_wait(b_o, (uint32_t)(nt - 1) & 1u, cta_abort, p.rows.err);
+    ok = ok && (nt == 0 || mbar_wait(b_o, (uint32_t)(nt - 1) & 1u, cta_abort, p.rows.err));
     ok = __all_sync(0xffffffffu, ok);
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const float inv = l > 0.f ? 1.f / l : 0.f;
     const bool out = ok && r < p.per * p.rep && ti < n;
     __nv_bfloat16* dst = p.out + ((tok0 + ti) * p.nh + head) * (int64_t)p.d;
 #pragma unroll 1
-    for (int c0 = 0; c0 < D; c0 += 32) {
+    for (int c0 = 0; c0 < D && p.slices == 1; c0 += 32) {
       uint32_t v[32];
       ld32(o_addr + c0, v);
       asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -469,10 +476,87 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
 
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  // ---- the blocks' shares ----
+  constexpr int LD = D + 4;
+  static_assert((size_t)NQ * 128 * LD * 4 <= NQ * Q_BYTES + 2 * KS * KV_BYTES, "the outputs lie over the tiles");
+  float* const part = (float*)gen;  // [NQ][128][LD] outputs of this block, for the cluster
+  __shared__ float part_m[NQ * 128], part_l[NQ * 128];
+  if (p.slices > 1) {
+    if (warp >= 4) {
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const int x = tid - 128, q = warp & 3;
+      const uint32_t o_addr = tmem_base + (uint32_t)(x >> 7) * TILE_COLS + ((uint32_t)(q * 32) << 16) + 2 * KT;
+      part_m[x] = m;
+      part_l[x] = l;
+#pragma unroll 1
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t v[32];
+        ld32(o_addr + c0, v);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < 32; i += 4)
+          *(uint4*)(part + x * LD + c0 + i) = l > 0.f ? make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]) : make_uint4(0u, 0u, 0u, 0u);  // (without tiles nothing was written)
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    }
+    __syncthreads();
+  }
   if (warp == 1) {
     __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(NCOLS) : "memory");
   }
+  if (p.slices == 1) return;
+  __shared__ float weight[4][NQ * 128];  // of the blocks' outputs of a row
+  cluster_sync_all();
+  if (tid < NQ * 128) {
+    float ms[4], ls[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      ms[s] = s < p.slices ? ld_cluster_f32(smem_u32(&part_m[tid]), (uint32_t)s) : -INFINITY;
+      ls[s] = s < p.slices ? ld_cluster_f32(smem_u32(&part_l[tid]), (uint32_t)s) : 0.f;
+    }
+    const float top = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])), at = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      ms[s] = fast_exp2(ms[s] - at);
+      sum = fmaf(ls[s], ms[s], sum);
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) weight[s][tid] = sum > 0.f ? ms[s] / sum : 0.f;
+  }
+  __syncthreads();
+  constexpr int U = 4;  // values of a thread on their way, 4 columns each
+  const int step = (int)blockDim.x * p.slices;
+  for (int i = slice * (int)blockDim.x + tid; i < NQ * 128 * (D / 4); i += U * step) {
+    float4 os[U][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        os[u][s] = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int k = i + u * step;
+        if (s < p.slices && k < NQ * 128 * (D / 4)) {
+          uint32_t at;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(part + k / (D / 4) * LD + k % (D / 4) * 4)), "r"(s));
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(os[u][s].x), "=f"(os[u][s].y), "=f"(os[u][s].z), "=f"(os[u][s].w) : "r"(at));
+        }
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = i + u * step, x = k / (D / 4), c = k % (D / 4) * 4, r = x & 127;
+      const int64_t ti = i0 + (x >> 7) * p.per + r / p.rep;
+      if (k >= NQ * 128 * (D / 4) || r >= p.per * p.rep || ti >= n || c >= p.d) continue;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const float f = weight[s][x];
+        v.x = fmaf(os[u][s].x, f, v.x); v.y = fmaf(os[u][s].y, f, v.y); v.z = fmaf(os[u][s].z, f, v.z); v.w = fmaf(os[u][s].w, f, v.w);
+      }
+      *(uint2*)(p.out + ((tok0 + ti) * p.nh + kvh * p.rep + r % p.rep) * (int64_t)p.d + c) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+    }
+  }
+  cluster_sync_all();
 }
 
 // q as [tokens, heads, d] in boxes of [per tokens, rep heads, 64 components]
@@ -523,8 +607,21 @@ int launch(cg_ctx* c, const PagedAttnArgs& a) {
   CG_TRY(make_map(c, &mk, a.k_pages, p.pool_rows, a.d, a.d, box));
   CG_TRY(make_map(c, &mv, a.v_pages, p.pool_rows, a.d, a.d, box));
   CG_TRY(make_q_map(c, &mq, a, p.per, p.rep));
-  const int64_t tiles = (a.most + (int64_t)NQ * p.per - 1) / ((int64_t)NQ * p.per);
-  CG_CUDA(c, launch_kernel(c, k_paged_fa<D, NQ, CAP>, dim3((unsigned)tiles, (unsigned)a.nkv, (unsigned)a.rows.rows), dim3(NQ == 2 ? 384 : 256), smem, 1, mq, mk, mv, p));
+  const int64_t tiles = (a.most + (int64_t)NQ * p.per - 1) / ((int64_t)NQ * p.per), longest = a.rows.cols << a.rows.lg;
+  // Shares of the keys (of several rows four fifths of the tiles count: they differ).  Us with 1 / 2 / 4, [the rule's]:
+  //   6 rows of 480 behind 3720, 4 x 2 heads of 256, window 4096    181  [157]  189  (rows that differ: 169 [152] 186)
+  //   1 of 63 behind 2937, the same, no window                     62.2   39.4 [25.5]
+  //   1 of 49 behind 3951, 8 x 4 heads of 128                      66.1   40.9 [26.1]
+  //   1 of 2000, the same                                         [60.1]  71.7  118
+  //   4 of 300 behind 1700, the same                              [72.7]  75.9  94
+  //   3 of 200 behind 8800, heads of 64                            140    146  [125]
+  static AtATime known;
+  const int64_t clusters = tiles * a.nkv * a.rows.rows;
+  p.slices = pick_shares([&](int i) { return at_a_time(known, c->core->device, i, k_paged_fa<D, NQ, CAP>, NQ == 2 ? 384 : 256, smem); }, 4,
+                         a.rows.rows > 1 ? std::max<int64_t>(clusters * 4 / 5, 1) : clusters, a.window > 0 ? std::min(longest, a.window + p.per * NQ) : longest, KT, 6.,
+                         D == 256 ? 1.25 : NQ == 2 ? 1.1 : 0.9, 0.);
+  CG_CUDA(c, launch_kernel(c, k_paged_fa<D, NQ, CAP>, dim3((unsigned)(tiles * p.slices), (unsigned)a.nkv, (unsigned)a.rows.rows), dim3(NQ == 2 ? 384 : 256), smem, -p.slices,
+                           mq, mk, mv, p));
   CG_LAUNCHED(c);
   return CG_OK;
 }
