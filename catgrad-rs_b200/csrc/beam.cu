@@ -372,6 +372,16 @@ __global__ void __launch_bounds__(SB * BT, 4 / SB) k_beam_select(SelectArgs a) {
     at0 = ((u - j * a.pieces) * (BT * VECS) + tid) * per - (int)(((uintptr_t)row & 15) / sizeof(T));
   };
   auto load = [&](uint32_t* x) {
+    const int first = at0 - tid * per;
+    if (first >= 0 && first + BT * VECS * per <= a.V) {  // (all of the piece's)
+      const uint4* from = (const uint4*)(row + at0);
+#pragma unroll
+      for (int v = 0; v < VECS; ++v) {
+        const uint4 q = __ldg(from + v * BT);
+        x[4 * v] = q.x; x[4 * v + 1] = q.y; x[4 * v + 2] = q.z; x[4 * v + 3] = q.w;
+      }
+      return;
+    }
     bool edge = false;  // (all whole vectors are asked for before any is waited for)
 #pragma unroll
     for (int v = 0; v < VECS; ++v) {
