@@ -465,7 +465,7 @@ class CudaBackend(TraitBackend):
     # a paged key/value cache and beam search ---------------------------------------
     def from_device(self, x) -> TaggedTensor:
         """A tensor over the device memory of `x` (a torch CUDA tensor: f32, bf16, or 32-bit integers as U32), which it
-        keeps alive.  Nothing is copied.  Work of other streams on that memory is the caller's to order."""
+        keeps alive (its views do not).  Nothing is copied.  Work of other streams on that memory is the caller's to order."""
         storage = {"torch.float32": 0, "torch.int32": 1, "torch.uint32": 1, "torch.bfloat16": 2}.get(str(x.dtype))
         if storage is None:
             raise TypeError(f"no storage for {x.dtype}")

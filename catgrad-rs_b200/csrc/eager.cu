@@ -511,7 +511,7 @@ int bf16_operand(cg_ctx* c, const cg_tensor* a, int64_t M, int64_t K, int64_t ro
   av.t->strides[0] = row_stride; av.t->strides[1] = col_stride;
   CG_TRY(copy_into(c, av.t, xa.t->data(), ST_BF16, xa.t->strides));
   *out = (const __nv_bfloat16*)xa.t->data();
-  if (b->owned) {  // (memory the library does not own may be rewritten behind its back)
+  if (b->owned && !b->rewritten) {  // (memory the library does not own may be rewritten behind its back)
     b->bf16_copy = xa.t->buf;  // the copy lives as long as the buffer it was made from
     memcpy(b->bf16_key, key, sizeof(key));
   }
@@ -774,7 +774,7 @@ int32_t cg_cast(cg_ctx* c, const cg_tensor* x, int32_t dtype, cg_tensor** out) {
     *out = const_cast<cg_tensor*>(x);
     return CG_OK;
   }
-  if (x->has_scalar && !x->node && x->numel() == 1) {
+  if (x->literal() && !x->node && x->numel() == 1) {
     // a literal whose value is known on the host (e.g. the element count an rmsnorm divides by,
     // cast from a Nat): convert it here and upload the result, no kernel
     uint32_t bits;
@@ -798,7 +798,7 @@ int32_t cg_cast(cg_ctx* c, const cg_tensor* x, int32_t dtype, cg_tensor** out) {
   Hold r;
   CG_TRY(new_tensor(c, dtype, dtype == CG_F32 ? ST_F32 : ST_U32, x->dims, x->rank, &r.t));
   CG_TRY(copy_into(c, src.t, r.t->data(), r.t->storage, r.t->strides, dtype == CG_U32 ? 4 : 5));
-  if (x->has_scalar) {
+  if (x->literal()) {
     // the literal's value follows it through the cast (f32 -> u32 saturates, NaN -> 0, as `as` does)
     r.t->has_scalar = true;
     if (dtype == CG_F32) {

@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(128) k_attn_f32(const float* q, const int64_t*
 // matching helpers
 
 bool scalar_f32(const cg_tensor* t, float* v) {
-  if (!t || t->node || !t->has_scalar || t->tag != CG_F32) return false;
+  if (!t || t->node || !t->literal() || t->tag != CG_F32) return false;
   memcpy(v, &t->scalar_bits, 4);
   return true;
 }
@@ -834,7 +834,7 @@ bool lazy_reduce(cg_ctx* c, int red, const cg_tensor* x, cg_tensor** out, int* s
 }
 
 bool lazy_cast(cg_ctx* c, const cg_tensor* x, int dtype, cg_tensor** out, int* st) {
-  if (!x->node && x->has_scalar) return false;  // a literal: cast it now so its value stays known
+  if (!x->node && x->literal()) return false;  // a literal: cast it now so its value stays known
   cg_tensor* t = pending_tensor(c, dtype, x->dims, x->rank);
   LazyNode* n = add_node(c, LZ_CAST, t, x, nullptr);
   n->a[0] = dtype;

@@ -51,6 +51,10 @@ __global__ void __launch_bounds__(256) k_paged_append(AppendArgs a) {
   if (row >= a.rows.rows) return;  // behind the last row
   int64_t tok0, n, len;
   if (!row_span(a.rows, row, a.rows.M, &tok0, &n, &len) || m < tok0) return;
+  if (m >= tok0 + n) {  // (starts that do not ascend)
+    *a.rows.err = DEV_INDEX;
+    return;
+  }
   const int64_t pos = len - n + (m - tok0);
   if (a.cos_t && pos >= a.T) {
     *a.rows.err = DEV_INDEX;
@@ -181,6 +185,10 @@ __global__ void __launch_bounds__(128, 5) k_paged_append_vec(AppendArgs a, int p
   if (row >= a.rows.rows) return;  // behind the last row
   int64_t tok0, n, len;
   if (!row_span(a.rows, row, a.rows.M, &tok0, &n, &len) || m < tok0) return;
+  if (m >= tok0 + n) {  // (starts that do not ascend)
+    *a.rows.err = DEV_INDEX;
+    return;
+  }
   const int64_t pos = len - n + (m - tok0);
   if (a.cos_t && pos >= a.T) {
     *a.rows.err = DEV_INDEX;

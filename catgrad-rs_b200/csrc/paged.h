@@ -105,10 +105,10 @@ inline bool overlap_any(const cg_tensor* const (&in)[NI], const cg_tensor* const
   return false;
 }
 // `t` is written in place: no two of its elements share memory (contiguous), a cached GEMM operand copy is stale, and a literal's value
-// is no longer known.
+// is no longer known, by this tensor and by all that share its memory.
 inline void written(cg_tensor* t) {
   t->buf->bf16_copy.reset();
-  t->has_scalar = false;
+  t->buf->rewritten = true;
 }
 
 // The pages: k and v alike, [n_pages, nkv, page, d] (with `layers`, [layers, n_pages, nkv, page, d]).

@@ -228,7 +228,7 @@ cg_tensor* new_view(const cg_tensor* x) {
   memcpy(t->strides, x->strides, sizeof(t->strides));
   t->offset = x->offset;
   t->buf = x->buf;
-  t->has_scalar = x->has_scalar;
+  t->has_scalar = x->literal();
   t->scalar_bits = x->scalar_bits;
   return t;
 }

@@ -39,6 +39,7 @@ struct Buffer {
   // it was made for: q, k and v (or gate and up) read the same activations, and trait tensors
   // are never written after they are made, so the copy serves every one of them.  Whoever does
   // write a tensor in place (cg_comm_all_reduce) drops it.
+  bool rewritten = false;  // an operator that writes in place had it: a captured graph may do so again, unseen, so no copy is kept
   std::shared_ptr<Buffer> bf16_copy;
   int64_t bf16_key[5] = {0, 0, 0, 0, 0};  // offset, rows, cols, row stride, col stride
   ~Buffer();
@@ -142,6 +143,7 @@ struct cg_tensor {
   // as x / sqrt(mean + eps) can be recognised without reading device memory
   bool has_scalar = false;
   uint32_t scalar_bits = 0;
+  bool literal() const { return has_scalar && !(buf && buf->rewritten); }
 
   int64_t numel() const {
     int64_t n = 1;
