@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
   // this lane's rows g and g + 8 of the warp's 16
   const int r0 = (QR == 64 ? warp * 16 : 0) + g, key0 = QR == 64 ? 0 : warp * (GK / 4);
   const int64_t qpos[2] = {pos0 + (x0 + r0) / rep, pos0 + (x0 + r0 + 8) / rep};
-  const float scale = a.scale * 1.4426950408889634f, cap2 = a.cap * 1.4426950408889634f, cap_unit = a.cap > 0.f ? -2.f * scale / a.cap : 0.f;
+  const float scale = a.scale * 1.4426950408889634f, cap2 = a.cap * 1.4426950408889634f, cap_in = a.cap > 0.f ? a.scale / a.cap : 0.f, cap_unit = -2.f * 1.4426950408889634f * cap_in;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[DG][4][4];
 #pragma unroll
   for (int c = 0; c < DG; ++c)
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float x = s[i][e] + less[i][e];
-        if (a.cap > 0.f) x = fmaf(2.f * cap2, rcp_newton(1.f + fast_exp2(x * cap_unit)), -cap2);
+        if (a.cap > 0.f) x = soft_cap(x, cap2, cap_in, cap_unit);
         else x *= scale;
         const int64_t key = k0 + i * 8 + 2 * t4 + (e & 1), pos = qpos[e >> 1];
         if (masked && (key > pos || (a.window > 0 && key <= pos - a.window))) x = -INFINITY;
@@ -441,9 +441,10 @@ extern "C" int32_t cg_paged_attention(cg_ctx* c, const cg_tensor* q, const cg_te
   a.q = q->data(); a.k_pages = k_pages->data(); a.v_pages = v_pages->data(); a.out = out->data();
   a.q_ld = q->strides[0]; a.q_hs = q->strides[1];
   a.most = max_new > 0 ? std::min(max_new, M) : M;
-  a.window = window;
+  a.window = window < a.rows.cols << lg ? window : 0;  // (one that reaches over all positions is none)
   a.scale = scale > 0.f ? scale : 1.f / sqrtf((float)d);
-  a.cap = softcap;
+  // (caps beyond 2^+-100 act as these: all scores are far below the one, and differ by nothing that an exponential shows under the other)
+  a.cap = softcap > 0.f ? fminf(fmaxf(softcap, 0x1p-100f), 0x1p100f) : 0.f;
   a.nh = (int)nh; a.nkv = (int)nkv; a.d = (int)d;
   written(out);
   if (q->storage == ST_BF16 && paged_fa_supported(a)) return paged_fa(c, a);

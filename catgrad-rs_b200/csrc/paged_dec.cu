@@ -30,7 +30,7 @@ struct DecArgs {
   __nv_bfloat16* out;
   int64_t q_ld, q_hs, most, window, pool_rows;
   int nh, nkv, rep, d;
-  float scale_log2e, cap_log2e, cap_unit;
+  float scale_log2e, cap_log2e, cap_in, cap_unit;
 };
 
 // keys of a warp's tile, tiles of its ring
@@ -179,7 +179,7 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float& x = s[i][2 * b + e];
-          if (CAP) x = fmaf(2.f * p.cap_log2e, rcp_newton(1.f + fast_exp2(x * p.cap_unit)), -p.cap_log2e);
+          if (CAP) x = soft_cap(x, p.cap_log2e, p.cap_in, p.cap_unit);
           else x *= p.scale_log2e;
           if (masked) {
             const int64_t key = k0 + i * 8 + t2 + e;
@@ -331,9 +331,10 @@ int launch(cg_ctx* c, const PagedAttnArgs& a) {
   p.pool_rows = (a.rows.n_pages * a.nkv) << a.rows.lg;
   p.nh = a.nh; p.nkv = a.nkv; p.rep = a.nh / a.nkv; p.d = a.d;
   p.scale_log2e = a.scale * LOG2E;
-  p.cap_log2e = p.cap_unit = 0.f;
+  p.cap_log2e = p.cap_in = p.cap_unit = 0.f;
   if (CAP) {
     p.cap_log2e = a.cap * LOG2E;
+    p.cap_in = a.scale / a.cap;
     p.cap_unit = -2.f * p.scale_log2e / a.cap;
   }
   CUtensorMap mk, mv;

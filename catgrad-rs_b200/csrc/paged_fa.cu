@@ -43,6 +43,7 @@ struct FaArgs {
   int slices;                       // blocks that share a tile's keys
   float scale_log2e, cap_log2e, cap_unit;  // soft-cap c: c log2(e), -2 log2(e) score factor / c
   float cap_in, cap_poly[6];               // score factor / c; c log2(e) times tanh's series
+  float lag;                               // LAG in products q k
 };
 
 // B operand stored [k rows][n contiguous] in 128-byte-swizzled boxes of [rows, 64 elements], chunk_bytes apart
@@ -183,6 +184,7 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   float m = -INFINITY, l = 0.f;  // of a row (m in units of log2: what a score is in the exponent of 2)
+  float limit = -INFINITY;       // the product q k from which m follows
   if (warp == 0 && nt > 0) {
     // ---- loads ----
     if (lane == 0) {
@@ -347,22 +349,29 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
       for (int i = 0; i < KT; i += 2) mx4[i / 2 & 3] = fmaxf(fmaxf(mx4[i / 2 & 3], __uint_as_float(v[i])), __uint_as_float(v[i + 1]));
       const float raw_max = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
       bool small = false;  // (uniform) no score is beyond 3/4 of the cap
-      if (CAP && !masked) {
+      if (CAP) {
+        if (masked)
+#pragma unroll
+          for (int i = 0; i < KT; ++i) v[i] = vis[i / 32] >> (i & 31) & 1u ? v[i] : 0u;  // (their probabilities are cleared)
         float low4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < KT; i += 2) low4[i / 2 & 3] = fminf(fminf(low4[i / 2 & 3], __uint_as_float(v[i])), __uint_as_float(v[i + 1]));
         const float far = fmaxf(raw_max, -fminf(fminf(low4[0], low4[1]), fminf(low4[2], low4[3])));
         small = __all_sync(0xffffffffu, far * p.cap_in <= 0.75f);
       }
-      float mx;  // (the soft-cap is monotone)
-      if (CAP) mx = raw_max == -INFINITY ? -INFINITY : fmaf(2.f * p.cap_log2e, rcp_newton(1.f + fast_exp2(raw_max * p.cap_unit)), -p.cap_log2e);
-      else mx = raw_max * p.scale_log2e;
+      // (the soft-cap is monotone, and what a score grows by is no less than what its cap does)
+      auto reference = [&]() {
+        if (CAP) return raw_max == -INFINITY ? -INFINITY : soft_cap(raw_max, p.cap_log2e, p.cap_in, p.cap_unit);
+        return raw_max * p.scale_log2e;
+      };
       if (j == 0) {
-        m = mx;
+        m = reference();
+        limit = raw_max + p.lag;
       } else {
-        const bool grown = mx > m + LAG;
+        const bool grown = raw_max > limit;
         if (__any_sync(0xffffffffu, grown)) {
-          const float m_new = grown ? mx : m;
+          const float m_new = grown ? reference() : m;
+          limit = grown ? raw_max + p.lag : limit;
           const float corr = grown ? fast_exp2(m - m_new) : 1.f;  // 0 while m is -inf
           // (the product before the last was complete before this tile's scores could be issued, so the parity is that
           // of the last)
@@ -391,7 +400,6 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
         for (int i = 0; i < 32; i += 2) {
           const float e0 = fast_exp2(exponent(__uint_as_float(v[c * 32 + i]))), e1 = fast_exp2(exponent(__uint_as_float(v[c * 32 + i + 1])));
           pk[i / 2] = pack_bf16(e0, e1);
-          // (masked scores are -inf, whose cap is not)
           if (CAP && masked) pk[i / 2] &= (vis[c] >> i & 1u ? 0xffffu : 0u) | (vis[c] >> i & 2u ? 0xffff0000u : 0u);
           ls[0] += __uint_as_float(pk[i / 2] << 16);
           ls[1] += __uint_as_float(pk[i / 2] & 0xffff0000u);
@@ -430,15 +438,21 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
             float x0, x1;
             asm("mov.b64 {%0, %1}, %2;" : "=f"(x0), "=f"(x1) : "l"(f));
             pk[i / 2] = pack_bf16(fast_exp2(x0), fast_exp2(x1));
-            ls[0] += __uint_as_float(pk[i / 2] << 16);
-            ls[1] += __uint_as_float(pk[i / 2] & 0xffff0000u);
+          }
+          if (masked)
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) pk[i / 2] &= (vis[c] >> i & 1u ? 0xffffu : 0u) | (vis[c] >> i & 2u ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            ls[0] += __uint_as_float(pk[i] << 16);
+            ls[1] += __uint_as_float(pk[i] & 0xffff0000u);
           }
           st16(s_addr + (uint32_t)c * 16u, pk);
         }
       } else
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        if (CAP) half(c, [&](float x) { return fmaf(2.f * p.cap_log2e, rcp_newton(1.f + fast_exp2(x * p.cap_unit)), -p.cap_log2e - mc); });
+        if (CAP) half(c, [&](float x) { return soft_cap(x, p.cap_log2e, p.cap_in, p.cap_unit) - mc; });
         else half(c, [&](float x) { return fmaf(x, p.scale_log2e, -mc); });
       }
       // (This warp may be a whole product ahead of the tensor core, and a parity tells only neighbouring phases apart: the
@@ -594,12 +608,11 @@ int launch(cg_ctx* c, const PagedAttnArgs& a) {
   p.scale_log2e = a.scale * LOG2E;
   p.cap_log2e = p.cap_unit = p.cap_in = 0.f;
   for (float& f : p.cap_poly) f = 0.f;
+  p.lag = std::min(LAG / p.scale_log2e, 1e38f);
   if (CAP) {
     p.cap_log2e = a.cap * LOG2E;
     p.cap_unit = -2.f * p.scale_log2e / a.cap;
-    // tanh(y) / y in y^2 up to 3/4, fitted to the least largest relative error, 3e-8: half a step of f32
-    const float series[6] = {1.f, -0.33332958817481995f, 0.1332540661096573f, -0.05334442853927612f, 0.019582903012633324f, -0.004716253839433193f};
-    for (int i = 0; i < 6; ++i) p.cap_poly[i] = p.cap_log2e * series[i];
+    for (int i = 0; i < 6; ++i) p.cap_poly[i] = p.cap_log2e * tanh_term(i);
     p.cap_in = a.scale / a.cap;
   }
   CUtensorMap mq, mk, mv;

@@ -307,8 +307,8 @@ int32_t cg_paged_append(cg_ctx*, const cg_tensor* q, const cg_tensor* k, const c
 /* Attention of the new tokens q [tokens, heads, d] over their rows' cached tokens up to their own
  * position (so after cg_paged_append), into out [tokens, heads, d]; q and out are stored as the
  * pages.  heads is a multiple of kv heads, grouped as in cg_fused_attention.  max_new: no row has
- * more new tokens (0 = not known); a row that has more is left out (CG_ERR_INDEX).  scale 0 =
- * 1 / sqrt(d).  window > 0: only the last `window` tokens are seen; pages before all windows of a
+ * more new tokens (0 = not known: every row gets the blocks of all tokens, which costs time where
+ * rows are many); a row that has more is left out (CG_ERR_INDEX).  scale 0 = 1 / sqrt(d).  window > 0: only the last `window` tokens are seen; pages before all windows of a
  * row are not read, so their table entries may be stale.  softcap > 0 as in cg_fused_attention.
  * What is cached at a row's positions is finite. */
 int32_t cg_paged_attention(cg_ctx*, const cg_tensor* q, const cg_tensor* k_pages, const cg_tensor* v_pages,
@@ -319,7 +319,7 @@ int32_t cg_paged_attention(cg_ctx*, const cg_tensor* q, const cg_tensor* k_pages
  * the K largest in descending order, equal ones by j, then v.  logits [B, J, V] f32 or bf16, scores
  * [B, J] f32 (-inf: a beam that is not there), finished U32 [B, J] or NULL: a finished beam's only
  * continuation is `end` at an unchanged score.  NaN logits count as -inf; a beam whose largest logit
- * or score is not finite has -inf everywhere.  Outputs [B, K] (K <= V, J and K at most 32): scores,
+ * or score is not finite has -inf everywhere.  Outputs [B, K] (K <= V <= 2^20 - 8, J and K at most 32): scores,
  * tokens, parents (beams of the group) and finished (the parent was, or the token is `end`).
  * scores_out and finished_out may be scores and finished themselves when K = J. */
 int32_t cg_beam_select(cg_ctx*, const cg_tensor* logits, const cg_tensor* scores, const cg_tensor* finished, uint32_t end,

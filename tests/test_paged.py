@@ -174,7 +174,7 @@ def attention(q, k, v, pos, scale, window, cap):
     return np.einsum("ht,thd->hd", p, v), np.einsum("ht,thd->hd", p, np.abs(v)), size
 
 
-def check_attention(B, b, store, nh, nkv, d, window=0, cap=0.0, scale=0.0, spread=1.0, stale=None, strided=False, max_new=None, check=None):
+def check_attention(B, b, store, nh, nkv, d, window=0, cap=0.0, scale=0.0, spread=1.0, stale=None, strided=False, max_new=None, check=None, offset=None):
     import torch
     rng = b.rng
     q = rounded(rng.standard_normal((b.M, nh, d)) * spread, store)
@@ -194,6 +194,11 @@ def check_attention(B, b, store, nh, nkv, d, window=0, cap=0.0, scale=0.0, sprea
         wide[:, :nh, :d] = torch.from_numpy(q).cuda()
         torch.cuda.synchronize()
         qd = (B.from_device(wide[:, :nh, :d]), wide)
+    elif offset is not None:   # from a place that no vector begins on
+        flat = torch.zeros(q.size + offset, device="cuda").to(kd[1].dtype)
+        flat[offset:] = torch.from_numpy(q).cuda().reshape(-1)
+        torch.cuda.synchronize()
+        qd = (B.from_device(flat[offset:].reshape(q.shape)), flat)
     else:
         qd = put(B, q, store)
     table, starts, lens = b.up(B)
@@ -229,6 +234,33 @@ def test_attention(cuda, store, nh, nkv, d, window, cap):
     for i, (new, total, page) in enumerate(SHAPES):
         check_attention(cuda, Batch(new, total, page, seed=i, spare=i % 3), store, nh, nkv, d, window, cap, spread=2.0, strided=i % 2 == 1,
                         scale=0.0 if i % 3 else 0.3)
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+@pytest.mark.parametrize("nh,nkv,d", [(4, 2, 64), (4, 2, 128), (6, 1, 40), (2, 2, 256)])
+@pytest.mark.parametrize("offset", [1, 2])
+def test_attention_of_unaligned_queries(cuda, store, nh, nkv, d, offset):
+    for i, (new, total, page) in enumerate(SHAPES):
+        check_attention(cuda, Batch(new, total, page, seed=i, spare=1), store, nh, nkv, d, 9 * (i % 2), spread=2.0, stale=np.nan, offset=offset)
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+@pytest.mark.parametrize("nh,nkv,d", [(4, 2, 64), (2, 1, 256), (4, 2, 128)])
+@pytest.mark.parametrize("cap,spread", [(1e4, 2.0), (1e30, 2.0), (2e38, 2.0), (0.5, 30.0), (8.0, 30.0), (1e-38, 2.0)])
+def test_attention_caps_far_above_and_below_the_scores(cuda, store, nh, nkv, d, cap, spread):
+    """A cap far above the scores leaves them their 24 bits; one far below makes them all but equal."""
+    for new, total in (([1, 1], [300, 77]), ([150, 3], [400, 300])):
+        check_attention(cuda, Batch(new, total, 16), store, nh, nkv, d, 0, cap, spread=spread)
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+@pytest.mark.parametrize("window", [303, 304, 305, 2 ** 31, 2 ** 63 - 1])
+def test_attention_windows_longer_than_all(cuda, store, window):
+    for new in ([1, 1], [150, 3]):
+        check_attention(cuda, Batch(new, [300, 304], 16), store, 4, 2, 128, window, stale=np.nan)
 
 
 # around tiles of 16 to 128 keys and queries, shares of the keys, pages that end inside a tile
@@ -692,6 +724,75 @@ def test_captured_steps_replay_with_new_lengths_and_tables(store):
             assert torch.equal(t, r)
     assert B.bytes_reserved() == reserved
     B.close()
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 40])
+def test_append_starts_that_do_not_ascend(cuda, d):
+    """Reported, and no token is placed by a row that it is not of: no page but the rows' own first ones is touched."""
+    B, page, cols, M = cuda, 8, 2, 12
+    for starts in ([0, 10, 2, 4], [0, 12, 0, 3], [5, 1, 9, 2], [0, 0xFFFFFFFF, 1, 2]):
+        k = put(B, np.ones((M, 2, d)))[0]
+        kp, vp = (put(B, np.zeros((6, 2, page, d))) for _ in range(2))
+        B.paged_append(k, k, kp[0], vp[0], put(B, np.arange(6, dtype=np.uint32).reshape(3, cols))[0], put(B, np.array(starts, np.uint32))[0],
+                       put(B, np.array([10, 10, 2], np.uint32))[0])
+        with pytest.raises(cg.BackendPanic) as e:
+            B.sync()
+        assert e.value.status == 6
+        got = back(B, kp[1])
+        n = [b - a for a, b in zip(starts, starts[1:])]
+        for r, (new, length) in enumerate(zip(n, (10, 10, 2))):
+            placed = got[r * cols:(r + 1) * cols, 0, :, 0].reshape(-1)
+            lo = length - new if 0 < new <= length else length
+            assert not placed[:lo].any() and not placed[length:].any()
+
+
+@gpu
+def test_what_the_library_knows_of_a_tensor_ends_when_it_is_written(cuda):
+    """A product's rounded copy of its operand and a literal's value are not used behind a write in place, a replayed one either."""
+    import torch
+    S = torch.cuda.Stream()
+    B = cg.CudaBackend(0, cg.PREC_BF16, stream=S.cuda_stream)
+    new, nh, nkv, d, page = 16, 2, 2, 64, 16
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    q, k = (torch.randn(new, h, d, generator=gen, device="cuda") for h in (nh, nkv))
+    eye = B.from_numpy(np.eye(nh * d, dtype=np.float32))
+    kp, vp, q_out = B.zeros((1, nkv, page, d), cg.F32), B.zeros((1, nkv, page, d), cg.F32), B.zeros((new, nh, d), cg.F32)
+    ints = [torch.tensor(x, device="cuda", dtype=torch.int32) for x in ([[0]], [0, new], [new])]
+    torch.cuda.synchronize()
+    hq, hk = B.from_device(q), B.from_device(k)
+    table, starts, lens = (B.from_device(x) for x in ints)
+
+    def append():
+        B.paged_append(hk, hk, kp, vp, table, starts, lens, q=hq, q_out=q_out)
+
+    def product():
+        return B.to_numpy(B.linear(B.reshape(q_out, (new, nh * d)), eye))   # (a bf16 weight: the operand is rounded)
+
+    append()
+    assert np.array_equal(product(), rounded(q.cpu().numpy(), "bf16").reshape(new, -1))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=S, capture_error_mode="relaxed"):
+        append()
+    for _ in range(2):
+        with torch.cuda.stream(S):
+            q.copy_(torch.randn(new, nh, d, generator=gen, device="cuda"))
+            g.replay()
+        S.synchronize()
+        assert np.array_equal(product(), rounded(q.cpu().numpy(), "bf16").reshape(new, -1))
+    B.close()
+    B = cuda
+    # one beam, one group: a literal is its score, and a view of it is read as another type
+    score = B.ndarray_from_vec_f32([7.0], (1, 1))
+    view = B.reshape(score, (1,))
+    outs = [B.zeros((1, 1), cg.U32) for _ in range(3)]
+    B.beam_select(B.from_numpy(np.zeros((1, 1, 1), np.float32)), score, 1, out=(score, *outs))
+    assert B.to_numpy(score)[0, 0] == 7.0
+    B.beam_select(B.from_numpy(np.array([[[3.0, 3.0, 3.0, 3.0]]], np.float32)), score, 1, out=(score, *outs))
+    want = np.float32(7 - math.log(4))
+    assert abs(B.to_numpy(score)[0, 0] - want) <= 8 * 2.0 ** -24 * 7
+    for t in (view, B.reshape(score, (1,))):
+        assert B.to_numpy(B.cast(t, cg.U32))[0] == int(want) == 5
 
 
 @gpu
