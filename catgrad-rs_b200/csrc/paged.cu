@@ -32,7 +32,7 @@ __device__ __forceinline__ float load1(const __nv_bfloat16* p) { return __bfloat
 __device__ __forceinline__ void store1(float* p, float x) { *p = x; }
 __device__ __forceinline__ void store1(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
-// A warp per vector (a head of a token); a lane has pairs lane, lane + 32, ..: with `rot_half` pair i < half is components
+// Every head size and alignment (k_paged_append_vec takes the usual ones; its long case below takes 225 us here).  A warp per vector (a head of a token); a lane has pairs lane, lane + 32, ..: with `rot_half` pair i < half is components
 // (i, i + half), else (2 i, 2 i + 1); pairs from `half` on are (2 i, 2 i + 1) and not turned.
 template <typename TI, typename TO>
 __global__ void __launch_bounds__(256) k_paged_append(AppendArgs a) {
@@ -151,6 +151,11 @@ struct Eight<__nv_bfloat16> {
 // The same for head sizes 16 G, G a power of two, aligned vectors and angles in eights: G lanes have a vector, each two pieces of eight values,
 // which are the two sides of its eight pairs (with `rot_half` where they turn), or 16 neighbours.  A warp has one of `parts` shares of a
 // token's heads, U times 32 / G of them, all on their way before the token's row is looked up.
+//
+// Bytes should bound it (read once, written once); what does is the instructions per value (widen, square, two factors of the norm,
+// four of the turn, round).  6 rows of up to 2903 tokens, 32 + 2 x 4 heads of 128 with norms, bf16: 251 MB in 56.8 us, 4.4 TB/s.  The steps
+// there, from 225 us: vectors in eights 77, all of a lane's vectors on their way at once 62, neighbouring heads in a warp, so that
+// gains stay in registers, 57.  Of a single step's tokens the call's 4.9 us are all.
 template <typename TI>
 constexpr int append_vectors() { return sizeof(TI) == 2 ? 4 : 2; }
 template <typename TI, typename TO, int G>
@@ -283,7 +288,8 @@ struct ReorderArgs {
 
 // Group blockIdx.y.  All of a group's copies go through the registers of the thread that makes them: it has read the K sources of
 // its 16 bytes before it writes them, so pages may change places.  The sources are the parents' own pages, which nobody
-// else's targets are.  What bounds it is the bytes; a block looks its group up once and then has pieces of all layers.
+// else's targets are.  What bounds it is the bytes; a block looks its group up once and then has pieces of all layers.  12 groups of 8
+// beams, 8 layers of 8 heads of 128: 77 MB in 18.4 us, 4.2 TB/s (with the call's 3.8 us, which is all that one group of 4 takes).
 template <int KM>
 __global__ void __launch_bounds__(256) k_paged_reorder(ReorderArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");

@@ -7,6 +7,9 @@
 //   O^T [d, rows] += V^T P^T   (S's accumulators are P^T's fragments; 8 rows fill the 8 columns)
 // What bounds it is the bytes of the cache, and for short contexts the chain tables -> page table -> keys -> product -> joining.
 //
+// 7 rows of up to 32002 tokens, 32 heads and 8 key heads of 128: 623 MB in 98.8 us, 6.3 TB/s, 0.96 of a copy.  8 rows of 578, heads of 64:
+// 7.4 us, of which some 4 are the call.  (A warp per query with plain loads: 1194 and 36.7 us.)
+//
 // Probabilities are split into two bf16 parts (the second product costs nothing where bytes bound the kernel), so that the output is
 // rounded once.  Exponents' references lag behind the maxima by up to 2^8, so that tiles need no shuffles.
 #include <algorithm>
