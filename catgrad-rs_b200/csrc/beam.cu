@@ -15,8 +15,8 @@
 // A group of beams is a thread-block cluster, over whose blocks, each of up to four times 256 threads, the pieces of its beams are
 // dealt; a warp then joins all sorted lists of a beam, and one warp those of the beams.
 //
-// 24 groups of 8 beams over 256000 tokens in bf16: 98 MB in 48 us.  That is 2 TB/s on 96 SMs (24 clusters of 4 blocks of 1024 threads), which
-// issue some ten instructions per value.  One group of 4 beams over 128256 in f32: 9.7 us, a chain of loads, barriers and joins behind a call of 4.
+// 24 groups of 8 beams over 256000 tokens in bf16: 98 MB in 43.7 us, 2.2 TB/s (24 clusters of 10 blocks of 512 threads, two blocks on most SMs):
+// some ten instructions per value, and rounds that end at barriers.  One group of 4 beams over 128256 in f32: 9.7 us, a chain of loads, barriers and joins behind a call of 4.
 //
 // Exponentials are f32, their sums over more than a warp, the logarithm and the totals 64 bits: totals of different
 // beams may lie close together.
@@ -663,11 +663,16 @@ int launch_select(cg_ctx* c, SelectArgs a, int64_t B) {
   if (pieces > 32 * MAX_OWN) return fail(c, CG_ERR_UNSUPPORTED, "vocabulary too large");
   a.pieces = (int)pieces;
   // Blocks of a group and times 256 threads of a block: what takes the least time by rounds of pieces, a round being a chain of
-  // 1.5 us and 0.7 per 256 threads that an SM has.
+  // 1.5 us and 0.4 per 256 threads that an SM has.  Us for blocks x times, of the ten numbers of blocks and three of times, the rule's first:
+  //   24 groups of 8 over 256000 in bf16    10 x 2: 43.6    4 x 4: 47.6   16 x 1: 48.1   8 x 2: 48.5   5 x 2: 52.5
+  //   1 of 4 over 128256 in f32             16 x 4: 9.8    16 x 2: 10.3   8 x 4: 12.6   10 x 2: 14.0
+  //   64 of 4 over 32000                     4 x 2: 12.9    2 x 4: 12.9    8 x 1: 13.4   2 x 2: 15.0
+  //   190 of 1 over 50257 in bf16            1 x 2: 13.8    2 x 1: 14.9    1 x 1: 16.3   4 x 1: 17.5
+  //   12 of 8 over 151936 in bf16           16 x 2: 22.2    8 x 4: 22.1   6 x 4: 25.5   10 x 2: 25.9
   int best_ranks = 0, best_sb = 1;
   double best = 1e300;
   const int device = c->core->device;
-  for (int ranks : {1, 2, 3, 4, 5, 6, 8, 12, 16})
+  for (int ranks : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16})
     for (int sb : {1, 2, 4}) {
       if (ranks * sb > 1 && (ranks * sb + 1) / 2 >= units + 1) continue;
       const int n = sb == 1 ? Blocks<T, 1>::at_a_time(device, ranks) : sb == 2 ? Blocks<T, 2>::at_a_time(device, ranks) : Blocks<T, 4>::at_a_time(device, ranks);
@@ -675,7 +680,7 @@ int launch_select(cg_ctx* c, SelectArgs a, int64_t B) {
       const double waves = (double)((B + n - 1) / n), rounds = (double)((units + ranks * sb - 1) / (ranks * sb));
       if (rounds * sb * a.K * 8 > 100 * 1024) continue;
       const double per_sm = std::max((double)sb, (double)(std::min<int64_t>(B, n) * ranks * sb) / 148.);
-      const double cost = waves * rounds * (1.5 + 0.7 * per_sm) + 0.1 * ranks;
+      const double cost = waves * rounds * (1.5 + 0.4 * per_sm) + 0.1 * ranks;
       if (cost < best) {
         best = cost;
         best_ranks = ranks;
