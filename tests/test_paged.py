@@ -1018,3 +1018,14 @@ def test_rows_that_cannot_be_are_not_followed(host):
     table, err = np.uint32([3, 9, 10, 0xFFFFFFFF, 0, 1, 2, 4]), np.zeros(1, np.int32)
     got = [host.host_page_of(vp(table), 4, 10, 4, r, p, vp(err)) for r in (0, 1) for p in (0, 15, 16, 31, 63, 47)]
     assert got == [3, 3, 9, 9, -1, -1, 0, 0, 1, 1, 4, 2] and err[0] == 1
+
+
+def test_prompt_attention_takes_tmem_between_its_dependency_and_its_trigger():
+    """After the wait no earlier kernel holds columns, and before the trigger no later one runs that could hold what this one waits for.
+    Blocks without tokens leave before they take any."""
+    text = open(os.path.join(os.path.dirname(cg.__file__), "csrc", "paged_fa.cu")).read()
+    body = text[text.index("k_paged_fa(const __grid_constant__"):]
+    body = body[:body.index("\n}\n")]
+    order = ["griddepcontrol.wait;", "if (i0 >= n) return;", "tcgen05.alloc.", "griddepcontrol.launch_dependents;", "tcgen05.dealloc."]
+    assert all(body.count(x) == 1 for x in order)
+    assert [body.index(x) for x in order] == sorted(body.index(x) for x in order)
