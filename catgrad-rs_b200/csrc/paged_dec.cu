@@ -65,29 +65,38 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncthreads();
+  // (query rows fit into 31 bits, and the blocks of a cluster are a power of two)
+  const uint32_t kvh = blockIdx.x % (uint32_t)p.nkv, x0 = blockIdx.x / (uint32_t)p.nkv * ROWS, rep = (uint32_t)p.rep;
+  const uint32_t i0 = x0 / rep, i_end = (x0 + ROWS - 1) / rep;
+  const int64_t row = blockIdx.y;
+  const int slices = (int)gridDim.z, slice = (int)blockIdx.z, lg_slices = 31 - __clz(slices);
+  const int lg = p.rows.lg, box = min(1 << lg, KT), parts = KT / box;
+  const int my_part = lane % parts, my_sub = lane / parts % SUB, my_pool = lane / (parts * SUB);  // (keys, values; others have nothing)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  const int kvh = (int)blockIdx.x % p.nkv;
-  const int64_t row = blockIdx.y, x0 = (int64_t)(blockIdx.x / p.nkv) * ROWS;
-  const int slices = (int)gridDim.z, slice = (int)blockIdx.z;
   int64_t tok0, n, len;
-  if (!row_span(p.rows, row, p.most, &tok0, &n, &len) || x0 >= n * p.rep) return;  // (the same in all blocks of a cluster)
-  const int64_t pos0 = len - n, i0 = x0 / p.rep, i1 = min(n - 1, (x0 + ROWS - 1) / p.rep);
+  if (!row_span(p.rows, row, p.most, &tok0, &n, &len) || x0 >= n * rep) return;  // (the same in all blocks of a cluster)
+  const int64_t pos0 = len - n, i1 = min(n - 1, (int64_t)i_end);
   const int64_t lo = p.window > 0 ? max((int64_t)0, pos0 + i0 - p.window + 1) : 0, hi = pos0 + i1;
-  const int64_t first = lo / KT, tiles = hi / KT + 1 - first, share = (tiles + slices - 1) / slices;
+  const int64_t first = (int64_t)((uint64_t)lo / KT), tiles = (int64_t)((uint64_t)hi / KT) + 1 - first, share = (tiles + slices - 1) >> lg_slices;
   const int64_t end = min(first + tiles, first + (slice + 1) * share);
 
   // A lane has a box of a tile: 64 components of a page's keys or values (of the whole tile's, if pages are longer).  Pages without a
   // visible key are not looked up and read as zeros (a box behind the pool's end).
-  const int lg = p.rows.lg, box = min(1 << lg, KT), parts = KT / box;
-  const int my_part = lane % parts, my_sub = lane / parts % SUB, my_pool = lane / (parts * SUB);  // (keys, values; others have nothing)
   const int off_end = (int)p.pool_rows;
-  auto place = [&](int64_t t) {
+  const uint32_t* pages = p.rows.table + row * p.rows.cols;
+  // (asked for apart from what is made of it: several are on their way at once)
+  auto ask = [&](int64_t t) {
     const int64_t key = t * KT + my_part * box;
-    if (key > hi || key + box <= lo) return off_end;
-    const int64_t id = page_of(p.rows, row, key);
-    return id < 0 ? off_end : (int)(((id * p.nkv + kvh) << lg) + (key & ((1 << lg) - 1)));
+    return t < end && key <= hi && key + box > lo ? (int64_t)pages[key >> lg] : (int64_t)-1;
+  };
+  auto place = [&](int64_t t, int64_t id) {
+    if (id >= p.rows.n_pages) {
+      *p.rows.err = DEV_INDEX;
+      id = -1;
+    }
+    return id < 0 ? off_end : (int)(((id * p.nkv + kvh) << lg) + ((t * KT + my_part * box) & ((1 << lg) - 1)));
   };
   auto request = [&](int stage, int at) {
     const uint32_t bar = bars + 8 * stage;
@@ -97,15 +106,15 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
       tma_load_2d(ring + stage * (2 * TILE) + my_pool * TILE + my_sub * BOX + my_part * box * 128, my_pool ? &map_v : &map_k, my_sub * 64, at, bar);
   };
   int64_t t = first + slice * share + warp;
-  int ahead_at = off_end;  // place of the tile that is asked for next
+  int64_t ahead_id;  // page of the tile that is asked for next
   {
-    int at[RING];
+    int64_t id[RING + 1];
 #pragma unroll
-    for (int i = 0; i < RING; ++i) at[i] = t + 4 * i < end ? place(t + 4 * i) : off_end;
+    for (int i = 0; i <= RING; ++i) id[i] = ask(t + 4 * i);
 #pragma unroll
     for (int i = 0; i < RING; ++i)
-      if (t + 4 * i < end) request(i, at[i]);
-    if (t + 4 * RING < end) ahead_at = place(t + 4 * RING);
+      if (t + 4 * i < end) request(i, place(t + 4 * i, id[i]));
+    ahead_id = id[RING];
   }
 
   // rows g and g + 8 of the tile
@@ -113,10 +122,10 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
   int64_t qpos[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    const int64_t x = x0 + g + 8 * b, i = x / p.rep;
-    const bool there = x < n * p.rep;
+    const uint32_t x = x0 + g + 8 * b, i = x / rep;
+    const bool there = x < n * rep;
     qpos[b] = pos0 + i;
-    const __nv_bfloat16* src = p.q + (tok0 + (there ? i : 0)) * p.q_ld + (kvh * p.rep + (there ? x % p.rep : 0)) * p.q_hs;
+    const __nv_bfloat16* src = p.q + (tok0 + (there ? i : 0u)) * p.q_ld + (int64_t)(kvh * rep + (there ? x - i * rep : 0u)) * p.q_hs;
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
       const int c = k * 16 + t2;
@@ -139,7 +148,7 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
   for (; t < end; t += 4, ++it) {
     const int stage = it % RING;
     const int64_t ahead = t + 4 * RING;
-    const int next = ahead + 4 < end ? place(ahead + 4) : off_end;  // (a whole round before it is asked for)
+    const int64_t next = ask(ahead + 4);  // (a whole round before it is asked for)
     ok = __all_sync(0xffffffffu, mbar_wait(bars + 8 * stage, (uint32_t)(it / RING) & 1u, &aborted, p.rows.err));
     if (!ok) break;
     const uint32_t kt = ring + stage * (2 * TILE), vt = kt + TILE;
@@ -235,8 +244,8 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
         }
       }
     __syncwarp();
-    if (ahead < end) request(stage, ahead_at);
-    ahead_at = next;
+    if (ahead < end) request(stage, place(ahead, ahead_id));
+    ahead_id = next;
   }
   if (!ok) {  // copies on their way are waited for: what lies over the ring is written next
     for (int i = 0; i < RING && t + 4 * i < end; ++i) mbar_drain(bars + 8 * ((it + i) % RING), (uint32_t)((it + i) / RING) & 1u, p.rows.err);
@@ -258,7 +267,7 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
 #pragma unroll
       for (int e = 0; e < 4; ++e) red_o[(warp * ROWS + b * 8 + t2 + (e & 1)) * LD + k * 16 + g + (e >> 1) * 8] = o[k][b][e];
   __syncthreads();
-  auto out_at = [&](int64_t x) { return p.out + ((tok0 + x / p.rep) * p.nh + kvh * p.rep + x % p.rep) * (int64_t)p.d; };
+  auto out_at = [&](uint32_t x) { return p.out + ((tok0 + x / rep) * p.nh + kvh * rep + x % rep) * (int64_t)p.d; };
   for (int i = tid; i < ROWS * (D / 4); i += 128) {
     const int r = i / (D / 4), c = i % (D / 4) * 4;
     const float top = fmaxf(fmaxf(red_m[0][r], red_m[1][r]), fmaxf(red_m[2][r], red_m[3][r])), mc = top == -INFINITY ? 0.f : top;
@@ -274,7 +283,7 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
     if (slices > 1) {
       *(float4*)(part + r * LD + c) = v;
       if (c == 0) { cta_m[r] = top; cta_l[r] = sum; }
-    } else if (x0 + r < n * p.rep && c < p.d && !aborted) {
+    } else if (x0 + r < n * rep && c < p.d && !aborted) {
       const float f = sum > 0.f ? 1.f / sum : 0.f;
       *(uint2*)(out_at(x0 + r) + c) = make_uint2(pack_bf16(v.x * f, v.y * f), pack_bf16(v.z * f, v.w * f));
     }
@@ -283,28 +292,39 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
 
   // ---- the blocks' shares: each finishes some of the values ----
   cluster_sync_all();
-  const int rows = (int)min((int64_t)ROWS, n * p.rep - x0);
-  for (int i = slice * 128 + tid; i < rows * (D / 4); i += 128 * slices) {
+  const int rows = (int)min((int64_t)ROWS, n * rep - x0);
+  for (int i = tid * slices + slice; i < rows * (D / 4); i += 128 * slices) {
     const int r = i / (D / 4), c = i % (D / 4) * 4;
-    float ms[16], top = -INFINITY;
-#pragma unroll
-    for (int s = 0; s < 16; ++s) {
-      ms[s] = s < slices ? ld_cluster_f32(smem_u32(&cta_m[r]), (uint32_t)s) : -INFINITY;
-      top = fmaxf(top, ms[s]);
-    }
-    const float mc = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
+    // (four shares on their way at a time)
+    float top = -INFINITY, sum = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = 0; s0 < slices; s0 += 4) {
+      float ms[4], ls[4];
+      float4 us[4];
 #pragma unroll
-    for (int s = 0; s < 16; ++s) {
-      if (s >= slices) break;
-      const float f = fast_exp2(ms[s] - mc);
-      uint32_t at;
-      float4 u;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(part + r * LD + c)), "r"(s));
-      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(u.x), "=f"(u.y), "=f"(u.z), "=f"(u.w) : "r"(at) : "memory");
-      sum = fmaf(ld_cluster_f32(smem_u32(&cta_l[r]), (uint32_t)s), f, sum);
-      v.x = fmaf(u.x, f, v.x); v.y = fmaf(u.y, f, v.y); v.z = fmaf(u.z, f, v.z); v.w = fmaf(u.w, f, v.w);
+      for (int s = 0; s < 4; ++s) {
+        ms[s] = -INFINITY;
+        ls[s] = 0.f;
+        us[s] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (s0 + s < slices) {
+          uint32_t at;
+          ms[s] = ld_cluster_f32(smem_u32(&cta_m[r]), (uint32_t)(s0 + s));
+          ls[s] = ld_cluster_f32(smem_u32(&cta_l[r]), (uint32_t)(s0 + s));
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(part + r * LD + c)), "r"(s0 + s));
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(us[s].x), "=f"(us[s].y), "=f"(us[s].z), "=f"(us[s].w) : "r"(at) : "memory");
+        }
+      }
+      const float before = top;
+      top = fmaxf(fmaxf(fmaxf(top, ms[0]), fmaxf(ms[1], ms[2])), ms[3]);
+      const float mc = top == -INFINITY ? 0.f : top, f0 = fast_exp2(before - mc);
+      sum *= f0;
+      v.x *= f0; v.y *= f0; v.z *= f0; v.w *= f0;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const float f = fast_exp2(ms[s] - mc);
+        sum = fmaf(ls[s], f, sum);
+        v.x = fmaf(us[s].x, f, v.x); v.y = fmaf(us[s].y, f, v.y); v.z = fmaf(us[s].z, f, v.z); v.w = fmaf(us[s].w, f, v.w);
+      }
     }
     if (c < p.d && !aborted) {
       const float f = sum > 0.f ? 1.f / sum : 0.f;
@@ -371,7 +391,7 @@ int pick(cg_ctx* c, const PagedAttnArgs& a) {
 }  // namespace
 
 bool paged_dec_supported(const PagedAttnArgs& a) {
-  return ((a.rows.n_pages * a.nkv) << a.rows.lg) < 0x7FFFFFFFll && (a.most * (a.nh / a.nkv) + 7) / 8 * a.nkv < 0x7FFFFFFFll && ((uintptr_t)a.q % 4) == 0 &&
+  return ((a.rows.n_pages * a.nkv) << a.rows.lg) < 0x7FFFFFFFll && (a.most * (a.nh / a.nkv) + 7) / 8 * a.nkv < 0x7FFFFFFFll && ((uintptr_t)a.q % 4) == 0 && a.most * (a.nh / a.nkv) < 0x7FFFFF00ll &&
          ((uintptr_t)a.out % 8) == 0 && a.q_ld % 2 == 0 && a.q_hs % 2 == 0;
 }
 
