@@ -529,8 +529,14 @@ __global__ void __launch_bounds__(SB * BT, 4 / SB) k_beam_select(SelectArgs a) {
           const uint32_t r = (uint32_t)(block - round * (int)n_ranks), from = remote_addr(lists + at * K, r);
           asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[i]) : "r"(remote_addr(tops + at, r)) : "memory");
           part[i] = __longlong_as_double((long long)remote_ld64(remote_addr(sums + at, r)));
-#pragma unroll 4
-          for (int k = 0; k < K; ++k) mine[p * K + k] = remote_ld64(from + (uint32_t)k * 8u);
+          for (int k = 0; k < K; k += 4) {  // (four on their way at a time)
+            uint64_t four[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) four[q] = k + q < K ? remote_ld64(from + (uint32_t)(k + q) * 8u) : 0;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (k + q < K) mine[p * K + k + q] = four[q];
+          }
           m = fmaxf(m, v[i]);
         }
       }
@@ -587,20 +593,23 @@ __global__ void __launch_bounds__(SB * BT, 4 / SB) k_beam_select(SelectArgs a) {
 
   // the best of the beams' sorted totals: a lane has a beam
   if (rank == 0 && threadIdx.x < 32) {
-    int at = 0;
+    int at = 0, beam = 0, place = 0;  // lane r keeps the r-th best's beam, and its place there
+    uint64_t total = 0;
     for (int r = 0; r < K; ++r) {
       const uint64_t key = lane < J && at < K ? totals[lane * K + at] : 0;
       int who;
       const uint64_t best = warp_best(key, &who);  // (of equal totals the lowest beam's)
-      if (lane == who) {
-        const uint32_t token = (uint32_t)(places[lane * K + at] - (uint64_t)lane * (uint64_t)a.V);
-        ++at;
-        const int64_t to = b * K + r;
-        a.out_scores[to] = (float)down64(best);
-        a.out_tokens[to] = token;
-        a.out_parents[to] = (uint32_t)lane;
-        a.out_finished[to] = marks[lane] || token == a.end;
-      }
+      const int from = __shfl_sync(0xffffffffu, at, who);
+      if (lane == r) { beam = who; place = from; total = best; }
+      if (lane == who) ++at;
+    }
+    if (lane < K) {
+      const uint32_t token = (uint32_t)(places[beam * K + place] - (uint64_t)beam * (uint64_t)a.V);
+      const int64_t to = b * K + lane;
+      a.out_scores[to] = (float)down64(total);
+      a.out_tokens[to] = token;
+      a.out_parents[to] = (uint32_t)beam;
+      a.out_finished[to] = marks[beam] || token == a.end;
     }
   }
 }
