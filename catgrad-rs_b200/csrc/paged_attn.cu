@@ -26,10 +26,10 @@ __device__ __forceinline__ float load_as(const float* p) { return *p; }
 __device__ __forceinline__ float load_as(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
 // An f32 as the sum of two tf32 values of 11 bits, operands of the tensor cores.  The upper one is rounded to nearest (an infinity stays
-// one, near the largest value it may become one), so that the lower one, cut off, has either sign.
+// one, near the largest value it may become one), so that the lower one has either sign; of that the product reads the upper 11 bits.
 __device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
   hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
-  lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
+  lo = __float_as_uint(x - __uint_as_float(hi));
 }
 __device__ __forceinline__ void mma_tf32(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -213,19 +213,44 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
     }
     // (scores and maxima in units of log2)
     const bool masked = k0 + GK / WK - 1 > pos0 + i0 || k0 < lo || (a.window > 0 && k0 <= hi - a.window);
+    // (conditions stand around the loops: one per score would cut them up)
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[i][e] += less[i][e];
+    if (a.cap > 0.f) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[i][e] = soft_cap(s[i][e], cap2, cap_in, cap_unit);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[i][e] *= scale;
+    }
+    if (masked) {
+      // key k0 + x is visible to row q iff low <= x <= lim
+      int low[2], lim[2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int64_t x = qpos[q] - k0;
+        lim[q] = x > GK ? GK : x < -1 ? -1 : (int)x;
+        low[q] = a.window > 0 ? (x - a.window >= GK ? GK : x - a.window < -1 ? 0 : (int)(x - a.window) + 1) : 0;
+      }
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int x = i * 8 + 2 * t4 + (e & 1);
+          s[i][e] = x <= lim[e >> 1] && x >= low[e >> 1] ? s[i][e] : -INFINITY;
+        }
+    }
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float x = s[i][e] + less[i][e];
-        if (a.cap > 0.f) x = soft_cap(x, cap2, cap_in, cap_unit);
-        else x *= scale;
-        const int64_t key = k0 + i * 8 + 2 * t4 + (e & 1), pos = qpos[e >> 1];
-        if (masked && (key > pos || (a.window > 0 && key <= pos - a.window))) x = -INFINITY;
-        s[i][e] = x;
-        top[e >> 1] = fmaxf(top[e >> 1], x);
-      }
+      for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], s[i][e]);
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       top[q] = fmaxf(top[q], __shfl_xor_sync(0xffffffffu, top[q], 1));
