@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
     float s[NT][4], less[NT][4];  // (the small products apart)
 #pragma unroll
     for (int i = 0; i < NT; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = less[i][0] = less[i][1] = less[i][2] = less[i][3] = 0.f;
-#pragma unroll 2
+#pragma unroll (D == 64 ? 4 : 2)
     for (int c = 0; c < D; c += 16) {  // components c + 4 t4 .. + 3: places t4 and t4 + 4 of two products
       uint32_t ah[2][4], al[2][4];
 #pragma unroll
@@ -198,17 +198,21 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
         ah[0][q] = h.x; ah[0][2 + q] = h.y; ah[1][q] = h.z; ah[1][2 + q] = h.w;
         al[0][q] = w.x; al[0][2 + q] = w.y; al[1][q] = w.z; al[1][2 + q] = w.w;
       }
+      // (products with the same sum as far apart as there are sums)
+      uint32_t h[NT][4], w[NT][4];
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         const float4 k = *(const float4*)(ks + (i * 8 + g) * LK + c + 4 * t4);
-        uint32_t h[4], w[4];
-        split(k.x, h[0], w[0]); split(k.y, h[1], w[1]); split(k.z, h[2], w[2]); split(k.w, h[3], w[3]);
+        split(k.x, h[i][0], w[i][0]); split(k.y, h[i][1], w[i][1]); split(k.z, h[i][2], w[i][2]); split(k.w, h[i][3], w[i][3]);
+      }
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          mma_tf32(less[i], al[u], h[2 * u], h[2 * u + 1]);
-          mma_tf32(less[i], ah[u], w[2 * u], w[2 * u + 1]);
-          mma_tf32(s[i], ah[u], h[2 * u], h[2 * u + 1]);
-        }
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) mma_tf32(less[i], al[u], h[i][2 * u], h[i][2 * u + 1]);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) mma_tf32(s[i], ah[u], h[i][2 * u], h[i][2 * u + 1]);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) mma_tf32(less[i], ah[u], w[i][2 * u], w[i][2 * u + 1]);
       }
     }
     // (scores and maxima in units of log2)
@@ -293,15 +297,18 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
       for (int i = 0; i < NT; ++i) {
         const float4 v0 = *(const float4*)(vs + (i * 8 + 2 * t4) * LV + 32 * c + 4 * g), v1 = *(const float4*)(vs + (i * 8 + 2 * t4 + 1) * LV + 32 * c + 4 * g);
         const float b0[4] = {v0.x, v0.y, v0.z, v0.w}, b1[4] = {v1.x, v1.y, v1.z, v1.w};
+        uint32_t h0[4], w0[4], h1[4], w1[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          uint32_t h0, w0, h1, w1;
-          split(b0[j], h0, w0);
-          split(b1[j], h1, w1);
-          mma_tf32(sum[j], pl[i], h0, h1);
-          mma_tf32(sum[j], ph[i], w0, w1);
-          mma_tf32(sum[j], ph[i], h0, h1);
+          split(b0[j], h0[j], w0[j]);
+          split(b1[j], h1[j], w1[j]);
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mma_tf32(sum[j], pl[i], h0[j], h1[j]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mma_tf32(sum[j], ph[i], w0[j], w1[j]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mma_tf32(sum[j], ph[i], h0[j], h1[j]);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j)
