@@ -15,8 +15,8 @@
 // A group of beams is a thread-block cluster, over whose blocks, each of up to four times 256 threads, the pieces of its beams are
 // dealt; a warp then joins all sorted lists of a beam, and one warp those of the beams.
 //
-// 24 groups of 8 beams over 256000 tokens in bf16: 98 MB in 43.7 us, 2.2 TB/s (24 clusters of 10 blocks of 512 threads, two blocks on most SMs):
-// some ten instructions per value, and rounds that end at barriers.  One group of 4 beams over 128256 in f32: 9.7 us, a chain of loads, barriers and joins behind a call of 4.
+// 24 groups of 8 beams over 256000 tokens in bf16: 98 MB in 42.4 us, 2.3 TB/s (24 clusters of 10 blocks of 512 threads, two blocks on most SMs):
+// some ten instructions per value, and rounds that end at barriers.  One group of 4 beams over 128256 in f32: 9.3 us, a chain of loads, barriers and joins behind a call of 4.
 //
 // Exponentials are f32, their sums over more than a warp, the logarithm and the totals 64 bits: totals of different
 // beams may lie close together.

@@ -42,7 +42,8 @@ __device__ __forceinline__ void mma_tf32(float* c, const uint32_t* a, uint32_t b
 // 11 bits, and three of the four products are summed in f32: what is left out is 2^-24 of a product.  The tensor cores cut sums off
 // instead of rounding them, so sums over more than a tile are made outside.  Error against 64 bits, 3 rows of up to 1713
 // tokens, heads of 64: 6.7e-7, of f32 sums 8.3e-7 (with one accumulator for all 2.1e-6, with parts cut off 3.1e-6).  On the
-// CUDA cores the same tiles are bound by shared memory, eight vectors for 16 x 4 products of a thread: 43 us, here 32.
+// CUDA cores the same tiles are bound by shared memory, eight vectors for 16 x 4 products of a thread: 43 us, here 29.8 (of which two blocks on
+// an SM take 6700 clocks for a tile of each, 3000 of them for Q K^T: loads, splitting and products share the schedulers).
 //
 // A block has QR queries of one row and key head (query x is token x / rep, head x % rep of the group) and a share of the visible
 // keys, GK at a time; its four warps share the rows (QR = 64) or the keys (QR = 16) of a tile, 16 rows each.  The blocks of a

@@ -7,8 +7,9 @@
 //   O^T [d, rows] += V^T P^T   (S's accumulators are P^T's fragments; 8 rows fill the 8 columns)
 // What bounds it is the bytes of the cache, and for short contexts the chain tables -> page table -> keys -> product -> joining.
 //
-// 7 rows of up to 32002 tokens, 32 heads and 8 key heads of 128: 623 MB in 98.8 us, 6.3 TB/s, 0.96 of a copy.  8 rows of 578, heads of 64:
-// 7.4 us, of which some 4 are the call.  (A warp per query with plain loads: 1194 and 36.7 us.)
+// 7 rows of up to 32002 tokens, 32 heads and 8 key heads of 128: 623 MB in 100 us, 6.2 TB/s, 0.95 of a copy.  8 rows of 578, heads of 64:
+// 6.4 us (7.4 while a page's number was waited for before the next one was asked for, and one block of a cluster joined all).  A warp per
+// query with plain loads: 1194 and 36.7 us.
 //
 // Probabilities are split into two bf16 parts (the second product costs nothing where bytes bound the kernel), so that the output is
 // rounded once.  Exponents' references lag behind the maxima by up to 2^8, so that tiles need no shuffles.
@@ -365,7 +366,7 @@ int launch(cg_ctx* c, const PagedAttnArgs& a) {
   CG_TRY(make_map(c, &mk, a.k_pages, p.pool_rows, a.d, a.d, box));
   CG_TRY(make_map(c, &mv, a.v_pages, p.pool_rows, a.d, a.d, box));
   const int64_t groups = (a.most * p.rep + ROWS - 1) / ROWS * a.nkv, longest = a.rows.cols << a.rows.lg;
-  // Shares of the keys.  Us with 1 / 2 / 4 / 8 / 16, [the rule's]:
+  // Shares of the keys.  Us with 1 / 2 / 4 / 8 / 16, [the rule's] (with a joining that took about 1 us more):
   //   8 rows x 8 key heads, 578 keys, d 64      8.7   8.2 [7.4]  13.5  37
   //   8 x 8, 2000, d 128                       29.4  19.7 [16.8] 23.8  48
   //   1 x 8, 4096, d 128                       52.2  29.9  18.0  12.5 [11.5]
