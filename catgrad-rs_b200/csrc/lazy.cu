@@ -802,9 +802,14 @@ void plan(cg_ctx* c) {
 // ------------------------------------------------------------------------------------------
 // recorders
 
+// A tensor whose memory may change before what is recorded runs, without a call that would run it first: the caller's own memory, and
+// what an operator has written in place (a captured graph may do so again).  It is read when the call is made.
+static bool read_now(const cg_tensor* t) { return t && !t->node && t->buf && (!t->buf->owned || t->buf->rewritten); }
+
 bool lazy_binary(cg_ctx* c, int op, const cg_tensor* a, const cg_tensor* b, cg_tensor** out, int* st) {
   if (a->tag != b->tag) { *st = fail(c, CG_ERR_DTYPE, "mixed dtypes in binary operation"); return true; }
   if (!same_shape(a, b)) { *st = fail(c, CG_ERR_SHAPE, "Shape mismatch in operation"); return true; }
+  if (read_now(a) || read_now(b)) return false;
   cg_tensor* t = pending_tensor(c, a->tag, a->dims, a->rank);
   static const int map[] = {LZ_ADD, LZ_SUB, LZ_MUL, LZ_DIV, LZ_POW, LZ_LT};
   add_node(c, map[op], t, a, b);
@@ -814,6 +819,7 @@ bool lazy_binary(cg_ctx* c, int op, const cg_tensor* a, const cg_tensor* b, cg_t
 }
 
 bool lazy_unary_neg(cg_ctx* c, const cg_tensor* x, cg_tensor** out, int* st) {
+  if (read_now(x)) return false;
   cg_tensor* t = pending_tensor(c, x->tag, x->dims, x->rank);
   add_node(c, LZ_NEG, t, x, nullptr);
   *out = t;
@@ -823,6 +829,7 @@ bool lazy_unary_neg(cg_ctx* c, const cg_tensor* x, cg_tensor** out, int* st) {
 
 bool lazy_reduce(cg_ctx* c, int red, const cg_tensor* x, cg_tensor** out, int* st) {
   if (x->dims[x->rank - 1] >= (1ll << 32)) return false;  // the eager path reports it
+  if (read_now(x)) return false;
   int64_t od[CG_MAX_RANK];
   for (int i = 0; i < x->rank; ++i) od[i] = x->dims[i];
   od[x->rank - 1] = 1;
@@ -835,6 +842,7 @@ bool lazy_reduce(cg_ctx* c, int red, const cg_tensor* x, cg_tensor** out, int* s
 
 bool lazy_cast(cg_ctx* c, const cg_tensor* x, int dtype, cg_tensor** out, int* st) {
   if (!x->node && x->literal()) return false;  // a literal: cast it now so its value stays known
+  if (read_now(x)) return false;
   cg_tensor* t = pending_tensor(c, dtype, x->dims, x->rank);
   LazyNode* n = add_node(c, LZ_CAST, t, x, nullptr);
   n->a[0] = dtype;
@@ -849,6 +857,7 @@ bool lazy_matmul(cg_ctx* c, const cg_tensor* a, const cg_tensor* b, cg_tensor** 
   if (a->tag != b->tag || ra < 2 || rb < 2 || ra != rb || a->dims[ra - 1] != b->dims[rb - 2]) return false;  // eager reports
   for (int i = 0; i < ra - 2; ++i)
     if (a->dims[i] != b->dims[i]) return false;
+  if (read_now(a) || read_now(b)) return false;
   int64_t od[CG_MAX_RANK];
   for (int i = 0; i < ra - 2; ++i) od[i] = a->dims[i];
   od[ra - 2] = a->dims[ra - 2];
@@ -865,6 +874,7 @@ bool lazy_concat(cg_ctx* c, const cg_tensor* a, const cg_tensor* b, int dim, cg_
   if (a->tag != b->tag || a->rank != b->rank || dim < 0 || dim >= a->rank) return false;  // eager reports
   for (int i = 0; i < a->rank; ++i)
     if (i != dim && a->dims[i] != b->dims[i]) return false;
+  if (read_now(a) || read_now(b)) return false;
   int64_t od[CG_MAX_RANK];
   for (int i = 0; i < a->rank; ++i) od[i] = a->dims[i];
   od[dim] += b->dims[dim];

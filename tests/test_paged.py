@@ -826,6 +826,56 @@ def test_recorded_mode_and_two_contexts(cuda):
 
 
 @gpu
+def test_recorded_calls_read_the_callers_memory_when_they_are_made():
+    """Recorded mode: the caller's memory, and what a replayed graph writes, may change before a recorded call would run."""
+    import torch
+    S = torch.cuda.Stream()
+    L = cg.CudaBackend(0, cg.PREC_F32, stream=S.cuda_stream)
+    L.set_option("lazy", 1)
+    rng = np.random.default_rng(4)
+    a, z = (rounded(rng.random((3, 5, 8)) + 0.5, "f32") for _ in range(2))
+    lz = L.from_numpy(z)
+    calls = [(lambda h: L.add(h, lz), a + z), (lambda h: L.sub(lz, h), z - a), (lambda h: L.mul(h, h), a * a), (lambda h: L.div(lz, h), z / a),
+             (lambda h: L.pow(h, L.from_numpy(np.full_like(a, 2.0))), a * a), (lambda h: L.lt(h, lz), (a < z).astype(np.float32)), (lambda h: L.neg(h), -a),
+             (lambda h: L.max(h), a.max(-1, keepdims=True)), (lambda h: L.sum(h), a.sum(-1, keepdims=True)), (lambda h: L.cast(h, cg.U32), a.astype(np.uint32)),
+             (lambda h: L.matmul(h, L.transpose(lz, 1, 2)), a @ z.transpose(0, 2, 1)), (lambda h: L.concat(L.neg(lz), h, 1), np.concatenate([-z, a], 1)),
+             (lambda h: L.add(L.transpose(L.slice(h, 1, 1, 3), 1, 2), L.transpose(L.slice(lz, 1, 1, 3), 1, 2)), (a + z)[:, 1:4].transpose(0, 2, 1)),
+             (lambda h: L.add(L.neg(L.neg(lz)), L.reshape(h, a.shape)), a + z)]
+    with torch.cuda.stream(S):
+        for i, (call, want) in enumerate(calls):
+            x = torch.from_numpy(a).cuda()
+            y = call(L.from_device(x))
+            x.fill_(0)
+            # sums of 8 products or values, each side in any order: 16 half steps of 8 values below 2.25 at most
+            assert np.abs(L.to_numpy(y).astype(np.float64) - want).max() <= (16 * F32 * 8 * 2.25 if want.dtype == np.float32 else 0), i
+        y = L.add(L.from_device(torch.from_numpy(a).cuda().float()), lz)        # (nobody else holds that memory)
+        others = [torch.full((3, 5, 8), 9.0, device="cuda") for _ in range(8)]
+        assert np.array_equal(L.to_numpy(y), a + z)
+        del others
+        # the library's own tensor, written by a replay
+        new, nh, nkv, d, page = 4, 2, 1, 64, 8
+        q, k = (torch.randn(new, h, d, device="cuda") for h in (nh, nkv))
+        ints = [torch.tensor(x, device="cuda", dtype=torch.int32) for x in ([[0]], [0, new], [new])]
+        hq, hk, *tables = (L.from_device(t) for t in (q, k, *ints))
+        kp, vp, q_out = L.zeros((1, nkv, page, d), cg.F32), L.zeros((1, nkv, page, d), cg.F32), L.zeros((new, nh, d), cg.F32)
+        append = lambda: L.paged_append(hk, hk, kp, vp, *tables, q=hq, q_out=q_out)
+        append()
+        L.sync()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=S, capture_error_mode="relaxed"):
+        append()
+    with torch.cuda.stream(S):
+        want = 2 * q.cpu().numpy()
+        y = L.add(q_out, q_out)
+        q.fill_(0)
+        g.replay()
+        assert np.array_equal(L.to_numpy(y), want)
+    assert L.lazy_stats()[0] > 0
+    S.synchronize()
+    L.close()
+
+
+@gpu
 def test_tensors_over_device_memory(cuda):
     import torch
     t = torch.arange(24, device="cuda", dtype=torch.float32).reshape(2, 3, 4)
@@ -891,6 +941,38 @@ class Host:
         fn.argtypes = [ctypes.c_void_p] + [type(w) if w is not None else ctypes.c_void_p for w in wrap]
         fn.restype = ctypes.c_int32
         return fn(self.ctx, *wrap)
+
+
+def test_recorded_mode_records_no_call_on_the_callers_memory(host):
+    """Without a device: a call over memory that the library does not own is made at once (here it finds no device to be made on)."""
+    H = Host(host)
+    L, c = H.lib, ctypes.c_void_p(H.ctx.value)
+    for f in (L.cg_set_option, L.cg_lazy_stats, L.cg_add, L.cg_neg, L.cg_max, L.cg_sum, L.cg_cast, L.cg_matmul, L.cg_concat, L.cg_arange, L.cg_reshape):
+        f.argtypes = None
+        f.restype = ctypes.c_int32
+    assert L.cg_set_option(c, b"lazy", ctypes.c_int64(1)) == 0
+
+    def recorded():
+        n = [ctypes.c_int64() for _ in range(3)]
+        assert L.cg_lazy_stats(c, *(ctypes.byref(x) for x in n)) == 0
+        return n[0].value
+
+    out = ctypes.c_void_p()
+    x, y, u = H.t(0, 4), H.t(4, 0), H.t(0, 4, store="u32")     # (no elements: nothing to launch wherever this runs)
+    L.cg_add(c, x, x, ctypes.byref(out))
+    L.cg_add(c, u, u, ctypes.byref(out))
+    L.cg_neg(c, x, ctypes.byref(out))
+    L.cg_max(c, x, ctypes.byref(out))
+    L.cg_sum(c, x, ctypes.byref(out))
+    L.cg_cast(c, x, 1, ctypes.byref(out))
+    L.cg_matmul(c, x, y, ctypes.byref(out))
+    assert recorded() == 0
+    end = ctypes.c_void_p()
+    assert L.cg_arange(c, ctypes.c_int64(0), ctypes.byref(end)) == 0 and recorded() == 1   # (what has no such input is)
+    assert L.cg_cast(c, end, 0, ctypes.byref(out)) == 0 and recorded() == 2
+    assert L.cg_set_option(c, b"lazy", ctypes.c_int64(1)) == 0
+    L.cg_concat(c, out, H.t(7), 0, ctypes.byref(out))
+    assert recorded() == 2
 
 
 def test_append_refusals(host):
