@@ -444,7 +444,7 @@ int32_t cg_paged_append(cg_ctx* c, const cg_tensor* q, const cg_tensor* k, const
   }
   if (overlap_any({q, k, v, q_gain, k_gain, cos_t, sin_t, table, starts, lens}, {k_pages, v_pages, q_out}))
     return fail(c, CG_ERR_INVALID, "what is written overlaps an input or each other");
-  if (M == 0 || a.rows.rows == 0) return CG_OK;
+  if (M == 0 || a.rows.rows == 0 || a.nh + 2 * nkv == 0) return CG_OK;
   a.q = q ? q->data() : nullptr; a.k = k->data(); a.v = v->data();
   if (q) { a.q_ld = q->strides[0]; a.q_hs = q->strides[1]; }
   a.k_ld = k->strides[0]; a.k_hs = k->strides[1];

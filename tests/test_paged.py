@@ -15,6 +15,7 @@ import ctypes
 import math
 import os
 import subprocess
+import threading
 
 import numpy as np
 import pytest
@@ -1011,6 +1012,21 @@ def test_append_refusals(host):
     far = t(6, 2, 64)
     host.host_device(far, 1)
     assert call(v=far) == INVALID and b"another device" in H.lib.cg_last_error(H.ctx)
+
+
+def test_append_without_heads_returns(host):
+    """Pages without heads and no queries, or queries without heads: there is nothing to write, and the call says so at once."""
+    H = Host(host)
+    u, t = (lambda *d: H.t(*d, store="u32")), H.t
+    for d in (64, 128, 40):
+        for q in (None, t(6, 0, d)):
+            wrap = [q, t(6, 0, d), t(6, 0, d), None, None, ctypes.c_float(1e-6), ctypes.c_int32(0), None, None, ctypes.c_int32(1), u(3, 5), u(4), u(3),
+                    t(20, 0, 16, d, store="bf16"), t(20, 0, 16, d, store="bf16"), None if q is None else t(6, 0, d, store="bf16")]
+            got = []
+            call = threading.Thread(target=lambda: got.append(H._call(H.lib.cg_paged_append, wrap)), daemon=True)
+            call.start()
+            call.join(20)
+            assert got == [0], (d, q is None)
 
 
 def test_attention_refusals(host):
