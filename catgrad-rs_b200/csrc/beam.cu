@@ -195,21 +195,34 @@ struct Values<__nv_bfloat16> {
   }
 };
 
-// A vector of which some values lie outside [0, limit).
+// A vector's values one at a time: -inf from `limit` on.
 template <typename T>
 __device__ __noinline__ uint4 load_edge(const T* row, int at, int limit) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if constexpr (sizeof(T) == 4) {
-      w[i] = at + i >= 0 && at + i < limit ? *(const uint32_t*)(row + at + i) : Values<T>::lowest;
+      w[i] = at + i < limit ? *(const uint32_t*)(row + at + i) : Values<T>::lowest;
     } else {
       const int lo = at + 2 * i, hi = lo + 1;
-      w[i] = (lo >= 0 && lo < limit ? *(const uint16_t*)(row + lo) : Values<T>::lowest & 0xffffu) |
-             (hi >= 0 && hi < limit ? *(const uint16_t*)(row + hi) : Values<T>::lowest & 0xffffu) << 16;
+      w[i] = (lo < limit ? *(const uint16_t*)(row + lo) : Values<T>::lowest & 0xffffu) |
+             (hi < limit ? *(const uint16_t*)(row + hi) : Values<T>::lowest & 0xffffu) << 16;
     }
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// The vector that begins `shift` values into the aligned vector x and ends in the next one.
+template <typename T>
+__device__ __forceinline__ void realign(uint32_t* x, uint4 next, int shift) {
+  const uint32_t a[8] = {x[0], x[1], x[2], x[3], next.x, next.y, next.z, next.w};
+  const int words = shift * (int)sizeof(T) / 4;
+  uint32_t b[6], c[5];
+#pragma unroll
+  for (int i = 0; i < 6; ++i) b[i] = words & 2 ? a[i + 2] : a[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) c[i] = words & 1 ? b[i + 1] : b[i];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = sizeof(T) == 4 ? c[i] : __funnelshift_r(c[i], c[i + 1], shift & 1 ? 16u : 0u);
 }
 
 // What is rare is kept out of the kernel's way (instructions are read once a call, so their number counts).
@@ -230,7 +243,7 @@ __device__ __noinline__ void rank_again(PieceWork& w, const T* row, int at0, int
 #pragma unroll
     for (int i = 0; i < per; ++i) {
       const int at = at0 + v * BT * per + i;
-      if (at >= 0 && at < V) mx = fmaxf(mx, (float)row[at]);
+      if (at < V) mx = fmaxf(mx, (float)row[at]);
     }
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -254,7 +267,7 @@ __device__ __noinline__ void rank_again(PieceWork& w, const T* row, int at0, int
 #pragma unroll 1
       for (int i = 0; i < per; ++i) {
         const int at = at0 + v * BT * per + i;
-        if (at >= 0 && at < V && side(at) > 0) take(at, (float)row[at]);
+        if (at < V && side(at) > 0) take(at, (float)row[at]);
       }
   sync();
   const int above = w.count[slot];
@@ -266,7 +279,7 @@ __device__ __noinline__ void rank_again(PieceWork& w, const T* row, int at0, int
 #pragma unroll
       for (int i = 0; i < per; ++i) {
         const int at = at0 + v * BT * per + i;
-        if (at >= 0 && at < V && side(at) == 0) level |= 1u << i;
+        if (at < V && side(at) == 0) level |= 1u << i;
       }
       int before = __popc(level);
 #pragma unroll
@@ -299,7 +312,7 @@ __device__ __noinline__ void rank_again(PieceWork& w, const T* row, int at0, int
 #pragma unroll
         for (int i = 0; i < per; ++i) {
           const int at = at0 + v * BT * per + i;
-          const uint64_t key = at >= 0 && at < V ? key_at((float)row[at], at) : 0;
+          const uint64_t key = at < V ? key_at((float)row[at], at) : 0;
           if (key < last && key > best) best = key;
         }
       int who;
@@ -315,20 +328,25 @@ __device__ __noinline__ void rank_again(PieceWork& w, const T* row, int at0, int
   }
   sync();
 }
-// This thread's sum of exponentials where some values are NaN.
+// This thread's sum of exponentials where some values are NaN, rounded as that of Values::exps is, so that NaN counts as a mask does.
 template <typename T>
 __device__ __noinline__ float sum_of_numbers(const T* row, int at0, int V, float peak) {
   constexpr int per = Values<T>::per;
   float sum = 0.f;
 #pragma unroll 1
-  for (int v = 0; v < VECS; ++v)
+  for (int q = 0; q < VECS; q += 4) {
+    float even = 0.f, odd = 0.f;
 #pragma unroll 1
-    for (int i = 0; i < per; ++i) {
-      const int at = at0 + v * BT * per + i;
-      if (at < 0 || at >= V) continue;
-      const float x = (float)row[at];
-      if (x == x) sum += fast_exp2((x - peak) * LOG2E);
-    }
+    for (int v = q; v < q + 4; ++v)
+#pragma unroll 1
+      for (int i = 0; i < per; i += 2) {
+        const int at = at0 + v * BT * per + i;
+        const float x = at < V ? (float)row[at] : -INFINITY, y = at + 1 < V ? (float)row[at + 1] : -INFINITY;
+        if (x == x) even += fast_exp2((x - peak) * LOG2E);
+        if (y == y) odd += fast_exp2((y - peak) * LOG2E);
+      }
+    sum += even + odd;
+  }
   return sum;
 }
 
@@ -365,18 +383,18 @@ __global__ void __launch_bounds__(SB * BT, 4 / SB) k_beam_select(SelectArgs a) {
   while (least_groups < K) least_groups *= 2;
 
   // Unit u, piece u % pieces of beam u / pieces, belongs to round i of 256 threads of a block where u = (i n_ranks + rank) SB + sb.
-  // Vectors begin on 16-byte boundaries, a beam's first one up to `per` - 1 values before the beam; those of this thread are BT
-  // apart, and their values count in [0, V).
+  // A piece's vectors are counted from the beam's first value, wherever that lies in memory: sums of exponentials then depend on the logits
+  // alone, and beams with the same logits have the same totals.  This thread's vectors are BT apart.
   const T* row;
   int at0;
   auto locate = [&](int u) {
     const int j = u / a.pieces;
     row = (const T*)a.logits + b * a.ld_b + (int64_t)j * a.ld_j;
-    at0 = ((u - j * a.pieces) * (BT * VECS) + tid) * per - (int)(((uintptr_t)row & 15) / sizeof(T));
+    at0 = ((u - j * a.pieces) * (BT * VECS) + tid) * per;
   };
   auto load = [&](uint32_t* x) {
-    const int first = at0 - tid * per;
-    if (first >= 0 && first + BT * VECS * per <= a.V) {  // (all of the piece's)
+    const int shift = (int)(((uintptr_t)row & 15) / sizeof(T));  // values from a 16-byte boundary to a vector's first one
+    if (shift == 0 && at0 - tid * per + BT * VECS * per <= a.V) {  // (all of the piece's)
       const uint4* from = (const uint4*)(row + at0);
 #pragma unroll
       for (int v = 0; v < VECS; ++v) {
@@ -385,21 +403,30 @@ __global__ void __launch_bounds__(SB * BT, 4 / SB) k_beam_select(SelectArgs a) {
       }
       return;
     }
-    bool edge = false;  // (all whole vectors are asked for before any is waited for)
+    // (all whole vectors are asked for before any is waited for: of those off a boundary the two aligned ones that they lie in, the
+    // second of which a neighbour has asked for as its first)
+    const int whole_to = a.V - per - (shift ? per - shift : 0);  // first values of whole vectors: from `shift` up to here
+    bool edge = false;
 #pragma unroll
     for (int v = 0; v < VECS; ++v) {
       const int at = at0 + v * BT * per;
       uint4 q = make_uint4(Vals::lowest, Vals::lowest, Vals::lowest, Vals::lowest);
-      const bool whole = at >= 0 && at + per <= a.V;
-      if (whole) q = __ldg((const uint4*)(row + at));
-      edge = edge || (!whole && at < a.V && at + per > 0);
+      const bool whole = at >= shift && at <= whole_to;
+      if (whole) q = __ldg((const uint4*)(row + at - shift));
+      edge = edge || (!whole && at < a.V);
       x[4 * v] = q.x; x[4 * v + 1] = q.y; x[4 * v + 2] = q.z; x[4 * v + 3] = q.w;
     }
+    if (shift)
+#pragma unroll
+      for (int v = 0; v < VECS; ++v) {
+        const int at = at0 + v * BT * per;
+        if (at >= shift && at <= whole_to) realign<T>(x + 4 * v, __ldg((const uint4*)(row + at - shift + per)), shift);
+      }
     if (edge)
 #pragma unroll
       for (int v = 0; v < VECS; ++v) {
         const int at = at0 + v * BT * per;
-        if (!(at >= 0 && at + per <= a.V) && at < a.V && at + per > 0) {
+        if (!(at >= shift && at <= whole_to) && at < a.V) {
           const uint4 q = load_edge<T>(row, at, a.V);
           x[4 * v] = q.x; x[4 * v + 1] = q.y; x[4 * v + 2] = q.z; x[4 * v + 3] = q.w;
         }
@@ -667,7 +694,7 @@ struct Blocks {
 template <typename T>
 int launch_select(cg_ctx* c, SelectArgs a, int64_t B) {
   constexpr int64_t per = 16 / sizeof(T), piece = BT * VECS;  // vectors of a piece
-  const int64_t all = (a.V + 2 * per - 2) / per;              // a beam's vectors, where it does not begin on a boundary
+  const int64_t all = (a.V + per - 1) / per;                  // a beam's vectors
   const int64_t pieces = (all + piece - 1) / piece, units = a.J * pieces;
   if (pieces > 32 * MAX_OWN) return fail(c, CG_ERR_UNSUPPORTED, "vocabulary too large");
   a.pieces = (int)pieces;

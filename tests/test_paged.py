@@ -507,6 +507,23 @@ def test_select_ties_and_masks(cuda, store, V):
 
 
 @gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [9, 999, 8195, 50257, 128255, 256000])
+@pytest.mark.parametrize("pitch", [0, 1, 4, 6])
+def test_select_equal_beams_at_any_alignment(cuda, store, V, pitch):
+    """Beams with the same logits and scores have the same totals, wherever their rows begin, and masked is masked, by -inf or by NaN: the
+    lower beam comes first, token by token."""
+    rng = np.random.default_rng(V + pitch)
+    row = rng.standard_normal(V) * 3
+    x = np.stack([row, row, rng.standard_normal(V) * 3, row, row, row])[None]
+    x[:, :, rng.random(V) < 0.05] = -np.inf
+    x[0, 3:5][:, np.isinf(x[0, 0])] = np.nan
+    K = min(24, V)
+    check_select(cuda, x, np.float32([[-7.25, -7.25, -8.0, -7.25, -7.25, -7.25]]), K, store=store, pitch=pitch)
+    check_select(cuda, np.repeat(x, 3, 0), np.full((3, 6), -1.0, np.float32), K, store=store, pitch=pitch)
+
+
+@gpu
 def test_select_in_place(cuda):
     rng = np.random.default_rng(1)
     x, s, f = rng.standard_normal((3, 4, 1000)) * 3, -np.abs(rng.standard_normal((3, 4))).astype(np.float32), np.uint32(rng.random((3, 4)) < 0.3)
