@@ -16,7 +16,9 @@
 // dealt; a warp then joins all sorted lists of a beam, and one warp those of the beams.
 //
 // 24 groups of 8 beams over 256000 tokens in bf16: 98 MB in 42.4 us, 2.3 TB/s (24 clusters of 10 blocks of 512 threads, two blocks on most SMs):
-// some ten instructions per value, and rounds that end at barriers.  One group of 4 beams over 128256 in f32: 9.3 us, a chain of loads, barriers and joins behind a call of 4.
+// some ten instructions per value, and rounds that end at barriers.  One group of 4 beams over 128256 in f32: 9.6 us, a chain of loads, barriers and joins behind a call of 4.
+//
+// Rows that begin off a 16-byte boundary take two loads a vector: 51.2 us over 255999.
 //
 // Exponentials are f32, their sums over more than a warp, the logarithm and the totals 64 bits: totals of different
 // beams may lie close together.
@@ -350,6 +352,49 @@ __device__ __noinline__ float sum_of_numbers(const T* row, int at0, int V, float
   return sum;
 }
 
+__device__ __forceinline__ double total_of(float score, float x, float m, double log_sum) { return (double)score + (((double)x - (double)m) - log_sum); }
+// Where 64 bits do not tell some totals of a beam apart (scores such as -1e30, logits next to 0): of those that equal the K-th the
+// lowest tokens, all in the order of totals, then tokens.  By a warp: lane i has the (i + 1)-th largest logit's total and token, and afterwards
+// those of the beam's (i + 1)-th continuation.  What is larger than the K-th total is among the K; what equals it is looked for in the beam up to
+// the last of these.  `found`: room for K tokens.
+struct Total {
+  double total;
+  uint32_t token;
+};
+template <typename T>
+__device__ __noinline__ Total settle(const T* row, float score, float m, double log_sum, int V, int K, uint64_t* found, double total, uint32_t token) {
+  const int lane = threadIdx.x & 31;
+  const double least = __shfl_sync(0xffffffffu, total, K - 1);
+  const int above = __popc(__ballot_sync(0xffffffffu, lane < K && total > least));
+  const uint32_t last = __reduce_max_sync(0xffffffffu, lane >= above && lane < K ? token : 0u);
+  int n = above;
+  for (uint32_t v0 = 0; v0 <= last && n < K; v0 += 32) {
+    const uint32_t v = v0 + lane;
+    const float x = v < (uint32_t)V ? (float)row[v] : -INFINITY;
+    const bool hit = v < (uint32_t)V && total_of(score, x == x ? x : -INFINITY, m, log_sum) == least;
+    const uint32_t hits = __ballot_sync(0xffffffffu, hit);
+    const int to = n + __popc(hits & ((1u << lane) - 1u));
+    if (hit && to < K) found[to] = v;
+    n += __popc(hits);
+  }
+  __syncwarp();
+  if (lane >= above && lane < K) {
+    total = least;
+    token = (uint32_t)found[lane];
+  }
+  int rank = 0;
+  for (int o = 0; o < K; ++o) {
+    const double t = __shfl_sync(0xffffffffu, total, o);
+    const uint32_t v = __shfl_sync(0xffffffffu, token, o);
+    rank += t > total || (t == total && v < token);
+  }
+  __syncwarp();
+  if (lane < K) found[rank] = (uint64_t)lane;
+  __syncwarp();
+  const int from = lane < K ? (int)found[lane] : lane;
+  return {__shfl_sync(0xffffffffu, total, from), __shfl_sync(0xffffffffu, token, from)};
+}
+
 // dynamic shared memory: PieceWork [SB]; lists u64 [rounds][SB][K]; sums f64 [rounds][SB]; totals u64 [J][K]; places u64 [J][K];
 // tops f32 [rounds][SB]; marks u32 [J]; then per joining warp a beam's lists of all blocks, u64 [pieces][K]
 template <typename T, int SB>
@@ -583,7 +628,7 @@ __global__ void __launch_bounds__(SB * BT, 4 / SB) k_beam_select(SelectArgs a) {
       };
       if (marks[j] && known) {
         // the end token, then -inf in the order of the vocabulary
-        for (int i = lane; i < K; i += 32) put(i, i == 0 ? (double)score : -INFINITY, i == 0 ? a.end : (uint32_t)(i - 1) + ((uint32_t)(i - 1) >= a.end ? 1u : 0u));
+        for (int i = lane; i < K; i += 32) put(i, i == 0 ? (double)score + 0. : -INFINITY, i == 0 ? a.end : (uint32_t)(i - 1) + ((uint32_t)(i - 1) >= a.end ? 1u : 0u));
       } else if (!known || !(m > -INFINITY && m < INFINITY)) {
         for (int i = lane; i < K; i += 32) put(i, -INFINITY, (uint64_t)i);
       } else {
@@ -613,7 +658,13 @@ __global__ void __launch_bounds__(SB * BT, 4 / SB) k_beam_select(SelectArgs a) {
           if (lane == (r & 31)) got = top;
           __syncwarp();
         }
-        if (lane < K) put(lane, (double)score + (((double)down((uint32_t)(got >> 32)) - (double)m) - log_sum), 0xffffffffu - (uint32_t)got);
+        const float x = lane < K ? down((uint32_t)(got >> 32)) : INFINITY;
+        Total best = {total_of(score, x, m, log_sum), 0xffffffffu - (uint32_t)got};
+        // (rare: a step of f32, at least 2^-24 of a logit, may be less than what the total's three roundings in 64 bits take: 2^-48 of its
+        // largest term; ln V < 32)
+        if (__any_sync(0xffffffffu, fabsf(x) * 0x1p24f < fmaxf(fmaxf(fabsf(score), fabsf(m)), 32.f)))
+          best = settle<T>((const T*)a.logits + b * a.ld_b + (int64_t)j * a.ld_j, score, m, log_sum, a.V, K, mine, best.total, best.token);
+        if (lane < K) put(lane, best.total, best.token);
       }
     }
   cluster_barrier();

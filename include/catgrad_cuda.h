@@ -316,7 +316,9 @@ int32_t cg_paged_attention(cg_ctx*, const cg_tensor* q, const cg_tensor* k_pages
                            float scale, int64_t window, float softcap, cg_tensor* out);
 /* One step of beam search for groups of J beams: of the continuations (beam j, token v) with
  *   scores[j] + log softmax(logits[j])[v]
- * the K largest in descending order, equal ones by j, then v.  logits [B, J, V] f32 or bf16, scores
+ * the K largest in descending order, equal ones (in 64 bits) by j, then v; beams of the same logits and
+ * score are equal.  Sums of exponentials are f32 within a warp, so totals of different beams that are
+ * nearer than some 1e-6 may change places.  logits [B, J, V] f32 or bf16, scores
  * [B, J] f32 (-inf: a beam that is not there), finished U32 [B, J] or NULL: a finished beam's only
  * continuation is `end` at an unchanged score.  NaN logits count as -inf; a beam whose largest logit
  * or score is not finite has -inf everywhere.  Outputs [B, K] (K <= V <= 2^20 - 8, J and K at most 32): scores,

@@ -524,6 +524,29 @@ def test_select_equal_beams_at_any_alignment(cuda, store, V, pitch):
 
 
 @gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [40, 1001, 70001])
+def test_select_totals_that_64_bits_do_not_tell_apart(cuda, store, V):
+    """Scores beside which logits vanish, logits beside which others do: equal totals go to the lower beam, then to the lower token."""
+    rng = np.random.default_rng(V)
+    x = rng.standard_normal((2, 3, V)) * 3
+    x[1, :, rng.random(V) < 0.5] = -np.inf
+    x[1, 2, V // 3:] = np.nan
+    for K in (1, 8, 32):
+        check_select(cuda, x, np.full((2, 3), -1e30, np.float32), K, store=store)
+        check_select(cuda, x, np.float32([[-3.0, -1e30, -1e25], [-1e25, -np.inf, 1e30]]), K, store=store)
+        check_select(cuda, x, np.float32([[-1e30, -1e30, 2.0]] * 2), K, np.uint32([[0, 0, 1], [1, 0, 0]]), V - 2, store=store, pitch=1)
+    tiny = np.where(rng.random((1, 2, V)) < 0.3, rng.integers(-3, 4, (1, 2, V)) * 1e-30, -1.0 - rng.random((1, 2, V)))
+    tiny[0, 0, V - 1] = tiny[0, 1, V // 2] = 4.0   # (a few tokens are told apart, the next are not)
+    tiny[0, 1, V // 2 + 3] = 3.0
+    for K in (1, 4, 31):
+        check_select(cuda, tiny, np.float32([[-1.0, -1.0]]), K, store=store)
+        check_select(cuda, tiny, np.float32([[-1.0, -2.5]]), K, store=store)
+    zeros = np.float32([[-0.0, 0.0, -0.0]] * 2)
+    check_select(cuda, x, zeros, 8, np.ones((2, 3), np.uint32), 5, store=store)
+
+
+@gpu
 def test_select_in_place(cuda):
     rng = np.random.default_rng(1)
     x, s, f = rng.standard_normal((3, 4, 1000)) * 3, -np.abs(rng.standard_normal((3, 4))).astype(np.float32), np.uint32(rng.random((3, 4)) < 0.3)
