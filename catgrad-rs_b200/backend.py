@@ -56,6 +56,7 @@ class TaggedTensor:
         self._h = handle
         self._dtype = dtype
         self._shape = None
+        self._memory = None   # what owns the memory that the tensor lies in, where the library does not
 
     @property
     def dtype(self) -> int:
@@ -167,6 +168,12 @@ class TraitBackend:
             self._check(status)
         return TaggedTensor(self, h)
 
+    def _view(self, name: str, x: TaggedTensor, *args) -> TaggedTensor:
+        """A result that may lie in x's memory, which it then keeps alive."""
+        t = self._out1(name, x._h, *args)
+        t._memory = x._memory
+        return t
+
     # -- trait methods (backend/mod.rs line in the comment) -----------------------
     def zeros(self, shape, target_dtype) -> TaggedTensor:  # :26
         d, r = _dims(shape)
@@ -193,7 +200,7 @@ class TraitBackend:
         return self._wrap(h, U32)
 
     def cast(self, x, target_dtype) -> TaggedTensor:  # :40
-        return self._out1("cast", x._h, int(target_dtype))
+        return self._view("cast", x, int(target_dtype))   # (x itself if it has that type)
 
     def matmul(self, a, b): return self._out1("matmul", a._h, b._h)  # :41
     def add(self, a, b): return self._out1("add", a._h, b._h)  # :42
@@ -209,14 +216,14 @@ class TraitBackend:
 
     def broadcast(self, x, shape) -> TaggedTensor:  # :52
         d, r = _dims(shape)
-        return self._out1("broadcast", x._h, d, r)
+        return self._view("broadcast", x, d, r)
 
     def reshape(self, x, new_shape) -> TaggedTensor:  # :53
         d, r = _dims(new_shape)
-        return self._out1("reshape", x._h, d, r)
+        return self._view("reshape", x, d, r)
 
     def transpose(self, x, dim0, dim1) -> TaggedTensor:  # :54
-        return self._out1("transpose", x._h, int(dim0), int(dim1))
+        return self._view("transpose", x, int(dim0), int(dim1))
 
     def max(self, x): return self._out1("max", x._h)  # :55
     def sum(self, x): return self._out1("sum", x._h)  # :56
@@ -239,7 +246,7 @@ class TraitBackend:
         return self._out1("index", x._h, int(dim), indices._h)
 
     def slice(self, x, dim, start, length) -> TaggedTensor:  # :72-78
-        return self._out1("slice", x._h, int(dim), int(start), int(length))
+        return self._view("slice", x, int(dim), int(start), int(length))
 
     def arange(self, end) -> TaggedTensor:  # :79
         return self._out1("arange", int(end))
@@ -464,8 +471,8 @@ class CudaBackend(TraitBackend):
 
     # a paged key/value cache and beam search ---------------------------------------
     def from_device(self, x) -> TaggedTensor:
-        """A tensor over the device memory of `x` (a torch CUDA tensor: f32, bf16, or 32-bit integers as U32), which it
-        keeps alive (its views do not).  Nothing is copied.  Work of other streams on that memory is the caller's to order."""
+        """A tensor over the device memory of `x` (a torch CUDA tensor: f32, bf16, or 32-bit integers as U32), which it and
+        its views keep alive.  Nothing is copied.  Work of other streams on that memory is the caller's to order."""
         storage = {"torch.float32": 0, "torch.int32": 1, "torch.uint32": 1, "torch.bfloat16": 2}.get(str(x.dtype))
         if storage is None:
             raise TypeError(f"no storage for {x.dtype}")

@@ -274,8 +274,9 @@ int32_t cg_fused_moe(cg_ctx*, const cg_tensor* x, const cg_tensor* router, const
 
 /* A tensor over device memory of the caller (storage as cg_storage_of; strides in elements, not
  * negative, NULL = contiguous): nothing is copied, and the memory stays the caller's, who keeps it
- * while the tensor or a view of it lives and orders its own work on other streams against the
- * context's.  Tensors are written by the operators below, which say so, and by cg_comm_all_reduce. */
+ * while the tensor or a view of it lives (a cast to the type that it has is a view) and orders its
+ * own work on other streams against the context's.  Tensors are written by the operators below, which
+ * say so, and by cg_comm_all_reduce. */
 int32_t cg_tensor_from_device(cg_ctx*, void* data, int32_t storage, const int64_t* dims, const int64_t* strides,
                               int32_t rank, cg_tensor** out);
 

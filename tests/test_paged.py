@@ -12,10 +12,12 @@ Tolerances.  2^-24 is half a step of f32, 2^-8 of bf16, relative to the value; e
   and below the fraction: 2 half steps of sum p |v|; the result one more.
 """
 import ctypes
+import gc
 import math
 import os
 import subprocess
 import threading
+import weakref
 
 import numpy as np
 import pytest
@@ -982,6 +984,41 @@ class Host:
         fn.argtypes = [ctypes.c_void_p] + [type(w) if w is not None else ctypes.c_void_p for w in wrap]
         fn.restype = ctypes.c_int32
         return fn(self.ctx, *wrap)
+
+
+VIEWS = [lambda B, t: B.reshape(t, (4, 6)), lambda B, t: B.transpose(t, 0, 1), lambda B, t: B.slice(t, 2, 1, 2), lambda B, t: B.broadcast(t, (5, 2, 3, 4)),
+         lambda B, t: B.cast(t, cg.F32)]
+
+
+@gpu
+def test_views_keep_the_callers_memory(cuda):
+    import torch
+    for i, view in enumerate(VIEWS):
+        x = torch.arange(24, device="cuda").reshape(2, 3, 4).to(torch.bfloat16)
+        want = cuda.to_numpy(view(cuda, cuda.from_numpy(np.arange(24, dtype=np.float32).reshape(2, 3, 4))))
+        torch.cuda.synchronize()
+        alive = weakref.ref(x)
+        t = view(cuda, cuda.from_device(x))
+        del x
+        gc.collect()
+        assert alive() is not None, i
+        t = cuda.transpose(t, 0, 1)
+        assert alive() is not None and np.array_equal(cuda.to_numpy(t), want.swapaxes(0, 1))
+        del t
+        gc.collect()
+        assert alive() is None, i
+
+
+def test_views_know_who_owns_their_memory(oracle):
+    """The same on the CPU: a view of a view too, and no new tensor."""
+    class Owner:
+        pass
+    for view in VIEWS:
+        t = oracle.from_numpy(np.arange(24, dtype=np.float32).reshape(2, 3, 4))
+        assert view(oracle, t)._memory is None
+        t._memory = Owner()
+        assert view(oracle, t)._memory is t._memory and oracle.transpose(view(oracle, t), 0, 1)._memory is t._memory
+        assert oracle.add(t, t)._memory is None
 
 
 def test_recorded_mode_records_no_call_on_the_callers_memory(host):
