@@ -104,13 +104,6 @@ inline bool overlap_any(const cg_tensor* const (&in)[NI], const cg_tensor* const
   }
   return false;
 }
-// `t` is written in place: no two of its elements share memory (contiguous), a cached GEMM operand copy is stale, and a literal's value
-// is no longer known, by this tensor and by all that share its memory.
-inline void written(cg_tensor* t) {
-  t->buf->bf16_copy.reset();
-  t->buf->rewritten = true;
-}
-
 // The pages: k and v alike, [n_pages, nkv, page, d] (with `layers`, [layers, n_pages, nkv, page, d]).
 inline int check_pages(cg_ctx* c, const cg_tensor* k, const cg_tensor* v, bool layers, int* lg) {
   const int64_t any[5] = {-1, -1, -1, -1, -1};

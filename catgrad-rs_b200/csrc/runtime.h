@@ -38,7 +38,7 @@ struct Buffer {
   // The last bf16-rounded copy made of (a view of) this buffer as a GEMM operand, with the view
   // it was made for: q, k and v (or gate and up) read the same activations, and trait tensors
   // are never written after they are made, so the copy serves every one of them.  Whoever does
-  // write a tensor in place (cg_comm_all_reduce) drops it.
+  // write a tensor in place says so (written()).
   bool rewritten = false;  // an operator that writes in place had it: a captured graph may do so again, unseen, so no copy is kept
   std::shared_ptr<Buffer> bf16_copy;
   int64_t bf16_key[5] = {0, 0, 0, 0, 0};  // offset, rows, cols, row stride, col stride
@@ -197,6 +197,13 @@ struct PerDeviceSize {
   size_t v[64] = {};
   size_t& at(int device) { return v[device & 63]; }
 };
+
+// `t` is written in place (by whoever does that, each time): no two of its elements share memory (contiguous), a cached GEMM operand copy
+// is stale, and a literal's value is no longer known, by this tensor and by all that share its memory.
+inline void written(cg_tensor* t) {
+  t->buf->bf16_copy.reset();
+  t->buf->rewritten = true;
+}
 
 // New contiguous tensor with fresh storage.
 int new_tensor(cg_ctx* c, int tag, int storage, const int64_t* dims, int rank, cg_tensor** out);
