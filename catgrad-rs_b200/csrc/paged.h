@@ -59,6 +59,7 @@ struct OnDevice {
 // ---- checks of arguments (host) ----
 
 inline int same_device(cg_ctx* c, const cg_tensor* t, const char* what) {
+  if (!t->buf) return fail(c, CG_ERR_INVALID, std::string(what) + " is recorded in another context");
   if (t->buf->core->device != c->core->device) return fail(c, CG_ERR_INVALID, std::string(what) + " is on another device");
   return CG_OK;
 }

@@ -16,6 +16,7 @@ import gc
 import math
 import os
 import subprocess
+import sys
 import threading
 import weakref
 
@@ -1166,6 +1167,46 @@ def test_select_and_reorder_refusals(host):
                                     (INVALID, dict(own=u(8, 5, at=at), table=u(8, 5, at=at))), (INVALID, dict(lens=u(8, at=at), k=t(3, 20, 2, 16, 64, at=at))),
                                     (INVALID, dict(table=u(8, 5, at=at), v=t(3, 20, 2, 16, 64, at=at)))]):
         assert reorder(**kw) == want, (i, want, H.lib.cg_last_error(H.ctx))
+
+
+def test_tensors_that_another_context_has_recorded_are_refused(host):
+    """They have no memory yet.  (In a process of its own, since a call that looked for that memory would end it.)"""
+    out = ctypes.CDLL(host._name)._name
+    r = subprocess.run([sys.executable, "-c", f"import sys; sys.path.insert(0, {os.path.dirname(__file__)!r}); import test_paged; test_paged.recorded_elsewhere({out!r})"],
+                       capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
+def recorded_elsewhere(path):
+    L = ctypes.CDLL(path)
+    L.host_ctx.restype = ctypes.c_void_p
+    L.host_tensor.restype, L.host_tensor.argtypes = ctypes.c_void_p, [ctypes.c_void_p, ctypes.c_uint64, ctypes.c_int, ctypes.c_int, ctypes.POINTER(ctypes.c_int64),
+                                                                      ctypes.POINTER(ctypes.c_int64)]
+    H = Host(L)
+    other, lib = ctypes.c_void_p(L.host_ctx()), H.lib
+    assert lib.cg_set_option(other, b"lazy", ctypes.c_int64(1)) == 0
+
+    def waiting(shape, dtype):
+        t = ctypes.c_void_p()
+        assert lib.cg_arange(other, ctypes.c_int64(int(np.prod(shape))), ctypes.byref(t)) == 0
+        if dtype == 0:
+            assert lib.cg_cast(other, t, 0, ctypes.byref(t)) == 0
+        assert lib.cg_reshape(other, t, (ctypes.c_int64 * len(shape))(*shape), len(shape), ctypes.byref(t)) == 0
+        return t
+
+    u, f, i32, i64 = (lambda *d: H.t(*d, store="u32")), H.t, ctypes.c_int32, ctypes.c_int64
+    calls = [(lib.cg_paged_attention, dict(q=f(6, 4, 64), k=f(20, 2, 16, 64), v=f(20, 2, 16, 64), table=u(3, 5), starts=u(4), lens=u(3)),
+              [i64(6), ctypes.c_float(0), i64(0), ctypes.c_float(0)], dict(out=f(6, 4, 64))),
+             (lib.cg_beam_select, dict(logits=f(2, 4, 100), scores=f(2, 4), finished=u(2, 4)), [ctypes.c_uint32(7)], dict(s=f(2, 3), t=u(2, 3), p=u(2, 3), f=u(2, 3))),
+             (lib.cg_paged_reorder, dict(parents=u(2, 4), lens=u(8), own=u(8, 5), table=u(8, 5), k=f(20, 2, 16, 64), v=f(20, 2, 16, 64)), [], {})]
+    shapes = dict(q=((6, 4, 64), 0), k=((20, 2, 16, 64), 0), v=((20, 2, 16, 64), 0), table=((3, 5), 1), starts=((4,), 1), lens=((3,), 1), out=((6, 4, 64), 0),
+                  logits=((2, 4, 100), 0), scores=((2, 4), 0), finished=((2, 4), 1), s=((2, 3), 0), t=((2, 3), 1), p=((2, 3), 1), f=((2, 3), 1))
+    for i, (fn, a, scalars, b) in enumerate(calls):
+        for name in {**a, **b}:
+            shape, dtype = dict(shapes, lens=((8,), 1), table=((8, 5), 1), own=((8, 5), 1), parents=((2, 4), 1))[name] if i == 2 else shapes[name]
+            w = waiting(shape, dtype)
+            assert H._call(fn, [w if n == name else x for n, x in a.items()] + scalars + [w if n == name else x for n, x in b.items()]) == 3, (i, name)
+            assert b"another context" in lib.cg_last_error(H.ctx)
 
 
 def test_rows_that_cannot_be_are_not_followed(host):
