@@ -322,6 +322,7 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
     const int64_t ti = first + r / p.rep;                       // this row's
     const int head = kvh * p.rep + r % p.rep;
     const int64_t qpos = pos0 + ti;
+    const bool mine = r < p.per * p.rep && ti < n;              // (others have what follows in q, or nothing that was loaded)
     const int64_t tile_last = min(pos0 + first + p.per - 1, last), tile_first = pos0 + first;
     bool ok = true;
     for (int j = 0; j < nt && ok; ++j) {
@@ -353,7 +354,7 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
 #pragma unroll
       for (int i = 0; i < KT; i += 2) mx4[i / 2 & 3] = fmaxf(fmaxf(mx4[i / 2 & 3], __uint_as_float(v[i])), __uint_as_float(v[i + 1]));
       const float raw_max = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-      bool small = false;  // (uniform) no score is beyond 3/4 of the cap
+      bool small = false;  // (uniform) no score of the sequence's rows is beyond 3/4 of the cap
       if (CAP) {
         if (masked)
 #pragma unroll
@@ -362,7 +363,7 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
 #pragma unroll
         for (int i = 0; i < KT; i += 2) low4[i / 2 & 3] = fminf(fminf(low4[i / 2 & 3], __uint_as_float(v[i])), __uint_as_float(v[i + 1]));
         const float far = fmaxf(raw_max, -fminf(fminf(low4[0], low4[1]), fminf(low4[2], low4[3])));
-        small = __all_sync(0xffffffffu, far * p.cap_in <= 0.75f);
+        small = __all_sync(0xffffffffu, !mine || far * p.cap_in <= 0.75f);
       }
       // (the soft-cap is monotone, and what a score grows by is no less than what its cap does)
       auto reference = [&]() {
@@ -473,7 +474,7 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
     ok = __all_sync(0xffffffffu, ok);
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const float inv = l > 0.f ? 1.f / l : 0.f;
-    const bool out = ok && r < p.per * p.rep && ti < n;
+    const bool out = ok && mine;
     __nv_bfloat16* dst = p.out + ((tok0 + ti) * p.nh + head) * (int64_t)p.d;
 #pragma unroll 1
     for (int c0 = 0; c0 < D && p.slices == 1; c0 += 32) {

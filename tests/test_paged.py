@@ -267,6 +267,30 @@ def test_attention_windows_longer_than_all(cuda, store, window):
         check_attention(cuda, Batch(new, [300, 304], 16), store, 4, 2, 128, window, stale=np.nan)
 
 
+@gpu
+@pytest.mark.parametrize("nh,nkv,d", [(6, 2, 64), (10, 2, 128), (6, 2, 256)])
+def test_capped_rows_do_not_depend_on_their_neighbours(cuda, nh, nkv, d):
+    """A row's outputs, bit for bit, beside rows of small and of huge scores, or of NaN."""
+    import torch
+    rng = np.random.default_rng(d)
+    R, n, t, page = 300, 8, 40, 16
+    b = Batch([n if r % 2 == 0 else 5 for r in range(R)], [t] * R, page)
+    mine = np.concatenate([np.arange(b.starts[r], b.starts[r + 1]) for r in range(0, R, 2)])
+    q = rounded(rng.standard_normal((b.M, nh, d)) * 2, "bf16")
+    k, v = (put(cuda, rounded(rng.standard_normal((b.n_pages, nkv, page, d)), "bf16"), "bf16") for _ in range(2))
+    tables = b.up(cuda)
+    got = []
+    for factor in (1.0, 1000.0, np.nan, 0.0, 1.0):
+        x = q * np.float32(factor)
+        x[mine] = q[mine]
+        out = put(cuda, np.zeros((b.M, nh, d), np.float32), "bf16")
+        cuda.paged_attention(put(cuda, x, "bf16")[0], k[0], v[0], *tables, max_new=n, softcap=20.0, out=out[0])
+        cuda.sync()
+        got.append(out[1].view(torch.int16).cpu().numpy()[mine])
+    assert np.abs(got[0]).max() > 0
+    assert [int((x != got[0]).sum()) for x in got[1:]] == [0] * 4
+
+
 # around tiles of 16 to 128 keys and queries, shares of the keys, pages that end inside a tile
 EDGES = [1, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 257, 300]
 
