@@ -291,6 +291,97 @@ def test_capped_rows_do_not_depend_on_their_neighbours(cuda, nh, nkv, d):
     assert [int((x != got[0]).sum()) for x in got[1:]] == [0] * 4
 
 
+# Errors of all outputs together, which show a part of the operands that was left out where the largest possible error of one does not.
+#
+# f32: operands are two tf32 parts, the upper one rounded (2^-11 at most left), of the lower one 11 bits read (2^-10 of it cut off at most: 2^-21 of the value),
+# and the product of the lower parts left out (2^-22).  A product q k is then 2^-21 + 2^-21 + 2^-22 < 3 2^-21 off at most, a score of d such
+# products of independent signs by `spread` (its standard deviation here) times as much, an output by that relative to itself, and as much again for p v.
+PARTS = 3 * 2.0 ** -21
+
+
+def relative(got, want):
+    return math.sqrt(((got - want) ** 2).sum() / (want ** 2).sum())
+
+
+def off_from_rounded(got, want):
+    """The share of values that are not the 64-bit result rounded to bf16."""
+    return float((got != rounded(want, "bf16").astype(np.float64)).mean())
+
+
+def attention_of(B, b, store, nh, nkv, d, spread, window=0):
+    """The kernel's outputs and the 64-bit ones."""
+    rng = b.rng
+    q = rounded(rng.standard_normal((b.M, nh, d)) * spread, store)
+    k, v = (rounded(rng.standard_normal((b.n_pages, nkv, b.page, d)), store) for _ in range(2))
+    out = put(B, np.zeros((b.M, nh, d), np.float32), store)
+    B.paged_attention(put(B, q, store)[0], put(B, k, store)[0], put(B, v, store)[0], *b.up(B), max_new=max(b.new), window=window, out=out[0])
+    got, want = back(B, out[1]), np.zeros((b.M, nh, d))
+    rows = [tuple(b.gather(x, r).astype(np.float64) for x in (k, v)) for r in range(len(b.new))]
+    for m, r, pos in b.tokens():
+        kk, vv = rows[r]
+        lo = max(0, pos - window + 1) if window else 0
+        want[m] = attention(q[m].astype(np.float64), kk[lo:pos + 1], vv[lo:pos + 1], pos - lo, 1.0 / math.sqrt(d), 0, 0.0)[0]
+    return got, want
+
+
+@gpu
+@pytest.mark.parametrize("nh,nkv,d", [(4, 2, 64), (4, 2, 128), (2, 1, 256), (6, 2, 96), (3, 3, 24)])
+@pytest.mark.parametrize("new,total", [([1, 1, 1], [300, 9001, 77]), ([3, 1], [3000, 40]), ([150, 40], [400, 300]), ([70], [2070])])
+def test_attention_f32_has_all_parts_of_its_operands(cuda, nh, nkv, d, new, total):
+    assert relative(*attention_of(cuda, Batch(new, total, 16, seed=d), "f32", nh, nkv, d, 2.0)) <= (2.0 + 1.0) * PARTS
+
+
+@gpu
+@pytest.mark.parametrize("nh,nkv,d", [(4, 2, 64), (4, 2, 128), (2, 1, 256), (8, 1, 64), (16, 1, 128), (6, 2, 96)])
+@pytest.mark.parametrize("new,total,window", [([1, 1, 1], [300, 9001, 77], 0), ([1] * 40, [50 + r for r in range(40)], 33), ([1], [4000], 0)])
+def test_attention_of_single_tokens_is_rounded_once(cuda, nh, nkv, d, new, total, window):
+    """Probabilities have two bf16 parts: 2^-16 of them is left out at most (and f32 sums of up to 256 products of either sign are as near).  An output is then 2^-16 of its usual size off
+    before it is rounded, which leads to the other neighbour where a border of bf16 is as near: 2^-16 / 2^-8 of the values of that size, four times as many
+    among smaller ones: 2 %."""
+    assert off_from_rounded(*attention_of(cuda, Batch(new, total, 16, seed=d), "bf16", nh, nkv, d, 2.0, window)) <= 0.02
+
+
+def tf32_parts(x):
+    """The upper and the lower part of f32 values, as the tensor cores read them."""
+    x = np.asarray(x, np.float32)
+    hi = ((x.view(np.uint32) + np.uint32(0x1000)) & np.uint32(0xFFFFE000)).view(np.float32)
+    lo = ((x - hi).view(np.uint32) & np.uint32(0xFFFFE000)).view(np.float32)
+    return hi.astype(np.float64), lo.astype(np.float64)
+
+
+@pytest.mark.parametrize("d,t", [(64, 300), (64, 9001), (128, 400), (256, 77), (24, 2070)])
+def test_bounds_show_a_part_that_is_left_out(d, t):
+    """The bounds above, on the CPU: what has all parts is within them, what lacks one is not."""
+    rng = np.random.default_rng(d + t)
+    rows = 40
+    for store in ("f32", "bf16"):
+        q = rounded(rng.standard_normal((rows, d)) * 2.0, store)
+        k, v = (rounded(rng.standard_normal((t, d)), store) for _ in range(2))
+        exact = [x.astype(np.float64) for x in (q, k, v)]
+        s = exact[0] @ exact[1].T / math.sqrt(d)
+        p = np.exp(s - s.max(1, keepdims=True))
+        want = p @ exact[2] / p.sum(1, keepdims=True)
+
+        def kernel(left_out):
+            part = {n: [np.where(f"{n}{i}" in left_out, 0.0, x) for i, x in enumerate(tf32_parts(a))] for n, a in dict(q=q, k=k, v=v).items()}
+            mul = lambda a, b: a[0] @ b[0] + a[1] @ b[0] + a[0] @ b[1]
+            s = mul(part["q"], [x.T for x in part["k"]]) / math.sqrt(d)
+            p = np.exp(s - s.max(1, keepdims=True)).astype(np.float32)
+            ps = [np.where(f"p{i}" in left_out, 0.0, x) for i, x in enumerate(tf32_parts(p))]
+            return mul(ps, part["v"]) / p.astype(np.float64).sum(1, keepdims=True)
+
+        if store == "f32":
+            assert relative(kernel(()), want) <= 3.0 * PARTS
+            for name in ("q1", "k1", "p1", "v1"):
+                assert relative(kernel((name,)), want) > 3 * 3.0 * PARTS, name
+        else:
+            hi = rounded(p, "bf16").astype(np.float64)
+            two = hi + rounded(p - hi, "bf16").astype(np.float64)
+            for probabilities, kept in ((two, True), (hi, False)):
+                got = rounded(probabilities @ exact[2] / p.sum(1, keepdims=True), "bf16").astype(np.float64)
+                assert (off_from_rounded(got, want) <= 0.02) == kept
+
+
 # around tiles of 16 to 128 keys and queries, shares of the keys, pages that end inside a tile
 EDGES = [1, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 257, 300]
 
