@@ -409,6 +409,19 @@ def test_attention_prompts(cuda, store, nh, nkv, d, page, window):
 
 @gpu
 @pytest.mark.parametrize("store", ["f32", "bf16"])
+@pytest.mark.parametrize("nh,nkv,d", [(4, 2, 64), (8, 1, 128), (2, 2, 256)])
+@pytest.mark.parametrize("columns", [40, 4000])
+def test_tables_much_wider_than_the_rows(cuda, store, nh, nkv, d, columns):
+    """What a captured step has: columns for rows that grow, naming nothing yet.  The width decides into how many shares the keys are cut."""
+    for new, total in (([1, 1, 1], [5, 130, 64]), ([1] * 20, [1 + 7 * r for r in range(20)]), ([40, 3, 90], [60, 100, 90]), ([70], [300])):
+        b = Batch(new, total, 16, spare=1)
+        b.table = np.concatenate([b.table, np.full((len(new), columns), 0xFFFFFFFF, np.uint32)], 1)
+        check_attention(cuda, b, store, nh, nkv, d, 0, spread=2.0, stale=np.nan)
+        check_attention(cuda, b, store, nh, nkv, d, 33, 20.0, spread=2.0, stale=np.nan)
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_attention_long(cuda, store, d):
     """Long contexts of unequal length, single tokens and a prompt's end; some tokens are checked."""
