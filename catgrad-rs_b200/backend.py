@@ -497,7 +497,8 @@ class CudaBackend(TraitBackend):
         return q_out
 
     def paged_attention(self, q, k_pages, v_pages, table, starts, lens, max_new=0, scale=0.0, window=0, softcap=0.0, out=None):
-        """Causal attention of the new tokens over the paged cache (cg_paged_attention)."""
+        """Causal attention of the new tokens over the paged cache (cg_paged_attention).  max_new: the most new tokens of a row (1 for
+        a decode step); 0 = not known, which costs time where rows are many."""
         if out is None:
             out = self._empty_like_pages(q.shape, k_pages)
         st = self._lib.cg_paged_attention(self._ctx, q._h, k_pages._h, v_pages._h, table._h, starts._h, lens._h, max_new, scale, window, softcap,

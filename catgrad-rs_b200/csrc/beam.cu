@@ -15,8 +15,9 @@
 // A group of beams is a thread-block cluster, over whose blocks, each of up to four times 256 threads, the pieces of its beams are
 // dealt; a warp then joins all sorted lists of a beam, and one warp those of the beams.
 //
-// 24 groups of 8 beams over 256000 tokens in bf16: 98 MB in 42.4 us, 2.3 TB/s (24 clusters of 10 blocks of 512 threads, two blocks on most SMs):
-// some ten instructions per value, and rounds that end at barriers.  One group of 4 beams over 128256 in f32: 9.6 us, a chain of loads, barriers and joins behind a call of 4.
+// 24 groups of 8 beams over 256000 tokens in bf16: 98 MB in 42.6 us, 2.3 TB/s (24 clusters of 10 blocks of 512 threads, two blocks on most SMs).
+// Neither bytes nor issue (33 % of its slots) is used up: between two of a warp's instructions 15 clocks pass, 4.8 of them at barriers and 2.3
+// for logits, none of which are on their way while a piece is ranked.  One group of 4 beams over 128256 in f32: 9.6 us, a chain of loads, barriers and joins behind a call of 4.
 //
 // Rows that begin off a 16-byte boundary take two loads a vector: 51.2 us over 255999.
 //
@@ -751,11 +752,11 @@ int launch_select(cg_ctx* c, SelectArgs a, int64_t B) {
   a.pieces = (int)pieces;
   // Blocks of a group and times 256 threads of a block: what takes the least time by rounds of pieces, a round being a chain of
   // 1.5 us and 0.4 per 256 threads that an SM has.  Us for blocks x times, of the ten numbers of blocks and three of times, the rule's first:
-  //   24 groups of 8 over 256000 in bf16    10 x 2: 43.6    4 x 4: 47.6   16 x 1: 48.1   8 x 2: 48.5   5 x 2: 52.5
-  //   1 of 4 over 128256 in f32             16 x 4: 9.8    16 x 2: 10.3   8 x 4: 12.6   10 x 2: 14.0
-  //   64 of 4 over 32000                     4 x 2: 12.9    2 x 4: 12.9    8 x 1: 13.4   2 x 2: 15.0
-  //   190 of 1 over 50257 in bf16            1 x 2: 13.8    2 x 1: 14.9    1 x 1: 16.3   4 x 1: 17.5
-  //   12 of 8 over 151936 in bf16           16 x 2: 22.2    8 x 4: 22.1   6 x 4: 25.5   10 x 2: 25.9
+  //   24 groups of 8 over 256000 in bf16    10 x 2: 42.8    5 x 4: 44.0   16 x 1: 45.3   8 x 2: 47.7   5 x 2: 52.0
+  //   1 of 4 over 128256 in f32             16 x 4: 9.6    16 x 2: 10.2   8 x 4: 12.4   10 x 2: 14.1
+  //   64 of 4 over 32000                     4 x 2: 12.8    8 x 1: 12.7    2 x 4: 13.3   2 x 2: 14.9
+  //   190 of 1 over 50257 in bf16            1 x 2: 16.8    2 x 1: 18.0    1 x 1: 18.6   4 x 1: 19.1  (rows off a boundary)
+  //   12 of 8 over 151936 in bf16           16 x 2: 21.7   16 x 1: 21.3    8 x 4: 22.0   6 x 4: 25.7
   int best_ranks = 0, best_sb = 1;
   double best = 1e300;
   const int device = c->core->device;

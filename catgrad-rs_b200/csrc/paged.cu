@@ -152,8 +152,8 @@ struct Eight<__nv_bfloat16> {
 // which are the two sides of its eight pairs (with `rot_half` where they turn), or 16 neighbours.  A warp has one of `parts` shares of a
 // token's heads, U times 32 / G of them, all on their way before the token's row is looked up.
 //
-// Bytes should bound it (read once, written once); what does is the instructions per value (widen, square, two factors of the norm,
-// four of the turn, round).  6 rows of up to 2903 tokens, 32 + 2 x 4 heads of 128 with norms, bf16: 251 MB in 56.8 us, 4.4 TB/s.  The steps
+// Bytes should bound it (read once, written once).  They do not (0.68 of the copy rate), nor does issue (56 % of its slots): 96 registers leave a scheduler 4
+// warps, each of which waits 6.8 clocks from one instruction to the next, 1.9 for dependent arithmetic, 0.8 for the norm's shuffles, 0.8 for memory.  6 rows of up to 2903 tokens, 32 + 2 x 4 heads of 128 with norms, bf16: 251 MB in 56.8 us, 4.4 TB/s.  The steps
 // there, from 225 us: vectors in eights 77, all of a lane's vectors on their way at once 62, neighbouring heads in a warp, so that
 // gains stay in registers, 57.  Of a single step's tokens the call's 4.9 us are all.
 template <typename TI>

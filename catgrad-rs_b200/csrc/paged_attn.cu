@@ -419,12 +419,12 @@ int launch_any(cg_ctx* c, const PagedAttnArgs& a) {
   }
   const int64_t tiles = (a.most * (a.nh / a.nkv) + QR - 1) / QR * a.nkv, longest = a.rows.cols << a.rows.lg;
   if (tiles > 0x7FFFFFFFll) return fail(c, CG_ERR_UNSUPPORTED, "too many tokens");
-  // Shares of the keys.  Us in f32, heads of 64, with 1 / 2 / 4 / 8:
-  //   3 rows of 213 behind 1500, 2 x 2 heads    137  72.9  51.9  56.6
-  //   1 row of 1000                             81.9 46.4  31.2  33.3
-  //   8 single tokens of 600                    18.6 13.6  10.9  15.3
-  //   32 of 1800                                54.1 33.5  36.6  52.8
-  //   1 of 4000                                 95.7 51.3  28.4  16.6
+  // Shares of the keys.  Us in f32, heads of 64, with 1 / 2 / 4 / 8, [the rule's] (the table's width stands for the lengths):
+  //   3 rows of 213 behind 1500, 2 x 2 heads    117  63.1  50.2 [54.7]
+  //   1 row of 1000                             70.3 40.8 [30.2] 32.3
+  //   8 single tokens of 600                    16.2 12.6 [10.4] 13.9
+  //   32 of 1800                                42.2 [26.5] 31.2 49.6
+  //   1 of 4000                                 80.4 43.5  24.5 [15.1]
   static AtATime known;
   const int slices = pick_shares([&](int i) { return at_a_time(known, c->core->device, i, k_paged_attn<T, D, QR>, 128, smem); }, 8, tiles * a.rows.rows, longest,
                                  Shape<D, QR>::GK, QR == 16 ? 4.5 : 3.5, QR == 16 ? 2.8 : D == 64 ? 2.4 : D == 128 ? 4.5 : 5.,

@@ -366,14 +366,15 @@ int launch(cg_ctx* c, const PagedAttnArgs& a) {
   CG_TRY(make_map(c, &mk, a.k_pages, p.pool_rows, a.d, a.d, box));
   CG_TRY(make_map(c, &mv, a.v_pages, p.pool_rows, a.d, a.d, box));
   const int64_t groups = (a.most * p.rep + ROWS - 1) / ROWS * a.nkv, longest = a.rows.cols << a.rows.lg;
-  // Shares of the keys.  Us with 1 / 2 / 4 / 8 / 16, [the rule's] (with a joining that took about 1 us more):
-  //   8 rows x 8 key heads, 578 keys, d 64      8.7   8.2 [7.4]  13.5  37
-  //   8 x 8, 2000, d 128                       29.4  19.7 [16.8] 23.8  48
-  //   1 x 8, 4096, d 128                       52.2  29.9  18.0  12.5 [11.5]
-  //   1 x 8, 32000, d 128                      394   200   104   57.6 [38.3]
-  //   32 x 8, 530, d 128                      [16.2] 23.7  34.0  59.9  147
-  //   4 x 4, 2080, d 256                       44.8  26.5 [17.2] 24.0  31.8
-  //   12 x 4, 167, d 256                       [8.4]  8.6  14.3  29.2  59
+  // Shares of the keys.  Us with 1 / 2 / 4 / 8 / 16, [the rule's]:
+  //   8 rows x 8 key heads, 578 keys, d 64      7.9   7.4 [6.5]  11.0  27.5
+  //   8 x 8, 2000, d 128                       29.9  19.3 [15.9] 22.1  39.6
+  //   1 x 8, 4096, d 128                       53.8  30.3  17.6  11.4 [9.7]
+  //   1 x 8, 32000, d 128                      410   211   108   57.7 [37.3]
+  //   32 x 8, 530, d 128                      [15.7] 23.5  31.7  53.6  119
+  //   4 x 4, 2080, d 256                       39.8  23.7 [15.2] 20.9  25.7
+  //   12 x 4, 167, d 256                        7.5 [7.9]  12.7  24.8  47.7
+  // (Lengths are on the device, so the table's width stands for them: 32 x 8 rows of 530 with columns for 32768 tokens get 2 shares, 23.4 us.)
   static AtATime known;
   const int slices = pick_shares([&](int i) { return at_a_time(known, c->core->device, i, k_paged_dec<D, ROWS, CAP>, 128, smem); }, 16, groups * a.rows.rows, longest,
                                  4 * dec_keys<D>(), 4., D == 64 ? 0.7 : D == 128 ? 0.75 : 1.25, 0.);

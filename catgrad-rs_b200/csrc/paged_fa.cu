@@ -12,13 +12,15 @@
 // Exponentials are taken against a reference that lags behind the row's maximum by up to 2^8: O and the sum are rescaled
 // only when it would be more.  bf16 has the same relative step everywhere, so this costs no precision but for
 // the largest probability, which is exactly 1 against the exact maximum; the denominator sums the
-// probabilities as bf16 holds them, so that a row that one key decides loses nothing either way.
+// probabilities as bf16 holds them, so that a row that one key decides loses nothing either way.  Probabilities are one bf16 operand: a
+// second part, as the decode form has, would double the second product, which is half of this kernel's work.  Their rounding
+// (2^-9 of each, of either sign) adds to the output's: errors against 64 bits 0.0021 of the result, where the output's alone are 0.0016.
 //
 // Where there are few tiles, or a little more than a whole number of turns, a cluster of 2 or 4 blocks shares a tile's keys; their outputs
 // are joined through shared memory.
 //
-// One row of 8191 tokens, 32 heads and 8 key heads of 128: 563 us, 976 TFLOP/s at about 1690 MHz under the power limit; the tensor pipe is
-// busy 54 % of the time, the exponentials' unit as much: what bounds it is the chain scores -> softmax -> product, which two tiles per SM
+// One row of 8191 tokens, 32 heads and 8 key heads of 128: 564 us, 975 TFLOP/s at about 1690 MHz under the power limit; the tensor pipe is
+// busy 51 % of the time, the exponentials' unit as much: what bounds it is the chain scores -> softmax -> product, which two tiles per SM
 // hide in part.  128-key tiles with one score buffer: 619 us.  6 rows of up to 700 behind 5003, 8 heads and 4 of 256, cap and
 // window: 150 us, 566 TFLOP/s, with one tile per SM (soft-caps as branches 523, as exponentials 214).
 //
@@ -628,12 +630,13 @@ int launch(cg_ctx* c, const PagedAttnArgs& a) {
   CG_TRY(make_q_map(c, &mq, a, p.per, p.rep));
   const int64_t tiles = (a.most + (int64_t)NQ * p.per - 1) / ((int64_t)NQ * p.per), longest = a.rows.cols << a.rows.lg;
   // Shares of the keys (of several rows four fifths of the tiles count: they differ).  Us with 1 / 2 / 4, [the rule's]:
-  //   6 rows of 480 behind 3720, 4 x 2 heads of 256, window 4096    181  [157]  189  (rows that differ: 169 [152] 186)
-  //   1 of 63 behind 2937, the same, no window                     62.2   39.4 [25.5]
-  //   1 of 49 behind 3951, 8 x 4 heads of 128                      66.1   40.9 [26.1]
-  //   1 of 2000, the same                                         [60.1]  71.7  118
-  //   4 of 300 behind 1700, the same                              [72.7]  75.9  94
-  //   3 of 200 behind 8800, heads of 64                            140    146  [125]
+  //   6 rows of 480 behind 3720, 4 x 2 heads of 256, window 4096    182  [157]  187
+  //   1 of 63 behind 2937, the same, no window                     61.6   38.0 [24.6]
+  //   1 of 49 behind 3951, 8 x 4 heads of 128                      65.5   40.8 [26.0]
+  //   1 of 2000, the same                                         [59.7]  71.5  118
+  //   4 of 300 behind 1700, the same                              [72.1]  75.7  94
+  //   3 of 200 behind 8800, heads of 64                            139    145  [124]
+  // (The table's width stands for the lengths, and 4 shares of a short tile of queries leave SMs idle: the second and third rows' bytes take 2 to 3 us.)
   static AtATime known;
   const int64_t clusters = tiles * a.nkv * a.rows.rows;
   p.slices = pick_shares([&](int i) { return at_a_time(known, c->core->device, i, k_paged_fa<D, NQ, CAP>, NQ == 2 ? 384 : 256, smem); }, 4,

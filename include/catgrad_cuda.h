@@ -309,8 +309,12 @@ int32_t cg_paged_append(cg_ctx*, const cg_tensor* q, const cg_tensor* k, const c
  * position (so after cg_paged_append), into out [tokens, heads, d]; q and out are stored as the
  * pages.  heads is a multiple of kv heads, grouped as in cg_fused_attention.  max_new: no row has
  * more new tokens (0 = not known: every row gets the blocks of all tokens, which costs time where
- * rows are many); a row that has more is left out (CG_ERR_INDEX).  scale 0 = 1 / sqrt(d).  window > 0: only the last `window` tokens are seen; pages before all windows of a
- * row are not read, so their table entries may be stale.  softcap > 0 as in cg_fused_attention.
+ * rows are many, and in bf16 takes the form of prompts where all tokens times a key head's query
+ * heads are more than 16); a row that has more is left out (CG_ERR_INDEX).  The table's width stands
+ * for the longest row when the keys are shared out among blocks: columns far beyond the rows cost time
+ * where rows are many and short.  scale 0 = 1 / sqrt(d).  window > 0: only the last `window` tokens are
+ * seen; pages before all windows of a row are not read, so their table entries may be stale.
+ * softcap > 0 as in cg_fused_attention.  bf16: the form of prompts rounds probabilities to bf16.
  * What is cached at a row's positions is finite. */
 int32_t cg_paged_attention(cg_ctx*, const cg_tensor* q, const cg_tensor* k_pages, const cg_tensor* v_pages,
                            const cg_tensor* table, const cg_tensor* starts, const cg_tensor* lens, int64_t max_new,
