@@ -170,7 +170,11 @@ class TraitBackend:
 
     def _view(self, name: str, x: TaggedTensor, *args) -> TaggedTensor:
         """A result that may lie in x's memory, which it then keeps alive."""
-        t = self._out1(name, x._h, *args)
+        h = _c_vp()
+        status = self._f(name)(self._ctx, x._h, *args, C.byref(h))
+        if status != 0:
+            self._check(status)
+        t = TaggedTensor(self, h)
         t._memory = x._memory
         return t
 
