@@ -1178,7 +1178,7 @@ def test_recorded_mode_records_no_call_on_the_callers_memory(host):
     assert L.cg_arange(c, ctypes.c_int64(0), ctypes.byref(end)) == 0 and recorded() == 1   # (what has no such input is)
     assert L.cg_cast(c, end, 0, ctypes.byref(out)) == 0 and recorded() == 2
     assert L.cg_set_option(c, b"lazy", ctypes.c_int64(1)) == 0
-    L.cg_concat(c, out, H.t(7), 0, ctypes.byref(out))
+    L.cg_concat(c, out, H.t(0), 0, ctypes.byref(out))
     assert recorded() == 2
 
 
