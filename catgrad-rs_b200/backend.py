@@ -366,6 +366,8 @@ class CudaBackend(TraitBackend):
             ("cg_paged_attention", [vp, vp, vp, vp, vp, vp, vp, i64, f32, i64, f32, vp], i32),
             ("cg_beam_select", [vp, vp, vp, vp, C.c_uint32, vp, vp, vp, vp], i32),
             ("cg_paged_reorder", [vp, vp, vp, vp, vp, vp, vp], i32),
+            ("cg_paged_assign", [vp, vp, vp, vp, vp, i64, i64, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp], i32),
+            ("cg_verify_drafts", [vp, vp, vp, vp, vp, vp, vp, vp, i64, vp, vp, vp], i32),
             ("cg_rope_tables", [vp, f32, i32, f32, f32, f32, f32, f32, i32, i64, i64, out, out], i32),
         ]:
             fn = getattr(L, name)
@@ -529,6 +531,28 @@ class CudaBackend(TraitBackend):
         st = self._lib.cg_paged_reorder(self._ctx, parents._h, lens._h, own._h, table._h, k_pages._h, v_pages._h)
         if st:
             self._check(st)
+
+    def paged_assign(self, lens, new, page, held, table, free, n_free, starts, done=None, first=None, max_tokens=0, lens_out=None, held_out=None,
+                     n_free_out=None, positions=None, slots=None):
+        """Pages, starts, positions and slots of the next step's tokens (cg_paged_assign); lens, held and n_free are written over
+        where no outputs are given for them."""
+        st = self._lib.cg_paged_assign(self._ctx, lens._h, new._h, done and done._h, first and first._h, page, max_tokens, held._h, n_free._h, free._h,
+                                       table._h, starts._h, (lens_out or lens)._h, (held_out or held)._h, (n_free_out or n_free)._h,
+                                       positions and positions._h, slots and slots._h)
+        if st:
+            self._check(st)
+
+    def verify_drafts(self, logits, tokens, starts, uniform, probs=None, temperature=None, lens=None, max_new=0, out=None):
+        """(accepted, next, lens without what was rejected) of every row's drafts (cg_verify_drafts); without lens the last is None."""
+        if out is None:
+            rows = (starts.shape[0] - 1,)
+            out = (self.zeros(rows, U32), self.zeros(rows, U32), None if lens is None else self.zeros(rows, U32))
+        a, t, n = out
+        st = self._lib.cg_verify_drafts(self._ctx, logits._h, probs and probs._h, tokens._h, starts._h, uniform._h, temperature and temperature._h,
+                                        lens and lens._h, max_new, a._h, t._h, n and n._h)
+        if st:
+            self._check(st)
+        return out
 
     def _empty_like_pages(self, shape, pages):
         t = self.zeros(shape, F32)

@@ -342,6 +342,41 @@ int32_t cg_beam_select(cg_ctx*, const cg_tensor* logits, const cg_tensor* scores
 int32_t cg_paged_reorder(cg_ctx*, const cg_tensor* parents, const cg_tensor* lens, const cg_tensor* own, cg_tensor* table,
                          cg_tensor* k_pages, cg_tensor* v_pages);
 
+/* The tables of a step of serving, from the rows' lengths, on the device: which rows' new tokens fit, the pages they get, and
+ * what the operators above read.  Row r has lens[r] cached tokens and new[r] more to come (0: none), and `held[r]` columns of
+ * its table name pages, of which the first `first[r]` are not its own (a prefix that others share; NULL: 0).  `free` U32 [n] holds
+ * the names of free pages, as a stack of n_free[0].
+ *   Rows with done[r] != 0 (NULL: none) have ended: the pages of columns first[r] .. held[r] go to the stack, by row, then column;
+ * first[r] columns and no tokens are left.  The others need the pages that hold lens + new tokens and are not held.  A row fits if the
+ * sum of needs up to and with it is at most the stack (or it needs none), and the sum of new tokens at most max_tokens (0 = no
+ * limit) and the places of positions and slots.  In these sums the rows that run (lens above first pages) come before those that begin,
+ * each kind by row.  Rows that fit take their pages from the stack's end in that order, by column; the others get no tokens.
+ *   Outputs: starts [rows + 1] (packed by row), lens_out (the new tokens among them), held_out, n_free_out [1], table and
+ * free in place (above n_free_out, free holds what has been taken), and for the packed tokens, where given, positions and slots
+ * (page * name + place), which stay as they are behind the last token.  lens_out, held_out and n_free_out may be lens, held and n_free.
+ *   A row whose numbers cannot be (more held than columns, more cached than held, more tokens than the table's columns) gets none and raises
+ * CG_ERR_INDEX at the next cg_sync, as do all rows where the stack would overflow.  Nothing is checked of the names themselves. */
+int32_t cg_paged_assign(cg_ctx*, const cg_tensor* lens, const cg_tensor* new_tokens, const cg_tensor* done, const cg_tensor* first,
+                        int64_t page, int64_t max_tokens, const cg_tensor* held, const cg_tensor* n_free, cg_tensor* free, cg_tensor* table,
+                        cg_tensor* starts, cg_tensor* lens_out, cg_tensor* held_out, cg_tensor* n_free_out, cg_tensor* positions,
+                        cg_tensor* slots);
+/* Verification of drafted tokens (speculative decoding).  Row r has run the packed tokens starts[r] .. starts[r + 1]: its last token, then
+ * its drafts; logits [M, V] f32 or bf16 stand behind each, and the draft at place m + 1 is judged at place m, with
+ * p = softmax(logits[m] / temperature[r]) (temperature F32 [rows], NULL: 1) and the drafter's q = probs[m] ([M, V] f32 or bf16; NULL: a draft
+ * is its drafter's only token): it stands if uniform[m] q(draft) < p(draft).  accepted[r] drafts stand, up to the first that does not.  next[r]
+ * is drawn by the last of the row's numbers u = uniform[starts[r + 1] - 1]: behind a rejected draft from w = max(p - q, 0)
+ * at its place (from p, if that is 0 everywhere), behind all drafts from w = p at the last place: the first token at which the sum of w
+ * up to and with it is above u times the whole sum (else the last with a w above 0).  A row of one token thus draws from its logits.
+ * A temperature of 0 (or less, or NaN) is greedy: a draft stands if it is the first of the largest logits, and that one is next[r].
+ *   NaN logits count as -inf, what of q is not above 0 as 0, temperatures beyond 2^+-100 as that.  Where the largest logit is not finite
+ * nothing stands, and next[r] is 0xFFFFFFFF.  Weights that are drawn from have 64 bits; sums that drafts are judged by are off by
+ * some 2^-22.  lens_out[r] = lens[r] less the drafts that do not stand, which so leave the cache (both U32 [rows] or NULL; may be one).
+ * max_new: no row has more tokens (0 = not known).  V is at most 2^19; rows of logits and probs may be apart, and begin anywhere.
+ *   A row without tokens is left out, one whose starts, length or drafts cannot be too, and raises CG_ERR_INDEX. */
+int32_t cg_verify_drafts(cg_ctx*, const cg_tensor* logits, const cg_tensor* probs, const cg_tensor* tokens, const cg_tensor* starts,
+                         const cg_tensor* uniform, const cg_tensor* temperature, const cg_tensor* lens, int64_t max_new, cg_tensor* accepted,
+                         cg_tensor* next, cg_tensor* lens_out);
+
 /* --- decoder runner: the greedy loop of catgrad-llm/examples/llama/main.rs:118-169 with a
  * device KV cache (cache semantics of catgrad-llm/src/legacy/models/utils.rs:210-228). --- */
 

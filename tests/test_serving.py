@@ -1,0 +1,499 @@
+"""Pages for the next step, attention over shared prefixes and the verification of drafted tokens, against plain restatements.
+
+Tolerances.  Pages, places and tokens are whole numbers and have to be equal.  A draft is judged by a sum of f32 exponentials: each has an
+argument rounded to 2^-24 of itself and is off by 2 half steps, so that a probability is within 2^-20 of itself for arguments up to some ten; drafts
+nearer to the border than that are left out of a comparison (tests assert that hardly any is).  Weights that tokens are drawn from have 64 bits:
+a draw nearer to a border than 2^-40 of the whole is left out.
+"""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+
+from conftest import cg
+from test_paged import BF16, F32, Host, attention, back, host, put, rounded  # noqa: F401
+
+gpu = pytest.mark.gpu
+INDEX = 6
+
+
+def raises_index(B):
+    with pytest.raises(cg.BackendPanic) as e:
+        B.sync()
+    assert e.value.status == INDEX
+
+
+# ---------------------------------------------------------------- pages for the next step
+
+
+def plain_assign(lens, new, done, first, held, table, free, n_free, page, budget):
+    """Row by row; (starts, lens, held, n_free, positions, slots), table and free in place, and whether something cannot be."""
+    rows, cols = table.shape
+    bad = n_free > len(free)
+    ask = []
+    for r in range(rows):
+        l, w, h, f = int(lens[r]), int(new[r]), int(held[r]), int(first[r])
+        ends = bool(done[r])
+        ok = h <= cols and f <= h and (ends or (l <= h * page and (w == 0 or -(-(l + w) // page) <= cols)))
+        bad = bad or not ok
+        ask.append((ok, ends, l, w, h, f))
+    give = [(r, c) for r, (ok, ends, l, w, h, f) in enumerate(ask) if ok and ends for c in range(f, h)]
+    valid = n_free + len(give) <= len(free) and n_free <= len(free)
+    bad = bad or not valid
+    count = n_free
+    if valid:
+        for r, c in give:
+            free[count] = table[r, c]
+            count += 1
+    sums = {}
+    needs = {r: max(-(-(l + w) // page) - h, 0) if w else 0 for r, (ok, ends, l, w, h, f) in enumerate(ask) if ok and valid and not ends}
+    pages = tokens = 0
+    for runs in (True, False):
+        for r, need in needs.items():
+            ok, ends, l, w, h, f = ask[r]
+            if (l > f * page) == runs:
+                sums[r] = (pages, need, w, w > 0 and (need == 0 or pages + need <= count) and tokens + w <= budget)
+                pages += need
+                tokens += w
+    starts, lens_out, held_out, positions, slots = [0], [], [], [], []
+    top = count
+    for r, (ok, ends, l, w, h, f) in enumerate(ask):
+        before, need, w, fits = sums.get(r, (0, 0, 0, False))
+        if ok and valid and ends:
+            lens_out.append(0)
+            held_out.append(f)
+            starts.append(starts[-1])
+            continue
+        n = w if fits else 0
+        if fits:
+            for j in range(need):
+                table[r, h + j] = free[top - 1 - before - j]
+            count -= need
+        starts.append(starts[-1] + n)
+        lens_out.append(l + n)
+        held_out.append(h + (need if fits else 0))
+        for p in range(l, l + n):
+            positions.append(p)
+            slots.append((int(table[r, p // page]) * page + p % page) & 0xFFFFFFFF)
+    return starts, lens_out, held_out, count, positions, slots, bad
+
+
+def requests(rng, rows, page, cached=300, prompt=200, drafts=4, spare=3, tight=0.6):
+    """Requests in the middle of their lives, and more pages asked for than there are."""
+    cols = -(-(max(cached, prompt) + drafts + 2) // page) + spare
+    kind = rng.random(rows)
+    lens = np.where(kind < 0.6, rng.integers(1, cached + 1, rows), 0)
+    new = np.where(kind < 0.6, rng.integers(0, drafts + 2, rows), rng.integers(0, prompt + 1, rows))
+    done = (rng.random(rows) < 0.15).astype(np.int64) * rng.integers(1, 9, rows)
+    held = np.minimum(-(-lens // page) + rng.integers(0, 2, rows), cols)
+    first = np.where(rng.random(rows) < 0.3, lens // page // 2, 0)
+    prefix = rng.random(rows) < 0.2     # rows that begin behind a prefix of others
+    first = np.where(prefix, np.minimum(2, cols - 1), first)
+    lens = np.where(prefix, first * page, lens)
+    held = np.where(prefix, first, held)
+    new = np.where(prefix, rng.integers(0, 20, rows), new)
+    table = rng.integers(0, 1 << 20, (rows, cols))
+    need = int(np.maximum(-(-(lens + new) // page) - held, 0).sum())
+    n_free = int(need * tight) + int(rng.integers(0, 3))
+    free = rng.integers(0, 1 << 20, n_free + int(held.sum()) + int(rng.integers(0, 5)))
+    return dict(lens=lens, new=new, done=done, first=first, held=held, table=table, free=free, n_free=n_free)
+
+
+def check_assign(B, s, page, budget, places=None, in_place=False, outputs=("positions", "slots"), optional=("done", "first"), raises=None):
+    rows = len(s["lens"])
+    places = budget if places is None else places
+    zero = np.zeros(rows, np.int64)
+    want_table, want_free = s["table"].copy(), s["free"].copy()
+    want = plain_assign(s["lens"], s["new"], s["done"] if "done" in optional else zero, s["first"] if "first" in optional else zero, s["held"], want_table, want_free,
+                        s["n_free"], page, min(budget or 1 << 40, places if outputs else 1 << 40))
+    up = {n: put(B, np.asarray(s[n], np.uint32)) for n in ("lens", "new", "done", "first", "held", "table", "free")}
+    up["n_free"] = put(B, np.uint32([s["n_free"]]))
+    old = np.arange(7, 7 + places).astype(np.uint32)
+    more = {n: put(B, old) for n in outputs}
+    starts = put(B, np.full(rows + 1, 99, np.uint32))
+    outs = {n: up[n[:-4]] if in_place else put(B, np.full(1 if n == "n_free_out" else rows, 98, np.uint32)) for n in ("lens_out", "held_out", "n_free_out")}
+    B.paged_assign(up["lens"][0], up["new"][0], page, up["held"][0], up["table"][0], up["free"][0], up["n_free"][0], starts[0],
+                   done=up["done"][0] if "done" in optional else None, first=up["first"][0] if "first" in optional else None, max_tokens=budget,
+                   **{n: t[0] for n, t in more.items()}, **({} if in_place else {n: t[0] for n, t in outs.items()}))
+    if want[6] if raises is None else raises:
+        raises_index(B)
+    get = lambda t: back(B, t[1]).astype(np.int64) & 0xFFFFFFFF
+    assert get(starts).tolist() == want[0]
+    assert get(outs["lens_out"]).tolist() == want[1] and get(outs["held_out"]).tolist() == want[2] and get(outs["n_free_out"]).tolist() == [want[3]]
+    assert np.array_equal(get(up["table"]), want_table)
+    # what is above the stack is nobody's
+    assert np.array_equal(get(up["free"])[:want[3]], want_free[:want[3]])
+    n = len(want[4])
+    for name, values in (("positions", want[4]), ("slots", want[5])):
+        if name in outputs:
+            got = get(more[name])
+            assert got[:n].tolist() == values and np.array_equal(got[n:], old[n:])
+    return want
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 2, 8, 31, 33, 127, 128, 129, 300, 512, 513])
+@pytest.mark.parametrize("page", [8, 16, 256])
+def test_assign(cuda, rows, page):
+    rng = np.random.default_rng(rows + page)
+    fits = 0
+    for i in range(4):
+        s = requests(rng, rows, page, cached=int(rng.integers(1, 400)), prompt=int(rng.integers(1, 300)), tight=(0.0, 0.5, 0.9, 1.0)[i])
+        want = check_assign(cuda, s, page, int(s["new"].sum() * (0.7 if i == 2 else 1)) + i, in_place=i % 2 == 0)
+        fits += want[0][-1]
+    assert fits > 0
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1024, 1025, 2100, 4096])
+def test_assign_many_rows(cuda, rows):
+    rng = np.random.default_rng(rows)
+    for tight in (0.4, 1.0):
+        s = requests(rng, rows, 16, cached=90, prompt=60, tight=tight)
+        check_assign(cuda, s, 16, int(s["new"].sum()), in_place=tight == 1.0)
+
+
+@gpu
+def test_assign_of_one_long_prompt_and_most_rows(cuda):
+    rng = np.random.default_rng(0)
+    s = requests(rng, 3, 16)
+    s.update(lens=np.int64([0, 5, 0]), new=np.int64([1, 1, 70001]), done=np.int64([0, 0, 0]), first=np.int64([0, 0, 0]), held=np.int64([0, 1, 0]),
+             table=rng.integers(0, 9, (3, 4400)), free=rng.permutation(6000), n_free=5000)
+    assert check_assign(cuda, s, 16, 80000)[0][-1] == 70003
+    rows = 65535
+    s = dict(lens=np.zeros(rows, np.int64), new=np.ones(rows, np.int64), done=np.zeros(rows, np.int64), first=np.zeros(rows, np.int64), held=np.zeros(rows, np.int64),
+             table=np.zeros((rows, 1), np.int64), free=rng.permutation(rows), n_free=rows - 5)
+    assert check_assign(cuda, s, 8, rows)[0][-1] == rows - 5
+
+
+@gpu
+@pytest.mark.parametrize("outputs", [(), ("positions",), ("slots",)])
+@pytest.mark.parametrize("optional", [(), ("done",), ("first",)])
+def test_assign_without_some_of_its_tensors(cuda, outputs, optional):
+    rng = np.random.default_rng(len(outputs) + 2 * len(optional))
+    s = requests(rng, 40, 16)
+    if "first" not in optional:
+        s["lens"] = np.minimum(s["lens"], s["held"] * 16)
+    check_assign(cuda, s, 16, 0 if not outputs else 5000, places=5000, outputs=outputs, optional=optional)
+    check_assign(cuda, s, 16, 300, places=5000, outputs=outputs, optional=optional, in_place=True)
+
+
+@gpu
+def test_assign_rows_that_cannot_be(cuda):
+    """They get nothing and raise; the others are served as if they were not there."""
+    rng = np.random.default_rng(5)
+    for i in range(12):
+        s = requests(rng, 20, 16, tight=2.0)
+        r = int(rng.integers(0, 20))
+        cols = s["table"].shape[1]
+        for name, value in [(("held", cols + 1),), (("first", s["held"][r] + 1),), (("lens", s["held"][r] * 16 + 1), ("done", 0)), (("new", cols * 16 + 1), ("done", 0)),
+                            (("new", 0xFFFFFFFF), ("done", 0)), (("lens", 0xFFFFFFFF), ("done", 0))][i % 6]:
+            s[name] = s[name].copy()
+            s[name][r] = value
+        assert check_assign(cuda, s, 16, 9000)[6]
+    s = requests(rng, 20, 16)
+    s["n_free"] = len(s["free"]) + 1
+    assert check_assign(cuda, s, 16, 9000)[0][-1] == 0
+    s = requests(rng, 20, 16)
+    s["done"][:] = 1
+    s["free"] = s["free"][:s["n_free"]]
+    want = check_assign(cuda, s, 16, 9000)
+    assert want[6] and want[1] == s["lens"].tolist()
+
+
+@gpu
+def test_assign_slots_beyond_32_bits(cuda):
+    s = dict(lens=np.int64([0, 0]), new=np.int64([2, 2]), done=np.int64([0, 0]), first=np.int64([0, 0]), held=np.int64([0, 0]), table=np.zeros((2, 2), np.int64),
+             free=np.int64([(1 << 28) - 1, 1 << 28]), n_free=2)
+    table, free = s["table"].copy(), s["free"].copy()
+    up = {n: put(cuda, np.asarray(s[n], np.uint32)) for n in ("lens", "new", "held", "table", "free")}
+    n_free, starts, slots = (put(cuda, np.zeros(n, np.uint32) + f) for n, f in ((1, 2), (3, 0), (4, 0)))
+    cuda.paged_assign(up["lens"][0], up["new"][0], 16, up["held"][0], up["table"][0], up["free"][0], n_free[0], starts[0], slots=slots[0])
+    raises_index(cuda)
+    assert (back(cuda, slots[1]).astype(np.int64) & 0xFFFFFFFF).tolist() == [0xFFFFFFFF] * 2 + [0xFFFFFFF0, 0xFFFFFFF1]
+
+
+# ---------------------------------------------------------------- drafted tokens
+
+
+def plain_verify(logits, probs, tokens, starts, uniform, heat, lens):
+    """Row by row in 64 bits: (accepted, next, lens), and the rows that a border is too near for."""
+    out, near = [], set()
+    for r in range(len(starts) - 1):
+        a, b = int(starts[r]), int(starts[r + 1])
+        if a == b:
+            out.append(None)
+            continue
+        T = float(heat[r])
+        for m in range(a, b):
+            x = logits[m].astype(np.float64)
+            x = np.where(np.isnan(x), -np.inf, x)
+            top = x.max()
+            last = m == b - 1
+            if not np.isfinite(top):
+                if last or True:
+                    w = None
+                    break
+            if not T > 0:
+                p = np.zeros_like(x)
+                p[int(np.argmax(x))] = 1.0
+            else:
+                p = np.exp((x - top) / min(max(T, 2.0 ** -100), 2.0 ** 100))
+                p /= p.sum()
+            if last:
+                w = p
+                break
+            d = int(tokens[m + 1])
+            q = np.zeros_like(x) if probs is None else probs[m].astype(np.float64)
+            q = np.where(q > 0, q, 0.0)
+            if probs is None:
+                q[d] = 1.0
+            if T > 0:
+                u = np.float64(uniform[m])
+                stands = u * q[d] < p[d]
+                if abs(u * q[d] - p[d]) <= 2.0 ** -20 * p[d]:
+                    near.add(r)
+            else:
+                stands = p[d] == 1.0
+            if not stands:
+                w = np.maximum(p - q, 0.0) if T > 0 else p
+                if T > 0 and probs is None:
+                    w = p.copy()
+                    w[d] = 0.0
+                if not w.sum() > 0:
+                    w = p
+                break
+        if w is None:
+            token = 0xFFFFFFFF
+        else:
+            c = np.cumsum(w)
+            t = np.float64(uniform[b - 1]) * c[-1]
+            if not T > 0:
+                token = int(np.argmax(w))
+            else:
+                above = np.nonzero((c > t) & (w > 0))[0]
+                token = int(above[0]) if len(above) else int(np.nonzero(w)[0][-1])
+                if len(w) > 1 and np.abs(c[:-1] - t).min() <= 2.0 ** -40 * c[-1] and 0 < t < c[-1]:
+                    near.add(r)
+        out.append((m - a, token, int(lens[r]) - (b - 1 - m)))
+    return out, near
+
+
+class Drafts:
+    """Rows of counts[r] tokens; the drafter's logits are much like the target's."""
+
+    def __init__(self, counts, V, seed=0, store="f32", probs="f32", heat=1.0, peak=True, spread=2.5, spare=1):
+        rng = self.rng = np.random.default_rng(seed)
+        self.counts, self.V, self.store, self.kind = counts, V, store, probs
+        self.starts = np.concatenate([[0], np.cumsum(counts)])
+        M = self.M = int(self.starts[-1]) + spare
+        x = rng.standard_normal((M, V)) * spread
+        if peak:
+            x[np.arange(M), rng.integers(0, V, M)] = math.log(V) + 3.0
+        self.logits = rounded(x, store)
+        d = x + rng.standard_normal((M, V)) * 0.7
+        q = np.exp(d - d.max(1, keepdims=True))
+        q /= q.sum(1, keepdims=True)
+        self.probs = None if probs == "none" else rounded(q, probs)
+        self.tokens = rng.integers(0, V, M)
+        for m in range(M - 1):
+            self.tokens[m + 1] = int(np.argmax(d[m])) if probs == "none" else int(np.argmax(q[m] / rng.exponential(size=V)))
+        self.uniform = rng.random(M).astype(np.float32)
+        self.uniform = np.minimum(self.uniform, np.float32(1 - 2.0 ** -24))
+        rows = len(counts)
+        self.heat = np.full(rows, heat, np.float32) if np.ndim(heat) == 0 else np.resize(np.asarray(heat, np.float32), rows)
+        self.lens = np.array([40 + 3 * r + n for r, n in enumerate(counts)])
+
+
+def device_rows(B, a, store, offset, pad):
+    """Rows `pad` values apart that begin `offset` values into their memory; what is between is NaN."""
+    import torch
+    M, V = a.shape
+    flat = torch.full((offset + M * (V + pad) + 8,), float("nan"), device="cuda").to({"f32": torch.float32, "bf16": torch.bfloat16}[store])
+    x = flat[offset:offset + M * (V + pad)].reshape(M, V + pad)[:, :V]
+    x.copy_(torch.from_numpy(np.ascontiguousarray(a)))
+    torch.cuda.synchronize()
+    return B.from_device(x), flat
+
+
+def check_verify(B, d, offset=0, pad=0, max_new=None, in_place=False, with_heat=True, limit=0.02):
+    logits = device_rows(B, d.logits, d.store, offset, pad)
+    probs = None if d.probs is None else device_rows(B, d.probs, d.kind, offset and 8 - offset, pad // 2)
+    tokens, starts, lens = (put(B, np.asarray(x, np.uint32)) for x in (d.tokens, d.starts, d.lens))
+    uniform, heat = put(B, d.uniform), put(B, d.heat)
+    rows = len(d.counts)
+    out = [put(B, np.full(rows, 77, np.uint32)) for _ in range(3)]
+    if in_place:
+        out[2] = lens
+    B.verify_drafts(logits[0], tokens[0], starts[0], uniform[0], probs=probs and probs[0], temperature=heat[0] if with_heat else None, lens=lens[0],
+                    max_new=max(d.counts) if max_new is None else max_new, out=[x[0] for x in out])
+    got = np.stack([back(B, x[1]).astype(np.int64) & 0xFFFFFFFF for x in out], 1)
+    want, near = plain_verify(d.logits, d.probs, d.tokens, d.starts, d.uniform, d.heat if with_heat else np.ones(rows), d.lens)
+    assert len(near) <= limit * rows + 1, near
+    for r, w in enumerate(want):
+        if w is None:
+            assert got[r].tolist() == [77, 77, int(d.lens[r]) if in_place else 77]
+        elif r not in near:
+            assert got[r].tolist() == list(w), (r, got[r], w)
+    return got
+
+
+COUNTS = [[1], [5], [1, 2, 0, 4, 9], [3] * 20, [0, 0, 1], [6] * 70]
+
+
+@gpu
+@pytest.mark.parametrize("store,probs", [("f32", "f32"), ("f32", "none"), ("bf16", "bf16"), ("bf16", "none"), ("f32", "bf16"), ("bf16", "f32")])
+@pytest.mark.parametrize("V", [1, 2, 3, 7, 31, 64, 257, 1000, 4099])
+@pytest.mark.parametrize("heat", [1.0, 0.0, [0.6, 0.0, 1.7]])
+def test_verify(cuda, store, probs, V, heat):
+    for i, counts in enumerate(COUNTS):
+        check_verify(cuda, Drafts(counts, V, seed=i + V, store=store, probs=probs, heat=heat), in_place=i % 2 == 0, with_heat=heat != 1.0 or i % 3 > 0)
+
+
+@gpu
+@pytest.mark.parametrize("store,probs,V,counts", [("f32", "f32", 50257, [4, 2, 5]), ("bf16", "bf16", 151936, [3, 5]), ("bf16", "none", 256000, [8]), ("f32", "none", 128256, [1, 3, 2]),
+                                                  ("f32", "f32", 1 << 19, [2]), ("bf16", "bf16", (1 << 19) - 3, [2, 2]), ("bf16", "f32", 32000, [4] * 40)])
+def test_verify_whole_vocabularies(cuda, store, probs, V, counts):
+    check_verify(cuda, Drafts(counts, V, seed=V, store=store, probs=probs))
+
+
+@gpu
+@pytest.mark.parametrize("store,probs", [("f32", "f32"), ("bf16", "bf16"), ("bf16", "none")])
+@pytest.mark.parametrize("offset,pad", [(0, 1), (1, 0), (3, 5), (2, 64), (7, 3)])
+def test_verify_rows_that_begin_anywhere(cuda, store, probs, offset, pad):
+    for V in (1, 9, 515, 3001):
+        check_verify(cuda, Drafts([3, 1, 6, 2], V, seed=V, store=store, probs=probs), offset=offset, pad=pad, max_new=0)
+
+
+@gpu
+@pytest.mark.parametrize("store,probs", [("f32", "f32"), ("bf16", "none")])
+@pytest.mark.parametrize("heat", [1.0, 0.0])
+def test_verify_long_rows(cuda, store, probs, heat):
+    """More positions than are held at a time; drafts that nearly all stand."""
+    d = Drafts([40, 9, 17, 33, 1], 600, seed=3, store=store, probs=probs, heat=heat, spread=0.2)
+    d.uniform[:] = d.uniform * 0.2
+    if heat == 0.0:
+        d.tokens[1:] = d.logits.argmax(1)[:-1]
+    got = check_verify(cuda, d)
+    assert got[0, 0] > 8
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+@pytest.mark.parametrize("probs", ["f32", "none"])
+@pytest.mark.parametrize("heat", [1.0, 0.0, 0.3])
+def test_verify_masked_logits(cuda, store, probs, heat):
+    """-inf, the lowest value of the type, and NaN in masked places; all masked; an infinity."""
+    lowest = float(np.float32(-3.0e38))
+    for fill in (-np.inf, lowest, np.nan):
+        d = Drafts([4] * 30, 700, seed=11, store=store, probs=probs, heat=heat)
+        mask = d.rng.random(d.logits.shape) < 0.9
+        mask[np.arange(d.M), d.rng.integers(0, 700, d.M)] = False
+        d.logits[mask] = rounded(np.float32([fill]), store)[0] if np.isfinite(fill) else fill
+        check_verify(cuda, d)
+        d.logits[::5] = fill if not np.isfinite(fill) else -np.inf   # nothing is left of these
+        got = check_verify(cuda, d)
+        assert (got[:, 1] == 0xFFFFFFFF).any()
+        d.logits[1::5, 3] = np.inf
+        check_verify(cuda, d)
+
+
+@gpu
+def test_verify_numbers_at_the_ends(cuda):
+    """u of 0 takes the first token with a weight, of 1 (or none) the last; the drafter's probabilities above the target's, negative and NaN."""
+    for store in ("f32", "bf16"):
+        d = Drafts([1] * 6 + [2] * 6, 900, seed=2, store=store)
+        for u in (0.0, 1.0, 2.0 ** -30, 1 - 2.0 ** -24):
+            d.uniform[:] = u
+            check_verify(cuda, d, limit=1.0 if 0 < u < 1 else 0.02)
+        d.logits[:, 0] = -np.inf
+        d.logits[:, -5:] = -np.inf
+        for u in (0.0, 1.0):
+            d.uniform[:] = u
+            got = check_verify(cuda, d)
+            assert (got[:6, 1] == (1 if u == 0 else 894)).all()
+        d = Drafts([2] * 12, 900, seed=2, store=store)
+        d.probs[:] = 2.0
+        d.uniform[::2] = 0.999
+        check_verify(cuda, d)
+        d.probs[:, ::3] = np.nan
+        d.probs[:, 1::3] = -1.0
+        check_verify(cuda, d)
+
+
+@gpu
+@pytest.mark.parametrize("heat", [1e-30, 2.0 ** -120, 1e-3, 50.0, 1e30, np.inf, np.nan, -1.0])
+def test_verify_temperatures(cuda, heat):
+    for store in ("f32", "bf16"):
+        d = Drafts([3] * 10, 300, seed=9, store=store, heat=heat)
+        check_verify(cuda, d, limit=0.2)
+
+
+@gpu
+def test_verify_equal_logits_go_to_the_first(cuda):
+    for store in ("f32", "bf16"):
+        d = Drafts([3] * 8, 2000, seed=4, store=store, probs="none", heat=0.0)
+        d.logits[:, [17, 900, 1999]] = 30.0
+        d.logits[::2, 5] = 0.0
+        d.tokens[:] = 17
+        got = check_verify(cuda, d)
+        assert (got[:, 0] == 2).all() and (got[:, 1] == 17).all()
+        d.logits[:] = -0.0
+        d.logits[:, 7] = 0.0
+        assert (check_verify(cuda, d)[:, 1] == 0).all()
+
+
+@gpu
+def test_verify_tokens_are_distributed_as_the_targets(cuda):
+    """The first token put out, over many rows of the same logits: within 5 standard deviations of the target's probability, whatever the drafter's."""
+    rows, V = 20000, 7
+    rng = np.random.default_rng(0)
+    logits = np.resize(rng.standard_normal(V) * 1.5, (2 * rows, V)).astype(np.float32)
+    q = rng.random(V)
+    q = (q / q.sum()).astype(np.float32)
+    drafts = rng.choice(V, rows, p=q.astype(np.float64) / q.astype(np.float64).sum())
+    tokens = np.zeros(2 * rows, np.uint32)
+    tokens[1::2] = drafts
+    B = cuda
+    for probs in (np.resize(q, (2 * rows, V)), None):
+        if probs is None:
+            tokens[1::2] = 3
+        out = [put(B, np.zeros(rows, np.uint32)) for _ in range(2)]
+        B.verify_drafts(put(B, logits)[0], put(B, tokens)[0], put(B, np.arange(0, 2 * rows + 1, 2).astype(np.uint32))[0],
+                        put(B, rng.random(2 * rows).astype(np.float32))[0], probs=None if probs is None else put(B, probs)[0], max_new=2,
+                        out=(out[0][0], out[1][0], None))
+        accepted, following = (back(B, x[1]) for x in out)
+        first = np.where(accepted == 1, tokens[1::2], following)
+        p = np.exp(logits[0].astype(np.float64))
+        p /= p.sum()
+        seen = np.bincount(first, minlength=V) / rows
+        assert (np.abs(seen - p) <= 5 * np.sqrt(p * (1 - p) / rows)).all()
+        # a draft stands with probability min(1, p / q): over all drafts sum min(p, q), and p of the one token that has no probabilities
+        stands = p[3] if probs is None else np.minimum(p, q).sum()
+        assert abs(accepted.mean() - stands) <= 5 * math.sqrt(stands * (1 - stands) / rows)
+
+
+@gpu
+def test_verify_rows_that_cannot_be(cuda):
+    import torch
+    B = cuda
+    d = Drafts([3, 4, 2, 3], 100, seed=1)
+    for what in ("draft", "starts", "most", "lens"):
+        tokens, starts, lens = d.tokens.copy(), d.starts.copy(), d.lens.copy()
+        most = 4
+        if what == "draft":
+            tokens[d.starts[1] + 3] = 100
+        elif what == "starts":
+            starts[1] = d.M + 5
+        elif what == "most":
+            most = 3
+        else:
+            lens[1] = 2
+        out = [put(B, np.full(4, 77, np.uint32)) for _ in range(3)]
+        B.verify_drafts(put(B, d.logits)[0], put(B, tokens.astype(np.uint32))[0], put(B, starts.astype(np.uint32))[0], put(B, d.uniform)[0], probs=put(B, d.probs)[0],
+                        lens=put(B, lens.astype(np.uint32))[0], max_new=most, out=[x[0] for x in out])
+        raises_index(B)
+        got = [back(B, x[1]) for x in out]
+        assert all(g[1] == 77 and g[3] != 77 for g in got), what
+        assert what == "starts" or all(g[0] != 77 for g in got)
