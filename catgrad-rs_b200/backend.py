@@ -366,6 +366,8 @@ class CudaBackend(TraitBackend):
             ("cg_paged_attention", [vp, vp, vp, vp, vp, vp, vp, i64, f32, i64, f32, vp], i32),
             ("cg_beam_select", [vp, vp, vp, vp, C.c_uint32, vp, vp, vp, vp], i32),
             ("cg_paged_reorder", [vp, vp, vp, vp, vp, vp, vp], i32),
+            ("cg_paged_shared_floats", [vp, vp, vp, vp, vp, i64, i64], i64),
+            ("cg_paged_shared_attention", [vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, f32, i64, f32, vp, vp], i32),
             ("cg_paged_assign", [vp, vp, vp, vp, vp, i64, i64, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp], i32),
             ("cg_verify_drafts", [vp, vp, vp, vp, vp, vp, vp, vp, i64, vp, vp, vp], i32),
             ("cg_rope_tables", [vp, f32, i32, f32, f32, f32, f32, f32, i32, i64, i64, out, out], i32),
@@ -509,6 +511,24 @@ class CudaBackend(TraitBackend):
             out = self._empty_like_pages(q.shape, k_pages)
         st = self._lib.cg_paged_attention(self._ctx, q._h, k_pages._h, v_pages._h, table._h, starts._h, lens._h, max_new, scale, window, softcap,
                                           out._h)
+        if st:
+            self._check(st)
+        return out
+
+    def paged_shared_work(self, q, k_pages, table, groups, max_new=0, max_shared=0):
+        """Room for the parts of paged_shared_attention calls of these sizes, kept by the caller (cg_paged_shared_floats)."""
+        n = self._lib.cg_paged_shared_floats(self._ctx, q._h, k_pages._h, table._h, groups._h, max_new, max_shared)
+        if n < 0:
+            raise BackendPanic(1, "Shape mismatch in operation: shared attention")
+        return self.zeros((max(n, 1),), F32)
+
+    def paged_shared_attention(self, q, k_pages, v_pages, table, starts, lens, groups, shared, work, max_new=0, max_shared=0, scale=0.0, window=0, softcap=0.0,
+                               out=None):
+        """paged_attention of groups of rows that have their first tokens in common, which are read once for a group (cg_paged_shared_attention)."""
+        if out is None:
+            out = self._empty_like_pages(q.shape, k_pages)
+        st = self._lib.cg_paged_shared_attention(self._ctx, q._h, k_pages._h, v_pages._h, table._h, starts._h, lens._h, groups._h, shared._h, max_new, max_shared,
+                                                 scale, window, softcap, work._h, out._h)
         if st:
             self._check(st)
         return out

@@ -46,6 +46,41 @@ CG_HD int64_t page_of(const PagedRows& p, int64_t row, int64_t pos) {
   return -1;
 }
 
+// Groups of neighbouring rows that have their first tokens in common.
+struct PagedGroups {
+  const uint32_t* rows;    // [n + 1], ascending: group g has the rows rows[g] .. rows[g + 1]
+  const uint32_t* shared;  // [n]: the tokens in common
+  int64_t n;
+  int64_t most;            // tokens in common, at most
+};
+// A group's first row, packed tokens and shared tokens.  False (raised): its numbers cannot be.
+CG_HD bool group_span(const PagedRows& p, const PagedGroups& s, int64_t g, int64_t* row0, int64_t* rows, int64_t* tok0, int64_t* n, int64_t* shared) {
+  const int64_t a = s.rows[g], b = s.rows[g + 1], keys = s.shared[g];
+  *row0 = a;
+  *rows = b - a;
+  *shared = keys;
+  *tok0 = *n = 0;
+  bool ok = a <= b && b <= p.rows && keys <= s.most && keys <= (p.cols << p.lg);
+  if (ok) {
+    const int64_t t0 = p.starts[a], t1 = p.starts[b];
+    *tok0 = t0;
+    *n = t1 - t0;
+    ok = t0 <= t1 && t1 <= p.M;
+  }
+  if (!ok) *p.err = DEV_INDEX;
+  return ok;
+}
+// The row of a packed token of the rows row0 .. row0 + rows (by halving; rows without tokens are passed over), and where the token stands.
+CG_HD int64_t position_of(const PagedRows& p, int64_t row0, int64_t rows, int64_t token) {
+  int64_t lo = row0, hi = row0 + rows;
+  while (hi - lo > 1) {
+    const int64_t mid = (lo + hi) >> 1;
+    if ((int64_t)p.starts[mid] <= token) lo = mid;
+    else hi = mid;
+  }
+  return (int64_t)p.lens[lo] - (int64_t)p.starts[lo + 1] + token;
+}
+
 // The context's device is current while this lives.
 struct OnDevice {
   int before = -1;

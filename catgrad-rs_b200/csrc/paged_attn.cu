@@ -64,7 +64,10 @@ constexpr size_t any_smem() {
   const size_t ring = (size_t)any_ring<T>() * S::STAGE, joined = (size_t)(QR == 64 ? 64 : 80) * S::LV;
   return ((size_t)2 * QR * S::LK + (ring > joined ? ring : joined)) * 4;
 }
-template <typename T, int D, int QR>
+// MODE: which keys of a row.  CHUNK: the queries are a group's, the keys (blockIdx.y) a chunk of what its rows have in common; OWN: those behind that, joined
+// with the chunks (of which the launch before has to be waited for; what comes before that one is complete when this one begins).
+enum KeysOf { ALL, CHUNK, OWN };
+template <typename T, int D, int QR, int MODE>
 __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
   using S = Shape<D, QR>;
   constexpr int GK = S::GK, LK = S::LK, LV = S::LV, RING = any_ring<T>();
@@ -77,16 +80,33 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
   float* part = ring;                   // behind the loop: the warps' outputs [4][16][LV] and, with WK = 4, the block's [16][LV]
   __shared__ float red[2][64], ml[2][QR];
   __shared__ int64_t places[2][GK];     // of the keys of the next tile to be asked for; -1: zeros
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  auto depend = []() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  };
+  if (MODE != OWN) depend();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int rep = a.nh / a.nkv, kvh = (int)blockIdx.x % a.nkv;
-  const int64_t row = blockIdx.y, x0 = (int64_t)(blockIdx.x / a.nkv) * QR;
+  int64_t row = blockIdx.y, x0 = (int64_t)(blockIdx.x / a.nkv) * QR;
   const int slices = (int)gridDim.z, slice = (int)blockIdx.z;
-  int64_t tok0, n, len;
-  if (!row_span(a.rows, row, a.most, &tok0, &n, &len) || x0 >= n * rep) return;  // (the same in all blocks of a cluster)
+  int64_t tok0, n, len, rows_of = 0, from = 0, group = -1;  // CHUNK: the group's rows; OWN: the first key, the group
+  if constexpr (MODE == CHUNK) {
+    int64_t tile, shared;
+    group = group_of_tile(a.rows, a.sh.groups, blockIdx.x / a.nkv, rep, QR, &tile);
+    if (group < 0 || !group_span(a.rows, a.sh.groups, group, &row, &rows_of, &tok0, &n, &shared)) return;
+    if ((int64_t)blockIdx.y * a.sh.chunk >= shared) return;
+    x0 = tile * QR;
+    len = n + min(shared, ((int64_t)blockIdx.y + 1) * a.sh.chunk);  // (so that the keys end before it)
+  } else {
+    if constexpr (MODE == OWN) group = group_of_row(a.sh.groups, row, &from);
+    if (!row_span(a.rows, row, a.most, &tok0, &n, &len) || x0 >= n * rep) {  // (the same in all blocks of a cluster)
+      if (MODE == OWN) depend();
+      return;
+    }
+  }
   const int64_t pos0 = len - n, i0 = x0 / rep, i1 = min(n - 1, (x0 + QR - 1) / rep);
-  const int64_t lo = a.window > 0 ? max((int64_t)0, pos0 + i0 - a.window + 1) : 0, hi = pos0 + i1;
+  const int64_t hi = MODE == CHUNK ? pos0 - 1 : pos0 + i1;
+  const int64_t lo = MODE == CHUNK ? (int64_t)blockIdx.y * a.sh.chunk : max(a.window > 0 ? max((int64_t)0, pos0 + i0 - a.window + 1) : 0, MODE == OWN ? min(from, hi + 1) : 0);
   const int64_t first = lo / GK, tiles = hi / GK + 1 - first, per = (tiles + slices - 1) / slices;
   const int64_t t0 = first + slice * per, t1 = min(first + tiles, t0 + per);
   const int64_t page_mask = ((int64_t)1 << a.rows.lg) - 1;
@@ -162,7 +182,10 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
   }
   // this lane's rows g and g + 8 of the warp's 16
   const int r0 = (QR == 64 ? warp * 16 : 0) + g, key0 = QR == 64 ? 0 : warp * (GK / 4);
-  const int64_t qpos[2] = {pos0 + (x0 + r0) / rep, pos0 + (x0 + r0 + 8) / rep};
+  int64_t qpos[2] = {pos0 + (x0 + r0) / rep, pos0 + (x0 + r0 + 8) / rep};
+  if constexpr (MODE == CHUNK)  // (a token stands where its row says)
+#pragma unroll
+    for (int q = 0; q < 2; ++q) qpos[q] = x0 + r0 + 8 * q < n * rep ? position_of(a.rows, row, rows_of, tok0 + (x0 + r0 + 8 * q) / rep) : hi;
   const float scale = a.scale * 1.4426950408889634f, cap2 = a.cap * 1.4426950408889634f, cap_in = a.cap > 0.f ? a.scale / a.cap : 0.f, cap_unit = -2.f * 1.4426950408889634f * cap_in;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[DG][4][4];
 #pragma unroll
@@ -217,7 +240,7 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
       }
     }
     // (scores and maxima in units of log2)
-    const bool masked = k0 + GK / WK - 1 > pos0 + i0 || k0 < lo || (a.window > 0 && k0 <= hi - a.window);
+    const bool masked = MODE == CHUNK || k0 + GK / WK - 1 > pos0 + i0 || k0 < lo || (a.window > 0 && k0 <= hi - a.window);
     // (conditions stand around the loops: one per score would cut them up)
 #pragma unroll
     for (int i = 0; i < NT; ++i)
@@ -239,9 +262,10 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
       int low[2], lim[2];
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        const int64_t x = qpos[q] - k0;
-        lim[q] = x > GK ? GK : x < -1 ? -1 : (int)x;
+        const int64_t x = qpos[q] - k0, y = MODE == CHUNK ? min(x, hi - k0) : x;
+        lim[q] = y > GK ? GK : y < -1 ? -1 : (int)y;
         low[q] = a.window > 0 ? (x - a.window >= GK ? GK : x - a.window < -1 ? 0 : (int)(x - a.window) + 1) : 0;
+        if (MODE == OWN) low[q] = max(low[q], (int)min(max(from - k0, (int64_t)0), (int64_t)GK));
       }
 #pragma unroll
       for (int i = 0; i < NT; ++i)
@@ -334,9 +358,33 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
       for (int e = 0; e < 2; ++e)
         *(float4*)(part + (warp * 16 + g + 8 * q) * LV + 32 * c + 8 * t4 + 4 * e) = make_float4(o[c][0][2 * q + e], o[c][1][2 * q + e], o[c][2][2 * q + e], o[c][3][2 * q + e]);
   __syncthreads();
-  auto put4 = [&](int x, int col, float4 v, float f) {
-    if (x0 + x >= n * rep || col >= a.d) return;
-    T* to = (T*)a.out + ((tok0 + (x0 + x) / rep) * a.nh + kvh * rep + (x0 + x) % rep) * a.d + col;
+  int chunks = 0;
+  bool there = true;
+  if constexpr (MODE == OWN) {
+    depend();
+    if (group >= 0) {
+      int64_t first_row, rows, t0, tokens, shared;
+      there = group_span(a.rows, a.sh.groups, group, &first_row, &rows, &t0, &tokens, &shared);
+      if (there && (tok0 < t0 || tok0 + n > t0 + tokens)) {  // (starts that do not ascend: the chunks have other tokens)
+        *a.rows.err = DEV_INDEX;
+        there = false;
+      }
+      if (there) chunks = (int)((shared + a.sh.chunk - 1) / a.sh.chunk);
+    }
+  }
+  // the output of query x at four components, v against `top`, whose exponentials' sum is `sum`
+  auto finish = [&](int x, int col, float4 v, float top, float sum) {
+    if (x0 + x >= n * rep || col >= a.d || !there) return;
+    const int64_t at = (tok0 + (x0 + x) / rep) * a.nh + kvh * rep + (x0 + x) % rep;
+    if constexpr (MODE == CHUNK) {
+      const int64_t to = (int64_t)blockIdx.y * a.rows.M * a.nh + at;
+      *(float4*)(a.sh.out + to * a.d + col) = v;
+      if (col == 0) a.sh.ml[to] = make_float2(top, sum);
+      return;
+    }
+    if constexpr (MODE == OWN) join_chunks(a.sh, chunks, a.rows.M * a.nh, at, a.d, col, top, sum, v);
+    const float f = sum > 0.f ? 1.f / sum : 0.f;
+    T* to = (T*)a.out + at * a.d + col;
     store_as(to, v.x * f); store_as(to + 1, v.y * f); store_as(to + 2, v.z * f); store_as(to + 3, v.w * f);
   };
   const float* joined = QR == 64 ? part : part + 64 * LV;
@@ -359,7 +407,7 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
         }
       }
       if (slices == 1) {
-        put4(x, c, v, sum > 0.f ? 1.f / sum : 0.f);
+        finish(x, c, v, top, sum);
       } else {
         *(float4*)(part + (64 + x) * LV + c) = v;
         if (c == 0) { ml[0][x] = top; ml[1][x] = sum; }
@@ -403,22 +451,28 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
       sum = fmaf(ls[s], f, sum);
       v.x = fmaf(os[s].x, f, v.x); v.y = fmaf(os[s].y, f, v.y); v.z = fmaf(os[s].z, f, v.z); v.w = fmaf(os[s].w, f, v.w);
     }
-    put4(x, c, v, sum > 0.f ? 1.f / sum : 0.f);
+    finish(x, c, v, top, sum);
   }
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-template <typename T, int D, int QR>
+template <typename T, int D, int QR, int MODE>
 int launch_any(cg_ctx* c, const PagedAttnArgs& a) {
   constexpr size_t smem = any_smem<T, D, QR>();
   static PerDeviceFlag configured_on;
   bool& configured = configured_on.at(c->core->device);
   if (!configured) {
-    CG_CUDA(c, cudaFuncSetAttribute(k_paged_attn<T, D, QR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    CG_CUDA(c, cudaFuncSetAttribute(k_paged_attn<T, D, QR, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     configured = true;
   }
-  const int64_t tiles = (a.most * (a.nh / a.nkv) + QR - 1) / QR * a.nkv, longest = a.rows.cols << a.rows.lg;
+  const int64_t rep = a.nh / a.nkv, longest = a.rows.cols << a.rows.lg;
+  const int64_t tiles = (MODE == CHUNK ? a.rows.M * rep / QR + a.sh.groups.n : (a.most * rep + QR - 1) / QR) * a.nkv;  // (a group has a tile that is not full)
   if (tiles > 0x7FFFFFFFll) return fail(c, CG_ERR_UNSUPPORTED, "too many tokens");
+  if (MODE == CHUNK) {
+    CG_CUDA(c, launch_kernel(c, k_paged_attn<T, D, QR, MODE>, dim3((unsigned)tiles, (unsigned)a.sh.chunks), dim3(128), smem, 1, a));
+    CG_LAUNCHED(c);
+    return CG_OK;
+  }
   // Shares of the keys.  Us in f32, heads of 64, with 1 / 2 / 4 / 8, [the rule's] (the table's width stands for the lengths):
   //   3 rows of 213 behind 1500, 2 x 2 heads    117  63.1  50.2 [54.7]
   //   1 row of 1000                             70.3 40.8 [30.2] 32.3
@@ -426,20 +480,80 @@ int launch_any(cg_ctx* c, const PagedAttnArgs& a) {
   //   32 of 1800                                42.2 [26.5] 31.2 49.6
   //   1 of 4000                                 80.4 43.5  24.5 [15.1]
   static AtATime known;
-  const int slices = pick_shares([&](int i) { return at_a_time(known, c->core->device, i, k_paged_attn<T, D, QR>, 128, smem); }, 8, tiles * a.rows.rows, longest,
+  const int slices = pick_shares([&](int i) { return at_a_time(known, c->core->device, i, k_paged_attn<T, D, QR, MODE>, 128, smem); }, 8, tiles * a.rows.rows, longest,
                                  Shape<D, QR>::GK, QR == 16 ? 4.5 : 3.5, QR == 16 ? 2.8 : D == 64 ? 2.4 : D == 128 ? 4.5 : 5.,
                                  std::max(0.5, 1. - 0.5 * (double)a.most / (double)std::max<int64_t>(longest, 1)));
-  CG_CUDA(c, launch_kernel(c, k_paged_attn<T, D, QR>, dim3((unsigned)tiles, (unsigned)a.rows.rows, (unsigned)slices), dim3(128), smem, slices, a));
+  CG_CUDA(c, launch_kernel(c, k_paged_attn<T, D, QR, MODE>, dim3((unsigned)tiles, (unsigned)a.rows.rows, (unsigned)slices), dim3(128), smem, slices, a));
   CG_LAUNCHED(c);
   return CG_OK;
 }
 
-template <typename T>
+template <typename T, int MODE>
 int launch_typed(cg_ctx* c, const PagedAttnArgs& a) {
-  const bool few = a.most * (a.nh / a.nkv) <= 32;
-  if (a.d <= 64) return few ? launch_any<T, 64, 16>(c, a) : launch_any<T, 64, 64>(c, a);
-  if (a.d <= 128) return few ? launch_any<T, 128, 16>(c, a) : launch_any<T, 128, 64>(c, a);
-  return few ? launch_any<T, 256, 16>(c, a) : launch_any<T, 256, 64>(c, a);
+  // (of a group there are more queries than of a row)
+  const bool few = (MODE == CHUNK ? a.rows.M : a.most) * (a.nh / a.nkv) <= 32;
+  if (a.d <= 64) return few ? launch_any<T, 64, 16, MODE>(c, a) : launch_any<T, 64, 64, MODE>(c, a);
+  if (a.d <= 128) return few ? launch_any<T, 128, 16, MODE>(c, a) : launch_any<T, 128, 64, MODE>(c, a);
+  return few ? launch_any<T, 256, 16, MODE>(c, a) : launch_any<T, 256, 64, MODE>(c, a);
+}
+
+// What both kinds of attention check of their arguments, and their form for the kernels; `nothing`: there is nothing to do.
+int attention_args(cg_ctx* c, const cg_tensor* q, const cg_tensor* k_pages, const cg_tensor* v_pages, const cg_tensor* table, const cg_tensor* starts,
+                   const cg_tensor* lens, int64_t max_new, float scale, int64_t window, float softcap, const cg_tensor* out, PagedAttnArgs* args, bool* nothing) {
+  PagedAttnArgs& a = *args;
+  if (!q || !out) return fail(c, CG_ERR_INVALID, "null argument");
+  int lg;
+  CG_TRY(check_pages(c, k_pages, v_pages, false, &lg));
+  const int64_t nkv = k_pages->dims[1], d = k_pages->dims[3], any[3] = {-1, -1, d};
+  CG_TRY(check_tensor(c, q, "q", CG_F32, 3, any, false));
+  const int64_t M = q->dims[0], nh = q->dims[1];
+  CG_TRY(check_tensor(c, out, "out", CG_F32, 3, q->dims));
+  CG_TRY(check_rows(c, table, starts, lens, M, k_pages->dims[0], lg, &a.rows));
+  if (q->storage != k_pages->storage || out->storage != k_pages->storage) return fail(c, CG_ERR_DTYPE, "q and out are stored as the pages are");
+  if (M > 0 && q->strides[2] != 1) return fail(c, CG_ERR_UNSUPPORTED, "q: the last axis must be contiguous");
+  if (nkv < 1 || nkv > 65535 || nh > 65535) return fail(c, CG_ERR_UNSUPPORTED, "too many heads");
+  if (nh % nkv) return fail(c, CG_ERR_SHAPE, "query heads are a multiple of key heads");
+  if (max_new < 0 || window < 0 || !(softcap >= 0.f) || !(scale >= 0.f) || scale > 3e38f || softcap > 3e38f) return fail(c, CG_ERR_INVALID, "bad argument");
+  if (overlap_any({q, k_pages, v_pages, table, starts, lens}, {out})) return fail(c, CG_ERR_INVALID, "out overlaps an input");
+  if (M == 0 || nh == 0 || a.rows.rows == 0) {
+    *nothing = true;
+    return CG_OK;
+  }
+  if (k_pages->dims[0] == 0) return fail(c, CG_ERR_SHAPE, "no pages");
+  a.q = q->data(); a.k_pages = k_pages->data(); a.v_pages = v_pages->data(); a.out = out->data();
+  a.q_ld = q->strides[0]; a.q_hs = q->strides[1];
+  a.most = max_new > 0 ? std::min(max_new, M) : M;
+  a.window = window < a.rows.cols << lg ? window : 0;  // (one that reaches over all positions is none)
+  a.scale = scale > 0.f ? scale : 1.f / sqrtf((float)d);
+  // (caps beyond 2^+-100 act as these: all scores are far below the one, and differ by nothing that an exponential shows under the other)
+  a.cap = softcap > 0.f ? fminf(fmaxf(softcap, 0x1p-100f), 0x1p100f) : 0.f;
+  a.nh = (int)nh; a.nkv = (int)nkv; a.d = (int)d;
+  return CG_OK;
+}
+// Attention over all of a row's keys.
+int attend(cg_ctx* c, const PagedAttnArgs& a, bool bf16) {
+  if (bf16 && paged_fa_supported(a)) return paged_fa(c, a);
+  if (bf16 && paged_dec_supported(a)) return paged_dec(c, a);
+  return bf16 ? launch_typed<__nv_bfloat16, ALL>(c, a) : launch_typed<float, ALL>(c, a);
+}
+
+// Into how many chunks shared keys are cut (0: rows read them for themselves).  A function of sizes alone, as the workspace's is.
+// Rows of so many tokens that they fill a tile of 128 queries by themselves gain nothing by others' beside them.
+void plan_chunks(cg_ctx* c, PagedAttnArgs* args, bool bf16) {
+  PagedAttnArgs& a = *args;
+  const int64_t rep = a.nh / a.nkv;
+  a.sh.chunks = 0;
+  a.sh.chunk = 0;
+  if (a.sh.groups.n == 0 || a.sh.groups.most == 0 || a.most * rep > 64) return;
+  if (bf16) {
+    a.sh.chunk = paged_fa_chunk(c, a);
+  } else {
+    // (blocks of 64 queries, or 16: two or four on an SM)
+    const int64_t size = a.rows.M * rep <= 32 ? 16 : 64, tiles = std::max((a.rows.M * rep + size - 1) / size, a.sh.groups.n) * a.nkv;
+    const int64_t chunks = std::max<int64_t>(2 * 148 / tiles, 1);
+    a.sh.chunk = std::max<int64_t>(((a.sh.groups.most + chunks - 1) / chunks + 63) / 64 * 64, 128);
+  }
+  a.sh.chunks = (int)std::min<int64_t>((a.sh.groups.most + a.sh.chunk - 1) / a.sh.chunk, 0x7FFFFFFF);
 }
 
 }  // namespace
@@ -454,33 +568,71 @@ extern "C" int32_t cg_paged_attention(cg_ctx* c, const cg_tensor* q, const cg_te
   if (!c) return CG_ERR_INVALID;
   CG_LAZY_EAGER_SCOPE(c);
   OnDevice on(c);
-  if (!q || !out) return fail(c, CG_ERR_INVALID, "null argument");
   PagedAttnArgs a = {};
-  int lg;
-  CG_TRY(check_pages(c, k_pages, v_pages, false, &lg));
-  const int64_t nkv = k_pages->dims[1], d = k_pages->dims[3], any[3] = {-1, -1, d};
-  CG_TRY(check_tensor(c, q, "q", CG_F32, 3, any, false));
-  const int64_t M = q->dims[0], nh = q->dims[1];
-  CG_TRY(check_tensor(c, out, "out", CG_F32, 3, q->dims));
-  CG_TRY(check_rows(c, table, starts, lens, M, k_pages->dims[0], lg, &a.rows));
-  if (q->storage != k_pages->storage || out->storage != k_pages->storage) return fail(c, CG_ERR_DTYPE, "q and out are stored as the pages are");
-  if (M > 0 && q->strides[2] != 1) return fail(c, CG_ERR_UNSUPPORTED, "q: the last axis must be contiguous");
-  if (nkv < 1 || nkv > 65535 || nh > 65535) return fail(c, CG_ERR_UNSUPPORTED, "too many heads");
-  if (nh % nkv) return fail(c, CG_ERR_SHAPE, "query heads are a multiple of key heads");
-  if (max_new < 0 || window < 0 || !(softcap >= 0.f) || !(scale >= 0.f) || scale > 3e38f || softcap > 3e38f) return fail(c, CG_ERR_INVALID, "bad argument");
-  if (overlap_any({q, k_pages, v_pages, table, starts, lens}, {out})) return fail(c, CG_ERR_INVALID, "out overlaps an input");
-  if (M == 0 || nh == 0 || a.rows.rows == 0) return CG_OK;
-  if (k_pages->dims[0] == 0) return fail(c, CG_ERR_SHAPE, "no pages");
-  a.q = q->data(); a.k_pages = k_pages->data(); a.v_pages = v_pages->data(); a.out = out->data();
-  a.q_ld = q->strides[0]; a.q_hs = q->strides[1];
-  a.most = max_new > 0 ? std::min(max_new, M) : M;
-  a.window = window < a.rows.cols << lg ? window : 0;  // (one that reaches over all positions is none)
-  a.scale = scale > 0.f ? scale : 1.f / sqrtf((float)d);
-  // (caps beyond 2^+-100 act as these: all scores are far below the one, and differ by nothing that an exponential shows under the other)
-  a.cap = softcap > 0.f ? fminf(fmaxf(softcap, 0x1p-100f), 0x1p100f) : 0.f;
-  a.nh = (int)nh; a.nkv = (int)nkv; a.d = (int)d;
+  bool nothing = false;
+  CG_TRY(attention_args(c, q, k_pages, v_pages, table, starts, lens, max_new, scale, window, softcap, out, &a, &nothing));
+  if (nothing) return CG_OK;
   written(out);
-  if (q->storage == ST_BF16 && paged_fa_supported(a)) return paged_fa(c, a);
-  if (q->storage == ST_BF16 && paged_dec_supported(a)) return paged_dec(c, a);
-  return q->storage == ST_BF16 ? launch_typed<__nv_bfloat16>(c, a) : launch_typed<float>(c, a);
+  return attend(c, a, q->storage == ST_BF16);
+}
+
+extern "C" int64_t cg_paged_shared_floats(cg_ctx* c, const cg_tensor* q, const cg_tensor* k_pages, const cg_tensor* table, const cg_tensor* groups,
+                                          int64_t max_new, int64_t max_shared) {
+  if (!c || !q || !k_pages || !table || !groups || q->rank != 3 || k_pages->rank != 4 || table->rank != 2 || groups->rank != 1 || groups->dims[0] < 1 || max_new < 0 ||
+      max_shared < 0 || k_pages->dims[1] < 1 || q->dims[1] % k_pages->dims[1] || q->dims[1] > 65535)
+    return -1;
+  PagedAttnArgs a = {};
+  a.rows.M = q->dims[0];
+  a.nh = (int)q->dims[1];
+  a.nkv = (int)k_pages->dims[1];
+  a.d = (int)k_pages->dims[3];
+  if (a.rows.M == 0 || a.nh == 0) return 0;
+  a.most = max_new > 0 ? std::min(max_new, a.rows.M) : a.rows.M;
+  const int64_t longest = table->dims[1] * k_pages->dims[2];
+  a.sh.groups.n = groups->dims[0] - 1;
+  a.sh.groups.most = max_shared > 0 ? std::min(max_shared, longest) : longest;
+  plan_chunks(c, &a, q->storage == ST_BF16);
+  return a.sh.chunks * a.rows.M * a.nh * (a.d + 2);
+}
+
+extern "C" int32_t cg_paged_shared_attention(cg_ctx* c, const cg_tensor* q, const cg_tensor* k_pages, const cg_tensor* v_pages, const cg_tensor* table,
+                                             const cg_tensor* starts, const cg_tensor* lens, const cg_tensor* groups, const cg_tensor* shared, int64_t max_new,
+                                             int64_t max_shared, float scale, int64_t window, float softcap, cg_tensor* work, cg_tensor* out) {
+  if (!c) return CG_ERR_INVALID;
+  CG_LAZY_EAGER_SCOPE(c);
+  OnDevice on(c);
+  PagedAttnArgs a = {};
+  bool nothing = false;
+  CG_TRY(attention_args(c, q, k_pages, v_pages, table, starts, lens, max_new, scale, window, softcap, out, &a, &nothing));
+  const int64_t any[1] = {-1};
+  CG_TRY(check_tensor(c, groups, "groups", CG_U32, 1, any));
+  if (groups->dims[0] < 1) return fail(c, CG_ERR_SHAPE, "Shape mismatch in operation: groups");
+  const int64_t G[1] = {groups->dims[0] - 1};
+  CG_TRY(check_tensor(c, shared, "shared", CG_U32, 1, G));
+  CG_TRY(check_tensor(c, work, "work", CG_F32, 1, any));
+  if (work->storage != ST_F32) return fail(c, CG_ERR_DTYPE, "work is f32");
+  if (G[0] > 65535) return fail(c, CG_ERR_UNSUPPORTED, "at most 65535 groups");
+  if (max_shared < 0) return fail(c, CG_ERR_INVALID, "bad argument");
+  if (overlap_any({q, k_pages, v_pages, table, starts, lens, groups, shared}, {out, work})) return fail(c, CG_ERR_INVALID, "what is written overlaps an input or each other");
+  if (nothing) return CG_OK;
+  const int64_t longest = a.rows.cols << a.rows.lg;
+  a.sh.groups.rows = (const uint32_t*)groups->data();
+  a.sh.groups.shared = (const uint32_t*)shared->data();
+  a.sh.groups.n = G[0];
+  a.sh.groups.most = max_shared > 0 ? std::min(max_shared, longest) : longest;
+  const bool bf16 = q->storage == ST_BF16;
+  plan_chunks(c, &a, bf16);
+  const int64_t parts = a.sh.chunks * a.rows.M * a.nh;
+  if (work->dims[0] < parts * (a.d + 2)) return fail(c, CG_ERR_SHAPE, "work holds less than cg_paged_shared_floats");
+  if (parts > 0 && (uintptr_t)work->data() % 16) return fail(c, CG_ERR_UNSUPPORTED, "work begins on a 16-byte boundary");
+  written(out);
+  if (parts == 0) return attend(c, a, bf16);
+  if (a.sh.chunks > 65535) return fail(c, CG_ERR_UNSUPPORTED, "too many tokens");
+  written(work);
+  a.sh.out = (float*)work->data();
+  a.sh.ml = (float2*)(a.sh.out + parts * a.d);
+  if (bf16 && paged_fa_prefix_supported(a)) CG_TRY(paged_fa_prefix(c, a));
+  else CG_TRY((bf16 ? launch_typed<__nv_bfloat16, CHUNK>(c, a) : launch_typed<float, CHUNK>(c, a)));
+  if (bf16 && paged_dec_supported(a)) return paged_dec_own(c, a);
+  return bf16 ? launch_typed<__nv_bfloat16, OWN>(c, a) : launch_typed<float, OWN>(c, a);
 }

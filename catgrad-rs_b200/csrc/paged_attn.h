@@ -6,6 +6,17 @@
 
 namespace cg {
 
+// Attention over keys that groups of rows have in common, in two launches: the first has all of a group's queries and a chunk of
+// the shared keys in a block, and leaves per token and head the chunk's output against its own maximum, that maximum (of scores in units of log2) and the sum
+// of exponentials; the second has a row's own keys, and joins them with the chunks.
+struct SharedParts {
+  PagedGroups groups;
+  int64_t chunk;   // keys of a chunk
+  int chunks;      // of the longest prefix
+  float* out;      // [chunks][M][heads][d]
+  float2* ml;      // [chunks][M][heads]
+};
+
 struct PagedAttnArgs {
   PagedRows rows;
   const void *q, *k_pages, *v_pages;
@@ -15,6 +26,7 @@ struct PagedAttnArgs {
   int64_t window;       // 0 = none
   float scale, cap;     // cap 0 = none
   int nh, nkv, d;
+  SharedParts sh;       // (of shared attention)
 };
 
 // Soft-caps c tanh(x / c), in units of log2: kernels take c log2(e) and the factors of a product q k in x / c (`in`) and in the exponent
@@ -25,6 +37,91 @@ constexpr CG_HD float tanh_term(int i) {
        : i == 4 ? 0.019582903012633324f : -0.004716253839433193f;
 }
 #ifdef __CUDACC__
+// By a whole warp: which group and which of its tiles tile `t` of all groups is; -1 if there is none.  A token has `heads` query rows of a tile's `size`.
+__device__ __forceinline__ int64_t group_of_tile(const PagedRows& p, const PagedGroups& s, int64_t t, int64_t heads, int64_t size, int64_t* tile) {
+  const int lane = threadIdx.x & 31;
+  int64_t before = 0;
+  for (int64_t g0 = 0; g0 < s.n; g0 += 32) {
+    int64_t row0, rows, tok0, n, keys, mine = 0;
+    if (g0 + lane < s.n && group_span(p, s, g0 + lane, &row0, &rows, &tok0, &n, &keys) && keys > 0) mine = (n * heads + size - 1) / size;
+    int64_t sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += y;
+    }
+    const uint32_t has = __ballot_sync(0xffffffffu, t < before + sum);
+    if (has) {
+      const int at = __ffs(has) - 1;
+      *tile = t - (before + __shfl_sync(0xffffffffu, sum - mine, at));
+      return g0 + at;
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return -1;
+}
+// By a whole warp: the group of a row (-1: it has none) and the tokens that it shares.
+__device__ __forceinline__ int64_t group_of_row(const PagedGroups& s, int64_t row, int64_t* shared) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t g0 = 0; g0 < s.n; g0 += 32) {
+    const int64_t g = g0 + lane;
+    uint32_t a = 0, b = 0, keys = 0;
+    if (g < s.n) {
+      a = s.rows[g];
+      b = s.rows[g + 1];
+      keys = s.shared[g];
+    }
+    const uint32_t has = __ballot_sync(0xffffffffu, (int64_t)a <= row && row < (int64_t)b);
+    if (has) {
+      const int at = __ffs(has) - 1;
+      *shared = __shfl_sync(0xffffffffu, keys, at);
+      return g0 + at;
+    }
+  }
+  *shared = 0;
+  return -1;
+}
+// Where the queries of a group's rows stand, by a whole warp: the first and the last position (of rows without tokens none).
+__device__ __forceinline__ void group_positions(const PagedRows& p, int64_t row0, int64_t rows, int64_t* first, int64_t* last) {
+  uint32_t lo = 0xffffffffu, hi = 0;
+  for (int64_t i = threadIdx.x & 31; i < rows; i += 32) {
+    const uint32_t len = p.lens[row0 + i], n = p.starts[row0 + i + 1] - p.starts[row0 + i];
+    if (n > 0 && n <= len) {
+      lo = min(lo, len - n);
+      hi = max(hi, len - 1);
+    }
+  }
+  *first = __reduce_min_sync(0xffffffffu, lo);
+  *last = __reduce_max_sync(0xffffffffu, hi);
+}
+// Joins what the chunks left of a token's head (place `at` = token heads + head) at four components with the row's own output v, against `top`, and its sum.
+__device__ __forceinline__ void join_chunks(const SharedParts& s, int n, int64_t per_chunk, int64_t at, int64_t d, int col, float& top, float& sum, float4& v) {
+  for (int c0 = 0; c0 < n; c0 += 4) {  // (four on their way at a time)
+    float2 ml[4];
+    float4 o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ml[i] = make_float2(-INFINITY, 0.f);
+      o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (c0 + i < n) {
+        const int64_t x = (c0 + i) * per_chunk + at;
+        ml[i] = __ldcg(s.ml + x);
+        o[i] = __ldcg((const float4*)(s.out + x * d + col));
+      }
+    }
+    const float before = top;
+    top = fmaxf(fmaxf(fmaxf(top, ml[0].x), fmaxf(ml[1].x, ml[2].x)), ml[3].x);
+    const float base = top == -INFINITY ? 0.f : top, f0 = fast_exp2(before - base);
+    sum *= f0;
+    v.x *= f0; v.y *= f0; v.z *= f0; v.w *= f0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float f = fast_exp2(ml[i].x - base);
+      sum = fmaf(ml[i].y, f, sum);
+      v.x = fmaf(o[i].x, f, v.x); v.y = fmaf(o[i].y, f, v.y); v.z = fmaf(o[i].z, f, v.z); v.w = fmaf(o[i].w, f, v.w);
+    }
+  }
+}
 __device__ __forceinline__ float soft_cap_near(float y, float cap_log2e) {
   const float u = y * y;
   float f = tanh_term(5);
@@ -43,9 +140,13 @@ __device__ __forceinline__ float soft_cap(float x, float cap_log2e, float in, fl
 // Prompts in bf16 on tcgen05 (paged_fa.cu)
 bool paged_fa_supported(const PagedAttnArgs& a);
 int paged_fa(cg_ctx* c, const PagedAttnArgs& a);
+bool paged_fa_prefix_supported(const PagedAttnArgs& a);
+int paged_fa_prefix(cg_ctx* c, const PagedAttnArgs& a);  // the chunks of shared keys
+int64_t paged_fa_chunk(cg_ctx* c, const PagedAttnArgs& a);
 // A few tokens per row, bf16 (paged_dec.cu)
 bool paged_dec_supported(const PagedAttnArgs& a);
 int paged_dec(cg_ctx* c, const PagedAttnArgs& a);
+int paged_dec_own(cg_ctx* c, const PagedAttnArgs& a);    // the rows' own keys, joined with the chunks
 
 // ---- into how many shares a row's keys are cut ----
 constexpr int SHARES = 5;  // 1, 2, 4, 8 or 16: the blocks of a cluster

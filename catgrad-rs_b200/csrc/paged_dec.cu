@@ -35,6 +35,7 @@ struct DecArgs {
   int64_t q_ld, q_hs, most, window, pool_rows;
   int nh, nkv, rep, d;
   float scale_log2e, cap_log2e, cap_in, cap_unit;
+  SharedParts sh;
 };
 
 // keys of a warp's tile, tiles of its ring
@@ -46,7 +47,10 @@ __host__ __device__ constexpr size_t dec_ring() { return (size_t)4 * RING * 2 * 
 template <int D>
 __host__ __device__ constexpr size_t dec_smem() { return 1024 + dec_ring<D>() + 4 * RING * 8; }
 
-template <int D, int ROWS, bool CAP>
+// OWN: of a row in a group only the keys behind the group's prefix; the chunks of that, which the launch before leaves, are joined at the
+// end.  What comes before that launch is complete when this one begins (it waits for it before it lets this one begin), so
+// only the chunks are waited for.
+template <int D, int ROWS, bool CAP, bool OWN>
 __global__ void __launch_bounds__(128)
 k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, DecArgs p) {
   constexpr int KT = dec_keys<D>(), SUB = D / 64, NB = ROWS / 8, KS = D / 16, LD = D + 4;
@@ -73,13 +77,21 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
   const int slices = (int)gridDim.z, slice = (int)blockIdx.z, lg_slices = 31 - __clz(slices);
   const int lg = p.rows.lg, box = min(1 << lg, KT), parts = KT / box;
   const int my_part = lane % parts, my_sub = lane / parts % SUB, my_pool = lane / (parts * SUB);  // (keys, values; others have nothing)
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  auto depend = []() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  };
+  if (!OWN) depend();
 
   int64_t tok0, n, len;
-  if (!row_span(p.rows, row, p.most, &tok0, &n, &len) || x0 >= n * rep) return;  // (the same in all blocks of a cluster)
+  int64_t from = 0, group = -1;  // OWN: the first key, the row's group
+  if (OWN) group = group_of_row(p.sh.groups, row, &from);
+  if (!row_span(p.rows, row, p.most, &tok0, &n, &len) || x0 >= n * rep) {  // (the same in all blocks of a cluster)
+    if (OWN) depend();
+    return;
+  }
   const int64_t pos0 = len - n, i1 = min(n - 1, (int64_t)i_end);
-  const int64_t lo = p.window > 0 ? max((int64_t)0, pos0 + i0 - p.window + 1) : 0, hi = pos0 + i1;
+  const int64_t hi = pos0 + i1, lo = max(p.window > 0 ? max((int64_t)0, pos0 + i0 - p.window + 1) : 0, OWN ? min(from, hi + 1) : 0);
   const int64_t first = (int64_t)((uint64_t)lo / KT), tiles = (int64_t)((uint64_t)hi / KT) + 1 - first, share = (tiles + slices - 1) >> lg_slices;
   const int64_t end = min(first + tiles, first + (slice + 1) * share);
 
@@ -181,7 +193,7 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
     for (int i = 0; i < KT / 8; ++i)
 #pragma unroll
       for (int e = 0; e < 2 * NB; ++e) s[i][e] += s2[i][e];
-    const bool masked = k0 + KT - 1 > pos0 + i0 || (p.window > 0 && k0 <= hi - p.window);
+    const bool masked = k0 + KT - 1 > pos0 + i0 || (p.window > 0 && k0 <= hi - p.window) || (OWN && k0 < from);
     float top[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) top[b] = -INFINITY;
@@ -196,7 +208,7 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
           else x *= p.scale_log2e;
           if (masked) {
             const int64_t key = k0 + i * 8 + t2 + e;
-            if (key > qpos[b] || (p.window > 0 && key <= qpos[b] - p.window)) x = -INFINITY;
+            if (key > qpos[b] || (p.window > 0 && key <= qpos[b] - p.window) || (OWN && key < from)) x = -INFINITY;
           }
           top[b] = fmaxf(top[b], x);
         }
@@ -269,6 +281,24 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
       for (int e = 0; e < 4; ++e) red_o[(warp * ROWS + b * 8 + t2 + (e & 1)) * LD + k * 16 + g + (e >> 1) * 8] = o[k][b][e];
   __syncthreads();
   auto out_at = [&](uint32_t x) { return p.out + ((tok0 + x / rep) * p.nh + kvh * rep + x % rep) * (int64_t)p.d; };
+  int chunks = 0;
+  if (OWN) {
+    depend();
+    if (group >= 0) {
+      int64_t row0, rows, t0, tokens, shared;
+      bool there = group_span(p.rows, p.sh.groups, group, &row0, &rows, &t0, &tokens, &shared);
+      if (there && (tok0 < t0 || tok0 + n > t0 + tokens)) {  // (starts that do not ascend: the chunks have other tokens)
+        *p.rows.err = DEV_INDEX;
+        there = false;
+      }
+      if (!there) aborted = 1;
+      else chunks = (int)((shared + p.sh.chunk - 1) / p.sh.chunk);
+    }
+    __syncthreads();
+  }
+  auto join = [&](uint32_t x, int c, float& top, float& sum, float4& v) {
+    if (OWN && chunks > 0) join_chunks(p.sh, chunks, p.rows.M * p.nh, (tok0 + x / rep) * p.nh + kvh * rep + x % rep, p.d, c, top, sum, v);
+  };
   for (int i = tid; i < ROWS * (D / 4); i += 128) {
     const int r = i / (D / 4), c = i % (D / 4) * 4;
     const float top = fmaxf(fmaxf(red_m[0][r], red_m[1][r]), fmaxf(red_m[2][r], red_m[3][r])), mc = top == -INFINITY ? 0.f : top;
@@ -285,6 +315,8 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
       *(float4*)(part + r * LD + c) = v;
       if (c == 0) { cta_m[r] = top; cta_l[r] = sum; }
     } else if (x0 + r < n * rep && c < p.d && !aborted) {
+      float m_all = top;
+      join(x0 + r, c, m_all, sum, v);
       const float f = sum > 0.f ? 1.f / sum : 0.f;
       *(uint2*)(out_at(x0 + r) + c) = make_uint2(pack_bf16(v.x * f, v.y * f), pack_bf16(v.z * f, v.w * f));
     }
@@ -328,6 +360,7 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
       }
     }
     if (c < p.d && !aborted) {
+      join(x0 + r, c, top, sum, v);
       const float f = sum > 0.f ? 1.f / sum : 0.f;
       *(uint2*)(out_at(x0 + r) + c) = make_uint2(pack_bf16(v.x * f, v.y * f), pack_bf16(v.z * f, v.w * f));
     }
@@ -335,18 +368,19 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
   cluster_sync_all();
 }
 
-template <int D, int ROWS, bool CAP>
+template <int D, int ROWS, bool CAP, bool OWN>
 int launch(cg_ctx* c, const PagedAttnArgs& a) {
   constexpr size_t smem = dec_smem<D>();
   static PerDeviceFlag configured_on;
   bool& configured = configured_on.at(c->core->device);
   if (!configured) {
-    CG_CUDA(c, cudaFuncSetAttribute(k_paged_dec<D, ROWS, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    CG_CUDA(c, cudaFuncSetAttribute(k_paged_dec<D, ROWS, CAP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    CG_CUDA(c, cudaFuncSetAttribute(k_paged_dec<D, ROWS, CAP, OWN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    CG_CUDA(c, cudaFuncSetAttribute(k_paged_dec<D, ROWS, CAP, OWN>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     configured = true;
   }
   DecArgs p;
   p.rows = a.rows;
+  p.sh = a.sh;
   p.q = (const __nv_bfloat16*)a.q;
   p.out = (__nv_bfloat16*)a.out;
   p.q_ld = a.q_ld; p.q_hs = a.q_hs;
@@ -376,18 +410,18 @@ int launch(cg_ctx* c, const PagedAttnArgs& a) {
   //   12 x 4, 167, d 256                        7.5 [7.9]  12.7  24.8  47.7
   // (Lengths are on the device, so the table's width stands for them: 32 x 8 rows of 530 with columns for 32768 tokens get 2 shares, 23.4 us.)
   static AtATime known;
-  const int slices = pick_shares([&](int i) { return at_a_time(known, c->core->device, i, k_paged_dec<D, ROWS, CAP>, 128, smem); }, 16, groups * a.rows.rows, longest,
+  const int slices = pick_shares([&](int i) { return at_a_time(known, c->core->device, i, k_paged_dec<D, ROWS, CAP, OWN>, 128, smem); }, 16, groups * a.rows.rows, longest,
                                  4 * dec_keys<D>(), 4., D == 64 ? 0.7 : D == 128 ? 0.75 : 1.25, 0.);
-  CG_CUDA(c, launch_kernel(c, k_paged_dec<D, ROWS, CAP>, dim3((unsigned)groups, (unsigned)a.rows.rows, (unsigned)slices), dim3(128), smem, slices, mk, mv, p));
+  CG_CUDA(c, launch_kernel(c, k_paged_dec<D, ROWS, CAP, OWN>, dim3((unsigned)groups, (unsigned)a.rows.rows, (unsigned)slices), dim3(128), smem, slices, mk, mv, p));
   CG_LAUNCHED(c);
   return CG_OK;
 }
 
-template <int D>
+template <int D, bool OWN>
 int pick(cg_ctx* c, const PagedAttnArgs& a) {
   const bool cap = a.cap > 0.f;
-  if (a.most * (a.nh / a.nkv) <= 8) return cap ? launch<D, 8, true>(c, a) : launch<D, 8, false>(c, a);
-  return cap ? launch<D, 16, true>(c, a) : launch<D, 16, false>(c, a);
+  if (a.most * (a.nh / a.nkv) <= 8) return cap ? launch<D, 8, true, OWN>(c, a) : launch<D, 8, false, OWN>(c, a);
+  return cap ? launch<D, 16, true, OWN>(c, a) : launch<D, 16, false, OWN>(c, a);
 }
 
 }  // namespace
@@ -398,9 +432,15 @@ bool paged_dec_supported(const PagedAttnArgs& a) {
 }
 
 int paged_dec(cg_ctx* c, const PagedAttnArgs& a) {
-  if (a.d <= 64) return pick<64>(c, a);
-  if (a.d <= 128) return pick<128>(c, a);
-  return pick<256>(c, a);
+  if (a.d <= 64) return pick<64, false>(c, a);
+  if (a.d <= 128) return pick<128, false>(c, a);
+  return pick<256, false>(c, a);
+}
+
+int paged_dec_own(cg_ctx* c, const PagedAttnArgs& a) {
+  if (a.d <= 64) return pick<64, true>(c, a);
+  if (a.d <= 128) return pick<128, true>(c, a);
+  return pick<256, true>(c, a);
 }
 
 }  // namespace cg

@@ -319,6 +319,20 @@ int32_t cg_paged_append(cg_ctx*, const cg_tensor* q, const cg_tensor* k, const c
 int32_t cg_paged_attention(cg_ctx*, const cg_tensor* q, const cg_tensor* k_pages, const cg_tensor* v_pages,
                            const cg_tensor* table, const cg_tensor* starts, const cg_tensor* lens, int64_t max_new,
                            float scale, int64_t window, float softcap, cg_tensor* out);
+/* The same where rows have their first tokens in common, as behind one system prompt or document: these are read once for all rows of a
+ * group.  Group g of groups [G + 1] (U32, ascending) has the rows groups[g] .. groups[g + 1], whose first shared[g] (U32 [G]) cached tokens are the
+ * same: their tables name the same pages there, or pages that hold the same.  Rows outside all groups share nothing.  Results are
+ * cg_paged_attention's but for the order of sums (in bf16, probabilities of shared tokens have one bf16 part); windows and new tokens may begin
+ * inside the prefix, and all of it is read.  max_shared: no group shares more (0 = not known: the table's width); a group that
+ * does, or whose numbers cannot be, is left out (CG_ERR_INDEX).  work F32 [n]: room for what is joined at the end, written over, n at
+ * least cg_paged_shared_floats of the same tensors and numbers (-1: they do not fit each other); calls that may overlap in time, as
+ * captured graphs on two streams, need one each.  Rows with many new tokens read the prefix for themselves, which costs them nothing. */
+int64_t cg_paged_shared_floats(cg_ctx*, const cg_tensor* q, const cg_tensor* k_pages, const cg_tensor* table, const cg_tensor* groups,
+                               int64_t max_new, int64_t max_shared);
+int32_t cg_paged_shared_attention(cg_ctx*, const cg_tensor* q, const cg_tensor* k_pages, const cg_tensor* v_pages,
+                                  const cg_tensor* table, const cg_tensor* starts, const cg_tensor* lens, const cg_tensor* groups,
+                                  const cg_tensor* shared, int64_t max_new, int64_t max_shared, float scale, int64_t window, float softcap,
+                                  cg_tensor* work, cg_tensor* out);
 /* One step of beam search for groups of J beams: of the continuations (beam j, token v) with
  *   scores[j] + log softmax(logits[j])[v]
  * the K largest in descending order, equal ones (in 64 bits) by j, then v; beams of the same logits and

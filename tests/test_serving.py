@@ -497,3 +497,212 @@ def test_verify_rows_that_cannot_be(cuda):
         got = [back(B, x[1]) for x in out]
         assert all(g[1] == 77 and g[3] != 77 for g in got), what
         assert what == "starts" or all(g[0] != 77 for g in got)
+
+
+# ---------------------------------------------------------------- attention over shared prefixes
+
+
+class Shared:
+    """Groups (rows, shared tokens), between them rows of none (shared None); new[r] tokens of row r, `own[r]` cached ones behind the prefix with them.  Full pages of a prefix
+    are one for all rows, its begun page is copied."""
+
+    def __init__(self, groups, new, own, page, seed=0, spare=0, extra=1):
+        rng = self.rng = np.random.default_rng(seed)
+        self.page, self.new = page, new
+        first, shared, prefix = [], [], []
+        r = 0
+        for n, s in groups:
+            if s is not None:
+                if first and first[-1] != r:   # rows of none in between: a group that shares nothing
+                    shared.append(0)
+                    first.append(r)
+                elif not first:
+                    first.append(r)
+                shared.append(s)
+                first.append(r + n)
+            prefix += [s or 0] * n
+            r += n
+        self.groups, self.shared = first or [0], shared
+        self.total = [p + o for p, o in zip(prefix, own)]
+        self.prefix = prefix
+        rows = len(new)
+        self.starts = np.concatenate([[0], np.cumsum(new)])
+        self.M = int(self.starts[-1]) + spare
+        self.cols = max(-(-t // page) for t in self.total) + extra
+        self.n_pages = rows * self.cols + 3
+        self.table = rng.permutation(self.n_pages)[:rows * self.cols].reshape(rows, self.cols)
+        r = 0
+        for n, s in groups:
+            if s:
+                self.table[r:r + n, :s // page] = self.table[r, :s // page]
+            r += n
+
+    def pool(self, nkv, d, store, stale):
+        """Pages whose places that are nobody's hold `stale`."""
+        x = rounded(self.rng.standard_normal((self.n_pages, nkv, self.page, d)), store)
+        used = np.zeros((self.n_pages, self.page), bool)
+        begin = 0
+        for r, t in enumerate(self.total):
+            s = self.prefix[r]
+            if not (r and s == self.prefix[r - 1] and (self.table[r, :s // self.page] == self.table[r - 1, :s // self.page]).all() and self.same_group(r)):
+                begin = r
+            c, k = divmod(s, self.page)
+            if k:
+                x[self.table[r, c], :, :k] = x[self.table[begin, c], :, :k]
+            at = np.arange(t)
+            used[self.table[r, at // self.page], at % self.page] = True
+        if stale is not None:
+            x.transpose(0, 2, 1, 3)[~used] = stale
+        return x
+
+    def same_group(self, r):
+        return any(a < r < b for a, b in zip(self.groups, self.groups[1:]))
+
+    def gather(self, pages, r):
+        at = np.arange(self.total[r])
+        return pages[self.table[r, at // self.page], :, at % self.page]
+
+
+def check_shared(B, b, store, nh, nkv, d, window=0, cap=0.0, scale=0.0, spread=1.5, stale=np.nan, strided=False, offset=None, max_new=None, max_shared=None, repeat=1):
+    import torch
+    rng = b.rng
+    k, v = (b.pool(nkv, d, store, stale) for _ in range(2))
+    q = rounded(rng.standard_normal((b.M, nh, d)) * spread, store)
+    old = rounded(rng.standard_normal((b.M, nh, d)), store)
+    out, kd, vd = put(B, old, store), put(B, k, store), put(B, v, store)
+    if strided or offset is not None:
+        flat = torch.zeros(b.M * (nh + 3) * (d + 8) + (offset or 0), device="cuda").to(kd[1].dtype)
+        wide = flat[offset or 0:].reshape(b.M, nh + 3, d + 8)[:, :nh, :d] if strided else flat[offset:offset + q.size].reshape(q.shape)
+        wide.copy_(torch.from_numpy(q))
+        torch.cuda.synchronize()
+        qd = (B.from_device(wide), flat)
+    else:
+        qd = put(B, q, store)
+    table, starts, lens, groups, shared = (put(B, np.asarray(x, np.uint32)) for x in (b.table, b.starts, b.total, b.groups, b.shared))
+    most, longest = max(b.new) if max_new is None else max_new, max(b.shared + [1]) if max_shared is None else max_shared
+    work = B.paged_shared_work(qd[0], kd[0], table[0], groups[0], max_new=most, max_shared=longest)
+    for _ in range(repeat):
+        B.paged_shared_attention(qd[0], kd[0], vd[0], table[0], starts[0], lens[0], groups[0], shared[0], work, max_new=most, max_shared=longest, scale=scale,
+                                 window=window, softcap=cap, out=out[0])
+    got = back(B, out[1])
+    want, lim = old.astype(np.float64), np.zeros((b.M, nh, d))
+    f = scale or 1.0 / math.sqrt(d)
+    for r, (n, t) in enumerate(zip(b.new, b.total)):
+        kk, vv = (b.gather(x, r).astype(np.float64) for x in (k, v))
+        for i in range(n):
+            m, pos = int(b.starts[r]) + i, t - n + i
+            lo = max(0, pos - window + 1) if window else 0
+            want[m], mass, size = attention(q[m].astype(np.float64), kk[lo:pos + 1], vv[lo:pos + 1], pos - lo, f, 0, cap)
+            off = 2 * (d + 6) * F32 * size[:, None] + (pos - lo + 24) * F32
+            lim[m] = off * np.abs(vv[lo:pos + 1]).max() + (BF16 * (np.abs(want[m]) + 2 * mass) * (1 + 2.0 ** -7) if store == "bf16" else 0)
+    bad = ~(np.abs(got - want) <= lim)
+    assert not bad.any(), (bad.sum(), np.argwhere(bad)[:4], np.abs(got - want).max())
+    return work.shape[0]
+
+
+# (rows, shared tokens) of the groups, new tokens, own cached tokens with them
+GROUPS = [([(1, 1)], [1], [1]), ([(3, 40)], [1, 1, 1], [1, 9, 30]), ([(2, 129), (3, 64)], [1, 2, 3, 1, 0], [5, 2, 40, 1, 0]),
+          ([(2, None), (4, 300), (1, None), (2, 77)], [1, 1, 4, 1, 2, 1, 3, 1, 1], [100, 3, 4, 70, 20, 1, 33, 200, 1]),
+          ([(9, 513)], [1] * 9, [1 + 11 * r for r in range(9)]), ([(40, 200), (1, 5), (3, 0)], [1] * 44, [1 + r for r in range(44)]),
+          ([(3, 640)], [5, 8, 2], [8, 64, 65]), ([(2, None)], [1, 2], [30, 40])]
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+@pytest.mark.parametrize("nh,nkv,d", [(4, 2, 64), (8, 1, 128), (2, 2, 256), (3, 3, 24), (6, 2, 96), (32, 4, 128), (8, 2, 40), (5, 1, 64)])
+@pytest.mark.parametrize("window,cap", [(0, 0.0), (70, 0.0), (0, 3.0), (33, 20.0)])
+def test_shared_attention(cuda, store, nh, nkv, d, window, cap):
+    for i, (groups, new, own) in enumerate(GROUPS):
+        check_shared(cuda, Shared(groups, new, own, (8, 16, 64, 256)[i % 4], seed=i, spare=i % 3), store, nh, nkv, d, window, cap, scale=0.0 if i % 3 else 0.3, strided=i % 2 == 1)
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+@pytest.mark.parametrize("nh,nkv,d", [(4, 2, 64), (8, 2, 128), (2, 1, 256)])
+@pytest.mark.parametrize("page", [8, 32, 1024])
+def test_shared_attention_many_chunks(cuda, store, nh, nkv, d, page):
+    """Prefixes of many chunks and of hardly more than some, that end anywhere."""
+    for i, shared in enumerate((127, 128, 129, 256, 1000, 3001)):
+        b = Shared([(3, shared), (2, shared // 2)], [1, 2, 1, 1, 3], [1, 5, 70, 33, 3], page, seed=i)
+        floats = check_shared(cuda, b, store, nh, nkv, d, repeat=2)
+        assert shared < 1000 or floats > 2 * b.M * nh * (d + 2)   # (several chunks)
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+@pytest.mark.parametrize("nh,nkv,d", [(4, 1, 64), (16, 2, 128), (4, 2, 256)])
+def test_shared_attention_many_queries(cuda, store, nh, nkv, d):
+    """Groups whose queries fill more than a tile, and rows that fill one by themselves."""
+    check_shared(cuda, Shared([(70, 300), (20, 129)], [1 + r % 4 for r in range(90)], [4 + r for r in range(90)], 16, seed=1), store, nh, nkv, d)
+    check_shared(cuda, Shared([(3, 500)], [150, 3, 40], [150, 60, 41], 16, seed=2), store, nh, nkv, d)
+    check_shared(cuda, Shared([(1, 200)] * 50, [1] * 50, [2] * 50, 16, seed=3), store, nh, nkv, d)
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+@pytest.mark.parametrize("window", [0, 5, 64, 150])
+def test_shared_attention_tokens_inside_the_prefix(cuda, store, window):
+    """New tokens that stand before the prefix's end, rows that end there, and rows shorter than that."""
+    b = Shared([(4, 200)], [3, 5, 1, 8], [2, 0, 30, 4], 16, seed=4)
+    assert [t - n for n, t in zip(b.new, b.total)][1] < 200
+    for d in (64, 128):
+        check_shared(cuda, b, store, 4, 2, d, window)
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+@pytest.mark.parametrize("offset", [1, 2, 8])
+def test_shared_attention_of_unaligned_queries(cuda, store, offset):
+    for d in (64, 128, 40):
+        check_shared(cuda, Shared([(4, 200), (2, 70)], [1, 2, 3, 1, 1, 1], [3, 9, 30, 1, 5, 6], 16, seed=offset), store, 4, 2, d, offset=offset)
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+def test_shared_attention_without_its_numbers(cuda, store):
+    """max_new and max_shared not known: the packed tokens and the table's width stand for them."""
+    for new in ([1, 2, 3, 1, 1, 1], [1, 20, 3, 1, 1, 1]):
+        b = Shared([(4, 200), (2, 70)], new, [3, 29, 30, 1, 5, 6], 16, seed=6, extra=40)
+        check_shared(cuda, b, store, 4, 2, 64, max_new=0, max_shared=0)
+        check_shared(cuda, b, store, 4, 2, 128, max_new=0, max_shared=200)
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+def test_shared_attention_groups_that_cannot_be(cuda, store):
+    """Such a group's rows are left as they were, and the others are not."""
+    B = cuda
+    nh, nkv, d = 4, 2, 64
+    for what in ("order", "rows", "shared", "starts"):
+        b = Shared([(2, 100), (2, 150)], [1, 1, 1, 2], [5, 6, 7, 8], 16, seed=7)
+        k, v = (put(B, b.pool(nkv, d, store, None), store) for _ in range(2))
+        groups, shared, starts = list(b.groups), list(b.shared), b.starts.copy()
+        if what == "order":
+            groups = [0, 4, 2]
+        elif what == "rows":
+            groups = [0, 2, 5]
+        elif what == "shared":
+            shared[1] = 151
+        else:
+            starts[4] = 99
+        q, out = put(B, rounded(b.rng.standard_normal((b.M, nh, d)), store), store), put(B, np.full((b.M, nh, d), 7.0, np.float32), store)
+        up = [put(B, np.asarray(x, np.uint32))[0] for x in (b.table, starts, b.total, groups, shared)]
+        work = B.paged_shared_work(q[0], k[0], up[0], up[3], max_new=2, max_shared=150)
+        B.paged_shared_attention(q[0], k[0], v[0], *up, work, max_new=2, max_shared=150, out=out[0])
+        raises_index(B)
+        got = back(B, out[1])
+        assert np.isfinite(got).all()
+        if what != "order":
+            assert (got[:2] != 7.0).all()
+        if what in ("rows", "shared"):
+            assert (got[2:] == 7.0).all()
+    # pages that do not exist count as zeros, and are not read
+    b = Shared([(2, 100)], [1, 1], [5, 6], 16, seed=7)
+    k, v = (put(B, b.pool(nkv, d, store, None), store) for _ in range(2))
+    b.table[0, 2] = b.n_pages + 4
+    q, out = put(B, rounded(b.rng.standard_normal((b.M, nh, d)), store), store), put(B, np.full((b.M, nh, d), 7.0, np.float32), store)
+    up = [put(B, np.asarray(x, np.uint32))[0] for x in (b.table, b.starts, b.total, b.groups, b.shared)]
+    work = B.paged_shared_work(q[0], k[0], up[0], up[3], max_new=1, max_shared=100)
+    B.paged_shared_attention(q[0], k[0], v[0], *up, work, max_new=1, max_shared=100, out=out[0])
+    raises_index(B)
+    assert np.isfinite(back(B, out[1])).all()
