@@ -12,6 +12,7 @@
 // A cluster has a row, its blocks equal slices of the vocabulary.  Logits are read once: a position's slice stays in shared memory, where
 // the draw finds it; positions behind the first rejected draft are not read unless they were asked for ahead.
 #include <algorithm>
+#include <type_traits>
 
 #include "mma.cuh"
 #include "paged.h"
@@ -23,9 +24,8 @@ namespace {
 
 using namespace tc;
 
-constexpr int VT = 512;          // threads of a block
 constexpr int MOST_BLOCKS = 16;  // of a cluster
-constexpr int MOST_AHEAD = 8;    // positions in shared memory
+constexpr int MOST_AHEAD = 8;    // positions judged at a time
 constexpr uint32_t NONE = 0xFFFFFFFFu;
 constexpr float NO_LOGIT = -INFINITY;
 
@@ -37,29 +37,42 @@ struct VerifyArgs {
   uint32_t *accepted, *next, *lens_out;
   int64_t rows, M, V, most;
   int slice;                   // tokens of a block
-  int ahead;                   // positions asked for at a time
+  int ahead;                   // positions judged at a time
   int probs16;
-  uint32_t stride;             // bytes of a position in shared memory
+  int staged;                  // the drafter's probabilities that are drawn from go through shared memory
   int32_t* err;
 };
 
-template <typename T>
-__device__ __forceinline__ float widen(T x);
-template <>
-__device__ __forceinline__ float widen<float>(float x) { return x; }
-template <>
-__device__ __forceinline__ float widen<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
-
+__device__ __forceinline__ float widen(float x) { return x; }
+__device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
 // (NaN counts as -inf)
 template <typename T>
 __device__ __forceinline__ float logit(T x) { return fmaxf(widen(x), NO_LOGIT); }
 
-__device__ __forceinline__ double exp64(double x) { return exp(x); }
-
+// e^x for x <= 0 to 2^-46 and better by Tang's method (1989): x = (16 m + j) ln2 / 16 + r, 2^(j/16) from a table (whose 16 values lie in different
+// banks), e^r by its series: 12 operations in 64 bits, where exp() takes twice as many, and no branch, so that several are under way.
+// Below e^-700 it is 0.
+__device__ __forceinline__ double exp64(double x, const double* power) {
+  const double magic = 6755399441055744.0;  // 1.5 2^52: sums with it are rounded to whole numbers
+  const double t = fma(x, 23.083120654223414, magic), r = fma(t - magic, -0.04332169878499658, x);
+  const int k = __double2loint(t);
+  double p = fma(r, 1.0 / 720.0, 1.0 / 120.0);
+  p = fma(r, p, 1.0 / 24.0);
+  p = fma(r, p, 1.0 / 6.0);
+  p = fma(r, p, 0.5);
+  p = fma(r, p, 1.0);
+  p = fma(r, p, 1.0) * power[k & 15];
+  return x < -700.0 ? 0.0 : __hiloint2double(__double2hiint(p) + ((k >> 4) << 20), __double2loint(p));
+}
 __device__ __forceinline__ double warp_sum(double x) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
   return x;
+}
+__device__ __forceinline__ float warp_max(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
 }
 // Of the lanes' parts x of a sum that begins at `begin`: the first one with which it is above t, and the sum before it; without one (`none`), the
 // last part above 0.  (Sums of other lanes come in another order: a part of 0 may seem to be above.)
@@ -88,182 +101,213 @@ __device__ __forceinline__ void put_remote(const void* p, uint32_t rank, uint32_
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(x) : "memory");
 }
-
+// A slice of `count` values from `src` on: `head` up to a 16-byte boundary, whole vectors, the rest.  The ends are one more value of the first threads.
 template <typename T>
-__global__ void __launch_bounds__(VT) k_verify_drafts(VerifyArgs a) {
-  constexpr int E = 16 / sizeof(T);  // values of a vector
-  extern __shared__ __align__(16) uint8_t ring[];
-  __shared__ double w_sum[VT / 32];
-  __shared__ float w_top[VT / 32];
-  __shared__ uint32_t w_at[VT / 32], w_last[VT / 32];
-  __shared__ double told_sum[2][MOST_AHEAD][MOST_BLOCKS], total[2][MOST_BLOCKS];
+struct Slice {
+  static constexpr int E = 16 / sizeof(T);
+  const T* src;
+  int head, vectors, tail;
+  __device__ __forceinline__ Slice(const T* s, int count) : src(s) {
+    head = min((E - (int)(((uintptr_t)s & 15) / sizeof(T))) % E, count);
+    vectors = (count - head) / E;
+    tail = count - head - vectors * E;
+  }
+  __device__ __forceinline__ int end_of(int tid) const { return tid < head ? tid : tid >= E && tid < E + tail ? head + vectors * E + tid - E : -1; }
+  __device__ __forceinline__ uint4 vector(int v) const { return __ldg((const uint4*)(src + head) + v); }
+};
+
+// VT: threads.  Of a position a thread has every VT-th vector, four a step; the next step's are on their way while these are judged.
+template <typename T, int VT>
+__global__ void __launch_bounds__(VT, 1024 / VT) k_verify_drafts(VerifyArgs a) {
+  constexpr int E = 16 / sizeof(T), W = VT / 32, U = 16 / E;  // values of a vector, warps, vectors of a step
+  constexpr int SUB = 32 / W;                            // parts of a warp's tokens, of which there are sums
+  extern __shared__ __align__(16) uint8_t staging[];  // the drafter's probabilities at a position
+  __shared__ double power[16];
+  __shared__ double w_sum[MOST_AHEAD][W];
+  __shared__ float w_top[MOST_AHEAD][W];
+  __shared__ uint32_t w_at[MOST_AHEAD][W];
+  // what the blocks tell each other of positions (two buffers, which take turns), and of what is drawn from
+  __shared__ double told_sum[2][MOST_AHEAD][MOST_BLOCKS], told_rest[3][MOST_BLOCKS];
   __shared__ uint32_t told_top[2][MOST_AHEAD][MOST_BLOCKS], told_at[2][MOST_AHEAD][MOST_BLOCKS];
   __shared__ double pos_sum[MOST_AHEAD];
   __shared__ float pos_top[MOST_AHEAD];
   __shared__ uint32_t pos_at[MOST_AHEAD];
-  __shared__ int verdict;            // of a group's positions: the place of the first that ends the row, or -1
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __shared__ int pos_ends[MOST_AHEAD];
+  __shared__ double r_sum[3][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int blocks = (int)gridDim.x, block = (int)blockIdx.x;
   const int64_t row = blockIdx.y;
+  if (tid < 16) power[tid] = exp2(tid / 16.0);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // (the same in all blocks of a cluster, as everything that decides which way they go)
   const int64_t s0 = a.starts[row], s1 = a.starts[row + 1], n = s1 - s0;
+  const float heat_in = a.temperature ? a.temperature[row] : 1.f;
+  const uint32_t len = a.lens ? a.lens[row] : 0xFFFFFFFFu;
   if (n == 0) return;
-  bool ok = s0 < s1 && s1 <= a.M && n <= a.most && (!a.lens || a.lens[row] >= n - 1);
-  if (ok) {
-    bool bad = false;
-    for (int64_t i = 1 + tid; i < n; i += VT) bad = bad || a.tokens[s0 + i] >= a.V;
-    ok = !__syncthreads_or(bad);
-  }
-  if (!ok) {
+  if (!(s0 < s1 && s1 <= a.M && n <= a.most && len >= n - 1)) {
     if (tid == 0) *a.err = DEV_INDEX;
     return;
   }
   // (nothing is put into another block's memory before it runs: waited for ahead of the first put)
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-  const float heat_in = a.temperature ? a.temperature[row] : 1.f;
+  const int64_t lo = std::min<int64_t>((int64_t)block * a.slice, a.V), hi = std::min<int64_t>(lo + a.slice, a.V);
+  const int count = (int)(hi - lo);
+  auto place = [&](int64_t pos) { return (const T*)a.logits + (s0 + pos) * a.l_ld + lo; };
+  const int steps = max(1, (count / E + U * VT - 1) / (U * VT));  // of a position
+  struct Step {
+    uint4 x[U];
+    T end;
+  };
+  auto load = [&](Step& to, int64_t pos, int step) {
+    const Slice<T> f(place(pos), count);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int v = tid + (step * U + i) * VT;
+      constexpr uint32_t none = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;  // (-inf)
+      to.x[i] = v < f.vectors ? f.vector(v) : make_uint4(none, none, none, none);
+    }
+    const int e = step == 0 ? f.end_of(tid) : -1;
+    to.end = e >= 0 ? f.src[e] : (T)NO_LOGIT;
+  };
+  int64_t first = 0;  // of the positions judged at a time
+  int parity = 0, group = (int)std::min<int64_t>(a.ahead, n), stop = -1;
+  Step ahead;
+  load(ahead, 0, 0);
+
+  bool bad = false;
+  for (int64_t i = 1 + tid; i < n; i += VT) bad = bad || a.tokens[s0 + i] >= a.V;
+  const float u_next = a.uniform[s1 - 1];
   const bool greedy = !(heat_in > 0.f);
   // (temperatures beyond 2^+-100 act as these)
   const float heat = fminf(fmaxf(heat_in, 0x1p-100f), 0x1p100f), unit = 1.4426950408889634f / heat;
   const double cold = 1.0 / (double)heat;
-  const int64_t lo = std::min<int64_t>((int64_t)block * a.slice, a.V), hi = std::min<int64_t>(lo + a.slice, a.V);
-  const int count = (int)(hi - lo);
-
-  // ---- a position's slice into shared memory: whole vectors as they lie, ragged ends value by value ----
-  auto place = [&](int64_t pos) { return (const T*)a.logits + (s0 + pos) * a.l_ld + lo; };
-  auto phase_of = [&](int64_t pos) { return (int)(((uintptr_t)place(pos) & 15) / sizeof(T)); };
-  auto request = [&](int64_t pos, int buffer) {
-    const T* src = place(pos);
-    const int phase = phase_of(pos), vectors = (phase + count + E - 1) / E;
-    uint8_t* dst = ring + (size_t)buffer * a.stride;
-    const T* base = src - phase;
-    for (int v = tid; v < vectors; v += VT) {
-      const int j0 = v * E - phase;
-      if (j0 >= 0 && j0 + E <= count) {
-        cp_async16(smem_u32(dst + v * 16), base + v * E, 16);
-      } else {
-        T* to = (T*)(dst + v * 16);
-        for (int e = 0; e < E; ++e) to[e] = j0 + e >= 0 && j0 + e < count ? src[j0 + e] : (T)NO_LOGIT;
-      }
-    }
-    cp_async_commit();
-  };
-
-  int64_t first = 0;  // of the group
-  int parity = 0, group = (int)std::min<int64_t>(a.ahead, n), stop = -1;
+  if (__syncthreads_or(bad)) {
+    if (tid == 0) *a.err = DEV_INDEX;
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    return;
+  }
   for (;;) {
-    for (int j = 0; j < group; ++j) request(first + j, j);
-    // what the drafts are judged by, asked for meanwhile
-    float draft_logit = 0.f, u = 0.f, q = 1.f;
-    uint32_t draft = NONE;
-    if (tid < group) {
-      const int64_t pos = first + tid, m = s0 + pos;
-      if (pos < n - 1) {
-        draft = a.tokens[m + 1];
-        u = a.uniform[m];
-        draft_logit = logit(((const T*)a.logits)[m * a.l_ld + draft]);
-        if (a.probs) {
-          q = a.probs16 ? __bfloat162float(((const __nv_bfloat16*)a.probs)[m * a.q_ld + draft]) : ((const float*)a.probs)[m * a.q_ld + draft];
-          q = q > 0.f ? q : 0.f;
-        }
-      }
-    }
-    cp_async_wait_all();
-    __syncthreads();
-    if (first == 0) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    // what the drafts are judged by, a warp each (used behind the sums)
+    struct Judged {
+      uint32_t draft, q;  // (q as it is stored)
+      float u;
+      T logit;
+    };
+    auto judge = [&](int j) {
+      Judged x = {NONE, 0, 0.f, (T)NO_LOGIT};
+      if (j >= group || first + j >= n - 1) return x;
+      const int64_t m = s0 + first + j;
+      x.draft = a.tokens[m + 1];
+      x.u = a.uniform[m];
+      x.logit = ((const T*)a.logits)[m * a.l_ld + x.draft];
+      if (a.probs) x.q = a.probs16 ? (uint32_t)((const uint16_t*)a.probs)[m * a.q_ld + x.draft] << 16 : ((const uint32_t*)a.probs)[m * a.q_ld + x.draft];
+      else x.q = 0x3F800000u;
+      return x;
+    };
+    const Judged mine = judge(warp);
     for (int j = 0; j < group; ++j) {
-      const int phase = phase_of(first + j), vectors = (phase + count + E - 1) / E;
-      const uint4* src = (const uint4*)(ring + (size_t)j * a.stride);
       float top = NO_LOGIT, sum = 0.f;
       uint32_t at = NONE;
-      for (int v = tid; v < vectors; v += VT) {
-        const uint4 w = src[v];
-        const T* x = (const T*)&w;
-        float y[E];
+      for (int step = 0; step < steps; ++step) {
+        const Step now = ahead;
+        const int64_t next_pos = step + 1 < steps ? first + j : first + j + 1;
+        if (next_pos < n) load(ahead, next_pos, step + 1 < steps ? step + 1 : 0);
+        auto value = [&](int i) { return widen(((const T*)&now.x[i / E])[i % E]); };  // (unpacked each time, which keeps registers)
+        const float end = widen(now.end);
+        float t[4] = {fmaxf(end, NO_LOGIT), NO_LOGIT, NO_LOGIT, NO_LOGIT};
 #pragma unroll
-        for (int e = 0; e < E; ++e) y[e] = logit(x[e]);
+        for (int i = 0; i < U * E; ++i) t[i & 3] = fmaxf(t[i & 3], value(i));
+        t[0] = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
         if (greedy) {
+          // (a thread's places ascend from step to step, but for the ends: before all others or behind them)
+          if (t[0] > NO_LOGIT && t[0] >= top) {
+            const Slice<T> f(place(first + j), count);
+            if (t[0] > top) at = NONE;
+            top = t[0];
+            if (step == 0 && end == top) at = min(at, (uint32_t)(lo + f.end_of(tid)));
 #pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (y[e] > top) {
-              top = y[e];
-              at = (uint32_t)(lo + v * E + e - phase);
-            }
+            for (int i = 0; i < U * E; ++i)
+              if (value(i) == top) at = min(at, (uint32_t)(lo + f.head + (tid + (step * U + i / E) * VT) * E + i % E));
+          }
         } else {
-          float t = y[0];
-#pragma unroll
-          for (int e = 1; e < E; ++e) t = fmaxf(t, y[e]);
-          if (t > top) {
-            sum *= fast_exp2((top - t) * unit);
-            top = t;
+          if (t[0] > top) {
+            sum *= fast_exp2((top - t[0]) * unit);
+            top = t[0];
           }
           if (top > NO_LOGIT) {
+            float s[4] = {fast_exp2((end - top) * unit), 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int e = 0; e < E; ++e) sum += fast_exp2((y[e] - top) * unit);
+            for (int i = 0; i < U * E; ++i) s[i & 3] += fast_exp2((value(i) - top) * unit);
+            float more = (s[0] + s[1]) + (s[2] + s[3]);
+            if (more != more) {  // (some are no numbers)
+              more = 0.f;
+#pragma unroll
+              for (int i = 0; i < U * E + 1; ++i) {
+                const float y = i < U * E ? value(i % (U * E)) : end;
+                more += y == y ? fast_exp2((y - top) * unit) : 0.f;
+              }
+            }
+            sum += more;
           }
         }
       }
-      // the block's
-      float t = top;
+      const float t = warp_max(top);
+      if (greedy) {
+        at = __reduce_min_sync(0xffffffffu, top == t ? at : NONE);
+      } else {
+        sum = top > NO_LOGIT ? sum * fast_exp2((top - t) * unit) : 0.f;
 #pragma unroll
-      for (int o = 16; o; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
-      double s = top > NO_LOGIT ? (double)sum * (double)fast_exp2((top - t) * unit) : 0.0;
-      s = warp_sum(s);
-      const uint32_t i = __reduce_min_sync(0xffffffffu, top == t ? at : NONE);
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      }
       if (lane == 0) {
-        w_top[warp] = t;
-        w_sum[warp] = s;
-        w_at[warp] = i;
+        w_top[j][warp] = t;
+        w_sum[j][warp] = (double)sum;
+        w_at[j][warp] = at;
       }
-      __syncthreads();
-      if (warp == 0) {
-        const bool there = lane < VT / 32;
-        float wt = there ? w_top[lane] : NO_LOGIT, bt = wt;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) bt = fmaxf(bt, __shfl_xor_sync(0xffffffffu, bt, o));
-        double ws = there && wt > NO_LOGIT ? w_sum[lane] * (double)fast_exp2((wt - bt) * unit) : 0.0;
-        ws = warp_sum(ws);
-        const uint32_t wi = __reduce_min_sync(0xffffffffu, there && wt == bt ? w_at[lane] : NONE);
-        if (lane < blocks) {
-          put_remote(&told_sum[parity][j][block], (uint32_t)lane, ws);
-          put_remote(&told_top[parity][j][block], (uint32_t)lane, __float_as_uint(bt));
-          put_remote(&told_at[parity][j][block], (uint32_t)lane, wi);
-        }
+    }
+    __syncthreads();
+    if (first == 0) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    if (warp < group) {
+      const bool there = lane < W;
+      const float wt = there ? w_top[warp][lane] : NO_LOGIT, bt = warp_max(wt);
+      const double ws = greedy ? 0.0 : warp_sum(there && wt > NO_LOGIT ? w_sum[warp][lane] * (double)fast_exp2((wt - bt) * unit) : 0.0);
+      const uint32_t wi = __reduce_min_sync(0xffffffffu, there && wt == bt ? w_at[warp][lane] : NONE);
+      if (lane < blocks) {
+        put_remote(&told_sum[parity][warp][block], (uint32_t)lane, ws);
+        put_remote(&told_top[parity][warp][block], (uint32_t)lane, __float_as_uint(bt));
+        put_remote(&told_at[parity][warp][block], (uint32_t)lane, wi);
       }
-      __syncthreads();
     }
     cluster_sync_all();
     // ---- the verdicts, in every block alike ----
-    if (warp == 0) {
-      bool ends = false;
-      if (lane < group) {
-        float top = NO_LOGIT;
-        for (int b = 0; b < blocks; ++b) top = fmaxf(top, __uint_as_float(told_top[parity][lane][b]));
-        double sum = 0.0;
-        uint32_t at = NONE;
-        for (int b = 0; b < blocks; ++b) {
-          const float t = __uint_as_float(told_top[parity][lane][b]);
-          if (t > NO_LOGIT) sum += told_sum[parity][lane][b] * (double)fast_exp2((t - top) * unit);
-          if (t == top) at = min(at, told_at[parity][lane][b]);
-        }
-        const bool some = top > NO_LOGIT && top < INFINITY;  // (else nothing has a probability)
-        pos_top[lane] = top;
-        pos_sum[lane] = sum;
-        pos_at[lane] = at;
-        ends = first + lane == n - 1;
-        if (!ends) {
-          const bool stands = greedy ? draft == at : (double)u * (double)q * sum < exp64(((double)draft_logit - (double)top) * cold);
-          ends = !(some && stands);
-        }
+    if (warp < group) {
+      const float q = __uint_as_float(mine.q);
+      const bool there = lane < blocks;
+      const float t = there ? __uint_as_float(told_top[parity][warp][lane]) : NO_LOGIT, top = warp_max(t);
+      const bool some = top > NO_LOGIT && top < INFINITY;  // (else nothing has a probability)
+      const double sum = greedy ? 0.0 : warp_sum(there && t > NO_LOGIT ? told_sum[parity][warp][lane] * (double)fast_exp2((t - top) * unit) : 0.0);
+      const uint32_t at = __reduce_min_sync(0xffffffffu, there && t == top ? told_at[parity][warp][lane] : NONE);
+      bool ends = first + warp == n - 1;
+      if (!ends) {
+        const bool stands = greedy ? mine.draft == at
+                                   : (double)mine.u * (double)(q > 0.f ? q : 0.f) * sum < exp64(((double)logit(mine.logit) - (double)top) * cold, power);
+        ends = !(some && stands);
       }
-      const uint32_t which = __ballot_sync(0xffffffffu, ends);
-      if (lane == 0) verdict = which ? __ffs(which) - 1 : -1;
+      if (lane == 0) {
+        pos_top[warp] = top;
+        pos_sum[warp] = sum;
+        pos_at[warp] = at;
+        pos_ends[warp] = ends;
+      }
     }
     parity ^= 1;
     __syncthreads();
-    stop = verdict;
-    if (stop >= 0) break;
+    const uint32_t which = __ballot_sync(0xffffffffu, lane < group && pos_ends[lane]);
+    if (which) {
+      stop = __ffs(which) - 1;
+      break;
+    }
     first += group;
     group = (int)std::min<int64_t>(a.ahead, n - first);
   }
@@ -278,102 +322,175 @@ __global__ void __launch_bounds__(VT) k_verify_drafts(VerifyArgs a) {
   } else if (greedy) {
     token = pos_at[stop];
   } else {
-    const T* values = (const T*)(ring + (size_t)stop * a.stride) + phase_of(pos);
-    const double t64 = (double)top;
-    // a warp has the same number of neighbouring tokens
-    const int per = ((count + VT / 32 - 1) / (VT / 32) + 31) & ~31, v0 = min(warp * per, count), v1 = min(v0 + per, count);
-    const uint32_t draft = pos < n - 1 ? a.tokens[m + 1] : NONE;
+    const T* values = place(pos);
+    int mode = pos < n - 1 ? (a.probs ? 2 : 1) : 0;  // what is drawn from: 0 weights e, 1 weights but the draft's, 2 what q leaves of them, max(e - q sum e, 0)
     const __nv_bfloat16* q16 = (const __nv_bfloat16*)a.probs + m * a.q_ld + lo;
     const float* q32 = (const float*)a.probs + m * a.q_ld + lo;
-    auto weight = [&](int j) { return exp64(((double)logit(values[j]) - t64) * cold); };
-    double whole = 0.0;  // sum of the weights, of all tokens
-    int mode = pos < n - 1 ? (a.probs ? 2 : 1) : 0;  // what is drawn from: 0 weights, 1 weights but the draft's, 2 what the drafter's probabilities leave
-    auto rest = [&](int j) {
-      const double e = weight(j);
-      if (mode == 0) return e;
-      if (mode == 1) return lo + j == draft ? 0.0 : e;
+    const double t64 = (double)top;
+    // 32 parts of neighbouring tokens, of which a warp has SUB
+    const int per = ((count + 31) / 32 + 31) & ~31;
+    auto part_begin = [&](int i) { return min(i * per, count); };
+    const uint32_t draft = pos < n - 1 ? a.tokens[m + 1] : NONE;
+    auto weigh = [&](float x) { return exp64(((double)x - t64) * cold, power); };
+    auto drafter = [&](int j) {
       const float q = a.probs16 ? __bfloat162float(q16[j]) : q32[j];
-      const double left = e - (double)(q > 0.f ? q : 0.f) * whole;
-      return left > 0.0 ? left : 0.0;
+      return q > 0.f ? q : 0.f;
     };
-    // sums of the warps (left in w_sum), and of all blocks (in total[parity])
-    auto sums = [&](auto f) {
-      double s = 0.0;
-      for (int j = v0 + lane; j < v1; j += 32) s += f(j);
-      s = warp_sum(s);
-      __syncthreads();
-      if (lane == 0) w_sum[warp] = s;
-      __syncthreads();
-      if (warp == 0) {
-        double b = lane < VT / 32 ? w_sum[lane] : 0.0;
-        b = warp_sum(b);
-        if (lane < blocks) put_remote(&total[parity][block], (uint32_t)lane, b);
+    // One pass for the sum of e, and for what is left once that is known: of the tokens with e > q s, where s is the sum that drafts were judged by,
+    // the sums of e and of q.  (Tokens on the wrong side of that border, 2^-20 of themselves from it, would add as little.)
+    const double s = mode == 2 ? pos_sum[stop] : 0.0;
+    auto sums = [&](auto probs) {  // (probs: of which type, or none)
+      typedef decltype(probs) Q;
+      constexpr bool HAS = !std::is_same<Q, char>::value;
+      constexpr int B = 4;  // logits of a thread at a time; the next ones are on their way
+      const int w0 = part_begin(warp * SUB), w1 = part_begin(warp * SUB + SUB);  // this warp's tokens
+      const Q* q_at = (const Q*)a.probs + m * a.q_ld + lo;
+      if constexpr (HAS) {
+        if (a.staged) {
+          // this warp's probabilities, whole vectors as they lie (before the row is the one before it, but in front of all)
+          constexpr int QE = 16 / sizeof(Q);
+          const int phase = (int)(((uintptr_t)(q_at + w0) & 15) / sizeof(Q));
+          uint8_t* to = staging + ((size_t)w0 * sizeof(Q) + 15) / 16 * 16 + warp * 16;
+          for (int v = lane; w0 < w1 && v * QE < phase + w1 - w0; v += 32) {
+            const int j0 = v * QE - phase;
+            if (j0 < 0 && m == 0 && lo + w0 == 0) {
+              for (int e = phase; e < QE; ++e)
+                if (e - phase < w1) ((Q*)to)[e] = q_at[e - phase];
+            } else {
+              cp_async16(smem_u32(to + v * 16), q_at + w0 + j0, (int)(std::min<int64_t>(QE, a.V - lo - w0 - j0) * (int64_t)sizeof(Q)));
+            }
+          }
+          cp_async_commit();
+          q_at = (const Q*)to + phase - w0;
+        }
       }
-      cluster_sync_all();
-      double all = 0.0;
-      for (int b = 0; b < blocks; ++b) all += total[parity][b];
-      parity ^= 1;
-      return all;
+      T x[B];
+      auto load = [&](int j0) {
+#pragma unroll
+        for (int i = 0; i < B; ++i) x[i] = j0 + 32 * i < w1 ? values[j0 + 32 * i] : (T)NO_LOGIT;
+      };
+      load(w0 + lane);
+      if (HAS && a.staged) {
+        cp_async_wait_group<0>();
+        __syncwarp();
+      }
+      for (int k = warp * SUB; k < warp * SUB + SUB; ++k) {
+        double e_all = 0.0, e_left = 0.0, q_left = 0.0;
+        const int v0 = part_begin(k), v1 = part_begin(k + 1);
+        for (int j0 = v0 + lane; j0 < v1; j0 += 32 * B) {
+          // (of the last ones some are the next part's, and read again)
+          float y[B];
+#pragma unroll
+          for (int i = 0; i < B; ++i) y[i] = j0 + 32 * i < v1 ? logit(x[i]) : NO_LOGIT;
+          load(j0 + 32 * B < v1 ? j0 + 32 * B : v1 + lane);
+#pragma unroll
+          for (int i = 0; i < B; ++i) {
+            const double e = weigh(y[i]);
+            e_all += e;
+            if constexpr (HAS) {
+              float q = j0 + 32 * i < v1 ? widen(q_at[j0 + 32 * i]) : 0.f;
+              q = q > 0.f ? q : 0.f;
+              const double p = (double)q;
+              if (e > p * s) {
+                e_left += e;
+                q_left += p;
+              }
+            }
+          }
+        }
+        e_all = warp_sum(e_all);
+        if (HAS) {
+          e_left = warp_sum(e_left);
+          q_left = warp_sum(q_left);
+        } else if (mode == 1) {
+          const int64_t d = (int64_t)draft - lo;
+          e_left = e_all - (d >= v0 && d < v1 ? weigh(logit(values[d])) : 0.0);
+        }
+        if (lane == 0) {
+          r_sum[0][k] = e_all;
+          r_sum[1][k] = e_left;
+          r_sum[2][k] = q_left;
+        }
+      }
     };
-    double all = 0.0;
-    if (mode == 2) whole = sums(weight);
-    all = sums(rest);
+    if (mode != 2) sums((char)0);
+    else if (a.probs16) sums(__nv_bfloat16());
+    else sums(0.f);
+    __syncthreads();
+    if (warp < 3) {
+      const double b = warp_sum(r_sum[warp][lane]);
+      if (lane < blocks) put_remote(&told_rest[warp][block], (uint32_t)lane, b);
+    }
+    cluster_sync_all();
+    const double b_e = lane < blocks ? told_rest[0][lane] : 0.0, b_left = lane < blocks ? told_rest[1][lane] : 0.0, b_q = lane < blocks ? told_rest[2][lane] : 0.0;
+    const double whole = mode == 2 ? warp_sum(b_e) : 0.0;
+    double part = mode == 0 ? b_e : mode == 1 ? b_left : fmax(b_left - b_q * whole, 0.0), all = warp_sum(part);
     if (!(all > 0.0)) {  // nothing is left: from the weights themselves
       mode = 0;
-      all = sums(rest);
+      part = b_e;
+      all = warp_sum(part);
     }
+    auto rest = [&](int j) {
+      const double e = weigh(logit(values[j]));
+      if (mode == 0) return e;
+      if (mode == 1) return lo + j == draft ? 0.0 : e;
+      return fmax(e - (double)drafter(j) * whole, 0.0);
+    };
     // ---- the first token whose inclusive sum is above u times the whole ----
-    const double t = (double)a.uniform[s1 - 1] * all;
+    const double t = (double)u_next * all;
     double before;
     bool lasts;  // (u is 1, or no number: the last token with a weight)
-    const int winner = first_above(lane < blocks ? total[parity ^ 1][lane] : 0.0, 0.0, t, &before, &lasts);
+    const int winner = first_above(part, 0.0, t, &before, &lasts);
     write = block == winner && tid == 0;
     if (block == winner) {
-      bool fallen;  // (sums of warps in another order than the blocks': the border is the block's end)
-      const int w = first_above(lane < VT / 32 ? w_sum[lane] : 0.0, before, lasts ? INFINITY : t, &before, &fallen);
-      // that warp's tokens, neighbours to each thread
-      const int a0 = min(w * per, count), a1 = min(a0 + per, count), each = (a1 - a0 + VT - 1) / VT, j0 = min(a0 + tid * each, a1), j1 = min(j0 + each, a1);
-      double s = 0.0;
-      for (int j = j0; j < j1; ++j) s += rest(j);
+      bool fallen;  // (sums of parts in another order than the blocks': the border is the block's end)
+      const double mine = mode == 0 ? r_sum[0][lane] : mode == 1 ? r_sum[1][lane] : fmax(r_sum[1][lane] - r_sum[2][lane] * whole, 0.0);
+      const int w = first_above(mine, before, lasts ? INFINITY : t, &before, &fallen);
+      // that part's tokens, neighbours to each thread
+      constexpr int KEPT = 4;  // (what they add, as far as it is kept)
+      const int a0 = part_begin(w), a1 = part_begin(w + 1), each = (a1 - a0 + VT - 1) / VT, j0 = min(a0 + tid * each, a1), j1 = min(j0 + each, a1);
+      double kept[KEPT], s = 0.0;
+#pragma unroll
+      for (int i = 0; i < KEPT; ++i) {
+        kept[i] = j0 + i < j1 ? rest(j0 + i) : 0.0;
+        s += kept[i];
+      }
+      for (int j = j0 + KEPT; j < j1; ++j) s += rest(j);
       double inc = s;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const double y = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += y;
       }
+      if (lane == 31) w_sum[0][warp] = inc;
       __syncthreads();
-      if (lane == 31) w_sum[warp] = inc;
-      __syncthreads();
-      double lower = before;
-      for (int i = 0; i < warp; ++i) lower += w_sum[i];
-      lower += inc - s;
+      double run = before + warp_sum(lane < warp ? w_sum[0][lane] : 0.0) + (inc - s);
       // the first token above t, or the last one with a weight (1 more than it, 0 if there is none)
       uint32_t above = NONE, weighs = 0;
-      double run = lower;
-      for (int j = j0; j < j1; ++j) {
-        const double x = rest(j);
+      auto look = [&](int j, double x) {
         run += x;
         if (x > 0.0) weighs = (uint32_t)(lo + j) + 1u;
         if (x > 0.0 && !lasts && !fallen && above == NONE && run > t) above = (uint32_t)(lo + j);
-      }
+      };
+#pragma unroll
+      for (int i = 0; i < KEPT; ++i) look(j0 + i, kept[i]);
+      for (int j = j0 + KEPT; j < j1; ++j) look(j, rest(j));
       above = __reduce_min_sync(0xffffffffu, above);
       weighs = __reduce_max_sync(0xffffffffu, weighs);
       if (lane == 0) {
-        w_at[warp] = above;
-        w_last[warp] = weighs;
+        w_at[0][warp] = above;
+        w_at[1][warp] = weighs;
       }
       __syncthreads();
-      for (int i = 0; i < VT / 32; ++i) {
-        above = min(above, w_at[i]);
-        weighs = max(weighs, w_last[i]);
-      }
+      above = __reduce_min_sync(0xffffffffu, lane < W ? w_at[0][lane] : NONE);
+      weighs = __reduce_max_sync(0xffffffffu, lane < W ? w_at[1][lane] : 0u);
       token = above != NONE ? above : weighs - 1u;
     }
   }
   if (write) {
     a.accepted[row] = (uint32_t)pos;
     a.next[row] = token;
-    if (a.lens) a.lens_out[row] = (uint32_t)(a.lens[row] - (n - 1 - pos));
+    if (a.lens) a.lens_out[row] = (uint32_t)(len - (n - 1 - pos));
   }
 }
 
@@ -386,26 +503,38 @@ int check_places(cg_ctx* c, const cg_tensor* t, const char* what, int64_t M, int
   return CG_OK;
 }
 
-template <typename T>
-int launch(cg_ctx* c, VerifyArgs& a) {
+template <typename T, int VT>
+int launch_threads(cg_ctx* c, VerifyArgs& a, int blocks) {
+  constexpr int smem_most = 96 * 1024;  // (two blocks on an SM)
   static PerDeviceFlag configured_on;
   bool& configured = configured_on.at(c->core->device);
-  constexpr int64_t smem_most = 200 * 1024;
   if (!configured) {
-    CG_CUDA(c, cudaFuncSetAttribute(k_verify_drafts<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_most));
-    CG_CUDA(c, cudaFuncSetAttribute(k_verify_drafts<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    CG_CUDA(c, cudaFuncSetAttribute(k_verify_drafts<T, VT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_most));
+    CG_CUDA(c, cudaFuncSetAttribute(k_verify_drafts<T, VT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     configured = true;
   }
-  int blocks = MOST_BLOCKS;
-  auto stride_of = [&](int b) { return ((a.V + b - 1) / b * (int64_t)sizeof(T) + 31) / 16 * 16; };
-  while (blocks > 1 && a.rows * blocks > 2 * 148 && stride_of(blocks / 2) * 2 <= smem_most) blocks /= 2;
   a.slice = (int)((a.V + blocks - 1) / blocks);
-  a.stride = (uint32_t)stride_of(blocks);
-  a.ahead = (int)std::min<int64_t>(std::min<int64_t>(smem_most / a.stride, a.most), MOST_AHEAD);
-  const size_t smem = (size_t)a.ahead * a.stride;
-  CG_CUDA(c, launch_kernel(c, k_verify_drafts<T>, dim3((unsigned)blocks, (unsigned)a.rows), dim3(VT), smem, -blocks, a));
+  // Positions judged at a time: two, where bytes count, so that few behind a rejected draft are read; of short ones all, for fewer rounds of
+  // sums and verdicts.  (16 rows x 50257 f32, greedy: 9.3 us with 8, 10.3 with 2; 32 x 256000 bf16: 69 and 54.)
+  a.ahead = a.rows * a.V * (int64_t)sizeof(T) > 8 << 20 ? 2 : MOST_AHEAD;
+  const int64_t staging = a.probs ? (int64_t)a.slice * (a.probs16 ? 2 : 4) + 32 * (VT / 32 + 1) : 0;
+  a.staged = staging > 0 && staging <= smem_most;
+  const size_t smem = a.staged ? (size_t)staging : 0;
+  CG_CUDA(c, launch_kernel(c, k_verify_drafts<T, VT>, dim3((unsigned)blocks, (unsigned)a.rows), dim3(VT), smem, -blocks, a));
   CG_LAUNCHED(c);
   return CG_OK;
+}
+template <typename T>
+int launch(cg_ctx* c, VerifyArgs& a) {
+  // Blocks of a row, and threads, us with blocks x threads, [the rule's]:
+  //   1 row x 128256, f32, 4 drafts          [16 x 512] 15.7  16 x 256 18.3  8 x 512 21.5  4 x 512 39
+  //   40 x 151936, bf16, 4                   [8 x 512] 55  8 x 256 55  16 x 256 54  16 x 512 67  4 x 512 57
+  //   32 x 256000, bf16, 7, no probabilities [8 x 512] 51  8 x 256 60  16 x 256 54
+  //   16 x 50257, f32, 3, greedy             [8 x 512] 10.1  8 x 256 9.3  16 x 256 10.8
+  //   38 x 2736, f32, 3                      [4 x 256] 14.5  8 x 256 15.7  16 x 512 35
+  int blocks = a.V >= 65536 && a.rows * MOST_BLOCKS <= 2 * 148 ? MOST_BLOCKS : 8;
+  while (blocks > 1 && (a.rows * blocks > 4 * 148 || a.V < 512 * blocks)) blocks /= 2;
+  return a.V >= 4096 * blocks ? launch_threads<T, 512>(c, a, blocks) : launch_threads<T, 256>(c, a, blocks);
 }
 
 }  // namespace
