@@ -64,9 +64,6 @@ constexpr size_t any_smem() {
   const size_t ring = (size_t)any_ring<T>() * S::STAGE, joined = (size_t)(QR == 64 ? 64 : 80) * S::LV;
   return ((size_t)2 * QR * S::LK + (ring > joined ? ring : joined)) * 4;
 }
-// MODE: which keys of a row.  CHUNK: the queries are a group's, the keys (blockIdx.y) a chunk of what its rows have in common; OWN: those behind that, joined
-// with the chunks (of which the launch before has to be waited for; what comes before that one is complete when this one begins).
-enum KeysOf { ALL, CHUNK, OWN };
 template <typename T, int D, int QR, int MODE>
 __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
   using S = Shape<D, QR>;
@@ -80,11 +77,9 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
   float* part = ring;                   // behind the loop: the warps' outputs [4][16][LV] and, with WK = 4, the block's [16][LV]
   __shared__ float red[2][64], ml[2][QR];
   __shared__ int64_t places[2][GK];     // of the keys of the next tile to be asked for; -1: zeros
-  auto depend = []() {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  };
+  auto depend = []() { asm volatile("griddepcontrol.wait;" ::: "memory"); };
   if (MODE != OWN) depend();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int rep = a.nh / a.nkv, kvh = (int)blockIdx.x % a.nkv;
   int64_t row = blockIdx.y, x0 = (int64_t)(blockIdx.x / a.nkv) * QR;
@@ -358,31 +353,16 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
       for (int e = 0; e < 2; ++e)
         *(float4*)(part + (warp * 16 + g + 8 * q) * LV + 32 * c + 8 * t4 + 4 * e) = make_float4(o[c][0][2 * q + e], o[c][1][2 * q + e], o[c][2][2 * q + e], o[c][3][2 * q + e]);
   __syncthreads();
-  int chunks = 0;
-  bool there = true;
-  if constexpr (MODE == OWN) {
-    depend();
-    if (group >= 0) {
-      int64_t first_row, rows, t0, tokens, shared;
-      there = group_span(a.rows, a.sh.groups, group, &first_row, &rows, &t0, &tokens, &shared);
-      if (there && (tok0 < t0 || tok0 + n > t0 + tokens)) {  // (starts that do not ascend: the chunks have other tokens)
-        *a.rows.err = DEV_INDEX;
-        there = false;
-      }
-      if (there) chunks = (int)((shared + a.sh.chunk - 1) / a.sh.chunk);
-    }
-  }
   // the output of query x at four components, v against `top`, whose exponentials' sum is `sum`
   auto finish = [&](int x, int col, float4 v, float top, float sum) {
-    if (x0 + x >= n * rep || col >= a.d || !there) return;
+    if (x0 + x >= n * rep || col >= a.d) return;
     const int64_t at = (tok0 + (x0 + x) / rep) * a.nh + kvh * rep + (x0 + x) % rep;
-    if constexpr (MODE == CHUNK) {
-      const int64_t to = (int64_t)blockIdx.y * a.rows.M * a.nh + at;
+    if constexpr (MODE != ALL) {
+      const int64_t to = (MODE == OWN ? (int64_t)a.sh.chunks : (int64_t)blockIdx.y) * a.rows.M * a.nh + at;
       *(float4*)(a.sh.out + to * a.d + col) = v;
       if (col == 0) a.sh.ml[to] = make_float2(top, sum);
       return;
     }
-    if constexpr (MODE == OWN) join_chunks(a.sh, chunks, a.rows.M * a.nh, at, a.d, col, top, sum, v);
     const float f = sum > 0.f ? 1.f / sum : 0.f;
     T* to = (T*)a.out + at * a.d + col;
     store_as(to, v.x * f); store_as(to + 1, v.y * f); store_as(to + 2, v.z * f); store_as(to + 3, v.w * f);
@@ -413,7 +393,10 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
         if (c == 0) { ml[0][x] = top; ml[1][x] = sum; }
       }
     }
-  if (slices == 1) return;
+  if (slices == 1) {
+    if (MODE == OWN) depend();
+    return;
+  }
   if (QR == 64 && tid < QR) { ml[0][tid] = red[0][tid]; ml[1][tid] = red[1][tid]; }
 
   // the blocks' shares: a block has some of the values
@@ -454,6 +437,7 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
     finish(x, c, v, top, sum);
   }
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (MODE == OWN) depend();
 }
 
 template <typename T, int D, int QR, int MODE>
@@ -465,8 +449,8 @@ int launch_any(cg_ctx* c, const PagedAttnArgs& a) {
     CG_CUDA(c, cudaFuncSetAttribute(k_paged_attn<T, D, QR, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     configured = true;
   }
-  const int64_t rep = a.nh / a.nkv, longest = a.rows.cols << a.rows.lg;
-  const int64_t tiles = (MODE == CHUNK ? a.rows.M * rep / QR + a.sh.groups.n : (a.most * rep + QR - 1) / QR) * a.nkv;  // (a group has a tile that is not full)
+  const int64_t rep = a.nh / a.nkv, width = a.rows.cols << a.rows.lg, longest = MODE == OWN ? a.sh.own(width) : width;
+  const int64_t tiles = (MODE == CHUNK ? (a.rows.M * rep + a.sh.groups.n * (QR - 1)) / QR : (a.most * rep + QR - 1) / QR) * a.nkv;  // (a group's last tile may not be full)
   if (tiles > 0x7FFFFFFFll) return fail(c, CG_ERR_UNSUPPORTED, "too many tokens");
   if (MODE == CHUNK) {
     CG_CUDA(c, launch_kernel(c, k_paged_attn<T, D, QR, MODE>, dim3((unsigned)tiles, (unsigned)a.sh.chunks), dim3(128), smem, 1, a));
@@ -495,6 +479,78 @@ int launch_typed(cg_ctx* c, const PagedAttnArgs& a) {
   if (a.d <= 64) return few ? launch_any<T, 64, 16, MODE>(c, a) : launch_any<T, 64, 64, MODE>(c, a);
   if (a.d <= 128) return few ? launch_any<T, 128, 16, MODE>(c, a) : launch_any<T, 128, 64, MODE>(c, a);
   return few ? launch_any<T, 256, 16, MODE>(c, a) : launch_any<T, 256, 64, MODE>(c, a);
+}
+
+// The parts of a token's head, joined: o = sum_c o_c 2^(m_c - m) / sum_c l_c 2^(m_c - m), m the largest m_c.  A thread has four components, a block
+// 256 / (d / 4) vectors or more; what the tables say is looked up before the parts are waited for.  (Joined by the blocks of the rows' own keys, after
+// those, the parts' latency stood in the way of the next block's keys: 64 rows behind 16001, 18 chunks, heads of 128: 62 us for all three, 55 here.)
+template <typename T>
+__global__ void __launch_bounds__(256) k_paged_join(PagedAttnArgs a) {
+  const int quads = a.d / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, vector = i / quads, m = vector / a.nh;
+  const int col = (int)(i - vector * quads) * 4;
+  const int64_t m0 = ((int64_t)blockIdx.x * 256 + (threadIdx.x & ~31)) / quads / a.nh, m1 = ((int64_t)blockIdx.x * 256 + (threadIdx.x | 31)) / quads / a.nh;  // tokens of the warp's ends
+  int chunks = -1;
+  for (int64_t t = m0; t <= m1 && t < a.rows.M; ++t) {
+    int64_t row = 0;
+    for (int64_t r = threadIdx.x & 31; r - (threadIdx.x & 31) < a.rows.rows; r += 32)
+      row += __popc(__ballot_sync(0xffffffffu, r < a.rows.rows && a.rows.starts[r + 1] <= t));
+    int64_t tok0, n, len, shared;
+    if (row >= a.rows.rows || !row_span(a.rows, row, a.most, &tok0, &n, &len) || t < tok0 || t >= tok0 + n) continue;
+    const int64_t group = group_of_row(a.sh.groups, row, &shared);
+    const int c = chunks_of(a.rows, a.sh, group, tok0, n);
+    if (t == m) chunks = c;
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (m >= a.rows.M || chunks < 0) return;
+  const int64_t per_chunk = a.rows.M * a.nh;
+  constexpr int U = 8;  // (on their way at a time)
+  float top = -INFINITY, sum = 0.f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c0 = 0; c0 <= chunks; c0 += U) {
+    float2 ml[U];
+    float4 o[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      ml[k] = make_float2(-INFINITY, 0.f);
+      if (c0 + k <= chunks) {
+        const int64_t x = (c0 + k < chunks ? c0 + k : a.sh.chunks) * per_chunk + vector;
+        ml[k] = __ldcg(a.sh.ml + x);
+        o[k] = __ldcg((const float4*)(a.sh.out + x * a.d + col));
+      }
+    }
+    const float before = top;
+#pragma unroll
+    for (int k = 0; k < U; ++k) top = fmaxf(top, ml[k].x);
+    const float base = top == -INFINITY ? 0.f : top, f0 = fast_exp2(before - base);
+    sum *= f0;
+    v.x *= f0; v.y *= f0; v.z *= f0; v.w *= f0;
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (ml[k].y > 0.f) {  // (a part without keys holds anything)
+        const float f = fast_exp2(ml[k].x - base);
+        sum = fmaf(ml[k].y, f, sum);
+        v.x = fmaf(o[k].x, f, v.x); v.y = fmaf(o[k].y, f, v.y); v.z = fmaf(o[k].z, f, v.z); v.w = fmaf(o[k].w, f, v.w);
+      }
+  }
+  const float f = sum > 0.f ? 1.f / sum : 0.f;
+  T* to = (T*)a.out + vector * a.d + col;
+  if constexpr (sizeof(T) == 4) {
+    store_as(to, v.x * f); store_as(to + 1, v.y * f); store_as(to + 2, v.z * f); store_as(to + 3, v.w * f);
+  } else if ((uintptr_t)a.out % 8 == 0) {
+    *(uint2*)to = make_uint2(pack_bf16(v.x * f, v.y * f), pack_bf16(v.z * f, v.w * f));
+  } else {
+    store_as(to, v.x * f); store_as(to + 1, v.y * f); store_as(to + 2, v.z * f); store_as(to + 3, v.w * f);
+  }
+}
+template <typename T>
+int launch_join(cg_ctx* c, const PagedAttnArgs& a) {
+  const int64_t blocks = (a.rows.M * a.nh * (a.d / 4) + 255) / 256;
+  if (blocks > 0x7FFFFFFFll) return fail(c, CG_ERR_UNSUPPORTED, "too many tokens");
+  CG_CUDA(c, launch_kernel(c, k_paged_join<T>, dim3((unsigned)blocks), dim3(256), 0, 1, a));
+  CG_LAUNCHED(c);
+  return CG_OK;
 }
 
 // What both kinds of attention check of their arguments, and their form for the kernels; `nothing`: there is nothing to do.
@@ -539,14 +595,14 @@ int attend(cg_ctx* c, const PagedAttnArgs& a, bool bf16) {
 
 // Into how many chunks shared keys are cut (0: rows read them for themselves).  A function of sizes alone, as the workspace's is.
 // Rows of so many tokens that they fill a tile of 128 queries by themselves gain nothing by others' beside them.
-void plan_chunks(cg_ctx* c, PagedAttnArgs* args, bool bf16) {
+void plan_chunks(PagedAttnArgs* args, bool bf16) {
   PagedAttnArgs& a = *args;
   const int64_t rep = a.nh / a.nkv;
   a.sh.chunks = 0;
   a.sh.chunk = 0;
   if (a.sh.groups.n == 0 || a.sh.groups.most == 0 || a.most * rep > 64) return;
   if (bf16) {
-    a.sh.chunk = paged_fa_chunk(c, a);
+    a.sh.chunk = paged_fa_chunk(a);
   } else {
     // (blocks of 64 queries, or 16: two or four on an SM)
     const int64_t size = a.rows.M * rep <= 32 ? 16 : 64, tiles = std::max((a.rows.M * rep + size - 1) / size, a.sh.groups.n) * a.nkv;
@@ -591,8 +647,8 @@ extern "C" int64_t cg_paged_shared_floats(cg_ctx* c, const cg_tensor* q, const c
   const int64_t longest = table->dims[1] * k_pages->dims[2];
   a.sh.groups.n = groups->dims[0] - 1;
   a.sh.groups.most = max_shared > 0 ? std::min(max_shared, longest) : longest;
-  plan_chunks(c, &a, q->storage == ST_BF16);
-  return a.sh.chunks * a.rows.M * a.nh * (a.d + 2);
+  plan_chunks(&a, q->storage == ST_BF16);
+  return a.sh.chunks ? (a.sh.chunks + 1) * a.rows.M * a.nh * (a.d + 2) : 0;
 }
 
 extern "C" int32_t cg_paged_shared_attention(cg_ctx* c, const cg_tensor* q, const cg_tensor* k_pages, const cg_tensor* v_pages, const cg_tensor* table,
@@ -621,8 +677,8 @@ extern "C" int32_t cg_paged_shared_attention(cg_ctx* c, const cg_tensor* q, cons
   a.sh.groups.n = G[0];
   a.sh.groups.most = max_shared > 0 ? std::min(max_shared, longest) : longest;
   const bool bf16 = q->storage == ST_BF16;
-  plan_chunks(c, &a, bf16);
-  const int64_t parts = a.sh.chunks * a.rows.M * a.nh;
+  plan_chunks(&a, bf16);
+  const int64_t parts = a.sh.chunks ? (a.sh.chunks + 1) * a.rows.M * a.nh : 0;
   if (work->dims[0] < parts * (a.d + 2)) return fail(c, CG_ERR_SHAPE, "work holds less than cg_paged_shared_floats");
   if (parts > 0 && (uintptr_t)work->data() % 16) return fail(c, CG_ERR_UNSUPPORTED, "work begins on a 16-byte boundary");
   written(out);
@@ -633,6 +689,8 @@ extern "C" int32_t cg_paged_shared_attention(cg_ctx* c, const cg_tensor* q, cons
   a.sh.ml = (float2*)(a.sh.out + parts * a.d);
   if (bf16 && paged_fa_prefix_supported(a)) CG_TRY(paged_fa_prefix(c, a));
   else CG_TRY((bf16 ? launch_typed<__nv_bfloat16, CHUNK>(c, a) : launch_typed<float, CHUNK>(c, a)));
-  if (bf16 && paged_dec_supported(a)) return paged_dec_own(c, a);
-  return bf16 ? launch_typed<__nv_bfloat16, OWN>(c, a) : launch_typed<float, OWN>(c, a);
+  if (bf16 && paged_fa_supported(a)) CG_TRY(paged_fa_own(c, a));
+  else if (bf16 && paged_dec_supported(a)) CG_TRY(paged_dec_own(c, a));
+  else CG_TRY((bf16 ? launch_typed<__nv_bfloat16, OWN>(c, a) : launch_typed<float, OWN>(c, a)));
+  return bf16 ? launch_join<__nv_bfloat16>(c, a) : launch_join<float>(c, a);
 }

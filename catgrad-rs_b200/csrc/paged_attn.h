@@ -6,16 +6,23 @@
 
 namespace cg {
 
-// Attention over keys that groups of rows have in common, in two launches: the first has all of a group's queries and a chunk of
-// the shared keys in a block, and leaves per token and head the chunk's output against its own maximum, that maximum (of scores in units of log2) and the sum
-// of exponentials; the second has a row's own keys, and joins them with the chunks.
+// Attention over keys that groups of rows have in common, in three launches: the first has all of a group's queries and a chunk of
+// the shared keys in a block, the second a row's own keys; both leave, per token and head, the output against their own maximum, that maximum (of scores in
+// units of log2) and the sum of exponentials, and the third joins these parts.
 struct SharedParts {
   PagedGroups groups;
   int64_t chunk;   // keys of a chunk
   int chunks;      // of the longest prefix
-  float* out;      // [chunks][M][heads][d]
-  float2* ml;      // [chunks][M][heads]
+  float* out;      // [chunks + 1][M][heads][d], the last for the rows' own keys
+  float2* ml;      // [chunks + 1][M][heads]
+  // keys of a row behind the prefix, by the table's width (which stands for the lengths)
+  int64_t own(int64_t longest) const { return longest > groups.most ? longest - groups.most : longest; }
 };
+
+// Which keys of a row a kernel takes: ALL of them; CHUNK: the queries are a group's, the keys a chunk of what its rows have in common; OWN: those behind that.
+// What comes before the launch of the chunks is complete when that lets the next one begin, so OWN waits for nothing until it ends; it does then, so
+// that what waits for it waits for the chunks too.
+enum KeysOf { ALL, CHUNK, OWN };
 
 struct PagedAttnArgs {
   PagedRows rows;
@@ -94,33 +101,16 @@ __device__ __forceinline__ void group_positions(const PagedRows& p, int64_t row0
   *first = __reduce_min_sync(0xffffffffu, lo);
   *last = __reduce_max_sync(0xffffffffu, hi);
 }
-// Joins what the chunks left of a token's head (place `at` = token heads + head) at four components with the row's own output v, against `top`, and its sum.
-__device__ __forceinline__ void join_chunks(const SharedParts& s, int n, int64_t per_chunk, int64_t at, int64_t d, int col, float& top, float& sum, float4& v) {
-  for (int c0 = 0; c0 < n; c0 += 4) {  // (four on their way at a time)
-    float2 ml[4];
-    float4 o[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      ml[i] = make_float2(-INFINITY, 0.f);
-      o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (c0 + i < n) {
-        const int64_t x = (c0 + i) * per_chunk + at;
-        ml[i] = __ldcg(s.ml + x);
-        o[i] = __ldcg((const float4*)(s.out + x * d + col));
-      }
-    }
-    const float before = top;
-    top = fmaxf(fmaxf(fmaxf(top, ml[0].x), fmaxf(ml[1].x, ml[2].x)), ml[3].x);
-    const float base = top == -INFINITY ? 0.f : top, f0 = fast_exp2(before - base);
-    sum *= f0;
-    v.x *= f0; v.y *= f0; v.z *= f0; v.w *= f0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float f = fast_exp2(ml[i].x - base);
-      sum = fmaf(ml[i].y, f, sum);
-      v.x = fmaf(o[i].x, f, v.x); v.y = fmaf(o[i].y, f, v.y); v.z = fmaf(o[i].z, f, v.z); v.w = fmaf(o[i].w, f, v.w);
-    }
+// The chunks of what a row's new tokens tok0 .. tok0 + n have in common with others; -1 (raised): what the tables say cannot be.
+__device__ __forceinline__ int chunks_of(const PagedRows& p, const SharedParts& s, int64_t group, int64_t tok0, int64_t n) {
+  if (group < 0) return 0;
+  int64_t row0, rows, t0, tokens, shared;
+  if (!group_span(p, s.groups, group, &row0, &rows, &t0, &tokens, &shared)) return -1;
+  if (tok0 < t0 || tok0 + n > t0 + tokens) {  // (starts that do not ascend: the chunks have other tokens)
+    *p.err = DEV_INDEX;
+    return -1;
   }
+  return (int)((shared + s.chunk - 1) / s.chunk);
 }
 __device__ __forceinline__ float soft_cap_near(float y, float cap_log2e) {
   const float u = y * y;
@@ -142,11 +132,12 @@ bool paged_fa_supported(const PagedAttnArgs& a);
 int paged_fa(cg_ctx* c, const PagedAttnArgs& a);
 bool paged_fa_prefix_supported(const PagedAttnArgs& a);
 int paged_fa_prefix(cg_ctx* c, const PagedAttnArgs& a);  // the chunks of shared keys
-int64_t paged_fa_chunk(cg_ctx* c, const PagedAttnArgs& a);
+int paged_fa_own(cg_ctx* c, const PagedAttnArgs& a);     // the rows' own keys
+int64_t paged_fa_chunk(const PagedAttnArgs& a);
 // A few tokens per row, bf16 (paged_dec.cu)
 bool paged_dec_supported(const PagedAttnArgs& a);
 int paged_dec(cg_ctx* c, const PagedAttnArgs& a);
-int paged_dec_own(cg_ctx* c, const PagedAttnArgs& a);    // the rows' own keys, joined with the chunks
+int paged_dec_own(cg_ctx* c, const PagedAttnArgs& a);    // the rows' own keys
 
 // ---- into how many shares a row's keys are cut ----
 constexpr int SHARES = 5;  // 1, 2, 4, 8 or 16: the blocks of a cluster

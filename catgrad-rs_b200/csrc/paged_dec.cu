@@ -41,29 +41,29 @@ struct DecArgs {
 // keys of a warp's tile, tiles of its ring
 template <int D>
 __host__ __device__ constexpr int dec_keys() { return D == 64 ? 32 : 16; }
-constexpr int RING = 3;
-template <int D>
-__host__ __device__ constexpr size_t dec_ring() { return (size_t)4 * RING * 2 * dec_keys<D>() * D * 2; }
-template <int D>
-__host__ __device__ constexpr size_t dec_smem() { return 1024 + dec_ring<D>() + 4 * RING * 8; }
+template <int MODE>
+__host__ __device__ constexpr int ring_of() { return MODE == OWN ? 2 : 3; }
+template <int D, int MODE>
+__host__ __device__ constexpr size_t dec_ring() { return (size_t)4 * ring_of<MODE>() * 2 * dec_keys<D>() * D * 2; }
+template <int D, int MODE>
+__host__ __device__ constexpr size_t dec_smem() { return 1024 + dec_ring<D, MODE>() + 4 * ring_of<MODE>() * 8; }
 
-// OWN: of a row in a group only the keys behind the group's prefix; the chunks of that, which the launch before leaves, are joined at the
-// end.  What comes before that launch is complete when this one begins (it waits for it before it lets this one begin), so
-// only the chunks are waited for.
-template <int D, int ROWS, bool CAP, bool OWN>
+template <int D, int ROWS, bool CAP, int MODE>
 __global__ void __launch_bounds__(128)
 k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, DecArgs p) {
+  constexpr bool OWN = MODE == KeysOf::OWN;
+  constexpr int RING = ring_of<MODE>();
   constexpr int KT = dec_keys<D>(), SUB = D / 64, NB = ROWS / 8, KS = D / 16, LD = D + 4;
   constexpr uint32_t BOX = KT * 128, TILE = SUB * BOX;  // bytes of 64 components, of a tile
   extern __shared__ uint8_t smem_raw[];
   __shared__ float red_m[4][ROWS], red_l[4][ROWS], cta_m[ROWS], cta_l[ROWS];
   __shared__ int aborted;
-  static_assert((size_t)4 * ROWS * LD * 4 + (size_t)ROWS * LD * 4 <= dec_ring<D>(), "the warps' outputs lie over the ring");
+  static_assert((size_t)4 * ROWS * LD * 4 + (size_t)ROWS * LD * 4 <= dec_ring<D, MODE>(), "the warps' outputs lie over the ring");
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   float* red_o = (float*)(smem_raw + (base - raw));       // [4][ROWS][LD]
   float* part = red_o + 4 * ROWS * LD;                    // [ROWS][LD]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t2 = (lane & 3) * 2;
-  const uint32_t ring = base + warp * (RING * 2 * TILE), bars = base + (uint32_t)dec_ring<D>() + warp * (RING * 8);
+  const uint32_t ring = base + warp * (RING * 2 * TILE), bars = base + (uint32_t)dec_ring<D, MODE>() + warp * (RING * 8);
   if (lane == 0)
     for (int i = 0; i < RING; ++i) mbar_init(bars + 8 * i, 1);
   if (tid == 0) aborted = 0;
@@ -77,11 +77,9 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
   const int slices = (int)gridDim.z, slice = (int)blockIdx.z, lg_slices = 31 - __clz(slices);
   const int lg = p.rows.lg, box = min(1 << lg, KT), parts = KT / box;
   const int my_part = lane % parts, my_sub = lane / parts % SUB, my_pool = lane / (parts * SUB);  // (keys, values; others have nothing)
-  auto depend = []() {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  };
+  auto depend = []() { asm volatile("griddepcontrol.wait;" ::: "memory"); };
   if (!OWN) depend();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   int64_t tok0, n, len;
   int64_t from = 0, group = -1;  // OWN: the first key, the row's group
@@ -281,23 +279,10 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
       for (int e = 0; e < 4; ++e) red_o[(warp * ROWS + b * 8 + t2 + (e & 1)) * LD + k * 16 + g + (e >> 1) * 8] = o[k][b][e];
   __syncthreads();
   auto out_at = [&](uint32_t x) { return p.out + ((tok0 + x / rep) * p.nh + kvh * rep + x % rep) * (int64_t)p.d; };
-  int chunks = 0;
-  if (OWN) {
-    depend();
-    if (group >= 0) {
-      int64_t row0, rows, t0, tokens, shared;
-      bool there = group_span(p.rows, p.sh.groups, group, &row0, &rows, &t0, &tokens, &shared);
-      if (there && (tok0 < t0 || tok0 + n > t0 + tokens)) {  // (starts that do not ascend: the chunks have other tokens)
-        *p.rows.err = DEV_INDEX;
-        there = false;
-      }
-      if (!there) aborted = 1;
-      else chunks = (int)((shared + p.sh.chunk - 1) / p.sh.chunk);
-    }
-    __syncthreads();
-  }
-  auto join = [&](uint32_t x, int c, float& top, float& sum, float4& v) {
-    if (OWN && chunks > 0) join_chunks(p.sh, chunks, p.rows.M * p.nh, (tok0 + x / rep) * p.nh + kvh * rep + x % rep, p.d, c, top, sum, v);
+  auto put_part = [&](uint32_t x, int c, float top, float sum, float4 v) {
+    const int64_t at = ((int64_t)p.sh.chunks * p.rows.M + tok0 + x / rep) * p.nh + kvh * rep + x % rep;
+    *(float4*)(p.sh.out + at * p.d + c) = v;
+    if (c == 0) p.sh.ml[at] = make_float2(top, sum);
   };
   for (int i = tid; i < ROWS * (D / 4); i += 128) {
     const int r = i / (D / 4), c = i % (D / 4) * 4;
@@ -315,13 +300,15 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
       *(float4*)(part + r * LD + c) = v;
       if (c == 0) { cta_m[r] = top; cta_l[r] = sum; }
     } else if (x0 + r < n * rep && c < p.d && !aborted) {
-      float m_all = top;
-      join(x0 + r, c, m_all, sum, v);
       const float f = sum > 0.f ? 1.f / sum : 0.f;
-      *(uint2*)(out_at(x0 + r) + c) = make_uint2(pack_bf16(v.x * f, v.y * f), pack_bf16(v.z * f, v.w * f));
+      if (OWN) put_part(x0 + r, c, top, sum, v);
+      else *(uint2*)(out_at(x0 + r) + c) = make_uint2(pack_bf16(v.x * f, v.y * f), pack_bf16(v.z * f, v.w * f));
     }
   }
-  if (slices == 1) return;
+  if (slices == 1) {
+    if (OWN) depend();
+    return;
+  }
 
   // ---- the blocks' shares: each finishes some of the values ----
   cluster_sync_all();
@@ -360,22 +347,23 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
       }
     }
     if (c < p.d && !aborted) {
-      join(x0 + r, c, top, sum, v);
       const float f = sum > 0.f ? 1.f / sum : 0.f;
-      *(uint2*)(out_at(x0 + r) + c) = make_uint2(pack_bf16(v.x * f, v.y * f), pack_bf16(v.z * f, v.w * f));
+      if (OWN) put_part(x0 + r, c, top, sum, v);
+      else *(uint2*)(out_at(x0 + r) + c) = make_uint2(pack_bf16(v.x * f, v.y * f), pack_bf16(v.z * f, v.w * f));
     }
   }
   cluster_sync_all();
+  if (OWN) depend();
 }
 
-template <int D, int ROWS, bool CAP, bool OWN>
+template <int D, int ROWS, bool CAP, int MODE>
 int launch(cg_ctx* c, const PagedAttnArgs& a) {
-  constexpr size_t smem = dec_smem<D>();
+  constexpr size_t smem = dec_smem<D, MODE>();
   static PerDeviceFlag configured_on;
   bool& configured = configured_on.at(c->core->device);
   if (!configured) {
-    CG_CUDA(c, cudaFuncSetAttribute(k_paged_dec<D, ROWS, CAP, OWN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    CG_CUDA(c, cudaFuncSetAttribute(k_paged_dec<D, ROWS, CAP, OWN>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    CG_CUDA(c, cudaFuncSetAttribute(k_paged_dec<D, ROWS, CAP, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    CG_CUDA(c, cudaFuncSetAttribute(k_paged_dec<D, ROWS, CAP, MODE>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     configured = true;
   }
   DecArgs p;
@@ -399,7 +387,7 @@ int launch(cg_ctx* c, const PagedAttnArgs& a) {
   const int box = std::min(1 << a.rows.lg, dec_keys<D>());
   CG_TRY(make_map(c, &mk, a.k_pages, p.pool_rows, a.d, a.d, box));
   CG_TRY(make_map(c, &mv, a.v_pages, p.pool_rows, a.d, a.d, box));
-  const int64_t groups = (a.most * p.rep + ROWS - 1) / ROWS * a.nkv, longest = a.rows.cols << a.rows.lg;
+  const int64_t groups = (a.most * p.rep + ROWS - 1) / ROWS * a.nkv, width = a.rows.cols << a.rows.lg, longest = MODE == OWN ? a.sh.own(width) : width;
   // Shares of the keys.  Us with 1 / 2 / 4 / 8 / 16, [the rule's]:
   //   8 rows x 8 key heads, 578 keys, d 64      7.9   7.4 [6.5]  11.0  27.5
   //   8 x 8, 2000, d 128                       29.9  19.3 [15.9] 22.1  39.6
@@ -410,18 +398,18 @@ int launch(cg_ctx* c, const PagedAttnArgs& a) {
   //   12 x 4, 167, d 256                        7.5 [7.9]  12.7  24.8  47.7
   // (Lengths are on the device, so the table's width stands for them: 32 x 8 rows of 530 with columns for 32768 tokens get 2 shares, 23.4 us.)
   static AtATime known;
-  const int slices = pick_shares([&](int i) { return at_a_time(known, c->core->device, i, k_paged_dec<D, ROWS, CAP, OWN>, 128, smem); }, 16, groups * a.rows.rows, longest,
+  const int slices = pick_shares([&](int i) { return at_a_time(known, c->core->device, i, k_paged_dec<D, ROWS, CAP, MODE>, 128, smem); }, 16, groups * a.rows.rows, longest,
                                  4 * dec_keys<D>(), 4., D == 64 ? 0.7 : D == 128 ? 0.75 : 1.25, 0.);
-  CG_CUDA(c, launch_kernel(c, k_paged_dec<D, ROWS, CAP, OWN>, dim3((unsigned)groups, (unsigned)a.rows.rows, (unsigned)slices), dim3(128), smem, slices, mk, mv, p));
+  CG_CUDA(c, launch_kernel(c, k_paged_dec<D, ROWS, CAP, MODE>, dim3((unsigned)groups, (unsigned)a.rows.rows, (unsigned)slices), dim3(128), smem, slices, mk, mv, p));
   CG_LAUNCHED(c);
   return CG_OK;
 }
 
-template <int D, bool OWN>
+template <int D, int MODE>
 int pick(cg_ctx* c, const PagedAttnArgs& a) {
   const bool cap = a.cap > 0.f;
-  if (a.most * (a.nh / a.nkv) <= 8) return cap ? launch<D, 8, true, OWN>(c, a) : launch<D, 8, false, OWN>(c, a);
-  return cap ? launch<D, 16, true, OWN>(c, a) : launch<D, 16, false, OWN>(c, a);
+  if (a.most * (a.nh / a.nkv) <= 8) return cap ? launch<D, 8, true, MODE>(c, a) : launch<D, 8, false, MODE>(c, a);
+  return cap ? launch<D, 16, true, MODE>(c, a) : launch<D, 16, false, MODE>(c, a);
 }
 
 }  // namespace
@@ -432,15 +420,15 @@ bool paged_dec_supported(const PagedAttnArgs& a) {
 }
 
 int paged_dec(cg_ctx* c, const PagedAttnArgs& a) {
-  if (a.d <= 64) return pick<64, false>(c, a);
-  if (a.d <= 128) return pick<128, false>(c, a);
-  return pick<256, false>(c, a);
+  if (a.d <= 64) return pick<64, ALL>(c, a);
+  if (a.d <= 128) return pick<128, ALL>(c, a);
+  return pick<256, ALL>(c, a);
 }
 
 int paged_dec_own(cg_ctx* c, const PagedAttnArgs& a) {
-  if (a.d <= 64) return pick<64, true>(c, a);
-  if (a.d <= 128) return pick<128, true>(c, a);
-  return pick<256, true>(c, a);
+  if (a.d <= 64) return pick<64, OWN>(c, a);
+  if (a.d <= 128) return pick<128, OWN>(c, a);
+  return pick<256, OWN>(c, a);
 }
 
 }  // namespace cg

@@ -118,12 +118,13 @@ __host__ __device__ constexpr size_t fa_smem() {
 // Warps: 0 loads, 1 and 3 issue the products of query tiles 0 and 1, 2 clears values that nobody sees, 4 to 7 and 8 to 11 are the rows
 // of tiles 0 and 1.
 //
-// SHARED: the queries are those of a group of rows, the keys a chunk of what the group has in common (through its first row's table), and
-// the outputs parts that the rows join with their own keys'.  A token's position is then its row's, and masks are only looked at
+// CHUNK: the queries are those of a group of rows, the keys a chunk of what the group has in common (through its first row's table), and
+// the outputs parts that the rows (OWN) join with their own keys'.  A token's position is then its row's, and masks are only looked at
 // where a query stands inside the prefix or a window ends there.
-template <int D, int NQ, bool CAP, bool SHARED>
+template <int D, int NQ, bool CAP, int MODE>
 __global__ void __launch_bounds__(NQ == 2 ? 384 : 256, NQ == 2 || D > 128 ? 1 : 2)
 k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, FaArgs p) {
+  constexpr bool SHARED = MODE == KeysOf::CHUNK, OWN = MODE == KeysOf::OWN, PART = SHARED || OWN;
   constexpr int SUB = D / 64, KS = fa_stages<D, NQ>();
   constexpr uint32_t BOX = 128 * 128, KBOX = KT * 128;
   constexpr uint32_t Q_BYTES = SUB * BOX, KV_BYTES = SUB * KBOX;
@@ -144,28 +145,32 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;  // (warp: known to be uniform)
   // q, the tables and the pages are written by the preceding kernels
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  auto dependency = []() { asm volatile("griddepcontrol.wait;" ::: "memory"); };
+  if (!OWN) dependency();
   const int slice = (int)blockIdx.x % p.slices;
   const int kvh = blockIdx.y;
   int64_t qt = ((int)gridDim.x - 1 - (int)blockIdx.x) / p.slices;  // longest first
-  int64_t row = blockIdx.z, tok0, n, len, rows = 0, shared = 0;
+  int64_t row = blockIdx.z, tok0, n, len, rows = 0, shared = 0;  // (OWN: shared are the keys in front)
+  int64_t group = -1;
   if (SHARED) {
     const int64_t tiles = (int)gridDim.x / (p.slices * p.sh.chunks), t = (int)blockIdx.x / p.slices % tiles;
     const int64_t g = group_of_tile(p.rows, p.sh.groups, t, 1, (int64_t)NQ * p.per, &qt);
     if (g < 0 || !group_span(p.rows, p.sh.groups, g, &row, &rows, &tok0, &n, &shared)) return;  // uniform over the CTA, before anything is allocated
     len = 0;
   } else {
-    if (!row_span(p.rows, row, p.most, &tok0, &n, &len)) return;
+    if (OWN) group = group_of_row(p.sh.groups, row, &shared);
+    if (!row_span(p.rows, row, p.most, &tok0, &n, &len)) n = 0;
   }
   const int64_t i0 = qt * NQ * p.per;                            // first token of the first tile
-  const int chunk = SHARED ? (int)blockIdx.x / p.slices / ((int)gridDim.x / (p.slices * p.sh.chunks)) : 0;
+  const int chunk = OWN ? p.sh.chunks : SHARED ? (int)blockIdx.x / p.slices / ((int)gridDim.x / (p.slices * p.sh.chunks)) : 0;
   if (SHARED && chunk * p.sh.chunk >= shared) n = 0;
+  if (OWN && i0 >= n) dependency();
   if (i0 >= n) return;
   const int64_t pos0 = SHARED ? 0 : len - n;
   const int64_t last = SHARED ? min(shared, (chunk + 1) * p.sh.chunk) - 1 : pos0 + min(n, i0 + NQ * p.per) - 1;  // the last key, position of the last query
-  const int64_t lo = SHARED ? chunk * p.sh.chunk : p.window > 0 ? max((int64_t)0, pos0 + i0 - p.window + 1) : 0;  // first visible key
+  const int64_t lo = SHARED ? chunk * p.sh.chunk : max(p.window > 0 ? max((int64_t)0, pos0 + i0 - p.window + 1) : 0, OWN ? min(shared, last + 1) : 0);  // first visible key
   // this block's share of the key tiles: [j0, j0 + nt)
-  const int all = (int)(last / KT + 1 - lo / KT), share = (all + p.slices - 1) / p.slices;
+  const int all = max((int)(last / KT + 1 - lo / KT), 0), share = (all + p.slices - 1) / p.slices;
   const int64_t j0 = lo / KT + (int64_t)slice * share;
   const int nt = min(share, max(0, all - slice * share));
   // Keys of the last tile that some query sees.  The values behind them (what nothing or another sequence wrote) are
@@ -364,11 +369,11 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
       ld32(s_addr + 32, v + 32);
       asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
       // uniform: some key may be masked for some row
-      const bool masked = k0 + KT - 1 > tile_first || (p.window > 0 && k0 <= tile_last - p.window);
+      const bool masked = k0 + KT - 1 > tile_first || (p.window > 0 && k0 <= tile_last - p.window) || (OWN && k0 < shared);
       uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
       if (masked) {
         // column c is visible to this row iff low <= c <= lim
-        const int64_t lim64 = (SHARED ? min(qpos, last) : qpos) - k0, low64 = p.window > 0 ? qpos - k0 - p.window + 1 : 0;
+        const int64_t lim64 = (SHARED ? min(qpos, last) : qpos) - k0, low64 = max(p.window > 0 ? qpos - k0 - p.window + 1 : 0, OWN ? shared - k0 : 0);
         const int lim = lim64 > KT ? KT : (lim64 < -1 ? -1 : (int)lim64), low = low64 < 0 ? 0 : (low64 > KT ? KT : (int)low64);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -502,18 +507,16 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const float inv = l > 0.f ? 1.f / l : 0.f;
     const bool out = ok && mine;
-    if (SHARED && p.slices == 1 && out) {
-      const int64_t at = ((int64_t)chunk * p.rows.M + tok0 + ti) * p.nh + head;
-      p.sh.ml[at] = make_float2(m, l);
-    }
+    const int64_t part_at = ((int64_t)chunk * p.rows.M + tok0 + ti) * p.nh + head;
+    if (PART && p.slices == 1 && out) p.sh.ml[part_at] = make_float2(m, l);
     __nv_bfloat16* dst = p.out + ((tok0 + ti) * p.nh + head) * (int64_t)p.d;
 #pragma unroll 1
     for (int c0 = 0; c0 < D && p.slices == 1; c0 += 32) {
       uint32_t v[32];
       ld32(o_addr + c0, v);
       asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-      if (SHARED) {
-        float* to = p.sh.out + (((int64_t)chunk * p.rows.M + tok0 + ti) * p.nh + head) * p.d + c0;
+      if (PART) {  // (without keys nothing was written: the sum says so)
+        float* to = p.sh.out + part_at * p.d + c0;
 #pragma unroll
         for (int u = 0; u < 8; ++u)
           if (out && c0 + 4 * u < p.d) *(uint4*)(to + 4 * u) = make_uint4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
@@ -561,7 +564,10 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
     __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(NCOLS) : "memory");
   }
-  if (p.slices == 1) return;
+  if (p.slices == 1) {
+    if (OWN) dependency();
+    return;
+  }
   __shared__ float weight[4][NQ * 128];  // of the blocks' outputs of a row
   cluster_sync_all();
   if (tid < NQ * 128) {
@@ -579,8 +585,8 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
       sum = fmaf(ls[s], ms[s], sum);
     }
 #pragma unroll
-    for (int s = 0; s < 4; ++s) weight[s][tid] = SHARED ? ms[s] : sum > 0.f ? ms[s] / sum : 0.f;
-    if (SHARED && slice == 0) {
+    for (int s = 0; s < 4; ++s) weight[s][tid] = PART ? ms[s] : sum > 0.f ? ms[s] / sum : 0.f;
+    if (PART && slice == 0) {
       const int r = tid & 127;
       const int64_t ti = i0 + (tid >> 7) * p.per + r / p.rep;
       if (r < p.per * p.rep && ti < n) p.sh.ml[((int64_t)chunk * p.rows.M + tok0 + ti) * p.nh + kvh * p.rep + r % p.rep] = make_float2(top, sum);
@@ -615,11 +621,12 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
         v.x = fmaf(os[u][s].x, f, v.x); v.y = fmaf(os[u][s].y, f, v.y); v.z = fmaf(os[u][s].z, f, v.z); v.w = fmaf(os[u][s].w, f, v.w);
       }
       const int64_t at = ((tok0 + ti) * p.nh + kvh * p.rep + r % p.rep) * (int64_t)p.d + c;
-      if (SHARED) *(float4*)(p.sh.out + (int64_t)chunk * p.rows.M * p.nh * p.d + at) = v;
+      if (PART) *(float4*)(p.sh.out + (int64_t)chunk * p.rows.M * p.nh * p.d + at) = v;
       else *(uint2*)(p.out + at) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
     }
   }
   cluster_sync_all();
+  if (OWN) dependency();
 }
 
 // q as [tokens, heads, d] in boxes of [per tokens, rep heads, 64 components]
@@ -636,13 +643,13 @@ int make_q_map(cg_ctx* c, CUtensorMap* map, const PagedAttnArgs& a, int per, int
 }
 
 // How a kernel is set up: once per device, and its arguments.
-template <int D, int NQ, bool CAP, bool SHARED>
+template <int D, int NQ, bool CAP, int MODE>
 int configure(cg_ctx* c, const PagedAttnArgs& a, FaArgs* out, CUtensorMap* mq, CUtensorMap* mk, CUtensorMap* mv) {
   constexpr size_t smem = fa_smem<D, NQ>();
   static PerDeviceFlag configured_on;
   bool& configured = configured_on.at(c->core->device);
   if (!configured) {
-    CG_CUDA(c, cudaFuncSetAttribute(k_paged_fa<D, NQ, CAP, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    CG_CUDA(c, cudaFuncSetAttribute(k_paged_fa<D, NQ, CAP, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     configured = true;
   }
   FaArgs& p = *out;
@@ -672,13 +679,13 @@ int configure(cg_ctx* c, const PagedAttnArgs& a, FaArgs* out, CUtensorMap* mq, C
   return make_q_map(c, mq, a, p.per, p.rep);
 }
 
-template <int D, int NQ, bool CAP>
+template <int D, int NQ, bool CAP, int MODE>
 int launch(cg_ctx* c, const PagedAttnArgs& a) {
   constexpr size_t smem = fa_smem<D, NQ>();
   FaArgs p;
   CUtensorMap mq, mk, mv;
-  CG_TRY((configure<D, NQ, CAP, false>(c, a, &p, &mq, &mk, &mv)));
-  const int64_t tiles = (a.most + (int64_t)NQ * p.per - 1) / ((int64_t)NQ * p.per), longest = a.rows.cols << a.rows.lg;
+  CG_TRY((configure<D, NQ, CAP, MODE>(c, a, &p, &mq, &mk, &mv)));
+  const int64_t tiles = (a.most + (int64_t)NQ * p.per - 1) / ((int64_t)NQ * p.per), width = a.rows.cols << a.rows.lg, longest = MODE == OWN ? a.sh.own(width) : width;
   // Shares of the keys (of several rows four fifths of the tiles count: they differ).  Us with 1 / 2 / 4, [the rule's]:
   //   6 rows of 480 behind 3720, 4 x 2 heads of 256, window 4096    182  [157]  187
   //   1 of 63 behind 2937, the same, no window                     61.6   38.0 [24.6]
@@ -689,10 +696,10 @@ int launch(cg_ctx* c, const PagedAttnArgs& a) {
   // (The table's width stands for the lengths, and 4 shares of a short tile of queries leave SMs idle: the second and third rows' bytes take 2 to 3 us.)
   static AtATime known;
   const int64_t clusters = tiles * a.nkv * a.rows.rows;
-  p.slices = pick_shares([&](int i) { return at_a_time(known, c->core->device, i, k_paged_fa<D, NQ, CAP, false>, NQ == 2 ? 384 : 256, smem); }, 4,
+  p.slices = pick_shares([&](int i) { return at_a_time(known, c->core->device, i, k_paged_fa<D, NQ, CAP, MODE>, NQ == 2 ? 384 : 256, smem); }, 4,
                          a.rows.rows > 1 ? std::max<int64_t>(clusters * 4 / 5, 1) : clusters, a.window > 0 ? std::min(longest, a.window + p.per * NQ) : longest, KT, 6.,
                          D == 256 ? 1.25 : NQ == 2 ? 1.1 : 0.9, 0.);
-  CG_CUDA(c, launch_kernel(c, k_paged_fa<D, NQ, CAP, false>, dim3((unsigned)(tiles * p.slices), (unsigned)a.nkv, (unsigned)a.rows.rows), dim3(NQ == 2 ? 384 : 256), smem, -p.slices,
+  CG_CUDA(c, launch_kernel(c, k_paged_fa<D, NQ, CAP, MODE>, dim3((unsigned)(tiles * p.slices), (unsigned)a.nkv, (unsigned)a.rows.rows), dim3(NQ == 2 ? 384 : 256), smem, -p.slices,
                            mq, mk, mv, p));
   CG_LAUNCHED(c);
   return CG_OK;
@@ -703,48 +710,36 @@ int pick(cg_ctx* c, const PagedAttnArgs& a) {
   const bool cap = a.cap > 0.f;
   if constexpr (D <= 128) {
     const int per = 128 / (a.nh / a.nkv);
-    if (a.most > per) return cap ? launch<D, 2, true>(c, a) : launch<D, 2, false>(c, a);
+    if (a.most > per) return cap ? launch<D, 2, true, ALL>(c, a) : launch<D, 2, false, ALL>(c, a);
   }
-  return cap ? launch<D, 1, true>(c, a) : launch<D, 1, false>(c, a);
+  return cap ? launch<D, 1, true, ALL>(c, a) : launch<D, 1, false, ALL>(c, a);
 }
 
 // ---- shared keys ----
 
-// Two tiles of queries share their keys where a group has more than one (by the packed tokens, as far as the host knows).
-template <int D>
-bool two_tiles(const PagedAttnArgs& a) { return D <= 128 && a.rows.M * (a.nh / a.nkv) > a.sh.groups.n * 128; }
-int64_t prefix_tiles(const PagedAttnArgs& a, int nq) {
-  const int64_t tokens = (int64_t)nq * (128 / (a.nh / a.nkv));
-  return a.rows.M / tokens + a.sh.groups.n;  // (a group has one that is not full)
+// (Two tiles of queries that share their keys in a block are no faster here: 64 rows over 16001 keys, heads of 128, 60.5 us with one, 62 with two, and
+// a group's second tile is often all but empty.)
+int64_t prefix_tiles(const PagedAttnArgs& a) {
+  const int64_t tokens = 128 / (a.nh / a.nkv);
+  return (a.rows.M + a.sh.groups.n * (tokens - 1)) / tokens;  // (a group's last one may not be full)
 }
-template <int D, int NQ, bool CAP>
+template <int D, bool CAP>
 int launch_prefix(cg_ctx* c, const PagedAttnArgs& a) {
   FaArgs p;
   CUtensorMap mq, mk, mv;
-  CG_TRY((configure<D, NQ, CAP, true>(c, a, &p, &mq, &mk, &mv)));
+  CG_TRY((configure<D, 1, CAP, CHUNK>(c, a, &p, &mq, &mk, &mv)));
   p.slices = 1;
-  const int64_t blocks = prefix_tiles(a, NQ) * a.sh.chunks * p.slices;
+  const int64_t blocks = prefix_tiles(a) * a.sh.chunks;
   if (blocks > 0x7FFFFFFFll) return fail(c, CG_ERR_UNSUPPORTED, "too many tokens");
-  CG_CUDA(c, launch_kernel(c, k_paged_fa<D, NQ, CAP, true>, dim3((unsigned)blocks, (unsigned)a.nkv), dim3(NQ == 2 ? 384 : 256), fa_smem<D, NQ>(), -p.slices, mq, mk, mv, p));
+  CG_CUDA(c, launch_kernel(c, k_paged_fa<D, 1, CAP, CHUNK>, dim3((unsigned)blocks, (unsigned)a.nkv), dim3(256), fa_smem<D, 1>(), 1, mq, mk, mv, p));
   CG_LAUNCHED(c);
   return CG_OK;
 }
 template <int D>
-int pick_prefix(cg_ctx* c, const PagedAttnArgs& a) {
-  const bool cap = a.cap > 0.f;
-  if constexpr (D <= 128) {
-    if (two_tiles<D>(a)) return cap ? launch_prefix<D, 2, true>(c, a) : launch_prefix<D, 2, false>(c, a);
-  }
-  return cap ? launch_prefix<D, 1, true>(c, a) : launch_prefix<D, 1, false>(c, a);
-}
-// Keys of a chunk: as many chunks as keep all SMs busy, two blocks on one where they fit.
+int pick_prefix(cg_ctx* c, const PagedAttnArgs& a) { return a.cap > 0.f ? launch_prefix<D, true>(c, a) : launch_prefix<D, false>(c, a); }
 template <int D>
-int64_t chunk_of(const PagedAttnArgs& a) {
-  const int nq = two_tiles<D>(a) ? 2 : 1;
-  const int64_t slots = nq == 1 && D <= 128 ? 296 : 148;
-  const int64_t queries = a.rows.M * (a.nh / a.nkv), tiles = std::max<int64_t>((queries + nq * 128 - 1) / (nq * 128), a.sh.groups.n) * a.nkv;
-  const int64_t chunks = std::max<int64_t>(slots / tiles, 1), keys = (a.sh.groups.most + chunks - 1) / chunks;
-  return std::max<int64_t>((keys + KT - 1) / KT * KT, 2 * KT);
+int pick_own(cg_ctx* c, const PagedAttnArgs& a) {
+  return a.cap > 0.f ? launch<D, 1, true, OWN>(c, a) : launch<D, 1, false, OWN>(c, a);  // (a row's tokens do not fill a tile)
 }
 
 }  // namespace
@@ -771,9 +766,16 @@ int paged_fa_prefix(cg_ctx* c, const PagedAttnArgs& a) {
   if (a.d <= 128) return pick_prefix<128>(c, a);
   return pick_prefix<256>(c, a);
 }
-int64_t paged_fa_chunk(cg_ctx* c, const PagedAttnArgs& a) {
-  (void)c;
-  return a.d <= 64 ? chunk_of<64>(a) : a.d <= 128 ? chunk_of<128>(a) : chunk_of<256>(a);
+int paged_fa_own(cg_ctx* c, const PagedAttnArgs& a) {
+  if (a.d <= 64) return pick_own<64>(c, a);
+  if (a.d <= 128) return pick_own<128>(c, a);
+  return pick_own<256>(c, a);
+}
+// Keys of a chunk: as many chunks as keep all SMs busy, two blocks on one where they fit, in one wave however the tokens are dealt to the groups.
+int64_t paged_fa_chunk(const PagedAttnArgs& a) {
+  const int64_t slots = a.d <= 128 ? 296 : 148, queries = a.rows.M * (a.nh / a.nkv), tiles = std::max<int64_t>((queries + a.sh.groups.n * 127) / 128, 1) * a.nkv;
+  const int64_t chunks = std::max<int64_t>(slots / tiles, 1), keys = (a.sh.groups.most + chunks - 1) / chunks;
+  return std::max<int64_t>((keys + KT - 1) / KT * KT, 2 * KT);
 }
 
 }  // namespace cg
