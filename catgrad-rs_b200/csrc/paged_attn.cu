@@ -86,12 +86,14 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
   const int slices = (int)gridDim.z, slice = (int)blockIdx.z;
   int64_t tok0, n, len, rows_of = 0, from = 0, group = -1;  // CHUNK: the group's rows; OWN: the first key, the group
   if constexpr (MODE == CHUNK) {
-    int64_t tile, shared;
-    group = group_of_tile(a.rows, a.sh.groups, blockIdx.x / a.nkv, rep, QR, &tile);
-    if (group < 0 || !group_span(a.rows, a.sh.groups, group, &row, &rows_of, &tok0, &n, &shared)) return;
-    if ((int64_t)blockIdx.y * a.sh.chunk >= shared) return;
-    x0 = tile * QR;
-    len = n + min(shared, ((int64_t)blockIdx.y + 1) * a.sh.chunk);  // (so that the keys end before it)
+    GroupTile t;
+    if (!group_of_tile(a.rows, a.sh.groups, blockIdx.x / a.nkv, rep, QR, &t) || (int64_t)blockIdx.y * a.sh.chunk >= t.shared) return;
+    row = t.row0;
+    rows_of = t.rows;
+    tok0 = t.tok0;
+    n = t.n;
+    x0 = t.tile * QR;
+    len = n + min(t.shared, ((int64_t)blockIdx.y + 1) * a.sh.chunk);  // (so that the keys end before it)
   } else {
     if constexpr (MODE == OWN) group = group_of_row(a.sh.groups, row, &from);
     if (!row_span(a.rows, row, a.most, &tok0, &n, &len) || x0 >= n * rep) {  // (the same in all blocks of a cluster)
@@ -593,14 +595,24 @@ int attend(cg_ctx* c, const PagedAttnArgs& a, bool bf16) {
   return bf16 ? launch_typed<__nv_bfloat16, ALL>(c, a) : launch_typed<float, ALL>(c, a);
 }
 
-// Into how many chunks shared keys are cut (0: rows read them for themselves).  A function of sizes alone, as the workspace's is.
-// Rows of so many tokens that they fill a tile of 128 queries by themselves gain nothing by others' beside them.
-void plan_chunks(PagedAttnArgs* args, bool bf16) {
+// Into how many chunks shared keys are cut (0: rows read them for themselves, out of L2).  A function of sizes alone, as the workspace's is.
+// Rows of so many tokens that they fill half a tile of 128 queries gain nothing by others' beside them.  Two launches more pay where 32 MB need not be read
+// again, whatever the type.  Us with chunks / row by row, rows of 1 token and [4]:
+//   12 rows behind  500, 8 key heads of 128, saves  23 MB   10.4  10.1  [12.3  12.9]
+//   40 behind       500, 4 of 128,                  40 MB   13.3  13.2  [18.7  15.4]
+//   12 behind      1500, 4 of 128,                  34 MB   11.8  12.1  [14.1  18.4]
+//   40 behind       500, 8 of 128,                  80 MB   18.9  22.7  [21.7  28.8]
+//   40 behind      5000, 8 of 128,                 799 MB   25.8  119   [34.6  144]
+//    4 behind      5000, 8 of 64,                   31 MB   15.5  10.6  [16.8  13.8]
+//   12 behind      1500, 4 of 256 with a cap,       68 MB   13.8  21.3  [14.4  22.2]
+//   40 behind       500, 2 of 64, f32,              20 MB   19.5  16.6  [19.5  16.8]
+//   40 behind      1500, 2 of 64, f32,              60 MB   20.0  40.6  [27.1  40.8]
+void plan_chunks(const cg_ctx* c, PagedAttnArgs* args, bool bf16) {
   PagedAttnArgs& a = *args;
-  const int64_t rep = a.nh / a.nkv;
+  const int64_t rep = a.nh / a.nkv, saved = (a.rows.rows - a.sh.groups.n) * a.sh.groups.most * 2 * a.nkv * a.d * (bf16 ? 2 : 4);
   a.sh.chunks = 0;
   a.sh.chunk = 0;
-  if (a.sh.groups.n == 0 || a.sh.groups.most == 0 || a.most * rep > 64) return;
+  if (a.sh.groups.n == 0 || a.sh.groups.most == 0 || a.most * rep > 64 || c->opt_shared == 0 || (c->opt_shared == 1 && saved < 32 << 20)) return;
   if (bf16) {
     a.sh.chunk = paged_fa_chunk(a);
   } else {
@@ -639,6 +651,7 @@ extern "C" int64_t cg_paged_shared_floats(cg_ctx* c, const cg_tensor* q, const c
     return -1;
   PagedAttnArgs a = {};
   a.rows.M = q->dims[0];
+  a.rows.rows = table->dims[0];
   a.nh = (int)q->dims[1];
   a.nkv = (int)k_pages->dims[1];
   a.d = (int)k_pages->dims[3];
@@ -647,7 +660,7 @@ extern "C" int64_t cg_paged_shared_floats(cg_ctx* c, const cg_tensor* q, const c
   const int64_t longest = table->dims[1] * k_pages->dims[2];
   a.sh.groups.n = groups->dims[0] - 1;
   a.sh.groups.most = max_shared > 0 ? std::min(max_shared, longest) : longest;
-  plan_chunks(&a, q->storage == ST_BF16);
+  plan_chunks(c, &a, q->storage == ST_BF16);
   return a.sh.chunks ? (a.sh.chunks + 1) * a.rows.M * a.nh * (a.d + 2) : 0;
 }
 
@@ -677,10 +690,10 @@ extern "C" int32_t cg_paged_shared_attention(cg_ctx* c, const cg_tensor* q, cons
   a.sh.groups.n = G[0];
   a.sh.groups.most = max_shared > 0 ? std::min(max_shared, longest) : longest;
   const bool bf16 = q->storage == ST_BF16;
-  plan_chunks(&a, bf16);
+  plan_chunks(c, &a, bf16);
   const int64_t parts = a.sh.chunks ? (a.sh.chunks + 1) * a.rows.M * a.nh : 0;
   if (work->dims[0] < parts * (a.d + 2)) return fail(c, CG_ERR_SHAPE, "work holds less than cg_paged_shared_floats");
-  if (parts > 0 && (uintptr_t)work->data() % 16) return fail(c, CG_ERR_UNSUPPORTED, "work begins on a 16-byte boundary");
+  if (parts > 0 && (uintptr_t)work->data() % 32) return fail(c, CG_ERR_UNSUPPORTED, "work begins on a 32-byte boundary");
   written(out);
   if (parts == 0) return attend(c, a, bf16);
   if (a.sh.chunks > 65535) return fail(c, CG_ERR_UNSUPPORTED, "too many tokens");

@@ -44,13 +44,18 @@ constexpr CG_HD float tanh_term(int i) {
        : i == 4 ? 0.019582903012633324f : -0.004716253839433193f;
 }
 #ifdef __CUDACC__
-// By a whole warp: which group and which of its tiles tile `t` of all groups is; -1 if there is none.  A token has `heads` query rows of a tile's `size`.
-__device__ __forceinline__ int64_t group_of_tile(const PagedRows& p, const PagedGroups& s, int64_t t, int64_t heads, int64_t size, int64_t* tile) {
+// A group of rows that a tile belongs to: its first row, rows, first packed token, tokens and shared tokens, and the tile's number in it.
+struct GroupTile {
+  int64_t row0, rows, tok0, n, shared, tile;
+};
+// By a whole warp: the group of tile `t` of all groups' tiles; false if there is none.  A token has `heads` query rows of a tile's `size`.
+__device__ __forceinline__ bool group_of_tile(const PagedRows& p, const PagedGroups& s, int64_t t, int64_t heads, int64_t size, GroupTile* out) {
   const int lane = threadIdx.x & 31;
   int64_t before = 0;
   for (int64_t g0 = 0; g0 < s.n; g0 += 32) {
-    int64_t row0, rows, tok0, n, keys, mine = 0;
-    if (g0 + lane < s.n && group_span(p, s, g0 + lane, &row0, &rows, &tok0, &n, &keys) && keys > 0) mine = (n * heads + size - 1) / size;
+    GroupTile x = {};
+    int64_t mine = 0;
+    if (g0 + lane < s.n && group_span(p, s, g0 + lane, &x.row0, &x.rows, &x.tok0, &x.n, &x.shared) && x.shared > 0) mine = (x.n * heads + size - 1) / size;
     int64_t sum = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -60,12 +65,17 @@ __device__ __forceinline__ int64_t group_of_tile(const PagedRows& p, const Paged
     const uint32_t has = __ballot_sync(0xffffffffu, t < before + sum);
     if (has) {
       const int at = __ffs(has) - 1;
-      *tile = t - (before + __shfl_sync(0xffffffffu, sum - mine, at));
-      return g0 + at;
+      out->tile = t - (before + __shfl_sync(0xffffffffu, sum - mine, at));
+      out->row0 = __shfl_sync(0xffffffffu, x.row0, at);
+      out->rows = __shfl_sync(0xffffffffu, x.rows, at);
+      out->tok0 = __shfl_sync(0xffffffffu, x.tok0, at);
+      out->n = __shfl_sync(0xffffffffu, x.n, at);
+      out->shared = __shfl_sync(0xffffffffu, x.shared, at);
+      return true;
     }
     before += __shfl_sync(0xffffffffu, sum, 31);
   }
-  return -1;
+  return false;
 }
 // By a whole warp: the group of a row (-1: it has none) and the tokens that it shares.
 __device__ __forceinline__ int64_t group_of_row(const PagedGroups& s, int64_t row, int64_t* shared) {

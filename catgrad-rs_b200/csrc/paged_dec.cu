@@ -41,29 +41,27 @@ struct DecArgs {
 // keys of a warp's tile, tiles of its ring
 template <int D>
 __host__ __device__ constexpr int dec_keys() { return D == 64 ? 32 : 16; }
-template <int MODE>
-__host__ __device__ constexpr int ring_of() { return MODE == OWN ? 2 : 3; }
-template <int D, int MODE>
-__host__ __device__ constexpr size_t dec_ring() { return (size_t)4 * ring_of<MODE>() * 2 * dec_keys<D>() * D * 2; }
-template <int D, int MODE>
-__host__ __device__ constexpr size_t dec_smem() { return 1024 + dec_ring<D, MODE>() + 4 * ring_of<MODE>() * 8; }
+constexpr int RING = 3;
+template <int D>
+__host__ __device__ constexpr size_t dec_ring() { return (size_t)4 * RING * 2 * dec_keys<D>() * D * 2; }
+template <int D>
+__host__ __device__ constexpr size_t dec_smem() { return 1024 + dec_ring<D>() + 4 * RING * 8; }
 
 template <int D, int ROWS, bool CAP, int MODE>
 __global__ void __launch_bounds__(128)
 k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, DecArgs p) {
   constexpr bool OWN = MODE == KeysOf::OWN;
-  constexpr int RING = ring_of<MODE>();
   constexpr int KT = dec_keys<D>(), SUB = D / 64, NB = ROWS / 8, KS = D / 16, LD = D + 4;
   constexpr uint32_t BOX = KT * 128, TILE = SUB * BOX;  // bytes of 64 components, of a tile
   extern __shared__ uint8_t smem_raw[];
   __shared__ float red_m[4][ROWS], red_l[4][ROWS], cta_m[ROWS], cta_l[ROWS];
   __shared__ int aborted;
-  static_assert((size_t)4 * ROWS * LD * 4 + (size_t)ROWS * LD * 4 <= dec_ring<D, MODE>(), "the warps' outputs lie over the ring");
+  static_assert((size_t)4 * ROWS * LD * 4 + (size_t)ROWS * LD * 4 <= dec_ring<D>(), "the warps' outputs lie over the ring");
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   float* red_o = (float*)(smem_raw + (base - raw));       // [4][ROWS][LD]
   float* part = red_o + 4 * ROWS * LD;                    // [ROWS][LD]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t2 = (lane & 3) * 2;
-  const uint32_t ring = base + warp * (RING * 2 * TILE), bars = base + (uint32_t)dec_ring<D, MODE>() + warp * (RING * 8);
+  const uint32_t ring = base + warp * (RING * 2 * TILE), bars = base + (uint32_t)dec_ring<D>() + warp * (RING * 8);
   if (lane == 0)
     for (int i = 0; i < RING; ++i) mbar_init(bars + 8 * i, 1);
   if (tid == 0) aborted = 0;
@@ -358,7 +356,7 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
 
 template <int D, int ROWS, bool CAP, int MODE>
 int launch(cg_ctx* c, const PagedAttnArgs& a) {
-  constexpr size_t smem = dec_smem<D, MODE>();
+  constexpr size_t smem = dec_smem<D>();
   static PerDeviceFlag configured_on;
   bool& configured = configured_on.at(c->core->device);
   if (!configured) {

@@ -154,8 +154,14 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
   int64_t group = -1;
   if (SHARED) {
     const int64_t tiles = (int)gridDim.x / (p.slices * p.sh.chunks), t = (int)blockIdx.x / p.slices % tiles;
-    const int64_t g = group_of_tile(p.rows, p.sh.groups, t, 1, (int64_t)NQ * p.per, &qt);
-    if (g < 0 || !group_span(p.rows, p.sh.groups, g, &row, &rows, &tok0, &n, &shared)) return;  // uniform over the CTA, before anything is allocated
+    GroupTile g;
+    if (!group_of_tile(p.rows, p.sh.groups, t, 1, (int64_t)NQ * p.per, &g)) return;  // uniform over the CTA, before anything is allocated
+    row = g.row0;
+    rows = g.rows;
+    tok0 = g.tok0;
+    n = g.n;
+    shared = g.shared;
+    qt = g.tile;
     len = 0;
   } else {
     if (OWN) group = group_of_row(p.sh.groups, row, &shared);
@@ -518,8 +524,11 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
       if (PART) {  // (without keys nothing was written: the sum says so)
         float* to = p.sh.out + part_at * p.d + c0;
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-          if (out && c0 + 4 * u < p.d) *(uint4*)(to + 4 * u) = make_uint4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+        for (int u = 0; u < 32; u += 8)  // (whole sectors: a row's values are a thread's)
+          if (out && c0 + u < p.d)
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + u), "r"(v[u]), "r"(v[u + 1]), "r"(v[u + 2]), "r"(v[u + 3]), "r"(v[u + 4]),
+                         "r"(v[u + 5]), "r"(v[u + 6]), "r"(v[u + 7])
+                         : "memory");
       } else if (out) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -771,9 +780,10 @@ int paged_fa_own(cg_ctx* c, const PagedAttnArgs& a) {
   if (a.d <= 128) return pick_own<128>(c, a);
   return pick_own<256>(c, a);
 }
-// Keys of a chunk: as many chunks as keep all SMs busy, two blocks on one where they fit, in one wave however the tokens are dealt to the groups.
+// Keys of a chunk: as many chunks as make a block per SM, or one and a half where two fit (the rows' own keys then begin beside them), in one wave however the
+// tokens are dealt to the groups.
 int64_t paged_fa_chunk(const PagedAttnArgs& a) {
-  const int64_t slots = a.d <= 128 ? 296 : 148, queries = a.rows.M * (a.nh / a.nkv), tiles = std::max<int64_t>((queries + a.sh.groups.n * 127) / 128, 1) * a.nkv;
+  const int64_t slots = a.d <= 128 ? 222 : 148, queries = a.rows.M * (a.nh / a.nkv), tiles = std::max<int64_t>((queries + a.sh.groups.n * 127) / 128, 1) * a.nkv;
   const int64_t chunks = std::max<int64_t>(slots / tiles, 1), keys = (a.sh.groups.most + chunks - 1) / chunks;
   return std::max<int64_t>((keys + KT - 1) / KT * KT, 2 * KT);
 }

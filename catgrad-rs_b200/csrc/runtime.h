@@ -110,6 +110,7 @@ struct cg_ctx {
   int opt_pair_cta = 1;   // 1: the largest of those take the CTA-pair (cta_group::2) kernel; 2: every GEMM that reaches gemm_tc does
   int opt_handover = 1;   // decode steps: residual GEMMs prepare the next norm, the next GEMM applies 1 / rms
   int opt_fa = 1;         // prefill attention on tcgen05 (attention_fa.cu) where it applies
+  int opt_shared = 1;     // prefixes that rows share are read once (2: always, 0: never)
   int opt_prefill_chunk = 8192;  // tokens per prefill chunk (bounds the decoder's workspace)
   int opt_peer = 1;       // small all-reduces over mapped peer memory instead of NCCL (when available)
   int opt_resident = 0;   // 1: decode steps of dense pre-norm models run as one resident kernel (decode_resident.cu)

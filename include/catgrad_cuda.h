@@ -172,6 +172,8 @@ int32_t cg_to_vec_u32(cg_ctx*, const cg_tensor* x, uint32_t* dst, int64_t n);
  *             applies 1 / rms in its epilogue (no separate norm kernel); 0 = norm kernels
  *   "fa"    : 1 (default) = prefill attention on tcgen05 / TMEM (rows of at least 17 tokens, 64 with distance biases; 2 = the variant
  *             that keeps outputs in registers, for head sizes 64 and 128 without soft-cap); 0 = the mma.sync kernel everywhere
+ *   "shared_prefix" : 1 (default) = cg_paged_shared_attention reads what rows have in common once where that saves enough; 2 = always
+ *             (tests), 0 = never.  cg_paged_shared_floats follows it
  *   "prefill_chunk" : tokens per prefill chunk (default 8192; bounds the decoder's workspace)
  *   "peer"  : 1 (default) = decode steps under tensor parallelism reduce over mapped peer
  *             memory (see cg_comm_peer_exchange); 0 = NCCL collectives.  Set before the first
@@ -326,7 +328,8 @@ int32_t cg_paged_attention(cg_ctx*, const cg_tensor* q, const cg_tensor* k_pages
  * inside the prefix, and all of it is read.  max_shared: no group shares more (0 = not known: the table's width); a group that
  * does, or whose numbers cannot be, is left out (CG_ERR_INDEX).  work F32 [n]: room for what is joined at the end, written over, n at
  * least cg_paged_shared_floats of the same tensors and numbers (-1: they do not fit each other); calls that may overlap in time, as
- * captured graphs on two streams, need one each.  Rows with many new tokens read the prefix for themselves, which costs them nothing. */
+ * captured graphs on two streams, need one each; it begins on a 32-byte boundary.  Where little would be saved, or rows have many new tokens, they read
+ * the prefix for themselves (then n may be 0). */
 int64_t cg_paged_shared_floats(cg_ctx*, const cg_tensor* q, const cg_tensor* k_pages, const cg_tensor* table, const cg_tensor* groups,
                                int64_t max_new, int64_t max_shared);
 int32_t cg_paged_shared_attention(cg_ctx*, const cg_tensor* q, const cg_tensor* k_pages, const cg_tensor* v_pages,

@@ -502,6 +502,14 @@ def test_verify_rows_that_cannot_be(cuda):
 # ---------------------------------------------------------------- attention over shared prefixes
 
 
+@pytest.fixture
+def always(cuda):
+    """Prefixes are read once however little that saves."""
+    cuda.set_option("shared_prefix", 2)
+    yield cuda
+    cuda.set_option("shared_prefix", 1)
+
+
 class Shared:
     """Groups (rows, shared tokens), between them rows of none (shared None); new[r] tokens of row r, `own[r]` cached ones behind the prefix with them.  Full pages of a prefix
     are one for all rows, its begun page is copied."""
@@ -611,67 +619,67 @@ GROUPS = [([(1, 1)], [1], [1]), ([(3, 40)], [1, 1, 1], [1, 9, 30]), ([(2, 129), 
 @pytest.mark.parametrize("store", ["f32", "bf16"])
 @pytest.mark.parametrize("nh,nkv,d", [(4, 2, 64), (8, 1, 128), (2, 2, 256), (3, 3, 24), (6, 2, 96), (32, 4, 128), (8, 2, 40), (5, 1, 64)])
 @pytest.mark.parametrize("window,cap", [(0, 0.0), (70, 0.0), (0, 3.0), (33, 20.0)])
-def test_shared_attention(cuda, store, nh, nkv, d, window, cap):
+def test_shared_attention(always, store, nh, nkv, d, window, cap):
     for i, (groups, new, own) in enumerate(GROUPS):
-        check_shared(cuda, Shared(groups, new, own, (8, 16, 64, 256)[i % 4], seed=i, spare=i % 3), store, nh, nkv, d, window, cap, scale=0.0 if i % 3 else 0.3, strided=i % 2 == 1)
+        check_shared(always, Shared(groups, new, own, (8, 16, 64, 256)[i % 4], seed=i, spare=i % 3), store, nh, nkv, d, window, cap, scale=0.0 if i % 3 else 0.3, strided=i % 2 == 1)
 
 
 @gpu
 @pytest.mark.parametrize("store", ["f32", "bf16"])
 @pytest.mark.parametrize("nh,nkv,d", [(4, 2, 64), (8, 2, 128), (2, 1, 256)])
 @pytest.mark.parametrize("page", [8, 32, 1024])
-def test_shared_attention_many_chunks(cuda, store, nh, nkv, d, page):
+def test_shared_attention_many_chunks(always, store, nh, nkv, d, page):
     """Prefixes of many chunks and of hardly more than some, that end anywhere."""
     for i, shared in enumerate((127, 128, 129, 256, 1000, 3001)):
         b = Shared([(3, shared), (2, shared // 2)], [1, 2, 1, 1, 3], [1, 5, 70, 33, 3], page, seed=i)
-        floats = check_shared(cuda, b, store, nh, nkv, d, repeat=2)
+        floats = check_shared(always, b, store, nh, nkv, d, repeat=2)
         assert shared < 1000 or floats > 2 * b.M * nh * (d + 2)   # (several chunks)
 
 
 @gpu
 @pytest.mark.parametrize("store", ["f32", "bf16"])
 @pytest.mark.parametrize("nh,nkv,d", [(4, 1, 64), (16, 2, 128), (4, 2, 256)])
-def test_shared_attention_many_queries(cuda, store, nh, nkv, d):
+def test_shared_attention_many_queries(always, store, nh, nkv, d):
     """Groups whose queries fill more than a tile, and rows that fill one by themselves."""
-    check_shared(cuda, Shared([(70, 300), (20, 129)], [1 + r % 4 for r in range(90)], [4 + r for r in range(90)], 16, seed=1), store, nh, nkv, d)
-    check_shared(cuda, Shared([(3, 500)], [150, 3, 40], [150, 60, 41], 16, seed=2), store, nh, nkv, d)
-    check_shared(cuda, Shared([(1, 200)] * 50, [1] * 50, [2] * 50, 16, seed=3), store, nh, nkv, d)
+    check_shared(always, Shared([(70, 300), (20, 129)], [1 + r % 4 for r in range(90)], [4 + r for r in range(90)], 16, seed=1), store, nh, nkv, d)
+    check_shared(always, Shared([(3, 500)], [150, 3, 40], [150, 60, 41], 16, seed=2), store, nh, nkv, d)
+    check_shared(always, Shared([(1, 200)] * 50, [1] * 50, [2] * 50, 16, seed=3), store, nh, nkv, d)
 
 
 @gpu
 @pytest.mark.parametrize("store", ["f32", "bf16"])
 @pytest.mark.parametrize("window", [0, 5, 64, 150])
-def test_shared_attention_tokens_inside_the_prefix(cuda, store, window):
+def test_shared_attention_tokens_inside_the_prefix(always, store, window):
     """New tokens that stand before the prefix's end, rows that end there, and rows shorter than that."""
     b = Shared([(4, 200)], [3, 5, 1, 8], [2, 0, 30, 4], 16, seed=4)
     assert [t - n for n, t in zip(b.new, b.total)][1] < 200
     for d in (64, 128):
-        check_shared(cuda, b, store, 4, 2, d, window)
+        check_shared(always, b, store, 4, 2, d, window)
 
 
 @gpu
 @pytest.mark.parametrize("store", ["f32", "bf16"])
 @pytest.mark.parametrize("offset", [1, 2, 8])
-def test_shared_attention_of_unaligned_queries(cuda, store, offset):
+def test_shared_attention_of_unaligned_queries(always, store, offset):
     for d in (64, 128, 40):
-        check_shared(cuda, Shared([(4, 200), (2, 70)], [1, 2, 3, 1, 1, 1], [3, 9, 30, 1, 5, 6], 16, seed=offset), store, 4, 2, d, offset=offset)
+        check_shared(always, Shared([(4, 200), (2, 70)], [1, 2, 3, 1, 1, 1], [3, 9, 30, 1, 5, 6], 16, seed=offset), store, 4, 2, d, offset=offset)
 
 
 @gpu
 @pytest.mark.parametrize("store", ["f32", "bf16"])
-def test_shared_attention_without_its_numbers(cuda, store):
+def test_shared_attention_without_its_numbers(always, store):
     """max_new and max_shared not known: the packed tokens and the table's width stand for them."""
     for new in ([1, 2, 3, 1, 1, 1], [1, 20, 3, 1, 1, 1]):
         b = Shared([(4, 200), (2, 70)], new, [3, 29, 30, 1, 5, 6], 16, seed=6, extra=40)
-        check_shared(cuda, b, store, 4, 2, 64, max_new=0, max_shared=0)
-        check_shared(cuda, b, store, 4, 2, 128, max_new=0, max_shared=200)
+        check_shared(always, b, store, 4, 2, 64, max_new=0, max_shared=0)
+        check_shared(always, b, store, 4, 2, 128, max_new=0, max_shared=200)
 
 
 @gpu
 @pytest.mark.parametrize("store", ["f32", "bf16"])
-def test_shared_attention_groups_that_cannot_be(cuda, store):
+def test_shared_attention_groups_that_cannot_be(always, store):
     """Such a group's rows are left as they were, and the others are not."""
-    B = cuda
+    B = always
     nh, nkv, d = 4, 2, 64
     for what in ("order", "rows", "shared", "starts"):
         b = Shared([(2, 100), (2, 150)], [1, 1, 1, 2], [5, 6, 7, 8], 16, seed=7)
@@ -706,3 +714,17 @@ def test_shared_attention_groups_that_cannot_be(cuda, store):
     B.paged_shared_attention(q[0], k[0], v[0], *up, work, max_new=1, max_shared=100, out=out[0])
     raises_index(B)
     assert np.isfinite(back(B, out[1])).all()
+
+
+@gpu
+@pytest.mark.parametrize("store,nh,nkv,d,rows,shared", [("bf16", 8, 8, 128, 12, 800), ("f32", 4, 2, 64, 24, 1500), ("bf16", 4, 4, 256, 10, 1000)])
+def test_shared_attention_where_it_saves_enough(cuda, store, nh, nkv, d, rows, shared):
+    """Without the option: prefixes that are read once, and the same ones row by row."""
+    b = Shared([(rows, shared)], [1 + r % 2 for r in range(rows)], [2 + 5 * r for r in range(rows)], 32, seed=rows)
+    assert check_shared(cuda, b, store, nh, nkv, d) > 1
+    try:
+        cuda.set_option("shared_prefix", 0)
+        assert check_shared(cuda, b, store, nh, nkv, d) == 1
+    finally:
+        cuda.set_option("shared_prefix", 1)
+    assert check_shared(cuda, Shared([(2, shared)], [1, 1], [2, 5], 32), store, nh, nkv, d) == 1
