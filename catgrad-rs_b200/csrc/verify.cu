@@ -35,7 +35,8 @@ struct VerifyArgs {
   const uint32_t *tokens, *starts, *lens;  // lens may be null
   const float *uniform, *temperature;      // temperature may be null: 1
   uint32_t *accepted, *next, *lens_out;
-  int64_t rows, M, V, most;
+  int64_t rows, M, most;
+  int V;
   int slice;                   // tokens of a block
   int ahead;                   // positions judged at a time
   int probs16;
@@ -45,6 +46,13 @@ struct VerifyArgs {
 
 __device__ __forceinline__ float widen(float x) { return x; }
 __device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
+// Word i of a vector, and value i of it as it is stored (i is known when compiling)
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+template <typename T>
+__device__ __forceinline__ float value_of(const uint4& v, int i) {
+  if (sizeof(T) == 4) return __uint_as_float(word_of(v, i));
+  return __uint_as_float(i & 1 ? word_of(v, i / 2) & 0xffff0000u : word_of(v, i / 2) << 16);
+}
 // (NaN counts as -inf)
 template <typename T>
 __device__ __forceinline__ float logit(T x) { return fmaxf(widen(x), NO_LOGIT); }
@@ -113,13 +121,12 @@ struct Slice {
     tail = count - head - vectors * E;
   }
   __device__ __forceinline__ int end_of(int tid) const { return tid < head ? tid : tid >= E && tid < E + tail ? head + vectors * E + tid - E : -1; }
-  __device__ __forceinline__ uint4 vector(int v) const { return __ldg((const uint4*)(src + head) + v); }
 };
 
-// VT: threads.  Of a position a thread has every VT-th vector, four a step; the next step's are on their way while these are judged.
-template <typename T, int VT>
-__global__ void __launch_bounds__(VT, 1024 / VT) k_verify_drafts(VerifyArgs a) {
-  constexpr int E = 16 / sizeof(T), W = VT / 32, U = 16 / E;  // values of a vector, warps, vectors of a step
+// VT: threads.  Of a position a thread has every VT-th vector, U a step; the next step's are on their way while these are judged.
+template <typename T, int VT, int ON_SM>
+__global__ void __launch_bounds__(VT, ON_SM) k_verify_drafts(VerifyArgs a) {
+  constexpr int E = 16 / sizeof(T), W = VT / 32, U = VT * ON_SM < 1024 ? 4 : 16 / E;  // values of a vector, warps, vectors of a step (as registers allow)
   constexpr int SUB = 32 / W;                            // parts of a warp's tokens, of which there are sums
   extern __shared__ __align__(16) uint8_t staging[];  // the drafter's probabilities at a position
   __shared__ double power[16];
@@ -141,42 +148,50 @@ __global__ void __launch_bounds__(VT, 1024 / VT) k_verify_drafts(VerifyArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // (the same in all blocks of a cluster, as everything that decides which way they go)
-  const int64_t s0 = a.starts[row], s1 = a.starts[row + 1], n = s1 - s0;
+  const uint32_t s0 = a.starts[row], s1 = a.starts[row + 1];
   const float heat_in = a.temperature ? a.temperature[row] : 1.f;
   const uint32_t len = a.lens ? a.lens[row] : 0xFFFFFFFFu;
-  if (n == 0) return;
-  if (!(s0 < s1 && s1 <= a.M && n <= a.most && len >= n - 1)) {
+  if (s0 == s1) return;
+  const int n = (int)(s1 - s0);  // (places are 31 bits)
+  if (!(s0 < s1 && s1 <= a.M && n <= a.most && len >= (uint32_t)n - 1u)) {
     if (tid == 0) *a.err = DEV_INDEX;
     return;
   }
   // (nothing is put into another block's memory before it runs: waited for ahead of the first put)
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-  const int64_t lo = std::min<int64_t>((int64_t)block * a.slice, a.V), hi = std::min<int64_t>(lo + a.slice, a.V);
-  const int count = (int)(hi - lo);
-  auto place = [&](int64_t pos) { return (const T*)a.logits + (s0 + pos) * a.l_ld + lo; };
-  const int steps = max(1, (count / E + U * VT - 1) / (U * VT));  // of a position
-  struct Step {
-    uint4 x[U];
+  const int lo = std::min(block * a.slice, a.V), count = std::min(lo + a.slice, a.V) - lo;
+  auto place = [&](int pos) { return (const T*)a.logits + (int64_t)(s0 + pos) * a.l_ld + lo; };
+  // A position's slice as this thread reads it: U of its vectors at a time, VT apart, and its value of the ends.
+  struct Cursor {
+    const uint4* at;  // the next vector
+    int left;         // vectors from that on, those of other threads among them
+    uint4 x[U];       // on their way
     T end;
   };
-  auto load = [&](Step& to, int64_t pos, int step) {
-    const Slice<T> f(place(pos), count);
+  auto load = [&](Cursor& c) {
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int v = tid + (step * U + i) * VT;
       constexpr uint32_t none = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;  // (-inf)
-      to.x[i] = v < f.vectors ? f.vector(v) : make_uint4(none, none, none, none);
+      c.x[i] = make_uint4(none, none, none, none);
+      if (i * VT < c.left) c.x[i] = __ldg(c.at + i * VT);
     }
-    const int e = step == 0 ? f.end_of(tid) : -1;
-    to.end = e >= 0 ? f.src[e] : (T)NO_LOGIT;
+    c.at += U * VT;
+    c.left -= U * VT;
   };
-  int64_t first = 0;  // of the positions judged at a time
-  int parity = 0, group = (int)std::min<int64_t>(a.ahead, n), stop = -1;
-  Step ahead;
-  load(ahead, 0, 0);
+  auto begin = [&](Cursor& c, int pos) {
+    const Slice<T> f(place(pos), count);
+    c.at = (const uint4*)(f.src + f.head) + tid;
+    c.left = f.vectors - tid;
+    load(c);
+    const int e = f.end_of(tid);
+    c.end = e >= 0 ? f.src[e] : (T)NO_LOGIT;
+  };
+  int first = 0, parity = 0, group = std::min(a.ahead, n), stop = -1;  // first: of the positions judged at a time
+  Cursor ahead;
+  begin(ahead, 0);
 
   bool bad = false;
-  for (int64_t i = 1 + tid; i < n; i += VT) bad = bad || a.tokens[s0 + i] >= a.V;
+  for (int i = 1 + tid; i < n; i += VT) bad = bad || a.tokens[s0 + i] >= (uint32_t)a.V;
   const float u_next = a.uniform[s1 - 1];
   const bool greedy = !(heat_in > 0.f);
   // (temperatures beyond 2^+-100 act as these)
@@ -197,7 +212,7 @@ __global__ void __launch_bounds__(VT, 1024 / VT) k_verify_drafts(VerifyArgs a) {
     auto judge = [&](int j) {
       Judged x = {NONE, 0, 0.f, (T)NO_LOGIT};
       if (j >= group || first + j >= n - 1) return x;
-      const int64_t m = s0 + first + j;
+      const int64_t m = (int64_t)s0 + first + j;
       x.draft = a.tokens[m + 1];
       x.u = a.uniform[m];
       x.logit = ((const T*)a.logits)[m * a.l_ld + x.draft];
@@ -207,17 +222,30 @@ __global__ void __launch_bounds__(VT, 1024 / VT) k_verify_drafts(VerifyArgs a) {
     };
     const Judged mine = judge(warp);
     for (int j = 0; j < group; ++j) {
-      float top = NO_LOGIT, sum = 0.f;
+      float top = NO_LOGIT, sum = 0.f, end = logit(ahead.end);  // (the ends count once)
       uint32_t at = NONE;
-      for (int step = 0; step < steps; ++step) {
-        const Step now = ahead;
-        const int64_t next_pos = step + 1 < steps ? first + j : first + j + 1;
-        if (next_pos < n) load(ahead, next_pos, step + 1 < steps ? step + 1 : 0);
-        auto value = [&](int i) { return widen(((const T*)&now.x[i / E])[i % E]); };  // (unpacked each time, which keeps registers)
-        const float end = widen(now.end);
-        float t[4] = {fmaxf(end, NO_LOGIT), NO_LOGIT, NO_LOGIT, NO_LOGIT};
+      for (int step = 0;; ++step) {
+        uint4 now[U];
 #pragma unroll
-        for (int i = 0; i < U * E; ++i) t[i & 3] = fmaxf(t[i & 3], value(i));
+        for (int i = 0; i < U; ++i) now[i] = ahead.x[i];
+        auto value = [&](int i) { return value_of<T>(now[i / E], i % E); };  // (unpacked where it is used, which keeps registers)
+        const bool more_steps = ahead.left > 0;
+        if (more_steps) load(ahead);
+        else if (first + j + 1 < n) begin(ahead, first + j + 1);
+        float t[4] = {end, NO_LOGIT, NO_LOGIT, NO_LOGIT};
+        if constexpr (sizeof(T) == 2) {  // (two values at a time)
+          uint32_t m[2] = {0xFF80FF80u, 0xFF80FF80u};
+#pragma unroll
+          for (int i = 0; i < U * E / 2; ++i) asm("max.bf16x2 %0, %0, %1;" : "+r"(m[i & 1]) : "r"(word_of(now[i / 4], i % 4)));
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            t[2 * i] = fmaxf(t[2 * i], __uint_as_float(m[i] << 16));
+            t[2 * i + 1] = fmaxf(t[2 * i + 1], __uint_as_float(m[i] & 0xffff0000u));
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < U * E; ++i) t[i & 3] = fmaxf(t[i & 3], value(i));
+        }
         t[0] = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
         if (greedy) {
           // (a thread's places ascend from step to step, but for the ends: before all others or behind them)
@@ -225,7 +253,7 @@ __global__ void __launch_bounds__(VT, 1024 / VT) k_verify_drafts(VerifyArgs a) {
             const Slice<T> f(place(first + j), count);
             if (t[0] > top) at = NONE;
             top = t[0];
-            if (step == 0 && end == top) at = min(at, (uint32_t)(lo + f.end_of(tid)));
+            if (end == top) at = min(at, (uint32_t)(lo + f.end_of(tid)));
 #pragma unroll
             for (int i = 0; i < U * E; ++i)
               if (value(i) == top) at = min(at, (uint32_t)(lo + f.head + (tid + (step * U + i / E) * VT) * E + i % E));
@@ -241,16 +269,15 @@ __global__ void __launch_bounds__(VT, 1024 / VT) k_verify_drafts(VerifyArgs a) {
             for (int i = 0; i < U * E; ++i) s[i & 3] += fast_exp2((value(i) - top) * unit);
             float more = (s[0] + s[1]) + (s[2] + s[3]);
             if (more != more) {  // (some are no numbers)
-              more = 0.f;
+              more = fast_exp2((end - top) * unit);
 #pragma unroll
-              for (int i = 0; i < U * E + 1; ++i) {
-                const float y = i < U * E ? value(i % (U * E)) : end;
-                more += y == y ? fast_exp2((y - top) * unit) : 0.f;
-              }
+              for (int i = 0; i < U * E; ++i) more += value(i) == value(i) ? fast_exp2((value(i) - top) * unit) : 0.f;
             }
             sum += more;
           }
         }
+        end = NO_LOGIT;
+        if (!more_steps) break;
       }
       const float t = warp_max(top);
       if (greedy) {
@@ -309,11 +336,12 @@ __global__ void __launch_bounds__(VT, 1024 / VT) k_verify_drafts(VerifyArgs a) {
       break;
     }
     first += group;
-    group = (int)std::min<int64_t>(a.ahead, n - first);
+    group = std::min(a.ahead, n - first);
   }
 
   // ---- the next token, at position first + stop ----
-  const int64_t pos = first + stop, m = s0 + pos;
+  const int pos = first + stop;
+  const int64_t m = (int64_t)s0 + pos;
   const float top = pos_top[stop];
   uint32_t token = NONE;
   bool write = block == 0 && tid == 0;
@@ -357,7 +385,7 @@ __global__ void __launch_bounds__(VT, 1024 / VT) k_verify_drafts(VerifyArgs a) {
               for (int e = phase; e < QE; ++e)
                 if (e - phase < w1) ((Q*)to)[e] = q_at[e - phase];
             } else {
-              cp_async16(smem_u32(to + v * 16), q_at + w0 + j0, (int)(std::min<int64_t>(QE, a.V - lo - w0 - j0) * (int64_t)sizeof(Q)));
+              cp_async16(smem_u32(to + v * 16), q_at + w0 + j0, std::min(QE, a.V - lo - w0 - j0) * (int)sizeof(Q));
             }
           }
           cp_async_commit();
@@ -403,7 +431,7 @@ __global__ void __launch_bounds__(VT, 1024 / VT) k_verify_drafts(VerifyArgs a) {
           e_left = warp_sum(e_left);
           q_left = warp_sum(q_left);
         } else if (mode == 1) {
-          const int64_t d = (int64_t)draft - lo;
+          const int d = (int)draft - lo;
           e_left = e_all - (d >= v0 && d < v1 ? weigh(logit(values[d])) : 0.0);
         }
         if (lane == 0) {
@@ -433,7 +461,7 @@ __global__ void __launch_bounds__(VT, 1024 / VT) k_verify_drafts(VerifyArgs a) {
     auto rest = [&](int j) {
       const double e = weigh(logit(values[j]));
       if (mode == 0) return e;
-      if (mode == 1) return lo + j == draft ? 0.0 : e;
+      if (mode == 1) return (uint32_t)(lo + j) == draft ? 0.0 : e;
       return fmax(e - (double)drafter(j) * whole, 0.0);
     };
     // ---- the first token whose inclusive sum is above u times the whole ----
@@ -490,7 +518,7 @@ __global__ void __launch_bounds__(VT, 1024 / VT) k_verify_drafts(VerifyArgs a) {
   if (write) {
     a.accepted[row] = (uint32_t)pos;
     a.next[row] = token;
-    if (a.lens) a.lens_out[row] = (uint32_t)(len - (n - 1 - pos));
+    if (a.lens) a.lens_out[row] = len - (uint32_t)(n - 1 - pos);
   }
 }
 
@@ -503,14 +531,14 @@ int check_places(cg_ctx* c, const cg_tensor* t, const char* what, int64_t M, int
   return CG_OK;
 }
 
-template <typename T, int VT>
+template <typename T, int VT, int ON_SM>
 int launch_threads(cg_ctx* c, VerifyArgs& a, int blocks) {
-  constexpr int smem_most = 96 * 1024;  // (two blocks on an SM)
+  constexpr int smem_most = 210 * 1024 / ON_SM;
   static PerDeviceFlag configured_on;
   bool& configured = configured_on.at(c->core->device);
   if (!configured) {
-    CG_CUDA(c, cudaFuncSetAttribute(k_verify_drafts<T, VT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_most));
-    CG_CUDA(c, cudaFuncSetAttribute(k_verify_drafts<T, VT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    CG_CUDA(c, cudaFuncSetAttribute(k_verify_drafts<T, VT, ON_SM>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_most));
+    CG_CUDA(c, cudaFuncSetAttribute(k_verify_drafts<T, VT, ON_SM>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     configured = true;
   }
   a.slice = (int)((a.V + blocks - 1) / blocks);
@@ -520,21 +548,26 @@ int launch_threads(cg_ctx* c, VerifyArgs& a, int blocks) {
   const int64_t staging = a.probs ? (int64_t)a.slice * (a.probs16 ? 2 : 4) + 32 * (VT / 32 + 1) : 0;
   a.staged = staging > 0 && staging <= smem_most;
   const size_t smem = a.staged ? (size_t)staging : 0;
-  CG_CUDA(c, launch_kernel(c, k_verify_drafts<T, VT>, dim3((unsigned)blocks, (unsigned)a.rows), dim3(VT), smem, -blocks, a));
+  CG_CUDA(c, launch_kernel(c, k_verify_drafts<T, VT, ON_SM>, dim3((unsigned)blocks, (unsigned)a.rows), dim3(VT), smem, -blocks, a));
   CG_LAUNCHED(c);
   return CG_OK;
 }
 template <typename T>
 int launch(cg_ctx* c, VerifyArgs& a) {
-  // Blocks of a row, and threads, us with blocks x threads, [the rule's]:
-  //   1 row x 128256, f32, 4 drafts          [16 x 512] 15.7  16 x 256 18.3  8 x 512 21.5  4 x 512 39
-  //   40 x 151936, bf16, 4                   [8 x 512] 55  8 x 256 55  16 x 256 54  16 x 512 67  4 x 512 57
-  //   32 x 256000, bf16, 7, no probabilities [8 x 512] 51  8 x 256 60  16 x 256 54
-  //   16 x 50257, f32, 3, greedy             [8 x 512] 10.1  8 x 256 9.3  16 x 256 10.8
-  //   38 x 2736, f32, 3                      [4 x 256] 14.5  8 x 256 15.7  16 x 512 35
-  int blocks = a.V >= 65536 && a.rows * MOST_BLOCKS <= 2 * 148 ? MOST_BLOCKS : 8;
-  while (blocks > 1 && (a.rows * blocks > 4 * 148 || a.V < 512 * blocks)) blocks /= 2;
-  return a.V >= 4096 * blocks ? launch_threads<T, 512>(c, a, blocks) : launch_threads<T, 256>(c, a, blocks);
+  // Blocks of a row, and their threads and how many run on an SM, us, [the rule's]:
+  //                                                 16 x 512, 1   8 x 512, 1   8 x 512, 2   8 x 256, 3   4 x 256, 3
+  //   1 row x 128256, f32, 4 drafts                 [14.4]        19.2         20           24           41
+  //   3 x 54082, bf16, 1                             11.1         [12.0]                    13.2         18.5
+  //   16 x 50257, f32, 3, greedy                     16           10.9         10.0         [8.0]        10.1
+  //   32 x 256000, bf16, 7, no probabilities         86           73           [48.8]       59           77
+  //   40 x 151936, bf16, 4                           84           59           54           [47.8]       59
+  //   38 x 2736, f32, 3                              46           25           23           13.6         [12.5]
+  // More threads for a row hide the draw's 64-bit chains; more of them than run at a time wait for whole clusters to end.
+  int blocks = a.V >= 65536 && a.rows * MOST_BLOCKS <= 148 ? MOST_BLOCKS : 8;
+  while (blocks > 1 && (a.rows * blocks > 3 * 148 || a.V < 512 * blocks)) blocks /= 2;
+  if (a.rows * blocks <= 74 && a.V >= 2048 * blocks) return launch_threads<T, 512, 1>(c, a, blocks);
+  if (a.rows * blocks > 148 && a.rows * blocks <= 2 * 148 && a.V >= 16384 * blocks) return launch_threads<T, 512, 2>(c, a, blocks);
+  return launch_threads<T, 256, 3>(c, a, blocks);
 }
 
 }  // namespace
@@ -594,7 +627,7 @@ extern "C" int32_t cg_verify_drafts(cg_ctx* c, const cg_tensor* logits, const cg
   a.lens_out = lens_out ? (uint32_t*)lens_out->data() : nullptr;
   a.rows = rows;
   a.M = M;
-  a.V = V;
+  a.V = (int)V;
   a.most = max_new > 0 ? std::min(max_new, M) : M;
   a.err = c->core->dev_err;
   written(accepted);
