@@ -7,12 +7,14 @@ a draw nearer to a border than 2^-40 of the whole is left out.
 """
 import ctypes
 import math
+import os
+import subprocess
 
 import numpy as np
 import pytest
 
-from conftest import cg
-from test_paged import BF16, F32, Host, attention, back, host, put, rounded  # noqa: F401
+from conftest import ROOT, cg
+from test_paged import BF16, F32, Host, attention, back, net, plain_logits, put, rounded
 
 gpu = pytest.mark.gpu
 INDEX = 6
@@ -217,7 +219,7 @@ def test_assign_slots_beyond_32_bits(cuda):
 # ---------------------------------------------------------------- drafted tokens
 
 
-def plain_verify(logits, probs, tokens, starts, uniform, heat, lens):
+def plain_verify(logits, probs, tokens, starts, uniform, heat, lens, judged=2.0 ** -20, drawn=2.0 ** -40):
     """Row by row in 64 bits: (accepted, next, lens), and the rows that a border is too near for."""
     out, near = [], set()
     for r in range(len(starts) - 1):
@@ -232,9 +234,8 @@ def plain_verify(logits, probs, tokens, starts, uniform, heat, lens):
             top = x.max()
             last = m == b - 1
             if not np.isfinite(top):
-                if last or True:
-                    w = None
-                    break
+                w = None
+                break
             if not T > 0:
                 p = np.zeros_like(x)
                 p[int(np.argmax(x))] = 1.0
@@ -252,7 +253,7 @@ def plain_verify(logits, probs, tokens, starts, uniform, heat, lens):
             if T > 0:
                 u = np.float64(uniform[m])
                 stands = u * q[d] < p[d]
-                if abs(u * q[d] - p[d]) <= 2.0 ** -20 * p[d]:
+                if abs(u * q[d] - p[d]) <= judged * p[d]:
                     near.add(r)
             else:
                 stands = p[d] == 1.0
@@ -274,7 +275,7 @@ def plain_verify(logits, probs, tokens, starts, uniform, heat, lens):
             else:
                 above = np.nonzero((c > t) & (w > 0))[0]
                 token = int(above[0]) if len(above) else int(np.nonzero(w)[0][-1])
-                if len(w) > 1 and np.abs(c[:-1] - t).min() <= 2.0 ** -40 * c[-1] and 0 < t < c[-1]:
+                if len(w) > 1 and np.abs(c[:-1] - t).min() <= drawn * c[-1] and 0 < t < c[-1]:
                     near.add(r)
         out.append((m - a, token, int(lens[r]) - (b - 1 - m)))
     return out, near
@@ -728,3 +729,397 @@ def test_shared_attention_where_it_saves_enough(cuda, store, nh, nkv, d, rows, s
     finally:
         cuda.set_option("shared_prefix", 1)
     assert check_shared(cuda, Shared([(2, shared)], [1, 1], [2, 5], 32), store, nh, nkv, d) == 1
+
+
+# ---------------------------------------------------------------- all of them together
+
+
+@gpu
+@pytest.mark.parametrize("heat,page", [(0.0, 8), (1.0, 16)])
+def test_drafts_are_served_from_one_cache(always, heat, page):
+    """Requests behind one system prompt, served with drafts: pages from a stack, append, attention over the shared prefix, verification, and lengths without
+    what was rejected, until each has its tokens; against the same decisions made from 64-bit logits of whole sequences without a cache.  2 layers of f32
+    sums of at most 128 products leave logits of some 10 within 1e-4, so decisions nearer to a border than 1e-3 are taken from the device."""
+    import torch
+    B = always
+    rng = np.random.default_rng(page)
+    hidden, nh, nkv, d, vocab, layers, T = 64, 4, 2, 32, 211, 2, 160
+    W = net(rng, hidden, nh, nkv, d, vocab, layers)
+    system, prompts = rng.integers(0, vocab, 2 * page), [rng.integers(0, vocab, n) for n in (5, 17, 1, 9)]
+    R, cols, pages = len(prompts), T // page, 60
+    cos_t, sin_t = B.rope_tables(10000.0, T, d)
+    cos, sin = B.to_numpy(cos_t), B.to_numpy(sin_t)
+    up = lambda a: B.from_numpy(np.ascontiguousarray(a))
+    Wd = {"embed": up(W["embed"]), "head": up(W["head"]), "layers": [{n: up(a) for n, a in L.items()} for L in W["layers"]]}
+    kc, vc = (torch.full((layers, pages, nkv, page, d), float("nan"), device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    pools = [(B.from_device(kc[i]), B.from_device(vc[i])) for i in range(layers)]
+    u32 = lambda *a: put(B, np.asarray(a, np.uint32))
+    free, n_free = u32(*rng.permutation(pages)), u32(pages)
+    work = []
+
+    def forward(tokens, table, starts, lens, most, groups):
+        M = len(tokens)
+        x = B.index(Wd["embed"], 0, B.from_numpy(np.uint32(tokens)))
+        for L, (kp, vp) in zip(Wd["layers"], pools):
+            y = B.reshape(B.linear(B.fused_rmsnorm(x, L["n"], 1e-6), L["qkv"]), (M, nh + 2 * nkv, d))
+            q, k, v = B.slice(y, 1, 0, nh), B.slice(y, 1, nh, nkv), B.slice(y, 1, nh + nkv, nkv)
+            q = B.paged_append(k, v, kp, vp, table, starts, lens, q=q, cos=cos_t, sin=sin_t, q_gain=L["qg"], k_gain=L["kg"], eps=1e-6)
+            if groups is None:
+                o = B.paged_attention(q, kp, vp, table, starts, lens, max_new=most)
+            else:
+                room = B.paged_shared_work(q, kp, table, groups[0], max_new=most, max_shared=len(system))
+                work.append(room.shape[0])
+                o = B.paged_shared_attention(q, kp, vp, table, starts, lens, *groups, room, max_new=most, max_shared=len(system))
+            x = B.add(x, B.linear(B.reshape(o, (M, nh * d)), L["o"]))
+        return B.linear(x, Wd["head"])
+
+    # the system prompt, once
+    one_table, one = u32(*([0] * cols))[0], {n: u32(v) for n, v in dict(lens=0, new=len(system), held=0).items()}
+    one_table = B.reshape(one_table, (1, cols))
+    starts1 = u32(0, 0)
+    B.paged_assign(one["lens"][0], one["new"][0], page, one["held"][0], one_table, free[0], n_free[0], starts1[0])
+    forward(system, one_table, starts1[0], one["lens"][0], len(system), None)
+    prefix = B.to_numpy(one_table)[0, :2]
+    assert back(B, one["held"][1]).tolist() == [2] and back(B, n_free[1]).tolist() == [pages - 2]
+    # the requests, each with the prefix's pages in front
+    table = np.zeros((R, cols), np.uint32)
+    table[:, :2] = prefix
+    table, first, held, lens = put(B, table), u32(*[2] * R), u32(*[2] * R), u32(*[len(system)] * R)
+    starts, slots = u32(*[0] * (R + 1)), u32(*[0] * 256)
+    groups = u32(0, R)[0], u32(len(system))[0]
+    texts, made = [list(system) + list(p) for p in prompts], [0] * R
+    goal, stood, near_any = 9, 0, 0
+    feed = [list(p) for p in prompts]
+    for step in range(40):
+        done = [m >= goal for m in made]
+        new = u32(*[0 if f else len(x) for f, x in zip(done, feed)])
+        B.paged_assign(lens[0], new[0], page, held[0], table[0], free[0], n_free[0], starts[0], done=u32(*[int(f) for f in done])[0], first=first[0], slots=slots[0])
+        at = back(B, starts[1])
+        active = [x if not f else [] for f, x in zip(done, feed)]
+        assert at.tolist() == np.concatenate([[0], np.cumsum([len(x) for x in active])]).tolist()
+        if all(done):
+            break
+        tokens = [t for x in active for t in x]
+        slot, tab = back(B, slots[1]), back(B, table[1])
+        for r, x in enumerate(active):
+            end = int(back(B, lens[1])[r])
+            assert slot[at[r]:at[r + 1]].tolist() == [tab[r, p // page] * page + p % page for p in range(end - len(x), end)]
+        logits = forward(tokens, table[0], starts[0], lens[0], max(len(x) for x in active), groups)
+        # a prompt's last token is drawn from, drafts are judged
+        if step == 0:
+            places = [int(at[r + 1]) - 1 for r in range(R)]
+            logits, counts, judged = B.index(logits, 0, B.from_numpy(np.uint32(places))), [1] * R, [x[-1] for x in feed]
+        else:
+            counts, judged = [len(x) for x in active], tokens
+        V = np.concatenate([[0], np.cumsum(counts)])
+        uniform = np.minimum(rng.random(V[-1]).astype(np.float32), np.float32(1 - 2.0 ** -24))
+        before = back(B, lens[1]).copy()
+        out = u32(*[0] * R), u32(*[0] * R)
+        B.verify_drafts(logits, B.from_numpy(np.uint32(judged)), put(B, V.astype(np.uint32))[0], put(B, uniform)[0], temperature=put(B, np.full(R, heat, np.float32))[0], lens=lens[0],
+                        max_new=max(counts), out=(out[0][0], out[1][0], lens[0]))
+        accepted, following, after = back(B, out[0][1]), back(B, out[1][1]), back(B, lens[1])
+        # the same from whole sequences
+        plain = np.zeros((V[-1], vocab))
+        for r in range(R):
+            for i in range(counts[r]):
+                whole = texts[r] + ([] if step == 0 else active[r][1:1 + i])
+                plain[V[r] + i] = plain_logits(W, np.array(whole), nh, nkv, d, cos, sin, 0)
+        want, near = plain_verify(plain, None, np.array(judged), V, uniform, np.full(R, heat), before, 1e-3, 1e-3)
+        near_any += len(near)
+        for r in range(R):
+            if counts[r] == 0:
+                continue
+            if r not in near:
+                assert (accepted[r], following[r], after[r]) == want[r], (step, r)
+            a = int(accepted[r])
+            stood += a
+            texts[r] += ([] if step == 0 else active[r][1:1 + a]) + [int(following[r])]
+            made[r] += a + 1
+            assert after[r] == len(texts[r]) - 1
+            # the next drafts: the model's own, some of them wrong
+            ahead, whole = [], list(texts[r])
+            for i in range(int(rng.integers(0, 4))):
+                t = int(np.argmax(plain_logits(W, np.array(whole), nh, nkv, d, cos, sin, 0)))
+                ahead.append(t if rng.random() < 0.7 else int(rng.integers(0, vocab)))
+                whole.append(ahead[-1])
+            feed[r] = [int(following[r])] + ahead
+    assert all(m >= goal for m in made) and stood > 0 and near_any <= 4 and min(work) > 1
+    # all pages but the prefix's are free again, each once
+    B.sync()
+    count = int(back(B, n_free[1])[0])
+    names = back(B, free[1])[:count]
+    assert count == pages - 2 and len(set(names.tolist()) | set(prefix.tolist())) == pages and back(B, held[1]).tolist() == [2] * R
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+def test_captured_serving_steps(store):
+    """The three operators in graphs, captured twice with a workspace each over the same buffers and replayed by turns while lengths, tables and inputs change."""
+    import torch
+    dtype = torch.bfloat16 if store == "bf16" else torch.float32
+    S = torch.cuda.Stream()
+    B = cg.CudaBackend(0, cg.PREC_F32, stream=S.cuda_stream)
+    B.set_option("shared_prefix", 2)
+    R, nh, nkv, d, page, cols, V, k = 6, 8, 2, 64, 16, 24, 3001, 3
+    M = R * k
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    rnd = lambda *s: torch.randn(s, generator=gen, device="cuda").to(dtype)
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    t = dict(q=rnd(M, nh, d), kp=rnd(R * cols, nkv, page, d), vp=rnd(R * cols, nkv, page, d), logits=rnd(M, V) * 3, probs=torch.softmax(rnd(M, V).float(), 1).to(dtype),
+             uniform=torch.rand(M, generator=gen, device="cuda"), heat=torch.ones(R, device="cuda"), tokens=torch.randint(0, V, (M,), generator=gen, device="cuda").int(),
+             lens=torch.full((R,), 200, device="cuda", dtype=torch.int32), new=torch.full((R,), k, device="cuda", dtype=torch.int32), done=ints(*[0] * R),
+             held=torch.full((R,), 13, device="cuda", dtype=torch.int32), table=torch.randperm(R * cols, generator=gen, device="cuda").int().reshape(R, cols).contiguous(),
+             free=torch.arange(R * cols, device="cuda").int(), n_free=ints(9), starts=ints(*[0] * (R + 1)), lens_out=ints(*[0] * R), held_out=ints(*[0] * R), n_free_out=ints(0),
+             positions=ints(*[0] * M), slots=ints(*[0] * M), groups=ints(0, 2, R), shared=ints(170, 128), out=rnd(M, nh, d), accepted=ints(*[0] * R), next=ints(*[0] * R),
+             left=ints(*[0] * R))
+    torch.cuda.synchronize()
+    h = {n: B.from_device(x) for n, x in t.items()}
+    outs = [t[n] for n in ("table", "free", "starts", "lens_out", "held_out", "n_free_out", "positions", "slots", "out", "accepted", "next", "left")]
+
+    def step(work):
+        B.paged_assign(h["lens"], h["new"], page, h["held"], h["table"], h["free"], h["n_free"], h["starts"], done=h["done"], lens_out=h["lens_out"], held_out=h["held_out"],
+                       n_free_out=h["n_free_out"], positions=h["positions"], slots=h["slots"])
+        B.paged_shared_attention(h["q"], h["kp"], h["vp"], h["table"], h["starts"], h["lens_out"], h["groups"], h["shared"], work, max_new=k, max_shared=170, out=h["out"])
+        B.verify_drafts(h["logits"], h["tokens"], h["starts"], h["uniform"], probs=h["probs"], temperature=h["heat"], lens=h["lens_out"], max_new=k,
+                        out=(h["accepted"], h["next"], h["left"]))
+
+    rooms = [B.paged_shared_work(h["q"], h["kp"], h["table"], h["groups"], max_new=k, max_shared=170) for _ in range(3)]
+    B.sync()
+    with torch.cuda.stream(S):
+        step(rooms[2])   # (what is set up on first use)
+    S.synchronize()
+    reserved, graphs = B.bytes_reserved(), []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=S, capture_error_mode="relaxed"):
+            step(rooms[i])
+        graphs.append(g)
+    moved = 0
+    for i in range(6):
+        with torch.cuda.stream(S):
+            t["q"].copy_(rnd(M, nh, d)); t["logits"].copy_(rnd(M, V) * 3)
+            t["uniform"].copy_(torch.rand(M, generator=gen, device="cuda"))
+            t["lens"].fill_(172 + 5 * i); t["held"].fill_((172 + 5 * i + page - 1) // page)
+            t["new"].copy_(torch.randint(0, k + 1, (R,), generator=gen, device="cuda"))
+            t["done"].copy_((torch.arange(R, device="cuda") == i).int())
+            t["heat"].fill_(float(i % 3))
+            before = [x.clone() for x in outs]
+            graphs[i % 2].replay()
+        S.synchronize()
+        replayed = [x.clone() for x in outs]
+        for x, b in zip(outs, before):
+            x.copy_(b)
+        torch.cuda.synchronize()
+        step(rooms[2])
+        B.sync()
+        torch.cuda.synchronize()
+        for x, r in zip(outs, replayed):
+            assert torch.equal(x, r)
+        moved += int(t["starts"][-1])
+    assert moved > 0 and B.bytes_reserved() == reserved
+    B.close()
+
+
+@gpu
+def test_calls_on_two_streams_with_a_workspace_each():
+    """Two contexts, each with its stream, at the same time over the same pages: every call's result is what it is alone."""
+    import torch
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ctx = [cg.CudaBackend(0, cg.PREC_F32, stream=s.cuda_stream) for s in streams]
+    b = Shared([(20, 900)], [1 + r % 3 for r in range(20)], [3 + 9 * r for r in range(20)], 16, seed=1)
+    nh, nkv, d = 8, 2, 128
+    host_side = [b.pool(nkv, d, "bf16", None) for _ in range(2)] + [rounded(b.rng.standard_normal((b.M, nh, d)), "bf16") for _ in range(2)]
+    calls = []
+    for i, B in enumerate(ctx):
+        B.set_option("shared_prefix", 2)
+        k, v, q = (put(B, host_side[j], "bf16") for j in (0, 1, 2 + i))
+        table, starts, lens, groups, shared = (put(B, np.asarray(x, np.uint32)) for x in (b.table, b.starts, b.total, b.groups, b.shared))
+        out = put(B, np.zeros((b.M, nh, d), np.float32), "bf16")
+        work = B.paged_shared_work(q[0], k[0], table[0], groups[0], max_new=3, max_shared=900)
+        keep = (k, v, q, table, starts, lens, groups, shared, out, work)
+        calls.append((lambda B=B, x=keep: B.paged_shared_attention(x[2][0], x[0][0], x[1][0], x[3][0], x[4][0], x[5][0], x[6][0], x[7][0], x[9], max_new=3, max_shared=900, out=x[8][0]), out[1]))
+    alone = []
+    for B, (call, out) in zip(ctx, calls):
+        call()
+        B.sync()
+        alone.append(out.clone())
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for call, out in calls:
+            call()
+    for B in ctx:
+        B.sync()
+    torch.cuda.synchronize()
+    for (call, out), want in zip(calls, alone):
+        assert torch.equal(out, want)
+    for B in ctx:
+        B.close()
+
+
+# ---------------------------------------------------------------- without a device
+
+
+@pytest.fixture(scope="module")
+def host(tmp_path_factory):
+    """The library's entry points with a context and tensors that no device stands behind."""
+    cg.load_library()
+    out = str(tmp_path_factory.mktemp("serving") / "serving_host.so")
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    tests = os.path.join(ROOT, "tests")
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-fPIC", "-shared", "-I", os.path.join(ROOT, "catgrad-rs_b200", "csrc"), "-I", f"{cuda}/include", "-I", tests,
+                           os.path.join(tests, "serving_host.cpp"), "-o", out, cg.library_path(), f"-Wl,-rpath,{os.path.dirname(cg.library_path())}", "-L", f"{cuda}/lib64", "-lcudart"])
+    L = ctypes.CDLL(out)
+    vp, i64, i64p = ctypes.c_void_p, ctypes.c_int64, ctypes.POINTER(ctypes.c_int64)
+    L.host_ctx.restype = vp
+    L.host_tensor.restype, L.host_tensor.argtypes = vp, [vp, ctypes.c_uint64, ctypes.c_int, ctypes.c_int, i64p, i64p]
+    L.host_device.argtypes = [vp, ctypes.c_int]
+    L.host_group_span.argtypes = [vp, vp, i64, i64, ctypes.c_int, i64, vp, vp, i64, i64, i64, vp, vp]
+    L.host_position_of.argtypes, L.host_position_of.restype = [vp, vp, i64, i64, i64, i64], i64
+    return L
+
+
+SHAPE, DTYPE, INVALID, UNSUPPORTED = 1, 2, 3, 8
+
+
+def refused(H, call, cases):
+    for i, (want, kw) in enumerate(cases):
+        assert call(**kw) == want, (i, want, H.lib.cg_last_error(H.ctx))
+
+
+def test_assign_refusals(host):
+    """Every call here is refused before anything is launched."""
+    H = Host(host)
+    u = lambda *d, **k: H.t(*d, store="u32", **k)
+    order = ("lens", "new", "done", "first", "page", "most", "held", "n_free", "free", "table", "starts", "lens_out", "held_out", "n_free_out", "positions", "slots")
+
+    def call(**kw):
+        a = dict(lens=u(5), new=u(5), done=u(5), first=u(5), page=16, most=0, held=u(5), n_free=u(1), free=u(40), table=u(5, 8), starts=u(6), lens_out=u(5), held_out=u(5),
+                 n_free_out=u(1), positions=u(99), slots=u(99))
+        a.update(kw)
+        return H._call(H.lib.cg_paged_assign, [ctypes.c_int64(a[n]) if n in ("page", "most") else a[n] for n in order])
+
+    for name in ("lens", "new", "held", "n_free", "free", "table", "starts", "lens_out", "held_out", "n_free_out"):
+        assert call(**{name: None}) == INVALID, name
+    at = 7 << 44
+    far = u(5)
+    host.host_device(far, 1)
+    refused(H, call, [(SHAPE, {n: u(4)}) for n in ("lens", "new", "done", "first", "held", "starts", "lens_out", "held_out", "n_free", "n_free_out")] +
+            [(SHAPE, dict(table=u(40))), (SHAPE, dict(slots=u(98))), (SHAPE, dict(free=u(5, 8)))] +
+            [(DTYPE, {n: H.t(5)}) for n in ("lens", "new", "done", "first", "held", "lens_out", "held_out")] + [(DTYPE, dict(table=H.t(5, 8))), (DTYPE, dict(free=H.t(40)))] +
+            [(UNSUPPORTED, dict(page=p)) for p in (0, 4, 12, 2048, -16)] + [(INVALID, dict(most=-1)), (UNSUPPORTED, dict(table=u(5, 8, strides=[9, 1]))),
+             (UNSUPPORTED, dict(lens=u(5, strides=[2]))), (INVALID, dict(lens=u(5, at=at), held_out=u(5, at=at))), (INVALID, dict(lens=u(5, at=at), lens_out=u(5, at=at, shift=4))),
+             (INVALID, dict(table=u(5, 8, at=at), slots=u(99, at=at, shift=64))), (INVALID, dict(new=u(5, at=at), starts=u(6, at=at))), (INVALID, dict(done=far))])
+    big = 65536
+    assert call(lens=u(big), new=u(big), done=None, first=None, held=u(big), table=u(big, 8), starts=u(big + 1), lens_out=u(big), held_out=u(big)) == UNSUPPORTED
+
+
+def test_verify_refusals(host):
+    H = Host(host)
+    u, t = (lambda *d, **k: H.t(*d, store="u32", **k)), H.t
+    order = ("logits", "probs", "tokens", "starts", "uniform", "heat", "lens", "most", "accepted", "next", "lens_out")
+
+    def call(**kw):
+        a = dict(logits=t(9, 100), probs=t(9, 100, store="bf16"), tokens=u(9), starts=u(4), uniform=t(9), heat=t(3), lens=u(3), most=4, accepted=u(3), next=u(3), lens_out=u(3))
+        a.update(kw)
+        return H._call(H.lib.cg_verify_drafts, [ctypes.c_int64(a[n]) if n == "most" else a[n] for n in order])
+
+    for name in ("logits", "tokens", "starts", "uniform", "accepted", "next", "lens", "lens_out"):
+        assert call(**{name: None}) == INVALID, name
+    at = 7 << 44
+    far = u(9)
+    host.host_device(far, 1)
+    refused(H, call, [(SHAPE, dict(probs=t(9, 99))), (SHAPE, dict(probs=t(8, 100))), (SHAPE, dict(tokens=u(8))), (SHAPE, dict(uniform=t(8))), (SHAPE, dict(heat=t(4))),
+                      (SHAPE, dict(accepted=u(4))), (SHAPE, dict(next=u(2))), (SHAPE, dict(lens_out=u(4))), (SHAPE, dict(starts=u(0))), (SHAPE, dict(logits=t(900))),
+                      (SHAPE, dict(logits=t(9, 0), probs=None)), (DTYPE, dict(logits=u(9, 100))), (DTYPE, dict(tokens=t(9))), (DTYPE, dict(uniform=t(9, store="bf16"))),
+                      (DTYPE, dict(heat=t(3, store="bf16"))), (DTYPE, dict(lens=t(3))), (INVALID, dict(most=-1)), (UNSUPPORTED, dict(logits=t(9, 100, strides=[200, 2]))),
+                      (UNSUPPORTED, dict(logits=t(9, 100, strides=[99, 1]))), (UNSUPPORTED, dict(probs=t(9, 100, strides=[1, 9]))), (UNSUPPORTED, dict(tokens=u(9, strides=[2]))),
+                      (UNSUPPORTED, dict(logits=t(9, (1 << 19) + 1), probs=None)), (INVALID, dict(accepted=u(3, at=at), next=u(3, at=at, shift=8))),
+                      (INVALID, dict(tokens=u(9, at=at), lens_out=u(3, at=at))), (INVALID, dict(lens=u(3, at=at), lens_out=u(3, at=at, shift=4))), (INVALID, dict(tokens=far))])
+
+
+def test_shared_attention_refusals(host):
+    H = Host(host)
+    u, t = (lambda *d, **k: H.t(*d, store="u32", **k)), (lambda *d, **k: H.t(*d, **{"store": "bf16", **k}))
+    H.lib.cg_set_option.argtypes = [ctypes.c_void_p, ctypes.c_char_p, ctypes.c_int64]
+    assert H.lib.cg_set_option(H.ctx, b"shared_prefix", 2) == 0
+    order = ("q", "k_pages", "v_pages", "table", "starts", "lens", "groups", "shared", "most", "longest", "scale", "window", "cap", "work", "out")
+    work = 10 * 6 * 4 * 66
+
+    def call(**kw):
+        a = dict(q=t(6, 4, 64), k_pages=t(20, 2, 16, 64), v_pages=t(20, 2, 16, 64), table=u(3, 20), starts=u(4), lens=u(3), groups=u(3), shared=u(2), most=2, longest=300, scale=0.0, window=0,
+                 cap=0.0, work=H.t(work), out=t(6, 4, 64))
+        a.update(kw)
+        return H._call(H.lib.cg_paged_shared_attention, [ctypes.c_int64(a[n]) if n in ("most", "longest", "window") else ctypes.c_float(a[n]) if n in ("scale", "cap") else a[n] for n in order])
+
+    for name in ("q", "k_pages", "v_pages", "table", "starts", "lens", "groups", "shared", "work", "out"):
+        assert call(**{name: None}) == INVALID, name
+    at = 7 << 44
+    far = u(3)
+    host.host_device(far, 1)
+    refused(H, call, [(SHAPE, dict(q=t(6, 5, 64), out=t(6, 5, 64))), (SHAPE, dict(shared=u(3))), (SHAPE, dict(groups=u(0))), (SHAPE, dict(groups=u(3, 1))), (SHAPE, dict(work=H.t(100))),
+                      (SHAPE, dict(work=H.t(work, 1))), (SHAPE, dict(starts=u(5))), (DTYPE, dict(groups=t(3))), (DTYPE, dict(work=u(work))), (DTYPE, dict(work=t(work))),
+                      (DTYPE, dict(out=t(6, 4, 64, store="f32"))), (INVALID, dict(most=-1)), (INVALID, dict(longest=-1)), (INVALID, dict(window=-1)), (INVALID, dict(cap=float("nan"))),
+                      (UNSUPPORTED, dict(work=H.t(work, shift=4))), (UNSUPPORTED, dict(work=H.t(work, strides=[2]))), (UNSUPPORTED, dict(q=t(6, 4, 64, strides=[512, 128, 2]))),
+                      (INVALID, dict(work=H.t(work, at=at), out=t(6, 4, 64, at=at))), (INVALID, dict(work=H.t(work, at=at), q=t(6, 4, 64, at=at, shift=64))),
+                      (INVALID, dict(groups=u(3, at=at), out=t(6, 4, 64, at=at))), (INVALID, dict(groups=far))])
+    # the workspace's size is what the call asks for
+    f = H.lib.cg_paged_shared_floats
+    f.restype, f.argtypes = ctypes.c_int64, [ctypes.c_void_p] * 5 + [ctypes.c_int64] * 2
+    size = lambda q=t(6, 4, 64), k=t(20, 2, 16, 64), table=u(3, 20), groups=u(3), most=2, longest=300: f(H.ctx, q, k, table, groups, most, longest)
+    n = size()
+    assert n == 4 * 6 * 4 * 66 and call(work=H.t(n - 1)) == SHAPE     # (3 chunks of 128 keys, and the rows' own)
+    assert size(most=33) == 0 or size(most=33) == n                    # (no row has more than all)
+    assert size(q=t(99, 4, 64), most=33) == 0 and size(groups=u(1)) == 0 and size(q=t(0, 4, 64)) == 0
+    assert [size(q=None), size(k=t(20, 2, 16)), size(q=t(6, 5, 64)), size(longest=-1), size(groups=u(0))] == [-1] * 5
+    assert H.lib.cg_set_option(H.ctx, b"shared_prefix", 0) == 0 and size() == 0
+    assert H.lib.cg_set_option(H.ctx, b"shared_prefix", 1) == 0 and size() == 0 and size(table=u(60, 4000), longest=9000) > 0
+
+
+def test_groups_that_cannot_be_are_not_followed(host):
+    """group_span and position_of, on the CPU: what they let through lies inside the tensors, and a token's row is found among rows without tokens."""
+    rng = np.random.default_rng(0)
+    vp = lambda a: a.ctypes.data_as(ctypes.c_void_p)
+    good = 0
+    for _ in range(4000):
+        rows, cols, lg, M = int(rng.integers(1, 7)), int(rng.integers(1, 5)), 4, int(rng.integers(0, 40))
+        starts = np.concatenate([[0], np.cumsum(rng.integers(0, 8, rows))]).astype(np.uint32)
+        if rng.random() < 0.3:
+            starts[rng.integers(0, rows + 1)] = rng.choice([0, 5, 41, 0xFFFFFFFF])
+        lens = (np.diff(starts.astype(np.int64)) + 50).astype(np.uint32)
+        G = int(rng.integers(1, 4))
+        groups = np.sort(rng.integers(0, rows + 1, G + 1)).astype(np.uint32)
+        if rng.random() < 0.3:
+            groups[rng.integers(0, G + 1)] = rng.choice([0, rows + 1, 0xFFFFFFFF])
+        shared, most = rng.choice([0, 1, 16, 60, cols * 16, cols * 16 + 1, 0xFFFFFFFF], G).astype(np.uint32), int(rng.choice([1, 60, 1 << 40]))
+        for g in range(G):
+            out, err = np.zeros(5, np.int64), np.zeros(1, np.int32)
+            ok = host.host_group_span(vp(starts), vp(lens), rows, cols, lg, M, vp(groups), vp(shared), G, most, g, vp(out), vp(err))
+            a, b, s = int(groups[g]), int(groups[g + 1]), int(shared[g])
+            can = a <= b <= rows and s <= min(most, cols * 16)
+            can = can and int(starts[a]) <= int(starts[b]) <= M
+            assert bool(ok) == can and err[0] == (0 if can else 1)
+            if ok:
+                good += 1
+                assert out.tolist() == [a, b - a, int(starts[a]), int(starts[b]) - int(starts[a]), s]
+                if (np.diff(starts[a:b + 1].astype(np.int64)) >= 0).all():
+                    for r in range(a, b):
+                        for m in range(int(starts[r]), int(starts[r + 1])):
+                            assert host.host_position_of(vp(starts), vp(lens), rows, a, b - a, m) == int(lens[r]) - int(starts[r + 1]) + m
+    assert good > 300
+
+
+def test_joined_parts_are_waited_for_by_what_follows():
+    """The kernels of the rows' own keys begin beside the chunks' and end behind them: each way out of them passes the dependency, so what waits for them
+    waits for the chunks."""
+    csrc = os.path.join(os.path.dirname(cg.__file__), "csrc")
+    for name, kernel, wait in (("paged_fa.cu", "k_paged_fa(const", "dependency();"), ("paged_dec.cu", "k_paged_dec(const", "depend();"), ("paged_attn.cu", "k_paged_attn(Paged", "depend();")):
+        body = open(os.path.join(csrc, name)).read()
+        body = body[body.index(kernel):]
+        body = body[:body.index("\n}\n")]
+        lines = body.split("\n")
+        at = [i for i, x in enumerate(lines) if x.strip().startswith("return;") or "return;" in x]
+        # of a kernel's ways out, those of OWN have the wait in the two lines before; the others are of blocks of chunks, or of all keys
+        for i in at + [len(lines)]:
+            near = " ".join(lines[max(0, i - 3):i + 1])
+            assert wait in near or "group_of_tile" in near or "x0 + x >= n * rep" in near or "MODE != ALL" in " ".join(lines[max(0, i - 5):i]), (name, lines[min(i, len(lines) - 1)])
