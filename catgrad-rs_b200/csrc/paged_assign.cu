@@ -79,17 +79,29 @@ __device__ __forceinline__ void block_sums(const int64_t (&x)[N], int64_t (&befo
 #pragma unroll
     for (int i = 0; i < N; ++i) sm[warp * N + i] = inc[i];
   __syncthreads();
+  // (every warp sums the warps' sums for itself)
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    int64_t lower = 0, sum = 0;
-    for (int w = 0; w < warps; ++w) {
-      const int64_t s = sm[w * N + i];
-      if (w < warp) lower += s;
-      sum += s;
+    const int64_t mine = lane < warps ? sm[lane * N + i] : 0;
+    int64_t sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += y;
     }
-    before[i] = lower + inc[i] - x[i];
-    all[i] = sum;
+    before[i] = __shfl_sync(0xffffffffu, sum - mine, warp) + inc[i] - x[i];
+    all[i] = __shfl_sync(0xffffffffu, sum, 31);
   }
+}
+// The last of the places 0 .. n whose start is at or before i
+__device__ __forceinline__ int row_of(const uint32_t* start, int n, uint32_t i) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (start[mid] <= i) lo = mid;
+    else hi = mid;
+  }
+  return lo;
 }
 
 __global__ void __launch_bounds__(CHUNK) k_paged_assign(AssignArgs a) {
@@ -114,14 +126,15 @@ __global__ void __launch_bounds__(CHUNK) k_paged_assign(AssignArgs a) {
     const int64_t x[3] = {mine.back, mine.runs ? mine.need : 0, mine.runs ? mine.fresh : 0};
     int64_t before[3], all[3];
     block_sums<3>(x, before, all, sums);
-    // ended rows, dealt to the blocks; a warp has its lanes' rows one after the other
-    const bool gives = mine.back > 0 && row % blocks == block;
-    for (uint32_t left = __ballot_sync(0xffffffffu, gives); left; left &= left - 1) {
-      const int l = __ffs(left) - 1;
-      const int64_t r = __shfl_sync(0xffffffffu, row, l), n = __shfl_sync(0xffffffffu, mine.back, l), f = __shfl_sync(0xffffffffu, mine.first, l),
-                    at = __shfl_sync(0xffffffffu, n_free + back + before[0], l);
-      for (int64_t j = lane; j < n; j += 32)
-        if (at + j < a.room) a.free[at + j] = a.table[r * a.cols + f + j];
+    if (all[0] > 0) {
+      // the chunk's pages, dealt to all threads of the cluster
+      s_start[tid] = (uint32_t)min(before[0], (int64_t)0xFFFFFFFF);
+      s_held[tid] = (uint32_t)mine.first;
+      __syncthreads();
+      for (int64_t i = (int64_t)block * threads + tid; i < all[0] && n_free + back + i < a.room; i += (int64_t)blocks * threads) {
+        const int r = row_of(s_start, threads, (uint32_t)i);
+        a.free[n_free + back + i] = a.table[(c * threads + r) * a.cols + s_held[r] + (i - s_start[r])];
+      }
     }
     back += all[0];
     needs += all[1];
@@ -187,13 +200,7 @@ __global__ void __launch_bounds__(CHUNK) k_paged_assign(AssignArgs a) {
     got = chunk(c, mine, &at, &n);
     __syncthreads();
     for (int64_t i = (int64_t)block * threads + tid; i < n; i += (int64_t)blocks * threads) {
-      // the last row that begins at or before the token
-      int lo = 0, hi = threads;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (s_start[mid] <= (uint32_t)i) lo = mid;
-        else hi = mid;
-      }
+      const int lo = row_of(s_start, threads, (uint32_t)i);
       const int64_t row = c * threads + lo, pos = (int64_t)s_len[lo] + (i - s_start[lo]), col = pos >> a.lg, in_page = pos & (((int64_t)1 << a.lg) - 1);
       const int64_t j = col - s_held[lo];
       const bool names = j >= 0 && in_page == 0;
