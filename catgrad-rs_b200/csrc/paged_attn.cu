@@ -494,9 +494,7 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedAttnArgs a) {
   const int64_t m0 = ((int64_t)blockIdx.x * 256 + (threadIdx.x & ~31)) / quads / a.nh, m1 = ((int64_t)blockIdx.x * 256 + (threadIdx.x | 31)) / quads / a.nh;  // tokens of the warp's ends
   int chunks = -1;
   for (int64_t t = m0; t <= m1 && t < a.rows.M; ++t) {
-    int64_t row = 0;
-    for (int64_t r = threadIdx.x & 31; r - (threadIdx.x & 31) < a.rows.rows; r += 32)
-      row += __popc(__ballot_sync(0xffffffffu, r < a.rows.rows && a.rows.starts[r + 1] <= t));
+    const int64_t row = rows_before(a.rows, 0, a.rows.rows, t);
     int64_t tok0, n, len, shared;
     if (row >= a.rows.rows || !row_span(a.rows, row, a.most, &tok0, &n, &len) || t < tok0 || t >= tok0 + n) continue;
     const int64_t group = group_of_row(a.sh.groups, row, &shared);
@@ -596,7 +594,8 @@ int attend(cg_ctx* c, const PagedAttnArgs& a, bool bf16) {
 }
 
 // Into how many chunks shared keys are cut (0: rows read them for themselves, out of L2).  A function of sizes alone, as the workspace's is.
-// Rows of so many tokens that they fill half a tile of 128 queries gain nothing by others' beside them.  Two launches more pay where 32 MB need not be read
+// Rows of so many tokens that they fill half a tile of 128 queries gain nothing by others' beside them, and blocks find their group by walking them (32 at
+// a time, 1 us).  Two launches more pay where 32 MB need not be read
 // again, whatever the type.  Us with chunks / row by row, rows of 1 token and [4]:
 //   12 rows behind  500, 8 key heads of 128, saves  23 MB   10.4  10.1  [12.3  12.9]
 //   40 behind       500, 4 of 128,                  40 MB   13.3  13.2  [18.7  15.4]
@@ -612,7 +611,7 @@ void plan_chunks(const cg_ctx* c, PagedAttnArgs* args, bool bf16) {
   const int64_t rep = a.nh / a.nkv, saved = (a.rows.rows - a.sh.groups.n) * a.sh.groups.most * 2 * a.nkv * a.d * (bf16 ? 2 : 4);
   a.sh.chunks = 0;
   a.sh.chunk = 0;
-  if (a.sh.groups.n == 0 || a.sh.groups.most == 0 || a.most * rep > 64 || c->opt_shared == 0 || (c->opt_shared == 1 && saved < 32 << 20)) return;
+  if (a.sh.groups.n == 0 || a.sh.groups.n > 256 || a.sh.groups.most == 0 || a.most * rep > 64 || c->opt_shared == 0 || (c->opt_shared == 1 && saved < 32 << 20)) return;
   if (bf16) {
     a.sh.chunk = paged_fa_chunk(a);
   } else {

@@ -98,10 +98,25 @@ __device__ __forceinline__ int64_t group_of_row(const PagedGroups& s, int64_t ro
   *shared = 0;
   return -1;
 }
-// Where the queries of a group's rows stand, by a whole warp: the first and the last position (of rows without tokens none).
-__device__ __forceinline__ void group_positions(const PagedRows& p, int64_t row0, int64_t rows, int64_t* first, int64_t* last) {
+// By a whole warp: of the rows row0 .. row0 + rows those that end at or before a packed token (32 places at a time, so that thousands of rows take three
+// loads); row0 + that is the token's row.
+__device__ __forceinline__ int64_t rows_before(const PagedRows& p, int64_t row0, int64_t rows, int64_t token) {
+  const int lane = threadIdx.x & 31;
+  int64_t base = 0, len = rows;
+  while (len > 0) {
+    const int64_t step = (len + 31) / 32, r = base + (lane + 1) * step - 1;
+    const bool before = r < base + len && (int64_t)p.starts[row0 + r + 1] <= token;
+    const int64_t k = __popc(__ballot_sync(0xffffffffu, before)), skip = min(k * step, len);
+    base += skip;
+    len = step == 1 ? 0 : min(len - skip, step - 1);  // (the next probe's row is not before the token)
+  }
+  return base;
+}
+// By a whole warp: where the new tokens of the rows of the packed tokens t0 .. t1 (of rows row0 .. row0 + rows) stand, the first and the last position.
+__device__ __forceinline__ void tile_positions(const PagedRows& p, int64_t row0, int64_t rows, int64_t t0, int64_t t1, int64_t* first, int64_t* last) {
+  const int64_t r0 = rows_before(p, row0, rows, t0), r1 = min(rows_before(p, row0, rows, t1), rows - 1);
   uint32_t lo = 0xffffffffu, hi = 0;
-  for (int64_t i = threadIdx.x & 31; i < rows; i += 32) {
+  for (int64_t i = r0 + (threadIdx.x & 31); i <= r1; i += 32) {
     const uint32_t len = p.lens[row0 + i], n = p.starts[row0 + i + 1] - p.starts[row0 + i];
     if (n > 0 && n <= len) {
       lo = min(lo, len - n);

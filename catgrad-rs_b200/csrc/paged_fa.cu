@@ -352,7 +352,7 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
     const bool mine = r < p.per * p.rep && ti < n;              // (others have what follows in q, or nothing that was loaded)
     int64_t qpos = pos0 + ti, tile_last = min(pos0 + first + p.per - 1, last), tile_first = pos0 + first;
     if (SHARED) {
-      group_positions(p.rows, row, rows, &tile_first, &tile_last);
+      tile_positions(p.rows, row, rows, tok0 + first, tok0 + min(first + p.per, n) - 1, &tile_first, &tile_last);
       qpos = last;
       if (tile_first < last || (p.window > 0 && tile_last >= p.window + lo)) {
         if (mine) qpos = position_of(p.rows, row, rows, tok0 + ti);

@@ -649,6 +649,20 @@ def test_shared_attention_many_queries(always, store, nh, nkv, d):
 
 @gpu
 @pytest.mark.parametrize("store", ["f32", "bf16"])
+@pytest.mark.parametrize("window", [0, 150])
+def test_shared_attention_many_rows(always, store, window):
+    """More rows than are looked up at a time, many of them without tokens; many groups, and more than share."""
+    rng = np.random.default_rng(window)
+    new = [int(x) for x in rng.integers(0, 3, 1500)]
+    check_shared(always, Shared([(1500, 140)], new, [n + 2 for n in new], 32, seed=1), store, 2, 1, 64, window)
+    new = [int(x) for x in rng.integers(0, 2, 150)]
+    floats = check_shared(always, Shared([(2, 64 + g) for g in range(75)], new, [n + 2 for n in new], 32, seed=2), store, 4, 2, 64, window)
+    assert floats > 1
+    assert check_shared(always, Shared([(1, 40)] * 300, [1] * 300, [3] * 300, 8, seed=3), store, 4, 2, 64, window) == 1
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
 @pytest.mark.parametrize("window", [0, 5, 64, 150])
 def test_shared_attention_tokens_inside_the_prefix(always, store, window):
     """New tokens that stand before the prefix's end, rows that end there, and rows shorter than that."""
