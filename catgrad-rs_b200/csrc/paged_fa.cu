@@ -119,8 +119,9 @@ __host__ __device__ constexpr size_t fa_smem() {
 // of tiles 0 and 1.
 //
 // CHUNK: the queries are those of a group of rows, the keys a chunk of what the group has in common (through its first row's table), and
-// the outputs parts that the rows (OWN) join with their own keys'.  A token's position is then its row's, and masks are only looked at
-// where a query stands inside the prefix or a window ends there.
+// the outputs parts that are joined with the rows' own keys' (OWN).  A token's position is then its row's, and masks are only looked at
+// where a query stands inside the prefix or a window ends there.  64 rows, 32 heads and 8 key heads of 128, over 16001 shared keys in chunks of 1280: 2.6 us to the
+// first loads, 2.2 to the first scores, 1.07 per 64 keys where an SM has two blocks, 2 to write the parts (4 in 16-byte pieces).
 template <int D, int NQ, bool CAP, int MODE>
 __global__ void __launch_bounds__(NQ == 2 ? 384 : 256, NQ == 2 || D > 128 ? 1 : 2)
 k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, FaArgs p) {

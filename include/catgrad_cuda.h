@@ -385,7 +385,7 @@ int32_t cg_paged_assign(cg_ctx*, const cg_tensor* lens, const cg_tensor* new_tok
  * at its place (from p, if that is 0 everywhere), behind all drafts from w = p at the last place: the first token at which the sum of w
  * up to and with it is above u times the whole sum (else the last with a w above 0).  A row of one token thus draws from its logits.
  * A temperature of 0 (or less, or NaN) is greedy: a draft stands if it is the first of the largest logits, and that one is next[r].
- *   NaN logits count as -inf, what of q is not above 0 as 0, temperatures beyond 2^+-100 as that.  Where the largest logit is not finite
+ *   NaN logits count as -inf, what of q is not above 0 as 0, temperatures beyond 2^+-100 as that, weights below e^-700 of the largest as 0.  Where the largest logit is not finite
  * nothing stands, and next[r] is 0xFFFFFFFF.  Weights that are drawn from have 64 bits; sums that drafts are judged by are off by
  * some 2^-22.  lens_out[r] = lens[r] less the drafts that do not stand, which so leave the cache (both U32 [rows] or NULL; may be one).
  * max_new: no row has more tokens (0 = not known).  V is at most 2^19; rows of logits and probs may be apart, and begin anywhere.
