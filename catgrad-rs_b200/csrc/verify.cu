@@ -132,7 +132,7 @@ struct Slice {
 // VT: threads.  Of a position a thread has every VT-th vector, U a step; the next step's are on their way while these are judged.
 template <typename T, int VT, int ON_SM>
 __global__ void __launch_bounds__(VT, ON_SM) k_verify_drafts(VerifyArgs a) {
-  constexpr int E = 16 / sizeof(T), W = VT / 32, U = VT * ON_SM < 1024 ? 4 : 16 / E;  // values of a vector, warps, vectors of a step (as registers allow)
+  constexpr int E = 16 / sizeof(T), W = VT / 32, U = 16 / E;  // values of a vector, warps, vectors of a step
   constexpr int SUB = 32 / W;                            // parts of a warp's tokens, of which there are sums
   extern __shared__ __align__(16) uint8_t staging[];  // the drafter's probabilities at a position
   __shared__ double power[16];
@@ -175,11 +175,16 @@ __global__ void __launch_bounds__(VT, ON_SM) k_verify_drafts(VerifyArgs a) {
     T end;
   };
   auto load = [&](Cursor& c) {
+    if ((U - 1) * VT < c.left) {
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      constexpr uint32_t none = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;  // (-inf)
-      c.x[i] = make_uint4(none, none, none, none);
-      if (i * VT < c.left) c.x[i] = __ldg(c.at + i * VT);
+      for (int i = 0; i < U; ++i) c.x[i] = __ldg(c.at + i * VT);
+    } else {
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        constexpr uint32_t none = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;  // (-inf)
+        c.x[i] = make_uint4(none, none, none, none);
+        if (i * VT < c.left) c.x[i] = __ldg(c.at + i * VT);
+      }
     }
     c.at += U * VT;
     c.left -= U * VT;
@@ -362,7 +367,7 @@ __global__ void __launch_bounds__(VT, ON_SM) k_verify_drafts(VerifyArgs a) {
     const float* q32 = (const float*)a.probs + m * a.q_ld + lo;
     const double t64 = (double)top;
     // 32 parts of neighbouring tokens, of which a warp has SUB
-    const int per = ((count + 31) / 32 + 31) & ~31;
+    const int unit = count >= 4096 ? 127 : 31, per = ((count + 31) / 32 + unit) & ~unit;  // (whole batches, of long slices)
     auto part_begin = [&](int i) { return min(i * per, count); };
     const uint32_t draft = pos < n - 1 ? a.tokens[m + 1] : NONE;
     auto weigh = [&](float x) { return exp64(((double)x - t64) * cold, power); };
@@ -399,38 +404,53 @@ __global__ void __launch_bounds__(VT, ON_SM) k_verify_drafts(VerifyArgs a) {
         }
       }
       T x[B];
-      auto load = [&](int j0) {
+      auto load = [&](int b) {
+        if (b + 32 * B <= w1) {
 #pragma unroll
-        for (int i = 0; i < B; ++i) x[i] = j0 + 32 * i < w1 ? values[j0 + 32 * i] : (T)NO_LOGIT;
+          for (int i = 0; i < B; ++i) x[i] = values[b + lane + 32 * i];
+        }
       };
-      load(w0 + lane);
+      int have = w0;  // x are the logits from here on
+      load(w0);
       if (HAS && a.staged) {
         cp_async_wait_group<0>();
         __syncwarp();
       }
       for (int k = warp * SUB; k < warp * SUB + SUB; ++k) {
         double e_all = 0.0, e_left = 0.0, q_left = 0.0;
-        const int v0 = part_begin(k), v1 = part_begin(k + 1);
-        for (int j0 = v0 + lane; j0 < v1; j0 += 32 * B) {
-          // (of the last ones some are the next part's, and read again)
-          float y[B];
-#pragma unroll
-          for (int i = 0; i < B; ++i) y[i] = j0 + 32 * i < v1 ? logit(x[i]) : NO_LOGIT;
-          load(j0 + 32 * B < v1 ? j0 + 32 * B : v1 + lane);
-#pragma unroll
-          for (int i = 0; i < B; ++i) {
-            const double e = weigh(y[i]);
-            e_all += e;
-            if constexpr (HAS) {
-              float q = j0 + 32 * i < v1 ? widen(q_at[j0 + 32 * i]) : 0.f;
-              q = q > 0.f ? q : 0.f;
-              const double p = (double)q;
-              if (e > p * s) {
-                e_left += e;
-                q_left += p;
-              }
+        auto add = [&](float y, float q) {
+          const double e = weigh(y);
+          e_all += e;
+          if constexpr (HAS) {
+            const double p = (double)(q > 0.f ? q : 0.f);
+            if (e > p * s) {
+              e_left += e;
+              q_left += p;
             }
           }
+        };
+        const int v0 = part_begin(k), v1 = part_begin(k + 1);
+        int b = v0;
+        if (have != b) load(b);
+        while (b + 32 * B <= v1) {
+          float y[B], q[B];
+#pragma unroll
+          for (int i = 0; i < B; ++i) {
+            y[i] = logit(x[i]);
+            q[i] = 0.f;
+            if constexpr (HAS) q[i] = widen(q_at[b + lane + 32 * i]);
+          }
+          b += 32 * B;
+          load(b);
+#pragma unroll
+          for (int i = 0; i < B; ++i) add(y[i], q[i]);
+        }
+        have = b;
+        for (; b < v1; b += 32) {
+          const int j = b + lane;
+          float q = 0.f;
+          if constexpr (HAS) q = j < v1 ? widen(q_at[j]) : 0.f;
+          add(j < v1 ? logit(values[j]) : NO_LOGIT, q);
         }
         e_all = warp_sum(e_all);
         if (HAS) {
@@ -561,18 +581,21 @@ int launch_threads(cg_ctx* c, VerifyArgs& a, int blocks) {
 template <typename T>
 int launch(cg_ctx* c, VerifyArgs& a) {
   // Blocks of a row, and their threads and how many run on an SM, us, [the rule's]:
-  //                                                 16 x 512, 1   8 x 512, 1   8 x 512, 2   8 x 256, 3   4 x 256, 3
-  //   1 row x 128256, f32, 4 drafts                 [14.4]        19.2         20           24           41
-  //   3 x 54082, bf16, 1                             11.1         [12.0]                    13.2         18.5
-  //   16 x 50257, f32, 3, greedy                     16           10.9         10.0         [8.0]        10.1
-  //   32 x 256000, bf16, 7, no probabilities         86           73           [48.8]       59           77
-  //   40 x 151936, bf16, 4                           84           59           54           [47.8]       59
-  //   38 x 2736, f32, 3                              46           25           23           13.6         [12.5]
-  // More threads for a row hide the draw's 64-bit chains; more of them than run at a time wait for whole clusters to end.
+  //                                                 16 x 512, 1   8 x 512, 2   8 x 256, 2   8 x 256, 3   4 x 256, 2
+  //   1 row x 128256, f32, 4 drafts                 [14.1]        20           24           24           41
+  //   16 x 50257, f32, 3, greedy                     16           10.0         [7.5]        8.1          10
+  //   25 x 54301, f32, 4                             45           24           [22.0]       25.7         30
+  //   32 x 256000, bf16, 7, no probabilities         86           [45.6]       59           59           77
+  //   40 x 151936, bf16, 4                           84           54           53           [42.9]       59
+  //   38 x 2736, f32, 3                              46           23           13.6         13.6         [11.5]
+  // More threads for a row hide the draw's 64-bit chains, more registers let more of them be under way; more blocks than run at a time wait for whole clusters to
+  // end.
   int blocks = a.V >= 65536 && a.rows * MOST_BLOCKS <= 148 ? MOST_BLOCKS : 8;
   while (blocks > 1 && (a.rows * blocks > 3 * 148 || a.V < 512 * blocks)) blocks /= 2;
-  if (a.rows * blocks <= 74 && a.V >= 2048 * blocks) return launch_threads<T, 512, 1>(c, a, blocks);
-  if (a.rows * blocks > 148 && a.rows * blocks <= 2 * 148 && a.V >= 16384 * blocks) return launch_threads<T, 512, 2>(c, a, blocks);
+  const int64_t all = a.rows * blocks;
+  if (all <= 74 && a.V >= 2048 * blocks) return launch_threads<T, 512, 1>(c, a, blocks);
+  if (all > 148 && all <= 2 * 148 && a.V >= 16384 * blocks) return launch_threads<T, 512, 2>(c, a, blocks);
+  if (all <= 2 * 148) return launch_threads<T, 256, 2>(c, a, blocks);
   return launch_threads<T, 256, 3>(c, a, blocks);
 }
 
