@@ -12,10 +12,10 @@
 // A cluster has a row, its blocks equal slices of the vocabulary.  Positions are judged a few at a time, and none behind the first rejected draft but those of its
 // group; the draw reads the slice again, out of L2, in one pass for the sum of the weights and for what q leaves of them.
 //
-// Bytes do not bound it (40 rows of up to 4 drafts over 151936 tokens, bf16: 41 MB in 47.6 us, 0.13 of the copy rate) but a row's chain: a round of positions is loads,
-// maxima and sums, the cluster's barrier, the verdict, 3 to 5 us; the draw's 64-bit exponentials 9 us at full rate, 18 here, its sums and the search for the
-// token 4 to 7.  Rows of several rounds go on when the others' SMs are idle: the busiest SM issues 1.6 times the mean's instructions.  One row of 4 drafts over
-// 128256, f32: 14 us; 32 rows of 7 over 256000 47.7; greedy, 16 rows of 3 over 50257, f32: 7.9.  First 26, 111, 99 and 19, with exp(), two passes and slices
+// Bytes do not bound it (40 rows of up to 4 drafts over 151936 tokens, bf16: 41 MB in 42 us, 0.15 of the copy rate) but a row's chain: a round of positions is loads,
+// maxima and sums, the cluster's barrier, the verdict, 3 to 5 us; the draw's 64-bit exponentials 9 us at full rate, its sums and the search for the token
+// 4 to 7.  Rows of several rounds go on when the others' SMs are idle: an SM has work for 0.69 of the time, the busiest issues 1.66 times the mean.  One row of 4 drafts over
+// 128256, f32: 14 us; 32 rows of 7 over 256000 45.5; greedy, 16 rows of 3 over 50257, f32: 7.3.  First 26, 111, 99 and 19, with exp(), two passes and slices
 // kept in shared memory for the draw (which takes the room of other rows' blocks).
 #include <algorithm>
 #include <type_traits>
