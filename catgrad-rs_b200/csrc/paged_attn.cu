@@ -609,7 +609,8 @@ int attend(cg_ctx* c, const PagedAttnArgs& a, bool bf16) {
 //   40 behind      1500, 2 of 64, f32,              60 MB   20.0  40.6  [27.1  40.8]
 void plan_chunks(const cg_ctx* c, PagedAttnArgs* args, bool bf16) {
   PagedAttnArgs& a = *args;
-  const int64_t rep = a.nh / a.nkv, saved = (a.rows.rows - a.sh.groups.n) * a.sh.groups.most * 2 * a.nkv * a.d * (bf16 ? 2 : 4);
+  const int64_t rep = a.nh / a.nkv;
+  const double saved = (double)(a.rows.rows - a.sh.groups.n) * (double)a.sh.groups.most * (2. * a.nkv * a.d * (bf16 ? 2 : 4));  // (bytes; wide tables name more than 63 bits hold)
   a.sh.chunks = 0;
   a.sh.chunk = 0;
   if (a.sh.groups.n == 0 || a.sh.groups.n > 256 || a.sh.groups.most == 0 || a.most * rep > 64 || c->opt_shared == 0 || (c->opt_shared == 1 && saved < 32 << 20)) return;

@@ -9,6 +9,7 @@ import ctypes
 import math
 import os
 import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -357,6 +358,14 @@ def test_verify(cuda, store, probs, V, heat):
                                                   ("f32", "f32", 1 << 19, [2]), ("bf16", "bf16", (1 << 19) - 3, [2, 2]), ("bf16", "f32", 32000, [4] * 40)])
 def test_verify_whole_vocabularies(cuda, store, probs, V, counts):
     check_verify(cuda, Drafts(counts, V, seed=V, store=store, probs=probs))
+
+
+@gpu
+@pytest.mark.parametrize("store,probs,V,counts,offset,pad", [("f32", "f32", 131077, [2] * 19, 0, 0), ("bf16", "bf16", 140001, [2, 1] * 13, 3, 5), ("bf16", "none", 131072, [1, 3] * 10, 0, 0),
+                                                             ("f32", "bf16", 20001, [3] * 20, 1, 2), ("f32", "none", 9001, [2] * 50, 0, 3)])
+def test_verify_rows_that_fill_the_device(cuda, store, probs, V, counts, offset, pad):
+    """Rows and vocabularies at which other numbers of threads and blocks are taken."""
+    check_verify(cuda, Drafts(counts, V, seed=V, store=store, probs=probs, heat=[1.0, 0.7, 0.0]), offset=offset, pad=pad)
 
 
 @gpu
@@ -971,6 +980,43 @@ def test_calls_on_two_streams_with_a_workspace_each():
         B.close()
 
 
+@gpu
+def test_recorded_mode(cuda):
+    """What is recorded runs before the calls that read it, and what they write is read by calls that are recorded behind them."""
+    L = cg.CudaBackend(0, cg.PREC_F32)
+    L.set_option("lazy", 1)
+    b = Shared([(6, 200)], [1, 2, 1, 3, 1, 2], [5, 9, 1, 30, 2, 64], 16, seed=8)
+    nh, nkv, d, V = 4, 2, 64, 515
+    pool = [b.pool(nkv, d, "f32", None) for _ in range(2)]
+    q = rounded(b.rng.standard_normal((b.M, nh, d)), "f32")
+    c = Drafts([2, 1, 4], V, seed=1)
+    s = requests(np.random.default_rng(5), 7, 16)
+    results = []
+    for B in (cuda, L):
+        B.set_option("shared_prefix", 2)
+        made = lambda x: B.cast(B.add(B.from_numpy(np.asarray(x, np.float32)), B.from_numpy(np.zeros(np.shape(x), np.float32))), cg.U32)   # (whole numbers, recorded)
+        twice = lambda x: B.add(B.from_numpy(x), B.from_numpy(x))
+        k, v = (put(B, x)[0] for x in pool)
+        table, starts, lens, groups, shared = (made(x) for x in (b.table, b.starts, b.total, b.groups, b.shared))
+        hq = twice(q)
+        work = B.paged_shared_work(hq, k, table, groups, max_new=3, max_shared=200)
+        o = B.paged_shared_attention(hq, k, v, table, starts, lens, groups, shared, work, max_new=3, max_shared=200)
+        results.append([B.to_numpy(B.add(o, o))])
+        got = B.verify_drafts(twice(c.logits), made(c.tokens), made(c.starts), B.mul(B.from_numpy(c.uniform), B.from_numpy(np.ones_like(c.uniform))), probs=twice(c.probs / 2),
+                              temperature=twice(c.heat), lens=made(c.lens))
+        results[-1] += [B.to_numpy(B.cast(x, cg.F32)) for x in got]
+        held, n_free, free = made(s["held"]), made([s["n_free"]]), made(s["free"])
+        tab, st, pos = made(s["table"]), B.zeros((8,), cg.U32), B.zeros((300,), cg.U32)
+        le = made(s["lens"])
+        B.paged_assign(le, made(s["new"]), 16, held, tab, free, n_free, st, done=made(s["done"]), first=made(s["first"]), positions=pos)
+        results[-1] += [B.to_numpy(B.cast(x, cg.F32)) for x in (le, held, n_free, tab, st, pos)]
+        B.set_option("shared_prefix", 1)
+    for x, y in zip(*results):
+        assert np.array_equal(x, y)
+    assert L.lazy_stats()[0] > 0 and np.abs(results[0][0]).max() > 0 and results[0][8][-1] > 0
+    L.close()
+
+
 # ---------------------------------------------------------------- without a device
 
 
@@ -1088,6 +1134,46 @@ def test_shared_attention_refusals(host):
     assert [size(q=None), size(k=t(20, 2, 16)), size(q=t(6, 5, 64)), size(longest=-1), size(groups=u(0))] == [-1] * 5
     assert H.lib.cg_set_option(H.ctx, b"shared_prefix", 0) == 0 and size() == 0
     assert H.lib.cg_set_option(H.ctx, b"shared_prefix", 1) == 0 and size() == 0 and size(table=u(60, 4000), longest=9000) > 0
+
+
+def test_tensors_that_another_context_has_recorded_are_refused(host):
+    """They have no memory yet.  (In a process of its own, since a call that looked for that memory would end it.)"""
+    out = ctypes.CDLL(host._name)._name
+    r = subprocess.run([sys.executable, "-c", f"import sys; sys.path.insert(0, {os.path.dirname(__file__)!r}); import test_serving; test_serving.recorded_elsewhere({out!r})"],
+                       capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
+def recorded_elsewhere(path):
+    L = ctypes.CDLL(path)
+    L.host_ctx.restype = ctypes.c_void_p
+    L.host_tensor.restype, L.host_tensor.argtypes = ctypes.c_void_p, [ctypes.c_void_p, ctypes.c_uint64, ctypes.c_int, ctypes.c_int, ctypes.POINTER(ctypes.c_int64),
+                                                                      ctypes.POINTER(ctypes.c_int64)]
+    H = Host(L)
+    other, lib = ctypes.c_void_p(L.host_ctx()), H.lib
+    assert lib.cg_set_option(other, b"lazy", ctypes.c_int64(1)) == 0
+
+    def waiting(shape, whole):
+        t = ctypes.c_void_p()
+        assert lib.cg_arange(other, ctypes.c_int64(int(np.prod(shape))), ctypes.byref(t)) == 0
+        if not whole:
+            assert lib.cg_cast(other, t, 0, ctypes.byref(t)) == 0
+        assert lib.cg_reshape(other, t, (ctypes.c_int64 * len(shape))(*shape), len(shape), ctypes.byref(t)) == 0
+        return t
+
+    i64, f = ctypes.c_int64, ctypes.c_float
+    calls = [(lib.cg_paged_assign, dict(lens=(5,), new=(5,), done=(5,), first=(5,), page=i64(16), most=i64(0), held=(5,), n_free=(1,), free=(40,), table=(5, 8), starts=(6,), lens_out=(5,),
+                                        held_out=(5,), n_free_out=(1,), positions=(99,), slots=(99,)), ()),
+             (lib.cg_verify_drafts, dict(logits=(9, 100), probs=(9, 100), tokens=(9,), starts=(4,), uniform=(9,), heat=(3,), lens=(3,), most=i64(4), accepted=(3,), next=(3,), lens_out=(3,)),
+              ("logits", "probs", "uniform", "heat")),
+             (lib.cg_paged_shared_attention, dict(q=(6, 4, 64), k=(20, 2, 16, 64), v=(20, 2, 16, 64), table=(3, 20), starts=(4,), lens=(3,), groups=(3,), shared=(2,), most=i64(2),
+                                                  longest=i64(300), scale=f(0), window=i64(0), cap=f(0), work=(9999,), out=(6, 4, 64)), ("q", "k", "v", "work", "out"))]
+    for fn, arguments, floats in calls:
+        for name, shape in arguments.items():
+            if isinstance(shape, tuple):
+                a = [(waiting(x, n not in floats) if n == name else H.t(*x, store="f32" if n in floats else "u32")) if isinstance(x, tuple) else x for n, x in arguments.items()]
+                assert H._call(fn, a) == INVALID, (fn, name)
+                assert b"another context" in lib.cg_last_error(H.ctx), (fn, name)
 
 
 def test_groups_that_cannot_be_are_not_followed(host):
