@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
   } else {
     if constexpr (MODE == OWN) group = group_of_row(a.sh.groups, row, &from);
     if (!row_span(a.rows, row, a.most, &tok0, &n, &len) || x0 >= n * rep) {  // (the same in all blocks of a cluster)
-      if (MODE == OWN) depend();
+      if (MODE == OWN && last_block()) depend();
       return;
     }
   }
@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
       }
     }
   if (slices == 1) {
-    if (MODE == OWN) depend();
+    if (MODE == OWN && last_block()) depend();
     return;
   }
   if (QR == 64 && tid < QR) { ml[0][tid] = red[0][tid]; ml[1][tid] = red[1][tid]; }
@@ -439,7 +439,7 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
     finish(x, c, v, top, sum);
   }
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  if (MODE == OWN) depend();
+  if (MODE == OWN && last_block()) depend();
 }
 
 template <typename T, int D, int QR, int MODE>

@@ -20,8 +20,8 @@ struct SharedParts {
 };
 
 // Which keys of a row a kernel takes: ALL of them; CHUNK: the queries are a group's, the keys a chunk of what its rows have in common; OWN: those behind that.
-// What comes before the launch of the chunks is complete when that lets the next one begin, so OWN waits for nothing until it ends; it does then, so
-// that what waits for it waits for the chunks too.
+// What comes before the launch of the chunks is complete when that lets the next one begin, so OWN waits for nothing until it ends; its last block does then, so
+// that what waits for it waits for the chunks too.  (While all its blocks did, those that ended beside the chunks kept their SMs to themselves: @@.)
 enum KeysOf { ALL, CHUNK, OWN };
 
 struct PagedAttnArgs {
@@ -44,6 +44,7 @@ constexpr CG_HD float tanh_term(int i) {
        : i == 4 ? 0.019582903012633324f : -0.004716253839433193f;
 }
 #ifdef __CUDACC__
+__device__ __forceinline__ bool last_block() { return blockIdx.x + 1 == gridDim.x && blockIdx.y + 1 == gridDim.y && blockIdx.z + 1 == gridDim.z; }
 // A group of rows that a tile belongs to: its first row, rows, first packed token, tokens and shared tokens, and the tile's number in it.
 struct GroupTile {
   int64_t row0, rows, tok0, n, shared, tile;

@@ -83,7 +83,7 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
   int64_t from = 0, group = -1;  // OWN: the first key, the row's group
   if (OWN) group = group_of_row(p.sh.groups, row, &from);
   if (!row_span(p.rows, row, p.most, &tok0, &n, &len) || x0 >= n * rep) {  // (the same in all blocks of a cluster)
-    if (OWN) depend();
+    if (OWN && last_block()) depend();
     return;
   }
   const int64_t pos0 = len - n, i1 = min(n - 1, (int64_t)i_end);
@@ -304,7 +304,7 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
     }
   }
   if (slices == 1) {
-    if (OWN) depend();
+    if (OWN && last_block()) depend();
     return;
   }
 
@@ -351,7 +351,7 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
     }
   }
   cluster_sync_all();
-  if (OWN) depend();
+  if (OWN && last_block()) depend();
 }
 
 template <int D, int ROWS, bool CAP, int MODE>

@@ -171,7 +171,7 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
   const int64_t i0 = qt * NQ * p.per;                            // first token of the first tile
   const int chunk = OWN ? p.sh.chunks : SHARED ? (int)blockIdx.x / p.slices / ((int)gridDim.x / (p.slices * p.sh.chunks)) : 0;
   if (SHARED && chunk * p.sh.chunk >= shared) n = 0;
-  if (OWN && i0 >= n) dependency();
+  if (OWN && i0 >= n && last_block()) dependency();
   if (i0 >= n) return;
   const int64_t pos0 = SHARED ? 0 : len - n;
   const int64_t last = SHARED ? min(shared, (chunk + 1) * p.sh.chunk) - 1 : pos0 + min(n, i0 + NQ * p.per) - 1;  // the last key, position of the last query
@@ -575,7 +575,7 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(NCOLS) : "memory");
   }
   if (p.slices == 1) {
-    if (OWN) dependency();
+    if (OWN && last_block()) dependency();
     return;
   }
   __shared__ float weight[4][NQ * 128];  // of the blocks' outputs of a row
@@ -636,7 +636,7 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
     }
   }
   cluster_sync_all();
-  if (OWN) dependency();
+  if (OWN && last_block()) dependency();
 }
 
 // q as [tokens, heads, d] in boxes of [per tokens, rep heads, 64 components]
