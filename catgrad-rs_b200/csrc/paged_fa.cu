@@ -781,10 +781,14 @@ int paged_fa_own(cg_ctx* c, const PagedAttnArgs& a) {
   if (a.d <= 128) return pick_own<128>(c, a);
   return pick_own<256>(c, a);
 }
-// Keys of a chunk: as many chunks as make a block per SM, or one and a half where two fit (the rows' own keys then begin beside them), in one wave however the
-// tokens are dealt to the groups.
+// Keys of a chunk: as many chunks as make a block per SM, or 1.4 where two fit (the rows' own keys then run beside them), in one wave however the
+// tokens are dealt to the groups.  Us with 1 / 1.25 / 1.4 / 1.5 / 2 on an SM:
+//   64 rows of 1 behind 16001, 8 key heads of 128              55.0  54.0 [53.9] 55.9  59.9
+//   30 of up to 5 in 3 groups behind 4003, 4 of 128            37.0  35.6 [35.2] 35.3  38.5
+//   14 of 5 in 4 groups behind 3588, 8 of 128                  29.4  25.3 [23.8] 23.8  23.1
+//   26 of 1 behind 13661, 4 of 128                             24.7  25.8 [25.9] 25.2  27.1
 int64_t paged_fa_chunk(const PagedAttnArgs& a) {
-  const int64_t slots = a.d <= 128 ? 222 : 148, queries = a.rows.M * (a.nh / a.nkv), tiles = std::max<int64_t>((queries + a.sh.groups.n * 127) / 128, 1) * a.nkv;
+  const int64_t slots = a.d <= 128 ? 204 : 148, queries = a.rows.M * (a.nh / a.nkv), tiles = std::max<int64_t>((queries + a.sh.groups.n * 127) / 128, 1) * a.nkv;
   const int64_t chunks = std::max<int64_t>(slots / tiles, 1), keys = (a.sh.groups.most + chunks - 1) / chunks;
   return std::max<int64_t>((keys + KT - 1) / KT * KT, 2 * KT);
 }
