@@ -2,7 +2,7 @@
 //
 // The query rows of a key head (token x / rep, head x % rep of the group) fill the rows of one mma.sync tile, 8 or
 // 16 at a time, so a key is read once for all of them.  A cluster has a row's keys and a key head; its blocks have equal
-// shares of the keys, a block's four warps every fourth tile of KT keys, each through a ring of its own that TMA fills.
+// shares of the keys, a block's W warps every W-th tile of KT keys, each through a ring of its own that TMA fills.
 //   S [rows, keys] = Q K^T     (Q's fragments stay in registers)
 //   O^T [d, rows] += V^T P^T   (S's accumulators are P^T's fragments; 8 rows fill the 8 columns)
 // What bounds it is the bytes of the cache, and for short contexts the chain tables -> page table -> keys -> product -> joining.
@@ -38,30 +38,33 @@ struct DecArgs {
   SharedParts sh;
 };
 
-// keys of a warp's tile, tiles of its ring
+// Keys of a warp's tile, tiles of its ring, warps.  (Four warps of heads of 256 fill an SM; two blocks of two deal rows of different lengths out more evenly: 14 rows behind
+// 3001 tokens, 4 key heads of 256, window, 40.7 us with four, 38.7 with two, 38.5 with one.  Rows that read all their keys keep four.)
 template <int D>
 __host__ __device__ constexpr int dec_keys() { return D == 64 ? 32 : 16; }
 constexpr int RING = 3;
-template <int D>
-__host__ __device__ constexpr size_t dec_ring() { return (size_t)4 * RING * 2 * dec_keys<D>() * D * 2; }
-template <int D>
-__host__ __device__ constexpr size_t dec_smem() { return 1024 + dec_ring<D>() + 4 * RING * 8; }
+template <int D, int MODE>
+__host__ __device__ constexpr int dec_warps() { return MODE == OWN && D == 256 ? 2 : 4; }
+template <int D, int MODE>
+__host__ __device__ constexpr size_t dec_ring() { return (size_t)dec_warps<D, MODE>() * RING * 2 * dec_keys<D>() * D * 2; }
+template <int D, int MODE>
+__host__ __device__ constexpr size_t dec_smem() { return 1024 + dec_ring<D, MODE>() + dec_warps<D, MODE>() * RING * 8; }
 
 template <int D, int ROWS, bool CAP, int MODE>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(dec_warps<D, MODE>() * 32)
 k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, DecArgs p) {
   constexpr bool OWN = MODE == KeysOf::OWN;
-  constexpr int KT = dec_keys<D>(), SUB = D / 64, NB = ROWS / 8, KS = D / 16, LD = D + 4;
+  constexpr int KT = dec_keys<D>(), SUB = D / 64, NB = ROWS / 8, KS = D / 16, LD = D + 4, W = dec_warps<D, MODE>();
   constexpr uint32_t BOX = KT * 128, TILE = SUB * BOX;  // bytes of 64 components, of a tile
   extern __shared__ uint8_t smem_raw[];
-  __shared__ float red_m[4][ROWS], red_l[4][ROWS], cta_m[ROWS], cta_l[ROWS];
+  __shared__ float red_m[W][ROWS], red_l[W][ROWS], cta_m[ROWS], cta_l[ROWS];
   __shared__ int aborted;
-  static_assert((size_t)4 * ROWS * LD * 4 + (size_t)ROWS * LD * 4 <= dec_ring<D>(), "the warps' outputs lie over the ring");
+  static_assert((size_t)W * ROWS * LD * 4 + (size_t)ROWS * LD * 4 <= dec_ring<D, MODE>(), "the warps' outputs lie over the ring");
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
-  float* red_o = (float*)(smem_raw + (base - raw));       // [4][ROWS][LD]
-  float* part = red_o + 4 * ROWS * LD;                    // [ROWS][LD]
+  float* red_o = (float*)(smem_raw + (base - raw));       // [W][ROWS][LD]
+  float* part = red_o + W * ROWS * LD;                    // [ROWS][LD]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t2 = (lane & 3) * 2;
-  const uint32_t ring = base + warp * (RING * 2 * TILE), bars = base + (uint32_t)dec_ring<D>() + warp * (RING * 8);
+  const uint32_t ring = base + warp * (RING * 2 * TILE), bars = base + (uint32_t)dec_ring<D, MODE>() + warp * (RING * 8);
   if (lane == 0)
     for (int i = 0; i < RING; ++i) mbar_init(bars + 8 * i, 1);
   if (tid == 0) aborted = 0;
@@ -119,10 +122,10 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
   {
     int64_t id[RING + 1];
 #pragma unroll
-    for (int i = 0; i <= RING; ++i) id[i] = ask(t + 4 * i);
+    for (int i = 0; i <= RING; ++i) id[i] = ask(t + W * i);
 #pragma unroll
     for (int i = 0; i < RING; ++i)
-      if (t + 4 * i < end) request(i, place(t + 4 * i, id[i]));
+      if (t + W * i < end) request(i, place(t + W * i, id[i]));
     ahead_id = id[RING];
   }
 
@@ -154,10 +157,10 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
   const int lkey = (lane >> 4) * 8 + (lane & 7), lpiece = (lane >> 3) & 1;
   bool ok = true;
   int it = 0;
-  for (; t < end; t += 4, ++it) {
+  for (; t < end; t += W, ++it) {
     const int stage = it % RING;
-    const int64_t ahead = t + 4 * RING;
-    const int64_t next = ask(ahead + 4);  // (a whole round before it is asked for)
+    const int64_t ahead = t + W * RING;
+    const int64_t next = ask(ahead + W);  // (a whole round before it is asked for)
     ok = __all_sync(0xffffffffu, mbar_wait(bars + 8 * stage, (uint32_t)(it / RING) & 1u, &aborted, p.rows.err));
     if (!ok) break;
     const uint32_t kt = ring + stage * (2 * TILE), vt = kt + TILE;
@@ -257,7 +260,7 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
     ahead_id = next;
   }
   if (!ok) {  // copies on their way are waited for: what lies over the ring is written next
-    for (int i = 0; i < RING && t + 4 * i < end; ++i) mbar_drain(bars + 8 * ((it + i) % RING), (uint32_t)((it + i) / RING) & 1u, p.rows.err);
+    for (int i = 0; i < RING && t + W * i < end; ++i) mbar_drain(bars + 8 * ((it + i) % RING), (uint32_t)((it + i) / RING) & 1u, p.rows.err);
     aborted = 1;
   }
 
@@ -282,13 +285,16 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
     *(float4*)(p.sh.out + at * p.d + c) = v;
     if (c == 0) p.sh.ml[at] = make_float2(top, sum);
   };
-  for (int i = tid; i < ROWS * (D / 4); i += 128) {
+  for (int i = tid; i < ROWS * (D / 4); i += W * 32) {
     const int r = i / (D / 4), c = i % (D / 4) * 4;
-    const float top = fmaxf(fmaxf(red_m[0][r], red_m[1][r]), fmaxf(red_m[2][r], red_m[3][r])), mc = top == -INFINITY ? 0.f : top;
+    float top = red_m[0][r];
+#pragma unroll
+    for (int w = 1; w < W; ++w) top = fmaxf(top, red_m[w][r]);
+    const float mc = top == -INFINITY ? 0.f : top;
     float sum = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float f = fast_exp2(red_m[w][r] - mc);
       const float4 u = *(const float4*)(red_o + (w * ROWS + r) * LD + c);
       sum += red_l[w][r] * f;
@@ -311,7 +317,7 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
   // ---- the blocks' shares: each finishes some of the values ----
   cluster_sync_all();
   const int rows = (int)min((int64_t)ROWS, n * rep - x0);
-  for (int i = tid * slices + slice; i < rows * (D / 4); i += 128 * slices) {
+  for (int i = tid * slices + slice; i < rows * (D / 4); i += W * 32 * slices) {
     const int r = i / (D / 4), c = i % (D / 4) * 4;
     // (four shares on their way at a time)
     float top = -INFINITY, sum = 0.f;
@@ -356,7 +362,8 @@ k_paged_dec(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
 
 template <int D, int ROWS, bool CAP, int MODE>
 int launch(cg_ctx* c, const PagedAttnArgs& a) {
-  constexpr size_t smem = dec_smem<D>();
+  constexpr size_t smem = dec_smem<D, MODE>();
+  constexpr int W = dec_warps<D, MODE>();
   static PerDeviceFlag configured_on;
   bool& configured = configured_on.at(c->core->device);
   if (!configured) {
@@ -396,9 +403,9 @@ int launch(cg_ctx* c, const PagedAttnArgs& a) {
   //   12 x 4, 167, d 256                        7.5 [7.9]  12.7  24.8  47.7
   // (Lengths are on the device, so the table's width stands for them: 32 x 8 rows of 530 with columns for 32768 tokens get 2 shares, 23.4 us.)
   static AtATime known;
-  const int slices = pick_shares([&](int i) { return at_a_time(known, c->core->device, i, k_paged_dec<D, ROWS, CAP, MODE>, 128, smem); }, 16, groups * a.rows.rows, longest,
-                                 4 * dec_keys<D>(), 4., D == 64 ? 0.7 : D == 128 ? 0.75 : 1.25, 0.);
-  CG_CUDA(c, launch_kernel(c, k_paged_dec<D, ROWS, CAP, MODE>, dim3((unsigned)groups, (unsigned)a.rows.rows, (unsigned)slices), dim3(128), smem, slices, mk, mv, p));
+  const int slices = pick_shares([&](int i) { return at_a_time(known, c->core->device, i, k_paged_dec<D, ROWS, CAP, MODE>, W * 32, smem); }, 16, groups * a.rows.rows, longest,
+                                 W * dec_keys<D>(), 4., D == 64 ? 0.7 : D == 128 ? 0.75 : 1.25, 0.);
+  CG_CUDA(c, launch_kernel(c, k_paged_dec<D, ROWS, CAP, MODE>, dim3((unsigned)groups, (unsigned)a.rows.rows, (unsigned)slices), dim3(W * 32), smem, slices, mk, mv, p));
   CG_LAUNCHED(c);
   return CG_OK;
 }

@@ -727,7 +727,7 @@ int pick(cg_ctx* c, const PagedAttnArgs& a) {
 
 // ---- shared keys ----
 
-// (Two tiles of queries that share their keys in a block are no faster here: 64 rows over 16001 keys, heads of 128, 60.5 us with one, 62 with two, and
+// (Two tiles of queries that share their keys in a block are no faster here: 64 rows over 16001 keys, heads of 128, 62 us where one took 60.5, and
 // a group's second tile is often all but empty.)
 int64_t prefix_tiles(const PagedAttnArgs& a) {
   const int64_t tokens = 128 / (a.nh / a.nkv);
