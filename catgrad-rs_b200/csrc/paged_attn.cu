@@ -529,13 +529,13 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedAttnArgs a) {
     v.x *= f0; v.y *= f0; v.z *= f0; v.w *= f0;
 #pragma unroll
     for (int k = 0; k < U; ++k)
-      if (ml[k].y > 0.f) {  // (a part without keys holds anything)
+      if (ml[k].y != 0.f) {  // (a part without keys holds anything; a sum that is no number is one, and all that it is joined with)
         const float f = fast_exp2(ml[k].x - base);
         sum = fmaf(ml[k].y, f, sum);
         v.x = fmaf(o[k].x, f, v.x); v.y = fmaf(o[k].y, f, v.y); v.z = fmaf(o[k].z, f, v.z); v.w = fmaf(o[k].w, f, v.w);
       }
   }
-  const float f = sum > 0.f ? 1.f / sum : 0.f;
+  const float f = sum != 0.f ? 1.f / sum : 0.f;
   T* to = (T*)a.out + vector * a.d + col;
   if constexpr (sizeof(T) == 4) {
     store_as(to, v.x * f); store_as(to + 1, v.y * f); store_as(to + 2, v.z * f); store_as(to + 3, v.w * f);

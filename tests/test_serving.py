@@ -754,6 +754,77 @@ def test_shared_attention_where_it_saves_enough(cuda, store, nh, nkv, d, rows, s
     assert check_shared(cuda, Shared([(2, shared)], [1, 1], [2, 5], 32), store, nh, nkv, d) == 1
 
 
+def sees(b, where, keep=None):
+    """Packed tokens that see cached position `where` of row `keep` (of every row of its group, where that is shared)."""
+    rows = [r for r in range(len(b.new)) if r == keep or (where < min(b.prefix[keep], b.prefix[r]) and group_of(b, r) == group_of(b, keep))]
+    return [int(b.starts[r]) + i for r in rows for i in range(b.new[r]) if b.total[r] - b.new[r] + i >= where]
+
+
+def group_of(b, r):
+    return sum(g <= r for g in b.groups)
+
+
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+@pytest.mark.parametrize("nh,nkv,d", [(4, 2, 64), (8, 2, 128), (4, 2, 256)])
+@pytest.mark.parametrize("new", [[1] * 7, [3, 1, 2, 4, 3, 1, 2]])
+def test_shared_attention_of_what_is_no_number(always, store, nh, nkv, d, new):
+    """NaN and infinities in a query, in a shared key and value, and in a key of the row's own: who sees them gets NaN where cg_paged_attention gives it, and
+    nobody else does.  The others' outputs are within the bound of check_shared of the formula's with and without, so within twice that of each other."""
+    B, rep = always, nh // nkv
+    b = Shared([(4, 700), (3, 300)], new, [5 + 9 * r for r in range(7)], 16, seed=d)
+    k, v = (b.pool(nkv, d, store, None) for _ in range(2))
+    q = rounded(b.rng.standard_normal((b.M, nh, d)) * 1.5, store)
+    table, starts, lens, groups, shared = (put(B, np.asarray(x, np.uint32))[0] for x in (b.table, b.starts, b.total, b.groups, b.shared))
+    most = max(new)
+
+    def outputs(q, k, v):
+        both = []
+        for option in (2, 0):
+            B.set_option("shared_prefix", option)
+            Q, K, V, out = (put(B, x, store) for x in (q, k, v, np.zeros_like(q)))
+            work = B.paged_shared_work(Q[0], K[0], table, groups, max_new=most, max_shared=700)
+            assert (work.shape[0] > 1) == (option == 2)
+            B.paged_shared_attention(Q[0], K[0], V[0], table, starts, lens, groups, shared, work, max_new=most, max_shared=700, out=out[0])
+            both.append(back(B, out[1]))
+        B.set_option("shared_prefix", 2)
+        return both
+
+    clean = outputs(q, k, v)[0]
+    assert np.isfinite(clean).all()
+    size = np.abs(q.astype(np.float64)).sum(2).max() * np.abs(k).max() / math.sqrt(d)
+    near = 2 * np.abs(v).max() * (2 * (d + 6) * F32 * size + 1000 * F32 + (4 * BF16 if store == "bf16" else 0))
+    place = lambda r, p: (b.table[r, p // b.page], slice(None), p % b.page)
+    for what, bad in [("query", np.nan), ("query", np.inf), ("key", np.nan), ("key", np.inf), ("own", np.nan), ("value", np.nan), ("value", np.inf)]:
+        Q, K, V = q.copy(), k.copy(), v.copy()
+        touched = np.zeros((b.M, nh, d), bool)
+        m = int(b.starts[2]) + new[2] - 1
+        if what == "query":
+            Q[m, 1, 7] = bad
+            touched[m, 1] = True
+        elif what == "own":
+            at = b.total[1] - new[1]
+            K[place(1, at)][0, 3] = bad
+            touched[sees(b, at, 1), :rep] = True
+        elif what == "key":
+            K[place(4, 150)][1, 3] = bad
+            touched[sees(b, 150, 4), rep:] = True
+            if bad == np.inf:   # (no number where the query's component is above 0; below it nothing is left of that key)
+                Q[..., 3] = np.abs(Q[..., 3]) + 0.5
+        else:
+            for r in range(4):   # (every row has its own copy of the prefix's begun page)
+                V[place(r, 699)][0, 5] = bad
+            touched[sees(b, 699, 0), :rep, 5] = True
+        assert touched.any() and not touched.all()
+        got, row_by_row = outputs(Q, K, V)
+        # (of infinite values there are infinities or, where a probability has two parts, NaN)
+        none, same = (~np.isfinite(x) if what == "value" else np.isnan(x) for x in (got, row_by_row))
+        assert np.array_equal(none, touched), (what, bad, np.argwhere(none != touched)[:4])
+        assert np.array_equal(none, same), (what, bad)
+        if (what, bad) != ("key", np.inf):
+            assert (np.abs(got - clean)[~touched] <= near).all(), (what, bad)
+
+
 # ---------------------------------------------------------------- all of them together
 
 
