@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(128) k_paged_attn(PagedAttnArgs a) {
         const int64_t x = qpos[q] - k0, y = MODE == CHUNK ? min(x, hi - k0) : x;
         lim[q] = y > GK ? GK : y < -1 ? -1 : (int)y;
         low[q] = a.window > 0 ? (x - a.window >= GK ? GK : x - a.window < -1 ? 0 : (int)(x - a.window) + 1) : 0;
-        if (MODE == OWN) low[q] = max(low[q], (int)min(max(from - k0, (int64_t)0), (int64_t)GK));
+        if (MODE != ALL) low[q] = max(low[q], (int)min(max((MODE == OWN ? from : lo) - k0, (int64_t)0), (int64_t)GK));  // (chunks may begin inside a tile)
       }
 #pragma unroll
       for (int i = 0; i < NT; ++i)

@@ -825,6 +825,20 @@ def test_shared_attention_of_what_is_no_number(always, store, nh, nkv, d, new):
             assert (np.abs(got - clean)[~touched] <= near).all(), (what, bad)
 
 
+@gpu
+@pytest.mark.parametrize("store,offset,rows,nh,nkv,shared", [("f32", None, 8, 32, 8, 2500), ("f32", None, 8, 32, 8, 5000), ("f32", None, 16, 4, 2, 10000), ("bf16", 1, 8, 32, 8, 4000),
+                                                            ("bf16", 1, 8, 32, 8, 8000)])
+@pytest.mark.parametrize("window", [0, 3000])
+def test_shared_attention_chunks_that_begin_inside_a_tile(cuda, store, offset, rows, nh, nkv, shared, window):
+    """Chunks of 192 and 320 keys of heads of 64, of which few queries take 128 at a time: every other one begins in the middle of a tile."""
+    cuda.set_option("shared_prefix", 1 if window == 0 and store == "f32" else 2)
+    try:
+        b = Shared([(rows, shared)], [1] * rows, [2 + r for r in range(rows)], 64, seed=shared)
+        assert check_shared(cuda, b, store, nh, nkv, 64, window=window, offset=offset) > 2 * b.M * nh * 66
+    finally:
+        cuda.set_option("shared_prefix", 1)
+
+
 # ---------------------------------------------------------------- all of them together
 
 
