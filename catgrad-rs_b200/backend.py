@@ -516,7 +516,7 @@ class CudaBackend(TraitBackend):
         return out
 
     def paged_shared_work(self, q, k_pages, table, groups, max_new=0, max_shared=0):
-        """Room for the parts of paged_shared_attention calls of these sizes, kept by the caller (cg_paged_shared_floats)."""
+        """Room for the parts of paged_shared_attention calls of these sizes and smaller ones, kept by the caller (cg_paged_shared_floats)."""
         n = self._lib.cg_paged_shared_floats(self._ctx, q._h, k_pages._h, table._h, groups._h, max_new, max_shared)
         if n < 0:
             raise BackendPanic(1, "Shape mismatch in operation: shared attention")

@@ -607,22 +607,34 @@ int attend(cg_ctx* c, const PagedAttnArgs& a, bool bf16) {
 //   12 behind      1500, 4 of 256 with a cap,       68 MB   13.8  21.3  [14.4  22.2]
 //   40 behind       500, 2 of 64, f32,              20 MB   19.5  16.6  [19.5  16.8]
 //   40 behind      1500, 2 of 64, f32,              60 MB   20.0  40.6  [27.1  40.8]
+constexpr int SHARED_QUERIES = 64;  // of a row and key head, at most
+bool saves_enough(const cg_ctx* c, const PagedAttnArgs& a, bool bf16) {
+  const double saved = (double)(a.rows.rows - a.sh.groups.n) * (double)a.sh.groups.most * (2. * a.nkv * a.d * (bf16 ? 2 : 4));  // (bytes; wide tables name more than 63 bits hold)
+  return a.sh.groups.n > 0 && a.sh.groups.n <= 256 && a.sh.groups.most > 0 && c->opt_shared != 0 && (c->opt_shared != 1 || saved >= 32 << 20);
+}
+constexpr int ANY_SLOTS = 2 * 148;  // blocks of 64 queries, or 16, in f32: two or four on an SM
 void plan_chunks(const cg_ctx* c, PagedAttnArgs* args, bool bf16) {
   PagedAttnArgs& a = *args;
   const int64_t rep = a.nh / a.nkv;
-  const double saved = (double)(a.rows.rows - a.sh.groups.n) * (double)a.sh.groups.most * (2. * a.nkv * a.d * (bf16 ? 2 : 4));  // (bytes; wide tables name more than 63 bits hold)
   a.sh.chunks = 0;
   a.sh.chunk = 0;
-  if (a.sh.groups.n == 0 || a.sh.groups.n > 256 || a.sh.groups.most == 0 || a.most * rep > 64 || c->opt_shared == 0 || (c->opt_shared == 1 && saved < 32 << 20)) return;
+  if (a.most * rep > SHARED_QUERIES || !saves_enough(c, a, bf16)) return;
   if (bf16) {
     a.sh.chunk = paged_fa_chunk(a);
   } else {
-    // (blocks of 64 queries, or 16: two or four on an SM)
     const int64_t size = a.rows.M * rep <= 32 ? 16 : 64, tiles = std::max((a.rows.M * rep + size - 1) / size, a.sh.groups.n) * a.nkv;
-    const int64_t chunks = std::max<int64_t>(2 * 148 / tiles, 1);
-    a.sh.chunk = std::max<int64_t>(((a.sh.groups.most + chunks - 1) / chunks + 63) / 64 * 64, 128);
+    const int64_t chunks = std::max<int64_t>(ANY_SLOTS / tiles, 1);
+    a.sh.chunk = std::max<int64_t>(((a.sh.groups.most + chunks - 1) / chunks + 63) / 64 * 64, SHARED_CHUNK);
   }
   a.sh.chunks = (int)std::min<int64_t>((a.sh.groups.most + a.sh.chunk - 1) / a.sh.chunk, 0x7FFFFFFF);
+}
+// Parts of a head, at most, of all calls of up to M tokens: fewer tokens are cut into more chunks, so their number times the tokens does not ascend with these.  A chunk
+// has SHARED_CHUNK keys or more, and there are no more chunks than slots / tiles, or one, where tiles of `size` queries are M rep nkv / size or more:
+//   (chunks + 1) M <= min(M most / SHARED_CHUNK, max(M, slots size / nh)) + M
+int64_t most_parts(const PagedAttnArgs& a, bool bf16) {
+  const int64_t slots = bf16 ? paged_fa_slots(a) : ANY_SLOTS, size = bf16 ? 128 : 64, M = a.rows.M;
+  const int64_t chunks = std::min((a.sh.groups.most + SHARED_CHUNK - 1) / SHARED_CHUNK, slots);
+  return std::min(M * chunks, std::max(M, slots * size / a.nh)) + M;
 }
 
 }  // namespace
@@ -661,8 +673,14 @@ extern "C" int64_t cg_paged_shared_floats(cg_ctx* c, const cg_tensor* q, const c
   const int64_t longest = table->dims[1] * k_pages->dims[2];
   a.sh.groups.n = groups->dims[0] - 1;
   a.sh.groups.most = max_shared > 0 ? std::min(max_shared, longest) : longest;
-  plan_chunks(c, &a, q->storage == ST_BF16);
-  return a.sh.chunks ? (a.sh.chunks + 1) * a.rows.M * a.nh * (a.d + 2) : 0;
+  const bool bf16 = q->storage == ST_BF16;
+  const int64_t rep = a.nh / a.nkv;
+  if (a.most * rep > SHARED_QUERIES) {
+    // Rows read for themselves in this step, but not in all smaller ones.  (Where prefixes are always read once, for tests, it is the step's own.)
+    if (c->opt_shared != 1) return 0;
+    a.rows.M = std::min(a.rows.M, a.rows.rows * (SHARED_QUERIES / rep));
+  }
+  return a.rows.M > 0 && saves_enough(c, a, bf16) ? most_parts(a, bf16) * a.nh * (a.d + 2) : 0;
 }
 
 extern "C" int32_t cg_paged_shared_attention(cg_ctx* c, const cg_tensor* q, const cg_tensor* k_pages, const cg_tensor* v_pages, const cg_tensor* table,

@@ -161,6 +161,8 @@ bool paged_fa_prefix_supported(const PagedAttnArgs& a);
 int paged_fa_prefix(cg_ctx* c, const PagedAttnArgs& a);  // the chunks of shared keys
 int paged_fa_own(cg_ctx* c, const PagedAttnArgs& a);     // the rows' own keys
 int64_t paged_fa_chunk(const PagedAttnArgs& a);
+int64_t paged_fa_slots(const PagedAttnArgs& a);          // blocks that chunks are cut for
+constexpr int SHARED_CHUNK = 128;                        // keys of a chunk, at least
 // A few tokens per row, bf16 (paged_dec.cu)
 bool paged_dec_supported(const PagedAttnArgs& a);
 int paged_dec(cg_ctx* c, const PagedAttnArgs& a);

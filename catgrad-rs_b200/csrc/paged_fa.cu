@@ -787,10 +787,11 @@ int paged_fa_own(cg_ctx* c, const PagedAttnArgs& a) {
 //   30 of up to 5 in 3 groups behind 4003, 4 of 128            37.0  35.6 [35.2] 35.3  38.5
 //   14 of 5 in 4 groups behind 3588, 8 of 128                  29.4  25.3 [23.8] 23.8  23.1
 //   26 of 1 behind 13661, 4 of 128                             24.7  25.8 [25.9] 25.2  27.1
+int64_t paged_fa_slots(const PagedAttnArgs& a) { return a.d <= 128 ? 204 : 148; }
 int64_t paged_fa_chunk(const PagedAttnArgs& a) {
-  const int64_t slots = a.d <= 128 ? 204 : 148, queries = a.rows.M * (a.nh / a.nkv), tiles = std::max<int64_t>((queries + a.sh.groups.n * 127) / 128, 1) * a.nkv;
+  const int64_t slots = paged_fa_slots(a), queries = a.rows.M * (a.nh / a.nkv), tiles = std::max<int64_t>((queries + a.sh.groups.n * 127) / 128, 1) * a.nkv;
   const int64_t chunks = std::max<int64_t>(slots / tiles, 1), keys = (a.sh.groups.most + chunks - 1) / chunks;
-  return std::max<int64_t>((keys + KT - 1) / KT * KT, 2 * KT);
+  return std::max<int64_t>((keys + KT - 1) / KT * KT, SHARED_CHUNK);
 }
 
 }  // namespace cg

@@ -173,7 +173,7 @@ int32_t cg_to_vec_u32(cg_ctx*, const cg_tensor* x, uint32_t* dst, int64_t n);
  *   "fa"    : 1 (default) = prefill attention on tcgen05 / TMEM (rows of at least 17 tokens, 64 with distance biases; 2 = the variant
  *             that keeps outputs in registers, for head sizes 64 and 128 without soft-cap); 0 = the mma.sync kernel everywhere
  *   "shared_prefix" : 1 (default) = cg_paged_shared_attention reads what rows have in common once where that saves enough; 2 = always
- *             (tests), 0 = never.  cg_paged_shared_floats follows it
+ *             (tests; rows have few tokens), 0 = never.  cg_paged_shared_floats follows it (at 2 for steps of that kind alone)
  *   "prefill_chunk" : tokens per prefill chunk (default 8192; bounds the decoder's workspace)
  *   "peer"  : 1 (default) = decode steps under tensor parallelism reduce over mapped peer
  *             memory (see cg_comm_peer_exchange); 0 = NCCL collectives.  Set before the first
@@ -327,9 +327,10 @@ int32_t cg_paged_attention(cg_ctx*, const cg_tensor* q, const cg_tensor* k_pages
  * cg_paged_attention's but for the order of sums (in bf16, probabilities of shared tokens have one bf16 part); windows and new tokens may begin
  * inside the prefix, and all of it is read.  max_shared: no group shares more (0 = not known: the table's width); a group that
  * does, or whose numbers cannot be, is left out (CG_ERR_INDEX).  work F32 [n]: room for what is joined at the end, written over, n at
- * least cg_paged_shared_floats of the same tensors and numbers (-1: they do not fit each other); calls that may overlap in time, as
- * captured graphs on two streams, need one each; it begins on a 32-byte boundary.  Where little would be saved, or rows have many new tokens, they read
- * the prefix for themselves (then n may be 0). */
+ * least cg_paged_shared_floats of the same tensors and numbers (-1: they do not fit each other), or of a larger step: what it gives for a step does for all
+ * others over the same table and as many groups that have no more tokens (q no longer, and no longer than rows * max_new) and share no more.  Calls that may
+ * overlap in time, as captured graphs on two streams, need one each; it begins on a 32-byte boundary.  Where little would be saved, or rows have many new
+ * tokens, they read the prefix for themselves (n is 0 if no smaller step would read it once either). */
 int64_t cg_paged_shared_floats(cg_ctx*, const cg_tensor* q, const cg_tensor* k_pages, const cg_tensor* table, const cg_tensor* groups,
                                int64_t max_new, int64_t max_shared);
 int32_t cg_paged_shared_attention(cg_ctx*, const cg_tensor* q, const cg_tensor* k_pages, const cg_tensor* v_pages,

@@ -839,6 +839,42 @@ def test_shared_attention_chunks_that_begin_inside_a_tile(cuda, store, offset, r
         cuda.set_option("shared_prefix", 1)
 
 
+@gpu
+@pytest.mark.parametrize("store,nh,nkv,d", [("f32", 32, 8, 64), ("bf16", 32, 8, 64), ("bf16", 16, 4, 256)])
+def test_one_workspace_for_all_smaller_steps(always, store, nh, nkv, d):
+    """Made for a step in which rows have drafts, used by steps with a token each, with rows that have none, and with shorter prefixes; against the same rows read for
+    themselves.  Both are within the bound of check_shared, which is less than (2 (d + 6) size + t + 24) 2^-24 (and 4 2^-8 in bf16) of the largest value."""
+    import torch
+    B, rows, page, T = always, 40, 64, 3200
+    gen = torch.Generator(device="cuda").manual_seed(d)
+    dtype = torch.float32 if store == "f32" else torch.bfloat16
+    cols = T // page + 1
+    n = T // page + rows
+    pages = [torch.randn(n, nkv, page, d, generator=gen, device="cuda").to(dtype) for _ in range(2)]
+    ids = torch.randperm(n, generator=gen, device="cuda").int()
+    table = torch.cat([ids[:T // page].repeat(rows, 1), ids[T // page:, None]], 1).contiguous()
+    torch.cuda.synchronize()
+    k, v, tab = (B.from_device(x) for x in (*pages, table))
+    u32 = lambda a: put(B, np.asarray(a, np.uint32))[0]
+    q_of = lambda M: torch.randn(M, nh, d, generator=gen, device="cuda").to(dtype)
+    steps = [(4, 40, T), (4, 17, T), (1, 40, T), (4, 40, 1900), (1, 33, T), (1, 32, T), (2, 16, T), (1, 31, T), (1, 9, T), (1, 1, T), (1, 32, 1900), (1, 33, 130)]
+    rooms = [B.paged_shared_work(B.from_device(q_of(each * count)), k, tab, u32([0, rows]), max_new=each, max_shared=T) for each, count in ((4, 40), (1, 33))]
+    for (each, count, shared), room in [(x, rooms[0]) for x in steps] + [(x, rooms[1]) for x in steps[4:]]:
+        new = [each if r < count else 0 for r in range(rows)]
+        M = sum(new)
+        Q = q_of(M)
+        starts, lens = np.concatenate([[0], np.cumsum(new)]), [T + 10 if x else 0 for x in new]
+        outs = [torch.zeros(M, nh, d, device="cuda", dtype=dtype) for _ in range(2)]
+        torch.cuda.synchronize()
+        at, ln, q = u32(starts), u32(lens), B.from_device(Q)
+        B.paged_shared_attention(q, k, v, tab, at, ln, u32([0, rows]), u32([shared]), room, max_new=each, max_shared=shared, out=B.from_device(outs[0]))
+        B.paged_attention(q, k, v, tab, at, ln, max_new=each, out=B.from_device(outs[1]))
+        B.sync()
+        size = float(Q.double().abs().sum(2).max() * pages[0].abs().max()) / math.sqrt(d)
+        near = 2 * float(pages[1].abs().max()) * ((2 * (d + 6) * size + T + 34) * F32 + (4 * BF16 if store == "bf16" else 0))
+        assert float((outs[0].double() - outs[1].double()).abs().max()) <= near, (each, count, shared)
+
+
 # ---------------------------------------------------------------- all of them together
 
 
@@ -1219,6 +1255,28 @@ def test_shared_attention_refusals(host):
     assert [size(q=None), size(k=t(20, 2, 16)), size(q=t(6, 5, 64)), size(longest=-1), size(groups=u(0))] == [-1] * 5
     assert H.lib.cg_set_option(H.ctx, b"shared_prefix", 0) == 0 and size() == 0
     assert H.lib.cg_set_option(H.ctx, b"shared_prefix", 1) == 0 and size() == 0 and size(table=u(60, 4000), longest=9000) > 0
+
+
+def test_shared_attention_room_for_smaller_steps(host):
+    """What cg_paged_shared_floats gives for a step is no less than for any with fewer tokens, fewer of a row or shorter prefixes."""
+    H = Host(host)
+    f = H.lib.cg_paged_shared_floats
+    f.restype, f.argtypes = ctypes.c_int64, [ctypes.c_void_p] * 5 + [ctypes.c_int64] * 2
+    rows, cols = 48, 2000
+    table = H.t(rows, cols, store="u32")
+    for store in ("f32", "bf16"):
+        for nh, nkv, d in [(32, 8, 128), (32, 8, 64), (32, 4, 128), (8, 4, 256), (4, 2, 64), (40, 1, 64), (12, 12, 40)]:
+            k = H.t(9000, nkv, 16, d, store=store)
+            for groups in (1, 3, 11):
+                at = H.t(groups + 1, store="u32")
+                size = lambda M, most, longest: f(H.ctx, H.t(M, nh, d, store=store), k, table, at, most, longest)
+                for longest in (1500, 16001, 0):
+                    # (all steps whose rows have up to `most` tokens and whose q is not padded)
+                    steps = sorted((M, most) for M in (1, 7, 31, 32, 33, 48, 64, 65, 96, 130, 240, 500, 768, 2000) for most in (1, 2, 5, 16, 17, 500) if most <= M <= rows * most)
+                    sizes = [size(M, most, longest) for M, most in steps]
+                    assert sizes == sorted(sizes), (store, nh, d, groups, longest, list(zip(steps, sizes)))
+                    assert sizes[-1] > 0 or longest == 1500
+                assert size(240, 5, 16001) >= size(240, 5, 1500) and size(240, 5, 0) >= size(240, 5, 16001)
 
 
 def test_tensors_that_another_context_has_recorded_are_refused(host):
