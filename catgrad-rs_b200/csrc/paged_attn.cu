@@ -595,7 +595,7 @@ int attend(cg_ctx* c, const PagedAttnArgs& a, bool bf16) {
 }
 
 // Into how many chunks shared keys are cut (0: rows read them for themselves, out of L2).  A function of sizes alone, as the workspace's is.
-// Rows of so many tokens that they fill half a tile of 128 queries gain nothing by others' beside them, and blocks find their group by walking them (32 at
+// Rows of so many tokens that they fill half a tile of 128 queries gain little by others' beside them, and blocks find their group by walking them (32 at
 // a time, 1 us).  Two launches more pay where 32 MB need not be read
 // again, whatever the type.  Us with chunks / row by row, rows of 1 token and [4]:
 //   12 rows behind  500, 8 key heads of 128, saves  23 MB   10.4  10.1  [12.3  12.9]
@@ -607,7 +607,10 @@ int attend(cg_ctx* c, const PagedAttnArgs& a, bool bf16) {
 //   12 behind      1500, 4 of 256 with a cap,       68 MB   13.8  21.3  [14.4  22.2]
 //   40 behind       500, 2 of 64, f32,              20 MB   19.5  16.6  [19.5  16.8]
 //   40 behind      1500, 2 of 64, f32,              60 MB   20.0  40.6  [27.1  40.8]
-constexpr int SHARED_QUERIES = 64;  // of a row and key head, at most
+constexpr int SHARED_QUERIES = 64;  // of a row and key head, at most, in the mean
+// (In the mean: a prompt among rows that run does not keep these from sharing, and takes the chunks' tiles as they do.  64 rows of 1, 8 key heads of 128, and with them one of
+// 100 or 500, behind 500: 45 and 108 us, row by row 62 and 88; behind 4000: 56 and 135, 267 and 312; behind 16000: 120 and 300, 1083 and 1083.)
+int64_t mean_new(const PagedAttnArgs& a) { return std::min(a.most, (a.rows.M + a.rows.rows - 1) / a.rows.rows); }
 bool saves_enough(const cg_ctx* c, const PagedAttnArgs& a, bool bf16) {
   const double saved = (double)(a.rows.rows - a.sh.groups.n) * (double)a.sh.groups.most * (2. * a.nkv * a.d * (bf16 ? 2 : 4));  // (bytes; wide tables name more than 63 bits hold)
   return a.sh.groups.n > 0 && a.sh.groups.n <= 256 && a.sh.groups.most > 0 && c->opt_shared != 0 && (c->opt_shared != 1 || saved >= 32 << 20);
@@ -618,7 +621,7 @@ void plan_chunks(const cg_ctx* c, PagedAttnArgs* args, bool bf16) {
   const int64_t rep = a.nh / a.nkv;
   a.sh.chunks = 0;
   a.sh.chunk = 0;
-  if (a.most * rep > SHARED_QUERIES || !saves_enough(c, a, bf16)) return;
+  if (mean_new(a) * rep > SHARED_QUERIES || !saves_enough(c, a, bf16)) return;
   if (bf16) {
     a.sh.chunk = paged_fa_chunk(a);
   } else {
@@ -668,14 +671,14 @@ extern "C" int64_t cg_paged_shared_floats(cg_ctx* c, const cg_tensor* q, const c
   a.nh = (int)q->dims[1];
   a.nkv = (int)k_pages->dims[1];
   a.d = (int)k_pages->dims[3];
-  if (a.rows.M == 0 || a.nh == 0) return 0;
+  if (a.rows.M == 0 || a.nh == 0 || a.rows.rows == 0) return 0;
   a.most = max_new > 0 ? std::min(max_new, a.rows.M) : a.rows.M;
   const int64_t longest = table->dims[1] * k_pages->dims[2];
   a.sh.groups.n = groups->dims[0] - 1;
   a.sh.groups.most = max_shared > 0 ? std::min(max_shared, longest) : longest;
   const bool bf16 = q->storage == ST_BF16;
   const int64_t rep = a.nh / a.nkv;
-  if (a.most * rep > SHARED_QUERIES) {
+  if (mean_new(a) * rep > SHARED_QUERIES) {
     // Rows read for themselves in this step, but not in all smaller ones.  (Where prefixes are always read once, for tests, it is the step's own.)
     if (c->opt_shared != 1) return 0;
     a.rows.M = std::min(a.rows.M, a.rows.rows * (SHARED_QUERIES / rep));

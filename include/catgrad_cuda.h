@@ -330,7 +330,7 @@ int32_t cg_paged_attention(cg_ctx*, const cg_tensor* q, const cg_tensor* k_pages
  * least cg_paged_shared_floats of the same tensors and numbers (-1: they do not fit each other), or of a larger step: what it gives for a step does for all
  * others over the same table and as many groups that have no more tokens (q no longer, and no longer than rows * max_new) and share no more.  Calls that may
  * overlap in time, as captured graphs on two streams, need one each; it begins on a 32-byte boundary.  Where little would be saved, or rows have many new
- * tokens, they read the prefix for themselves (n is 0 if no smaller step would read it once either). */
+ * tokens in the mean (more than 64 queries of a key head), they read the prefix for themselves (n is 0 if no smaller step would read it once either). */
 int64_t cg_paged_shared_floats(cg_ctx*, const cg_tensor* q, const cg_tensor* k_pages, const cg_tensor* table, const cg_tensor* groups,
                                int64_t max_new, int64_t max_shared);
 int32_t cg_paged_shared_attention(cg_ctx*, const cg_tensor* q, const cg_tensor* k_pages, const cg_tensor* v_pages,

@@ -875,6 +875,39 @@ def test_one_workspace_for_all_smaller_steps(always, store, nh, nkv, d):
         assert float((outs[0].double() - outs[1].double()).abs().max()) <= near, (each, count, shared)
 
 
+def shared_launches(B, store, nh, nkv, d, new, shared, own=100, groups=1, window=0, max_new=None, page=64):
+    """Launches of a call over rows behind one prefix: 3 where it is read once, 1 where rows read it for themselves."""
+    import torch
+    dtype, rows = torch.float32 if store == "f32" else torch.bfloat16, len(new)
+    cols = -(-(shared + max(max(new), own)) // page)
+    pages = [torch.zeros(cols, nkv, page, d, device="cuda", dtype=dtype) for _ in range(2)]
+    q = torch.zeros(sum(new), nh, d, device="cuda", dtype=dtype)
+    torch.cuda.synchronize()
+    u32 = lambda a: put(B, np.asarray(a, np.uint32))[0]
+    at = u32([g * rows // groups for g in range(groups + 1)])
+    h = [B.from_device(x) for x in (q, *pages)] + [u32(x) for x in (np.tile(np.arange(cols), (rows, 1)), np.concatenate([[0], np.cumsum(new)]), [shared + max(n, own) for n in new])]
+    most = max(new) if max_new is None else max_new
+    work, out = B.paged_shared_work(h[0], h[1], h[3], at, max_new=most, max_shared=shared), B.from_device(torch.empty_like(q))
+    B.sync()
+    before = B.launch_count()
+    B.paged_shared_attention(*h, at, u32([shared] * groups), work, max_new=most, max_shared=shared, window=window, out=out)
+    B.sync()
+    return B.launch_count() - before
+
+
+@gpu
+@pytest.mark.parametrize("store,nh,nkv,d", [("bf16", 8, 4, 128), ("bf16", 32, 8, 64), ("f32", 8, 4, 128)])
+def test_shared_attention_with_a_prompt_in_the_batch(cuda, store, nh, nkv, d):
+    """Rows that run share although one of the batch has a prompt, inside its group or outside all, or it is not known how many tokens a row has."""
+    prompt, rows = 40, 24
+    for groups, new in [([(rows + 1, 1500)], [1] * 10 + [prompt] + [1] * (rows - 10)), ([(rows, 1500), (1, None)], [1] * rows + [prompt])]:
+        check_shared(cuda, Shared(groups, new, [n + 2 for n in new], 64, seed=nh), store, nh, nkv, d)
+    check_shared(cuda, Shared([(rows, 1500)], [1] * rows, [3] * rows, 64, seed=nh), store, nh, nkv, d, max_new=0)
+    assert shared_launches(cuda, store, nh, nkv, d, [1] * rows + [prompt], 1500) == 3
+    assert shared_launches(cuda, store, nh, nkv, d, [1] * 64, 1500, max_new=0) == 3
+    assert shared_launches(cuda, store, nh, nkv, d, [1, prompt, 100], 30000) == 1
+
+
 # ---------------------------------------------------------------- all of them together
 
 
