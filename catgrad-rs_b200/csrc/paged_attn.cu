@@ -611,8 +611,14 @@ constexpr int SHARED_QUERIES = 64;  // of a row and key head, at most, in the me
 // (In the mean: a prompt among rows that run does not keep these from sharing, and takes the chunks' tiles as they do.  64 rows of 1, 8 key heads of 128, and with them one of
 // 100 or 500, behind 500: 45 and 108 us, row by row 62 and 88; behind 4000: 56 and 135, 267 and 312; behind 16000: 120 and 300, 1083 and 1083.)
 int64_t mean_new(const PagedAttnArgs& a) { return std::min(a.most, (a.rows.M + a.rows.rows - 1) / a.rows.rows); }
+// Under a window rows read no more than that of the prefix, and the chunks all of it.  Us with chunks / row by row, 4 key heads of 256 [8 of 128], window 512, 1024, 4096:
+//   14 rows behind  3000     21.3  11.4 [17.7   9.8]    21.2  16.0 [17.5  13.4]    20.3  34.6 [17.4  27.5]
+//   14 behind      16000     32.0  17.0 [24.9  15.0]    31.8  22.1 [24.9  18.8]    31.7  50.3 [24.8  40.3]
+//   40 behind      16000     36.7  41.2 [38.8  35.9]    36.5  54.0 [38.8  45.5]    36.0   125 [38.8  98.6]
+//    2 behind      16000     31.0  15.2 [24.0   6.8]    30.9  17.5 [23.6   7.8]    30.2  23.0 [23.6  13.2]
 bool saves_enough(const cg_ctx* c, const PagedAttnArgs& a, bool bf16) {
-  const double saved = (double)(a.rows.rows - a.sh.groups.n) * (double)a.sh.groups.most * (2. * a.nkv * a.d * (bf16 ? 2 : 4));  // (bytes; wide tables name more than 63 bits hold)
+  const double most = (double)a.sh.groups.most, seen = a.window > 0 ? std::min(most, (double)(a.window + mean_new(a) - 1)) : most;
+  const double saved = ((double)a.rows.rows * seen - (double)a.sh.groups.n * most) * (2. * a.nkv * a.d * (bf16 ? 2 : 4));  // (bytes; wide tables name more than 63 bits hold)
   return a.sh.groups.n > 0 && a.sh.groups.n <= 256 && a.sh.groups.most > 0 && c->opt_shared != 0 && (c->opt_shared != 1 || saved >= 32 << 20);
 }
 constexpr int ANY_SLOTS = 2 * 148;  // blocks of 64 queries, or 16, in f32: two or four on an SM

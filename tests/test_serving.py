@@ -908,6 +908,16 @@ def test_shared_attention_with_a_prompt_in_the_batch(cuda, store, nh, nkv, d):
     assert shared_launches(cuda, store, nh, nkv, d, [1, prompt, 100], 30000) == 1
 
 
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+def test_shared_attention_reads_no_more_than_windows_would(cuda, store):
+    """Rows whose windows reach over less than the prefix read it for themselves where that is less than the prefix once."""
+    e = 4 if store == "f32" else 2
+    for rows, shared, window, launches in [(2, 16000, 4096, 1), (14, 16000, 512, 1), (14, 16000, 1024, 1), (14, 16000, 4096, 3), (40, 16000, 1024, 3), (40, 16000, 20000, 3), (14, 16000, 0, 3)]:
+        assert shared_launches(cuda, store, 8, 8 // e * 2, 128, [1] * rows, shared, window=window) == launches, (rows, shared, window)
+    check_shared(cuda, Shared([(3, 5000)], [1, 2, 1], [4, 90, 3], 64, seed=1), store, 4, 2, 128, window=300)
+
+
 # ---------------------------------------------------------------- all of them together
 
 
