@@ -596,30 +596,31 @@ int attend(cg_ctx* c, const PagedAttnArgs& a, bool bf16) {
 
 // Into how many chunks shared keys are cut (0: rows read them for themselves, out of L2).  A function of sizes alone, as the workspace's is.
 // Rows of so many tokens that they fill half a tile of 128 queries gain little by others' beside them, and blocks find their group by walking them (32 at
-// a time, 1 us).  Two launches more pay where 32 MB need not be read
-// again, whatever the type.  Us with chunks / row by row, rows of 1 token and [4]:
-//   12 rows behind  500, 8 key heads of 128, saves  23 MB   10.4  10.1  [12.3  12.9]
-//   40 behind       500, 4 of 128,                  40 MB   13.3  13.2  [18.7  15.4]
-//   12 behind      1500, 4 of 128,                  34 MB   11.8  12.1  [14.1  18.4]
-//   40 behind       500, 8 of 128,                  80 MB   18.9  22.7  [21.7  28.8]
-//   40 behind      5000, 8 of 128,                 799 MB   25.8  119   [34.6  144]
-//    4 behind      5000, 8 of 64,                   31 MB   15.5  10.6  [16.8  13.8]
-//   12 behind      1500, 4 of 256 with a cap,       68 MB   13.8  21.3  [14.4  22.2]
-//   40 behind       500, 2 of 64, f32,              20 MB   19.5  16.6  [19.5  16.8]
-//   40 behind      1500, 2 of 64, f32,              60 MB   20.0  40.6  [27.1  40.8]
+// a time, 1 us).  Two launches more pay where 32 MB need not be read again, whatever the type, and 12 keys for each query, whose parts are written, read and
+// joined.  Us with chunks / row by row, [the rule's], rows of 1, 4 and 8 tokens:
+//   12 rows behind  500, 8 key heads of 128, saves  23 MB    10.1 [10.1]    14.4 [12.9]    15.7 [13.0]
+//   40 behind       500, 4 of 128,                  40 MB    12.8 [13.1]    23.4 [15.4]    29.6 [15.6]
+//   12 behind      1500, 4 of 128,                  34 MB    11.8 [12.1]    15.8 [18.3]    18.2 [18.3]
+//   40 behind       500, 8 of 128,                  80 MB   [15.3] 23.6    [26.5] 29.3     31.7 [26.6]
+//   40 behind      1500, 4 of 128,                 120 MB   [17.3] 26.5    [26.3] 29.8    [33.0] 29.9
+//   40 behind      5000, 8 of 128,                 799 MB   [23.4] 119     [37.6] 142     [60.1] 150
+//    4 behind      5000, 8 of 64,                   31 MB    15.4 [10.4]    16.8 [13.5]    15.7 [20.1]
+//   12 behind      1500, 4 of 256 with a cap,       68 MB   [13.6] 20.7    [15.2] 21.6    [27.4] 29.7
+//   40 behind       500, 2 of 64, f32,              20 MB    18.9 [16.5]    19.4 [16.9]    21.3 [17.0]
+//   40 behind      1500, 2 of 64, f32,              60 MB   [19.9] 42.6    [26.3] 43.0    [32.3] 43.1
 constexpr int SHARED_QUERIES = 64;  // of a row and key head, at most, in the mean
 // (In the mean: a prompt among rows that run does not keep these from sharing, and takes the chunks' tiles as they do.  64 rows of 1, 8 key heads of 128, and with them one of
-// 100 or 500, behind 500: 45 and 108 us, row by row 62 and 88; behind 4000: 56 and 135, 267 and 312; behind 16000: 120 and 300, 1083 and 1083.)
+// 100 or 500, behind 500: [45] and 108 us, row by row 62 and [88]; behind 4000: [56] and [135], 267 and 312; behind 16000: [120] and [300], 1083 and 1083.)
 int64_t mean_new(const PagedAttnArgs& a) { return std::min(a.most, (a.rows.M + a.rows.rows - 1) / a.rows.rows); }
 // Under a window rows read no more than that of the prefix, and the chunks all of it.  Us with chunks / row by row, 4 key heads of 256 [8 of 128], window 512, 1024, 4096:
 //   14 rows behind  3000     21.3  11.4 [17.7   9.8]    21.2  16.0 [17.5  13.4]    20.3  34.6 [17.4  27.5]
 //   14 behind      16000     32.0  17.0 [24.9  15.0]    31.8  22.1 [24.9  18.8]    31.7  50.3 [24.8  40.3]
 //   40 behind      16000     36.7  41.2 [38.8  35.9]    36.5  54.0 [38.8  45.5]    36.0   125 [38.8  98.6]
 //    2 behind      16000     31.0  15.2 [24.0   6.8]    30.9  17.5 [23.6   7.8]    30.2  23.0 [23.6  13.2]
-bool saves_enough(const cg_ctx* c, const PagedAttnArgs& a, bool bf16) {
+bool saves_enough(const cg_ctx* c, const PagedAttnArgs& a, bool bf16, int64_t queries) {
   const double most = (double)a.sh.groups.most, seen = a.window > 0 ? std::min(most, (double)(a.window + mean_new(a) - 1)) : most;
-  const double saved = ((double)a.rows.rows * seen - (double)a.sh.groups.n * most) * (2. * a.nkv * a.d * (bf16 ? 2 : 4));  // (bytes; wide tables name more than 63 bits hold)
-  return a.sh.groups.n > 0 && a.sh.groups.n <= 256 && a.sh.groups.most > 0 && c->opt_shared != 0 && (c->opt_shared != 1 || saved >= 32 << 20);
+  const double keys = (double)a.rows.rows * seen - (double)a.sh.groups.n * most - 12. * (double)queries;  // (wide tables name more bytes than 63 bits hold)
+  return a.sh.groups.n > 0 && a.sh.groups.n <= 256 && a.sh.groups.most > 0 && c->opt_shared != 0 && (c->opt_shared != 1 || keys * (2. * a.nkv * a.d * (bf16 ? 2 : 4)) >= 32 << 20);
 }
 constexpr int ANY_SLOTS = 2 * 148;  // blocks of 64 queries, or 16, in f32: two or four on an SM
 void plan_chunks(const cg_ctx* c, PagedAttnArgs* args, bool bf16) {
@@ -627,7 +628,7 @@ void plan_chunks(const cg_ctx* c, PagedAttnArgs* args, bool bf16) {
   const int64_t rep = a.nh / a.nkv;
   a.sh.chunks = 0;
   a.sh.chunk = 0;
-  if (mean_new(a) * rep > SHARED_QUERIES || !saves_enough(c, a, bf16)) return;
+  if (mean_new(a) * rep > SHARED_QUERIES || !saves_enough(c, a, bf16, a.rows.M * rep)) return;
   if (bf16) {
     a.sh.chunk = paged_fa_chunk(a);
   } else {
@@ -689,7 +690,7 @@ extern "C" int64_t cg_paged_shared_floats(cg_ctx* c, const cg_tensor* q, const c
     if (c->opt_shared != 1) return 0;
     a.rows.M = std::min(a.rows.M, a.rows.rows * (SHARED_QUERIES / rep));
   }
-  return a.rows.M > 0 && saves_enough(c, a, bf16) ? most_parts(a, bf16) * a.nh * (a.d + 2) : 0;
+  return a.rows.M > 0 && saves_enough(c, a, bf16, 0) ? most_parts(a, bf16) * a.nh * (a.d + 2) : 0;
 }
 
 extern "C" int32_t cg_paged_shared_attention(cg_ctx* c, const cg_tensor* q, const cg_tensor* k_pages, const cg_tensor* v_pages, const cg_tensor* table,

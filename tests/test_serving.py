@@ -918,6 +918,13 @@ def test_shared_attention_reads_no_more_than_windows_would(cuda, store):
     check_shared(cuda, Shared([(3, 5000)], [1, 2, 1], [4, 90, 3], 64, seed=1), store, 4, 2, 128, window=300)
 
 
+@gpu
+def test_shared_attention_counts_what_its_parts_cost(cuda):
+    """Rows of several tokens behind a short prefix read it for themselves where the parts of their queries cost more than that: so much the rule has to save."""
+    for nh, nkv, each, shared, launches in [(32, 4, 4, 500, 1), (32, 4, 8, 500, 1), (32, 4, 4, 5000, 3), (32, 8, 4, 500, 3), (32, 8, 8, 500, 1), (32, 8, 1, 500, 3)]:
+        assert shared_launches(cuda, "bf16", nh, nkv, 128, [each] * 40, shared) == launches, (nkv, each, shared)
+
+
 # ---------------------------------------------------------------- all of them together
 
 
