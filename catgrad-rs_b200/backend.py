@@ -563,10 +563,11 @@ class CudaBackend(TraitBackend):
             self._check(st)
 
     def verify_drafts(self, logits, tokens, starts, uniform, probs=None, temperature=None, lens=None, max_new=0, out=None):
-        """(accepted, next, lens without what was rejected) of every row's drafts (cg_verify_drafts); without lens the last is None."""
+        """(accepted, next, lens without what was rejected) of every row's drafts (cg_verify_drafts); without lens the last is None.  Rows without tokens
+        have 0, 0 and their lens, or what is in `out`."""
         if out is None:
             rows = (starts.shape[0] - 1,)
-            out = (self.zeros(rows, U32), self.zeros(rows, U32), None if lens is None else self.zeros(rows, U32))
+            out = (self.zeros(rows, U32), self.zeros(rows, U32), None if lens is None else self.add(lens, self.zeros(rows, U32)))
         a, t, n = out
         st = self._lib.cg_verify_drafts(self._ctx, logits._h, probs and probs._h, tokens._h, starts._h, uniform._h, temperature and temperature._h,
                                         lens and lens._h, max_new, a._h, t._h, n and n._h)

@@ -390,7 +390,8 @@ int32_t cg_paged_assign(cg_ctx*, const cg_tensor* lens, const cg_tensor* new_tok
  * nothing stands, and next[r] is 0xFFFFFFFF.  Weights that are drawn from have 64 bits; sums that drafts are judged by are off by
  * some 2^-22.  lens_out[r] = lens[r] less the drafts that do not stand, which so leave the cache (both U32 [rows] or NULL; may be one).
  * max_new: no row has more tokens (0 = not known).  V is at most 2^19; rows of logits and probs may be apart, and begin anywhere.
- *   A row without tokens is left out, one whose starts, length or drafts cannot be too, and raises CG_ERR_INDEX. */
+ *   A row without tokens is left out, one whose starts, length or drafts cannot be too, and raises CG_ERR_INDEX.  Of these, accepted, next and lens_out
+ * stay as they are: in place the length does; a lens_out of its own begins as a copy of lens. */
 int32_t cg_verify_drafts(cg_ctx*, const cg_tensor* logits, const cg_tensor* probs, const cg_tensor* tokens, const cg_tensor* starts,
                          const cg_tensor* uniform, const cg_tensor* temperature, const cg_tensor* lens, int64_t max_new, cg_tensor* accepted,
                          cg_tensor* next, cg_tensor* lens_out);

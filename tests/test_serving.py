@@ -509,6 +509,28 @@ def test_verify_rows_that_cannot_be(cuda):
         assert what == "starts" or all(g[0] != 77 for g in got)
 
 
+@gpu
+@pytest.mark.parametrize("lazy", [0, 1])
+def test_verify_lengths_of_rows_without_tokens(lazy):
+    """Without an output of its own the call returns all rows' lengths: those of rows that had no tokens are what they were."""
+    B = cg.CudaBackend(0, cg.PREC_F32)
+    B.set_option("lazy", lazy)
+    d = Drafts([2, 0, 3, 0, 1], 300, seed=1)
+    t = [B.from_numpy(np.asarray(x, np.uint32)) for x in (d.tokens, d.starts, d.lens)]
+    lens = B.cast(B.add(B.from_numpy(d.lens.astype(np.float32)), B.from_numpy(np.zeros(5, np.float32))), cg.U32) if lazy else t[2]
+    accepted, following, left = B.verify_drafts(B.from_numpy(d.logits), t[0], t[1], B.from_numpy(d.uniform), probs=B.from_numpy(d.probs), lens=lens)
+    want, near = plain_verify(d.logits, d.probs, d.tokens, d.starts, d.uniform, d.heat, d.lens)
+    assert not near
+    got = [B.to_numpy(x).astype(np.int64) for x in (accepted, following, left)]
+    assert [g[r] for r, w in enumerate(want) if w for g in got] == [x for w in want if w for x in w]
+    assert [got[2][r] for r in (1, 3)] == [d.lens[r] for r in (1, 3)]
+    assert B.to_numpy(lens).tolist() == d.lens.tolist()   # (which stay as they are)
+    # a step in which no row has any
+    none = B.verify_drafts(B.zeros((0, 300), cg.F32), B.zeros((0,), cg.U32), B.zeros((6,), cg.U32), B.zeros((0,), cg.F32), lens=lens)
+    assert B.to_numpy(none[2]).tolist() == d.lens.tolist()
+    B.close()
+
+
 # ---------------------------------------------------------------- attention over shared prefixes
 
 
