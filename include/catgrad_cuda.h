@@ -379,7 +379,7 @@ int32_t cg_paged_assign(cg_ctx*, const cg_tensor* lens, const cg_tensor* new_tok
                         cg_tensor* starts, cg_tensor* lens_out, cg_tensor* held_out, cg_tensor* n_free_out, cg_tensor* positions,
                         cg_tensor* slots);
 /* Verification of drafted tokens (speculative decoding).  Row r has run the packed tokens starts[r] .. starts[r + 1]: its last token, then
- * its drafts; logits [M, V] f32 or bf16 stand behind each, and the draft at place m + 1 is judged at place m, with
+ * its drafts (of a row that has just run its prompt, the caller gives the prompt's last token alone); logits [M, V] f32 or bf16 stand behind each, and the draft at place m + 1 is judged at place m, with
  * p = softmax(logits[m] / temperature[r]) (temperature F32 [rows], NULL: 1) and the drafter's q = probs[m] ([M, V] f32 or bf16; NULL: a draft
  * is its drafter's only token): it stands if uniform[m] q(draft) < p(draft).  accepted[r] drafts stand, up to the first that does not.  next[r]
  * is drawn by the last of the row's numbers u = uniform[starts[r + 1] - 1]: behind a rejected draft from w = max(p - q, 0)

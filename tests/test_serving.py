@@ -1210,6 +1210,66 @@ def test_recorded_mode(cuda):
     L.close()
 
 
+@gpu
+@pytest.mark.parametrize("store,heat", [("f32", 1.0), ("bf16", 0.0)])
+def test_prompts_begin_beside_drafts(cuda, store, heat):
+    """Steps in which some rows run with drafts, one begins with its prompt and one waits for pages: what is judged is gathered from the packed tokens, a prompt's last one of
+    its own.  Against the same steps on the host: lengths lose rejected drafts and nothing else, and what waited begins when pages come back."""
+    B, rows, page, V, cols = cuda, 5, 8, 97, 12
+    rng = np.random.default_rng(3)
+    u32 = lambda a: put(B, np.asarray(a, np.uint32))
+    n_pages = 30
+    lens, held, first, done = np.array([40, 21, 0, 0, 16]), np.array([5, 3, 0, 0, 2]), np.array([0, 0, 0, 0, 2]), np.zeros(rows, int)   # (the last begins behind two shared pages)
+    names = rng.permutation(n_pages)
+    table = np.zeros((rows, cols), np.int64)
+    at = 0
+    for r in range(rows):
+        table[r, :held[r]] = names[at:at + held[r]]
+        at += held[r]
+    stack = np.zeros(n_pages, np.int64)
+    stack[:6] = names[at:at + 6]
+    t = {n: u32(x) for n, x in dict(lens=lens, held=held, table=table, free=stack, n_free=[6], starts=[0] * (rows + 1), first=first).items()}
+    feed = [[5, 6, 7, 8], [9], list(rng.integers(0, V, 11)), list(rng.integers(0, V, 40)), list(rng.integers(0, V, 4))]
+    drafts, began = np.array([3, 0, 0, 0, 0]), [True, True, False, False, False]
+    waited = 0
+    for step in range(4):
+        before, table_before, free_before, left = lens.copy(), table.copy(), stack.copy(), int(back(B, t["n_free"][1])[0])
+        new = np.array([0 if done[r] else len(feed[r]) for r in range(rows)])
+        want = plain_assign(before, new, done, first, held, table_before, free_before, left, page, 1 << 40)
+        B.paged_assign(t["lens"][0], u32(new)[0], page, t["held"][0], t["table"][0], t["free"][0], t["n_free"][0], t["starts"][0], done=u32(done)[0], first=t["first"][0])
+        starts = back(B, t["starts"][1])
+        assert starts.tolist() == want[0]
+        held, table, stack = np.array(want[2]), table_before, free_before
+        places, counts = [], []
+        for r in range(rows):
+            counts.append(min(int(starts[r + 1] - starts[r]), 1 + int(drafts[r])))
+            places += range(starts[r + 1] - counts[r], starts[r + 1])
+        V0 = np.concatenate([[0], np.cumsum(counts)])
+        tokens = np.array([x for r in range(rows) if starts[r + 1] > starts[r] for x in feed[r]], np.uint32)
+        judged = B.index(B.from_numpy(tokens), 0, B.from_numpy(np.uint32(places)))
+        logits = rounded(rng.standard_normal((len(places), V)) * 3, store)
+        uniform = np.minimum(rng.random(len(places)).astype(np.float32), np.float32(1 - 2.0 ** -24))
+        accepted, following, _ = out = *(u32([77] * rows) for _ in range(2)), t["lens"]
+        B.verify_drafts(put(B, logits, store)[0], judged, u32(V0)[0], put(B, uniform)[0], temperature=put(B, np.full(rows, heat, np.float32))[0], lens=t["lens"][0],
+                        max_new=4, out=[x[0] for x in out])
+        verdicts, near = plain_verify(logits, None, tokens[places], V0, uniform, np.full(rows, heat), np.array(want[1]))
+        assert not near
+        B.sync()
+        lens = back(B, t["lens"][1]).astype(np.int64)
+        for r in range(rows):
+            if counts[r] == 0:
+                assert lens[r] == want[1][r]
+                waited += not done[r]
+                continue
+            assert (back(B, accepted[1])[r], back(B, following[1])[r], lens[r]) == verdicts[r]
+            assert lens[r] == before[r] + (int(back(B, accepted[1])[r]) + 1 if began[r] else len(feed[r]))
+            began[r] = True
+            drafts[r] = int(rng.integers(0, 4))
+            feed[r] = [int(back(B, following[1])[r])] + list(rng.integers(0, V, drafts[r]))
+        done[0] = step >= 1   # its pages go to the one that waits
+    assert waited >= 1 and all(began) and done[0]
+
+
 # ---------------------------------------------------------------- without a device
 
 
