@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(VT, ON_SM) k_verify_drafts(VerifyArgs a) {
   __shared__ float w_top[MOST_AHEAD][W];
   __shared__ uint32_t w_at[MOST_AHEAD][W];
   // what the blocks tell each other of positions (two buffers, which take turns), and of what is drawn from
-  __shared__ double told_sum[2][MOST_AHEAD][MOST_BLOCKS], told_rest[3][MOST_BLOCKS];
+  __shared__ double told_sum[2][MOST_AHEAD][MOST_BLOCKS], told_rest[4][MOST_BLOCKS];
   __shared__ uint32_t told_top[2][MOST_AHEAD][MOST_BLOCKS], told_at[2][MOST_AHEAD][MOST_BLOCKS];
   __shared__ double pos_sum[MOST_AHEAD];
   __shared__ float pos_top[MOST_AHEAD];
@@ -376,7 +376,8 @@ __global__ void __launch_bounds__(VT, ON_SM) k_verify_drafts(VerifyArgs a) {
       return q > 0.f ? q : 0.f;
     };
     // One pass for the sum of e, and for what is left once that is known: of the tokens with e > q s, where s is the sum that drafts were judged by,
-    // the sums of e and of q.  (Tokens on the wrong side of that border, 2^-20 of themselves from it, would add as little.)
+    // the sums of e and of q.  (Tokens on the wrong side of that border, 2^-20 of themselves from it, would add as little.)  Where less than 2^-10 of the whole is left
+    // that is too much, as of a drafter that agrees with the target to the last bits, and what is left is summed by itself: 7 us for so rare a row.
     const double s = mode == 2 ? pos_sum[stop] : 0.0;
     auto sums = [&](auto probs) {  // (probs: of which type, or none)
       typedef decltype(probs) Q;
@@ -479,17 +480,38 @@ __global__ void __launch_bounds__(VT, ON_SM) k_verify_drafts(VerifyArgs a) {
     const double b_e = lane < blocks ? told_rest[0][lane] : 0.0, b_left = lane < blocks ? told_rest[1][lane] : 0.0, b_q = lane < blocks ? told_rest[2][lane] : 0.0;
     const double whole = mode == 2 ? warp_sum(b_e) : 0.0;
     double part = mode == 0 ? b_e : mode == 1 ? b_left : fmax(b_left - b_q * whole, 0.0), all = warp_sum(part);
-    if (!(all > 0.0)) {  // nothing is left: from the weights themselves
-      mode = 0;
-      part = b_e;
-      all = warp_sum(part);
-    }
     auto rest = [&](int j) {
       const double e = weigh(logit(values[j]));
       if (mode == 0) return e;
       if (mode == 1) return (uint32_t)(lo + j) == draft ? 0.0 : e;
       return fmax(e - (double)drafter(j) * whole, 0.0);
     };
+    if (mode == 2 && all < 0x1p-10 * whole) {  // (the same in all blocks)
+#pragma unroll 1
+      for (int k = warp * SUB; k < warp * SUB + SUB; ++k) {
+        double left = 0.0;
+#pragma unroll 1
+        for (int j = part_begin(k) + lane; j < part_begin(k + 1); j += 32) left += rest(j);
+        left = warp_sum(left);
+        if (lane == 0) {
+          r_sum[1][k] = left;
+          r_sum[2][k] = 0.0;
+        }
+      }
+      __syncthreads();
+      if (warp == 0) {
+        const double b = warp_sum(r_sum[1][lane]);
+        if (lane < blocks) put_remote(&told_rest[3][block], (uint32_t)lane, b);
+      }
+      cluster_sync_all();
+      part = lane < blocks ? told_rest[3][lane] : 0.0;
+      all = warp_sum(part);
+    }
+    if (!(all > 0.0)) {  // nothing is left: from the weights themselves
+      mode = 0;
+      part = b_e;
+      all = warp_sum(part);
+    }
     // ---- the first token whose inclusive sum is above u times the whole ----
     const double t = (double)u_next * all;
     double before;

@@ -531,6 +531,32 @@ def test_verify_lengths_of_rows_without_tokens(lazy):
     B.close()
 
 
+@gpu
+@pytest.mark.parametrize("V", [700, 20001])
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+def test_verify_drafters_that_agree_with_the_target(cuda, V, store):
+    """The drafter's probabilities are the target's, rounded to f32, but for the draft's, which are twice that: what is left of the target are roundings of some 2^-26 of it.
+    The kernel's weights are within 2^-46 of themselves, so what is left of the sums within 2^-44 / 2^-28 of that, and draws nearer to a border are left out."""
+    rows = 60
+    d = Drafts([2] * rows, V, seed=V, store=store, probs="f32", spread=1.0, peak=False)
+    x = d.logits.astype(np.float64)
+    p = np.exp(x - x.max(1, keepdims=True))
+    p /= p.sum(1, keepdims=True)
+    d.probs = p.astype(np.float32)
+    at = np.arange(0, 2 * rows, 2)
+    d.probs[at, d.tokens[at + 1]] *= 2
+    d.uniform[at] = 0.9
+    rest = np.maximum(p - d.probs, 0.0)[at].sum(1)
+    assert (rest > 2.0 ** -28).all() and (rest < 2.0 ** -20).all()
+    out = [put(cuda, np.zeros(rows, np.uint32)) for _ in range(2)]
+    u32 = lambda a: put(cuda, np.asarray(a, np.uint32))[0]
+    cuda.verify_drafts(put(cuda, d.logits, store)[0], u32(d.tokens), u32(d.starts), put(cuda, d.uniform)[0], probs=put(cuda, d.probs)[0], max_new=2, out=(out[0][0], out[1][0], None))
+    want, near = plain_verify(d.logits, d.probs, d.tokens, d.starts, d.uniform, d.heat, d.lens, drawn=2.0 ** -16)
+    assert len(near) < rows / 3
+    for r in set(range(rows)) - near:
+        assert (back(cuda, out[0][1])[r], back(cuda, out[1][1])[r]) == want[r][:2], r
+
+
 # ---------------------------------------------------------------- attention over shared prefixes
 
 
