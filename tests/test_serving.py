@@ -973,6 +973,34 @@ def test_shared_attention_counts_what_its_parts_cost(cuda):
         assert shared_launches(cuda, "bf16", nh, nkv, 128, [each] * 40, shared) == launches, (nkv, each, shared)
 
 
+@gpu
+@pytest.mark.parametrize("store,nh,nkv,d,most", [("bf16", 8, 2, 128, 1), ("bf16", 8, 2, 128, 5), ("bf16", 4, 2, 256, 1), ("bf16", 8, 2, 64, 2), ("f32", 4, 2, 64, 1), ("f32", 4, 1, 128, 8)])
+def test_shared_attention_joins_what_is_complete(always, store, nh, nkv, d, most):
+    """Calls back to back over a workspace that is filled with NaN before each: the rows' own keys are few and read long before the chunks are, and the last rows, whose
+    blocks leave at once, have no tokens.  Every call's outputs are the same, and the formula's."""
+    import torch
+    B = always
+    rows = 30
+    b = Shared([(rows, 6000)], [1 + r % most if r < rows - 3 else 0 for r in range(rows)], [most + r % 3 for r in range(rows)], 64, seed=d)
+    check_shared(B, b, store, nh, nkv, d, stale=0.0)
+    k, v = (put(B, b.pool(nkv, d, store, 0.0), store) for _ in range(2))
+    q, out = (put(B, rounded(b.rng.standard_normal((b.M, nh, d)), store), store) for _ in range(2))
+    table, starts, lens, groups, shared = (put(B, np.asarray(x, np.uint32))[0] for x in (b.table, b.starts, b.total, b.groups, b.shared))
+    n = B.paged_shared_work(q[0], k[0], table, groups, max_new=most, max_shared=6000).shape[0]
+    room = torch.zeros(n, device="cuda")
+    work, seen = B.from_device(room), []
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.ExternalStream(B.stream)):
+        for _ in range(40):
+            room.fill_(float("nan"))
+            B.paged_shared_attention(q[0], k[0], v[0], table, starts, lens, groups, shared, work, max_new=most, max_shared=6000, out=out[0])
+            seen.append(out[1].clone())
+    B.sync()
+    torch.cuda.synchronize()
+    assert torch.isfinite(seen[0]).all()
+    assert all(torch.equal(x, seen[0]) for x in seen[1:])
+
+
 # ---------------------------------------------------------------- all of them together
 
 
