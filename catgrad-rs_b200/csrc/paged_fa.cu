@@ -14,7 +14,9 @@
 // the largest probability, which is exactly 1 against the exact maximum; the denominator sums the
 // probabilities as bf16 holds them, so that a row that one key decides loses nothing either way.  Probabilities are one bf16 operand: a
 // second part, as the decode form has, would double the second product, which is half of this kernel's work.  Their rounding
-// (2^-9 of each, of either sign) adds to the output's: errors against 64 bits 0.0021 of the result, where the output's alone are 0.0016.
+// (2^-9 of each, of either sign) adds to the output's: errors against 64 bits 0.0021 of the result, where the output's alone are 0.0016.  Those of chunks of shared
+// keys (CHUNK below) have the second part, so that sharing costs no bits: 0.00166, for 57.3 us instead of 54.2 (64 rows of 1 behind 16001), 36.7 instead of 34.3 (30 of up to
+// 5 in 3 groups behind 4003).  The rows' own keys in OWN have one, as these tokens' have in the form of prompts (with two 43.3).
 //
 // Where there are few tiles, or a little more than a whole number of turns, a cluster of 2 or 4 blocks shares a tile's keys; their outputs
 // are joined through shared memory.
@@ -303,6 +305,9 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
 #pragma unroll
         for (int kk = 0; kk < KT / UMMA_K; ++kk)
           umma_ts(o_cols, cols + buf * KT + kk * (UMMA_K / 2), dvs + (((uint32_t)kk * (UMMA_K * 128u)) >> 4), idesc_o, j > 0 || kk > 0 ? 1u : 0u);
+        if (SHARED)  // (the probabilities' second parts, in the other half of the columns)
+#pragma unroll
+          for (int kk = 0; kk < KT / UMMA_K; ++kk) umma_ts(o_cols, cols + buf * KT + KT / 2 + kk * (UMMA_K / 2), dvs + (((uint32_t)kk * (UMMA_K * 128u)) >> 4), idesc_o, 1u);
         umma_commit(b_o);
         umma_commit(b_v_empty + 8 * stage);
       }
@@ -438,18 +443,38 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
       }
       const float mc = m == -INFINITY ? 0.f : m;
       float ls[2] = {0.f, 0.f};
+      // Two probabilities as bf16, and (of shared keys) what their rounding left, in the place of the scores.
+      auto split = [&](uint32_t* pk, int c, int i, float e0, float e1) {
+        pk[i / 2] = pack_bf16(e0, e1);
+        if (SHARED) v[c * 32 + i / 2] = pack_bf16(e0 - __uint_as_float(pk[i / 2] << 16), e1 - __uint_as_float(pk[i / 2] & 0xffff0000u));
+      };
+      // Masked ones are cleared, the sum is made, and all go to TMEM.
+      auto put = [&](uint32_t* pk, int c) {
+        if (CAP && masked)
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const uint32_t seen = (vis[c] >> i & 1u ? 0xffffu : 0u) | (vis[c] >> i & 2u ? 0xffff0000u : 0u);
+            pk[i / 2] &= seen;
+            if (SHARED) v[c * 32 + i / 2] &= seen;
+          }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          ls[0] += __uint_as_float(pk[i] << 16);
+          ls[1] += __uint_as_float(pk[i] & 0xffff0000u);
+          if (SHARED) {
+            ls[0] += __uint_as_float(v[c * 32 + i] << 16);
+            ls[1] += __uint_as_float(v[c * 32 + i] & 0xffff0000u);
+          }
+        }
+        st16(s_addr + (uint32_t)c * 16u, pk);
+        if (SHARED) st16(s_addr + KT / 2 + (uint32_t)c * 16u, v + c * 32);
+      };
       // probabilities of a half of the tile; `exponent` of a score
       auto half = [&](int c, auto exponent) {
         uint32_t pk[16];
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          const float e0 = fast_exp2(exponent(__uint_as_float(v[c * 32 + i]))), e1 = fast_exp2(exponent(__uint_as_float(v[c * 32 + i + 1])));
-          pk[i / 2] = pack_bf16(e0, e1);
-          if (CAP && masked) pk[i / 2] &= (vis[c] >> i & 1u ? 0xffffu : 0u) | (vis[c] >> i & 2u ? 0xffff0000u : 0u);
-          ls[0] += __uint_as_float(pk[i / 2] << 16);
-          ls[1] += __uint_as_float(pk[i / 2] & 0xffff0000u);
-        }
-        st16(s_addr + (uint32_t)c * 16u, pk);
+        for (int i = 0; i < 32; i += 2) split(pk, c, i, fast_exp2(exponent(__uint_as_float(v[c * 32 + i]))), fast_exp2(exponent(__uint_as_float(v[c * 32 + i + 1]))));
+        put(pk, c);
       };
       if (CAP && small) {
         // c tanh(y), |y| <= 3/4, as y times a polynomial of y^2, two scores at a time: one exponential a score instead of two and a
@@ -482,17 +507,9 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
             f = fma(f, y, less);
             float x0, x1;
             asm("mov.b64 {%0, %1}, %2;" : "=f"(x0), "=f"(x1) : "l"(f));
-            pk[i / 2] = pack_bf16(fast_exp2(x0), fast_exp2(x1));
+            split(pk, c, i, fast_exp2(x0), fast_exp2(x1));
           }
-          if (masked)
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) pk[i / 2] &= (vis[c] >> i & 1u ? 0xffffu : 0u) | (vis[c] >> i & 2u ? 0xffff0000u : 0u);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            ls[0] += __uint_as_float(pk[i] << 16);
-            ls[1] += __uint_as_float(pk[i] & 0xffff0000u);
-          }
-          st16(s_addr + (uint32_t)c * 16u, pk);
+          put(pk, c);
         }
       } else
 #pragma unroll

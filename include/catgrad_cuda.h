@@ -324,7 +324,7 @@ int32_t cg_paged_attention(cg_ctx*, const cg_tensor* q, const cg_tensor* k_pages
 /* The same where rows have their first tokens in common, as behind one system prompt or document: these are read once for all rows of a
  * group.  Group g of groups [G + 1] (U32, ascending) has the rows groups[g] .. groups[g + 1], whose first shared[g] (U32 [G]) cached tokens are the
  * same: their tables name the same pages there, or pages that hold the same.  Rows outside all groups share nothing.  Results are
- * cg_paged_attention's but for the order of sums (in bf16, probabilities of shared tokens have one bf16 part); windows and new tokens may begin
+ * cg_paged_attention's but for the order of sums; windows and new tokens may begin
  * inside the prefix, and all of it is read, where it is read once.  max_shared: no group shares more (0 = not known: the table's width); a group that
  * does, or whose numbers cannot be, is left out (CG_ERR_INDEX).  work F32 [n]: room for what is joined at the end, written over, n at
  * least cg_paged_shared_floats of the same tensors and numbers (-1: they do not fit each other), or of a larger step: what it gives for a step does for all

@@ -15,7 +15,7 @@ import numpy as np
 import pytest
 
 from conftest import ROOT, cg
-from test_paged import BF16, F32, Host, attention, back, net, plain_logits, put, rounded
+from test_paged import BF16, F32, PARTS, Host, attention, back, net, off_from_rounded, plain_logits, put, relative, rounded
 
 gpu = pytest.mark.gpu
 INDEX = 6
@@ -999,6 +999,30 @@ def test_shared_attention_joins_what_is_complete(always, store, nh, nkv, d, most
     torch.cuda.synchronize()
     assert torch.isfinite(seen[0]).all()
     assert all(torch.equal(x, seen[0]) for x in seen[1:])
+
+
+@gpu
+@pytest.mark.parametrize("store,nh,nkv,d", [("bf16", 4, 2, 64), ("bf16", 32, 8, 128), ("bf16", 4, 4, 256), ("bf16", 6, 2, 96), ("bf16", 16, 1, 128), ("f32", 4, 2, 64), ("f32", 8, 2, 128), ("f32", 4, 4, 256)])
+@pytest.mark.parametrize("cap,window", [(0.0, 0), (30.0, 1500)])
+def test_shared_attention_of_single_tokens_has_all_parts(always, store, nh, nkv, d, cap, window):
+    """Whether a prefix is read once or by each row does not change how many bits count: the bounds of cg_paged_attention's single tokens (test_paged.py)."""
+    B = always
+    b = Shared([(9, 2000), (4, 900)], [1] * 13, [3 + 25 * r for r in range(13)], 16, seed=d)
+    k, v = (b.pool(nkv, d, store, None) for _ in range(2))
+    q = rounded(b.rng.standard_normal((b.M, nh, d)) * 2.0, store)
+    table, starts, lens, groups, shared = (put(B, np.asarray(x, np.uint32))[0] for x in (b.table, b.starts, b.total, b.groups, b.shared))
+    Q, K, V, out = (put(B, x, store) for x in (q, k, v, np.zeros_like(q)))
+    work = B.paged_shared_work(Q[0], K[0], table, groups, max_new=1, max_shared=2000)
+    B.paged_shared_attention(Q[0], K[0], V[0], table, starts, lens, groups, shared, work, max_new=1, max_shared=2000, softcap=cap, window=window, out=out[0])
+    got, want = back(B, out[1]), np.zeros((b.M, nh, d))
+    for r, t in enumerate(b.total):
+        kk, vv = (b.gather(x, r).astype(np.float64) for x in (k, v))
+        lo = max(0, t - window) if window else 0
+        want[r] = attention(q[r].astype(np.float64), kk[lo:], vv[lo:], t - 1 - lo, 1.0 / math.sqrt(d), 0, cap)[0]
+    if store == "bf16":
+        assert off_from_rounded(got, want) <= 0.02
+    else:
+        assert relative(got, want) <= (2.0 + 1.0) * PARTS
 
 
 # ---------------------------------------------------------------- all of them together
