@@ -581,7 +581,7 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
         for (int i = 0; i < 32; i += 4)
-          *(uint4*)(part + x * LD + c0 + i) = l > 0.f ? make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]) : make_uint4(0u, 0u, 0u, 0u);  // (without tiles nothing was written)
+          *(uint4*)(part + x * LD + c0 + i) = l != 0.f ? make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]) : make_uint4(0u, 0u, 0u, 0u);  // (without tiles nothing was written)
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     }
@@ -612,7 +612,7 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
       sum = fmaf(ls[s], ms[s], sum);
     }
 #pragma unroll
-    for (int s = 0; s < 4; ++s) weight[s][tid] = PART ? ms[s] : sum > 0.f ? ms[s] / sum : 0.f;
+    for (int s = 0; s < 4; ++s) weight[s][tid] = PART ? ms[s] : sum != 0.f ? ms[s] / sum : 0.f;
     if (PART && slice == 0) {
       const int r = tid & 127;
       const int64_t ti = i0 + (tid >> 7) * p.per + r / p.rep;

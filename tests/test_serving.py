@@ -1025,6 +1025,23 @@ def test_shared_attention_of_single_tokens_has_all_parts(always, store, nh, nkv,
         assert relative(got, want) <= (2.0 + 1.0) * PARTS
 
 
+@gpu
+@pytest.mark.parametrize("store", ["f32", "bf16"])
+@pytest.mark.parametrize("nh,nkv,d,new,total", [(4, 2, 64, 100, 3000), (8, 4, 128, 70, 3000), (4, 2, 256, 63, 3000), (4, 2, 64, 1, 5000), (4, 2, 128, 2, 3000)])
+def test_attention_of_a_query_that_is_no_number(cuda, store, nh, nkv, d, new, total):
+    """One row, whose keys are shared out among blocks: NaN comes out of that token's head, and of nothing else."""
+    rng = np.random.default_rng(d)
+    cols = total // 8
+    k, v = (put(cuda, rounded(rng.standard_normal((cols, nkv, 8, d)), store), store) for _ in range(2))
+    q = rounded(rng.standard_normal((new, nh, d)), store)
+    q[new // 2, 1, 5] = np.nan
+    out = put(cuda, np.zeros((new, nh, d), np.float32), store)
+    u32 = lambda a: put(cuda, np.asarray(a, np.uint32))[0]
+    cuda.paged_attention(put(cuda, q, store)[0], k[0], v[0], u32(rng.permutation(cols)[None]), u32([0, new]), u32([total]), max_new=new, out=out[0])
+    none = np.isnan(back(cuda, out[1]))
+    assert none[new // 2, 1].all() and none.sum() == d
+
+
 # ---------------------------------------------------------------- all of them together
 
 
