@@ -9,7 +9,7 @@
 // What bounds it is the chain loads -> sums -> sums -> pages -> stores, some 0.5 to 1 us each, and the call.  Every block of a cluster makes the sums for itself (which
 // needs no memory for them) and has its part of the tokens and of the pages that are given back: the row of each is looked up in shared memory, by halving, so that
 // long prompts and single tokens cost the same.  The first token of a page that is new also writes the table.  8 rows 4.9 us, most of it the call; 391 rows,
-// some ended, prompts that wait, 16384 places 10.6 us (12.9 while a warp had an ended row's pages).
+// some ended, prompts that wait, 16384 places 10.6 us.
 #include <algorithm>
 
 #include "paged.h"

@@ -485,8 +485,8 @@ int launch_typed(cg_ctx* c, const PagedAttnArgs& a) {
 
 // The parts of a token's head, joined: o = sum_c o_c 2^(m_c - m) / sum_c l_c 2^(m_c - m), m the largest m_c.  A thread has four components, a block
 // 256 / (d / 4) vectors or more; what the tables say is looked up before the parts are waited for.  What bounds it is that chain and the parts' way out of L2: 64 x 32
-// heads of 128 and 14 parts, 15 MB, some 5 us behind the others.  (Joined by the blocks of the rows' own keys, a round of loads from L2 per 12 parts stood in the way of
-// the next block's keys: 30 rows of drafts 50 us, so 39.)
+// heads of 128 and 14 parts, 15 MB, some 5 us behind the others.  (A launch of its own: in the blocks of the rows' own keys the loads of parts would stand in the way of the
+// next block's keys.)
 template <typename T>
 __global__ void __launch_bounds__(256) k_paged_join(PagedAttnArgs a) {
   const int quads = a.d / 4;

@@ -15,8 +15,8 @@
 // Bytes do not bound it (40 rows of up to 4 drafts over 151936 tokens, bf16: 41 MB in 42 us, 0.15 of the copy rate) but a row's chain: a round of positions is loads,
 // maxima and sums, the cluster's barrier, the verdict, 3 to 5 us; the draw's 64-bit exponentials 9 us at full rate, its sums and the search for the token
 // 4 to 7.  Rows of several rounds go on when the others' SMs are idle: an SM has work for 0.69 of the time, the busiest issues 1.66 times the mean.  One row of 4 drafts over
-// 128256, f32: 14 us; 32 rows of 7 over 256000 45.5; greedy, 16 rows of 3 over 50257, f32: 7.3.  First 26, 111, 99 and 19, with exp(), two passes and slices
-// kept in shared memory for the draw (which takes the room of other rows' blocks).
+// 128256, f32: 14 us; 32 rows of 7 over 256000 45.5; greedy, 16 rows of 3 over 50257, f32: 7.4.  Rows of one token, which draw from their logits: 64 over 128256, bf16, 26.6 us,
+// one in f32 9.4.
 #include <algorithm>
 #include <type_traits>
 
@@ -63,7 +63,7 @@ __device__ __forceinline__ float value_of(const uint4& v, int i) {
 template <typename T>
 __device__ __forceinline__ float logit(T x) { return fmaxf(widen(x), NO_LOGIT); }
 
-// e^x for x <= 0 to 2^-46 and better by Tang's method (1989): x = (16 m + j) ln2 / 16 + r, 2^(j/16) from a table (whose 16 values lie in different
+// e^x for x <= 0 by Tang's method (1989), to 2^-49 down to e^-30 and 2^-45 down to e^-700 (ln2 / 16 is off by 2^-59, the whole numbers by which it is taken go up to 16158): x = (16 m + j) ln2 / 16 + r, 2^(j/16) from a table (whose 16 values lie in different
 // banks), e^r by its series: 12 operations in 64 bits, where exp() takes twice as many, and no branch, so that several are under way.
 // Below e^-700 it is 0.
 __device__ __forceinline__ double exp64(double x, const double* power) {
@@ -591,7 +591,7 @@ int launch_threads(cg_ctx* c, VerifyArgs& a, int blocks) {
   }
   a.slice = (int)((a.V + blocks - 1) / blocks);
   // Positions judged at a time: two, where bytes count, so that few behind a rejected draft are read; of short ones all, for fewer rounds of
-  // sums and verdicts.  (16 rows x 50257 f32, greedy: 9.3 us with 8, 10.3 with 2; 32 x 256000 bf16: 69 and 54.)
+  // sums and verdicts.  (Us with 2 / 8: 32 rows of 7 drafts x 256000, bf16, 39.7  52.8, 40 of 4 x 151936 42.2  43.4; 16 of 3 x 50257, f32, greedy 8.3  7.4, 4 of 4 x 128256, bf16, 15.4  13.4.)
   a.ahead = a.rows * a.V * (int64_t)sizeof(T) > 8 << 20 ? 2 : MOST_AHEAD;
   const int64_t staging = a.probs ? (int64_t)a.slice * (a.probs16 ? 2 : 4) + 32 * (VT / 32 + 1) : 0;
   a.staged = staging > 0 && staging <= smem_most;
@@ -602,7 +602,7 @@ int launch_threads(cg_ctx* c, VerifyArgs& a, int blocks) {
 }
 template <typename T>
 int launch(cg_ctx* c, VerifyArgs& a) {
-  // Blocks of a row, and their threads and how many run on an SM, us, [the rule's]:
+  // Blocks of a row, and their threads and how many run on an SM (those of 512, 2 have 64 registers and spill 60 to 170 bytes, of 256, 3 some 80 and 0 to 16), us, [the rule's]:
   //                                                 16 x 512, 1   8 x 512, 2   8 x 256, 2   8 x 256, 3   4 x 256, 2
   //   1 row x 128256, f32, 4 drafts                 [14.1]        20           24           24           41
   //   16 x 50257, f32, 3, greedy                     16           10.0         [7.5]        8.1          10
