@@ -15,8 +15,8 @@
 // probabilities as bf16 holds them, so that a row that one key decides loses nothing either way.  Probabilities are one bf16 operand: a
 // second part, as the decode form has, would double the second product, which is half of this kernel's work.  Their rounding
 // (2^-9 of each, of either sign) adds to the output's: errors against 64 bits 0.0021 of the result, where the output's alone are 0.0016.  Those of chunks of shared
-// keys (CHUNK below) have the second part, so that sharing costs no bits: 0.00166, for 57.3 us instead of 54.2 (64 rows of 1 behind 16001), 36.7 instead of 34.3 (30 of up to
-// 5 in 3 groups behind 4003).  The rows' own keys in OWN have one, as these tokens' have in the form of prompts (with two 43.3).
+// keys (CHUNK below) have the second part, and the denominator sums them unrounded, so that sharing costs no bits: 0.00166, for 56.1 us instead of 53.9 (64 rows of 1 behind
+// 16001), 37.2 instead of 35.1 (30 of up to 5 in 3 groups behind 4003).  The rows' own keys in OWN have one, as these tokens' have in the form of prompts (with two 43.3).
 //
 // Where there are few tiles, or a little more than a whole number of turns, a cluster of 2 or 4 blocks shares a tile's keys; their outputs
 // are joined through shared memory.
@@ -445,25 +445,27 @@ k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
       float ls[2] = {0.f, 0.f};
       // Two probabilities as bf16, and (of shared keys) what their rounding left, in the place of the scores.
       auto split = [&](uint32_t* pk, int c, int i, float e0, float e1) {
+        if (SHARED) {
+          if (CAP && masked) {
+            e0 = vis[c] >> i & 1u ? e0 : 0.f;
+            e1 = vis[c] >> i & 2u ? e1 : 0.f;
+          }
+          ls[0] += e0;
+          ls[1] += e1;
+        }
         pk[i / 2] = pack_bf16(e0, e1);
         if (SHARED) v[c * 32 + i / 2] = pack_bf16(e0 - __uint_as_float(pk[i / 2] << 16), e1 - __uint_as_float(pk[i / 2] & 0xffff0000u));
       };
-      // Masked ones are cleared, the sum is made, and all go to TMEM.
+      // All go to TMEM; of one part, masked ones are cleared here and the sum is of what the products use.
       auto put = [&](uint32_t* pk, int c) {
-        if (CAP && masked)
+        if (!SHARED) {
+          if (CAP && masked)
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const uint32_t seen = (vis[c] >> i & 1u ? 0xffffu : 0u) | (vis[c] >> i & 2u ? 0xffff0000u : 0u);
-            pk[i / 2] &= seen;
-            if (SHARED) v[c * 32 + i / 2] &= seen;
-          }
+            for (int i = 0; i < 32; i += 2) pk[i / 2] &= (vis[c] >> i & 1u ? 0xffffu : 0u) | (vis[c] >> i & 2u ? 0xffff0000u : 0u);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          ls[0] += __uint_as_float(pk[i] << 16);
-          ls[1] += __uint_as_float(pk[i] & 0xffff0000u);
-          if (SHARED) {
-            ls[0] += __uint_as_float(v[c * 32 + i] << 16);
-            ls[1] += __uint_as_float(v[c * 32 + i] & 0xffff0000u);
+          for (int i = 0; i < 16; ++i) {
+            ls[0] += __uint_as_float(pk[i] << 16);
+            ls[1] += __uint_as_float(pk[i] & 0xffff0000u);
           }
         }
         st16(s_addr + (uint32_t)c * 16u, pk);
