@@ -598,25 +598,26 @@ int attend(cg_ctx* c, const PagedAttnArgs& a, bool bf16) {
 // Rows of so many tokens that they fill half a tile of 128 queries gain little by others' beside them, and blocks find their group by walking them (32 at
 // a time, 1 us).  Two launches more pay where 32 MB need not be read again, whatever the type, and 12 keys for each query, whose parts are written, read and
 // joined.  Us with chunks / row by row, [the rule's], rows of 1, 4 and 8 tokens:
-//   12 rows behind  500, 8 key heads of 128, saves  23 MB    10.1 [10.1]    14.4 [12.9]    15.7 [13.0]
-//   40 behind       500, 4 of 128,                  40 MB    12.8 [13.1]    23.4 [15.4]    29.6 [15.6]
-//   12 behind      1500, 4 of 128,                  34 MB    11.8 [12.1]    15.8 [18.3]    18.2 [18.3]
-//   40 behind       500, 8 of 128,                  80 MB   [15.3] 23.6    [26.5] 29.3     31.7 [26.6]
-//   40 behind      1500, 4 of 128,                 120 MB   [17.3] 26.5    [26.3] 29.8    [33.0] 29.9
-//   40 behind      5000, 8 of 128,                 799 MB   [23.4] 119     [37.6] 142     [60.1] 150
-//    4 behind      5000, 8 of 64,                   31 MB    15.4 [10.4]    16.8 [13.5]    15.7 [20.1]
-//   12 behind      1500, 4 of 256 with a cap,       68 MB   [13.6] 20.7    [15.2] 21.6    [27.4] 29.7
-//   40 behind       500, 2 of 64, f32,              20 MB    18.9 [16.5]    19.4 [16.9]    21.3 [17.0]
-//   40 behind      1500, 2 of 64, f32,              60 MB   [19.9] 42.6    [26.3] 43.0    [32.3] 43.1
+//   12 rows behind  500, 8 key heads of 128, saves  23 MB    10.4 [10.0]    14.4 [12.9]    16.3 [13.1]
+//   40 behind       500, 4 of 128,                  40 MB    13.1 [13.1]    23.8 [15.5]    30.4 [15.6]
+//   12 behind      1500, 4 of 128,                  34 MB    12.3 [12.2]    15.9 [18.3]    18.6 [18.3]
+//   40 behind       500, 8 of 128,                  80 MB   [15.4] 23.5    [26.7] 29.3     32.4 [26.5]
+//   40 behind      1500, 4 of 128,                 120 MB   [17.6] 26.6    [27.2] 29.5    [35.4] 29.6
+//   40 behind      5000, 8 of 128,                 799 MB   [23.8] 119     [39.1] 144     [67.0] 150
+//    4 behind      5000, 8 of 64,                   31 MB    15.7 [10.4]    17.2 [13.6]    16.1 [20.2]
+//   12 behind      1500, 4 of 256 with a cap,       68 MB   [13.9] 20.7    [15.6] 21.6    [28.1] 29.8
+//   40 behind       500, 2 of 64, f32,              20 MB    19.3 [16.7]    19.4 [16.9]    21.3 [17.0]
+//   40 behind      1500, 2 of 64, f32,              60 MB   [19.9] 42.5    [26.4] 42.8    [32.4] 43.0
 constexpr int SHARED_QUERIES = 64;  // of a row and key head, at most, in the mean
 // (In the mean: a prompt among rows that run does not keep these from sharing, and takes the chunks' tiles as they do.  64 rows of 1, 8 key heads of 128, and with them one of
-// 100 or 500, behind 500: [45] and 108 us, row by row 62 and [88]; behind 4000: [56] and [135], 267 and 312; behind 16000: [120] and [300], 1083 and 1083.)
+// 100 or 500, behind 500: [45] and 109 us, row by row 62 and [89]; behind 4000: [60] and [135], 269 and 301; behind 16000: [139] and [345], 1073 and 1046.)
 int64_t mean_new(const PagedAttnArgs& a) { return std::min(a.most, (a.rows.M + a.rows.rows - 1) / a.rows.rows); }
-// Under a window rows read no more than that of the prefix, and the chunks all of it.  Us with chunks / row by row, 4 key heads of 256 [8 of 128], window 512, 1024, 4096:
-//   14 rows behind  3000     21.3  11.4 [17.7   9.8]    21.2  16.0 [17.5  13.4]    20.3  34.6 [17.4  27.5]
-//   14 behind      16000     32.0  17.0 [24.9  15.0]    31.8  22.1 [24.9  18.8]    31.7  50.3 [24.8  40.3]
-//   40 behind      16000     36.7  41.2 [38.8  35.9]    36.5  54.0 [38.8  45.5]    36.0   125 [38.8  98.6]
-//    2 behind      16000     31.0  15.2 [24.0   6.8]    30.9  17.5 [23.6   7.8]    30.2  23.0 [23.6  13.2]
+// Under a window rows read no more than that of the prefix, and the chunks all of it.  Us with chunks / row by row, the rule's with a *, windows of 512, 1024 and 4096 for
+// 4 key heads of 256, then for 8 of 128:
+//   14 rows behind  3000    21.5  11.4*   21.4* 16.1    20.8* 34.7       18.1   9.8*   18.0* 13.3    18.1* 27.6
+//   14 behind      16000    31.8  17.0*   31.8  22.1*   31.8* 50.3       26.4  15.0*   26.2  18.8*   26.0* 40.4
+//   40 behind      16000    37.7  41.1*   37.7* 54.1    37.4* 125        41.1  35.9*   41.2* 45.3    41.1* 98.8
+//    2 behind      16000    31.1  15.1*   31.0  17.4*   30.7  23.0*      25.3   6.9*   24.9   7.8*   24.8  13.2*
 bool saves_enough(const cg_ctx* c, const PagedAttnArgs& a, bool bf16, int64_t queries) {
   const double most = (double)a.sh.groups.most, seen = a.window > 0 ? std::min(most, (double)(a.window + mean_new(a) - 1)) : most;
   const double keys = (double)a.rows.rows * seen - (double)a.sh.groups.n * most - 12. * (double)queries;  // (wide tables name more bytes than 63 bits hold)

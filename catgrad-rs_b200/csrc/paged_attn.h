@@ -22,7 +22,7 @@ struct SharedParts {
 // Which keys of a row a kernel takes: ALL of them; CHUNK: the queries are a group's, the keys a chunk of what its rows have in common; OWN: those behind that.
 // What comes before the launch of the chunks is complete when that lets the next one begin, so OWN waits for nothing until it ends; its last block does then, so
 // that what waits for it waits for the chunks too. (While all its blocks did, those that ended beside the chunks kept their
-// room on an SM to themselves: 64 rows behind 16001 tokens, 8 key heads of 128, 61 us instead of 54.)
+// room on an SM to themselves: 64 rows behind 16001 tokens, 8 key heads of 128, 70.5 us instead of 56.4.)
 enum KeysOf { ALL, CHUNK, OWN };
 
 struct PagedAttnArgs {

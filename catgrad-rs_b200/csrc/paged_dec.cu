@@ -39,7 +39,7 @@ struct DecArgs {
 };
 
 // Keys of a warp's tile, tiles of its ring, warps.  (Four warps of heads of 256 fill an SM; two blocks of two deal rows of different lengths out more evenly: 14 rows behind
-// 3001 tokens, 4 key heads of 256, window, 40.7 us with four, 38.7 with two, 38.5 with one.  Rows that read all their keys keep four.)
+// 3001 tokens, 4 key heads of 256, window, 41.3 us with four, 39.2 with two, 39.2 with one.  Rows that read all their keys keep four.)
 template <int D>
 __host__ __device__ constexpr int dec_keys() { return D == 64 ? 32 : 16; }
 constexpr int RING = 3;

@@ -15,8 +15,8 @@
 // probabilities as bf16 holds them, so that a row that one key decides loses nothing either way.  Probabilities are one bf16 operand: a
 // second part, as the decode form has, would double the second product, which is half of this kernel's work.  Their rounding
 // (2^-9 of each, of either sign) adds to the output's: errors against 64 bits 0.0021 of the result, where the output's alone are 0.0016.  Those of chunks of shared
-// keys (CHUNK below) have the second part, and the denominator sums them unrounded, so that sharing costs no bits: 0.00166, for 56.1 us instead of 53.9 (64 rows of 1 behind
-// 16001), 37.2 instead of 35.1 (30 of up to 5 in 3 groups behind 4003).  The rows' own keys in OWN have one, as these tokens' have in the form of prompts (with two 43.3).
+// keys (CHUNK below) have the second part, and the denominator sums them unrounded, so that sharing costs no bits: 0.00166, for 56.4 us instead of 53.9 (64 rows of 1 behind
+// 16001), 36.2 instead of 35.1 (30 of up to 5 in 3 groups behind 4003).  The rows' own keys in OWN have one, as these tokens' have in the form of prompts (with two 43.3).
 //
 // Where there are few tiles, or a little more than a whole number of turns, a cluster of 2 or 4 blocks shares a tile's keys; their outputs
 // are joined through shared memory.
@@ -123,7 +123,7 @@ __host__ __device__ constexpr size_t fa_smem() {
 // CHUNK: the queries are those of a group of rows, the keys a chunk of what the group has in common (through its first row's table), and
 // the outputs parts that are joined with the rows' own keys' (OWN).  A token's position is then its row's, and masks are only looked at
 // where a query stands inside the prefix or a window ends there.  64 rows, 32 heads and 8 key heads of 128, over 16001 shared keys in chunks of 1280: 2.6 us to the
-// first loads, 2.2 to the first scores, 1.07 per 64 keys where an SM has two blocks, 2 to write the parts (4 in 16-byte pieces).
+// first loads, 2.2 to the first scores, 1.2 per 64 keys where an SM has two blocks (1.07 with one part of the probabilities), 2 to write the parts (4 in 16-byte pieces).
 template <int D, int NQ, bool CAP, int MODE>
 __global__ void __launch_bounds__(NQ == 2 ? 384 : 256, NQ == 2 || D > 128 ? 1 : 2)
 k_paged_fa(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, FaArgs p) {
@@ -802,10 +802,10 @@ int paged_fa_own(cg_ctx* c, const PagedAttnArgs& a) {
 }
 // Keys of a chunk: as many chunks as make a block per SM, or 1.4 where two fit (the rows' own keys then run beside them), in one wave however the
 // tokens are dealt to the groups.  Us with 1 / 1.25 / 1.4 / 1.5 / 2 on an SM:
-//   64 rows of 1 behind 16001, 8 key heads of 128              55.0  54.0 [53.9] 55.9  59.9
-//   30 of up to 5 in 3 groups behind 4003, 4 of 128            37.0  35.6 [35.2] 35.3  38.5
-//   14 of 5 in 4 groups behind 3588, 8 of 128                  29.4  25.3 [23.8] 23.8  23.1
-//   26 of 1 behind 13661, 4 of 128                             24.7  25.8 [25.9] 25.2  27.1
+//   64 rows of 1 behind 16001, 8 key heads of 128              57.1  55.9 [56.4] 57.5  62.3
+//   30 of up to 5 in 3 groups behind 4003, 4 of 128            38.0  35.8 [36.2] 36.3  39.5
+//   14 of 5 in 4 groups behind 3588, 8 of 128                  31.0  26.7 [26.0] 26.0  24.1
+//   26 of 1 behind 13661, 4 of 128                             26.0  27.2 [26.5] 27.1  28.2
 int64_t paged_fa_slots(const PagedAttnArgs& a) { return a.d <= 128 ? 204 : 148; }
 int64_t paged_fa_chunk(const PagedAttnArgs& a) {
   const int64_t slots = paged_fa_slots(a), queries = a.rows.M * (a.nh / a.nkv), tiles = std::max<int64_t>((queries + a.sh.groups.n * 127) / 128, 1) * a.nkv;
