@@ -15,7 +15,8 @@ import numpy as np
 import pytest
 
 from conftest import ROOT, cg
-from test_paged import BF16, F32, PARTS, Host, attention, back, net, off_from_rounded, plain_logits, put, relative, rounded
+from test_paged import BF16, F32, Host, attention, back, net, plain_logits, put, rounded
+from test_paged import PARTS, off_from_rounded, relative
 
 gpu = pytest.mark.gpu
 INDEX = 6
